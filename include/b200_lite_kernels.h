@@ -142,6 +142,45 @@ int b2l_rope_kv_write(void* q, void* k, const void* v, const void* cos, const vo
                       int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride, int64_t cs_batch_stride,
                       int64_t cs_seq_stride, int64_t d_tok_stride, int64_t d_head_stride, int dtype, void* stream);
 
+/* ---- Key/value cache in 4 bits (csrc/kv_int4.cuh) ----------------------------------------------------------------
+ * One row of bytes per token: for every kv head in turn the codes of K, the codes of V (head_dim / 2 bytes each, element 2i in the
+ * low four bits of byte i), then K's and V's (scale, minimum) per group of `group` elements in the activations' type; filled up to a
+ * multiple of 16 bytes.  An element is minimum + scale * code.  head_dim 32, 64 or 128, groups of 32, 64 or 128 (at most head_dim);
+ * others: 0 bytes. */
+int64_t b2l_kv_int4_row_bytes(int num_kv_heads, int head_dim, int group);
+/* Rotary positions on q [T, n_qh, D] and k [T, n_kh, D] (32-bit arithmetic, one rounding) into q_out and k_out (k_out may be null, both
+ * may be their inputs), and k and v [T, n_kh, D] rounded to codes into the rows select_index[t] of the cache; an index outside
+ * [0, max_tokens) stores nothing.  Without cos and sin (n_qh = 0) k and v are stored as they are.  Token t reads cos / sin
+ * [t / seq_len, t % seq_len].  Strides in elements, the cache's in bytes. */
+int b2l_kv_int4_write(void* q_out, void* k_out, const void* q, const void* k, const void* v, const void* cos, const void* sin,
+                      const void* select_index, int index_width, void* cache, int64_t cache_row_stride, int64_t max_tokens,
+                      int64_t tokens, int64_t seq_len, int n_qh, int n_kh, int head_dim, int group, int64_t q_tok_stride,
+                      int64_t q_head_stride, int64_t k_tok_stride, int64_t k_head_stride, int64_t v_tok_stride,
+                      int64_t v_head_stride, int64_t cs_batch_stride, int64_t cs_seq_stride, int64_t qo_tok_stride,
+                      int64_t qo_head_stride, int64_t ko_tok_stride, int64_t ko_head_stride, int dtype, void* stream);
+/* out [tokens, 2 * n_kh, D] = the values of the rows select_index (K heads, then V heads); zeros for an index outside the cache. */
+int b2l_kv_int4_read(void* out, const void* cache, int64_t cache_row_stride, int64_t max_tokens, const void* select_index,
+                     int index_width, int64_t tokens, int n_kh, int head_dim, int group, int dtype, void* stream);
+/* b2l_flash_decoding over that cache.  Lengths count up to max_seq_len and the table's width; a request outside the table is empty,
+ * a table entry outside the cache reads row 0. */
+int64_t b2l_flash_decoding_int4_workspace_bytes(int64_t batch, int num_q_heads, int num_kv_heads, int head_dim, int group,
+                                                int64_t max_seq_len);
+int b2l_flash_decoding_int4(void* out, const void* q, const void* cache, int64_t cache_row_stride, int64_t max_tokens,
+                            const void* b_req_tokens_table, int64_t table_req_stride, int64_t table_seq_stride,
+                            int64_t table_requests, int64_t table_width, const void* b_req_idx, int req_idx_width,
+                            const void* b_seq_len, int seq_len_width, int64_t batch, int num_q_heads, int num_kv_heads,
+                            int head_dim, int group, int64_t max_seq_len, float qk_scale, int64_t q_batch_stride,
+                            int64_t q_head_stride, int64_t o_batch_stride, int64_t o_head_stride, void* workspace,
+                            int64_t workspace_bytes, int dtype, void* stream);
+/* Slot maps of a ragged step: start[b] = sum of new_len over the requests before b, length[b] = ctx_len[b] + new_len[b] (int32 [batch]);
+ * for token t of the flat batch, the j-th new one of request b: position[t] = ctx_len[b] + j (int64), rows[t] (int32) =
+ * table[req_idx[b], position], or, with pool_rows, pool_rows[t], which is entered there.  Tokens behind the last request: row -1,
+ * position 0; a request or position outside the table: row -1.  Negative lengths count as 0. */
+int b2l_slot_maps(void* rows, void* position, void* start, void* length, const void* req_idx, int req_width, const void* ctx_len,
+                  int ctx_width, const void* new_len, int new_width, const void* pool_rows, int pool_width, void* table,
+                  int64_t table_req_stride, int64_t table_seq_stride, int64_t requests, int64_t width, int64_t batch,
+                  int64_t total_tokens, void* stream);
+
 /* Greedy sampling: out[r] = argmax_j x[r, j] (int64; ties -> lowest index).  Reference: temperature-0 path of the
  * Sampler, torch.argmax over the [batch, vocab] logits (lite_llama/engine/sampler.py, engine/llm_engine.py:172). */
 int b2l_argmax_rows(void* out_index_i64, const void* x, int64_t rows, int64_t n, int64_t row_stride, int dtype,

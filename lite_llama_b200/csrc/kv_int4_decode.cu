@@ -1,0 +1,719 @@
+// flash_decoding_int4: one query per sequence over a cache held in 4 bits (kv_int4.cuh).
+//
+//   out_h = sum_t softmax_t(scale q_h . k_t) v_t,   k_t = minimum + scale_t * code per group of elements (v_t too)
+//
+// Elements are not formed.  With codes c, q . k = sum over groups (s q . c + m sum(q)), so a key's scales meet the finished sums of
+// its codes; and out = sum_t (p s) c + sum_t p m, so a value's scale is multiplied into the probability.  What is left of unpacking is
+// a mask: the four bits of a code, in a half's lowest bits, ARE the subnormal half 2^-24 c (one place higher 2^-20 c), and a product
+// of it is exact.  Five integer instructions turn a word of eight key codes into operands, six one of value codes.
+// The tokens are the 16 rows of an mma.sync tile and the group's query heads its 8 columns: the cache is the operand that fills the
+// tile.  Queries are scaled by a power of two per head to the middle of the range of halves, which is exact down to 2^-29 of the
+// head's largest element.  Probabilities are not rounded to 11 bits: what rounding leaves of p s is multiplied as well -- in the
+// columns that up to four heads leave free, else in a second product -- since a code's products are larger than its value's.
+//
+// Work: tiles of 16 * TS tokens of all rows, in equal shares over one wave of CTAs, whatever rows they belong to (the lengths are device
+// data).  A producer warp copies whole token rows by the TMA engine into a ring; a consumer warp takes 16 tokens of one kv head.  A row
+// that lies in one share is written out; else its parts go to the workspace and a second kernel adds them up.
+#include "kv_int4.cuh"
+
+namespace {
+
+constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16;
+constexpr int kMinTokens = 64;                    // of a share: below that the merge costs more than the share
+
+struct Int4DecodeParams {
+  const void* q; int64_t q_bs, q_hs; int q_vec;   // q_vec: heads on 16-byte boundaries
+  void* out; int64_t o_bs, o_hs;
+  const uint8_t* cache; int64_t row_stride, max_tokens;
+  const int32_t* table; int64_t tab_rs, tab_cs, requests, width;
+  const void* req_idx; int req_w;
+  const void* seq_len; int len_w;
+  int batch, Hq, Hkv, G, HB, qblocks, TS, stages, pitch;
+  int64_t most;                                   // tokens of a row that the call's bound lets count
+  float scale_log2;
+  float* ws_o; float* ws_ml; int2* ws_info;       // parts [cta][2][HB * G]: rows, (largest score, sum); first and last CTA of a row
+};
+
+__device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+// 2^e, e clamped to the range of normal numbers
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e < -126 ? 1 : e > 127 ? 254 : e + 127) << 23); }
+
+// the row of a tile's unit that stands at place i of eight: rows 0 - 3 and 4 - 7 as well as the even and the odd ones then lie in
+// different banks (a row's pitch is 32 bytes past a multiple of 128)
+__device__ __forceinline__ int place(int i) { return i ^ ((i >> 2) & 1); }
+
+// One consumer warp's work: up to 8 query heads of one kv head, units of 16 tokens in turn.
+// DUP: at most 4 heads; columns 4 - 7 are the same heads again and take what rounding leaves of p s.
+template <typename T, int D, int GS, bool DUP>
+struct Int4Consumer {
+  static constexpr int NG = D / GS, NW = D / 32, MT = D / 16;
+  uint32_t qb[NW][4];                             // a key word's query elements: nibbles (0, 4), (2, 6), (1, 5) / 16, (3, 7) / 16
+  float f[2], sq[2][NG];                          // per column: what a sum of codes is multiplied by; scaled sums of the query
+  float O[MT][4], z[2][NG];                       // sums of p s c (rows r + 8 hold 16 times theirs) and of p m
+  float m[2], l[2], m_lim[2];                     // scores are relative to m; above m_lim it is raised
+  float v_scale, v_lim;                           // value scales are multiplied by v_scale = 2^-e before p s is rounded
+  int lane, r, c;
+
+  static __device__ __forceinline__ int word_at(int k, int c) { return GS == 32 ? k * 4 + c : (k >> 1) * 8 + c * 2 + (k & 1); }
+  static __device__ __forceinline__ constexpr int group_of(int k) { return GS == 32 ? k : GS == 64 ? k >> 1 : 0; }
+
+  __device__ __forceinline__ void begin(const Int4DecodeParams& p, int b, int kvh, int head0, int heads) {
+    const int col = DUP ? r & 3 : r;
+    const bool live = col < heads;
+    float qv[NW][8], big = 0.f;
+    const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_bs + (int64_t)(kvh * p.G + head0 + (live ? col : 0)) * p.q_hs;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      const T* w = q + word_at(k, c) * 8;
+      __align__(16) T e[8];
+      if (p.q_vec) {
+        *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(w);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = w[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        qv[k][i] = live ? to_f32(e[i]) : 0.f;
+        big = fmaxf(big, fabsf(qv[k][i]));
+      }
+    }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    // largest element to [2^8, 2^9); an infinity stays one
+    int e = 8 - ((int)(__float_as_uint(big) >> 23) - 127);
+    if (!(big < INFINITY) || big == 0.f) e = 0;
+    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    const float up = exp2i(e);
+    float sums[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) sums[g] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sums[group_of(k)] += qv[k][i];
+      const float lo = up, hi = up * 0.0625f;
+      qb[k][0] = pack2<__half>(qv[k][0] * lo, qv[k][4] * lo);
+      qb[k][1] = pack2<__half>(qv[k][2] * lo, qv[k][6] * lo);
+      qb[k][2] = pack2<__half>(qv[k][1] * hi, qv[k][5] * hi);
+      qb[k][3] = pack2<__half>(qv[k][3] * hi, qv[k][7] * hi);
+    }
+    const float back = p.scale_log2 * exp2i(-e) * 16777216.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) f[j] = __shfl_sync(0xffffffffu, back, (2 * c + j) * 4);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float s = sums[g];
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      s *= p.scale_log2;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) sq[j][g] = __shfl_sync(0xffffffffu, s, (2 * c + j) * 4);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) O[t][i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      m[j] = m_lim[j] = -INFINITY;
+      l[j] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) z[j][g] = 0.f;
+    }
+    v_scale = 1.f;
+    v_lim = -1.f;
+  }
+
+  // a score above what the sums are scaled for, or a value scale: raise either
+  __device__ __forceinline__ void raise(const float (&v)[2][2], float vs) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float mx = fmaxf(v[0][j], v[1][j]);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (mx > m[j]) {
+        const float a = fast_exp2(m[j] - mx);     // m[j] = -inf at first: 0
+        m[j] = mx;
+        l[j] *= a;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) z[j][g] *= a;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) { O[t][j] *= a; O[t][2 + j] *= a; }
+      }
+      m_lim[j] = m[j] + 8.f;
+    }
+    const uint32_t top = __reduce_max_sync(0xffffffffu, vs > v_lim && vs < INFINITY ? __float_as_uint(vs) : 0u);
+    if (v_lim < 0.f || top != 0u) {
+      int e = (int)(top >> 23) - 127;
+      e = e < -100 ? -100 : e > 120 ? 120 : e;
+      const float next = exp2i(-e), by = v_lim < 0.f ? 1.f : next / v_scale;
+      v_scale = next;
+      v_lim = exp2i(e + 6);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[t][i] *= by;
+    }
+  }
+
+  // 16 tokens at `at` (the head's bytes of the first), of which `valid` count
+  template <bool MASKED>
+  __device__ __forceinline__ void unit(const uint8_t* at, int pitch, int valid) {
+    constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+    const uint8_t* row0 = at + place(r) * pitch;
+    const uint8_t* row1 = row0 + 8 * pitch;
+    // ---- scores of 16 tokens (rows) and 8 heads (columns) ----
+    uint32_t w0[NW], w1[NW];
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      if (GS == 32) {
+        w0[k] = reinterpret_cast<const uint32_t*>(row0)[k * 4 + c];
+        w1[k] = reinterpret_cast<const uint32_t*>(row1)[k * 4 + c];
+      } else if ((k & 1) == 0) {
+        const uint2 x = reinterpret_cast<const uint2*>(row0)[(k >> 1) * 4 + c], y = reinterpret_cast<const uint2*>(row1)[(k >> 1) * 4 + c];
+        w0[k] = x.x; w0[k + 1] = x.y;
+        w1[k] = y.x; w1[k + 1] = y.y;
+      }
+    }
+    float acc[NG][4];
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[g][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      const uint32_t x0 = w0[k] >> 8, x1 = w1[k] >> 8;
+      const uint32_t lo[4] = {w0[k] & kLow, w1[k] & kLow, x0 & kLow, x1 & kLow};
+      const uint32_t hi[4] = {w0[k] & kHigh, w1[k] & kHigh, x0 & kHigh, x1 & kHigh};
+      mma_m16n8k16<__half>(acc[group_of(k)], lo, qb[k][0], qb[k][1]);
+      mma_m16n8k16<__half>(acc[group_of(k)], hi, qb[k][2], qb[k][3]);
+    }
+    float2 ks[2][NG], vs[2][NG];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t* gp = reinterpret_cast<const uint32_t*>((i ? row1 : row0) + D);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        ks[i][g] = kv4::scale_min<T>(gp[g]);
+        vs[i][g] = kv4::scale_min<T>(gp[NG + g]);
+      }
+    }
+    float v[2][2], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool in = !MASKED || place(r) + 8 * i < valid;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float t = ks[i][0].x * acc[0][2 * i + j], u = ks[i][0].y * sq[j][0];
+#pragma unroll
+        for (int g = 1; g < NG; ++g) {
+          t = fmaf(ks[i][g].x, acc[g][2 * i + j], t);
+          u = fmaf(ks[i][g].y, sq[j][g], u);
+        }
+        v[i][j] = in ? fmaf(t, f[j], u) : -INFINITY;
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        if (MASKED && !in) vs[i][g] = make_float2(0.f, 0.f);
+        top = fmaxf(top, vs[i][g].x);
+      }
+    }
+    const bool over = fmaxf(v[0][0], v[1][0]) > m_lim[0] || fmaxf(v[0][1], v[1][1]) > m_lim[1] || top > v_lim;
+    if (__any_sync(0xffffffffu, over)) raise(v, top);
+    // ---- probabilities, times the values' scales, as the second product's columns ----
+    float pr[2][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float base = m[j] == -INFINITY ? 0.f : m[j];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) pr[i][j] = fast_exp2(v[i][j] - base);
+      l[j] += pr[0][j] + pr[1][j];
+    }
+    uint32_t pb[NG][2], rest[NG][2];
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) z[j][g] = fmaf(pr[i][j], vs[i][g].y, z[j][g]);
+        const float s = vs[i][g].x * v_scale, x = pr[i][0] * s, y = pr[i][1] * s;
+        const uint32_t near = pack2<__half>(x, y);
+        const float2 back = halves(near);
+        const uint32_t left = pack2<__half>(x - back.x, y - back.y);
+        if (DUP) {
+          pb[g][i] = trans8x8(c < 2 ? near : left);
+        } else {
+          pb[g][i] = trans8x8(near);
+          rest[g][i] = trans8x8(left);
+        }
+      }
+    // ---- values: rows are elements, columns heads, the products run over tokens ----
+    const uint8_t* t0 = at + D / 2 + place(2 * c) * pitch;
+    const uint8_t* t1 = at + D / 2 + place(2 * c + 1) * pitch;
+    auto add = [&](int tile, int g, const uint32_t (&a)[4]) {
+      mma_m16n8k16<__half>(O[tile], a, pb[g][0], pb[g][1]);
+      if (!DUP) mma_m16n8k16<__half>(O[tile], a, rest[g][0], rest[g][1]);
+    };
+    if (GS == 32) {
+      const uint32_t pick = (r & 1) ? 0x7632u : 0x5410u;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int o = (g * 4 + (r >> 1)) * 4;
+        auto word = [&](const uint8_t* t) { return *reinterpret_cast<const uint32_t*>(t + o); };
+        const uint32_t x = __byte_perm(word(t0), word(t1), pick), y = __byte_perm(word(t0 + 8 * pitch), word(t1 + 8 * pitch), pick);
+        const uint32_t a0[4] = {x & kLow, x & kHigh, y & kLow, y & kHigh};
+        const uint32_t x8 = x >> 8, y8 = y >> 8;
+        const uint32_t a1[4] = {x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh};
+        add(g * 2, g, a0);
+        add(g * 2 + 1, g, a1);
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < D / 64; ++b) {
+        const int o = (b * 8 + r) * 4, g = b * 64 / GS;
+        auto word = [&](const uint8_t* t) { return *reinterpret_cast<const uint32_t*>(t + o); };
+        const uint32_t e0 = word(t0), e1 = word(t1), e2 = word(t0 + 8 * pitch), e3 = word(t1 + 8 * pitch);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t x = __byte_perm(e0, e1, h ? 0x7632 : 0x5410), y = __byte_perm(e2, e3, h ? 0x7632 : 0x5410);
+          const uint32_t a0[4] = {x & kLow, x & kHigh, y & kLow, y & kHigh};
+          const uint32_t x8 = x >> 8, y8 = y >> 8;
+          const uint32_t a1[4] = {x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh};
+          add(b * 4 + h * 2, g, a0);
+          add(b * 4 + h * 2 + 1, g, a1);
+        }
+      }
+    }
+  }
+
+  // the element that O[t][0] (and [1]) of this lane belongs to; O[t][2] (and [3]) to the next one
+  __device__ __forceinline__ int element(int t) const {
+    return GS == 32 ? (t >> 1) * 32 + r * 4 + (t & 1) * 2 : (t >> 2) * 64 + r * 8 + (t & 3) * 2;
+  }
+  // sums in true units, complete over the lanes
+  __device__ __forceinline__ void finish() {
+    const float by = 16777216.f / v_scale;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) z[j][g] += __shfl_xor_sync(0xffffffffu, z[j][g], o);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        float lo = O[t][j], hi = O[t][2 + j];
+        if (DUP) {
+          lo += __shfl_xor_sync(0xffffffffu, lo, 2);
+          hi += __shfl_xor_sync(0xffffffffu, hi, 2);
+        }
+        const int g = GS == 32 ? t >> 1 : (t >> 2) * 64 / GS;
+        O[t][j] = fmaf(lo, by, z[j][g]);
+        O[t][2 + j] = fmaf(hi, by * 0.0625f, z[j][g]);
+      }
+    }
+  }
+};
+
+struct Segment { int b, first, last, tiles; };    // tiles [first, last) of a row of `tiles`
+
+template <typename T, int D, int GS, bool DUP>
+__global__ void __launch_bounds__((kMaxConsumers + 1) * 32, 2) kv4_decode_kernel(const Int4DecodeParams p) {
+  pdl_prologue();   // everything below reads what earlier kernels of the step wrote
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int warp_sum[kMaxConsumers + 1];
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* empty_bar = full_bar + kMaxStages;
+  uint8_t* ring = smem + 128;
+  const int unit_bytes = kUnit * p.pitch, stage_bytes = p.TS * unit_bytes, tile = p.TS * kUnit;
+  float* join = reinterpret_cast<float*>(ring + p.stages * stage_bytes);      // sums of the warps that share a head
+  const int per_head = p.qblocks * 8 * (D + 2);
+  int* prefix = reinterpret_cast<int*>(join + (p.TS - 1) * p.HB * per_head);  // tiles of the rows before, [batch + 1]
+  int* lens = prefix + p.batch + 1;
+  int* reqs = lens + p.batch;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nconsumers = p.HB * p.qblocks * p.TS;
+  const int nblk = p.Hkv / p.HB;
+
+  // ---- tiles of the rows before each; a thread owns neighbouring rows ----
+  const int per = (p.batch + blockDim.x - 1) / blockDim.x, r_lo = threadIdx.x * per;
+  const int r_hi = r_lo + per < p.batch ? r_lo + per : p.batch;
+  int own = 0;
+  for (int r = r_lo; r < r_hi; ++r) {
+    const int64_t n = load_index(p.seq_len, r, p.len_w), q = load_index(p.req_idx, r, p.req_w);
+    reqs[r] = (int)q;
+    lens[r] = q < 0 || q >= p.requests || n <= 0 ? 0 : n > p.most ? (int)p.most : (int)n;
+    own += (lens[r] + tile - 1) / tile;
+  }
+  int upto = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) warp_sum[warp] = upto;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], nconsumers);
+    }
+    mbar_fence_init();
+  }
+  __syncthreads();
+  int at = upto - own, all = 0;
+  for (int w = 0; w <= nconsumers; ++w) {
+    if (w < warp) at += warp_sum[w];
+    all += warp_sum[w];
+  }
+  for (int r = r_lo; r < r_hi; ++r) {
+    prefix[r] = at;
+    at += (lens[r] + tile - 1) / tile;
+  }
+  if (threadIdx.x == 0) prefix[p.batch] = all;
+  __syncthreads();
+
+  // ---- this CTA's share of all tiles, heads' blocks one after the other ----
+  const int64_t total = (int64_t)all * nblk;
+  const int least = (kMinTokens + tile - 1) / tile;
+  const int64_t worth = (total + least - 1) / least;
+  const int64_t shares = worth < gridDim.x ? worth : gridDim.x;
+  if (blockIdx.x >= shares) return;
+  int64_t item = blockIdx.x * total / shares;
+  const int64_t item_end = (blockIdx.x + 1) * total / shares;
+  // the next part of a row, and the block of heads it is in
+  auto next = [&](Segment& s, int& blk) -> bool {
+    if (item >= item_end) return false;
+    blk = (int)(item / all);
+    const int x = (int)(item - (int64_t)blk * all);
+    int lo = 0, n = p.batch;                      // the last row that begins at or before x and has tiles
+    while (n > 1) {
+      const int half = n / 2;
+      if (prefix[lo + half] <= x) { lo += half; n -= half; }
+      else n = half;
+    }
+    s.b = lo;
+    s.first = x - prefix[lo];
+    s.tiles = prefix[lo + 1] - prefix[lo];
+    const int64_t left = item_end - item;
+    s.last = left < s.tiles - s.first ? s.first + (int)left : s.tiles;
+    item += s.last - s.first;
+    return true;
+  };
+
+  Segment seg;
+  int blk, s = 0;
+  uint32_t phase = 0;
+  const int hb = kv4::head_bytes(D, GS);
+  if (warp == nconsumers) {
+    // ===================== producer: token rows by the copy engine =====================
+    while (next(seg, blk)) {
+      const int len = lens[seg.b];
+      const int32_t* entry = p.table + (int64_t)reqs[seg.b] * p.tab_rs;
+      const int from = blk * p.HB * hb, shift = from & 15;
+      const uint32_t bytes = (uint32_t)((shift + p.HB * hb + 15) & ~15);
+      const uint8_t* src = p.cache + (from - shift);
+      for (int t = seg.first; t < seg.last; ++t) {
+        mbar_wait(&empty_bar[s], phase ^ 1);
+        const int here = len - t * tile < tile ? len - t * tile : tile;
+        if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], (uint32_t)here * bytes);
+        __syncwarp();
+        for (int i = lane; i < here; i += 32) {
+          int64_t row = entry[(int64_t)(t * tile + i) * p.tab_cs];
+          if (row < 0 || row >= p.max_tokens) row = 0;
+          bulk_g2s(ring + s * stage_bytes + i * p.pitch, src + row * p.row_stride, bytes, &full_bar[s]);
+        }
+        if (++s == p.stages) { s = 0; phase ^= 1; }
+      }
+    }
+    return;
+  }
+  // ===================== consumers: (kv head, block of query heads, unit of the tile) =====================
+  const int ts = warp / (p.HB * p.qblocks), wh = warp - ts * p.HB * p.qblocks;
+  const int hl = wh / p.qblocks, qblk = wh - hl * p.qblocks;
+  const int head0 = qblk * 8, heads = p.G - head0 < 8 ? p.G - head0 : 8;
+  Int4Consumer<T, D, GS, DUP> c;
+  c.lane = lane; c.r = lane >> 2; c.c = lane & 3;
+  while (next(seg, blk)) {
+    const int len = lens[seg.b], kvh = blk * p.HB + hl;
+    const int off = ((blk * p.HB * hb) & 15) + hl * hb + ts * unit_bytes;
+    c.begin(p, seg.b, kvh, head0, heads);
+    for (int t = seg.first; t < seg.last; ++t) {
+      mbar_wait(&full_bar[s], phase);
+      const int valid = len - t * tile - ts * kUnit;
+      const uint8_t* u = ring + s * stage_bytes + off;
+      if (valid >= kUnit) c.template unit<false>(u, p.pitch, kUnit);
+      else if (valid > 0) c.template unit<true>(u, p.pitch, valid);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty_bar[s]);
+      if (++s == p.stages) { s = 0; phase ^= 1; }
+    }
+    c.finish();
+    // columns of this lane: heads 2c and 2c + 1 (DUP: the upper half of the columns repeats the lower)
+    const bool mine = !DUP || c.c < 2;
+    if (p.TS > 1) {
+      auto bar = [&] { asm volatile("bar.sync 1, %0;" ::"r"(nconsumers * 32) : "memory"); };
+      bar();                                      // the sums before these have been read
+      float* mineat = join + ((ts - 1) * p.HB * p.qblocks + wh) * 8 * (D + 2);
+      if (ts > 0 && mine) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float* to = mineat + (2 * c.c + j) * (D + 2);
+#pragma unroll
+          for (int t = 0; t < D / 16; ++t) *reinterpret_cast<float2*>(to + c.element(t)) = make_float2(c.O[t][j], c.O[t][2 + j]);
+          if (c.r == 0) *reinterpret_cast<float2*>(to + D) = make_float2(c.m[j], c.l[j]);
+        }
+      }
+      bar();
+      if (ts > 0) continue;
+      for (int o = 1; o < p.TS; ++o) {
+        const float* from = join + ((o - 1) * p.HB * p.qblocks + wh) * 8 * (D + 2);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (!mine) continue;
+          const float* x = from + (2 * c.c + j) * (D + 2);
+          const float2 ml = *reinterpret_cast<const float2*>(x + D);
+          const float mm = fmaxf(c.m[j], ml.x), base = mm == -INFINITY ? 0.f : mm;
+          const float a = fast_exp2(c.m[j] - base), e = fast_exp2(ml.x - base);
+          c.m[j] = mm;
+          c.l[j] = c.l[j] * a + ml.y * e;
+#pragma unroll
+          for (int t = 0; t < D / 16; ++t) {
+            const float2 y = *reinterpret_cast<const float2*>(x + c.element(t));
+            c.O[t][j] = c.O[t][j] * a + y.x * e;
+            c.O[t][2 + j] = c.O[t][2 + j] * a + y.y * e;
+          }
+        }
+      }
+    }
+    const bool whole = seg.first == 0 && seg.last == seg.tiles;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int head = head0 + 2 * c.c + j;
+      if (!mine || 2 * c.c + j >= heads) continue;
+      if (whole) {
+        const float inv = 1.f / c.l[j];
+        T* to = reinterpret_cast<T*>(p.out) + (int64_t)seg.b * p.o_bs + (int64_t)(kvh * p.G + head) * p.o_hs;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+          to[c.element(t)] = from_f32<T>(c.O[t][j] * inv);
+          to[c.element(t) + 1] = from_f32<T>(c.O[t][2 + j] * inv);
+        }
+      } else {
+        const int64_t part = ((int64_t)blockIdx.x * 2 + (seg.first == 0 ? 1 : 0)) * p.HB * p.G + hl * p.G + head;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+          *reinterpret_cast<float2*>(p.ws_o + part * D + c.element(t)) = make_float2(c.O[t][j], c.O[t][2 + j]);
+        if (c.r == 0) *reinterpret_cast<float2*>(p.ws_ml + part * 2) = make_float2(c.m[j], c.l[j]);
+      }
+    }
+    if (wh == 0 && lane == 0) {
+      int* note = reinterpret_cast<int*>(p.ws_info + (int64_t)blk * p.batch + seg.b);
+      if (seg.first == 0) note[0] = blockIdx.x;
+      if (seg.last == seg.tiles) note[1] = blockIdx.x;
+    }
+  }
+}
+
+// The rows that several CTAs met in, and zeros for the empty ones.  Eight warps take the parts in turn, so that their loads are on
+// their way together, and meet in shared memory.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_decode_merge_kernel(const Int4DecodeParams p) {
+  pdl_prologue();
+  constexpr int E = D / 32;                       // neighbouring elements of a lane
+  __shared__ float sums[8][D + 2];
+  const int b = blockIdx.x, head = blockIdx.y, kvh = head / p.G, blk = kvh / p.HB;
+  const int local = (kvh - blk * p.HB) * p.G + head - kvh * p.G;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t len = load_index(p.seq_len, b, p.len_w), q = load_index(p.req_idx, b, p.req_w);
+  T* out = reinterpret_cast<T*>(p.out) + (int64_t)b * p.o_bs + (int64_t)head * p.o_hs;
+  if (len <= 0 || q < 0 || q >= p.requests || p.most <= 0) {
+    for (int d = threadIdx.x; d < D; d += blockDim.x) out[d] = from_f32<T>(0.f);
+    return;
+  }
+  const int2 who = __ldcg(p.ws_info + (int64_t)blk * p.batch + b);
+  const int n = who.y - who.x + 1;
+  if (n < 2) return;                              // written by its only CTA
+  auto part = [&](int i) { return ((int64_t)(who.x + i) * 2 + (i == 0 ? 1 : 0)) * p.HB * p.G + local; };
+  float acc[E], M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int i0 = warp; i0 < n; i0 += 32) {         // four parts of this warp at a time
+    float x[4][E];
+    float2 ml[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + 8 * k;
+      ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[k][e] = 0.f;
+      if (i < n) {
+        ml[k] = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + part(i));
+        const float* o = p.ws_o + part(i) * D + lane * E;
+        if (E == 4) {
+          const float4 y = __ldcg(reinterpret_cast<const float4*>(o));
+          x[k][0] = y.x; x[k][1 % E] = y.y; x[k][2 % E] = y.z; x[k][3 % E] = y.w;
+        } else if (E == 2) {
+          const float2 y = __ldcg(reinterpret_cast<const float2*>(o));
+          x[k][0] = y.x; x[k][1 % E] = y.y;
+        } else {
+          x[k][0] = __ldcg(o);
+        }
+      }
+    }
+    float mm = M;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mm = fmaxf(mm, ml[k].x);
+    const float base = mm == -INFINITY ? 0.f : mm, a = fast_exp2(M - base);
+    L *= a;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= a;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = fast_exp2(ml[k].x - base);
+      L = fmaf(ml[k].y, w, L);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(x[k][e], w, acc[e]);
+    }
+    M = mm;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[e];
+  if (lane == 0) { sums[warp][D] = M; sums[warp][D + 1] = L; }
+  __syncthreads();
+  if ((int)threadIdx.x < D) {
+    float mm = -INFINITY, o = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) mm = fmaxf(mm, sums[w][D]);
+    const float base = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float a = fast_exp2(sums[w][D] - base);
+      o = fmaf(sums[w][threadIdx.x], a, o);
+      l = fmaf(sums[w][D + 1], a, l);
+    }
+    out[threadIdx.x] = from_f32<T>(o / l);
+  }
+}
+
+constexpr int kMaxBatch = 4096;                   // rows of one launch (their lengths lie in shared memory)
+
+struct Int4Plan { int HB, qblocks, TS, pitch, stages, smem, grid; };
+
+// A function of sizes that the host knows, hence the same inside and outside a captured graph.
+Int4Plan make_plan(int64_t batch, int G, int Hkv, int D, int group, int64_t max_len) {
+  Int4Plan pl;
+  pl.qblocks = (G + 7) / 8;
+  pl.HB = 1;
+  for (int h = 1; h * pl.qblocks <= kMaxConsumers; ++h)
+    if (Hkv % h == 0) pl.HB = h;
+  pl.TS = kMaxConsumers / (pl.HB * pl.qblocks);
+  const int hb = kv4::head_bytes(D, group);
+  const int bytes = ((pl.HB * hb + (pl.HB == Hkv ? 0 : 8)) + 15) / 16 * 16;
+  pl.pitch = (bytes + 95) / 128 * 128 + 32;       // 32 bytes past a multiple of 128
+  const int stage = pl.TS * kUnit * pl.pitch;
+  const int rows = (int)(batch < kMaxBatch ? batch : kMaxBatch);
+  const int fixed = 128 + (pl.TS - 1) * pl.HB * pl.qblocks * 8 * (D + 2) * 4 + (3 * rows + 1) * 4;
+  // two CTAs to an SM, each with a ring of what is left
+  const int cap = b2l_max_smem_optin() / 2 - 1536;
+  pl.stages = (cap - fixed) / stage;
+  if (pl.stages > kMaxStages) pl.stages = kMaxStages;
+  if (pl.stages < 2) pl.stages = 2;
+  pl.smem = fixed + pl.stages * stage;
+  const int64_t most = (int64_t)rows * cdiv64(max_len > 0 ? max_len : 1, kMinTokens) * (Hkv / pl.HB);
+  const int64_t wave = 2ll * b2l_num_sms();
+  pl.grid = (int)(most < wave ? most : wave);
+  return pl;
+}
+
+template <typename T, int D, int GS>
+int launch_int4_decode(const Int4DecodeParams& p, const Int4Plan& pl, cudaStream_t st) {
+  const dim3 grid((unsigned)pl.grid), block((pl.HB * pl.qblocks * pl.TS + 1) * 32);
+  static int configured[2][64] = {{0}};
+  auto kern = p.G <= 4 ? kv4_decode_kernel<T, D, GS, true> : kv4_decode_kernel<T, D, GS, false>;
+  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured[p.G <= 4]));
+  b2l_launch(kern, grid, block, (size_t)pl.smem, st, p);
+  B2L_LAUNCH_CHECK();
+  b2l_launch(kv4_decode_merge_kernel<T, D>, dim3((unsigned)p.batch, (unsigned)p.Hq), dim3(256), (size_t)0, st, p);
+  B2L_LAUNCH_CHECK();
+  return B2L_OK;
+}
+
+int64_t part_rows(const Int4Plan& pl, int G) { return 2ll * pl.grid * pl.HB * G; }
+
+}  // namespace
+
+extern "C" int64_t b2l_flash_decoding_int4_workspace_bytes(int64_t batch, int num_q_heads, int num_kv_heads, int head_dim, int group,
+                                                           int64_t max_seq_len) {
+  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || !kv4::shape_ok(head_dim, group)) return 0;
+  const int G = num_q_heads / num_kv_heads;
+  if (G > 8 * kMaxConsumers) return 0;
+  const Int4Plan pl = make_plan(batch, G, num_kv_heads, head_dim, group, max_seq_len);
+  const int64_t rows = batch < kMaxBatch ? batch : kMaxBatch;
+  return part_rows(pl, G) * (head_dim + 2) * 4 + rows * (num_kv_heads / pl.HB) * 8 + 16;
+}
+
+extern "C" int b2l_flash_decoding_int4(void* out, const void* q, const void* cache, int64_t cache_row_stride, int64_t max_tokens,
+                                       const void* b_req_tokens_table, int64_t table_req_stride, int64_t table_seq_stride,
+                                       int64_t table_requests, int64_t table_width, const void* b_req_idx, int req_idx_width,
+                                       const void* b_seq_len, int seq_len_width, int64_t batch, int num_q_heads, int num_kv_heads,
+                                       int head_dim, int group, int64_t max_seq_len, float qk_scale, int64_t q_batch_stride,
+                                       int64_t q_head_stride, int64_t o_batch_stride, int64_t o_head_stride, void* workspace,
+                                       int64_t workspace_bytes, int dtype, void* stream) {
+  B2L_REQUIRE(out && q && cache && b_req_tokens_table && b_req_idx && b_seq_len, "flash_decoding_int4: null pointer");
+  B2L_REQUIRE(num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0,
+              "flash_decoding_int4: num_q_heads (%d) must be a multiple of num_kv_heads (%d)", num_q_heads, num_kv_heads);
+  B2L_REQUIRE(num_q_heads / num_kv_heads <= 8 * kMaxConsumers, "flash_decoding_int4: more than %d query heads to a kv head", 8 * kMaxConsumers);
+  B2L_REQUIRE(num_q_heads <= 65535, "flash_decoding_int4: too many heads");
+  B2L_REQUIRE(kv4::shape_ok(head_dim, group), "flash_decoding_int4: head_dim %d with groups of %d (head_dim 32, 64 or 128; groups of 32, 64 or 128, at most head_dim)",
+              head_dim, group);
+  B2L_REQUIRE((req_idx_width == 4 || req_idx_width == 8) && (seq_len_width == 4 || seq_len_width == 8),
+              "flash_decoding_int4: index widths must be 4 or 8");
+  B2L_REQUIRE(cache_row_stride >= kv4::row_bytes(num_kv_heads, head_dim, group) && cache_row_stride % 16 == 0 && (uintptr_t)cache % 16 == 0,
+              "flash_decoding_int4: cache rows must be 16-byte aligned and hold %lld bytes",
+              (long long)kv4::row_bytes(num_kv_heads, head_dim, group));
+  B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "flash_decoding_int4: dtype %d", dtype);
+  B2L_REQUIRE(batch >= 0 && max_tokens > 0 && table_requests >= 0 && table_width >= 0 && max_seq_len < (1ll << 31) - 256,
+              "flash_decoding_int4: bad shape");
+  if (batch == 0) return B2L_OK;
+  const int G = num_q_heads / num_kv_heads, elem = 2;
+  const Int4Plan pl = make_plan(batch, G, num_kv_heads, head_dim, group, max_seq_len);
+  B2L_REQUIRE(pl.smem <= b2l_max_smem_optin(), "flash_decoding_int4: cache rows too long");
+  B2L_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
+                  workspace_bytes >= b2l_flash_decoding_int4_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, group, max_seq_len),
+              "flash_decoding_int4: workspace too small");
+  Int4DecodeParams p;
+  p.q_bs = q_batch_stride; p.q_hs = q_head_stride; p.o_bs = o_batch_stride; p.o_hs = o_head_stride;
+  p.cache = (const uint8_t*)cache; p.row_stride = cache_row_stride; p.max_tokens = max_tokens;
+  p.table = (const int32_t*)b_req_tokens_table; p.tab_rs = table_req_stride; p.tab_cs = table_seq_stride;
+  p.requests = table_requests; p.width = table_width;
+  p.req_w = req_idx_width; p.len_w = seq_len_width;
+  p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = G; p.HB = pl.HB; p.qblocks = pl.qblocks; p.TS = pl.TS;
+  p.stages = pl.stages; p.pitch = pl.pitch;
+  p.most = max_seq_len < table_width ? max_seq_len : table_width;
+  if (p.most < 0) p.most = 0;
+  p.q_vec = (uintptr_t)q % 16 == 0 && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0;
+  p.scale_log2 = qk_scale * 1.4426950408889634f;
+  p.ws_o = (float*)workspace;
+  p.ws_ml = p.ws_o + part_rows(pl, G) * head_dim;
+  p.ws_info = (int2*)(p.ws_ml + part_rows(pl, G) * 2);
+  cudaStream_t st = (cudaStream_t)stream;
+  for (int64_t b0 = 0; b0 < batch; b0 += kMaxBatch) {
+    p.batch = (int)(batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch);
+    p.q = (const char*)q + b0 * q_batch_stride * elem;
+    p.out = (char*)out + b0 * o_batch_stride * elem;
+    p.req_idx = (const char*)b_req_idx + b0 * req_idx_width;
+    p.seq_len = (const char*)b_seq_len + b0 * seq_len_width;
+    int rc;
+    if (dtype == B2L_F16) { KV4_DISPATCH_SHAPE(head_dim, group, { rc = launch_int4_decode<__half, D, GS>(p, pl, st); }); }
+    else { KV4_DISPATCH_SHAPE(head_dim, group, { rc = launch_int4_decode<__nv_bfloat16, D, GS>(p, pl, st); }); }
+    if (rc != B2L_OK) return rc;
+  }
+  return B2L_OK;
+}

@@ -10,6 +10,8 @@ from .flashdecoding import flash_decoding
 from .fused_moe import fused_moe, grouped_experts, moe_align_block_size, route_sigmoid_groups, route_topk
 from .gated_linear import gated_linear_scan, head_mix, head_norm_gate, mlstm, mlstm_head_floats, swiglu_scaled
 from .hyper_stream import stream_embed, stream_mix
+from .kv_int4 import (flash_decoding_int4, kv_int4_row_bytes, read_kv_buffer_int4, rope_kv_write_int4,
+                      update_kv_buffer_int4)
 from .latent import head_linear, latent_prepare, rope_heads, rope_table
 from .linear import linear, linear_simt
 from .parallel_stream import branch_sum_residual, depth_mix_norms, embed_rmsnorm, gelu_mul_gather
@@ -21,6 +23,7 @@ from .ssm import causal_conv_silu, decay_attention, gated_group_norm, gated_scan
 from .tanh_norm import tanh_norm_stream
 from .rope_emb import rope_emb_forward, rope_emb_inplace, rope_kv_write
 from .sampling import argmax_rows
+from .slot_maps import build_slot_maps
 from .skip_rmsnorm import can_fuse_int8_quant, skip_rmsnorm, skip_rmsnorm_quant_int8
 from .swiglu import swiglu_forward
 from .update_kv_buffer import update_kv_buffer, update_kv_buffer_split
@@ -79,6 +82,12 @@ __all__ = [
     "rope_emb_forward",
     "rope_emb_inplace",
     "rope_kv_write",
+    "rope_kv_write_int4",
+    "update_kv_buffer_int4",
+    "read_kv_buffer_int4",
+    "kv_int4_row_bytes",
+    "flash_decoding_int4",
+    "build_slot_maps",
     "skip_rmsnorm",
     "skip_rmsnorm_quant_int8",
     "can_fuse_int8_quant",
