@@ -172,6 +172,19 @@ int b2l_flash_decoding_int4(void* out, const void* q, const void* cache, int64_t
                             int head_dim, int group, int64_t max_seq_len, float qk_scale, int64_t q_batch_stride,
                             int64_t q_head_stride, int64_t o_batch_stride, int64_t o_head_stride, void* workspace,
                             int64_t workspace_bytes, int dtype, void* stream);
+/* Portions of prompts over that cache, causal: the new_len[b] rows of q [total_tokens, Hq, D] from start_loc[b] on stand at the positions
+ * seq_len[b] - new_len[b], ... and see the cached tokens up to their own.  Rows of no sequence are not written, a row that sees
+ * nothing is zero; rows past total_tokens, new tokens past max_new_len and keys past max_seq_len or the table's width do not count. */
+int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64_t total_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                                                 int group, int64_t max_seq_len);
+int b2l_flash_attention_int4(void* out, const void* q, const void* cache, int64_t cache_row_stride, int64_t max_tokens,
+                             const void* b_start_loc, int start_width, const void* b_new_len, int new_width,
+                             const void* b_req_tokens_table, int64_t table_req_stride, int64_t table_seq_stride,
+                             int64_t table_requests, int64_t table_width, const void* b_req_idx, int req_width,
+                             const void* b_seq_len, int len_width, int64_t batch, int64_t total_tokens, int64_t max_new_len,
+                             int num_q_heads, int num_kv_heads, int head_dim, int group, int64_t max_seq_len, float qk_scale,
+                             int64_t q_tok_stride, int64_t q_head_stride, int64_t o_tok_stride, int64_t o_head_stride,
+                             void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 /* Slot maps of a ragged step: start[b] = sum of new_len over the requests before b, length[b] = ctx_len[b] + new_len[b] (int32 [batch]);
  * for token t of the flat batch, the j-th new one of request b: position[t] = ctx_len[b] + j (int64), rows[t] (int32) =
  * table[req_idx[b], position], or, with pool_rows, pool_rows[t], which is entered there.  Tokens behind the last request: row -1,

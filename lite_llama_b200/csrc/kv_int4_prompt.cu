@@ -1,0 +1,759 @@
+// flash_attention_int4: portions of prompts over a cache held in 4 bits (kv_int4.cuh), on the 5th-generation tensor cores.
+//
+// Query j of a sequence's new tokens stands at position len - new + j and sees the cached tokens up to itself.
+//
+// A CTA works on 256 query rows of one kv head -- rows are (token, query head of the group), so that a key tile serves all heads of
+// the group and a portion of few tokens still fills a tile -- as two tiles of 128 rows, over tiles of 128 keys:
+//   warps 0, 1    tensor-core issuers: the scores S = Q K^T, and O += P V (A = P from tensor memory)
+//   warps 4 - 7   K and V rows from the cache through the request table, codes to halves minimum + scale * code, into the operands'
+//                 swizzled layout.  A word of eight codes turns into one 16-byte chunk in the order 0 4 1 5 2 6 3 7: with the queries stored in
+//                 the same order the scores are the same, and the outputs' order is undone at the end.
+//   warps 8 - 15  softmax, a thread to a row of either tile: the row's scores from tensor memory once, P written back, the output rescaled
+//                 where the running maximum rises by more than 2^8 (both by one factor, hence exact)
+// Tensor memory: S | P0 P1 | O0 | O1, as in flash_attention_tc.cu.
+// The operands are halves for both activation types: elements are rounded to 11 bits (as the 16-bit cache of an fp16 model rounds
+// them), which for bf16 models are three bits more than reading the cache into their type would leave; elements of those beyond 65504
+// count as 65504.  Queries of bf16 models are scaled by a power of two per row.  Probabilities are rounded to 11 bits, as in
+// flash_attention_tc.cu; sums, maxima and outputs are held in 32.
+// A value that is NaN enters as 0 and makes NaN of the rows that see it at the end, since 0 * NaN would reach the rows that do not.
+//
+// Work: key tiles of all row blocks of all sequences, in equal shares over one wave of CTAs (lengths are device data).  A row block in
+// several shares leaves parts in the workspace, which a second kernel adds up.
+#include "kv_int4.cuh"
+#include "attention_tmem.cuh"
+#include <climits>
+#include <type_traits>
+
+namespace kv4p {
+
+constexpr int kBM = 128, kBN = 128, kRows = 2 * kBM;
+constexpr int kThreads = 512, kKStages = 2, kVStages = 2, kSegs = 4;
+constexpr int kMaxBatch = 1024;
+constexpr int kMinSteps = 2;                      // key tiles of a share: below that the parts cost more than the tiles
+
+struct Params {
+  const void* q; int64_t q_ts, q_hs; int q_vec;
+  void* out; int64_t o_ts, o_hs; int o_vec;
+  const uint8_t* cache; int64_t row_stride, max_tokens;
+  const int32_t* table; int64_t tab_rs, tab_cs, requests;
+  const void *start, *fresh, *req, *len;
+  int start_w, fresh_w, req_w, len_w;
+  int batch, Hkv, G;
+  int64_t total, max_new, most;
+  float scale_log2;
+  float* ws_o; float2* ws_ml; int2* ws_info; int* ws_item;
+};
+
+// a sequence: its new tokens begin at row `start` of q, the first stands at position ctx, keys below `keys` are cached
+struct Seq { int m, ctx, keys; };
+__device__ __forceinline__ Seq sequence(const Params& p, int b) {
+  const int64_t n = load_index(p.len, b, p.len_w), f = load_index(p.fresh, b, p.fresh_w), s = load_index(p.start, b, p.start_w);
+  const int64_t r = load_index(p.req, b, p.req_w);
+  Seq q;
+  int64_t m = f < 0 ? 0 : f, ctx = (n < 0 ? 0 : n) - m;
+  if (m > p.max_new) m = p.max_new;
+  if (s < 0 || s >= p.total) m = 0;
+  else if (m > p.total - s) m = p.total - s;
+  q.m = (int)m;
+  q.ctx = (int)(ctx < -(1ll << 30) ? -(1ll << 30) : ctx > (1ll << 30) ? (1ll << 30) : ctx);
+  q.keys = r < 0 || r >= p.requests || n <= 0 ? 0 : (int)(n < p.most ? n : p.most);
+  return q;
+}
+__device__ __forceinline__ int row_blocks(const Seq& s, int G) { return (int)(((int64_t)s.m * G + kRows - 1) / kRows); }
+// key tiles of tile t of row block rb: up to its last row's position (0: no rows; a tile that sees nothing takes one step for its zeros)
+__device__ __forceinline__ int key_tiles(const Seq& s, int G, int rb, int t) {
+  const int64_t first = (int64_t)rb * kRows + t * kBM, rows = (int64_t)s.m * G;
+  if (first >= rows) return 0;
+  const int64_t last = (first + kBM < rows ? first + kBM : rows) - 1;
+  int64_t k = s.ctx + last / G + 1;
+  if (k > s.keys) k = s.keys;
+  return k > 0 ? (int)((k + kBN - 1) / kBN) : 1;
+}
+__device__ __forceinline__ int block_steps(const Seq& s, int G, int rb) {
+  const int a = key_tiles(s, G, rb, 0), b = key_tiles(s, G, rb, 1);
+  return a > b ? a : b;
+}
+
+struct __align__(16) Ctl {
+  uint64_t q_full[2], k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
+  uint64_t s_full[2], s_free, p_full[2], pv_done[2], seg_done[kSegs];
+  int nan_at[kSegs][4];                           // first key whose value group is NaN
+  uint32_t tmem_base;
+};
+static_assert(sizeof(Ctl) <= 512, "control block");
+
+// steps [j0, j1) of a row block
+struct Segment { int b, kvh, rb, j0, j1, steps, item; };
+
+#define kv4_wait(bar, parity) mbar_wait_short_at<true>((bar), (parity), b2l_file_hash(__FILE__), __LINE__)
+
+// codes of a word to halves minimum + scale * code, in the order 0 4 1 5 2 6 3 7
+__device__ __forceinline__ uint4 to_halves(uint32_t w, __half2 s, __half2 m) {
+  const uint32_t magic = 0x64006400u;             // 1024 + code
+  const __half2 big = *reinterpret_cast<const __half2*>(&magic);
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = ((w >> (4 * i)) & 0x000f000fu) | magic;
+    const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&x), big), s, m);
+    r[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+// the same for scales or minima that may lead past the halves' range, or NaN
+__device__ __noinline__ uint4 to_halves_wide(uint32_t w, float s, float m) {
+  uint32_t r[4];
+  for (int i = 0; i < 4; ++i) {
+    float x = fmaf((float)(w >> (4 * i) & 15u), s, m), y = fmaf((float)(w >> (4 * i + 16) & 15u), s, m);
+    x = x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;
+    y = y > 65504.f ? 65504.f : y < -65504.f ? -65504.f : y;
+    r[i] = pack2<__half>(x, y);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+template <typename T> struct Group;
+template <> struct Group<__half> {
+  static constexpr uint32_t kAdd = 0x18001800u;   // carries into the top bit from 2048 on
+  static __device__ __forceinline__ __half2 both(uint32_t g, int which) {
+    const uint32_t x = __byte_perm(g, g, which ? 0x3232 : 0x1010);
+    return *reinterpret_cast<const __half2*>(&x);
+  }
+};
+template <> struct Group<__nv_bfloat16> {
+  static constexpr uint32_t kAdd = 0x3b003b00u;
+  static __device__ __forceinline__ __half2 both(uint32_t g, int which) {
+    const float2 f = kv4::scale_min<__nv_bfloat16>(g);
+    return __float2half2_rn(which ? f.y : f.x);
+  }
+};
+
+template <typename T, int D, int GS>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p) {
+  constexpr int DP = D < 64 ? 64 : D;             // a row of an operand is whole swizzle atoms of 64 halves
+  constexpr int kTile = kBN * DP * 2, kHalf = kBN * 64 * 2, NG = D / GS;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Ctl* ctl = reinterpret_cast<Ctl*>(smem);
+  uint8_t* q_s = smem + 1024;
+  uint8_t* k_ring = q_s + 2 * kTile;
+  uint8_t* v_ring = k_ring + kKStages * kTile;
+  int64_t* prefix = reinterpret_cast<int64_t*>(v_ring + kVStages * kTile);   // steps of the sequences before, [batch + 1]
+  int* items = reinterpret_cast<int*>(prefix + p.batch + 1);                 // row blocks (of all kv heads) before
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.G;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&ctl->q_full[t], 4); mbar_init(&ctl->s_full[t], 1); mbar_init(&ctl->p_full[t], 4); mbar_init(&ctl->pv_done[t], 1);
+    }
+    for (int s = 0; s < kKStages; ++s) { mbar_init(&ctl->k_full[s], 4); mbar_init(&ctl->k_empty[s], 1); }
+    for (int s = 0; s < kVStages; ++s) { mbar_init(&ctl->v_full[s], 4); mbar_init(&ctl->v_empty[s], 1); }
+    for (int s = 0; s < kSegs; ++s) mbar_init(&ctl->seg_done[s], 8);
+    mbar_init(&ctl->s_free, 4);
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl->tmem_base, 512);
+    tmem_relinquish();
+    pdl_launch_dependents();                      // only once this CTA owns its tensor memory
+  }
+  pdl_wait_prior();                               // lengths, table, cache, q are upstream data
+
+  // ---- steps and row blocks per sequence (a warp each), then their sums ----
+  for (int b = warp; b < p.batch; b += kThreads / 32) {
+    const Seq s = sequence(p, b);
+    const int nb = row_blocks(s, G);
+    int n = 0;
+    for (int rb = lane; rb < nb; rb += 32) n += block_steps(s, G, rb);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) {
+      prefix[b + 1] = (int64_t)n * p.Hkv;
+      items[b] = nb * p.Hkv;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) {
+    int64_t steps = 0;
+    int blocks = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      const int b = b0 + lane;
+      int64_t s = b < p.batch ? prefix[b + 1] : 0;
+      const int own = b < p.batch ? items[b] : 0;
+      int k = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, s, o);
+        const int y = __shfl_up_sync(0xffffffffu, k, o);
+        if (lane >= o) { s += x; k += y; }
+      }
+      if (b < p.batch) {
+        prefix[b + 1] = steps + s;
+        items[b] = blocks + k - own;
+        if (blockIdx.x == 0) p.ws_item[b] = blocks + k - own;
+      }
+      steps += __shfl_sync(0xffffffffu, s, 31);
+      blocks += __shfl_sync(0xffffffffu, k, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+  }
+  __syncthreads();
+  const uint32_t tmem_base = ctl->tmem_base;
+
+  const int64_t total = prefix[p.batch];
+  const int64_t worth = (total + kMinSteps - 1) / kMinSteps;
+  const int64_t shares = worth < gridDim.x ? worth : gridDim.x;
+  int64_t step = 0, step_end = 0;
+  if (blockIdx.x < shares) {
+    step = blockIdx.x * total / shares;
+    step_end = (blockIdx.x + 1) * total / shares;
+  }
+  auto next = [&](Segment& g, Seq& s) -> bool {
+    if (step >= step_end) return false;
+    int lo = 0, n = p.batch;                      // the last sequence that begins at or before `step` and has steps
+    while (n > 1) {
+      const int half = n / 2;
+      if (prefix[lo + half] <= step) { lo += half; n -= half; }
+      else n = half;
+    }
+    s = sequence(p, lo);
+    const int64_t x = step - prefix[lo];
+    const int per_head = (int)((prefix[lo + 1] - prefix[lo]) / p.Hkv);
+    const int nb = row_blocks(s, G);
+    g.b = lo;
+    g.kvh = (int)(x / per_head);
+    int y = (int)(x - (int64_t)g.kvh * per_head);
+    g.rb = 0;
+    for (; g.rb < nb - 1; ++g.rb) {
+      const int n_rb = block_steps(s, G, g.rb);
+      if (y < n_rb) break;
+      y -= n_rb;
+    }
+    g.steps = block_steps(s, G, g.rb);
+    g.j0 = y;
+    const int64_t left = step_end - step;
+    g.j1 = left < g.steps - y ? y + (int)left : g.steps;
+    g.item = items[lo] + g.kvh * nb + g.rb;
+    step += g.j1 - g.j0;
+    return true;
+  };
+
+  Segment seg;
+  Seq seq;
+  // registers per lane: 16 warps x 128 at launch = 4 x 32 + 4 x 96 + 8 x 192
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp < 2) {
+      // ===================== tensor-core issuers: warp 0 the scores, warp 1 P V =====================
+      constexpr uint32_t idesc_s = umma_idesc(1u, 0u, 0u, 0u, 0u, kBM, kBN);
+      constexpr uint32_t idesc_o = umma_idesc(1u, 0u, 0u, 0u, 1u, kBM, DP);
+      int ring = 0;
+      uint32_t phase = 0, free_phase = 1, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      while (next(seg, seq)) {
+        const int nt[2] = {key_tiles(seq, G, seg.rb, 0), key_tiles(seq, G, seg.rb, 1)};
+        for (int j = seg.j0; j < seg.j1; ++j) {
+          kv4_wait(warp == 0 ? &ctl->k_full[ring] : &ctl->v_full[ring], phase);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= nt[t]) continue;
+            const bool last = t == 1 || j >= nt[1];              // the key tile's last reader
+            if (warp == 0) {
+              if (j == seg.j0) { kv4_wait(&ctl->q_full[t], q_phase[t]); q_phase[t] ^= 1u; }
+              kv4_wait(&ctl->s_free, free_phase);
+              free_phase ^= 1u;
+              tc_fence_after();
+              if (elect_one()) {
+                const uint64_t q_desc = umma_desc_sw128_kmajor(smem_u32(q_s + t * kTile));
+                const uint64_t k_desc = umma_desc_sw128_kmajor(smem_u32(k_ring + ring * kTile));
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                  const uint64_t off = (uint64_t)(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4);
+                  umma_f16(tmem_base, q_desc + off, k_desc + off, idesc_s, kk ? 1u : 0u);
+                }
+                if (last) tc_commit(&ctl->k_empty[ring]);
+                tc_commit(&ctl->s_full[t]);
+              }
+            } else {
+              kv4_wait(&ctl->p_full[t], p_phase[t]);
+              p_phase[t] ^= 1u;
+              tc_fence_after();
+              if (elect_one()) {
+                const uint32_t v_addr = smem_u32(v_ring + ring * kTile);
+#pragma unroll
+                for (int kk = 0; kk < kBN / 16; ++kk) {
+                  // 16 keys per step = two 8-row groups of 1024 B; elements 64 .. 127 are one LBO away
+                  const uint64_t v_desc = umma_desc_sw128_mnmajor(v_addr + kk * 2048, kHalf, 1024);
+                  umma_ts(tmem_base + 256u + (uint32_t)t * 128u, tmem_base + 128u + (uint32_t)t * 64u + kk * 8, v_desc, idesc_o,
+                          (j > seg.j0 || kk) ? 1u : 0u);
+                }
+                if (last) tc_commit(&ctl->v_empty[ring]);
+                tc_commit(&ctl->pv_done[t]);
+              }
+            }
+            __syncwarp();
+          }
+          if (++ring == (warp == 0 ? kKStages : kVStages)) { ring = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp < 8) {
+    // ===================== cache rows to operands =====================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    constexpr int NWD = D == 128 ? 2 : 1;         // words of a row and side that a thread takes (eight threads to a row)
+    const int tid = threadIdx.x - 128, l = tid & 7, kq = tid >> 3;
+    const bool on = l < D / 8;                    // D = 32: half of the threads store zeros
+    const uint32_t spot = (uint32_t)(kq * 128 + ((l ^ (kq & 7)) << 4));
+    struct Raw { uint32_t w[4][NWD], g[4][NWD]; };
+    // 64 keys (four rows of this thread) of one side
+    auto fetch = [&](Raw& x, const int (&rows)[8], int half, int side, int kvh) {
+      const int64_t off = (int64_t)kvh * kv4::head_bytes(D, GS);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = rows[half * 4 + i];
+#pragma unroll
+        for (int k = 0; k < NWD; ++k) {
+          x.w[i][k] = x.g[i][k] = 0u;
+          if (row >= 0 && on) {
+            const uint32_t* head = reinterpret_cast<const uint32_t*>(p.cache + (int64_t)row * p.row_stride + off);
+            x.w[i][k] = __ldcg(head + side * (D / 8) + k * 8 + l);
+            x.g[i][k] = __ldcg(head + D / 4 + side * NG + (k * 8 + l) * 8 / GS);
+          }
+        }
+      }
+    };
+    auto store = [&](const Raw& x, uint8_t* tile, int half, int side, int key0, int slot) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < NWD; ++k) {
+          const uint32_t g = x.g[i][k];
+          uint4 v;
+          if ((((g & 0x7fff7fffu) + Group<T>::kAdd) & 0x80008000u) == 0u) {
+            v = to_halves(x.w[i][k], Group<T>::both(g, 0), Group<T>::both(g, 1));
+          } else {
+            float2 f = kv4::scale_min<T>(g);
+            if (side == 1 && (f.x != f.x || f.y != f.y)) {
+              f = make_float2(0.f, 0.f);
+              atomicMin(&ctl->nan_at[slot][(k * 8 + l) * 8 / GS], key0 + half * 64 + i * 16 + kq);
+            }
+            v = to_halves_wide(x.w[i][k], f.x, f.y);
+          }
+          *reinterpret_cast<uint4*>(tile + k * kHalf + (half * 64 + i * 16) * 128 + spot) = v;
+        }
+    };
+    auto entries = [&](int (&rows)[8], const Segment& g, const Seq& s, int j) {
+      const int32_t* entry = p.table + load_index(p.req, g.b, p.req_w) * p.tab_rs;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = j * kBN + i * 16 + kq;
+        rows[i] = -1;
+        if (key < s.keys) {
+          const int row = ld_upstream(entry + (int64_t)key * p.tab_cs);
+          rows[i] = row >= 0 && row < p.max_tokens ? row : 0;
+        }
+      }
+    };
+    int ks = 0, vs = 0, nseg = 0;
+    uint32_t kp = 1, vp = 1;
+    bool more = next(seg, seq);
+    int j = more ? seg.j0 : 0;
+    int rows[8];
+    Raw a, b;
+    if (more) {
+      entries(rows, seg, seq, j);
+      fetch(a, rows, 0, 0, seg.kvh);
+      fetch(b, rows, 1, 0, seg.kvh);
+    }
+    while (more) {
+      const int slot = nseg % kSegs, key0 = j * kBN, kvh = seg.kvh;
+      if (j == seg.j0) {
+        if (nseg >= kSegs) kv4_wait(&ctl->seg_done[slot], (uint32_t)(nseg / kSegs - 1) & 1u);
+        if (tid < 4) ctl->nan_at[slot][tid] = INT_MAX;
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+      }
+      uint8_t* kt = k_ring + ks * kTile;
+      uint8_t* vt = v_ring + vs * kTile;
+      kv4_wait(&ctl->k_empty[ks], kp);
+      store(a, kt, 0, 0, key0, slot);
+      fetch(a, rows, 0, 1, kvh);
+      store(b, kt, 1, 0, key0, slot);
+      fetch(b, rows, 1, 1, kvh);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->k_full[ks]);
+      if (++ks == kKStages) { ks = 0; kp ^= 1u; }
+      // the next tile's rows
+      if (++j == seg.j1) {
+        more = next(seg, seq);
+        j = more ? seg.j0 : 0;
+        ++nseg;
+      }
+      if (more) entries(rows, seg, seq, j);
+      kv4_wait(&ctl->v_empty[vs], vp);
+      store(a, vt, 0, 1, key0, slot);
+      if (more) fetch(a, rows, 0, 0, seg.kvh);
+      store(b, vt, 1, 1, key0, slot);
+      if (more) fetch(b, rows, 1, 0, seg.kvh);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->v_full[vs]);
+      if (++vs == kVStages) { vs = 0; vp ^= 1u; }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    // ===================== softmax: thread = query row = TMEM lane of tile t =====================
+    const int t = (warp - 8) >> 2, quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quad * 32) << 16);
+    const uint32_t pb = lane_base + 128u + (uint32_t)t * 64u, ob = lane_base + 256u + (uint32_t)t * 128u;
+    constexpr float kLazy = 8.0f;                 // log2 units: rescale only when a tile exceeds m_used by 2^8
+    uint32_t s_phase = 0, pv_phase = 0;
+    int nseg = 0;
+    for (; next(seg, seq); ++nseg) {
+      const int nt = key_tiles(seq, G, seg.rb, t), j_end = nt < seg.j1 ? nt : seg.j1;
+      const int64_t r = (int64_t)seg.rb * kRows + t * kBM + row;
+      const int token = (int)(r / G), head = seg.kvh * G + (int)(r - (int64_t)token * G);
+      const bool live = token < seq.m;
+      const int64_t place = live ? load_index(p.start, seg.b, p.start_w) + token : 0;
+      const int64_t part = ((int64_t)blockIdx.x * 2 + (seg.j0 == 0 ? 1 : 0)) * kRows + t * kBM + row;
+      const bool whole = seg.j0 == 0 && seg.j1 == seg.steps;
+      float m_used = -INFINITY, l_run = 0.f;      // m_used: the maximum the accumulated P / O / l are scaled by
+      if (j_end > seg.j0) {
+        // the row of Q, in the operands' order
+        float scale = p.scale_log2;
+        {
+          const T* src = reinterpret_cast<const T*>(p.q) + place * p.q_ts + (int64_t)(live ? head : 0) * p.q_hs;
+          uint32_t w[D / 2];
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (live) {
+              if (p.q_vec) {
+                x = *reinterpret_cast<const uint4*>(src + c * 8);
+              } else {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(src + c * 8);
+                x = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+              }
+            }
+            w[c * 4] = x.x; w[c * 4 + 1] = x.y; w[c * 4 + 2] = x.z; w[c * 4 + 3] = x.w;
+          }
+          if (std::is_same<T, __nv_bfloat16>::value) {
+            float big = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 2; ++c)
+              big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w[c] << 16)), fabsf(__uint_as_float(w[c] & 0xffff0000u))));
+            int e = 8 - ((int)(__float_as_uint(big) >> 23) - 127);
+            if (!(big < INFINITY) || big == 0.f) e = 0;
+            e = e < -100 ? -100 : e > 100 ? 100 : e;
+            const float up = __int_as_float((e + 127) << 23);
+            scale *= __int_as_float((127 - e) << 23);
+#pragma unroll
+            for (int c = 0; c < D / 2; ++c)
+              w[c] = pack2<__half>(__uint_as_float(w[c] << 16) * up, __uint_as_float(w[c] & 0xffff0000u) * up);
+          }
+          uint8_t* dst = q_s + t * kTile + row * 128;
+#pragma unroll
+          for (int c = 0; c < DP / 8; ++c) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (c < D / 8) {
+              const uint32_t* y = w + (c < D / 8 ? c : 0) * 4;
+              x = make_uint4(__byte_perm(y[0], y[2], 0x5410), __byte_perm(y[0], y[2], 0x7632), __byte_perm(y[1], y[3], 0x5410),
+                             __byte_perm(y[1], y[3], 0x7632));
+            }
+            *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalf + (((c & 7) ^ (row & 7)) << 4)) = x;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->q_full[t]);
+        }
+        const int pos = seq.ctx + token, see = live ? (pos < seq.keys - 1 ? pos : seq.keys - 1) : -1;   // last key that counts
+        const int see_all = __reduce_min_sync(0xffffffffu, live ? see : INT_MAX);
+
+        auto tile = [&](const int j, auto masked) {
+          constexpr bool kMasked = decltype(masked)::value;
+          kv4_wait(&ctl->s_full[t], s_phase);
+          s_phase ^= 1u;
+          tc_fence_after();
+          uint32_t sv[kBN];
+#pragma unroll
+          for (int c = 0; c < kBN; c += 32) tmem_ld_32x32b_x32(lane_base + c, *reinterpret_cast<uint32_t(*)[32]>(sv + c));
+          tc_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->s_free);
+          const int limit = see - j * kBN;        // masked tile: key column i is visible iff i <= limit
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < kBN; i += 8) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float x = __uint_as_float(sv[i + 2 * c]), y = __uint_as_float(sv[i + 2 * c + 1]);
+              if (kMasked) {
+                x = i + 2 * c <= limit ? x : -INFINITY;
+                y = i + 2 * c + 1 <= limit ? y : -INFINITY;
+              }
+              mx[c] = max3(mx[c], x, y);
+            }
+          }
+          const float m_tile = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
+          const bool grow = m_tile > m_used + kLazy;               // first tile: m_used = -inf -> true
+          const float m_new = grow ? m_tile : m_used;
+          const float base = m_new == -INFINITY ? 0.f : m_new;     // nothing visible yet: avoid inf - inf
+          const float alpha = grow ? fast_exp2(m_used - base) : 1.0f;
+          const uint64_t scale2 = f32x2(scale, scale), base2 = f32x2(-base, -base);
+          uint64_t lsum2 = 0ull;
+          if (j > seg.j0) { kv4_wait(&ctl->pv_done[t], pv_phase); pv_phase ^= 1u; tc_fence_after(); }
+#pragma unroll
+          for (int c = 0; c < kBN; c += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float p0, p1;
+              f32x2_split(f32x2_fma(f32x2(__uint_as_float(sv[c + i]), __uint_as_float(sv[c + i + 1])), scale2, base2), p0, p1);
+              p0 = fast_exp2(p0);
+              p1 = fast_exp2(p1);
+              if (kMasked) {
+                p0 = c + i <= limit ? p0 : 0.f;
+                p1 = c + i + 1 <= limit ? p1 : 0.f;
+              }
+              lsum2 = f32x2_add(lsum2, f32x2(p0, p1));
+              pk[i >> 1] = pack2<__half>(p0, p1);
+            }
+            tmem_st_32x32b_x16(pb + (c >> 1), pk);
+          }
+          float l0, l1;
+          f32x2_split(lsum2, l0, l1);
+          l_run = l_run * alpha + (l0 + l1);
+          m_used = m_new;
+          if (j > seg.j0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+              uint32_t v[32];
+              tmem_ld_32x32b_x32(ob + c, v);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+              tmem_st_32x32b_x32(ob + c, v);
+            }
+          }
+          tc_wait_st_();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->p_full[t]);
+        };
+        for (int j = seg.j0; j < j_end; ++j) {
+          if ((j + 1) * kBN - 1 > see_all) tile(j, std::true_type{});
+          else tile(j, std::false_type{});
+        }
+        kv4_wait(&ctl->pv_done[t], pv_phase);
+        pv_phase ^= 1u;
+        tc_fence_after();
+        // columns are in the operands' order: of eight, 0 4 1 5 2 6 3 7
+        const float inv = whole ? (l_run == 0.f ? 0.f : 1.0f / l_run) : 1.f;
+        T* orow = reinterpret_cast<T*>(p.out) + place * p.o_ts + (int64_t)(live ? head : 0) * p.o_hs;
+        float* prow = p.ws_o + part * D;
+        constexpr int kFrom[8] = {0, 2, 4, 6, 1, 3, 5, 7};
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(ob + c, v);          // warp-collective: outside the row predicate
+          tc_wait_ld();
+          const bool nan = see >= ctl->nan_at[nseg % kSegs][c / GS];
+          if (live) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float x[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] = nan ? __int_as_float(0x7fc00000) : __uint_as_float(v[i + kFrom[k]]) * inv;
+              if (whole) {
+                const uint4 w = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+                if (p.o_vec) {
+                  *reinterpret_cast<uint4*>(orow + c + i) = w;
+                } else {
+#pragma unroll
+                  for (int k = 0; k < 8; ++k) orow[c + i + k] = from_f32<T>(x[k]);
+                }
+              } else {
+                *reinterpret_cast<float4*>(prow + c + i) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(prow + c + i + 4) = make_float4(x[4], x[5], x[6], x[7]);
+              }
+            }
+          }
+        }
+      }
+      if (!whole) {
+        p.ws_ml[part] = make_float2(m_used, l_run);
+        if (t == 0 && row == 0) {
+          int* note = reinterpret_cast<int*>(p.ws_info + seg.item);
+          if (seg.j0 == 0) note[0] = blockIdx.x;
+          if (seg.j1 == seg.steps) note[1] = blockIdx.x;
+        }
+      } else if (t == 0 && row == 0) {
+        p.ws_info[seg.item] = make_int2(blockIdx.x, blockIdx.x);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->seg_done[nseg % kSegs]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
+}
+
+// Row blocks that several CTAs met in.  A warp takes rows; the parts of a row are added in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(const Params p) {
+  pdl_prologue();
+  constexpr int E = D / 32, kRowsHere = 32;
+  const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Seq s = sequence(p, b);
+  const int64_t r0 = (int64_t)blockIdx.x * kRowsHere, rows = (int64_t)s.m * p.G;
+  if (r0 >= rows) return;
+  const int rb = (int)(r0 / kRows);
+  const int2 who = __ldcg(p.ws_info + __ldcg(p.ws_item + b) + kvh * row_blocks(s, p.G) + rb);
+  const int n = who.y - who.x + 1;
+  if (n < 2) return;                              // written by its only CTA
+  const int64_t start = load_index(p.start, b, p.start_w);
+  for (int64_t r = r0 + warp; r < r0 + kRowsHere && r < rows; r += 8) {
+    float acc[E], M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    const int64_t in_block = r - (int64_t)rb * kRows;
+    for (int i0 = 0; i0 < n; i0 += 4) {
+      float x[4][E];
+      float2 ml[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k;
+        ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[k][e] = 0.f;
+        if (i < n) {
+          const int64_t part = ((int64_t)(who.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + in_block;
+          ml[k] = __ldcg(p.ws_ml + part);
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[k][e] = __ldcg(p.ws_o + part * D + e * 32 + lane);
+        }
+      }
+      float mm = M;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mm = fmaxf(mm, ml[k].x);
+      const float base = mm == -INFINITY ? 0.f : mm, a = fast_exp2(M - base);
+      L *= a;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= a;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (ml[k].y == 0.f) continue;             // a part of keys that the row does not see: nothing was stored
+        const float w = fast_exp2(ml[k].x - base);
+        L = fmaf(ml[k].y, w, L);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(x[k][e], w, acc[e]);
+      }
+      M = mm;
+    }
+    const int token = (int)(r / p.G), head = kvh * p.G + (int)(r - (int64_t)token * p.G);
+    T* out = reinterpret_cast<T*>(p.out) + (start + token) * p.o_ts + (int64_t)head * p.o_hs;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e * 32 + lane] = from_f32<T>(L == 0.f ? 0.f : acc[e] / L);
+  }
+}
+
+struct Plan { int grid, smem; int64_t items, rows; };
+
+Plan make_plan(int64_t batch, int64_t total, int G, int Hkv, int D, int64_t max_len) {
+  Plan pl;
+  const int DP = D < 64 ? 64 : D;
+  const int64_t rows = batch < kMaxBatch ? batch : kMaxBatch;
+  pl.smem = 1024 + (2 + kKStages + kVStages) * kBN * DP * 2 + (int)(rows + 1) * 8 + (int)rows * 4;
+  pl.items = (cdiv64(total * G, kRows) + rows) * Hkv;
+  const int64_t steps = pl.items * cdiv64(max_len > 0 ? max_len : 1, kBN), worth = cdiv64(steps, kMinSteps);
+  pl.grid = (int)(worth < b2l_num_sms() ? worth : b2l_num_sms());
+  if (pl.grid < 1) pl.grid = 1;
+  pl.rows = 2ll * pl.grid * kRows;
+  return pl;
+}
+
+template <typename T, int D, int GS>
+int launch(const Params& p, const Plan& pl, cudaStream_t st) {
+  static int configured[64] = {0};
+  auto kern = kv4_prompt_kernel<T, D, GS>;
+  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured));
+  b2l_launch(kern, dim3((unsigned)pl.grid), dim3(kThreads), (size_t)pl.smem, st, p);
+  B2L_LAUNCH_CHECK();
+  const int64_t x = cdiv64(p.max_new * p.G, 32);
+  b2l_launch(kv4_prompt_merge_kernel<T, D>, dim3((unsigned)x, (unsigned)p.Hkv, (unsigned)p.batch), dim3(256), (size_t)0, st, p);
+  B2L_LAUNCH_CHECK();
+  return B2L_OK;
+}
+
+}  // namespace kv4p
+
+extern "C" int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64_t total_tokens, int num_q_heads, int num_kv_heads,
+                                                            int head_dim, int group, int64_t max_seq_len) {
+  if (batch <= 0 || total_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || !kv4::shape_ok(head_dim, group))
+    return 0;
+  const kv4p::Plan pl = kv4p::make_plan(batch, total_tokens, num_q_heads / num_kv_heads, num_kv_heads, head_dim, max_seq_len);
+  return pl.rows * (head_dim + 2) * 4 + pl.items * 8 + (int64_t)kv4p::kMaxBatch * 4;
+}
+
+extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* cache, int64_t cache_row_stride, int64_t max_tokens,
+                                        const void* b_start_loc, int start_width, const void* b_new_len, int new_width,
+                                        const void* b_req_tokens_table, int64_t table_req_stride, int64_t table_seq_stride,
+                                        int64_t table_requests, int64_t table_width, const void* b_req_idx, int req_width,
+                                        const void* b_seq_len, int len_width, int64_t batch, int64_t total_tokens, int64_t max_new_len,
+                                        int num_q_heads, int num_kv_heads, int head_dim, int group, int64_t max_seq_len, float qk_scale,
+                                        int64_t q_tok_stride, int64_t q_head_stride, int64_t o_tok_stride, int64_t o_head_stride,
+                                        void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+  using namespace kv4p;
+  const char* what = "flash_attention_int4";
+  B2L_REQUIRE(out && q && cache && b_start_loc && b_new_len && b_req_tokens_table && b_req_idx && b_seq_len, "%s: null pointer", what);
+  B2L_REQUIRE(num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0 && num_kv_heads <= 65535,
+              "%s: num_q_heads (%d) must be a multiple of num_kv_heads (%d)", what, num_q_heads, num_kv_heads);
+  B2L_REQUIRE(kv4::shape_ok(head_dim, group), "%s: head_dim %d with groups of %d (head_dim 32, 64 or 128; groups of 32, 64 or 128, at most head_dim)",
+              what, head_dim, group);
+  for (int w : {start_width, new_width, req_width, len_width}) B2L_REQUIRE(w == 4 || w == 8, "%s: index widths must be 4 or 8", what);
+  B2L_REQUIRE(cache_row_stride >= kv4::row_bytes(num_kv_heads, head_dim, group) && cache_row_stride % 16 == 0 && (uintptr_t)cache % 16 == 0,
+              "%s: cache rows must be 16-byte aligned and hold %lld bytes", what, (long long)kv4::row_bytes(num_kv_heads, head_dim, group));
+  B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "%s: dtype %d", what, dtype);
+  B2L_REQUIRE(batch >= 0 && total_tokens >= 0 && max_tokens > 0 && max_tokens < (1ll << 31) && table_requests >= 0 && table_width >= 0 &&
+                  max_new_len >= 0 && max_new_len < (1ll << 30) && max_seq_len < (1ll << 30), "%s: bad shape", what);
+  if (batch == 0 || total_tokens == 0 || max_new_len == 0) return B2L_OK;
+  const int G = num_q_heads / num_kv_heads;
+  const Plan pl = make_plan(batch, total_tokens, G, num_kv_heads, head_dim, max_seq_len);
+  B2L_REQUIRE(pl.items < (1ll << 31) && total_tokens * G < (1ll << 31), "%s: too many tokens", what);
+  B2L_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
+                  workspace_bytes >= b2l_flash_attention_int4_workspace_bytes(batch, total_tokens, num_q_heads, num_kv_heads, head_dim, group, max_seq_len),
+              "%s: workspace too small", what);
+  Params p;
+  p.q = q; p.q_ts = q_tok_stride; p.q_hs = q_head_stride;
+  p.q_vec = (uintptr_t)q % 16 == 0 && q_tok_stride % 8 == 0 && q_head_stride % 8 == 0;
+  p.out = out; p.o_ts = o_tok_stride; p.o_hs = o_head_stride;
+  p.o_vec = (uintptr_t)out % 16 == 0 && o_tok_stride % 8 == 0 && o_head_stride % 8 == 0;
+  p.cache = (const uint8_t*)cache; p.row_stride = cache_row_stride; p.max_tokens = max_tokens;
+  p.table = (const int32_t*)b_req_tokens_table; p.tab_rs = table_req_stride; p.tab_cs = table_seq_stride; p.requests = table_requests;
+  p.start_w = start_width; p.fresh_w = new_width; p.req_w = req_width; p.len_w = len_width;
+  p.Hkv = num_kv_heads; p.G = G;
+  p.total = total_tokens; p.max_new = max_new_len < total_tokens ? max_new_len : total_tokens;
+  p.most = max_seq_len < table_width ? max_seq_len : table_width;
+  if (p.most < 0) p.most = 0;
+  p.scale_log2 = qk_scale * 1.4426950408889634f;
+  p.ws_o = (float*)workspace;
+  p.ws_ml = (float2*)(p.ws_o + pl.rows * head_dim);
+  p.ws_info = (int2*)(p.ws_ml + pl.rows);
+  p.ws_item = (int*)(p.ws_info + pl.items);
+  cudaStream_t st = (cudaStream_t)stream;
+  for (int64_t b0 = 0; b0 < batch; b0 += kMaxBatch) {
+    p.batch = (int)(batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch);
+    p.start = (const char*)b_start_loc + b0 * start_width;
+    p.fresh = (const char*)b_new_len + b0 * new_width;
+    p.req = (const char*)b_req_idx + b0 * req_width;
+    p.len = (const char*)b_seq_len + b0 * len_width;
+    int rc;
+    if (dtype == B2L_F16) { KV4_DISPATCH_SHAPE(head_dim, group, { rc = launch<__half, D, GS>(p, pl, st); }); }
+    else { KV4_DISPATCH_SHAPE(head_dim, group, { rc = launch<__nv_bfloat16, D, GS>(p, pl, st); }); }
+    if (rc != B2L_OK) return rc;
+  }
+  return B2L_OK;
+}

@@ -10,8 +10,8 @@ from .flashdecoding import flash_decoding
 from .fused_moe import fused_moe, grouped_experts, moe_align_block_size, route_sigmoid_groups, route_topk
 from .gated_linear import gated_linear_scan, head_mix, head_norm_gate, mlstm, mlstm_head_floats, swiglu_scaled
 from .hyper_stream import stream_embed, stream_mix
-from .kv_int4 import (flash_decoding_int4, kv_int4_row_bytes, read_kv_buffer_int4, rope_kv_write_int4,
-                      update_kv_buffer_int4)
+from .kv_int4 import (flash_attention_int4, flash_decoding_int4, kv_int4_row_bytes, read_kv_buffer_int4,
+                      rope_kv_write_int4, update_kv_buffer_int4)
 from .latent import head_linear, latent_prepare, rope_heads, rope_table
 from .linear import linear, linear_simt
 from .parallel_stream import branch_sum_residual, depth_mix_norms, embed_rmsnorm, gelu_mul_gather
@@ -87,6 +87,7 @@ __all__ = [
     "read_kv_buffer_int4",
     "kv_int4_row_bytes",
     "flash_decoding_int4",
+    "flash_attention_int4",
     "build_slot_maps",
     "skip_rmsnorm",
     "skip_rmsnorm_quant_int8",

@@ -1,4 +1,4 @@
-"""K and V cached in 4 bits: the writer, the reader and decode attention over it.
+"""K and V cached in 4 bits: the writer, the reader, decode and prompt attention over it.
 
 The counterparts of ``rope_kv_write``, ``update_kv_buffer_split`` and ``flash_decoding`` for a pool ``[max_tokens, row_bytes]`` of
 bytes.  A row holds one token: for every kv head the codes of K, the codes of V (4 bits each, element ``2i`` in the low half of byte
@@ -179,4 +179,49 @@ def flash_decoding_int4(q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b
         b_req_idx.data_ptr(), index_width(b_req_idx, "b_req_idx"), b_seq_len.data_ptr(), index_width(b_seq_len, "b_seq_len"),
         batch, hq, num_kv_heads, d, group_size, max_len, float(qk_scale), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
         ws.data_ptr(), nbytes, code, stream_handle()))
+    return out
+
+
+@no_grad
+def flash_attention_int4(q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_tokens_table, b_req_idx, b_seq_len, max_new_len,
+                         max_actual_seq_len, num_kv_heads: int, group_size: int = 64, out=None) -> torch.Tensor:
+    """Portions of prompts over a 4-bit cache that already holds them: sequence ``b`` brings the ``b_new_len[b]`` rows of ``q [T, Hq, D]``
+    from ``b_start_loc[b]`` on, its last tokens of ``b_seq_len[b]`` cached ones; each sees the cached tokens up to itself.
+
+    The products are of 16-bit operands: cached elements are rounded to halves (for bf16 models too, whose elements beyond 65504 count as
+    65504), and so are the probabilities; sums and the softmax are held in 32 bits.  ``max_new_len`` and ``max_actual_seq_len`` are
+    bounds that the host knows: new tokens and keys past them do not count.  A row that sees nothing is zero; rows of ``q`` that belong to no
+    sequence are not written (``out``, by default a new tensor, keeps what it held there); a table entry outside the cache reads row 0.
+
+    The same arguments give the same bits; where a row's keys are parted for the sum follows from all lengths of the step."""
+    what = "flash_attention_int4"
+    code = dtype_code(q, "q")
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q must be [tokens, heads, head_dim]")
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    tokens, hq, d = q.shape
+    if num_kv_heads < 1 or hq % num_kv_heads:
+        raise ValueError(f"{what}: {hq} query heads are no multiple of {num_kv_heads} kv heads")
+    batch = b_req_idx.shape[0]
+    for t, name in ((b_start_loc, "b_start_loc"), (b_new_len, "b_new_len"), (b_req_idx, "b_req_idx"), (b_seq_len, "b_seq_len")):
+        _vector(t, batch, name, what)
+    address, stride, rows = _cache_rows(kv_buffer, num_kv_heads, d, group_size, what)
+    table = _table(b_req_tokens_table, what)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
+        raise ValueError(f"{what}: out has the shape and type of q and a contiguous head_dim")
+    _same_device(what, q, kv_buffer, b_start_loc, b_new_len, b_req_tokens_table, b_req_idx, b_seq_len, out)
+    if out is None:
+        out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
+    if batch == 0 or tokens == 0:
+        return out
+    max_len = int(max_actual_seq_len)
+    nbytes = lib().b2l_flash_attention_int4_workspace_bytes(batch, tokens, hq, num_kv_heads, d, group_size, max_len)
+    ws = workspace(max(nbytes, 16), q.device)
+    check(lib().b2l_flash_attention_int4(
+        out.data_ptr(), q.data_ptr(), address, stride, rows, b_start_loc.data_ptr(), index_width(b_start_loc, "b_start_loc"),
+        b_new_len.data_ptr(), index_width(b_new_len, "b_new_len"), b_req_tokens_table.data_ptr(), *table,
+        b_req_idx.data_ptr(), index_width(b_req_idx, "b_req_idx"), b_seq_len.data_ptr(), index_width(b_seq_len, "b_seq_len"),
+        batch, tokens, int(max_new_len), hq, num_kv_heads, d, group_size, max_len, float(qk_scale),
+        q.stride(0), q.stride(1), out.stride(0), out.stride(1), ws.data_ptr(), nbytes, code, stream_handle()))
     return out

@@ -75,6 +75,26 @@ def attention(q, rows, heads: int, group: int, scale: float):
     return out, weight * ((64 * 2.0**-23 * big + 2.0**-20).T[..., None])
 
 
+def prompt_attention(q, rows, heads: int, group: int, scale: float):
+    """``(out, error)`` as ``attention``, for operands and weights of 16 bits: keys, values, weights (and bf16 queries not at all) are rounded to
+    halves, off by 2^-11 of themselves, so a score is off by 2^-11 of A' (its products in absolute value, base 2) and every weight by
+    2 ln 2 times that and 2^-11, each value by 2^-11; what lies below the halves' range is off by 2^-25 a weight and a value, where weights
+    are scaled up to 2^8."""
+    out, error = attention(q, rows, heads, group, scale)
+    m, hq, d = q.shape
+    n = rows.shape[0]
+    if n == 0:
+        return out, error
+    k, v, _, _ = (t.repeat_interleave(hq // heads, 1) for t in values(rows, heads, d, group, q.dtype))
+    x = q.double()
+    seen = torch.arange(n, device=q.device) <= torch.arange(n - m, n, device=q.device)[:, None]
+    p = torch.nan_to_num(torch.softmax((torch.einsum("mhd,nhd->hmn", x, k) * scale).masked_fill(~seen, -math.inf), -1))
+    big = (torch.einsum("mhd,nhd->hmn", x.abs(), k.abs()) * scale * math.log2(math.e)).masked_fill(~seen, 0).amax(-1).T[..., None]
+    weight = torch.einsum("hmn,nhd->mhd", p, v.abs())
+    tiny = n * 2.0**-25 * (v.abs().amax(0) + 1)
+    return out, error + weight * 2.0**-11 * (2 + 2 * math.log(2) * big) * 1.01 + tiny
+
+
 def within(got: torch.Tensor, want: torch.Tensor, error: torch.Tensor) -> torch.Tensor:
     """Where ``got`` is a rounding of something within ``error`` of ``want`` (64 bits)."""
     fi = torch.finfo(got.dtype)

@@ -49,6 +49,7 @@ def test_shims_refuse_cpu_tensors():
     for call in (lambda: K.update_kv_buffer_int4(k, v, idx, cache), lambda: K.rope_kv_write_int4(q, k, v, cos, cos, idx, cache, 1, 3),
                  lambda: K.read_kv_buffer_int4(cache, idx, 2, 64, torch.float16),
                  lambda: K.flash_decoding_int4(q, cache, 0.1, table, idx, idx, 8, 2),
+                 lambda: K.flash_attention_int4(q, cache, 0.1, idx, idx, table, idx, idx, 2, 8, 2),
                  lambda: K.build_slot_maps(idx, idx, idx, table, 5)):
         with pytest.raises(ValueError, match="no CPU fallback"):
             call()
@@ -91,6 +92,11 @@ def test_attention_and_maps_refuse_what_does_not_fit():
         (lambda: K.flash_decoding_int4(q, cache, 0.1, table.long(), idx, idx, 8, 2), "int32 matrix"),
         (lambda: K.flash_decoding_int4(q, cache, 0.1, table, idx[:2], idx, 8, 2), "one entry per sequence"),
         (lambda: K.flash_decoding_int4(q, cache, 0.1, table, idx, idx, 8, 4), "takes 288 bytes"),
+        (lambda: K.flash_attention_int4(q, cache, 0.1, idx, idx, table, idx, idx, 2, 8, 3), "no multiple"),
+        (lambda: K.flash_attention_int4(q, cache, 0.1, idx[:2], idx, table, idx, idx, 2, 8, 2), "one entry per sequence"),
+        (lambda: K.flash_attention_int4(q, cache, 0.1, idx, idx, table, idx, idx, 2, 8, 2, out=q[:2]), "shape and type of q"),
+        (lambda: K.flash_attention_int4(q, cache, 0.1, idx, idx, table, idx, idx, 2, 8, 2, 128), "groups of 128"),
+        (lambda: K.flash_attention_int4(q, cache.view(-1), 0.1, idx, idx, table, idx, idx, 2, 8, 2), "uint8 matrix"),
         (lambda: K.build_slot_maps(idx, idx[:2], idx, table, 5), "one entry per sequence"),
         (lambda: K.build_slot_maps(idx, idx, idx, table.long(), 5), "int32 matrix"),
         (lambda: K.build_slot_maps(idx, idx, idx, table, -1), "total_tokens"),
