@@ -13,6 +13,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -36,6 +37,18 @@ struct {
   int (*norm)(void*, const void*, void*, const void*, i64, i64, i64, i64, i64, float, int, void*);
   int (*norm_quant)(void*, void*, const void*, void*, const void*, i64, i64, i64, i64, i64, float, int, void*);
   int (*swiglu)(void*, const void*, const void*, i64, i64, i64, i64, i64, int, void*);
+  int64_t (*kv4_row_bytes)(int, int, int);
+  int (*kv4_write)(void*, void*, const void*, const void*, const void*, const void*, const void*, const void*, int, void*, i64, i64, i64, i64,
+                   int, int, int, int, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, int, void*);
+  int (*kv4_read)(void*, const void*, i64, i64, const void*, int, i64, int, int, int, int, void*);
+  int64_t (*kv4_decode_workspace)(i64, int, int, int, int, i64);
+  int (*kv4_decode)(void*, const void*, const void*, i64, i64, const void*, i64, i64, i64, i64, const void*, int, const void*, int, i64, int,
+                    int, int, int, i64, float, i64, i64, i64, i64, void*, i64, int, void*);
+  int64_t (*kv4_prompt_workspace)(i64, i64, int, int, int, int, i64);
+  int (*kv4_prompt)(void*, const void*, const void*, i64, i64, const void*, int, const void*, int, const void*, i64, i64, i64, i64, const void*,
+                    int, const void*, int, i64, i64, i64, int, int, int, int, i64, float, i64, i64, i64, i64, void*, i64, int, void*);
+  int (*slot_maps)(void*, void*, void*, void*, const void*, int, const void*, int, const void*, int, const void*, int, void*, i64, i64, i64,
+                   i64, i64, i64, void*);
   const char* (*last_error)();
 } abi;
 PyObject* py_zeroed = nullptr;      // kernels._common.zeroed_workspace(bytes, device)
@@ -373,6 +386,195 @@ PyObject* swiglu(PyObject*, PyObject* const* a, Py_ssize_t count) {
   FAST_END
 }
 
+// ---- the cache in 4 bits and slot maps (kernels/kv_int4.py, kernels/slot_maps.py) ----
+// heads inside token rows, unit stride in a head; at least one element
+bool heads3(const at::Tensor& t) { return t.dim() == 3 && t.stride(2) == 1 && t.numel() > 0; }
+// bytes of an index vector's elements: 4 or 8; 0 for anything but a contiguous vector of n
+int indices(const at::Tensor& t, i64 n) {
+  if (t.dim() != 1 || t.size(0) != n || !t.is_contiguous()) return 0;
+  return t.scalar_type() == at::kInt ? 4 : t.scalar_type() == at::kLong ? 8 : 0;
+}
+bool table2(const at::Tensor& t) { return t.dim() == 2 && t.scalar_type() == at::kInt; }
+// rows of a 4-bit cache that hold such heads
+bool cache4(const at::Tensor& t, i64 heads, i64 d, i64 group) {
+  if (t.scalar_type() != at::kByte || t.dim() != 2 || t.stride(1) != 1 || t.size(0) < 2 || t.stride(0) < t.size(1)) return false;
+  if (heads < 1 || heads > 65535 || d > 65535 || group < 1 || group > 65535) return false;
+  const i64 need = abi.kv4_row_bytes((int)heads, (int)d, (int)group);
+  return need > 0 && t.size(1) >= need;
+}
+// whole numbers from Python; false: one of them is something else
+bool numbers(PyObject* const* a, std::initializer_list<int> at, i64* to) {
+  for (int i : at) {
+    if (!PyLong_CheckExact(a[i])) return false;
+    *to = PyLong_AsLongLong(a[i]);
+    if (*to == -1 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    ++to;
+  }
+  return true;
+}
+
+// (q, k, v, cos, sin, select_index, kv_buffer, batch, seq, group, out_q or None, out_k or None) -> (out_q or q, out_k or k)
+PyObject* kv4_rope_write(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(12)
+  FAST_BEGIN
+  const at::Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *c = plain(a[3]), *s = plain(a[4]), *idx = plain(a[5]), *kv = plain(a[6]);
+  const at::Tensor *oq = a[10] == Py_None ? q : plain(a[10]), *ok = a[11] == Py_None ? k : plain(a[11]);
+  const int device = device_for(abi.kv4_write, {q, k, v, c, s, idx, kv, oq, ok});
+  i64 n[3];
+  if (device < 0 || !numbers(a, {7, 8, 9}, n)) return none();
+  const int code = half_code(*q);
+  if (code < 0 || !heads3(*q) || !heads3(*k) || !heads3(*v) || !heads3(*oq) || !heads3(*ok)) return none();
+  for (const at::Tensor* t : {k, v, c, s, oq, ok})
+    if (t->scalar_type() != q->scalar_type()) return none();
+  const i64 tokens = q->size(0), hq = q->size(1), d = q->size(2), hkv = k->size(1);
+  if (n[0] < 1 || n[1] < 1 || n[0] > tokens || n[1] > tokens || n[0] * n[1] != tokens || k->size(0) != tokens || k->size(2) != d || v->sizes() != k->sizes() ||
+      oq->sizes() != q->sizes() || ok->sizes() != k->sizes())
+    return none();
+  if (c->dim() != 3 || c->sizes() != s->sizes() || c->strides() != s->strides() || c->stride(2) != 1 || c->size(0) != n[0] || c->size(1) != n[1] ||
+      c->size(2) < d / 2)
+    return none();
+  const int width = indices(*idx, tokens);
+  if (!width || !cache4(*kv, hkv, d, n[2])) return none();
+  int rc;
+  {
+    const Unlocked unlocked;
+    rc = abi.kv4_write(oq->data_ptr(), ok->data_ptr(), q->data_ptr(), k->data_ptr(), v->data_ptr(), c->data_ptr(), s->data_ptr(), idx->data_ptr(),
+                       width, kv->data_ptr(), kv->stride(0), kv->size(0), tokens, n[1], (int)hq, (int)hkv, (int)d, (int)n[2], q->stride(0),
+                       q->stride(1), k->stride(0), k->stride(1), v->stride(0), v->stride(1), c->stride(0), c->stride(1), oq->stride(0),
+                       oq->stride(1), ok->stride(0), ok->stride(1), code, stream(device));
+  }
+  if (rc) return failed(rc);
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, Py_NewRef(a[10] == Py_None ? a[0] : a[10]));
+  PyTuple_SET_ITEM(out, 1, Py_NewRef(a[11] == Py_None ? a[1] : a[11]));
+  return out;
+  FAST_END
+}
+
+// (kv_buffer, select_index, kv heads, head_dim, dtype, group) -> values
+PyObject* kv4_read(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(6)
+  FAST_BEGIN
+  const at::Tensor *kv = plain(a[0]), *idx = plain(a[1]);
+  const int device = device_for(abi.kv4_read, {kv, idx});
+  i64 n[3];
+  if (device < 0 || !numbers(a, {2, 3, 5}, n) || !THPDtype_Check(a[4])) return none();
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+  if ((type != at::kHalf && type != at::kBFloat16) || idx->dim() != 1 || idx->size(0) < 1 || !cache4(*kv, n[0], n[1], n[2])) return none();
+  const i64 tokens = idx->size(0);
+  const int width = indices(*idx, tokens);
+  if (!width) return none();
+  at::Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = at::empty({tokens, 2 * n[0], n[1]}, kv->options().dtype(type));
+    rc = abi.kv4_read(out.data_ptr(), kv->data_ptr(), kv->stride(0), kv->size(0), idx->data_ptr(), width, tokens, (int)n[0], (int)n[1], (int)n[2],
+                      half_code(out), stream(device));
+  }
+  return rc ? failed(rc) : THPVariable_Wrap(std::move(out));
+  FAST_END
+}
+
+// (q, kv_buffer, scale, table, req_idx, seq_len, max_len, kv heads, group) -> out
+PyObject* kv4_decode(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(9)
+  FAST_BEGIN
+  const at::Tensor *q = plain(a[0]), *kv = plain(a[1]), *table = plain(a[3]), *req = plain(a[4]), *len = plain(a[5]);
+  const int device = device_for(abi.kv4_decode, {q, kv, table, req, len});
+  i64 n[3];
+  if (device < 0 || !PyFloat_CheckExact(a[2]) || !numbers(a, {6, 7, 8}, n)) return none();
+  const int code = half_code(*q);
+  if (code < 0 || !heads3(*q) || !table2(*table)) return none();
+  const i64 batch = q->size(0), hq = q->size(1), d = q->size(2);
+  const int rw = indices(*req, batch), lw = indices(*len, batch);
+  if (!rw || !lw || !cache4(*kv, n[1], d, n[2]) || hq % n[1] != 0) return none();
+  const i64 bytes = abi.kv4_decode_workspace(batch, (int)hq, (int)n[1], (int)d, (int)n[2], n[0]);
+  at::Tensor out, ws;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = at::empty({batch, hq, d}, q->options());
+    ws = at::empty({bytes > 16 ? bytes : 16}, q->options().dtype(at::kByte));
+    rc = abi.kv4_decode(out.data_ptr(), q->data_ptr(), kv->data_ptr(), kv->stride(0), kv->size(0), table->data_ptr(), table->stride(0),
+                        table->stride(1), table->size(0), table->size(1), req->data_ptr(), rw, len->data_ptr(), lw, batch, (int)hq, (int)n[1],
+                        (int)d, (int)n[2], n[0], (float)PyFloat_AS_DOUBLE(a[2]), q->stride(0), q->stride(1), hq * d, d, ws.data_ptr(), bytes,
+                        code, stream(device));
+  }
+  return rc ? failed(rc) : THPVariable_Wrap(std::move(out));
+  FAST_END
+}
+
+// (q, kv_buffer, scale, start, new_len, table, req_idx, seq_len, max_new, max_len, kv heads, group, out or None) -> out
+PyObject* kv4_prompt(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(13)
+  FAST_BEGIN
+  const at::Tensor *q = plain(a[0]), *kv = plain(a[1]), *start = plain(a[3]), *fresh = plain(a[4]), *table = plain(a[5]), *req = plain(a[6]),
+                   *len = plain(a[7]);
+  const at::Tensor* given = a[12] == Py_None ? q : plain(a[12]);
+  const int device = device_for(abi.kv4_prompt, {q, kv, start, fresh, table, req, len, given});
+  i64 n[4];
+  if (device < 0 || !PyFloat_CheckExact(a[2]) || !numbers(a, {8, 9, 10, 11}, n)) return none();
+  const int code = half_code(*q);
+  if (code < 0 || !heads3(*q) || !table2(*table) || req->dim() != 1 || req->size(0) < 1) return none();
+  const i64 tokens = q->size(0), hq = q->size(1), d = q->size(2), batch = req->size(0);
+  const int sw = indices(*start, batch), fw = indices(*fresh, batch), rw = indices(*req, batch), lw = indices(*len, batch);
+  if (!sw || !fw || !rw || !lw || !cache4(*kv, n[2], d, n[3]) || hq % n[2] != 0) return none();
+  if (given != q && (given->scalar_type() != q->scalar_type() || given->sizes() != q->sizes() || given->stride(2) != 1)) return none();
+  const i64 bytes = abi.kv4_prompt_workspace(batch, tokens, (int)hq, (int)n[2], (int)d, (int)n[3], n[1]);
+  at::Tensor out, ws;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = a[12] == Py_None ? at::empty({tokens, hq, d}, q->options()) : *given;
+    ws = at::empty({bytes > 16 ? bytes : 16}, q->options().dtype(at::kByte));
+    rc = abi.kv4_prompt(out.data_ptr(), q->data_ptr(), kv->data_ptr(), kv->stride(0), kv->size(0), start->data_ptr(), sw, fresh->data_ptr(), fw,
+                        table->data_ptr(), table->stride(0), table->stride(1), table->size(0), table->size(1), req->data_ptr(), rw,
+                        len->data_ptr(), lw, batch, tokens, n[0], (int)hq, (int)n[2], (int)d, (int)n[3], n[1], (float)PyFloat_AS_DOUBLE(a[2]),
+                        q->stride(0), q->stride(1), out.stride(0), out.stride(1), ws.data_ptr(), bytes, code, stream(device));
+  }
+  if (rc) return failed(rc);
+  return a[12] == Py_None ? THPVariable_Wrap(std::move(out)) : Py_NewRef(a[12]);
+  FAST_END
+}
+
+// (req_idx, ctx_len, new_len, table, total, rows or None) -> (select_index, position_ids, start, length)
+PyObject* slot_maps(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(6)
+  FAST_BEGIN
+  const at::Tensor *req = plain(a[0]), *ctx = plain(a[1]), *fresh = plain(a[2]), *table = plain(a[3]);
+  const at::Tensor* pool = a[5] == Py_None ? table : plain(a[5]);
+  const int device = device_for(abi.slot_maps, {req, ctx, fresh, table, pool});
+  i64 total;
+  if (device < 0 || !numbers(a, {4}, &total) || total < 1 || req->dim() != 1 || req->size(0) < 1 || !table2(*table)) return none();
+  const i64 batch = req->size(0);
+  const int rw = indices(*req, batch), cw = indices(*ctx, batch), fw = indices(*fresh, batch);
+  if (!rw || !cw || !fw) return none();
+  int pw = 4;
+  if (pool != table && (pool->dim() != 1 || pool->size(0) < total || !(pw = indices(*pool, pool->size(0))))) return none();
+  at::Tensor rows, position, start, length;
+  int rc;
+  {
+    const Unlocked unlocked;
+    const auto i32 = table->options();
+    rows = at::empty({total}, i32);
+    position = at::empty({total}, i32.dtype(at::kLong));
+    start = at::empty({batch}, i32);
+    length = at::empty({batch}, i32);
+    rc = abi.slot_maps(rows.data_ptr(), position.data_ptr(), start.data_ptr(), length.data_ptr(), req->data_ptr(), rw, ctx->data_ptr(), cw,
+                       fresh->data_ptr(), fw, pool == table ? nullptr : pool->data_ptr(), pw, table->data_ptr(), table->stride(0),
+                       table->stride(1), table->size(0), table->size(1), batch, total, stream(device));
+  }
+  if (rc) return failed(rc);
+  PyObject* out = PyTuple_New(4);
+  if (!out) return nullptr;
+  int i = 0;
+  for (at::Tensor* t : {&rows, &position, &start, &length}) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(std::move(*t)));
+  return out;
+  FAST_END
+}
+
 // (addresses of the C functions in the order of `abi`, zeroed_workspace, counters)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t count) {
   constexpr Py_ssize_t n = sizeof(abi) / sizeof(void*);
@@ -389,7 +591,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t count) {
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(init), FAST(w8a16), FAST(w4a16_packed), FAST(linear), FAST(w8a8), FAST(quantize), FAST(norm),
-                         FAST(norm_quant), FAST(swiglu), {nullptr, nullptr, 0, nullptr}};
+                         FAST(norm_quant), FAST(swiglu), FAST(kv4_rope_write), FAST(kv4_read), FAST(kv4_decode), FAST(kv4_prompt),
+                         FAST(slot_maps), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods};
 
 }  // namespace

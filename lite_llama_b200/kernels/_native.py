@@ -16,8 +16,11 @@ from . import _common
 # the order of the function table in fast_calls.cpp
 _ABI = ("b2l_quant_gemm_workspace_bytes", "b2l_linear_workspace_bytes", "b2l_w8a16_matmul", "b2l_w4a16_matmul_packed",
         "b2l_linear", "b2l_w8a8_gemm", "b2l_quantize_activations_int8", "b2l_skip_rmsnorm", "b2l_skip_rmsnorm_quant_int8",
-        "b2l_swiglu", "b2l_last_error")
-NAMES = ("w8a16", "w4a16_packed", "linear", "w8a8", "quantize", "norm", "norm_quant", "swiglu")
+        "b2l_swiglu", "b2l_kv_int4_row_bytes", "b2l_kv_int4_write", "b2l_kv_int4_read", "b2l_flash_decoding_int4_workspace_bytes",
+        "b2l_flash_decoding_int4", "b2l_flash_attention_int4_workspace_bytes", "b2l_flash_attention_int4", "b2l_slot_maps",
+        "b2l_last_error")
+NAMES = ("w8a16", "w4a16_packed", "linear", "w8a8", "quantize", "norm", "norm_quant", "swiglu", "kv4_rope_write", "kv4_read",
+         "kv4_decode", "kv4_prompt", "slot_maps")
 
 
 def _address(name: str) -> int:
@@ -52,4 +55,5 @@ def _first(name: str):
     return call
 
 
-w8a16, w4a16_packed, linear, w8a8, quantize, norm, norm_quant, swiglu = map(_first, NAMES)
+(w8a16, w4a16_packed, linear, w8a8, quantize, norm, norm_quant, swiglu, kv4_rope_write, kv4_read, kv4_decode, kv4_prompt,
+ slot_maps) = map(_first, NAMES)

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _native
 from ._common import check, dtype_code, index_width, lib, no_grad, require_cuda, stream_handle, workspace
 
 
@@ -77,13 +78,18 @@ def update_kv_buffer_int4(K_Values, V_Values, Select_Index, KV_Buffer, group_siz
             0, 0, code, stream_handle()))
 
 
-@no_grad
 def rope_kv_write_int4(q, k, v, cos, sin, select_index, kv_buffer, batch_size, seq_len, group_size: int = 64, out_q=None, out_k=None):
     """``rope_kv_write`` into a 4-bit cache: rotate ``q [T, Hq, D]`` and ``k [T, Hkv, D]`` by ``cos/sin [batch, seq, D]`` (the first half
     of a row is read) and store the rotated, rounded keys and ``v`` at ``select_index``, in one launch.
 
     The rotated tensors go to ``out_q`` and ``out_k``, by default to ``q`` and ``k`` themselves; both are returned.  The rotation is done in
     32 bits and rounded once.  Rows as in ``update_kv_buffer_int4``."""
+    out = _native.kv4_rope_write(q, k, v, cos, sin, select_index, kv_buffer, batch_size, seq_len, group_size, out_q, out_k)
+    return _rope_kv_write_int4(q, k, v, cos, sin, select_index, kv_buffer, batch_size, seq_len, group_size, out_q, out_k) if out is None else out
+
+
+@no_grad
+def _rope_kv_write_int4(q, k, v, cos, sin, select_index, kv_buffer, batch_size, seq_len, group_size: int = 64, out_q=None, out_k=None):
     out_q, out_k = q if out_q is None else out_q, k if out_k is None else out_k
     code = dtype_code(q, "q")
     qs, ks, vs = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
@@ -114,10 +120,15 @@ def rope_kv_write_int4(q, k, v, cos, sin, select_index, kv_buffer, batch_size, s
     return out_q, out_k
 
 
-@no_grad
 def read_kv_buffer_int4(KV_Buffer, Select_Index, num_kv_heads: int, head_dim: int, dtype: torch.dtype, group_size: int = 64) -> torch.Tensor:
     """The values of the rows ``Select_Index`` as ``[tokens, 2 * Hkv, D]`` (K heads, then V heads) in ``dtype``, the type the cache was
     written in, at most its largest finite number.  An index outside the cache reads as zeros."""
+    out = _native.kv4_read(KV_Buffer, Select_Index, num_kv_heads, head_dim, dtype, group_size)
+    return _read_kv_buffer_int4(KV_Buffer, Select_Index, num_kv_heads, head_dim, dtype, group_size) if out is None else out
+
+
+@no_grad
+def _read_kv_buffer_int4(KV_Buffer, Select_Index, num_kv_heads: int, head_dim: int, dtype: torch.dtype, group_size: int = 64) -> torch.Tensor:
     if Select_Index.dim() != 1 or not Select_Index.is_contiguous():
         raise ValueError("read_kv_buffer_int4: Select_Index is a contiguous vector")
     address, stride, rows = _cache_rows(KV_Buffer, num_kv_heads, head_dim, group_size, "read_kv_buffer_int4")
@@ -142,7 +153,6 @@ def _vector(t: torch.Tensor, n: int, name: str, what: str) -> None:
         raise ValueError(f"{what}: {name} is a contiguous vector with one entry per sequence")
 
 
-@no_grad
 def flash_decoding_int4(q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b_seq_len, max_actual_seq_len, num_kv_heads: int,
                         group_size: int = 64) -> torch.Tensor:
     """``flash_decoding`` over a 4-bit cache: one query ``q [B, Hq, D]`` per sequence against its cached tokens, ``qk_scale = 1/sqrt(D)``.
@@ -154,6 +164,14 @@ def flash_decoding_int4(q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b
 
     The same arguments give the same bits.  Where a row's tokens are parted for the sum follows from the lengths of all rows, so a
     sequence's last bits may change with what stands beside it."""
+    args = (q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b_seq_len, max_actual_seq_len, num_kv_heads, group_size)
+    out = _native.kv4_decode(*args)
+    return _flash_decoding_int4(*args) if out is None else out
+
+
+@no_grad
+def _flash_decoding_int4(q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b_seq_len, max_actual_seq_len, num_kv_heads: int,
+                        group_size: int = 64) -> torch.Tensor:
     what = "flash_decoding_int4"
     code = dtype_code(q, "q")
     if q.dim() != 3:
@@ -182,7 +200,6 @@ def flash_decoding_int4(q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b
     return out
 
 
-@no_grad
 def flash_attention_int4(q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_tokens_table, b_req_idx, b_seq_len, max_new_len,
                          max_actual_seq_len, num_kv_heads: int, group_size: int = 64, out=None) -> torch.Tensor:
     """Portions of prompts over a 4-bit cache that already holds them: sequence ``b`` brings the ``b_new_len[b]`` rows of ``q [T, Hq, D]``
@@ -194,6 +211,15 @@ def flash_attention_int4(q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_t
     sequence are not written (``out``, by default a new tensor, keeps what it held there); a table entry outside the cache reads row 0.
 
     The same arguments give the same bits; where a row's keys are parted for the sum follows from all lengths of the step."""
+    args = (q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_tokens_table, b_req_idx, b_seq_len, max_new_len, max_actual_seq_len,
+            num_kv_heads, group_size, out)
+    got = _native.kv4_prompt(*args)
+    return _flash_attention_int4(*args) if got is None else got
+
+
+@no_grad
+def _flash_attention_int4(q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_tokens_table, b_req_idx, b_seq_len, max_new_len,
+                         max_actual_seq_len, num_kv_heads: int, group_size: int = 64, out=None) -> torch.Tensor:
     what = "flash_attention_int4"
     code = dtype_code(q, "q")
     if q.dim() != 3:

@@ -4,11 +4,11 @@ from __future__ import annotations
 
 import torch
 
+from . import _native
 from ._common import check, index_width, lib, no_grad, stream_handle
 from .kv_int4 import _same_device, _table, _vector
 
 
-@no_grad
 def build_slot_maps(b_req_idx, b_ctx_len, b_new_len, b_req_tokens_table, total_tokens: int, rows=None):
     """Where the new tokens of a flat batch lie: request ``b`` (row ``b_req_idx[b]`` of ``b_req_tokens_table [requests, width]`` int32)
     has ``b_ctx_len[b]`` tokens cached and brings ``b_new_len[b]``, behind those of the requests before it.
@@ -18,6 +18,12 @@ def build_slot_maps(b_req_idx, b_ctx_len, b_new_len, b_req_tokens_table, total_t
     or from ``rows`` (at least ``total`` entries, int32 or int64), which are then entered into the table.  ``total_tokens`` may exceed the sum of the
     lengths (a captured size): the tokens behind it get row -1, which ``update_kv_buffer_int4`` skips, and position 0, and take nothing from
     ``rows``.  A position or request outside the table gets row -1.  Nothing is read by the host, so the call can be captured."""
+    maps = _native.slot_maps(b_req_idx, b_ctx_len, b_new_len, b_req_tokens_table, total_tokens, rows)
+    return _build_slot_maps(b_req_idx, b_ctx_len, b_new_len, b_req_tokens_table, total_tokens, rows) if maps is None else maps
+
+
+@no_grad
+def _build_slot_maps(b_req_idx, b_ctx_len, b_new_len, b_req_tokens_table, total_tokens: int, rows=None):
     what = "build_slot_maps"
     batch, total = b_req_idx.shape[0], int(total_tokens)
     for t, name in ((b_req_idx, "b_req_idx"), (b_ctx_len, "b_ctx_len"), (b_new_len, "b_new_len")):
