@@ -162,8 +162,8 @@ struct Int4Consumer {
     }
   }
 
-  // 16 tokens at `at` (the head's bytes of the first), of which `valid` count
-  template <bool MASKED>
+  // 16 tokens at `at` (the head's bytes of the first), of which `valid` count (one form for all: a copy without the mask costs more in
+  // the instruction cache than the mask)
   __device__ __forceinline__ void unit(const uint8_t* at, int pitch, int valid) {
     constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
     const uint8_t* row0 = at + place(r) * pitch;
@@ -207,7 +207,7 @@ struct Int4Consumer {
     float v[2][2], top = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bool in = !MASKED || place(r) + 8 * i < valid;
+      const bool in = place(r) + 8 * i < valid;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float t = ks[i][0].x * acc[0][2 * i + j], u = ks[i][0].y * sq[j][0];
@@ -220,7 +220,7 @@ struct Int4Consumer {
       }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        if (MASKED && !in) vs[i][g] = make_float2(0.f, 0.f);
+        if (!in) vs[i][g] = make_float2(0.f, 0.f);
         top = fmaxf(top, vs[i][g].x);
       }
     }
@@ -444,12 +444,12 @@ __global__ void __launch_bounds__((kMaxConsumers + 1) * 32, 2) kv4_decode_kernel
     const int len = lens[seg.b], kvh = blk * p.HB + hl;
     const int off = ((blk * p.HB * hb) & 15) + hl * hb + ts * unit_bytes;
     c.begin(p, seg.b, kvh, head0, heads);
+#pragma unroll 1
     for (int t = seg.first; t < seg.last; ++t) {
       mbar_wait(&full_bar[s], phase);
       const int valid = len - t * tile - ts * kUnit;
       const uint8_t* u = ring + s * stage_bytes + off;
-      if (valid >= kUnit) c.template unit<false>(u, p.pitch, kUnit);
-      else if (valid > 0) c.template unit<true>(u, p.pitch, valid);
+      if (valid > 0) c.unit(u, p.pitch, valid);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[s]);
       if (++s == p.stages) { s = 0; phase ^= 1; }

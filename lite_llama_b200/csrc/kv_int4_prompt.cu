@@ -5,12 +5,14 @@
 // A CTA works on 256 query rows of one kv head -- rows are (token, query head of the group), so that a key tile serves all heads of
 // the group and a portion of few tokens still fills a tile -- as two tiles of 128 rows, over tiles of 128 keys:
 //   warps 0, 1    tensor-core issuers: the scores S = Q K^T, and O += P V (A = P from tensor memory)
-//   warps 4 - 7   K and V rows from the cache through the request table, codes to halves minimum + scale * code, into the operands'
-//                 swizzled layout.  A word of eight codes turns into one 16-byte chunk in the order 0 4 1 5 2 6 3 7: with the queries stored in
-//                 the same order the scores are the same, and the outputs' order is undone at the end.
+//   warps 2, 3    the head's bytes of the cache rows, through the request table, by asynchronous copies into a ring of units (64 keys of K
+//                 or of V), a tile ahead
+//   warps 4 - 7   codes to halves minimum + scale * code in the operands' swizzled layout.  A word of eight codes turns into one 16-byte
+//                 chunk in the order 0 4 1 5 2 6 3 7: with the queries stored in the same order the scores are the same, and the
+//                 outputs' order is undone at the end.
 //   warps 8 - 15  softmax, a thread to a row of either tile: the row's scores from tensor memory once, P written back, the output rescaled
 //                 where the running maximum rises by more than 2^8 (both by one factor, hence exact)
-// Tensor memory: S | P0 P1 | O0 | O1, as in flash_attention_tc.cu.
+// Tensor memory: S0 S1 (64 keys each) | P0 P1 | O0 | O1.
 // The operands are halves for both activation types: elements are rounded to 11 bits (as the 16-bit cache of an fp16 model rounds
 // them), which for bf16 models are three bits more than reading the cache into their type would leave; elements of those beyond 65504
 // count as 65504.  Queries of bf16 models are scaled by a power of two per row.  Probabilities are rounded to 11 bits, as in
@@ -27,8 +29,9 @@
 namespace kv4p {
 
 constexpr int kBM = 128, kBN = 128, kRows = 2 * kBM;
-constexpr int kThreads = 512, kKStages = 2, kVStages = 2, kSegs = 4;
-constexpr int kMaxBatch = 1024;
+constexpr int kThreads = 640, kConvert = 256, kKStages = 2, kVStages = 2, kSegs = 4;
+constexpr int kUnits = 5, kUnitKeys = 64, kUnitPitch = 96;   // pitch: rows of four neighbours in different banks
+constexpr int kMaxBatch = 128;                    // sequences of a launch (their sizes lie in shared memory)
 constexpr int kMinSteps = 2;                      // key tiles of a share: below that the parts cost more than the tiles
 
 struct Params {
@@ -39,44 +42,50 @@ struct Params {
   const void *start, *fresh, *req, *len;
   int start_w, fresh_w, req_w, len_w;
   int batch, Hkv, G;
+  uint64_t by_G;                                  // 2^64 / G, rounded up: n / G is the high half of n * by_G for n < 2^32 (G > 1)
   int64_t total, max_new, most;
   float scale_log2;
   float* ws_o; float2* ws_ml; int2* ws_info; int* ws_item;
 };
 
-// a sequence: its new tokens begin at row `start` of q, the first stands at position ctx, keys below `keys` are cached
-struct Seq { int m, ctx, keys; };
+// a sequence: its m new tokens begin at row `start` of q, the first stands at position ctx, keys below `keys` are cached
+struct Seq { int m, ctx, keys, start, req; };
 __device__ __forceinline__ Seq sequence(const Params& p, int b) {
   const int64_t n = load_index(p.len, b, p.len_w), f = load_index(p.fresh, b, p.fresh_w), s = load_index(p.start, b, p.start_w);
   const int64_t r = load_index(p.req, b, p.req_w);
-  Seq q;
   int64_t m = f < 0 ? 0 : f, ctx = (n < 0 ? 0 : n) - m;
   if (m > p.max_new) m = p.max_new;
   if (s < 0 || s >= p.total) m = 0;
   else if (m > p.total - s) m = p.total - s;
+  Seq q;
   q.m = (int)m;
   q.ctx = (int)(ctx < -(1ll << 30) ? -(1ll << 30) : ctx > (1ll << 30) ? (1ll << 30) : ctx);
   q.keys = r < 0 || r >= p.requests || n <= 0 ? 0 : (int)(n < p.most ? n : p.most);
+  q.start = (int)s;
+  q.req = (int)r;
   return q;
 }
-__device__ __forceinline__ int row_blocks(const Seq& s, int G) { return (int)(((int64_t)s.m * G + kRows - 1) / kRows); }
+__device__ __forceinline__ int over_G(const Params& p, int n) { return p.G == 1 ? n : (int)__umul64hi((uint64_t)(uint32_t)n, p.by_G); }
+__device__ __forceinline__ int row_blocks(const Params& p, const Seq& s) { return (s.m * p.G + kRows - 1) / kRows; }
 // key tiles of tile t of row block rb: up to its last row's position (0: no rows; a tile that sees nothing takes one step for its zeros)
-__device__ __forceinline__ int key_tiles(const Seq& s, int G, int rb, int t) {
-  const int64_t first = (int64_t)rb * kRows + t * kBM, rows = (int64_t)s.m * G;
+__device__ __forceinline__ int key_tiles(const Params& p, const Seq& s, int rb, int t) {
+  const int first = rb * kRows + t * kBM, rows = s.m * p.G;
   if (first >= rows) return 0;
-  const int64_t last = (first + kBM < rows ? first + kBM : rows) - 1;
-  int64_t k = s.ctx + last / G + 1;
+  const int last = (first + kBM < rows ? first + kBM : rows) - 1;
+  int k = s.ctx + over_G(p, last) + 1;
   if (k > s.keys) k = s.keys;
-  return k > 0 ? (int)((k + kBN - 1) / kBN) : 1;
+  return k > 0 ? (k + kBN - 1) / kBN : 1;
 }
-__device__ __forceinline__ int block_steps(const Seq& s, int G, int rb) {
-  const int a = key_tiles(s, G, rb, 0), b = key_tiles(s, G, rb, 1);
-  return a > b ? a : b;
+// of both: the second sees no less, where it has rows
+__device__ __forceinline__ int block_steps(const Params& p, const Seq& s, int rb) {
+  const int b = key_tiles(p, s, rb, 1);
+  return b > 0 ? b : key_tiles(p, s, rb, 0);
 }
 
 struct __align__(16) Ctl {
   uint64_t q_full[2], k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
-  uint64_t s_full[2], s_free, p_full[2], pv_done[2], seg_done[kSegs];
+  uint64_t raw_full[kUnits], raw_empty[kUnits];
+  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], seg_done[kSegs];
   int nan_at[kSegs][4];                           // first key whose value group is NaN
   uint32_t tmem_base;
 };
@@ -86,6 +95,18 @@ static_assert(sizeof(Ctl) <= 512, "control block");
 struct Segment { int b, kvh, rb, j0, j1, steps, item; };
 
 #define kv4_wait(bar, parity) mbar_wait_short_at<true>((bar), (parity), b2l_file_hash(__FILE__), __LINE__)
+
+// an asynchronous copy of 4, 8 or 16 bytes to shared memory; zeros where `read` is false
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool read) {
+  const int n = read ? BYTES : 0;
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n), "n"(BYTES) : "memory");
+}
+// the barrier's arrival of this thread, once its copies so far are done
+__device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 // codes of a word to halves minimum + scale * code, in the order 0 4 1 5 2 6 3 7
 __device__ __forceinline__ uint4 to_halves(uint32_t w, __half2 s, __half2 m) {
@@ -101,8 +122,9 @@ __device__ __forceinline__ uint4 to_halves(uint32_t w, __half2 s, __half2 m) {
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 // the same for scales or minima that may lead past the halves' range, or NaN
-__device__ __noinline__ uint4 to_halves_wide(uint32_t w, float s, float m) {
+__device__ __forceinline__ uint4 to_halves_wide(uint32_t w, float s, float m) {
   uint32_t r[4];
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
     float x = fmaf((float)(w >> (4 * i) & 15u), s, m), y = fmaf((float)(w >> (4 * i + 16) & 15u), s, m);
     x = x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;
@@ -136,19 +158,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
   uint8_t* q_s = smem + 1024;
   uint8_t* k_ring = q_s + 2 * kTile;
   uint8_t* v_ring = k_ring + kKStages * kTile;
-  int64_t* prefix = reinterpret_cast<int64_t*>(v_ring + kVStages * kTile);   // steps of the sequences before, [batch + 1]
-  int* items = reinterpret_cast<int*>(prefix + p.batch + 1);                 // row blocks (of all kv heads) before
+  uint8_t* raw_ring = v_ring + kVStages * kTile;
+  int* prefix = reinterpret_cast<int*>(raw_ring + kUnits * kUnitKeys * kUnitPitch);   // steps of the sequences before, [batch + 1]
+  int* items = prefix + kMaxBatch + 1;            // row blocks (of all kv heads) before
+  Seq* seqs = reinterpret_cast<Seq*>(items + kMaxBatch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.G;
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&ctl->q_full[t], 4); mbar_init(&ctl->s_full[t], 1); mbar_init(&ctl->p_full[t], 4); mbar_init(&ctl->pv_done[t], 1);
+      mbar_init(&ctl->s_free[t], 4);
     }
-    for (int s = 0; s < kKStages; ++s) { mbar_init(&ctl->k_full[s], 4); mbar_init(&ctl->k_empty[s], 1); }
-    for (int s = 0; s < kVStages; ++s) { mbar_init(&ctl->v_full[s], 4); mbar_init(&ctl->v_empty[s], 1); }
+    for (int s = 0; s < kKStages; ++s) { mbar_init(&ctl->k_full[s], kConvert / 32); mbar_init(&ctl->k_empty[s], 1); }
+    for (int s = 0; s < kVStages; ++s) { mbar_init(&ctl->v_full[s], kConvert / 32); mbar_init(&ctl->v_empty[s], 1); }
+    for (int s = 0; s < kUnits; ++s) { mbar_init(&ctl->raw_full[s], 64); mbar_init(&ctl->raw_empty[s], kConvert / 32); }
     for (int s = 0; s < kSegs; ++s) mbar_init(&ctl->seg_done[s], 8);
-    mbar_init(&ctl->s_free, 4);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -161,12 +186,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
   // ---- steps and row blocks per sequence (a warp each), then their sums ----
   for (int b = warp; b < p.batch; b += kThreads / 32) {
     const Seq s = sequence(p, b);
-    const int nb = row_blocks(s, G);
+    const int nb = row_blocks(p, s);
     int n = 0;
-    for (int rb = lane; rb < nb; rb += 32) n += block_steps(s, G, rb);
+    for (int rb = lane; rb < nb; rb += 32) n += block_steps(p, s, rb);
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) {
-      prefix[b + 1] = (int64_t)n * p.Hkv;
+      seqs[b] = s;
+      prefix[b + 1] = n * p.Hkv;
       items[b] = nb * p.Hkv;
     }
   }
@@ -174,17 +200,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
   __syncthreads();
   tc_fence_after();
   if (warp == 0) {
-    int64_t steps = 0;
-    int blocks = 0;
+    int steps = 0, blocks = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       const int b = b0 + lane;
-      int64_t s = b < p.batch ? prefix[b + 1] : 0;
+      int s = b < p.batch ? prefix[b + 1] : 0;
       const int own = b < p.batch ? items[b] : 0;
       int k = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, s, o);
-        const int y = __shfl_up_sync(0xffffffffu, k, o);
+        const int x = __shfl_up_sync(0xffffffffu, s, o), y = __shfl_up_sync(0xffffffffu, k, o);
         if (lane >= o) { s += x; k += y; }
       }
       if (b < p.batch) {
@@ -200,13 +224,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
   __syncthreads();
   const uint32_t tmem_base = ctl->tmem_base;
 
-  const int64_t total = prefix[p.batch];
-  const int64_t worth = (total + kMinSteps - 1) / kMinSteps;
-  const int64_t shares = worth < gridDim.x ? worth : gridDim.x;
-  int64_t step = 0, step_end = 0;
-  if (blockIdx.x < shares) {
-    step = blockIdx.x * total / shares;
-    step_end = (blockIdx.x + 1) * total / shares;
+  const int total = prefix[p.batch], worth = (total + kMinSteps - 1) / kMinSteps;
+  const int shares = worth < (int)gridDim.x ? worth : (int)gridDim.x;
+  int step = 0, step_end = 0;
+  if ((int)blockIdx.x < shares) {
+    step = (int)((int64_t)blockIdx.x * total / shares);
+    step_end = (int)((int64_t)(blockIdx.x + 1) * total / shares);
   }
   auto next = [&](Segment& g, Seq& s) -> bool {
     if (step >= step_end) return false;
@@ -216,23 +239,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
       if (prefix[lo + half] <= step) { lo += half; n -= half; }
       else n = half;
     }
-    s = sequence(p, lo);
-    const int64_t x = step - prefix[lo];
-    const int per_head = (int)((prefix[lo + 1] - prefix[lo]) / p.Hkv);
-    const int nb = row_blocks(s, G);
+    s = seqs[lo];
+    const int per_head = (prefix[lo + 1] - prefix[lo]) / p.Hkv, nb = row_blocks(p, s);
+    int y = step - prefix[lo];
     g.b = lo;
-    g.kvh = (int)(x / per_head);
-    int y = (int)(x - (int64_t)g.kvh * per_head);
-    g.rb = 0;
-    for (; g.rb < nb - 1; ++g.rb) {
-      const int n_rb = block_steps(s, G, g.rb);
-      if (y < n_rb) break;
-      y -= n_rb;
+    g.kvh = y / per_head;
+    y -= g.kvh * per_head;
+    g.steps = block_steps(p, s, 0);
+    for (g.rb = 0; g.rb < nb - 1 && y >= g.steps;) {
+      y -= g.steps;
+      g.steps = block_steps(p, s, ++g.rb);
     }
-    g.steps = block_steps(s, G, g.rb);
     g.j0 = y;
-    const int64_t left = step_end - step;
-    g.j1 = left < g.steps - y ? y + (int)left : g.steps;
+    const int left = step_end - step;
+    g.j1 = left < g.steps - y ? y + left : g.steps;
     g.item = items[lo] + g.kvh * nb + g.rb;
     step += g.j1 - g.j0;
     return true;
@@ -240,42 +260,47 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
 
   Segment seg;
   Seq seq;
-  // registers per lane: 16 warps x 128 at launch = 4 x 32 + 4 x 96 + 8 x 192
+  // registers per lane: 20 warps x 96 at launch >= 4 x 56 + 8 x 72 + 8 x 136
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp < 2) {
       // ===================== tensor-core issuers: warp 0 the scores, warp 1 P V =====================
-      constexpr uint32_t idesc_s = umma_idesc(1u, 0u, 0u, 0u, 0u, kBM, kBN);
+      constexpr uint32_t idesc_s = umma_idesc(1u, 0u, 0u, 0u, 0u, kBM, kBN / 2);
       constexpr uint32_t idesc_o = umma_idesc(1u, 0u, 0u, 0u, 1u, kBM, DP);
       int ring = 0;
-      uint32_t phase = 0, free_phase = 1, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      uint32_t phase = 0, free_phase = 3, q_phase = 0, p_phase = 0;   // a bit to a tile
       while (next(seg, seq)) {
-        const int nt[2] = {key_tiles(seq, G, seg.rb, 0), key_tiles(seq, G, seg.rb, 1)};
+        const int nt[2] = {key_tiles(p, seq, seg.rb, 0), key_tiles(p, seq, seg.rb, 1)};
         for (int j = seg.j0; j < seg.j1; ++j) {
           kv4_wait(warp == 0 ? &ctl->k_full[ring] : &ctl->v_full[ring], phase);
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (j >= nt[t]) continue;
-            const bool last = t == 1 || j >= nt[1];              // the key tile's last reader
-            if (warp == 0) {
-              if (j == seg.j0) { kv4_wait(&ctl->q_full[t], q_phase[t]); q_phase[t] ^= 1u; }
-              kv4_wait(&ctl->s_free, free_phase);
-              free_phase ^= 1u;
+          if (warp == 0) {
+#pragma unroll 1
+            for (int x = 0; x < 4; ++x) {
+              const int t = x & 1, h = x >> 1;
+              if (j >= (t ? nt[1] : nt[0])) continue;
+              if (h == 0 && j == seg.j0) { kv4_wait(&ctl->q_full[t], q_phase >> t & 1u); q_phase ^= 1u << t; }
+              kv4_wait(&ctl->s_free[t], free_phase >> t & 1u);
+              free_phase ^= 1u << t;
               tc_fence_after();
               if (elect_one()) {
                 const uint64_t q_desc = umma_desc_sw128_kmajor(smem_u32(q_s + t * kTile));
-                const uint64_t k_desc = umma_desc_sw128_kmajor(smem_u32(k_ring + ring * kTile));
+                const uint64_t k_desc = umma_desc_sw128_kmajor(smem_u32(k_ring + ring * kTile + h * (kBN / 2) * 128));
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
                   const uint64_t off = (uint64_t)(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4);
-                  umma_f16(tmem_base, q_desc + off, k_desc + off, idesc_s, kk ? 1u : 0u);
+                  umma_f16(tmem_base + (uint32_t)t * 64u, q_desc + off, k_desc + off, idesc_s, kk ? 1u : 0u);
                 }
-                if (last) tc_commit(&ctl->k_empty[ring]);
+                if (h == 1 && (t == 1 || j >= nt[1])) tc_commit(&ctl->k_empty[ring]);   // the key tile's last reader
                 tc_commit(&ctl->s_full[t]);
               }
-            } else {
-              kv4_wait(&ctl->p_full[t], p_phase[t]);
-              p_phase[t] ^= 1u;
+              __syncwarp();
+            }
+          } else {
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+              if (j >= (t ? nt[1] : nt[0])) continue;
+              kv4_wait(&ctl->p_full[t], p_phase >> t & 1u);
+              p_phase ^= 1u << t;
               tc_fence_after();
               if (elect_one()) {
                 const uint32_t v_addr = smem_u32(v_ring + ring * kTile);
@@ -286,123 +311,124 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
                   umma_ts(tmem_base + 256u + (uint32_t)t * 128u, tmem_base + 128u + (uint32_t)t * 64u + kk * 8, v_desc, idesc_o,
                           (j > seg.j0 || kk) ? 1u : 0u);
                 }
-                if (last) tc_commit(&ctl->v_empty[ring]);
+                if (t == 1 || j >= nt[1]) tc_commit(&ctl->v_empty[ring]);
                 tc_commit(&ctl->pv_done[t]);
               }
+              __syncwarp();
             }
-            __syncwarp();
           }
           if (++ring == (warp == 0 ? kKStages : kVStages)) { ring = 0; phase ^= 1u; }
         }
       }
+    } else {
+      // ===================== cache rows: codes and groups of 64 keys of one side, a unit =====================
+      constexpr int kPiece = kv4::head_bytes(D, GS) % 16 == 0 ? 16 : 8, kLanes = D / 2 / kPiece, kGroupBytes = 4 * NG;
+      const int wk = (warp - 2) * 32;             // this warp's keys of a unit
+      int us = 0;
+      uint32_t up = 1;
+      while (next(seg, seq)) {
+        const int32_t* entry = p.table + (int64_t)seq.req * p.tab_rs;
+        const uint8_t* head = p.cache + (int64_t)seg.kvh * kv4::head_bytes(D, GS);
+        auto row_of = [&](int j, int h) -> int {  // -1: past the sequence
+          const int key = j * kBN + h * kUnitKeys + wk + lane;
+          if (key >= seq.keys) return -1;
+          const int row = ld_upstream(entry + (int64_t)key * p.tab_cs);
+          return row >= 0 && row < p.max_tokens ? row : 0;
+        };
+        int ahead[2] = {row_of(seg.j0, 0), row_of(seg.j0, 1)};
+        for (int j = seg.j0; j < seg.j1; ++j) {
+          const int rows[2] = {ahead[0], ahead[1]};
+          if (j + 1 < seg.j1) { ahead[0] = row_of(j + 1, 0); ahead[1] = row_of(j + 1, 1); }
+#pragma unroll 1
+          for (int u = 0; u < 4; ++u) {
+            const int side = u >> 1, row = (u & 1) ? rows[1] : rows[0];
+            kv4_wait(&ctl->raw_empty[us], up);
+            uint8_t* unit = raw_ring + us * kUnitKeys * kUnitPitch + wk * kUnitPitch;
+#pragma unroll
+            for (int i = 0; i < kLanes; ++i) {    // 32 / kLanes keys at a time, kLanes neighbours to a key
+              const int k = i * (32 / kLanes) + lane / kLanes, c = lane % kLanes * kPiece;
+              const int r = __shfl_sync(0xffffffffu, row, k);
+              copy_async<kPiece>(unit + k * kUnitPitch + c, head + (int64_t)(r < 0 ? 0 : r) * p.row_stride + side * (D / 2) + c, r >= 0);
+            }
+            copy_async<kGroupBytes>(unit + lane * kUnitPitch + D / 2, head + (int64_t)(row < 0 ? 0 : row) * p.row_stride + D + side * kGroupBytes,
+                                    row >= 0);
+            copy_async_arrive(&ctl->raw_full[us]);
+            if (++us == kUnits) { us = 0; up ^= 1u; }
+          }
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
-  } else if (warp < 8) {
-    // ===================== cache rows to operands =====================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+  } else if (warp < 12) {
+    // ===================== codes to operands =====================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     constexpr int NWD = D == 128 ? 2 : 1;         // words of a row and side that a thread takes (eight threads to a row)
     const int tid = threadIdx.x - 128, l = tid & 7, kq = tid >> 3;
     const bool on = l < D / 8;                    // D = 32: half of the threads store zeros
     const uint32_t spot = (uint32_t)(kq * 128 + ((l ^ (kq & 7)) << 4));
-    struct Raw { uint32_t w[4][NWD], g[4][NWD]; };
-    // 64 keys (four rows of this thread) of one side
-    auto fetch = [&](Raw& x, const int (&rows)[8], int half, int side, int kvh) {
-      const int64_t off = (int64_t)kvh * kv4::head_bytes(D, GS);
+    int ks = 0, vs = 0, us = 0, nseg = 0;
+    uint32_t kp = 1, vp = 1, up = 0;
+    for (; next(seg, seq); ++nseg) {
+      const int slot = nseg % kSegs;
+      if (nseg >= kSegs) kv4_wait(&ctl->seg_done[slot], (uint32_t)(nseg / kSegs - 1) & 1u);
+      if (tid < 4) ctl->nan_at[slot][tid] = INT_MAX;
+      asm volatile("bar.sync 2, %0;" ::"n"(kConvert) : "memory");
+#pragma unroll 1
+      for (int j = seg.j0; j < seg.j1; ++j) {
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+          const int side = u >> 1, half = u & 1;
+          if (half == 0) kv4_wait(side ? &ctl->v_empty[vs] : &ctl->k_empty[ks], side ? vp : kp);
+          uint8_t* to = (side ? v_ring + vs * kTile : k_ring + ks * kTile) + half * kUnitKeys * 128 + spot;
+          kv4_wait(&ctl->raw_full[us], up);
+          const uint8_t* unit = raw_ring + us * kUnitKeys * kUnitPitch + kq * kUnitPitch;
+          constexpr int kPass = kConvert / 8, NI = kUnitKeys / kPass;   // rows of all threads; rows of a thread and unit
+          uint32_t w[NI][NWD], g[NI][NWD], large = 0u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = rows[half * 4 + i];
+          for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int k = 0; k < NWD; ++k) {
-          x.w[i][k] = x.g[i][k] = 0u;
-          if (row >= 0 && on) {
-            const uint32_t* head = reinterpret_cast<const uint32_t*>(p.cache + (int64_t)row * p.row_stride + off);
-            x.w[i][k] = __ldcg(head + side * (D / 8) + k * 8 + l);
-            x.g[i][k] = __ldcg(head + D / 4 + side * NG + (k * 8 + l) * 8 / GS);
-          }
-        }
-      }
-    };
-    auto store = [&](const Raw& x, uint8_t* tile, int half, int side, int key0, int slot) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < NWD; ++k) {
-          const uint32_t g = x.g[i][k];
-          uint4 v;
-          if ((((g & 0x7fff7fffu) + Group<T>::kAdd) & 0x80008000u) == 0u) {
-            v = to_halves(x.w[i][k], Group<T>::both(g, 0), Group<T>::both(g, 1));
-          } else {
-            float2 f = kv4::scale_min<T>(g);
-            if (side == 1 && (f.x != f.x || f.y != f.y)) {
-              f = make_float2(0.f, 0.f);
-              atomicMin(&ctl->nan_at[slot][(k * 8 + l) * 8 / GS], key0 + half * 64 + i * 16 + kq);
+            for (int k = 0; k < NWD; ++k) {
+              const uint32_t* row = reinterpret_cast<const uint32_t*>(unit + i * kPass * kUnitPitch);
+              w[i][k] = on ? row[k * 8 + l] : 0u;
+              g[i][k] = on ? row[D / 8 + (k * 8 + l) * 8 / GS] : 0u;
+              large |= (g[i][k] & 0x7fff7fffu) + Group<T>::kAdd;
             }
-            v = to_halves_wide(x.w[i][k], f.x, f.y);
-          }
-          *reinterpret_cast<uint4*>(tile + k * kHalf + (half * 64 + i * 16) * 128 + spot) = v;
-        }
-    };
-    auto entries = [&](int (&rows)[8], const Segment& g, const Seq& s, int j) {
-      const int32_t* entry = p.table + load_index(p.req, g.b, p.req_w) * p.tab_rs;
+          if ((large & 0x80008000u) == 0u) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = j * kBN + i * 16 + kq;
-        rows[i] = -1;
-        if (key < s.keys) {
-          const int row = ld_upstream(entry + (int64_t)key * p.tab_cs);
-          rows[i] = row >= 0 && row < p.max_tokens ? row : 0;
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+              for (int k = 0; k < NWD; ++k)
+                *reinterpret_cast<uint4*>(to + k * kHalf + i * kPass * 128) = to_halves(w[i][k], Group<T>::both(g[i][k], 0), Group<T>::both(g[i][k], 1));
+          } else {                                // past the range of halves somewhere, or NaN
+#pragma unroll 1
+            for (int x = 0; x < NI * NWD; ++x) {
+              const int i = x / NWD, k = x % NWD, group = (k * 8 + l) * 8 / GS;
+              const uint32_t* row = reinterpret_cast<const uint32_t*>(unit + i * kPass * kUnitPitch);
+              float2 f = on ? kv4::scale_min<T>(row[D / 8 + group]) : make_float2(0.f, 0.f);
+              if (side == 1 && (f.x != f.x || f.y != f.y)) {
+                f = make_float2(0.f, 0.f);
+                atomicMin(&ctl->nan_at[slot][group], j * kBN + half * kUnitKeys + i * kPass + kq);
+              }
+              *reinterpret_cast<uint4*>(to + k * kHalf + i * kPass * 128) = to_halves_wide(on ? row[k * 8 + l] : 0u, f.x, f.y);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->raw_empty[us]);
+          if (++us == kUnits) { us = 0; up ^= 1u; }
+          if (half == 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(side ? &ctl->v_full[vs] : &ctl->k_full[ks]);
+            if (side) { if (++vs == kVStages) { vs = 0; vp ^= 1u; } }
+            else if (++ks == kKStages) { ks = 0; kp ^= 1u; }
+          }
         }
       }
-    };
-    int ks = 0, vs = 0, nseg = 0;
-    uint32_t kp = 1, vp = 1;
-    bool more = next(seg, seq);
-    int j = more ? seg.j0 : 0;
-    int rows[8];
-    Raw a, b;
-    if (more) {
-      entries(rows, seg, seq, j);
-      fetch(a, rows, 0, 0, seg.kvh);
-      fetch(b, rows, 1, 0, seg.kvh);
-    }
-    while (more) {
-      const int slot = nseg % kSegs, key0 = j * kBN, kvh = seg.kvh;
-      if (j == seg.j0) {
-        if (nseg >= kSegs) kv4_wait(&ctl->seg_done[slot], (uint32_t)(nseg / kSegs - 1) & 1u);
-        if (tid < 4) ctl->nan_at[slot][tid] = INT_MAX;
-        asm volatile("bar.sync 2, 128;" ::: "memory");
-      }
-      uint8_t* kt = k_ring + ks * kTile;
-      uint8_t* vt = v_ring + vs * kTile;
-      kv4_wait(&ctl->k_empty[ks], kp);
-      store(a, kt, 0, 0, key0, slot);
-      fetch(a, rows, 0, 1, kvh);
-      store(b, kt, 1, 0, key0, slot);
-      fetch(b, rows, 1, 1, kvh);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->k_full[ks]);
-      if (++ks == kKStages) { ks = 0; kp ^= 1u; }
-      // the next tile's rows
-      if (++j == seg.j1) {
-        more = next(seg, seq);
-        j = more ? seg.j0 : 0;
-        ++nseg;
-      }
-      if (more) entries(rows, seg, seq, j);
-      kv4_wait(&ctl->v_empty[vs], vp);
-      store(a, vt, 0, 1, key0, slot);
-      if (more) fetch(a, rows, 0, 0, seg.kvh);
-      store(b, vt, 1, 1, key0, slot);
-      if (more) fetch(b, rows, 1, 0, seg.kvh);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->v_full[vs]);
-      if (++vs == kVStages) { vs = 0; vp ^= 1u; }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     // ===================== softmax: thread = query row = TMEM lane of tile t =====================
-    const int t = (warp - 8) >> 2, quad = warp & 3;
+    const int t = (warp - 12) >> 2, quad = warp & 3;
     const int row = quad * 32 + lane;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quad * 32) << 16);
     const uint32_t pb = lane_base + 128u + (uint32_t)t * 64u, ob = lane_base + 256u + (uint32_t)t * 128u;
@@ -410,11 +436,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
     uint32_t s_phase = 0, pv_phase = 0;
     int nseg = 0;
     for (; next(seg, seq); ++nseg) {
-      const int nt = key_tiles(seq, G, seg.rb, t), j_end = nt < seg.j1 ? nt : seg.j1;
-      const int64_t r = (int64_t)seg.rb * kRows + t * kBM + row;
-      const int token = (int)(r / G), head = seg.kvh * G + (int)(r - (int64_t)token * G);
+      const int nt = key_tiles(p, seq, seg.rb, t), j_end = nt < seg.j1 ? nt : seg.j1;
+      const int r = seg.rb * kRows + t * kBM + row;
+      const int token = over_G(p, r), head = seg.kvh * G + r - token * G;
       const bool live = token < seq.m;
-      const int64_t place = live ? load_index(p.start, seg.b, p.start_w) + token : 0;
+      const int64_t place = live ? seq.start + token : 0;
       const int64_t part = ((int64_t)blockIdx.x * 2 + (seg.j0 == 0 ? 1 : 0)) * kRows + t * kBM + row;
       const bool whole = seg.j0 == 0 && seg.j1 == seg.steps;
       float m_used = -INFINITY, l_run = 0.f;      // m_used: the maximum the accumulated P / O / l are scaled by
@@ -469,81 +495,95 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
         const int pos = seq.ctx + token, see = live ? (pos < seq.keys - 1 ? pos : seq.keys - 1) : -1;   // last key that counts
         const int see_all = __reduce_min_sync(0xffffffffu, live ? see : INT_MAX);
 
-        auto tile = [&](const int j, auto masked) {
-          constexpr bool kMasked = decltype(masked)::value;
-          kv4_wait(&ctl->s_full[t], s_phase);
-          s_phase ^= 1u;
-          tc_fence_after();
-          uint32_t sv[kBN];
+        // The row's scores come in two halves of 64, for which a thread's registers suffice beside eight converting warps, and a tile's
+        // columns are free for the next half once they are read: the products of one half run under the exponentials of the other.
+        // Either may raise the maximum; the second one then rescales the first one's probabilities too (rarely).
+        // Loops stay rolled and the mask is a pass of its own: with copies for masked tiles and for either half the roles' code did not
+        // fit into the instruction cache (6000 cycles a step, most of them waiting for instructions).
+#pragma unroll 1
+        for (int j = seg.j0; j < j_end; ++j) {
+          const bool masked = (j + 1) * kBN - 1 > see_all;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            constexpr int kN = kBN / 2;
+            kv4_wait(&ctl->s_full[t], s_phase);
+            s_phase ^= 1u;
+            tc_fence_after();
+            uint32_t sv[kN];
 #pragma unroll
-          for (int c = 0; c < kBN; c += 32) tmem_ld_32x32b_x32(lane_base + c, *reinterpret_cast<uint32_t(*)[32]>(sv + c));
-          tc_wait_ld();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->s_free);
-          const int limit = see - j * kBN;        // masked tile: key column i is visible iff i <= limit
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int c = 0; c < kN; c += 32) tmem_ld_32x32b_x32(lane_base + (uint32_t)t * 64u + c, *reinterpret_cast<uint32_t(*)[32]>(sv + c));
+            tc_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->s_free[t]);
+            if (masked) {
+              const int limit = see - j * kBN - h * kN;            // key column i is visible iff i <= limit
 #pragma unroll
-          for (int i = 0; i < kBN; i += 8) {
+              for (int i = 0; i < kN; ++i) sv[i] = i <= limit ? sv[i] : 0xff800000u;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float x = __uint_as_float(sv[i + 2 * c]), y = __uint_as_float(sv[i + 2 * c + 1]);
-              if (kMasked) {
-                x = i + 2 * c <= limit ? x : -INFINITY;
-                y = i + 2 * c + 1 <= limit ? y : -INFINITY;
+            for (int i = 0; i < kN; i += 8)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(sv[i + 2 * c]), __uint_as_float(sv[i + 2 * c + 1]));
+            const float m_half = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
+            const bool grow = m_half > m_used + kLazy;             // at first m_used = -inf: true
+            const float m_new = grow ? m_half : m_used;
+            const float base = m_new == -INFINITY ? 0.f : m_new;   // nothing visible yet: avoid inf - inf
+            if (h == 0 && j > seg.j0) { kv4_wait(&ctl->pv_done[t], pv_phase); pv_phase ^= 1u; tc_fence_after(); }
+            if (__any_sync(0xffffffffu, grow)) {
+              const float alpha = grow ? fast_exp2(m_used - base) : 1.0f;
+              l_run *= alpha;
+              if (h == 1) {                                        // the first half's probabilities
+                tc_wait_st_();
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(pb, v);
+                tc_wait_ld();
+                const __half2 a2 = __float2half2_rn(alpha);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                  const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&v[i]), a2);
+                  v[i] = *reinterpret_cast<const uint32_t*>(&x);
+                }
+                tmem_st_32x32b_x32(pb, v);
               }
-              mx[c] = max3(mx[c], x, y);
-            }
-          }
-          const float m_tile = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
-          const bool grow = m_tile > m_used + kLazy;               // first tile: m_used = -inf -> true
-          const float m_new = grow ? m_tile : m_used;
-          const float base = m_new == -INFINITY ? 0.f : m_new;     // nothing visible yet: avoid inf - inf
-          const float alpha = grow ? fast_exp2(m_used - base) : 1.0f;
-          const uint64_t scale2 = f32x2(scale, scale), base2 = f32x2(-base, -base);
-          uint64_t lsum2 = 0ull;
-          if (j > seg.j0) { kv4_wait(&ctl->pv_done[t], pv_phase); pv_phase ^= 1u; tc_fence_after(); }
+              if (j > seg.j0) {
+#pragma unroll 1
+                for (int c = 0; c < DP; c += 32) {
+                  uint32_t v[32];
+                  tmem_ld_32x32b_x32(ob + c, v);
+                  tc_wait_ld();
 #pragma unroll
-          for (int c = 0; c < kBN; c += 32) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float p0, p1;
-              f32x2_split(f32x2_fma(f32x2(__uint_as_float(sv[c + i]), __uint_as_float(sv[c + i + 1])), scale2, base2), p0, p1);
-              p0 = fast_exp2(p0);
-              p1 = fast_exp2(p1);
-              if (kMasked) {
-                p0 = c + i <= limit ? p0 : 0.f;
-                p1 = c + i + 1 <= limit ? p1 : 0.f;
+                  for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                  tmem_st_32x32b_x32(ob + c, v);
+                }
               }
-              lsum2 = f32x2_add(lsum2, f32x2(p0, p1));
-              pk[i >> 1] = pack2<__half>(p0, p1);
             }
-            tmem_st_32x32b_x16(pb + (c >> 1), pk);
-          }
-          float l0, l1;
-          f32x2_split(lsum2, l0, l1);
-          l_run = l_run * alpha + (l0 + l1);
-          m_used = m_new;
-          if (j > seg.j0 && __any_sync(0xffffffffu, grow)) {
+            m_used = m_new;
+            const uint64_t scale2 = f32x2(scale, scale), base2 = f32x2(-base, -base);
+            uint64_t lsum2 = 0ull;
 #pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-              uint32_t v[32];
-              tmem_ld_32x32b_x32(ob + c, v);
-              tc_wait_ld();
+            for (int c = 0; c < kN; c += 32) {
+              uint32_t pk[16];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-              tmem_st_32x32b_x32(ob + c, v);
+              for (int i = 0; i < 32; i += 2) {
+                float p0, p1;
+                f32x2_split(f32x2_fma(f32x2(__uint_as_float(sv[c + i]), __uint_as_float(sv[c + i + 1])), scale2, base2), p0, p1);
+                p0 = fast_exp2(p0);
+                p1 = fast_exp2(p1);
+                lsum2 = f32x2_add(lsum2, f32x2(p0, p1));
+                pk[i >> 1] = pack2<__half>(p0, p1);
+              }
+              tmem_st_32x32b_x16(pb + h * (kN / 2) + (c >> 1), pk);
             }
+            float l0, l1;
+            f32x2_split(lsum2, l0, l1);
+            l_run += l0 + l1;
           }
           tc_wait_st_();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctl->p_full[t]);
-        };
-        for (int j = seg.j0; j < j_end; ++j) {
-          if ((j + 1) * kBN - 1 > see_all) tile(j, std::true_type{});
-          else tile(j, std::false_type{});
         }
         kv4_wait(&ctl->pv_done[t], pv_phase);
         pv_phase ^= 1u;
@@ -553,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
         T* orow = reinterpret_cast<T*>(p.out) + place * p.o_ts + (int64_t)(live ? head : 0) * p.o_hs;
         float* prow = p.ws_o + part * D;
         constexpr int kFrom[8] = {0, 2, 4, 6, 1, 3, 5, 7};
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t v[32];
           tmem_ld_32x32b_x32(ob + c, v);          // warp-collective: outside the row predicate
@@ -608,18 +648,17 @@ __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(const Params p) {
   constexpr int E = D / 32, kRowsHere = 32;
   const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Seq s = sequence(p, b);
-  const int64_t r0 = (int64_t)blockIdx.x * kRowsHere, rows = (int64_t)s.m * p.G;
+  const int r0 = blockIdx.x * kRowsHere, rows = s.m * p.G;
   if (r0 >= rows) return;
-  const int rb = (int)(r0 / kRows);
-  const int2 who = __ldcg(p.ws_info + __ldcg(p.ws_item + b) + kvh * row_blocks(s, p.G) + rb);
+  const int rb = r0 / kRows;
+  const int2 who = __ldcg(p.ws_info + __ldcg(p.ws_item + b) + kvh * row_blocks(p, s) + rb);
   const int n = who.y - who.x + 1;
   if (n < 2) return;                              // written by its only CTA
-  const int64_t start = load_index(p.start, b, p.start_w);
-  for (int64_t r = r0 + warp; r < r0 + kRowsHere && r < rows; r += 8) {
+  for (int r = r0 + warp; r < r0 + kRowsHere && r < rows; r += 8) {
     float acc[E], M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    const int64_t in_block = r - (int64_t)rb * kRows;
+    const int in_block = r - rb * kRows;
     for (int i0 = 0; i0 < n; i0 += 4) {
       float x[4][E];
       float2 ml[4];
@@ -653,22 +692,24 @@ __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(const Params p) {
       }
       M = mm;
     }
-    const int token = (int)(r / p.G), head = kvh * p.G + (int)(r - (int64_t)token * p.G);
-    T* out = reinterpret_cast<T*>(p.out) + (start + token) * p.o_ts + (int64_t)head * p.o_hs;
+    const int token = over_G(p, r), head = kvh * p.G + r - token * p.G;
+    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(s.start + token) * p.o_ts + (int64_t)head * p.o_hs;
 #pragma unroll
     for (int e = 0; e < E; ++e) out[e * 32 + lane] = from_f32<T>(L == 0.f ? 0.f : acc[e] / L);
   }
 }
 
-struct Plan { int grid, smem; int64_t items, rows; };
+struct Plan { int grid, smem; int64_t items, rows, steps; };
 
 Plan make_plan(int64_t batch, int64_t total, int G, int Hkv, int D, int64_t max_len) {
   Plan pl;
   const int DP = D < 64 ? 64 : D;
   const int64_t rows = batch < kMaxBatch ? batch : kMaxBatch;
-  pl.smem = 1024 + (2 + kKStages + kVStages) * kBN * DP * 2 + (int)(rows + 1) * 8 + (int)rows * 4;
+  pl.smem = 1024 + (2 + kKStages + kVStages) * kBN * DP * 2 + kUnits * kUnitKeys * kUnitPitch +
+            (2 * kMaxBatch + 1) * 4 + kMaxBatch * (int)sizeof(Seq);
   pl.items = (cdiv64(total * G, kRows) + rows) * Hkv;
-  const int64_t steps = pl.items * cdiv64(max_len > 0 ? max_len : 1, kBN), worth = cdiv64(steps, kMinSteps);
+  pl.steps = pl.items * cdiv64(max_len > 0 ? max_len : 1, kBN);
+  const int64_t worth = cdiv64(pl.steps, kMinSteps);
   pl.grid = (int)(worth < b2l_num_sms() ? worth : b2l_num_sms());
   if (pl.grid < 1) pl.grid = 1;
   pl.rows = 2ll * pl.grid * kRows;
@@ -717,12 +758,13 @@ extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* ca
   B2L_REQUIRE(cache_row_stride >= kv4::row_bytes(num_kv_heads, head_dim, group) && cache_row_stride % 16 == 0 && (uintptr_t)cache % 16 == 0,
               "%s: cache rows must be 16-byte aligned and hold %lld bytes", what, (long long)kv4::row_bytes(num_kv_heads, head_dim, group));
   B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "%s: dtype %d", what, dtype);
+  B2L_REQUIRE(qk_scale > 0.f && qk_scale < INFINITY, "%s: qk_scale must be positive", what);
   B2L_REQUIRE(batch >= 0 && total_tokens >= 0 && max_tokens > 0 && max_tokens < (1ll << 31) && table_requests >= 0 && table_width >= 0 &&
                   max_new_len >= 0 && max_new_len < (1ll << 30) && max_seq_len < (1ll << 30), "%s: bad shape", what);
   if (batch == 0 || total_tokens == 0 || max_new_len == 0) return B2L_OK;
   const int G = num_q_heads / num_kv_heads;
   const Plan pl = make_plan(batch, total_tokens, G, num_kv_heads, head_dim, max_seq_len);
-  B2L_REQUIRE(pl.items < (1ll << 31) && total_tokens * G < (1ll << 31), "%s: too many tokens", what);
+  B2L_REQUIRE(pl.steps < (1ll << 31) && total_tokens * G < (1ll << 31), "%s: too many tokens", what);
   B2L_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
                   workspace_bytes >= b2l_flash_attention_int4_workspace_bytes(batch, total_tokens, num_q_heads, num_kv_heads, head_dim, group, max_seq_len),
               "%s: workspace too small", what);
@@ -734,7 +776,7 @@ extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* ca
   p.cache = (const uint8_t*)cache; p.row_stride = cache_row_stride; p.max_tokens = max_tokens;
   p.table = (const int32_t*)b_req_tokens_table; p.tab_rs = table_req_stride; p.tab_cs = table_seq_stride; p.requests = table_requests;
   p.start_w = start_width; p.fresh_w = new_width; p.req_w = req_width; p.len_w = len_width;
-  p.Hkv = num_kv_heads; p.G = G;
+  p.Hkv = num_kv_heads; p.G = G; p.by_G = G > 1 ? ~0ull / G + 1 : 0;
   p.total = total_tokens; p.max_new = max_new_len < total_tokens ? max_new_len : total_tokens;
   p.most = max_seq_len < table_width ? max_seq_len : table_width;
   if (p.most < 0) p.most = 0;
