@@ -12,13 +12,14 @@
 // columns that up to four heads leave free, else in a second product -- since a code's products are larger than its value's.
 //
 // Work: tiles of 16 * TS tokens of all rows, in equal shares over one wave of CTAs, whatever rows they belong to (the lengths are device
-// data).  A producer warp copies whole token rows by the TMA engine into a ring; a consumer warp takes 16 tokens of one kv head.  A row
+// data).  Whole token rows come by the TMA engine into a ring, asked for by the warps in turn (with a warp of its own for that, two
+// CTAs leave a thread 96 registers, and spill); a warp takes 16 tokens of one kv head.  A row
 // that lies in one share is written out; else its parts go to the workspace and a second kernel adds them up.
 #include "kv_int4.cuh"
 
 namespace {
 
-constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16;
+constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kAhead = 4;   // five warps at least: a warp's tiles lie further apart
 constexpr int kMinTokens = 64;                    // of a share: below that the merge costs more than the share
 
 struct Int4DecodeParams {
@@ -57,7 +58,8 @@ struct Int4Consumer {
   float O[MT][4], z[2][NG];                       // sums of p s c (rows r + 8 hold 16 times theirs) and of p m
   float m[2], l[2], m_lim[2];                     // scores are relative to m; above m_lim it is raised
   float v_scale, v_lim;                           // value scales are multiplied by v_scale = 2^-e before p s is rounded
-  int lane, r, c;
+  int r, c;
+  int k_at, g_at, v_at[2], step;                   // bytes from a unit's first row: key words, groups, value words of two tokens; eight rows
 
   static __device__ __forceinline__ int word_at(int k, int c) { return GS == 32 ? k * 4 + c : (k >> 1) * 8 + c * 2 + (k & 1); }
   static __device__ __forceinline__ constexpr int group_of(int k) { return GS == 32 ? k : GS == 64 ? k >> 1 : 0; }
@@ -162,21 +164,29 @@ struct Int4Consumer {
     }
   }
 
+  __device__ __forceinline__ Int4Consumer(int lane, int pitch) {
+    r = lane >> 2;
+    c = lane & 3;
+    step = 8 * pitch;
+    k_at = place(r) * pitch + c * (GS == 32 ? 4 : 8);
+    g_at = place(r) * pitch + D;
+    v_at[0] = place(2 * c) * pitch + D / 2 + (GS == 32 ? r >> 1 : r) * 4;
+    v_at[1] = place(2 * c + 1) * pitch + D / 2 + (GS == 32 ? r >> 1 : r) * 4;
+  }
+
   // 16 tokens at `at` (the head's bytes of the first), of which `valid` count (one form for all: a copy without the mask costs more in
   // the instruction cache than the mask)
-  __device__ __forceinline__ void unit(const uint8_t* at, int pitch, int valid) {
+  __device__ __forceinline__ void unit(const uint8_t* at, int valid) {
     constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-    const uint8_t* row0 = at + place(r) * pitch;
-    const uint8_t* row1 = row0 + 8 * pitch;
     // ---- scores of 16 tokens (rows) and 8 heads (columns) ----
     uint32_t w0[NW], w1[NW];
 #pragma unroll
     for (int k = 0; k < NW; ++k) {
       if (GS == 32) {
-        w0[k] = reinterpret_cast<const uint32_t*>(row0)[k * 4 + c];
-        w1[k] = reinterpret_cast<const uint32_t*>(row1)[k * 4 + c];
+        w0[k] = *reinterpret_cast<const uint32_t*>(at + k_at + k * 16);
+        w1[k] = *reinterpret_cast<const uint32_t*>(at + k_at + step + k * 16);
       } else if ((k & 1) == 0) {
-        const uint2 x = reinterpret_cast<const uint2*>(row0)[(k >> 1) * 4 + c], y = reinterpret_cast<const uint2*>(row1)[(k >> 1) * 4 + c];
+        const uint2 x = *reinterpret_cast<const uint2*>(at + k_at + k * 16), y = *reinterpret_cast<const uint2*>(at + k_at + step + k * 16);
         w0[k] = x.x; w0[k + 1] = x.y;
         w1[k] = y.x; w1[k + 1] = y.y;
       }
@@ -197,11 +207,17 @@ struct Int4Consumer {
     float2 ks[2][NG], vs[2][NG];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t* gp = reinterpret_cast<const uint32_t*>((i ? row1 : row0) + D);
+      uint32_t g[2 * NG];                         // of K, then of V
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        ks[i][g] = kv4::scale_min<T>(gp[g]);
-        vs[i][g] = kv4::scale_min<T>(gp[NG + g]);
+      for (int x = 0; x < NG; ++x) {
+        const uint2 y = *reinterpret_cast<const uint2*>(at + g_at + i * step + x * 8);
+        g[2 * x] = y.x;
+        g[2 * x + 1] = y.y;
+      }
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        ks[i][x] = kv4::scale_min<T>(g[x]);
+        vs[i][x] = kv4::scale_min<T>(g[NG + x]);
       }
     }
     float v[2][2], top = 0.f;
@@ -254,8 +270,6 @@ struct Int4Consumer {
         }
       }
     // ---- values: rows are elements, columns heads, the products run over tokens ----
-    const uint8_t* t0 = at + D / 2 + place(2 * c) * pitch;
-    const uint8_t* t1 = at + D / 2 + place(2 * c + 1) * pitch;
     auto add = [&](int tile, int g, const uint32_t (&a)[4]) {
       mma_m16n8k16<__half>(O[tile], a, pb[g][0], pb[g][1]);
       if (!DUP) mma_m16n8k16<__half>(O[tile], a, rest[g][0], rest[g][1]);
@@ -264,9 +278,8 @@ struct Int4Consumer {
       const uint32_t pick = (r & 1) ? 0x7632u : 0x5410u;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const int o = (g * 4 + (r >> 1)) * 4;
-        auto word = [&](const uint8_t* t) { return *reinterpret_cast<const uint32_t*>(t + o); };
-        const uint32_t x = __byte_perm(word(t0), word(t1), pick), y = __byte_perm(word(t0 + 8 * pitch), word(t1 + 8 * pitch), pick);
+        auto word = [&](int o) { return *reinterpret_cast<const uint32_t*>(at + o + g * 16); };
+        const uint32_t x = __byte_perm(word(v_at[0]), word(v_at[1]), pick), y = __byte_perm(word(v_at[0] + step), word(v_at[1] + step), pick);
         const uint32_t a0[4] = {x & kLow, x & kHigh, y & kLow, y & kHigh};
         const uint32_t x8 = x >> 8, y8 = y >> 8;
         const uint32_t a1[4] = {x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh};
@@ -276,9 +289,9 @@ struct Int4Consumer {
     } else {
 #pragma unroll
       for (int b = 0; b < D / 64; ++b) {
-        const int o = (b * 8 + r) * 4, g = b * 64 / GS;
-        auto word = [&](const uint8_t* t) { return *reinterpret_cast<const uint32_t*>(t + o); };
-        const uint32_t e0 = word(t0), e1 = word(t1), e2 = word(t0 + 8 * pitch), e3 = word(t1 + 8 * pitch);
+        const int g = b * 64 / GS;
+        auto word = [&](int o) { return *reinterpret_cast<const uint32_t*>(at + o + b * 32); };
+        const uint32_t e0 = word(v_at[0]), e1 = word(v_at[1]), e2 = word(v_at[0] + step), e3 = word(v_at[1] + step);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t x = __byte_perm(e0, e1, h ? 0x7632 : 0x5410), y = __byte_perm(e2, e3, h ? 0x7632 : 0x5410);
@@ -325,10 +338,10 @@ struct Int4Consumer {
 struct Segment { int b, first, last, tiles; };    // tiles [first, last) of a row of `tiles`
 
 template <typename T, int D, int GS, bool DUP>
-__global__ void __launch_bounds__((kMaxConsumers + 1) * 32, 2) kv4_decode_kernel(const Int4DecodeParams p) {
+__global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const Int4DecodeParams p) {
   pdl_prologue();   // everything below reads what earlier kernels of the step wrote
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int warp_sum[kMaxConsumers + 1];
+  __shared__ int warp_sum[kMaxConsumers];
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem);
   uint64_t* empty_bar = full_bar + kMaxStages;
   uint8_t* ring = smem + 128;
@@ -339,7 +352,7 @@ __global__ void __launch_bounds__((kMaxConsumers + 1) * 32, 2) kv4_decode_kernel
   int* lens = prefix + p.batch + 1;
   int* reqs = lens + p.batch;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int nconsumers = p.HB * p.qblocks * p.TS;
+  const int nwarps = p.HB * p.qblocks * p.TS;
   const int nblk = p.Hkv / p.HB;
 
   // ---- tiles of the rows before each; a thread owns neighbouring rows ----
@@ -362,13 +375,13 @@ __global__ void __launch_bounds__((kMaxConsumers + 1) * 32, 2) kv4_decode_kernel
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full_bar[s], 1);
-      mbar_init(&empty_bar[s], nconsumers);
+      mbar_init(&empty_bar[s], nwarps);
     }
     mbar_fence_init();
   }
   __syncthreads();
   int at = upto - own, all = 0;
-  for (int w = 0; w <= nconsumers; ++w) {
+  for (int w = 0; w < nwarps; ++w) {
     if (w < warp) at += warp_sum[w];
     all += warp_sum[w];
   }
@@ -387,11 +400,11 @@ __global__ void __launch_bounds__((kMaxConsumers + 1) * 32, 2) kv4_decode_kernel
   if (blockIdx.x >= shares) return;
   int64_t item = blockIdx.x * total / shares;
   const int64_t item_end = (blockIdx.x + 1) * total / shares;
-  // the next part of a row, and the block of heads it is in
-  auto next = [&](Segment& s, int& blk) -> bool {
+  // the part of a row at `item`, and the block of heads it is in
+  auto next = [&](int64_t& item, Segment& s, int& blk) -> bool {
     if (item >= item_end) return false;
-    blk = (int)(item / all);
-    const int x = (int)(item - (int64_t)blk * all);
+    blk = (int)((uint32_t)item / (uint32_t)all);
+    const int x = (int)item - blk * all;
     int lo = 0, n = p.batch;                      // the last row that begins at or before x and has tiles
     while (n > 1) {
       const int half = n / 2;
@@ -407,49 +420,82 @@ __global__ void __launch_bounds__((kMaxConsumers + 1) * 32, 2) kv4_decode_kernel
     return true;
   };
 
-  Segment seg;
-  int blk, s = 0;
-  uint32_t phase = 0;
+  // ---- the ring's copies: tile f of the share is brought by warp f % nwarps.  It reads the table kAhead tiles before its stage is due and
+  // waits for that stage when the tile before this one has been worked on. ----
   const int hb = kv4::head_bytes(D, GS);
-  if (warp == nconsumers) {
-    // ===================== producer: token rows by the copy engine =====================
-    while (next(seg, blk)) {
-      const int len = lens[seg.b];
-      const int32_t* entry = p.table + (int64_t)reqs[seg.b] * p.tab_rs;
-      const int from = blk * p.HB * hb, shift = from & 15;
-      const uint32_t bytes = (uint32_t)((shift + p.HB * hb + 15) & ~15);
-      const uint8_t* src = p.cache + (from - shift);
-      for (int t = seg.first; t < seg.last; ++t) {
-        mbar_wait(&empty_bar[s], phase ^ 1);
-        const int here = len - t * tile < tile ? len - t * tile : tile;
-        if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], (uint32_t)here * bytes);
-        __syncwarp();
-        for (int i = lane; i < here; i += 32) {
-          int64_t row = entry[(int64_t)(t * tile + i) * p.tab_cs];
-          if (row < 0 || row >= p.max_tokens) row = 0;
-          bulk_g2s(ring + s * stage_bytes + i * p.pitch, src + row * p.row_stride, bytes, &full_bar[s]);
-        }
-        if (++s == p.stages) { s = 0; phase ^= 1; }
+  struct Fill { int row[kMaxConsumers / 2]; int here, f, from; } fill;
+  Segment ahead;                                  // of the tile whose entries are read next
+  int ahead_blk, ahead_t = 0, ahead_f = 0;
+  int64_t ahead_item = item;
+  bool more = next(ahead_item, ahead, ahead_blk);
+  if (more) ahead_t = ahead.first;
+  fill.f = -1;
+  auto look = [&] {
+    if (!more) return;
+    if (ahead_f % nwarps == warp) {
+      const int len = lens[ahead.b];
+      const int32_t* entry = p.table + (int64_t)reqs[ahead.b] * p.tab_rs;
+      fill.f = ahead_f;
+      fill.here = len - ahead_t * tile < tile ? len - ahead_t * tile : tile;
+      fill.from = ahead_blk * p.HB * hb;
+#pragma unroll
+      for (int k = 0; k < kMaxConsumers / 2; ++k) {
+        const int i = k * 32 + lane;
+        if (i < fill.here) fill.row[k] = ld_upstream(entry + (int64_t)(ahead_t * tile + i) * p.tab_cs);
       }
     }
-    return;
+    ++ahead_f;
+    if (++ahead_t == ahead.last) {
+      more = next(ahead_item, ahead, ahead_blk);
+      if (more) ahead_t = ahead.first;
+    }
+  };
+  auto bring = [&](int f, int s, uint32_t empty_parity, bool wait) {
+    if (fill.f != f) return;
+    const int shift = fill.from & 15;
+    const uint32_t bytes = (uint32_t)((shift + p.HB * hb + 15) & ~15);
+    const uint8_t* src = p.cache + (fill.from - shift);
+    if (wait) mbar_wait(&empty_bar[s], empty_parity);
+    if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], (uint32_t)fill.here * bytes);
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kMaxConsumers / 2; ++k) {
+      const int i = k * 32 + lane;
+      if (i < fill.here) {
+        const int64_t row = fill.row[k] < 0 || fill.row[k] >= p.max_tokens ? 0 : fill.row[k];
+        bulk_g2s(ring + s * stage_bytes + i * p.pitch, src + row * p.row_stride, bytes, &full_bar[s]);
+      }
+    }
+    fill.f = -1;
+  };
+  for (int f = 0; f < p.stages; ++f) {
+    look();
+    bring(f, f, 0, false);
   }
-  // ===================== consumers: (kv head, block of query heads, unit of the tile) =====================
+  for (int k = 0; k < kAhead; ++k) look();
+
+  Segment seg;
+  int blk, s = 0, at_tile = 0;
+  uint32_t phase = 0;
+  // ===================== a warp: (kv head, block of query heads, unit of the tile) =====================
   const int ts = warp / (p.HB * p.qblocks), wh = warp - ts * p.HB * p.qblocks;
   const int hl = wh / p.qblocks, qblk = wh - hl * p.qblocks;
   const int head0 = qblk * 8, heads = p.G - head0 < 8 ? p.G - head0 : 8;
-  Int4Consumer<T, D, GS, DUP> c;
-  c.lane = lane; c.r = lane >> 2; c.c = lane & 3;
-  while (next(seg, blk)) {
+  Int4Consumer<T, D, GS, DUP> c(lane, p.pitch);
+  while (next(item, seg, blk)) {
     const int len = lens[seg.b], kvh = blk * p.HB + hl;
     const int off = ((blk * p.HB * hb) & 15) + hl * hb + ts * unit_bytes;
     c.begin(p, seg.b, kvh, head0, heads);
 #pragma unroll 1
-    for (int t = seg.first; t < seg.last; ++t) {
+    for (int t = seg.first; t < seg.last; ++t, ++at_tile) {
+      if (at_tile > 0) {                          // into the stage of the tile before this one
+        const int b = s == 0 ? p.stages - 1 : s - 1;
+        bring(at_tile - 1 + p.stages, b, s == 0 ? phase ^ 1u : phase, true);
+        look();
+      }
       mbar_wait(&full_bar[s], phase);
       const int valid = len - t * tile - ts * kUnit;
-      const uint8_t* u = ring + s * stage_bytes + off;
-      if (valid > 0) c.unit(u, p.pitch, valid);
+      if (valid > 0) c.unit(ring + s * stage_bytes + off, valid);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[s]);
       if (++s == p.stages) { s = 0; phase ^= 1; }
@@ -458,7 +504,7 @@ __global__ void __launch_bounds__((kMaxConsumers + 1) * 32, 2) kv4_decode_kernel
     // columns of this lane: heads 2c and 2c + 1 (DUP: the upper half of the columns repeats the lower)
     const bool mine = !DUP || c.c < 2;
     if (p.TS > 1) {
-      auto bar = [&] { asm volatile("bar.sync 1, %0;" ::"r"(nconsumers * 32) : "memory"); };
+      auto bar = [&] { asm volatile("bar.sync 1, %0;" ::"r"(nwarps * 32) : "memory"); };
       bar();                                      // the sums before these have been read
       float* mineat = join + ((ts - 1) * p.HB * p.qblocks + wh) * 8 * (D + 2);
       if (ts > 0 && mine) {
@@ -521,35 +567,37 @@ __global__ void __launch_bounds__((kMaxConsumers + 1) * 32, 2) kv4_decode_kernel
   }
 }
 
-// The rows that several CTAs met in, and zeros for the empty ones.  Eight warps take the parts in turn, so that their loads are on
-// their way together, and meet in shared memory.
+// The rows that several CTAs met in, and zeros for the empty ones.  Bound by latency: a block takes one head of a row, its warps the
+// parts in turn, eight of each on their way together, and meet in shared memory.
+constexpr int kMergeWarps = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_decode_merge_kernel(const Int4DecodeParams p) {
+__global__ void __launch_bounds__(kMergeWarps * 32) kv4_decode_merge_kernel(const Int4DecodeParams p) {
   pdl_prologue();
-  constexpr int E = D / 32;                       // neighbouring elements of a lane
-  __shared__ float sums[8][D + 2];
+  constexpr int E = D / 32, kAsk = 8;             // neighbouring elements of a lane
+  __shared__ float sums[kMergeWarps][D + 2];
   const int b = blockIdx.x, head = blockIdx.y, kvh = head / p.G, blk = kvh / p.HB;
   const int local = (kvh - blk * p.HB) * p.G + head - kvh * p.G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int2 who = __ldcg(p.ws_info + (int64_t)blk * p.batch + b);   // of an empty row: an earlier call's
   const int64_t len = load_index(p.seq_len, b, p.len_w), q = load_index(p.req_idx, b, p.req_w);
   T* out = reinterpret_cast<T*>(p.out) + (int64_t)b * p.o_bs + (int64_t)head * p.o_hs;
   if (len <= 0 || q < 0 || q >= p.requests || p.most <= 0) {
     for (int d = threadIdx.x; d < D; d += blockDim.x) out[d] = from_f32<T>(0.f);
     return;
   }
-  const int2 who = __ldcg(p.ws_info + (int64_t)blk * p.batch + b);
   const int n = who.y - who.x + 1;
   if (n < 2) return;                              // written by its only CTA
   auto part = [&](int i) { return ((int64_t)(who.x + i) * 2 + (i == 0 ? 1 : 0)) * p.HB * p.G + local; };
   float acc[E], M = -INFINITY, L = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int i0 = warp; i0 < n; i0 += 32) {         // four parts of this warp at a time
-    float x[4][E];
-    float2 ml[4];
+#pragma unroll 1
+  for (int i0 = warp; i0 < n; i0 += kMergeWarps * kAsk) {
+    float x[kAsk][E];
+    float2 ml[kAsk];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = i0 + 8 * k;
+    for (int k = 0; k < kAsk; ++k) {
+      const int i = i0 + kMergeWarps * k;
       ml[k] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int e = 0; e < E; ++e) x[k][e] = 0.f;
@@ -569,13 +617,13 @@ __global__ void __launch_bounds__(256) kv4_decode_merge_kernel(const Int4DecodeP
     }
     float mm = M;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) mm = fmaxf(mm, ml[k].x);
+    for (int k = 0; k < kAsk; ++k) mm = fmaxf(mm, ml[k].x);
     const float base = mm == -INFINITY ? 0.f : mm, a = fast_exp2(M - base);
     L *= a;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= a;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kAsk; ++k) {
       const float w = fast_exp2(ml[k].x - base);
       L = fmaf(ml[k].y, w, L);
 #pragma unroll
@@ -590,10 +638,10 @@ __global__ void __launch_bounds__(256) kv4_decode_merge_kernel(const Int4DecodeP
   if ((int)threadIdx.x < D) {
     float mm = -INFINITY, o = 0.f, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) mm = fmaxf(mm, sums[w][D]);
+    for (int w = 0; w < kMergeWarps; ++w) mm = fmaxf(mm, sums[w][D]);
     const float base = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < kMergeWarps; ++w) {
       const float a = fast_exp2(sums[w][D] - base);
       o = fmaf(sums[w][threadIdx.x], a, o);
       l = fmaf(sums[w][D + 1], a, l);
@@ -634,13 +682,13 @@ Int4Plan make_plan(int64_t batch, int G, int Hkv, int D, int group, int64_t max_
 
 template <typename T, int D, int GS>
 int launch_int4_decode(const Int4DecodeParams& p, const Int4Plan& pl, cudaStream_t st) {
-  const dim3 grid((unsigned)pl.grid), block((pl.HB * pl.qblocks * pl.TS + 1) * 32);
+  const dim3 grid((unsigned)pl.grid), block(pl.HB * pl.qblocks * pl.TS * 32);
   static int configured[2][64] = {{0}};
   auto kern = p.G <= 4 ? kv4_decode_kernel<T, D, GS, true> : kv4_decode_kernel<T, D, GS, false>;
   B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured[p.G <= 4]));
   b2l_launch(kern, grid, block, (size_t)pl.smem, st, p);
   B2L_LAUNCH_CHECK();
-  b2l_launch(kv4_decode_merge_kernel<T, D>, dim3((unsigned)p.batch, (unsigned)p.Hq), dim3(256), (size_t)0, st, p);
+  b2l_launch(kv4_decode_merge_kernel<T, D>, dim3((unsigned)p.batch, (unsigned)p.Hq), dim3(kMergeWarps * 32), (size_t)0, st, p);
   B2L_LAUNCH_CHECK();
   return B2L_OK;
 }
@@ -698,6 +746,7 @@ extern "C" int b2l_flash_decoding_int4(void* out, const void* q, const void* cac
   p.stages = pl.stages; p.pitch = pl.pitch;
   p.most = max_seq_len < table_width ? max_seq_len : table_width;
   if (p.most < 0) p.most = 0;
+  B2L_REQUIRE((batch < kMaxBatch ? batch : kMaxBatch) * cdiv64(p.most, kUnit) * num_kv_heads < (1ll << 31), "flash_decoding_int4: too many tokens");
   p.q_vec = (uintptr_t)q % 16 == 0 && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0;
   p.scale_log2 = qk_scale * 1.4426950408889634f;
   p.ws_o = (float*)workspace;

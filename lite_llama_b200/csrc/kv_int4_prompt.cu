@@ -45,7 +45,7 @@ struct Params {
   uint64_t by_G;                                  // 2^64 / G, rounded up: n / G is the high half of n * by_G for n < 2^32 (G > 1)
   int64_t total, max_new, most;
   float scale_log2;
-  float* ws_o; float2* ws_ml; int2* ws_info; int* ws_item;
+  float* ws_o; float2* ws_ml; int2* ws_info; int4* ws_item;
 };
 
 // a sequence: its m new tokens begin at row `start` of q, the first stands at position ctx, keys below `keys` are cached
@@ -94,7 +94,7 @@ static_assert(sizeof(Ctl) <= 512, "control block");
 // steps [j0, j1) of a row block
 struct Segment { int b, kvh, rb, j0, j1, steps, item; };
 
-#define kv4_wait(bar, parity) mbar_wait_short_at<true>((bar), (parity), b2l_file_hash(__FILE__), __LINE__)
+#define kv4_wait(bar, parity) mbar_wait_at<true>((bar), (parity), b2l_file_hash(__FILE__), __LINE__)
 
 // an asynchronous copy of 4, 8 or 16 bytes to shared memory; zeros where `read` is false
 template <int BYTES>
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
       if (b < p.batch) {
         prefix[b + 1] = steps + s;
         items[b] = blocks + k - own;
-        if (blockIdx.x == 0) p.ws_item[b] = blocks + k - own;
+        if (blockIdx.x == 0) p.ws_item[b] = make_int4(blocks + k - own, seqs[b].m, seqs[b].start, 0);
       }
       steps += __shfl_sync(0xffffffffu, s, 31);
       blocks += __shfl_sync(0xffffffffu, k, 31);
@@ -641,61 +641,70 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
   if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
-// Row blocks that several CTAs met in.  A warp takes rows; the parts of a row are added in order.
+// Row blocks that several CTAs met in.  Bound by latency: a warp asks for the parts of its four rows together, and lengths and notes
+// were left in the workspace by the first CTA.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(const Params p) {
   pdl_prologue();
-  constexpr int E = D / 32, kRowsHere = 32;
+  constexpr int E = D / 32, kR = 4, kRowsHere = 8 * kR;
   const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Seq s = sequence(p, b);
-  const int r0 = blockIdx.x * kRowsHere, rows = s.m * p.G;
+  const int r0 = blockIdx.x * kRowsHere;
+  const int4 s = __ldcg(p.ws_item + b);           // row blocks before, m, start
+  const int rows = s.y * p.G;
   if (r0 >= rows) return;
-  const int rb = r0 / kRows;
-  const int2 who = __ldcg(p.ws_info + __ldcg(p.ws_item + b) + kvh * row_blocks(p, s) + rb);
+  const int rb = r0 / kRows, nb = (rows + kRows - 1) / kRows;
+  const int2 who = __ldcg(p.ws_info + s.x + kvh * nb + rb);
   const int n = who.y - who.x + 1;
   if (n < 2) return;                              // written by its only CTA
-  for (int r = r0 + warp; r < r0 + kRowsHere && r < rows; r += 8) {
-    float acc[E], M = -INFINITY, L = 0.f;
+  const int in_block = r0 - rb * kRows + warp * kR;
+  float acc[kR][E], M[kR], L[kR];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    const int in_block = r - rb * kRows;
-    for (int i0 = 0; i0 < n; i0 += 4) {
-      float x[4][E];
-      float2 ml[4];
+  for (int k = 0; k < kR; ++k) {
+    M[k] = -INFINITY;
+    L[k] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = i0 + k;
-        ml[k] = make_float2(-INFINITY, 0.f);
+    for (int e = 0; e < E; ++e) acc[k][e] = 0.f;
+  }
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += 2) {
+    float x[2][kR][E];
+    float2 ml[2][kR];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[k][e] = 0.f;
-        if (i < n) {
-          const int64_t part = ((int64_t)(who.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + in_block;
-          ml[k] = __ldcg(p.ws_ml + part);
+    for (int i = 0; i < 2; ++i) {
+      if (i0 + i >= n) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) x[k][e] = __ldcg(p.ws_o + part * D + e * 32 + lane);
-        }
+        for (int k = 0; k < kR; ++k) ml[i][k] = make_float2(-INFINITY, 0.f);
+        continue;
       }
-      float mm = M;
+      const int64_t part = ((int64_t)(who.x + i0 + i) * 2 + (i0 + i == 0 ? 1 : 0)) * kRows + in_block;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mm = fmaxf(mm, ml[k].x);
-      const float base = mm == -INFINITY ? 0.f : mm, a = fast_exp2(M - base);
-      L *= a;
+      for (int k = 0; k < kR; ++k) {
+        ml[i][k] = __ldcg(p.ws_ml + part + k);
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] *= a;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (ml[k].y == 0.f) continue;             // a part of keys that the row does not see: nothing was stored
-        const float w = fast_exp2(ml[k].x - base);
-        L = fmaf(ml[k].y, w, L);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(x[k][e], w, acc[e]);
+        for (int e = 0; e < E; ++e) x[i][k][e] = __ldcg(p.ws_o + (part + k) * D + e * 32 + lane);
       }
-      M = mm;
     }
-    const int token = over_G(p, r), head = kvh * p.G + r - token * p.G;
-    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(s.start + token) * p.o_ts + (int64_t)head * p.o_hs;
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[e * 32 + lane] = from_f32<T>(L == 0.f ? 0.f : acc[e] / L);
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < kR; ++k) {
+        if (ml[i][k].y == 0.f) continue;          // a part of keys that the row does not see: nothing was stored
+        const float mm = fmaxf(M[k], ml[i][k].x), base = mm == -INFINITY ? 0.f : mm;
+        const float a = fast_exp2(M[k] - base), w = fast_exp2(ml[i][k].x - base);
+        M[k] = mm;
+        L[k] = L[k] * a + ml[i][k].y * w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[k][e] = acc[k][e] * a + x[i][k][e] * w;
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < kR; ++k) {
+    const int r = r0 + warp * kR + k;
+    if (r >= rows) return;
+    const int token = over_G(p, r), head = kvh * p.G + r - token * p.G;
+    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(s.z + token) * p.o_ts + (int64_t)head * p.o_hs;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e * 32 + lane] = from_f32<T>(L[k] == 0.f ? 0.f : acc[k][e] / L[k]);
   }
 }
 
@@ -736,7 +745,7 @@ extern "C" int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64
   if (batch <= 0 || total_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || !kv4::shape_ok(head_dim, group))
     return 0;
   const kv4p::Plan pl = kv4p::make_plan(batch, total_tokens, num_q_heads / num_kv_heads, num_kv_heads, head_dim, max_seq_len);
-  return pl.rows * (head_dim + 2) * 4 + pl.items * 8 + (int64_t)kv4p::kMaxBatch * 4;
+  return pl.rows * (head_dim + 2) * 4 + pl.items * 8 + (int64_t)kv4p::kMaxBatch * 16 + 16;
 }
 
 extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* cache, int64_t cache_row_stride, int64_t max_tokens,
@@ -784,7 +793,7 @@ extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* ca
   p.ws_o = (float*)workspace;
   p.ws_ml = (float2*)(p.ws_o + pl.rows * head_dim);
   p.ws_info = (int2*)(p.ws_ml + pl.rows);
-  p.ws_item = (int*)(p.ws_info + pl.items);
+  p.ws_item = (int4*)(((uintptr_t)(p.ws_info + pl.items) + 15) & ~(uintptr_t)15);
   cudaStream_t st = (cudaStream_t)stream;
   for (int64_t b0 = 0; b0 < batch; b0 += kMaxBatch) {
     p.batch = (int)(batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch);
