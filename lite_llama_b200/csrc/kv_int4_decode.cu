@@ -12,14 +12,14 @@
 // columns that up to four heads leave free, else in a second product -- since a code's products are larger than its value's.
 //
 // Work: tiles of 16 * TS tokens of all rows, in equal shares over one wave of CTAs, whatever rows they belong to (the lengths are device
-// data).  Whole token rows come by the TMA engine into a ring, asked for by the warps in turn (with a warp of its own for that, two
-// CTAs leave a thread 96 registers, and spill); a warp takes 16 tokens of one kv head.  A row
+// data).  Whole token rows come by asynchronous copies into a ring (of the working warps: with a warp of its own for that, two CTAs to
+// an SM leave a thread 96 registers, and spill); a warp takes 16 or 32 tokens of one kv head.  A row
 // that lies in one share is written out; else its parts go to the workspace and a second kernel adds them up.
 #include "kv_int4.cuh"
 
 namespace {
 
-constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kAhead = 4;   // five warps at least: a warp's tiles lie further apart
+constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kCluster = 8;
 constexpr int kMinTokens = 64;                    // of a share: below that the merge costs more than the share
 
 struct Int4DecodeParams {
@@ -29,7 +29,7 @@ struct Int4DecodeParams {
   const int32_t* table; int64_t tab_rs, tab_cs, requests, width;
   const void* req_idx; int req_w;
   const void* seq_len; int len_w;
-  int batch, Hq, Hkv, G, HB, qblocks, TS, stages, pitch;
+  int batch, Hq, Hkv, G, HB, qblocks, TS, stages, pitch, bulk;
   int64_t most;                                   // tokens of a row that the call's bound lets count
   float scale_log2;
   float* ws_o; float* ws_ml; int2* ws_info;       // parts [cta][2][HB * G]: rows, (largest score, sum); first and last CTA of a row
@@ -40,6 +40,12 @@ __device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+// as common.cuh's, but not volatile: products of the two units of a tile may change places
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
 // 2^e, e clamped to the range of normal numbers
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e < -126 ? 1 : e > 127 ? 254 : e + 127) << 23); }
@@ -48,15 +54,19 @@ __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e < -126 
 // different banks (a row's pitch is 32 bytes past a multiple of 128)
 __device__ __forceinline__ int place(int i) { return i ^ ((i >> 2) & 1); }
 
-// One consumer warp's work: up to 8 query heads of one kv head, units of 16 tokens in turn.
+// units of 16 tokens that a warp takes together: two where their groups' scales leave the registers
+constexpr int units_of(int d, int group) { return d / group > 2 ? 1 : 2; }
+
+// One warp's work: up to 8 query heads of one kv head, U units of 16 tokens in turn.
 // DUP: at most 4 heads; columns 4 - 7 are the same heads again and take what rounding leaves of p s.
 template <typename T, int D, int GS, bool DUP>
 struct Int4Consumer {
-  static constexpr int NG = D / GS, NW = D / 32, MT = D / 16;
+  static constexpr int NG = D / GS, NW = D / 32, MT = D / 16, U = units_of(D, GS);
+  uint4 raw[NW];                                  // the query as it is in memory, between ask() and begin()
   uint32_t qb[NW][4];                             // a key word's query elements: nibbles (0, 4), (2, 6), (1, 5) / 16, (3, 7) / 16
   float f[2], sq[2][NG];                          // per column: what a sum of codes is multiplied by; scaled sums of the query
   float O[MT][4], z[2][NG];                       // sums of p s c (rows r + 8 hold 16 times theirs) and of p m
-  float m[2], l[2], m_lim[2];                     // scores are relative to m; above m_lim it is raised
+  float m[2], base[2], l[2], m_lim[2];            // the maximum (base: 0 instead of -inf) that sums are relative to; above m_lim it is raised
   float v_scale, v_lim;                           // value scales are multiplied by v_scale = 2^-e before p s is rounded
   int r, c;
   int k_at, g_at, v_at[2], step;                   // bytes from a unit's first row: key words, groups, value words of two tokens; eight rows
@@ -64,25 +74,35 @@ struct Int4Consumer {
   static __device__ __forceinline__ int word_at(int k, int c) { return GS == 32 ? k * 4 + c : (k >> 1) * 8 + c * 2 + (k & 1); }
   static __device__ __forceinline__ constexpr int group_of(int k) { return GS == 32 ? k : GS == 64 ? k >> 1 : 0; }
 
-  __device__ __forceinline__ void begin(const Int4DecodeParams& p, int b, int kvh, int head0, int heads) {
+  // the query's words of this lane's column, on their way while the ring is filled
+  __device__ __forceinline__ void ask(const Int4DecodeParams& p, int b, int kvh, int head0, int heads) {
     const int col = DUP ? r & 3 : r;
-    const bool live = col < heads;
-    float qv[NW][8], big = 0.f;
-    const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_bs + (int64_t)(kvh * p.G + head0 + (live ? col : 0)) * p.q_hs;
+    const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_bs + (int64_t)(kvh * p.G + head0 + col) * p.q_hs;
 #pragma unroll
     for (int k = 0; k < NW; ++k) {
-      const T* w = q + word_at(k, c) * 8;
-      __align__(16) T e[8];
-      if (p.q_vec) {
-        *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(w);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = w[i];
+      raw[k] = make_uint4(0, 0, 0, 0);
+      if (col < heads) {
+        const T* w = q + word_at(k, c) * 8;
+        if (p.q_vec) {
+          raw[k] = *reinterpret_cast<const uint4*>(w);
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(w);
+          raw[k] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+        }
       }
+    }
+  }
+  __device__ __forceinline__ void begin(const Int4DecodeParams& p) {
+    float qv[NW][8], big = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        qv[k][i] = live ? to_f32(e[i]) : 0.f;
-        big = fmaxf(big, fabsf(qv[k][i]));
+    for (int k = 0; k < NW; ++k) {
+      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = kv4::scale_min<T>(w[i]);
+        qv[k][2 * i] = x.x;
+        qv[k][2 * i + 1] = x.y;
+        big = fmaxf(big, fmaxf(fabsf(x.x), fabsf(x.y)));
       }
     }
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
@@ -124,7 +144,7 @@ struct Int4Consumer {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       m[j] = m_lim[j] = -INFINITY;
-      l[j] = 0.f;
+      l[j] = base[j] = 0.f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) z[j][g] = 0.f;
     }
@@ -133,15 +153,17 @@ struct Int4Consumer {
   }
 
   // a score above what the sums are scaled for, or a value scale: raise either
-  __device__ __forceinline__ void raise(const float (&v)[2][2], float vs) {
+  __device__ __forceinline__ void raise(const float (&v)[U][2][2], float vs) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float mx = fmaxf(v[0][j], v[1][j]);
+      float mx = v[0][0][j];
+#pragma unroll
+      for (int x = 1; x < 2 * U; ++x) mx = fmaxf(mx, v[x >> 1][x & 1][j]);
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       if (mx > m[j]) {
         const float a = fast_exp2(m[j] - mx);     // m[j] = -inf at first: 0
-        m[j] = mx;
+        m[j] = base[j] = mx;
         l[j] *= a;
 #pragma unroll
         for (int g = 0; g < NG; ++g) z[j][g] *= a;
@@ -174,132 +196,154 @@ struct Int4Consumer {
     v_at[1] = place(2 * c + 1) * pitch + D / 2 + (GS == 32 ? r >> 1 : r) * 4;
   }
 
-  // 16 tokens at `at` (the head's bytes of the first), of which `valid` count (one form for all: a copy without the mask costs more in
-  // the instruction cache than the mask)
-  __device__ __forceinline__ void unit(const uint8_t* at, int valid) {
+  // 16 U tokens at `at` (the head's bytes of the first), of which `valid` count
+  __device__ __forceinline__ void tile(const uint8_t* at, int valid) {
     constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-    // ---- scores of 16 tokens (rows) and 8 heads (columns) ----
-    uint32_t w0[NW], w1[NW];
+    // ---- scores: 16 tokens (rows) and 8 heads (columns) to a unit ----
+    float acc[U][NG][4];
+    uint32_t vg[U][2][NG];                        // the values' groups
+    float v[U][2][2];
 #pragma unroll
-    for (int k = 0; k < NW; ++k) {
-      if (GS == 32) {
-        w0[k] = *reinterpret_cast<const uint32_t*>(at + k_at + k * 16);
-        w1[k] = *reinterpret_cast<const uint32_t*>(at + k_at + step + k * 16);
-      } else if ((k & 1) == 0) {
-        const uint2 x = *reinterpret_cast<const uint2*>(at + k_at + k * 16), y = *reinterpret_cast<const uint2*>(at + k_at + step + k * 16);
-        w0[k] = x.x; w0[k + 1] = x.y;
-        w1[k] = y.x; w1[k + 1] = y.y;
-      }
-    }
-    float acc[NG][4];
+    for (int n = 0; n < U; ++n) {
+      const uint8_t* u = at + 2 * n * step;
+      uint32_t w0[NW], w1[NW];
 #pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[g][i] = 0.f;
-#pragma unroll
-    for (int k = 0; k < NW; ++k) {
-      const uint32_t x0 = w0[k] >> 8, x1 = w1[k] >> 8;
-      const uint32_t lo[4] = {w0[k] & kLow, w1[k] & kLow, x0 & kLow, x1 & kLow};
-      const uint32_t hi[4] = {w0[k] & kHigh, w1[k] & kHigh, x0 & kHigh, x1 & kHigh};
-      mma_m16n8k16<__half>(acc[group_of(k)], lo, qb[k][0], qb[k][1]);
-      mma_m16n8k16<__half>(acc[group_of(k)], hi, qb[k][2], qb[k][3]);
-    }
-    float2 ks[2][NG], vs[2][NG];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t g[2 * NG];                         // of K, then of V
-#pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        const uint2 y = *reinterpret_cast<const uint2*>(at + g_at + i * step + x * 8);
-        g[2 * x] = y.x;
-        g[2 * x + 1] = y.y;
-      }
-#pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        ks[i][x] = kv4::scale_min<T>(g[x]);
-        vs[i][x] = kv4::scale_min<T>(g[NG + x]);
-      }
-    }
-    float v[2][2], top = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool in = place(r) + 8 * i < valid;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float t = ks[i][0].x * acc[0][2 * i + j], u = ks[i][0].y * sq[j][0];
-#pragma unroll
-        for (int g = 1; g < NG; ++g) {
-          t = fmaf(ks[i][g].x, acc[g][2 * i + j], t);
-          u = fmaf(ks[i][g].y, sq[j][g], u);
+      for (int k = 0; k < NW; ++k) {
+        if (GS == 32) {
+          w0[k] = *reinterpret_cast<const uint32_t*>(u + k_at + k * 16);
+          w1[k] = *reinterpret_cast<const uint32_t*>(u + k_at + step + k * 16);
+        } else if ((k & 1) == 0) {
+          const uint2 x = *reinterpret_cast<const uint2*>(u + k_at + k * 16), y = *reinterpret_cast<const uint2*>(u + k_at + step + k * 16);
+          w0[k] = x.x; w0[k + 1] = x.y;
+          w1[k] = y.x; w1[k + 1] = y.y;
         }
-        v[i][j] = in ? fmaf(t, f[j], u) : -INFINITY;
       }
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        if (!in) vs[i][g] = make_float2(0.f, 0.f);
-        top = fmaxf(top, vs[i][g].x);
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][g][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        const uint32_t x0 = w0[k] >> 8, x1 = w1[k] >> 8;
+        const uint32_t lo[4] = {w0[k] & kLow, w1[k] & kLow, x0 & kLow, x1 & kLow};
+        const uint32_t hi[4] = {w0[k] & kHigh, w1[k] & kHigh, x0 & kHigh, x1 & kHigh};
+        mma(acc[n][group_of(k)], lo, qb[k][0], qb[k][1]);
+        mma(acc[n][group_of(k)], hi, qb[k][2], qb[k][3]);
       }
     }
-    const bool over = fmaxf(v[0][0], v[1][0]) > m_lim[0] || fmaxf(v[0][1], v[1][1]) > m_lim[1] || top > v_lim;
-    if (__any_sync(0xffffffffu, over)) raise(v, top);
-    // ---- probabilities, times the values' scales, as the second product's columns ----
-    float pr[2][2];
+    float top = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float base = m[j] == -INFINITY ? 0.f : m[j];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) pr[i][j] = fast_exp2(v[i][j] - base);
-      l[j] += pr[0][j] + pr[1][j];
-    }
-    uint32_t pb[NG][2], rest[NG][2];
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
+    for (int n = 0; n < U; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        uint32_t word[2 * NG];                    // groups of K, then of V
 #pragma unroll
-        for (int j = 0; j < 2; ++j) z[j][g] = fmaf(pr[i][j], vs[i][g].y, z[j][g]);
-        const float s = vs[i][g].x * v_scale, x = pr[i][0] * s, y = pr[i][1] * s;
-        const uint32_t near = pack2<__half>(x, y);
-        const float2 back = halves(near);
-        const uint32_t left = pack2<__half>(x - back.x, y - back.y);
-        if (DUP) {
-          pb[g][i] = trans8x8(c < 2 ? near : left);
-        } else {
-          pb[g][i] = trans8x8(near);
-          rest[g][i] = trans8x8(left);
+        for (int x = 0; x < NG; ++x) {
+          const uint2 y = *reinterpret_cast<const uint2*>(at + g_at + (2 * n + i) * step + x * 8);
+          word[2 * x] = y.x;
+          word[2 * x + 1] = y.y;
+        }
+        float2 ks[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          ks[g] = kv4::scale_min<T>(word[g]);
+          vg[n][i][g] = word[NG + g];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float t = ks[0].x * acc[n][0][2 * i + j], u = ks[0].y * sq[j][0];
+#pragma unroll
+          for (int g = 1; g < NG; ++g) {
+            t = fmaf(ks[g].x, acc[n][g][2 * i + j], t);
+            u = fmaf(ks[g].y, sq[j][g], u);
+          }
+          v[n][i][j] = fmaf(t, f[j], u);
         }
       }
-    // ---- values: rows are elements, columns heads, the products run over tokens ----
-    auto add = [&](int tile, int g, const uint32_t (&a)[4]) {
-      mma_m16n8k16<__half>(O[tile], a, pb[g][0], pb[g][1]);
-      if (!DUP) mma_m16n8k16<__half>(O[tile], a, rest[g][0], rest[g][1]);
-    };
-    if (GS == 32) {
-      const uint32_t pick = (r & 1) ? 0x7632u : 0x5410u;
+    if (valid < 16 * U) {                         // a row's last tokens
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        auto word = [&](int o) { return *reinterpret_cast<const uint32_t*>(at + o + g * 16); };
-        const uint32_t x = __byte_perm(word(v_at[0]), word(v_at[1]), pick), y = __byte_perm(word(v_at[0] + step), word(v_at[1] + step), pick);
-        const uint32_t a0[4] = {x & kLow, x & kHigh, y & kLow, y & kHigh};
-        const uint32_t x8 = x >> 8, y8 = y >> 8;
-        const uint32_t a1[4] = {x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh};
-        add(g * 2, g, a0);
-        add(g * 2 + 1, g, a1);
+      for (int n = 0; n < U; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (place(r) + 16 * n + 8 * i >= valid) {
+            v[n][i][0] = v[n][i][1] = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) vg[n][i][g] = 0u;
+          }
+    }
+    bool over = false;
+#pragma unroll
+    for (int n = 0; n < U; ++n) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) over |= fmaxf(v[n][0][j], v[n][1][j]) > m_lim[j];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) top = fmaxf(top, kv4::scale_min<T>(vg[n][i][g]).x);
+    }
+    if (__any_sync(0xffffffffu, over || top > v_lim)) raise(v, top);
+#pragma unroll
+    for (int n = 0; n < U; ++n) {
+      // ---- probabilities, times the values' scales, as the second product's columns ----
+      float pr[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) pr[i][j] = fast_exp2(v[n][i][j] - base[j]);
+        l[j] += pr[0][j] + pr[1][j];
       }
-    } else {
+      uint32_t pb[NG][2], rest[NG][2];
 #pragma unroll
-      for (int b = 0; b < D / 64; ++b) {
-        const int g = b * 64 / GS;
-        auto word = [&](int o) { return *reinterpret_cast<const uint32_t*>(at + o + b * 32); };
-        const uint32_t e0 = word(v_at[0]), e1 = word(v_at[1]), e2 = word(v_at[0] + step), e3 = word(v_at[1] + step);
+      for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t x = __byte_perm(e0, e1, h ? 0x7632 : 0x5410), y = __byte_perm(e2, e3, h ? 0x7632 : 0x5410);
+        for (int i = 0; i < 2; ++i) {
+          const float2 vs = kv4::scale_min<T>(vg[n][i][g]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) z[j][g] = fmaf(pr[i][j], vs.y, z[j][g]);
+          const float s = vs.x * v_scale, x = pr[i][0] * s, y = pr[i][1] * s;
+          const uint32_t near = pack2<__half>(x, y);
+          const float2 back = halves(near);
+          const uint32_t left = pack2<__half>(x - back.x, y - back.y);
+          if (DUP) {
+            pb[g][i] = trans8x8(c < 2 ? near : left);
+          } else {
+            pb[g][i] = trans8x8(near);
+            rest[g][i] = trans8x8(left);
+          }
+        }
+      // ---- values: rows are elements, columns heads, the products run over tokens ----
+      const uint8_t* u = at + 2 * n * step;
+      auto add = [&](int tile, int g, const uint32_t (&a)[4]) {
+        mma(O[tile], a, pb[g][0], pb[g][1]);
+        if (!DUP) mma(O[tile], a, rest[g][0], rest[g][1]);
+      };
+      if (GS == 32) {
+        const uint32_t pick = (r & 1) ? 0x7632u : 0x5410u;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          auto word = [&](int o) { return *reinterpret_cast<const uint32_t*>(u + o + g * 16); };
+          const uint32_t x = __byte_perm(word(v_at[0]), word(v_at[1]), pick), y = __byte_perm(word(v_at[0] + step), word(v_at[1] + step), pick);
           const uint32_t a0[4] = {x & kLow, x & kHigh, y & kLow, y & kHigh};
           const uint32_t x8 = x >> 8, y8 = y >> 8;
           const uint32_t a1[4] = {x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh};
-          add(b * 4 + h * 2, g, a0);
-          add(b * 4 + h * 2 + 1, g, a1);
+          add(g * 2, g, a0);
+          add(g * 2 + 1, g, a1);
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < D / 64; ++b) {
+          const int g = b * 64 / GS;
+          auto word = [&](int o) { return *reinterpret_cast<const uint32_t*>(u + o + b * 32); };
+          const uint32_t e0 = word(v_at[0]), e1 = word(v_at[1]), e2 = word(v_at[0] + step), e3 = word(v_at[1] + step);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t x = __byte_perm(e0, e1, h ? 0x7632 : 0x5410), y = __byte_perm(e2, e3, h ? 0x7632 : 0x5410);
+            const uint32_t a0[4] = {x & kLow, x & kHigh, y & kLow, y & kHigh};
+            const uint32_t x8 = x >> 8, y8 = y >> 8;
+            const uint32_t a1[4] = {x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh};
+            add(b * 4 + h * 2, g, a0);
+            add(b * 4 + h * 2 + 1, g, a1);
+          }
         }
       }
     }
@@ -335,9 +379,32 @@ struct Int4Consumer {
   }
 };
 
-struct Segment { int b, first, last, tiles; };    // tiles [first, last) of a row of `tiles`
+struct Segment { int b, blk, first, last, tiles; };   // tiles [first, last) of a row of `tiles`
 
-template <typename T, int D, int GS, bool DUP>
+// 16 bytes to shared memory
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// the barrier's arrival of this thread, once its copies so far are done
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_peer(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// CLUSTER: a row and block of heads to a cluster of kCluster CTAs, whose parts meet in shared memory; else equal shares of all tiles.
+template <typename T, int D, int GS, bool DUP, bool CLUSTER>
 __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const Int4DecodeParams p) {
   pdl_prologue();   // everything below reads what earlier kernels of the step wrote
   extern __shared__ __align__(128) uint8_t smem[];
@@ -345,7 +412,8 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem);
   uint64_t* empty_bar = full_bar + kMaxStages;
   uint8_t* ring = smem + 128;
-  const int unit_bytes = kUnit * p.pitch, stage_bytes = p.TS * unit_bytes, tile = p.TS * kUnit;
+  constexpr int kWarpTokens = kUnit * units_of(D, GS);
+  const int warp_bytes = kWarpTokens * p.pitch, stage_bytes = p.TS * warp_bytes, tile = p.TS * kWarpTokens;
   float* join = reinterpret_cast<float*>(ring + p.stages * stage_bytes);      // sums of the warps that share a head
   const int per_head = p.qblocks * 8 * (D + 2);
   int* prefix = reinterpret_cast<int*>(join + (p.TS - 1) * p.HB * per_head);  // tiles of the rows before, [batch + 1]
@@ -353,59 +421,79 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
   int* reqs = lens + p.batch;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nwarps = p.HB * p.qblocks * p.TS;
-  const int nblk = p.Hkv / p.HB;
-
-  // ---- tiles of the rows before each; a thread owns neighbouring rows ----
-  const int per = (p.batch + blockDim.x - 1) / blockDim.x, r_lo = threadIdx.x * per;
-  const int r_hi = r_lo + per < p.batch ? r_lo + per : p.batch;
-  int own = 0;
-  for (int r = r_lo; r < r_hi; ++r) {
+  auto length = [&](int r, int& req) {
     const int64_t n = load_index(p.seq_len, r, p.len_w), q = load_index(p.req_idx, r, p.req_w);
-    reqs[r] = (int)q;
-    lens[r] = q < 0 || q >= p.requests || n <= 0 ? 0 : n > p.most ? (int)p.most : (int)n;
-    own += (lens[r] + tile - 1) / tile;
-  }
-  int upto = own;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
-  }
-  if (lane == 31) warp_sum[warp] = upto;
+    req = (int)q;
+    return q < 0 || q >= p.requests || n <= 0 ? 0 : n > p.most ? (int)p.most : (int)n;
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full_bar[s], 1);
+      mbar_init(&full_bar[s], p.bulk ? nwarps : nwarps * 32);
       mbar_init(&empty_bar[s], nwarps);
     }
     mbar_fence_init();
   }
-  __syncthreads();
-  int at = upto - own, all = 0;
-  for (int w = 0; w < nwarps; ++w) {
-    if (w < warp) at += warp_sum[w];
-    all += warp_sum[w];
-  }
-  for (int r = r_lo; r < r_hi; ++r) {
-    prefix[r] = at;
-    at += (lens[r] + tile - 1) / tile;
-  }
-  if (threadIdx.x == 0) prefix[p.batch] = all;
-  __syncthreads();
 
-  // ---- this CTA's share of all tiles, heads' blocks one after the other ----
-  const int64_t total = (int64_t)all * nblk;
-  const int least = (kMinTokens + tile - 1) / tile;
-  const int64_t worth = (total + least - 1) / least;
-  const int64_t shares = worth < gridDim.x ? worth : gridDim.x;
-  if (blockIdx.x >= shares) return;
-  int64_t item = blockIdx.x * total / shares;
-  const int64_t item_end = (blockIdx.x + 1) * total / shares;
-  // the part of a row at `item`, and the block of heads it is in
-  auto next = [&](int64_t& item, Segment& s, int& blk) -> bool {
+  Segment seg;
+  int all = 0, item = 0, item_end = 0, len0 = 0, req0 = 0;
+  if (CLUSTER) {
+    const int id = blockIdx.x / kCluster, rank = blockIdx.x - id * kCluster;
+    seg.blk = id / p.batch;
+    seg.b = id - seg.blk * p.batch;
+    len0 = length(seg.b, req0);
+    seg.tiles = (len0 + tile - 1) / tile;
+    seg.first = seg.tiles * rank / kCluster;
+    seg.last = seg.tiles * (rank + 1) / kCluster;
+    item_end = seg.first < seg.last;
+    __syncthreads();
+  } else {
+    // ---- tiles of the rows before each; a thread owns neighbouring rows ----
+    const int per = (p.batch + blockDim.x - 1) / blockDim.x, r_lo = threadIdx.x * per;
+    const int r_hi = r_lo + per < p.batch ? r_lo + per : p.batch;
+    int own = 0;
+#pragma unroll 1
+    for (int r = r_lo; r < r_hi; ++r) {
+      lens[r] = length(r, reqs[r]);
+      own += (lens[r] + tile - 1) / tile;
+    }
+    int upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    int at = upto - own;
+    const int of_warp = lane < nwarps ? warp_sum[lane] : 0;
+    all = __reduce_add_sync(0xffffffffu, of_warp);
+    at += __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0);
+#pragma unroll 1
+    for (int r = r_lo; r < r_hi; ++r) {
+      prefix[r] = at;
+      at += (lens[r] + tile - 1) / tile;
+    }
+    if (threadIdx.x == 0) prefix[p.batch] = all;
+    __syncthreads();
+    // ---- this CTA's share of all tiles, heads' blocks one after the other ----
+    const int total = all * (p.Hkv / p.HB), least = (kMinTokens + tile - 1) / tile, worth = (total + least - 1) / least;
+    const int shares = worth < (int)gridDim.x ? worth : (int)gridDim.x;
+    if ((int)blockIdx.x >= shares) return;
+    item = (int)((int64_t)blockIdx.x * total / shares);
+    item_end = (int)((int64_t)(blockIdx.x + 1) * total / shares);
+  }
+  // the part of a row at `item`
+  auto next = [&](int& item, Segment& s) -> bool {
     if (item >= item_end) return false;
-    blk = (int)((uint32_t)item / (uint32_t)all);
-    const int x = (int)item - blk * all;
+    if (CLUSTER) {
+      s = seg;
+      item = item_end;
+      return true;
+    }
+    s.blk = item / all;
+    const int x = item - s.blk * all;
     int lo = 0, n = p.batch;                      // the last row that begins at or before x and has tiles
+#pragma unroll 1
     while (n > 1) {
       const int half = n / 2;
       if (prefix[lo + half] <= x) { lo += half; n -= half; }
@@ -414,157 +502,214 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     s.b = lo;
     s.first = x - prefix[lo];
     s.tiles = prefix[lo + 1] - prefix[lo];
-    const int64_t left = item_end - item;
-    s.last = left < s.tiles - s.first ? s.first + (int)left : s.tiles;
+    const int left = item_end - item;
+    s.last = left < s.tiles - s.first ? s.first + left : s.tiles;
     item += s.last - s.first;
     return true;
   };
 
-  // ---- the ring's copies: tile f of the share is brought by warp f % nwarps.  It reads the table kAhead tiles before its stage is due and
-  // waits for that stage when the tile before this one has been worked on. ----
-  const int hb = kv4::head_bytes(D, GS);
-  struct Fill { int row[kMaxConsumers / 2]; int here, f, from; } fill;
-  Segment ahead;                                  // of the tile whose entries are read next
-  int ahead_blk, ahead_t = 0, ahead_f = 0;
-  int64_t ahead_item = item;
-  bool more = next(ahead_item, ahead, ahead_blk);
-  if (more) ahead_t = ahead.first;
-  fill.f = -1;
-  auto look = [&] {
+  // ---- the ring's copies: each warp brings its part of a tile's token rows, whose table entries are read a tile ahead.  One bulk copy to
+  // a row costs the warp least, but the engine ~40 cycles: 32 rows 1400, which a cluster's few tiles wait for, and rows of 160 bytes
+  // limited the whole kernel (150 sequences of 200 - 400 tokens, 2 kv heads of 64: 20.5 us, this 18.0).  Else 16 bytes a lane (32 of
+  // 1000 - 2000, 8 kv heads of 128: 34 us, bulk 31). ----
+  const int hb = kv4::head_bytes(D, GS), mine = (tile + nwarps - 1) / nwarps;   // token rows of this warp, at most 32
+  Segment ahead;                                  // of the tile that is brought next
+  int ahead_item = item, ahead_t = 0, row = 0, ahead_here = 0;
+  bool more = next(ahead_item, ahead);
+  auto entries = [&] {
+    const int len = CLUSTER ? len0 : lens[ahead.b], req = CLUSTER ? req0 : reqs[ahead.b];
+    const int left = len - ahead_t * tile, i = warp * mine + lane;
+    ahead_here = left < tile ? left : tile;
+    if (lane < mine && i < ahead_here)
+      row = ld_upstream(p.table + (int64_t)req * p.tab_rs + (int64_t)(ahead_t * tile + i) * p.tab_cs);
+  };
+  if (more) { ahead_t = ahead.first; entries(); }
+  auto bring = [&](int s) {
     if (!more) return;
-    if (ahead_f % nwarps == warp) {
-      const int len = lens[ahead.b];
-      const int32_t* entry = p.table + (int64_t)reqs[ahead.b] * p.tab_rs;
-      fill.f = ahead_f;
-      fill.here = len - ahead_t * tile < tile ? len - ahead_t * tile : tile;
-      fill.from = ahead_blk * p.HB * hb;
-#pragma unroll
-      for (int k = 0; k < kMaxConsumers / 2; ++k) {
-        const int i = k * 32 + lane;
-        if (i < fill.here) fill.row[k] = ld_upstream(entry + (int64_t)(ahead_t * tile + i) * p.tab_cs);
+    const int from = ahead.blk * p.HB * hb, shift = from & 15, pieces = (shift + p.HB * hb + 15) >> 4;
+    const int first = warp * mine, mine_here = ahead_here - first < mine ? ahead_here - first : mine;
+    const uint8_t* src = p.cache + (from - shift);
+    uint8_t* dst = ring + s * stage_bytes + first * p.pitch;
+    const int at = row < 0 || row >= p.max_tokens ? 0 : row;
+    if (p.bulk) {
+      if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], (uint32_t)((mine_here > 0 ? mine_here : 0) * pieces * 16));
+      __syncwarp();
+      if (lane < mine_here) bulk_g2s(dst + lane * p.pitch, src + (int64_t)at * p.row_stride, (uint32_t)pieces * 16u, &full_bar[s]);
+    } else if (pieces >= 32) {                           // a row at a time
+#pragma unroll 1
+      for (int i = 0; i < mine_here; ++i) {
+        const uint8_t* x = src + (int64_t)__shfl_sync(0xffffffffu, at, i) * p.row_stride;
+        uint8_t* y = dst + i * p.pitch;
+        for (int c = lane; c < pieces; c += 32) copy16(y + c * 16, x + c * 16);
+      }
+    } else {                                      // several rows at a time
+      const int rows = 32 / pieces, i0 = lane / pieces, c = lane - i0 * pieces;
+#pragma unroll 1
+      for (int i = 0; i < mine_here; i += rows) {
+        const int64_t r = __shfl_sync(0xffffffffu, at, (i + i0) & 31);
+        if (i0 < rows && i + i0 < mine_here) copy16(dst + (i + i0) * p.pitch + c * 16, src + r * p.row_stride + c * 16);
       }
     }
-    ++ahead_f;
+    if (!p.bulk) copies_arrive(&full_bar[s]);
     if (++ahead_t == ahead.last) {
-      more = next(ahead_item, ahead, ahead_blk);
+      more = next(ahead_item, ahead);
       if (more) ahead_t = ahead.first;
     }
+    if (more) entries();
   };
-  auto bring = [&](int f, int s, uint32_t empty_parity, bool wait) {
-    if (fill.f != f) return;
-    const int shift = fill.from & 15;
-    const uint32_t bytes = (uint32_t)((shift + p.HB * hb + 15) & ~15);
-    const uint8_t* src = p.cache + (fill.from - shift);
-    if (wait) mbar_wait(&empty_bar[s], empty_parity);
-    if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], (uint32_t)fill.here * bytes);
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < kMaxConsumers / 2; ++k) {
-      const int i = k * 32 + lane;
-      if (i < fill.here) {
-        const int64_t row = fill.row[k] < 0 || fill.row[k] >= p.max_tokens ? 0 : fill.row[k];
-        bulk_g2s(ring + s * stage_bytes + i * p.pitch, src + row * p.row_stride, bytes, &full_bar[s]);
-      }
-    }
-    fill.f = -1;
-  };
-  for (int f = 0; f < p.stages; ++f) {
-    look();
-    bring(f, f, 0, false);
-  }
-  for (int k = 0; k < kAhead; ++k) look();
 
-  Segment seg;
-  int blk, s = 0, at_tile = 0;
-  uint32_t phase = 0;
   // ===================== a warp: (kv head, block of query heads, unit of the tile) =====================
   const int ts = warp / (p.HB * p.qblocks), wh = warp - ts * p.HB * p.qblocks;
   const int hl = wh / p.qblocks, qblk = wh - hl * p.qblocks;
   const int head0 = qblk * 8, heads = p.G - head0 < 8 ? p.G - head0 : 8;
   Int4Consumer<T, D, GS, DUP> c(lane, p.pitch);
-  while (next(item, seg, blk)) {
-    const int len = lens[seg.b], kvh = blk * p.HB + hl;
-    const int off = ((blk * p.HB * hb) & 15) + hl * hb + ts * unit_bytes;
-    c.begin(p, seg.b, kvh, head0, heads);
+  // columns of this lane: heads 2c and 2c + 1 (DUP: the upper half of the columns repeats the lower)
+  const bool counts = !DUP || c.c < 2;
+  int s = 0, at_tile = 0;
+  uint32_t phase = 0;
+  bool got = next(item, seg);
+  if (got) c.ask(p, seg.b, seg.blk * p.HB + hl, head0, heads);
+  for (int f = 0; f < p.stages; ++f) bring(f);
+  while (got) {
+    const int len = CLUSTER ? len0 : lens[seg.b], kvh = seg.blk * p.HB + hl;
+    const int off = ((seg.blk * p.HB * hb) & 15) + hl * hb + ts * warp_bytes;
+    c.begin(p);
 #pragma unroll 1
     for (int t = seg.first; t < seg.last; ++t, ++at_tile) {
-      if (at_tile > 0) {                          // into the stage of the tile before this one
-        const int b = s == 0 ? p.stages - 1 : s - 1;
-        bring(at_tile - 1 + p.stages, b, s == 0 ? phase ^ 1u : phase, true);
-        look();
-      }
       mbar_wait(&full_bar[s], phase);
-      const int valid = len - t * tile - ts * kUnit;
-      if (valid > 0) c.unit(ring + s * stage_bytes + off, valid);
+      const int valid = len - t * tile - ts * kWarpTokens;
+      if (valid > 0) c.tile(ring + s * stage_bytes + off, valid);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[s]);
+      if (at_tile > 0 && more) {                  // into the stage of the tile before this one, which the others have left by now
+        const int b = s == 0 ? p.stages - 1 : s - 1;
+        mbar_wait(&empty_bar[b], s == 0 ? phase ^ 1u : phase);
+        bring(b);
+      }
       if (++s == p.stages) { s = 0; phase ^= 1; }
     }
+    const Segment done = seg;
+    got = next(item, seg);
     c.finish();
-    // columns of this lane: heads 2c and 2c + 1 (DUP: the upper half of the columns repeats the lower)
-    const bool mine = !DUP || c.c < 2;
     if (p.TS > 1) {
       auto bar = [&] { asm volatile("bar.sync 1, %0;" ::"r"(nwarps * 32) : "memory"); };
       bar();                                      // the sums before these have been read
-      float* mineat = join + ((ts - 1) * p.HB * p.qblocks + wh) * 8 * (D + 2);
-      if (ts > 0 && mine) {
+      float* to_join = join + ((ts - 1) * p.HB * p.qblocks + wh) * 8 * (D + 2);
+      if (ts > 0 && counts) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float* to = mineat + (2 * c.c + j) * (D + 2);
+          float* to = to_join + (2 * c.c + j) * (D + 2);
 #pragma unroll
           for (int t = 0; t < D / 16; ++t) *reinterpret_cast<float2*>(to + c.element(t)) = make_float2(c.O[t][j], c.O[t][2 + j]);
           if (c.r == 0) *reinterpret_cast<float2*>(to + D) = make_float2(c.m[j], c.l[j]);
         }
       }
       bar();
-      if (ts > 0) continue;
-      for (int o = 1; o < p.TS; ++o) {
-        const float* from = join + ((o - 1) * p.HB * p.qblocks + wh) * 8 * (D + 2);
+      if (ts == 0 && counts) {
+#pragma unroll 1
+        for (int o = 1; o < p.TS; ++o) {
+          const float* from = join + ((o - 1) * p.HB * p.qblocks + wh) * 8 * (D + 2);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if (!mine) continue;
-          const float* x = from + (2 * c.c + j) * (D + 2);
-          const float2 ml = *reinterpret_cast<const float2*>(x + D);
-          const float mm = fmaxf(c.m[j], ml.x), base = mm == -INFINITY ? 0.f : mm;
-          const float a = fast_exp2(c.m[j] - base), e = fast_exp2(ml.x - base);
-          c.m[j] = mm;
-          c.l[j] = c.l[j] * a + ml.y * e;
+          for (int j = 0; j < 2; ++j) {
+            const float* x = from + (2 * c.c + j) * (D + 2);
+            const float2 ml = *reinterpret_cast<const float2*>(x + D);
+            const float mm = fmaxf(c.m[j], ml.x), base = mm == -INFINITY ? 0.f : mm;
+            const float a = fast_exp2(c.m[j] - base), e = fast_exp2(ml.x - base);
+            c.m[j] = mm;
+            c.l[j] = c.l[j] * a + ml.y * e;
 #pragma unroll
-          for (int t = 0; t < D / 16; ++t) {
-            const float2 y = *reinterpret_cast<const float2*>(x + c.element(t));
-            c.O[t][j] = c.O[t][j] * a + y.x * e;
-            c.O[t][2 + j] = c.O[t][2 + j] * a + y.y * e;
+            for (int t = 0; t < D / 16; ++t) {
+              const float2 y = *reinterpret_cast<const float2*>(x + c.element(t));
+              c.O[t][j] = c.O[t][j] * a + y.x * e;
+              c.O[t][2 + j] = c.O[t][2 + j] * a + y.y * e;
+            }
           }
         }
       }
     }
-    const bool whole = seg.first == 0 && seg.last == seg.tiles;
+    if (got) c.ask(p, seg.b, seg.blk * p.HB + hl, head0, heads);
+    if (CLUSTER) break;
+    const bool whole = done.first == 0 && done.last == done.tiles;
+    if (ts == 0 && counts) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int head = head0 + 2 * c.c + j;
-      if (!mine || 2 * c.c + j >= heads) continue;
-      if (whole) {
-        const float inv = 1.f / c.l[j];
-        T* to = reinterpret_cast<T*>(p.out) + (int64_t)seg.b * p.o_bs + (int64_t)(kvh * p.G + head) * p.o_hs;
+      for (int j = 0; j < 2; ++j) {
+        const int head = head0 + 2 * c.c + j;
+        if (2 * c.c + j >= heads) continue;
+        if (whole) {
+          const float inv = 1.f / c.l[j];
+          T* to = reinterpret_cast<T*>(p.out) + (int64_t)done.b * p.o_bs + (int64_t)(kvh * p.G + head) * p.o_hs;
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) {
-          to[c.element(t)] = from_f32<T>(c.O[t][j] * inv);
-          to[c.element(t) + 1] = from_f32<T>(c.O[t][2 + j] * inv);
+          for (int t = 0; t < D / 16; ++t) {
+            to[c.element(t)] = from_f32<T>(c.O[t][j] * inv);
+            to[c.element(t) + 1] = from_f32<T>(c.O[t][2 + j] * inv);
+          }
+        } else {
+          const int64_t part = ((int64_t)blockIdx.x * 2 + (done.first == 0 ? 1 : 0)) * p.HB * p.G + hl * p.G + head;
+#pragma unroll
+          for (int t = 0; t < D / 16; ++t)
+            *reinterpret_cast<float2*>(p.ws_o + part * D + c.element(t)) = make_float2(c.O[t][j], c.O[t][2 + j]);
+          if (c.r == 0) *reinterpret_cast<float2*>(p.ws_ml + part * 2) = make_float2(c.m[j], c.l[j]);
         }
-      } else {
-        const int64_t part = ((int64_t)blockIdx.x * 2 + (seg.first == 0 ? 1 : 0)) * p.HB * p.G + hl * p.G + head;
-#pragma unroll
-        for (int t = 0; t < D / 16; ++t)
-          *reinterpret_cast<float2*>(p.ws_o + part * D + c.element(t)) = make_float2(c.O[t][j], c.O[t][2 + j]);
-        if (c.r == 0) *reinterpret_cast<float2*>(p.ws_ml + part * 2) = make_float2(c.m[j], c.l[j]);
+      }
+      if (wh == 0 && lane == 0) {
+        int* note = reinterpret_cast<int*>(p.ws_info + (int64_t)done.blk * p.batch + done.b);
+        if (done.first == 0) note[0] = blockIdx.x;
+        if (done.last == done.tiles) note[1] = blockIdx.x;
       }
     }
-    if (wh == 0 && lane == 0) {
-      int* note = reinterpret_cast<int*>(p.ws_info + (int64_t)blk * p.batch + seg.b);
-      if (seg.first == 0) note[0] = blockIdx.x;
-      if (seg.last == seg.tiles) note[1] = blockIdx.x;
-    }
   }
+  if (!CLUSTER) return;
+
+  // ---- the cluster's parts, in the memory of the rings: [heads][D + 2] with the largest score and the sum; each CTA adds up its heads ----
+  __syncthreads();                                // the ring has been read
+  float* part = reinterpret_cast<float*>(ring);
+  const int block_heads = p.HB * p.G, rank = blockIdx.x % kCluster;
+  if (seg.first < seg.last) {
+    if (ts == 0 && counts) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (2 * c.c + j >= heads) continue;
+        float* to = part + (hl * p.G + head0 + 2 * c.c + j) * (D + 2);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) *reinterpret_cast<float2*>(to + c.element(t)) = make_float2(c.O[t][j], c.O[t][2 + j]);
+        if (c.r == 0) *reinterpret_cast<float2*>(to + D) = make_float2(c.m[j], c.l[j]);
+      }
+    }
+  } else {
+    for (int h = threadIdx.x; h < block_heads; h += blockDim.x) *reinterpret_cast<float2*>(part + h * (D + 2) + D) = make_float2(-INFINITY, 0.f);
+  }
+  __syncwarp();
+  cluster_sync_all();
+  constexpr int E = D / 32;
+  for (int h = warp * kCluster + rank; h < block_heads; h += nwarps * kCluster) {
+    float m[kCluster], l[kCluster], x[kCluster][E], M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kCluster; ++k) {
+      const uint32_t peer = peer_smem(smem_u32(part + h * (D + 2)), k);
+      m[k] = ld_peer(peer + D * 4);
+      l[k] = ld_peer(peer + D * 4 + 4);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[k][e] = ld_peer(peer + (e * 32 + lane) * 4);
+      M = fmaxf(M, m[k]);
+    }
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kCluster; ++k) {
+      if (l[k] == 0.f && m[k] == -INFINITY) continue;   // a part without tokens: nothing was stored
+      const float w = fast_exp2(m[k] - base);
+      L = fmaf(l[k], w, L);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(x[k][e], w, o[e]);
+    }
+    T* to = reinterpret_cast<T*>(p.out) + (int64_t)seg.b * p.o_bs + (int64_t)(seg.blk * block_heads + h) * p.o_hs;
+#pragma unroll
+    for (int e = 0; e < E; ++e) to[e * 32 + lane] = from_f32<T>(len0 == 0 ? 0.f : o[e] / L);
+  }
+  __syncwarp();
+  cluster_sync_all();                             // the peers have read this CTA's part
 }
 
 // The rows that several CTAs met in, and zeros for the empty ones.  Bound by latency: a block takes one head of a row, its warps the
@@ -651,8 +796,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_decode_merge_kernel(cons
 }
 
 constexpr int kMaxBatch = 4096;                   // rows of one launch (their lengths lie in shared memory)
+constexpr int kClusterMost = 1024;                // tokens of a row that a cluster takes
 
-struct Int4Plan { int HB, qblocks, TS, pitch, stages, smem, grid; };
+struct Int4Plan { int HB, qblocks, TS, pitch, stages, smem, grid; bool cluster; };
 
 // A function of sizes that the host knows, hence the same inside and outside a captured graph.
 Int4Plan make_plan(int64_t batch, int G, int Hkv, int D, int group, int64_t max_len) {
@@ -661,30 +807,57 @@ Int4Plan make_plan(int64_t batch, int G, int Hkv, int D, int group, int64_t max_
   pl.HB = 1;
   for (int h = 1; h * pl.qblocks <= kMaxConsumers; ++h)
     if (Hkv % h == 0) pl.HB = h;
+  const int units = units_of(D, group);
   pl.TS = kMaxConsumers / (pl.HB * pl.qblocks);
+  if (pl.TS > 8 / units) pl.TS = 8 / units;       // 128 tokens to a tile at most
   const int hb = kv4::head_bytes(D, group);
   const int bytes = ((pl.HB * hb + (pl.HB == Hkv ? 0 : 8)) + 15) / 16 * 16;
   pl.pitch = (bytes + 95) / 128 * 128 + 32;       // 32 bytes past a multiple of 128
-  const int stage = pl.TS * kUnit * pl.pitch;
+  const int stage = pl.TS * units * kUnit * pl.pitch;
   const int rows = (int)(batch < kMaxBatch ? batch : kMaxBatch);
   const int fixed = 128 + (pl.TS - 1) * pl.HB * pl.qblocks * 8 * (D + 2) * 4 + (3 * rows + 1) * 4;
-  // two CTAs to an SM, each with a ring of what is left
-  const int cap = b2l_max_smem_optin() / 2 - 1536;
+  // sixteen warps to an SM, each CTA with a ring of its part of the shared memory (1 KB of it is the system's)
+  const int per_sm = 2 * kMaxConsumers / (pl.HB * pl.qblocks * pl.TS);
+  const int cap = (b2l_max_smem_optin() + 1024) / per_sm - 1024 - 128;
   pl.stages = (cap - fixed) / stage;
   if (pl.stages > kMaxStages) pl.stages = kMaxStages;
   if (pl.stages < 2) pl.stages = 2;
   pl.smem = fixed + pl.stages * stage;
   const int64_t most = (int64_t)rows * cdiv64(max_len > 0 ? max_len : 1, kMinTokens) * (Hkv / pl.HB);
-  const int64_t wave = 2ll * b2l_num_sms();
+  const int64_t wave = (int64_t)per_sm * b2l_num_sms();
   pl.grid = (int)(most < wave ? most : wave);
+  pl.cluster = batch * (Hkv / pl.HB) * kCluster <= wave && max_len <= kClusterMost && pl.HB * G * (D + 2) * 4 <= pl.stages * stage;
+  if (pl.cluster) pl.grid = (int)(batch * (Hkv / pl.HB) * kCluster);
   return pl;
 }
 
 template <typename T, int D, int GS>
 int launch_int4_decode(const Int4DecodeParams& p, const Int4Plan& pl, cudaStream_t st) {
   const dim3 grid((unsigned)pl.grid), block(pl.HB * pl.qblocks * pl.TS * 32);
+  if (pl.cluster) {
+    static int configured_cluster[2][64] = {{0}};
+    auto kern = p.G <= 4 ? kv4_decode_kernel<T, D, GS, true, true> : kv4_decode_kernel<T, D, GS, false, true>;
+    B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured_cluster[p.G <= 4]));
+    b2l_hang_arm(st);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = pl.smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = b2l_pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kern, p);
+    B2L_LAUNCH_CHECK();
+    return B2L_OK;
+  }
   static int configured[2][64] = {{0}};
-  auto kern = p.G <= 4 ? kv4_decode_kernel<T, D, GS, true> : kv4_decode_kernel<T, D, GS, false>;
+  auto kern = p.G <= 4 ? kv4_decode_kernel<T, D, GS, true, false> : kv4_decode_kernel<T, D, GS, false, false>;
   B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured[p.G <= 4]));
   b2l_launch(kern, grid, block, (size_t)pl.smem, st, p);
   B2L_LAUNCH_CHECK();
@@ -744,6 +917,7 @@ extern "C" int b2l_flash_decoding_int4(void* out, const void* q, const void* cac
   p.req_w = req_idx_width; p.len_w = seq_len_width;
   p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = G; p.HB = pl.HB; p.qblocks = pl.qblocks; p.TS = pl.TS;
   p.stages = pl.stages; p.pitch = pl.pitch;
+  p.bulk = !pl.cluster && pl.HB * kv4::head_bytes(head_dim, group) >= 512;   // rows that take all lanes a piece
   p.most = max_seq_len < table_width ? max_seq_len : table_width;
   if (p.most < 0) p.most = 0;
   B2L_REQUIRE((batch < kMaxBatch ? batch : kMaxBatch) * cdiv64(p.most, kUnit) * num_kv_heads < (1ll << 31), "flash_decoding_int4: too many tokens");
