@@ -16,10 +16,11 @@
 // an SM leave a thread 96 registers, and spill); a warp takes 16 or 32 tokens of one kv head.  A row
 // that lies in one share is written out; else its parts go to the workspace and a second kernel adds them up.
 #include "kv_int4.cuh"
+#include <type_traits>
 
 namespace {
 
-constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kCluster = 8;
+constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kCluster = 8, kRowCost = 1;
 constexpr int kMinTokens = 64;                    // of a share: below that the merge costs more than the share
 
 struct Int4DecodeParams {
@@ -71,6 +72,18 @@ struct Int4Consumer {
   int r, c;
   int k_at, g_at, v_at[2], step;                   // bytes from a unit's first row: key words, groups, value words of two tokens; eight rows
 
+  using Pair = typename Vec2<T>::type;
+  static __device__ __forceinline__ Pair as2(uint32_t w) { return *reinterpret_cast<Pair*>(&w); }
+  static __device__ __forceinline__ Pair pair2(float x) {
+    const uint32_t w = pack2<T>(x, x);
+    return as2(w);
+  }
+  // a pair of elements as halves (bf16: after scaling, within their range)
+  static __device__ __forceinline__ uint32_t to_half2(Pair x) {
+    const uint32_t w = *reinterpret_cast<uint32_t*>(&x);
+    if (std::is_same<T, __half>::value) return w;
+    return pack2<__half>(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
   static __device__ __forceinline__ int word_at(int k, int c) { return GS == 32 ? k * 4 + c : (k >> 1) * 8 + c * 2 + (k & 1); }
   static __device__ __forceinline__ constexpr int group_of(int k) { return GS == 32 ? k : GS == 64 ? k >> 1 : 0; }
 
@@ -92,50 +105,47 @@ struct Int4Consumer {
       }
     }
   }
+  // Packed arithmetic, and the sums by the tensor cores from codes of 1: straight-line code runs from a cold instruction cache once a
+  // segment, so its length is its time.
   __device__ __forceinline__ void begin(const Int4DecodeParams& p) {
-    float qv[NW][8], big = 0.f;
+    using T2 = typename Vec2<T>::type;
+    T2 most = as2(raw[0].x & 0x7fff7fffu);
 #pragma unroll
-    for (int k = 0; k < NW; ++k) {
-      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+    for (int k = 0; k < NW; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 x = kv4::scale_min<T>(w[i]);
-        qv[k][2 * i] = x.x;
-        qv[k][2 * i + 1] = x.y;
-        big = fmaxf(big, fmaxf(fabsf(x.x), fabsf(x.y)));
-      }
-    }
+      for (int i = 0; i < 4; ++i) most = __hmax2_nan(most, as2((&raw[k].x)[i] & 0x7fff7fffu));
+    const float2 ends = kv4::scale_min<T>(*reinterpret_cast<const uint32_t*>(&most));
+    float big = ends.x > ends.y || ends.x != ends.x ? ends.x : ends.y;
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    // largest element to [2^8, 2^9); an infinity stays one
+    // largest element to [2^8, 2^9), by 2^15 at most (a half multiplies); an infinity stays one
     int e = 8 - ((int)(__float_as_uint(big) >> 23) - 127);
     if (!(big < INFINITY) || big == 0.f) e = 0;
-    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    constexpr int kMost = std::is_same<T, __half>::value ? 15 : 100;
+    e = e < -kMost ? -kMost : e > kMost ? kMost : e;
     const float up = exp2i(e);
-    float sums[NG];
+    const T2 lo = pair2(up), hi = pair2(up * 0.0625f);
+    float sums[NG][4];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) sums[g] = 0.f;
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[g][i] = 0.f;
+    const uint32_t one[4] = {0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u}, one16[4] = {0x00100010u, 0x00100010u, 0x00100010u, 0x00100010u};
 #pragma unroll
     for (int k = 0; k < NW; ++k) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sums[group_of(k)] += qv[k][i];
-      const float lo = up, hi = up * 0.0625f;
-      qb[k][0] = pack2<__half>(qv[k][0] * lo, qv[k][4] * lo);
-      qb[k][1] = pack2<__half>(qv[k][2] * lo, qv[k][6] * lo);
-      qb[k][2] = pack2<__half>(qv[k][1] * hi, qv[k][5] * hi);
-      qb[k][3] = pack2<__half>(qv[k][3] * hi, qv[k][7] * hi);
+      qb[k][0] = to_half2(__hmul2(as2(__byte_perm(raw[k].x, raw[k].z, 0x5410)), lo));
+      qb[k][1] = to_half2(__hmul2(as2(__byte_perm(raw[k].y, raw[k].w, 0x5410)), lo));
+      qb[k][2] = to_half2(__hmul2(as2(__byte_perm(raw[k].x, raw[k].z, 0x7632)), hi));
+      qb[k][3] = to_half2(__hmul2(as2(__byte_perm(raw[k].y, raw[k].w, 0x7632)), hi));
+      mma(sums[group_of(k)], one, qb[k][0], qb[k][1]);
+      mma(sums[group_of(k)], one16, qb[k][2], qb[k][3]);
     }
     const float back = p.scale_log2 * exp2i(-e) * 16777216.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) f[j] = __shfl_sync(0xffffffffu, back, (2 * c + j) * 4);
+    for (int j = 0; j < 2; ++j) {
+      f[j] = __shfl_sync(0xffffffffu, back, (2 * c + j) * 4);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float s = sums[g];
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      s *= p.scale_log2;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) sq[j][g] = __shfl_sync(0xffffffffu, s, (2 * c + j) * 4);
+      for (int g = 0; g < NG; ++g) sq[j][g] = sums[g][j] * f[j];
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -434,6 +444,7 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     mbar_fence_init();
   }
 
+  auto cost = [&](int len) { return len > 0 ? (len + tile - 1) / tile + kRowCost : 0; };
   Segment seg;
   int all = 0, item = 0, item_end = 0, len0 = 0, req0 = 0;
   if (CLUSTER) {
@@ -447,14 +458,14 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     item_end = seg.first < seg.last;
     __syncthreads();
   } else {
-    // ---- tiles of the rows before each; a thread owns neighbouring rows ----
+    // ---- tiles of the rows before each (a row counts kRowCost more: its start and end); a thread owns neighbouring rows ----
     const int per = (p.batch + blockDim.x - 1) / blockDim.x, r_lo = threadIdx.x * per;
     const int r_hi = r_lo + per < p.batch ? r_lo + per : p.batch;
     int own = 0;
 #pragma unroll 1
     for (int r = r_lo; r < r_hi; ++r) {
       lens[r] = length(r, reqs[r]);
-      own += (lens[r] + tile - 1) / tile;
+      own += cost(lens[r]);
     }
     int upto = own;
 #pragma unroll
@@ -462,19 +473,20 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
       const int x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
-    if (lane == 31) warp_sum[warp] = upto;
-    __syncthreads();
     int at = upto - own;
-    const int of_warp = lane < nwarps ? warp_sum[lane] : 0;
-    all = __reduce_add_sync(0xffffffffu, of_warp);
-    at += __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0);
+    if (p.batch > 32) {                           // else the first warp has all rows
+      if (lane == 31) warp_sum[warp] = upto;
+      __syncthreads();
+      at += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
+    }
 #pragma unroll 1
     for (int r = r_lo; r < r_hi; ++r) {
       prefix[r] = at;
-      at += (lens[r] + tile - 1) / tile;
+      at += cost(lens[r]);
     }
-    if (threadIdx.x == 0) prefix[p.batch] = all;
+    if (r_hi == p.batch && r_lo < r_hi) prefix[p.batch] = at;
     __syncthreads();
+    all = prefix[p.batch];
     // ---- this CTA's share of all tiles, heads' blocks one after the other ----
     const int total = all * (p.Hkv / p.HB), least = (kMinTokens + tile - 1) / tile, worth = (total + least - 1) / least;
     const int shares = worth < (int)gridDim.x ? worth : (int)gridDim.x;
@@ -483,7 +495,7 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     item_end = (int)((int64_t)(blockIdx.x + 1) * total / shares);
   }
   // the part of a row at `item`
-  auto next = [&](int& item, Segment& s) -> bool {
+  auto part_at = [&](int& item, Segment& s) -> bool {
     if (item >= item_end) return false;
     if (CLUSTER) {
       s = seg;
@@ -500,12 +512,18 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
       else n = half;
     }
     s.b = lo;
-    s.first = x - prefix[lo];
-    s.tiles = prefix[lo + 1] - prefix[lo];
-    const int left = item_end - item;
-    s.last = left < s.tiles - s.first ? s.first + left : s.tiles;
-    item += s.last - s.first;
+    s.tiles = prefix[lo + 1] - prefix[lo] - kRowCost;
+    const int left = item_end - item, from = x - prefix[lo], to = left < prefix[lo + 1] - x ? from + left : s.tiles + kRowCost;
+    s.first = from > kRowCost ? from - kRowCost : 0;
+    s.last = to > kRowCost ? to - kRowCost : 0;   // may be empty: the part of a row's start that is only cost
+    item += to - from;
     return true;
+  };
+  auto next = [&](int& item, Segment& s) -> bool {
+    bool any;
+    do any = part_at(item, s);
+    while (any && s.first >= s.last);
+    return any;
   };
 
   // ---- the ring's copies: each warp brings its part of a tile's token rows, whose table entries are read a tile ahead.  One bulk copy to
@@ -712,37 +730,38 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
   cluster_sync_all();                             // the peers have read this CTA's part
 }
 
-// The rows that several CTAs met in, and zeros for the empty ones.  Bound by latency: a block takes one head of a row, its warps the
-// parts in turn, eight of each on their way together, and meet in shared memory.
-constexpr int kMergeWarps = 4;
-template <typename T, int D>
-__global__ void __launch_bounds__(kMergeWarps * 32) kv4_decode_merge_kernel(const Int4DecodeParams p) {
+// The rows that several CTAs met in, and zeros for the empty ones.  Bound by latency: W warps take the parts of a row's head in turn,
+// eight of each on their way together, and meet in shared memory (W = 1: four heads to a block, no meeting).
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) kv4_decode_merge_kernel(const Int4DecodeParams p) {
   pdl_prologue();
   constexpr int E = D / 32, kAsk = 8;             // neighbouring elements of a lane
-  __shared__ float sums[kMergeWarps][D + 2];
-  const int b = blockIdx.x, head = blockIdx.y, kvh = head / p.G, blk = kvh / p.HB;
-  const int local = (kvh - blk * p.HB) * p.G + head - kvh * p.G;
+  __shared__ float sums[W][W == 1 ? 1 : D + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.x, head = W == 1 ? blockIdx.y * 4 + warp : blockIdx.y;
+  if (head >= p.Hq) return;
+  const int kvh = head / p.G, blk = kvh / p.HB, local = (kvh - blk * p.HB) * p.G + head - kvh * p.G;
   const int2 who = __ldcg(p.ws_info + (int64_t)blk * p.batch + b);   // of an empty row: an earlier call's
   const int64_t len = load_index(p.seq_len, b, p.len_w), q = load_index(p.req_idx, b, p.req_w);
   T* out = reinterpret_cast<T*>(p.out) + (int64_t)b * p.o_bs + (int64_t)head * p.o_hs;
   if (len <= 0 || q < 0 || q >= p.requests || p.most <= 0) {
-    for (int d = threadIdx.x; d < D; d += blockDim.x) out[d] = from_f32<T>(0.f);
+    for (int d = W == 1 ? lane : threadIdx.x; d < D; d += W * 32) out[d] = from_f32<T>(0.f);
     return;
   }
   const int n = who.y - who.x + 1;
   if (n < 2) return;                              // written by its only CTA
+  const int first = W == 1 ? 0 : warp;
   auto part = [&](int i) { return ((int64_t)(who.x + i) * 2 + (i == 0 ? 1 : 0)) * p.HB * p.G + local; };
   float acc[E], M = -INFINITY, L = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll 1
-  for (int i0 = warp; i0 < n; i0 += kMergeWarps * kAsk) {
+  for (int i0 = first; i0 < n; i0 += W * kAsk) {
     float x[kAsk][E];
     float2 ml[kAsk];
 #pragma unroll
     for (int k = 0; k < kAsk; ++k) {
-      const int i = i0 + kMergeWarps * k;
+      const int i = i0 + W * k;
       ml[k] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int e = 0; e < E; ++e) x[k][e] = 0.f;
@@ -776,6 +795,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_decode_merge_kernel(cons
     }
     M = mm;
   }
+  if (W == 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[lane * E + e] = from_f32<T>(acc[e] / L);
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[e];
   if (lane == 0) { sums[warp][D] = M; sums[warp][D + 1] = L; }
@@ -783,10 +807,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_decode_merge_kernel(cons
   if ((int)threadIdx.x < D) {
     float mm = -INFINITY, o = 0.f, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) mm = fmaxf(mm, sums[w][D]);
+    for (int w = 0; w < W; ++w) mm = fmaxf(mm, sums[w][D]);
     const float base = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float a = fast_exp2(sums[w][D] - base);
       o = fmaf(sums[w][threadIdx.x], a, o);
       l = fmaf(sums[w][D + 1], a, l);
@@ -861,7 +885,11 @@ int launch_int4_decode(const Int4DecodeParams& p, const Int4Plan& pl, cudaStream
   B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured[p.G <= 4]));
   b2l_launch(kern, grid, block, (size_t)pl.smem, st, p);
   B2L_LAUNCH_CHECK();
-  b2l_launch(kv4_decode_merge_kernel<T, D>, dim3((unsigned)p.batch, (unsigned)p.Hq), dim3(kMergeWarps * 32), (size_t)0, st, p);
+  // many parts to a row, or few
+  if ((int64_t)pl.grid > 24 * (int64_t)p.batch)
+    b2l_launch(kv4_decode_merge_kernel<T, D, 16>, dim3((unsigned)p.batch, (unsigned)p.Hq), dim3(512), (size_t)0, st, p);
+  else
+    b2l_launch(kv4_decode_merge_kernel<T, D, 1>, dim3((unsigned)p.batch, (unsigned)((p.Hq + 3) / 4)), dim3(128), (size_t)0, st, p);
   B2L_LAUNCH_CHECK();
   return B2L_OK;
 }
