@@ -11,7 +11,7 @@
 // head's largest element.  Probabilities are not rounded to 11 bits: what rounding leaves of p s is multiplied as well -- in the
 // columns that up to four heads leave free, else in a second product -- since a code's products are larger than its value's.
 //
-// Work: tiles of 16 * TS tokens of all rows, in equal shares over one wave of CTAs, whatever rows they belong to (the lengths are device
+// Work: tiles of 16 * TS or 32 * TS tokens of all rows, in equal shares over one wave of CTAs, whatever rows they belong to (the lengths are device
 // data).  Whole token rows come by asynchronous copies into a ring (of the working warps: with a warp of its own for that, two CTAs to
 // an SM leave a thread 96 registers, and spill); a warp takes 16 or 32 tokens of one kv head.  A row
 // that lies in one share is written out; else its parts go to the workspace and a second kernel adds them up.
@@ -20,8 +20,8 @@
 
 namespace {
 
-constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kCluster = 8, kRowCost = 1;
-constexpr int kMinTokens = 64;                    // of a share: below that the merge costs more than the share
+constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kCluster = 8, kRowCost = 1, kFirst = 3;
+constexpr int kMinLog2 = 6, kMinTokens = 1 << kMinLog2;   // of a share: below that the merge costs more than the share
 
 struct Int4DecodeParams {
   const void* q; int64_t q_bs, q_hs; int q_vec;   // q_vec: heads on 16-byte boundaries
@@ -30,7 +30,7 @@ struct Int4DecodeParams {
   const int32_t* table; int64_t tab_rs, tab_cs, requests, width;
   const void* req_idx; int req_w;
   const void* seq_len; int len_w;
-  int batch, Hq, Hkv, G, HB, qblocks, TS, stages, pitch, bulk;
+  int batch, Hq, Hkv, G, HB, nblk, qblocks, TS, TS_log2, stages, pitch, bulk;
   int64_t most;                                   // tokens of a row that the call's bound lets count
   float scale_log2;
   float* ws_o; float* ws_ml; int2* ws_info;       // parts [cta][2][HB * G]: rows, (largest score, sum); first and last CTA of a row
@@ -423,7 +423,8 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
   uint64_t* empty_bar = full_bar + kMaxStages;
   uint8_t* ring = smem + 128;
   constexpr int kWarpTokens = kUnit * units_of(D, GS);
-  const int warp_bytes = kWarpTokens * p.pitch, stage_bytes = p.TS * warp_bytes, tile = p.TS * kWarpTokens;
+  const int tile_log2 = p.TS_log2 + (kWarpTokens == 32 ? 5 : 4), tile = 1 << tile_log2;
+  const int warp_bytes = kWarpTokens * p.pitch, stage_bytes = warp_bytes << p.TS_log2;
   float* join = reinterpret_cast<float*>(ring + p.stages * stage_bytes);      // sums of the warps that share a head
   const int per_head = p.qblocks * 8 * (D + 2);
   int* prefix = reinterpret_cast<int*>(join + (p.TS - 1) * p.HB * per_head);  // tiles of the rows before, [batch + 1]
@@ -431,6 +432,7 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
   int* reqs = lens + p.batch;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nwarps = p.HB * p.qblocks * p.TS;
+  const int heads_warps = p.HB * p.qblocks;
   auto length = [&](int r, int& req) {
     const int64_t n = load_index(p.seq_len, r, p.len_w), q = load_index(p.req_idx, r, p.req_w);
     req = (int)q;
@@ -444,7 +446,7 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     mbar_fence_init();
   }
 
-  auto cost = [&](int len) { return len > 0 ? (len + tile - 1) / tile + kRowCost : 0; };
+  auto cost = [&](int len) { return len > 0 ? ((len + tile - 1) >> tile_log2) + kRowCost : 0; };
   Segment seg;
   int all = 0, item = 0, item_end = 0, len0 = 0, req0 = 0;
   if (CLUSTER) {
@@ -452,14 +454,14 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     seg.blk = id / p.batch;
     seg.b = id - seg.blk * p.batch;
     len0 = length(seg.b, req0);
-    seg.tiles = (len0 + tile - 1) / tile;
+    seg.tiles = (len0 + tile - 1) >> tile_log2;
     seg.first = seg.tiles * rank / kCluster;
     seg.last = seg.tiles * (rank + 1) / kCluster;
     item_end = seg.first < seg.last;
     __syncthreads();
   } else {
     // ---- tiles of the rows before each (a row counts kRowCost more: its start and end); a thread owns neighbouring rows ----
-    const int per = (p.batch + blockDim.x - 1) / blockDim.x, r_lo = threadIdx.x * per;
+    const int per = p.batch <= 32 ? 1 : (p.batch + (int)blockDim.x - 1) / (int)blockDim.x, r_lo = threadIdx.x * per;
     const int r_hi = r_lo + per < p.batch ? r_lo + per : p.batch;
     int own = 0;
 #pragma unroll 1
@@ -488,11 +490,12 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     __syncthreads();
     all = prefix[p.batch];
     // ---- this CTA's share of all tiles, heads' blocks one after the other ----
-    const int total = all * (p.Hkv / p.HB), least = (kMinTokens + tile - 1) / tile, worth = (total + least - 1) / least;
+    const int total = all * p.nblk, least = tile_log2 < kMinLog2 ? kMinLog2 - tile_log2 : 0, worth = (total + (1 << least) - 1) >> least;
     const int shares = worth < (int)gridDim.x ? worth : (int)gridDim.x;
     if ((int)blockIdx.x >= shares) return;
-    item = (int)((int64_t)blockIdx.x * total / shares);
-    item_end = (int)((int64_t)(blockIdx.x + 1) * total / shares);
+    const int each = total / shares, more_by_one = total - each * shares;
+    item = blockIdx.x * each + ((int)blockIdx.x < more_by_one ? blockIdx.x : more_by_one);
+    item_end = item + each + ((int)blockIdx.x < more_by_one);
   }
   // the part of a row at `item`
   auto part_at = [&](int& item, Segment& s) -> bool {
@@ -502,14 +505,15 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
       item = item_end;
       return true;
     }
-    s.blk = item / all;
+    s.blk = p.nblk == 1 ? 0 : item / all;
     const int x = item - s.blk * all;
-    int lo = 0, n = p.batch;                      // the last row that begins at or before x and has tiles
+    int lo = 0, n = p.batch;                      // the last row that begins at or before x, 32 at a look
 #pragma unroll 1
     while (n > 1) {
-      const int half = n / 2;
-      if (prefix[lo + half] <= x) { lo += half; n -= half; }
-      else n = half;
+      const int stride = (n + 31) >> 5, i = lane * stride;
+      const int k = __popc(__ballot_sync(0xffffffffu, i < n && prefix[lo + i] <= x)) - 1;
+      lo += k * stride;
+      n = n - k * stride < stride ? n - k * stride : stride;
     }
     s.b = lo;
     s.tiles = prefix[lo + 1] - prefix[lo] - kRowCost;
@@ -530,22 +534,31 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
   // a row costs the warp least, but the engine ~40 cycles: 32 rows 1400, which a cluster's few tiles wait for, and rows of 160 bytes
   // limited the whole kernel (150 sequences of 200 - 400 tokens, 2 kv heads of 64: 20.5 us, this 18.0).  Else 16 bytes a lane (32 of
   // 1000 - 2000, 8 kv heads of 128: 34 us, bulk 31). ----
-  const int hb = kv4::head_bytes(D, GS), mine = (tile + nwarps - 1) / nwarps;   // token rows of this warp, at most 32
-  Segment ahead;                                  // of the tile that is brought next
-  int ahead_item = item, ahead_t = 0, row = 0, ahead_here = 0;
-  bool more = next(ahead_item, ahead);
-  auto entries = [&] {
-    const int len = CLUSTER ? len0 : lens[ahead.b], req = CLUSTER ? req0 : reqs[ahead.b];
-    const int left = len - ahead_t * tile, i = warp * mine + lane;
-    ahead_here = left < tile ? left : tile;
-    if (lane < mine && i < ahead_here)
-      row = ld_upstream(p.table + (int64_t)req * p.tab_rs + (int64_t)(ahead_t * tile + i) * p.tab_cs);
+  const int hb = kv4::head_bytes(D, GS), mine = nwarps == 8 ? tile >> 3 : (tile + nwarps - 1) / nwarps;   // token rows of this warp, at most 32
+  struct Place { Segment s; int item, t; bool more; };   // a tile of the share
+  auto start_of = [&](Place& x) {
+    x.item = item;
+    x.more = next(x.item, x.s);
+    x.t = x.s.first;
   };
-  if (more) { ahead_t = ahead.first; entries(); }
-  auto bring = [&](int s) {
-    if (!more) return;
-    const int from = ahead.blk * p.HB * hb, shift = from & 15, pieces = (shift + p.HB * hb + 15) >> 4;
-    const int first = warp * mine, mine_here = ahead_here - first < mine ? ahead_here - first : mine;
+  auto step_on = [&](Place& x) {
+    if (++x.t == x.s.last) {
+      x.more = next(x.item, x.s);
+      x.t = x.s.first;
+    }
+  };
+  auto rows_of = [&](const Place& x) {            // token rows of the tile
+    const int left = (CLUSTER ? len0 : lens[x.s.b]) - x.t * tile;
+    return left < tile ? left : tile;
+  };
+  auto entry = [&](const Place& x) -> int {       // this lane's
+    const int i = warp * mine + lane;
+    if (!x.more || lane >= mine || i >= rows_of(x)) return 0;
+    return ld_upstream(p.table + (int64_t)(CLUSTER ? req0 : reqs[x.s.b]) * p.tab_rs + (int64_t)(x.t * tile + i) * p.tab_cs);
+  };
+  auto bring = [&](const Place& x, int row, int s) {
+    const int from = x.s.blk * p.HB * hb, shift = from & 15, pieces = (shift + p.HB * hb + 15) >> 4;
+    const int first = warp * mine, rows_here = rows_of(x) - first, mine_here = rows_here < mine ? rows_here : mine;
     const uint8_t* src = p.cache + (from - shift);
     uint8_t* dst = ring + s * stage_bytes + first * p.pitch;
     const int at = row < 0 || row >= p.max_tokens ? 0 : row;
@@ -553,7 +566,9 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
       if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], (uint32_t)((mine_here > 0 ? mine_here : 0) * pieces * 16));
       __syncwarp();
       if (lane < mine_here) bulk_g2s(dst + lane * p.pitch, src + (int64_t)at * p.row_stride, (uint32_t)pieces * 16u, &full_bar[s]);
-    } else if (pieces >= 32) {                           // a row at a time
+      return;
+    }
+    if (pieces >= 32) {                           // a row at a time
 #pragma unroll 1
       for (int i = 0; i < mine_here; ++i) {
         const uint8_t* x = src + (int64_t)__shfl_sync(0xffffffffu, at, i) * p.row_stride;
@@ -568,26 +583,43 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
         if (i0 < rows && i + i0 < mine_here) copy16(dst + (i + i0) * p.pitch + c * 16, src + r * p.row_stride + c * 16);
       }
     }
-    if (!p.bulk) copies_arrive(&full_bar[s]);
-    if (++ahead_t == ahead.last) {
-      more = next(ahead_item, ahead);
-      if (more) ahead_t = ahead.first;
-    }
-    if (more) entries();
+    copies_arrive(&full_bar[s]);
   };
 
   // ===================== a warp: (kv head, block of query heads, unit of the tile) =====================
-  const int ts = warp / (p.HB * p.qblocks), wh = warp - ts * p.HB * p.qblocks;
-  const int hl = wh / p.qblocks, qblk = wh - hl * p.qblocks;
+  const int ts = p.TS == 1 ? 0 : warp / heads_warps, wh = warp - ts * heads_warps;
+  const int hl = p.qblocks == 1 ? wh : wh / p.qblocks, qblk = wh - hl * p.qblocks;
   const int head0 = qblk * 8, heads = p.G - head0 < 8 ? p.G - head0 : 8;
   Int4Consumer<T, D, GS, DUP> c(lane, p.pitch);
   // columns of this lane: heads 2c and 2c + 1 (DUP: the upper half of the columns repeats the lower)
   const bool counts = !DUP || c.c < 2;
   int s = 0, at_tile = 0;
   uint32_t phase = 0;
+  // The first tiles are much of what a share reads: their entries are read together, and their rows asked for at once (the query before
+  // them: behind them it waits for all of their bytes).
+  Place ahead;
+  start_of(ahead);
   bool got = next(item, seg);
   if (got) c.ask(p, seg.b, seg.blk * p.HB + hl, head0, heads);
-  for (int f = 0; f < p.stages; ++f) bring(f);
+  int row = 0;
+  {
+    Place look = ahead;
+    int first_rows[kFirst];
+#pragma unroll
+    for (int f = 0; f < kFirst; ++f) {
+      first_rows[f] = entry(look);
+      if (look.more) step_on(look);
+    }
+    for (int f = 0; f < p.stages && ahead.more; ++f) {
+      row = first_rows[0];
+#pragma unroll
+      for (int k = 1; k < kFirst; ++k) row = f == k ? first_rows[k] : row;
+      if (f >= kFirst) row = entry(ahead);
+      bring(ahead, row, f);
+      step_on(ahead);
+    }
+    row = entry(ahead);
+  }
   while (got) {
     const int len = CLUSTER ? len0 : lens[seg.b], kvh = seg.blk * p.HB + hl;
     const int off = ((seg.blk * p.HB * hb) & 15) + hl * hb + ts * warp_bytes;
@@ -599,15 +631,18 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
       if (valid > 0) c.tile(ring + s * stage_bytes + off, valid);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[s]);
-      if (at_tile > 0 && more) {                  // into the stage of the tile before this one, which the others have left by now
+      if (at_tile > 0 && ahead.more) {            // into the stage of the tile before this one, which the others have left by now
         const int b = s == 0 ? p.stages - 1 : s - 1;
         mbar_wait(&empty_bar[b], s == 0 ? phase ^ 1u : phase);
-        bring(b);
+        bring(ahead, row, b);
+        step_on(ahead);
+        row = entry(ahead);
       }
       if (++s == p.stages) { s = 0; phase ^= 1; }
     }
     const Segment done = seg;
     got = next(item, seg);
+    if (got) c.ask(p, seg.b, seg.blk * p.HB + hl, head0, heads);
     c.finish();
     if (p.TS > 1) {
       auto bar = [&] { asm volatile("bar.sync 1, %0;" ::"r"(nwarps * 32) : "memory"); };
@@ -645,7 +680,6 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
         }
       }
     }
-    if (got) c.ask(p, seg.b, seg.blk * p.HB + hl, head0, heads);
     if (CLUSTER) break;
     const bool whole = done.first == 0 && done.last == done.tiles;
     if (ts == 0 && counts) {
@@ -795,11 +829,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) kv4_decode_merge_kernel
     }
     M = mm;
   }
-  if (W == 1) {
+  if constexpr (W == 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e) out[lane * E + e] = from_f32<T>(acc[e] / L);
-    return;
-  }
+  } else {
 #pragma unroll
   for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[e];
   if (lane == 0) { sums[warp][D] = M; sums[warp][D + 1] = L; }
@@ -817,6 +850,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) kv4_decode_merge_kernel
     }
     out[threadIdx.x] = from_f32<T>(o / l);
   }
+  }
 }
 
 constexpr int kMaxBatch = 4096;                   // rows of one launch (their lengths lie in shared memory)
@@ -832,7 +866,7 @@ Int4Plan make_plan(int64_t batch, int G, int Hkv, int D, int group, int64_t max_
   for (int h = 1; h * pl.qblocks <= kMaxConsumers; ++h)
     if (Hkv % h == 0) pl.HB = h;
   const int units = units_of(D, group);
-  pl.TS = kMaxConsumers / (pl.HB * pl.qblocks);
+  for (pl.TS = 1; 2 * pl.TS * pl.HB * pl.qblocks <= kMaxConsumers;) pl.TS *= 2;
   if (pl.TS > 8 / units) pl.TS = 8 / units;       // 128 tokens to a tile at most
   const int hb = kv4::head_bytes(D, group);
   const int bytes = ((pl.HB * hb + (pl.HB == Hkv ? 0 : 8)) + 15) / 16 * 16;
@@ -944,7 +978,8 @@ extern "C" int b2l_flash_decoding_int4(void* out, const void* q, const void* cac
   p.requests = table_requests; p.width = table_width;
   p.req_w = req_idx_width; p.len_w = seq_len_width;
   p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = G; p.HB = pl.HB; p.qblocks = pl.qblocks; p.TS = pl.TS;
-  p.stages = pl.stages; p.pitch = pl.pitch;
+  p.stages = pl.stages; p.pitch = pl.pitch; p.nblk = num_kv_heads / pl.HB;
+  for (p.TS_log2 = 0; 1 << p.TS_log2 < pl.TS;) ++p.TS_log2;     // a power of two
   p.bulk = !pl.cluster && pl.HB * kv4::head_bytes(head_dim, group) >= 512;   // rows that take all lanes a piece
   p.most = max_seq_len < table_width ? max_seq_len : table_width;
   if (p.most < 0) p.most = 0;
