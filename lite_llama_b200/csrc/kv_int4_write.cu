@@ -121,7 +121,8 @@ struct Grid {
 
 // A thread holds eight elements of a head's lower half and the eight that rotate with them of its upper half; a head's threads are
 // neighbours in a warp and find their groups' ends with one to four shuffles.  All of a token's heads -- q rotated, k rotated and
-// stored, v stored -- are units of one grid: a decode step is one trip through L2, not one per head.
+// stored, v stored -- are units of one grid: a decode step is one trip through L2, not one per head.  (8000 tokens of 28 + 4 + 4 heads of
+// 128, bf16, 147 MB: blocks of 96 threads 29 us, of 288, a token's all heads, 33, with two tokens to a thread 42.)
 template <typename T, int D, int GS, bool VEC>
 __global__ void __launch_bounds__(128) kv4_write_kernel(const WriteParams p) {
   pdl_prologue();
@@ -129,33 +130,34 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(const WriteParams p) {
   using T2 = typename X::T2;
   constexpr int HALF = D / 2, UNITS = HALF / 8;
   constexpr int NG = D / GS, LANES = (GS < HALF ? GS : HALF) / 8;   // threads that share a group of one half
-  const int64_t tok = blockIdx.x;
-  const int i = blockIdx.y * 128 + threadIdx.x;
+  const int i = blockIdx.y * blockDim.x + threadIdx.x;
   const int h = i / UNITS, c = (i % UNITS) * 8;
   const bool is_q = h < p.n_qh, is_v = h >= p.n_qh + p.n_kh;
-  const bool live = h < p.n_qh + 2 * p.n_kh;       // a head's threads are live together; a warp's heads need not be
-  uint32_t a[4] = {0, 0, 0, 0}, b[4] = {0, 0, 0, 0};
-  int64_t row = -1;
   const int hk = is_v ? h - p.n_qh - p.n_kh : h - p.n_qh;
-  if (live) {
-    if (!is_q) row = load_index(p.index, tok, p.index_w);
-    const T* src = is_q ? (const T*)p.q + tok * p.q_ts + (int64_t)h * p.q_hs
-                 : is_v ? (const T*)p.v + tok * p.v_ts + (int64_t)hk * p.v_hs : (const T*)p.k + tok * p.k_ts + (int64_t)hk * p.k_hs;
-    load8<T, VEC>(a, src + c);
-    load8<T, VEC>(b, src + c + HALF);
-    if (!is_v && p.cos != nullptr) {
-      const int64_t cs = (tok / p.seq_len) * p.cs_b + (tok % p.seq_len) * p.cs_s + c;
-      uint32_t cv[4], sv[4];
-      load8<T, VEC>(cv, (const T*)p.cos + cs);
-      load8<T, VEC>(sv, (const T*)p.sin + cs);
-      rotate<T>(a, b, cv, sv);
-      T* dst = is_q ? (T*)p.q_out + tok * p.qo_ts + (int64_t)h * p.qo_hs : (T*)p.k_out + tok * p.ko_ts + (int64_t)hk * p.ko_hs;
-      if (dst != nullptr && (is_q || p.k_out != nullptr)) {
-        store8<T, VEC>(dst + c, a);
-        store8<T, VEC>(dst + c + HALF, b);
-      }
+  if (h >= p.n_qh + 2 * p.n_kh) return;             // a head's threads leave together; a warp's heads need not
+  const T* src = is_q ? (const T*)p.q + (int64_t)h * p.q_hs : is_v ? (const T*)p.v + (int64_t)hk * p.v_hs : (const T*)p.k + (int64_t)hk * p.k_hs;
+  const int64_t ts = is_q ? p.q_ts : is_v ? p.v_ts : p.k_ts;
+  const bool turn = !is_v && p.cos != nullptr;
+  const int64_t tok = blockIdx.x;
+  uint32_t a[4], b[4];
+  int64_t row = -1;
+  load8<T, VEC>(a, src + tok * ts + c);
+  load8<T, VEC>(b, src + tok * ts + c + HALF);
+  if (!is_q) row = load_index(p.index, tok, p.index_w);
+  if (turn) {
+    uint32_t cv[4], sv[4];
+    const int64_t at = p.seq_len == 1 ? tok : blockIdx.x / (unsigned)p.seq_len;
+    const int64_t cs = at * p.cs_b + (tok - at * p.seq_len) * p.cs_s + c;
+    load8<T, VEC>(cv, (const T*)p.cos + cs);
+    load8<T, VEC>(sv, (const T*)p.sin + cs);
+    rotate<T>(a, b, cv, sv);
+    T* dst = is_q ? (T*)p.q_out + tok * p.qo_ts + (int64_t)h * p.qo_hs : (T*)p.k_out + tok * p.ko_ts + (int64_t)hk * p.ko_hs;
+    if (is_q || p.k_out != nullptr) {
+      store8<T, VEC>(dst + c, a);
+      store8<T, VEC>(dst + c + HALF, b);
     }
   }
+  if (is_q) return;
   // ends of this thread's group in either half (one group over both: of both)
   T2 lo_a = as_pair<T2>(a[0]), hi_a = lo_a, lo_b = as_pair<T2>(b[0]), hi_b = lo_b;
 #pragma unroll
@@ -164,14 +166,16 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(const WriteParams p) {
     lo_b = X::lo(lo_b, as_pair<T2>(b[j])); hi_b = X::hi(hi_b, as_pair<T2>(b[j]));
   }
   if (GS == D) { lo_a = lo_b = X::lo(lo_a, lo_b); hi_a = hi_b = X::hi(hi_a, hi_b); }
+  // the head's threads: other heads of the warp may have left or be queries
+  const unsigned mine = UNITS == 32 ? 0xffffffffu : ((1u << UNITS) - 1u) << ((threadIdx.x & 31) / UNITS * UNITS);
 #pragma unroll
   for (int o = 1; o < LANES; o <<= 1) {
-    lo_a = X::lo(lo_a, as_pair<T2>(__shfl_xor_sync(0xffffffffu, bits(lo_a), o)));
-    hi_a = X::hi(hi_a, as_pair<T2>(__shfl_xor_sync(0xffffffffu, bits(hi_a), o)));
-    lo_b = X::lo(lo_b, as_pair<T2>(__shfl_xor_sync(0xffffffffu, bits(lo_b), o)));
-    hi_b = X::hi(hi_b, as_pair<T2>(__shfl_xor_sync(0xffffffffu, bits(hi_b), o)));
+    lo_a = X::lo(lo_a, as_pair<T2>(__shfl_xor_sync(mine, bits(lo_a), o)));
+    hi_a = X::hi(hi_a, as_pair<T2>(__shfl_xor_sync(mine, bits(hi_a), o)));
+    lo_b = X::lo(lo_b, as_pair<T2>(__shfl_xor_sync(mine, bits(lo_b), o)));
+    hi_b = X::hi(hi_b, as_pair<T2>(__shfl_xor_sync(mine, bits(hi_b), o)));
   }
-  if (!live || is_q || row < 0 || row >= p.max_tokens) return;   // a padded token has no row
+  if (row < 0 || row >= p.max_tokens) return;   // a padded token has no row
   auto low = [](T2 v) { const float2 f = X::f2(v); return f.x != f.x || f.x < f.y ? f.x : f.y; };
   auto high = [](T2 v) { const float2 f = X::f2(v); return f.x != f.x || f.x > f.y ? f.x : f.y; };
   Grid<T> ga, gb;
@@ -189,32 +193,51 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(const WriteParams p) {
   }
 }
 
-// Eight elements a thread.
-template <typename T, int D, int GS>
-__global__ void __launch_bounds__(128) kv4_read_kernel(T* out, const uint8_t* cache, const void* index, int index_w, int n_kh,
-                                                       int64_t row_stride, int64_t max_tokens) {
+// Eight elements and R tokens a thread.
+template <typename T, int D, int GS, int R>
+__global__ void __launch_bounds__(256) kv4_read_kernel(T* out, const uint8_t* cache, const void* index, int index_w, int n_kh,
+                                                       int64_t row_stride, int64_t max_tokens, int64_t tokens) {
   pdl_prologue();
   constexpr int NG = D / GS, UNITS = D / 8;
-  const int64_t tok = blockIdx.x;
-  const int i = blockIdx.y * 128 + threadIdx.x, h = i / UNITS, c = i % UNITS;
+  const int i = blockIdx.y * blockDim.x + threadIdx.x, h = i / UNITS, c = i % UNITS;
   if (h >= 2 * n_kh) return;
-  const int64_t row = load_index(index, tok, index_w);
   const bool is_v = h >= n_kh;
-  uint4 o = make_uint4(0, 0, 0, 0);
-  if (row >= 0 && row < max_tokens) {
-    const uint8_t* head = cache + row * row_stride + (int64_t)(is_v ? h - n_kh : h) * kv4::head_bytes(D, GS);
-    const uint32_t w = reinterpret_cast<const uint32_t*>(head + (is_v ? D / 2 : 0))[c];
-    const float2 sm = kv4::scale_min<T>(reinterpret_cast<const uint32_t*>(head + D)[(is_v ? NG : 0) + c * 8 / GS]);
+  int64_t row[R];
+  uint32_t w[R], g[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t tok = (int64_t)blockIdx.x * R + r;
+    row[r] = tok < tokens ? load_index(index, tok, index_w) : -1;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    w[r] = g[r] = 0u;
+    if (row[r] < 0 || row[r] >= max_tokens) continue;   // zeros
+    const uint8_t* head = cache + row[r] * row_stride + (int64_t)(is_v ? h - n_kh : h) * kv4::head_bytes(D, GS);
+    w[r] = reinterpret_cast<const uint32_t*>(head + (is_v ? D / 2 : 0))[c];
+    g[r] = reinterpret_cast<const uint32_t*>(head + D)[(is_v ? NG : 0) + c * 8 / GS];
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t tok = (int64_t)blockIdx.x * R + r;
+    if (tok >= tokens) break;
+    const float2 sm = kv4::scale_min<T>(g[r]);
     // 15 rounded steps may end above the type's largest number, which the group's maximum then was: no infinity (a NaN stays)
     constexpr float kMost = std::is_same<T, __half>::value ? 65504.f : 3.38953139e38f;
     auto one = [&](int at) {
-      const float x = fmaf((float)(w >> at & 15u), sm.x, sm.y);
+      const float x = fmaf((float)(w[r] >> at & 15u), sm.x, sm.y);
       return x > kMost ? kMost : x;
     };
     auto two = [&](int at) { return pack2<T>(one(at), one(at + 4)); };
-    o = make_uint4(two(0), two(8), two(16), two(24));
+    reinterpret_cast<uint4*>(out)[(tok * 2 * n_kh + h) * UNITS + c] = make_uint4(two(0), two(8), two(16), two(24));
   }
-  reinterpret_cast<uint4*>(out)[(tok * 2 * n_kh + h) * UNITS + c] = o;
+}
+
+// blocks of whole warps that share `units` threads evenly
+struct Blocks { unsigned parts, threads; };
+Blocks blocks_of(int64_t units, int most) {
+  const int64_t parts = cdiv64(units, most);
+  return {(unsigned)parts, (unsigned)(cdiv64(cdiv64(units, parts), 32) * 32)};
 }
 
 int check_cache(const char* what, const void* cache, int64_t row_stride, int64_t max_tokens, int n_kh, int head_dim, int group) {
@@ -259,13 +282,13 @@ extern "C" int b2l_kv_int4_write(void* q_out, void* k_out, const void* q, const 
                              cs_seq_stride, qo_tok_stride, qo_head_stride, ko_tok_stride, ko_head_stride};
   bool vec = ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cos | (uintptr_t)sin | (uintptr_t)q_out | (uintptr_t)k_out) % 16 == 0;
   for (int64_t s : strides) vec = vec && s % 8 == 0;
-  const int64_t parts = cdiv64(((int64_t)n_qh + 2 * (int64_t)n_kh) * (head_dim / 16), 128);
-  B2L_REQUIRE(parts <= 65535, "kv_int4_write: too many heads");
-  const dim3 grid((unsigned)tokens, (unsigned)parts);
+  const Blocks bl = blocks_of(((int64_t)n_qh + 2 * (int64_t)n_kh) * (head_dim / 16), 128);
+  B2L_REQUIRE(bl.parts <= 65535, "kv_int4_write: too many heads");
+  const dim3 grid((unsigned)tokens, bl.parts);
   cudaStream_t st = (cudaStream_t)stream;
 #define KV4_WRITE(TT)                                                                                   \
   KV4_DISPATCH_SHAPE(head_dim, group, {                                                                 \
-    b2l_launch(vec ? kv4_write_kernel<TT, D, GS, true> : kv4_write_kernel<TT, D, GS, false>, grid, dim3(128), (size_t)0, st, p); \
+    b2l_launch(vec ? kv4_write_kernel<TT, D, GS, true> : kv4_write_kernel<TT, D, GS, false>, grid, dim3(bl.threads), (size_t)0, st, p); \
   })
   if (dtype == B2L_F16) KV4_WRITE(__half);
   else KV4_WRITE(__nv_bfloat16);
@@ -282,14 +305,15 @@ extern "C" int b2l_kv_int4_read(void* out, const void* cache, int64_t cache_row_
   B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "kv_int4_read: dtype %d", dtype);
   B2L_REQUIRE(tokens >= 0 && tokens < (1ll << 31) && (uintptr_t)out % 16 == 0, "kv_int4_read: bad shape");
   if (tokens == 0) return B2L_OK;
-  const int64_t parts = cdiv64(2 * (int64_t)n_kh * (head_dim / 8), 128);
-  B2L_REQUIRE(parts <= 65535, "kv_int4_read: too many heads");
-  const dim3 grid((unsigned)tokens, (unsigned)parts);
+  const Blocks bl = blocks_of(2 * (int64_t)n_kh * (head_dim / 8), 256);
+  B2L_REQUIRE(bl.parts <= 65535, "kv_int4_read: too many heads");
+  const bool four = tokens * bl.parts * bl.threads > 2ll * 2048 * b2l_num_sms();   // as above
+  const dim3 grid((unsigned)cdiv64(tokens, four ? 4 : 1), bl.parts);
   cudaStream_t st = (cudaStream_t)stream;
 #define KV4_READ(TT)                                                                                                             \
   KV4_DISPATCH_SHAPE(head_dim, group, {                                                                                          \
-    b2l_launch(kv4_read_kernel<TT, D, GS>, grid, dim3(128), (size_t)0, st, (TT*)out, (const uint8_t*)cache, select_index,        \
-               index_width, n_kh, cache_row_stride, max_tokens);                                                                 \
+    b2l_launch(four ? kv4_read_kernel<TT, D, GS, 4> : kv4_read_kernel<TT, D, GS, 1>, grid, dim3(bl.threads), (size_t)0, st, (TT*)out, \
+               (const uint8_t*)cache, select_index, index_width, n_kh, cache_row_stride, max_tokens, tokens);                    \
   })
   if (dtype == B2L_F16) KV4_READ(__half);
   else KV4_READ(__nv_bfloat16);
