@@ -44,7 +44,7 @@ struct {
   int64_t (*kv4_decode_workspace)(i64, int, int, int, int, i64);
   int (*kv4_decode)(void*, const void*, const void*, i64, i64, const void*, i64, i64, i64, i64, const void*, int, const void*, int, i64, int,
                     int, int, int, i64, float, i64, i64, i64, i64, void*, i64, int, void*);
-  int64_t (*kv4_prompt_workspace)(i64, i64, int, int, int, int, i64);
+  int64_t (*kv4_prompt_workspace)(i64, i64, i64, int, int, int, int, i64);
   int (*kv4_prompt)(void*, const void*, const void*, i64, i64, const void*, int, const void*, int, const void*, i64, i64, i64, i64, const void*,
                     int, const void*, int, i64, i64, i64, int, int, int, int, i64, float, i64, i64, i64, i64, void*, i64, int, void*);
   int (*slot_maps)(void*, void*, void*, void*, const void*, int, const void*, int, const void*, int, const void*, int, void*, i64, i64, i64,
@@ -522,7 +522,7 @@ PyObject* kv4_prompt(PyObject*, PyObject* const* a, Py_ssize_t count) {
   const int sw = indices(*start, batch), fw = indices(*fresh, batch), rw = indices(*req, batch), lw = indices(*len, batch);
   if (!sw || !fw || !rw || !lw || !cache4(*kv, n[2], d, n[3]) || hq % n[2] != 0) return none();
   if (given != q && (given->scalar_type() != q->scalar_type() || given->sizes() != q->sizes() || given->stride(2) != 1)) return none();
-  const i64 bytes = abi.kv4_prompt_workspace(batch, tokens, (int)hq, (int)n[2], (int)d, (int)n[3], n[1]);
+  const i64 bytes = abi.kv4_prompt_workspace(batch, tokens, n[0], (int)hq, (int)n[2], (int)d, (int)n[3], n[1]);
   at::Tensor out, ws;
   int rc;
   {

@@ -7,12 +7,21 @@
 //   warps 0, 1    tensor-core issuers: the scores S = Q K^T, and O += P V (A = P from tensor memory)
 //   warps 2, 3    the head's bytes of the cache rows, through the request table, by asynchronous copies into a ring of units (64 keys of K
 //                 or of V), a tile ahead
-//   warps 4 - 7   codes to halves minimum + scale * code in the operands' swizzled layout.  A word of eight codes turns into one 16-byte
+//   warps 4 - 11  codes to halves minimum + scale * code in the operands' swizzled layout.  A word of eight codes turns into one 16-byte
 //                 chunk in the order 0 4 1 5 2 6 3 7: with the queries stored in the same order the scores are the same, and the
 //                 outputs' order is undone at the end.
-//   warps 8 - 15  softmax, a thread to a row of either tile: the row's scores from tensor memory once, P written back, the output rescaled
+//   warps 12 - 19 softmax, a thread to a row of either tile: the row's scores from tensor memory once, P written back, the output rescaled
 //                 where the running maximum rises by more than 2^8 (both by one factor, hence exact)
-// Tensor memory: S0 S1 (64 keys each) | P0 P1 | O0 | O1.
+// Tensor memory: two buffers of 64 keys' scores for either tile, whose place the probabilities take | O0 | O1.  A softmax thread works on
+// one half of a key tile (its registers suffice for that beside eight converting warps) while the products of the other run.  A step
+// (a key tile of both row tiles) takes about 5000 cycles, bound by the conversion's and the softmax's instructions together; its four
+// products would take 2050.
+//
+// READY: where five row blocks or more read a key tile, a kernel before this one converts each tile once into the workspace, as the
+// tensor cores read it, and one warp fetches whole operands; the softmax warps then have registers for a whole row of 128 scores
+// (S for both tiles in turn | P0 P1 | O0 | O1), which they free before the exponentials.  A step takes 2800 cycles, of which 2050 are
+// the exponentials' issue alone.  The kernel before takes 6 us for 8000 keys of 8 heads.
+// 512 tokens over 7500, 32 / 8 heads: 89 us (101 the other way), 256: 66 both ways, 128: 59 (54).
 // The operands are halves for both activation types: elements are rounded to 11 bits (as the 16-bit cache of an fp16 model rounds
 // them), which for bf16 models are three bits more than reading the cache into their type would leave; elements of those beyond 65504
 // count as 65504.  Queries of bf16 models are scaled by a power of two per row.  Probabilities are rounded to 11 bits, as in
@@ -29,7 +38,7 @@
 namespace kv4p {
 
 constexpr int kBM = 128, kBN = 128, kRows = 2 * kBM;
-constexpr int kThreads = 640, kConvert = 256, kKStages = 2, kVStages = 2, kSegs = 4;
+constexpr int kThreads = 640, kConvert = 256, kReadyThreads = 384, kKStages = 2, kVStages = 2, kSegs = 4;
 constexpr int kUnits = 5, kUnitKeys = 64, kUnitPitch = 96;   // pitch: rows of four neighbours in different banks
 constexpr int kMaxBatch = 128;                    // sequences of a launch (their sizes lie in shared memory)
 constexpr int kMinSteps = 2;                      // key tiles of a share: below that the parts cost more than the tiles
@@ -46,6 +55,7 @@ struct Params {
   int64_t total, max_new, most;
   float scale_log2;
   float* ws_o; float2* ws_ml; int2* ws_info; int4* ws_item;
+  uint8_t* ready; int4* ready_nan; int ready_tiles;   // operands made before: tiles [sequence][kv head][ready_tiles], K's image and V's
 };
 
 // a sequence: its m new tokens begin at row `start` of q, the first stands at position ctx, keys below `keys` are cached
@@ -85,11 +95,13 @@ __device__ __forceinline__ int block_steps(const Params& p, const Seq& s, int rb
 struct __align__(16) Ctl {
   uint64_t q_full[2], k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
   uint64_t raw_full[kUnits], raw_empty[kUnits];
-  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], seg_done[kSegs];
+  uint64_t s_free;                                // READY: one buffer for both tiles' scores
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], seg_done[kSegs];   // of either half of a tile's scores: a phase is a key tile
   int nan_at[kSegs][4];                           // first key whose value group is NaN
+  int8_t q_exp[2][kBM];                           // bf16: the power of two that a row of Q was divided by
   uint32_t tmem_base;
 };
-static_assert(sizeof(Ctl) <= 512, "control block");
+static_assert(sizeof(Ctl) <= 1024, "control block");
 
 // steps [j0, j1) of a row block
 struct Segment { int b, kvh, rb, j0, j1, steps, item; };
@@ -149,29 +161,33 @@ template <> struct Group<__nv_bfloat16> {
   }
 };
 
-template <typename T, int D, int GS>
-__global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p) {
+// READY: operands that a kernel before this one has made come as whole tiles, and there are no converting warps.
+template <typename T, int D, int GS, bool READY>
+__global__ void __launch_bounds__(READY ? kReadyThreads : kThreads, 1) kv4_prompt_kernel(const Params p) {
+  constexpr int kSoftmaxWarp = READY ? 4 : 12, kAll = READY ? kReadyThreads : kThreads;
   constexpr int DP = D < 64 ? 64 : D;             // a row of an operand is whole swizzle atoms of 64 halves
   constexpr int kTile = kBN * DP * 2, kHalf = kBN * 64 * 2, NG = D / GS;
+  constexpr int kN = READY ? kBN : kBN / 2, kParts = kBN / kN;     // keys of a product; products of a key tile
   extern __shared__ __align__(1024) uint8_t smem[];
   Ctl* ctl = reinterpret_cast<Ctl*>(smem);
   uint8_t* q_s = smem + 1024;
   uint8_t* k_ring = q_s + 2 * kTile;
   uint8_t* v_ring = k_ring + kKStages * kTile;
   uint8_t* raw_ring = v_ring + kVStages * kTile;
-  int* prefix = reinterpret_cast<int*>(raw_ring + kUnits * kUnitKeys * kUnitPitch);   // steps of the sequences before, [batch + 1]
+  int* prefix = reinterpret_cast<int*>(raw_ring + (READY ? 0 : kUnits * kUnitKeys * kUnitPitch));   // steps of the sequences before, [batch + 1]
   int* items = prefix + kMaxBatch + 1;            // row blocks (of all kv heads) before
   Seq* seqs = reinterpret_cast<Seq*>(items + kMaxBatch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.G;
 
   if (threadIdx.x == 0) {
+    mbar_init(&ctl->s_free, 4);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&ctl->q_full[t], 4); mbar_init(&ctl->s_full[t], 1); mbar_init(&ctl->p_full[t], 4); mbar_init(&ctl->pv_done[t], 1);
-      mbar_init(&ctl->s_free[t], 4);
+      mbar_init(&ctl->q_full[t], 4);
+      for (int h = 0; h < 2; ++h) { mbar_init(&ctl->s_full[t][h], 1); mbar_init(&ctl->p_full[t][h], 4); mbar_init(&ctl->pv_done[t][h], 1); }
     }
-    for (int s = 0; s < kKStages; ++s) { mbar_init(&ctl->k_full[s], kConvert / 32); mbar_init(&ctl->k_empty[s], 1); }
-    for (int s = 0; s < kVStages; ++s) { mbar_init(&ctl->v_full[s], kConvert / 32); mbar_init(&ctl->v_empty[s], 1); }
+    for (int s = 0; s < kKStages; ++s) { mbar_init(&ctl->k_full[s], READY ? 1 : kConvert / 32); mbar_init(&ctl->k_empty[s], 1); }
+    for (int s = 0; s < kVStages; ++s) { mbar_init(&ctl->v_full[s], READY ? 1 : kConvert / 32); mbar_init(&ctl->v_empty[s], 1); }
     for (int s = 0; s < kUnits; ++s) { mbar_init(&ctl->raw_full[s], 64); mbar_init(&ctl->raw_empty[s], kConvert / 32); }
     for (int s = 0; s < kSegs; ++s) mbar_init(&ctl->seg_done[s], 8);
     mbar_fence_init();
@@ -184,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
   pdl_wait_prior();                               // lengths, table, cache, q are upstream data
 
   // ---- steps and row blocks per sequence (a warp each), then their sums ----
-  for (int b = warp; b < p.batch; b += kThreads / 32) {
+  for (int b = warp; b < p.batch; b += kAll / 32) {
     const Seq s = sequence(p, b);
     const int nb = row_blocks(p, s);
     int n = 0;
@@ -265,22 +281,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp < 2) {
       // ===================== tensor-core issuers: warp 0 the scores, warp 1 P V =====================
-      constexpr uint32_t idesc_s = umma_idesc(1u, 0u, 0u, 0u, 0u, kBM, kBN / 2);
+      // Halves of a tile's scores alternate between its two buffers, and the probabilities take their place there: a buffer is written
+      // again when P V of the half that was in it is done, half a tile after it was asked for.
+      constexpr uint32_t idesc_s = umma_idesc(1u, 0u, 0u, 0u, 0u, kBM, kN);
       constexpr uint32_t idesc_o = umma_idesc(1u, 0u, 0u, 0u, 1u, kBM, DP);
       int ring = 0;
-      uint32_t phase = 0, free_phase = 3, q_phase = 0, p_phase = 0;   // a bit to a tile
+      uint32_t phase = 0, q_phase = 0, par = 0, used = 0;   // a bit to a tile: of its Q, of its key tiles; whether it had one
       while (next(seg, seq)) {
-        const int nt[2] = {key_tiles(p, seq, seg.rb, 0), key_tiles(p, seq, seg.rb, 1)};
+        const int nt0 = key_tiles(p, seq, seg.rb, 0), nt1 = key_tiles(p, seq, seg.rb, 1);
         for (int j = seg.j0; j < seg.j1; ++j) {
           kv4_wait(warp == 0 ? &ctl->k_full[ring] : &ctl->v_full[ring], phase);
-          if (warp == 0) {
 #pragma unroll 1
-            for (int x = 0; x < 4; ++x) {
-              const int t = x & 1, h = x >> 1;
-              if (j >= (t ? nt[1] : nt[0])) continue;
+          for (int x = 0; x < 2 * kParts; ++x) {
+            const int t = x & 1, h = x >> 1;
+            if (j >= (t ? nt1 : nt0)) continue;
+            const bool last = h == kParts - 1 && (t == 1 || j >= nt1);    // the key tile's last reader
+            if (warp == 0) {
               if (h == 0 && j == seg.j0) { kv4_wait(&ctl->q_full[t], q_phase >> t & 1u); q_phase ^= 1u << t; }
-              kv4_wait(&ctl->s_free[t], free_phase >> t & 1u);
-              free_phase ^= 1u << t;
+              if (READY) {
+                if (used) { kv4_wait(&ctl->s_free, par); par ^= 1u; }      // the product before is in its threads' registers
+                used = 1u;
+              } else {
+                if (used >> t & 1u) kv4_wait(&ctl->pv_done[t][h], (par >> t & 1u) ^ 1u);   // of the key tile before
+                if (h == 1) { used |= 1u << t; par ^= 1u << t; }
+              }
               tc_fence_after();
               if (elect_one()) {
                 const uint64_t q_desc = umma_desc_sw128_kmajor(smem_u32(q_s + t * kTile));
@@ -288,36 +312,62 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
                   const uint64_t off = (uint64_t)(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4);
-                  umma_f16(tmem_base + (uint32_t)t * 64u, q_desc + off, k_desc + off, idesc_s, kk ? 1u : 0u);
+                  umma_f16(tmem_base + (uint32_t)(READY ? 0 : t * 128 + h * 64), q_desc + off, k_desc + off, idesc_s, kk ? 1u : 0u);
                 }
-                if (h == 1 && (t == 1 || j >= nt[1])) tc_commit(&ctl->k_empty[ring]);   // the key tile's last reader
-                tc_commit(&ctl->s_full[t]);
+                if (last) tc_commit(&ctl->k_empty[ring]);
+                tc_commit(&ctl->s_full[t][h]);
               }
-              __syncwarp();
-            }
-          } else {
-#pragma unroll 1
-            for (int t = 0; t < 2; ++t) {
-              if (j >= (t ? nt[1] : nt[0])) continue;
-              kv4_wait(&ctl->p_full[t], p_phase >> t & 1u);
-              p_phase ^= 1u << t;
+            } else {
+              kv4_wait(&ctl->p_full[t][h], par >> t & 1u);
+              if (h == kParts - 1) par ^= 1u << t;
               tc_fence_after();
               if (elect_one()) {
-                const uint32_t v_addr = smem_u32(v_ring + ring * kTile);
+                const uint32_t v_addr = smem_u32(v_ring + ring * kTile + h * (kBN / 2) * 128);
 #pragma unroll
-                for (int kk = 0; kk < kBN / 16; ++kk) {
+                for (int kk = 0; kk < kN / 16; ++kk) {
                   // 16 keys per step = two 8-row groups of 1024 B; elements 64 .. 127 are one LBO away
                   const uint64_t v_desc = umma_desc_sw128_mnmajor(v_addr + kk * 2048, kHalf, 1024);
-                  umma_ts(tmem_base + 256u + (uint32_t)t * 128u, tmem_base + 128u + (uint32_t)t * 64u + kk * 8, v_desc, idesc_o,
-                          (j > seg.j0 || kk) ? 1u : 0u);
+                  umma_ts(tmem_base + 256u + (uint32_t)t * 128u, tmem_base + (uint32_t)(READY ? 128 + t * 64 : t * 128 + h * 64) + kk * 8, v_desc, idesc_o,
+                          (j > seg.j0 || h || kk) ? 1u : 0u);
                 }
-                if (t == 1 || j >= nt[1]) tc_commit(&ctl->v_empty[ring]);
-                tc_commit(&ctl->pv_done[t]);
+                if (last) tc_commit(&ctl->v_empty[ring]);
+                tc_commit(&ctl->pv_done[t][h]);
               }
-              __syncwarp();
             }
+            __syncwarp();
           }
           if (++ring == (warp == 0 ? kKStages : kVStages)) { ring = 0; phase ^= 1u; }
+        }
+      }
+    } else if (READY) {
+      // ===================== operands' tiles =====================
+      int ks = 0, vs = 0, nseg = 0;
+      uint32_t kp = 1, vp = 1;
+      for (; warp == 2 && next(seg, seq); ++nseg) {
+        const int slot = nseg % kSegs;
+        if (nseg >= kSegs) kv4_wait(&ctl->seg_done[slot], (uint32_t)(nseg / kSegs - 1) & 1u);
+        if (lane < 4) ctl->nan_at[slot][lane] = INT_MAX;
+        __syncwarp();
+        int64_t at = ((int64_t)seg.b * p.Hkv + seg.kvh) * p.ready_tiles + seg.j0;
+        for (int j = seg.j0; j < seg.j1; ++j, ++at) {
+          const uint8_t* tile = p.ready + at * 2 * kTile;
+          const int nan = lane < NG ? __ldcg(reinterpret_cast<const int*>(p.ready_nan + at) + lane) : INT_MAX;
+          kv4_wait(&ctl->k_empty[ks], kp);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&ctl->k_full[ks], kTile);
+            bulk_g2s(k_ring + ks * kTile, tile, kTile, &ctl->k_full[ks]);
+          }
+          __syncwarp();
+          if (++ks == kKStages) { ks = 0; kp ^= 1u; }
+          if (nan != INT_MAX) atomicMin(&ctl->nan_at[slot][lane], nan);
+          __syncwarp();
+          kv4_wait(&ctl->v_empty[vs], vp);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&ctl->v_full[vs], kTile);
+            bulk_g2s(v_ring + vs * kTile, tile + kTile, kTile, &ctl->v_full[vs]);
+          }
+          __syncwarp();
+          if (++vs == kVStages) { vs = 0; vp ^= 1u; }
         }
       }
     } else {
@@ -359,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
-  } else if (warp < 12) {
+  } else if (warp < kSoftmaxWarp) {
     // ===================== codes to operands =====================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     constexpr int NWD = D == 128 ? 2 : 1;         // words of a row and side that a thread takes (eight threads to a row)
@@ -426,14 +476,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    if (READY) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");   // 12 warps x 168 at launch >= 4 x 56 + 8 x 216
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     // ===================== softmax: thread = query row = TMEM lane of tile t =====================
-    const int t = (warp - 12) >> 2, quad = warp & 3;
+    const int t = (warp - kSoftmaxWarp) >> 2, quad = warp & 3;
     const int row = quad * 32 + lane;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quad * 32) << 16);
-    const uint32_t pb = lane_base + 128u + (uint32_t)t * 64u, ob = lane_base + 256u + (uint32_t)t * 128u;
+    const uint32_t sb = lane_base + (READY ? 0u : (uint32_t)t * 128u), ob = lane_base + 256u + (uint32_t)t * 128u;
     constexpr float kLazy = 8.0f;                 // log2 units: rescale only when a tile exceeds m_used by 2^8
-    uint32_t s_phase = 0, pv_phase = 0;
+    uint32_t par = 0;                             // of the key tiles
     int nseg = 0;
     for (; next(seg, seq); ++nseg) {
       const int nt = key_tiles(p, seq, seg.rb, t), j_end = nt < seg.j1 ? nt : seg.j1;
@@ -445,77 +496,104 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
       const bool whole = seg.j0 == 0 && seg.j1 == seg.steps;
       float m_used = -INFINITY, l_run = 0.f;      // m_used: the maximum the accumulated P / O / l are scaled by
       if (j_end > seg.j0) {
-        // the row of Q, in the operands' order
+        // The tile's rows of Q, in the operands' order: neighbouring threads take a row's 16-byte pieces, all asked for
+        // before the first is converted (a row to a thread took 7 us, this 4).
         float scale = p.scale_log2;
         {
-          const T* src = reinterpret_cast<const T*>(p.q) + place * p.q_ts + (int64_t)(live ? head : 0) * p.q_hs;
-          uint32_t w[D / 2];
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (live) {
+          constexpr int kLanes = D / 8, kPass = 128 / kLanes;      // pieces of a row; rows at a time
+          const int tid = quad * 32 + lane, c = tid % kLanes;
+          const int y0 = tid / kLanes, yr = seg.rb * kRows + t * kBM + y0;
+          uint8_t* dst = q_s + t * kTile + (c >> 3) * kHalf + y0 * 128 + (((c & 7) ^ (y0 & 7)) << 4);
+          {
+            const int by = over_G(p, kPass), on = kPass - by * G;  // tokens and heads from a row to the next
+            int yt = over_G(p, yr), yh = yr - yt * G;
+            const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(seq.start + yt) * p.q_ts + (int64_t)(seg.kvh * G + yh) * p.q_hs + c * 8;
+            const int64_t step = by * p.q_ts + on * p.q_hs, wrap = p.q_ts - G * p.q_hs;
+#pragma unroll 2
+            for (int i = 0; i < kBM / kPass; ++i) {
+              const bool live_row = yt < seq.m;
+              const T* from = live_row ? src : reinterpret_cast<const T*>(p.q);
               if (p.q_vec) {
-                x = *reinterpret_cast<const uint4*>(src + c * 8);
+                copy_async<16>(dst + i * kPass * 128, from, live_row);
               } else {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(src + c * 8);
-                x = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+#pragma unroll 1
+                for (int e = 0; e < 8; ++e)
+                  reinterpret_cast<uint16_t*>(dst + i * kPass * 128)[e] = live_row ? reinterpret_cast<const uint16_t*>(from)[e] : (uint16_t)0;
+              }
+              yt += by;
+              yh += on;
+              src += step;
+              if (yh >= G) { yh -= G; ++yt; src += wrap; }
+            }
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          constexpr int kTogether = 4;
+#pragma unroll 1
+          for (int i = 0; i < kBM / kPass; i += kTogether) {       // in place: a thread's own pieces
+            uint4 x[kTogether];
+#pragma unroll
+            for (int k = 0; k < kTogether; ++k) x[k] = *reinterpret_cast<const uint4*>(dst + (i + k) * kPass * 128);
+            if (std::is_same<T, __nv_bfloat16>::value) {
+              float big[kTogether];
+#pragma unroll
+              for (int k = 0; k < kTogether; ++k) {
+                const uint32_t* w = &x[k].x;
+                big[k] = 0.f;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) big[k] = max3(big[k], fabsf(__uint_as_float(w[n] << 16)), fabsf(__uint_as_float(w[n] & 0xffff0000u)));
+              }
+#pragma unroll
+              for (int o = 1; o < kLanes; o <<= 1)
+#pragma unroll
+                for (int k = 0; k < kTogether; ++k) big[k] = fmaxf(big[k], __shfl_xor_sync(0xffffffffu, big[k], o));
+#pragma unroll
+              for (int k = 0; k < kTogether; ++k) {
+                uint32_t* w = &x[k].x;
+                int e = 8 - ((int)(__float_as_uint(big[k]) >> 23) - 127);
+                if (!(big[k] < INFINITY) || big[k] == 0.f) e = 0;
+                e = e < -100 ? -100 : e > 100 ? 100 : e;
+                const float up = __int_as_float((e + 127) << 23);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) w[n] = pack2<__half>(__uint_as_float(w[n] << 16) * up, __uint_as_float(w[n] & 0xffff0000u) * up);
+                if (c == 0) ctl->q_exp[t][y0 + (i + k) * kPass] = (int8_t)e;
               }
             }
-            w[c * 4] = x.x; w[c * 4 + 1] = x.y; w[c * 4 + 2] = x.z; w[c * 4 + 3] = x.w;
+#pragma unroll
+            for (int k = 0; k < kTogether; ++k)
+              *reinterpret_cast<uint4*>(dst + (i + k) * kPass * 128) = make_uint4(
+                  __byte_perm(x[k].x, x[k].z, 0x5410), __byte_perm(x[k].x, x[k].z, 0x7632), __byte_perm(x[k].y, x[k].w, 0x5410), __byte_perm(x[k].y, x[k].w, 0x7632));
           }
-          if (std::is_same<T, __nv_bfloat16>::value) {
-            float big = 0.f;
-#pragma unroll
-            for (int c = 0; c < D / 2; ++c)
-              big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w[c] << 16)), fabsf(__uint_as_float(w[c] & 0xffff0000u))));
-            int e = 8 - ((int)(__float_as_uint(big) >> 23) - 127);
-            if (!(big < INFINITY) || big == 0.f) e = 0;
-            e = e < -100 ? -100 : e > 100 ? 100 : e;
-            const float up = __int_as_float((e + 127) << 23);
-            scale *= __int_as_float((127 - e) << 23);
-#pragma unroll
-            for (int c = 0; c < D / 2; ++c)
-              w[c] = pack2<__half>(__uint_as_float(w[c] << 16) * up, __uint_as_float(w[c] & 0xffff0000u) * up);
-          }
-          uint8_t* dst = q_s + t * kTile + row * 128;
-#pragma unroll
-          for (int c = 0; c < DP / 8; ++c) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (c < D / 8) {
-              const uint32_t* y = w + (c < D / 8 ? c : 0) * 4;
-              x = make_uint4(__byte_perm(y[0], y[2], 0x5410), __byte_perm(y[0], y[2], 0x7632), __byte_perm(y[1], y[3], 0x5410),
-                             __byte_perm(y[1], y[3], 0x7632));
-            }
-            *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalf + (((c & 7) ^ (row & 7)) << 4)) = x;
+          if (D < DP) {                                            // the atom's other half
+            for (int i = tid; i < kBM * 4; i += 128)
+              *reinterpret_cast<uint4*>(q_s + t * kTile + (i >> 2) * 128 + ((((i & 3) + 4) ^ ((i >> 2) & 7)) << 4)) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
-          __syncwarp();
+          asm volatile("bar.sync %0, 128;" ::"r"(3 + t) : "memory");
+          if (std::is_same<T, __nv_bfloat16>::value) scale *= __int_as_float((127 - (int)ctl->q_exp[t][row]) << 23);
           if (lane == 0) mbar_arrive(&ctl->q_full[t]);
         }
         const int pos = seq.ctx + token, see = live ? (pos < seq.keys - 1 ? pos : seq.keys - 1) : -1;   // last key that counts
         const int see_all = __reduce_min_sync(0xffffffffu, live ? see : INT_MAX);
 
-        // The row's scores come in two halves of 64, for which a thread's registers suffice beside eight converting warps, and a tile's
-        // columns are free for the next half once they are read: the products of one half run under the exponentials of the other.
-        // Either may raise the maximum; the second one then rescales the first one's probabilities too (rarely).
         // Loops stay rolled and the mask is a pass of its own: with copies for masked tiles and for either half the roles' code did not
         // fit into the instruction cache (6000 cycles a step, most of them waiting for instructions).
 #pragma unroll 1
         for (int j = seg.j0; j < j_end; ++j) {
           const bool masked = (j + 1) * kBN - 1 > see_all;
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            constexpr int kN = kBN / 2;
-            kv4_wait(&ctl->s_full[t], s_phase);
-            s_phase ^= 1u;
+          for (int h = 0; h < kParts; ++h) {
+            kv4_wait(&ctl->s_full[t][h], par);
             tc_fence_after();
+            const uint32_t buf = sb + (uint32_t)h * 64u;
             uint32_t sv[kN];
 #pragma unroll
-            for (int c = 0; c < kN; c += 32) tmem_ld_32x32b_x32(lane_base + (uint32_t)t * 64u + c, *reinterpret_cast<uint32_t(*)[32]>(sv + c));
+            for (int c = 0; c < kN; c += 32) tmem_ld_32x32b_x32(buf + c, *reinterpret_cast<uint32_t(*)[32]>(sv + c));
             tc_wait_ld();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->s_free[t]);
+            if (READY) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&ctl->s_free);
+            }
             if (masked) {
               const int limit = see - j * kBN - h * kN;            // key column i is visible iff i <= limit
 #pragma unroll
@@ -530,24 +608,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
             const bool grow = m_half > m_used + kLazy;             // at first m_used = -inf: true
             const float m_new = grow ? m_half : m_used;
             const float base = m_new == -INFINITY ? 0.f : m_new;   // nothing visible yet: avoid inf - inf
-            if (h == 0 && j > seg.j0) { kv4_wait(&ctl->pv_done[t], pv_phase); pv_phase ^= 1u; tc_fence_after(); }
+            if (READY && j > seg.j0) { kv4_wait(&ctl->pv_done[t][0], par ^ 1u); tc_fence_after(); }   // P's place is free, O rests
             if (__any_sync(0xffffffffu, grow)) {
               const float alpha = grow ? fast_exp2(m_used - base) : 1.0f;
               l_run *= alpha;
-              if (h == 1) {                                        // the first half's probabilities
-                tc_wait_st_();
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(pb, v);
-                tc_wait_ld();
-                const __half2 a2 = __float2half2_rn(alpha);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&v[i]), a2);
-                  v[i] = *reinterpret_cast<const uint32_t*>(&x);
-                }
-                tmem_st_32x32b_x32(pb, v);
-              }
-              if (j > seg.j0) {
+              if (j > seg.j0 || h) {
+                if (!READY) { kv4_wait(&ctl->pv_done[t][h ^ 1], h ? par : par ^ 1u); tc_fence_after(); }   // of the half before, the last one asked for
 #pragma unroll 1
                 for (int c = 0; c < DP; c += 32) {
                   uint32_t v[32];
@@ -574,19 +640,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
                 lsum2 = f32x2_add(lsum2, f32x2(p0, p1));
                 pk[i >> 1] = pack2<__half>(p0, p1);
               }
-              tmem_st_32x32b_x16(pb + h * (kN / 2) + (c >> 1), pk);
+              tmem_st_32x32b_x16((READY ? lane_base + 128u + (uint32_t)t * 64u : buf) + (c >> 1), pk);
             }
             float l0, l1;
             f32x2_split(lsum2, l0, l1);
             l_run += l0 + l1;
+            tc_wait_st_();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->p_full[t][h]);
           }
-          tc_wait_st_();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->p_full[t]);
+          par ^= 1u;
         }
-        kv4_wait(&ctl->pv_done[t], pv_phase);
-        pv_phase ^= 1u;
+        kv4_wait(&ctl->pv_done[t][kParts - 1], par ^ 1u);      // the last half's, and with it all before
         tc_fence_after();
         // columns are in the operands' order: of eight, 0 4 1 5 2 6 3 7
         const float inv = whole ? (l_run == 0.f ? 0.f : 1.0f / l_run) : 1.f;
@@ -639,6 +705,68 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Params p)
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem_base, 512);
+}
+
+// Operands of one tile of 128 keys of a kv head, as the tensor cores read them.  Where many row blocks read a tile, its codes are
+// converted once here instead of beside the products of each.
+template <typename T, int D, int GS>
+__global__ void __launch_bounds__(256, 6) kv4_prompt_ready_kernel(const Params p) {
+  pdl_prologue();
+  constexpr int DP = D < 64 ? 64 : D, kTile = kBN * DP * 2, kHalf = kBN * 64 * 2, NG = D / GS, NWD = D == 128 ? 2 : 1, NI = kBN / 32;
+  __shared__ int nan_at[4];
+  const int tile = blockIdx.x >> 1, side = blockIdx.x & 1, kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, l = tid & 7, kq = tid >> 3;
+  const Seq s = sequence(p, b);
+  if (s.m == 0 || tile * kBN >= s.keys) {
+    // a sequence that sees nothing takes one step for its zeros: of zero operands
+    if (s.m == 0 || tile > 0) return;
+  }
+  if (tid < 4) nan_at[tid] = INT_MAX;
+  __syncthreads();
+  uint32_t w[NI][NWD], g[NI][NWD];
+  int row[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int key = tile * kBN + i * 32 + kq;
+    row[i] = -1;
+    if (key < s.keys && l < D / 8) {
+      const int r = ld_upstream(p.table + (int64_t)s.req * p.tab_rs + (int64_t)key * p.tab_cs);
+      row[i] = r >= 0 && r < p.max_tokens ? r : 0;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int k = 0; k < NWD; ++k) {
+      w[i][k] = g[i][k] = 0u;
+      if (row[i] >= 0) {
+        const uint32_t* head = reinterpret_cast<const uint32_t*>(p.cache + (int64_t)row[i] * p.row_stride + (int64_t)kvh * kv4::head_bytes(D, GS));
+        w[i][k] = __ldcg(head + side * (D / 8) + k * 8 + l);
+        g[i][k] = __ldcg(head + D / 4 + side * NG + (k * 8 + l) * 8 / GS);
+      }
+    }
+  const int64_t at = ((int64_t)b * p.Hkv + kvh) * p.ready_tiles + tile;
+  uint8_t* to = p.ready + (at * 2 + side) * kTile + kq * 128 + ((l ^ (kq & 7)) << 4);
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int k = 0; k < NWD; ++k) {
+      const uint32_t x = g[i][k];
+      uint4 v;
+      if ((((x & 0x7fff7fffu) + Group<T>::kAdd) & 0x80008000u) == 0u) {
+        v = to_halves(w[i][k], Group<T>::both(x, 0), Group<T>::both(x, 1));
+      } else {
+        float2 f = kv4::scale_min<T>(x);
+        if (side == 1 && (f.x != f.x || f.y != f.y)) {
+          f = make_float2(0.f, 0.f);
+          atomicMin(&nan_at[(k * 8 + l) * 8 / GS], tile * kBN + i * 32 + kq);
+        }
+        v = to_halves_wide(w[i][k], f.x, f.y);
+      }
+      *reinterpret_cast<uint4*>(to + k * kHalf + i * 32 * 128) = v;
+    }
+  if (side == 0) return;
+  __syncthreads();
+  if (tid < 4) reinterpret_cast<int*>(p.ready_nan + at)[tid] = nan_at[tid];
 }
 
 // Row blocks that several CTAs met in.  Bound by latency: a warp asks for the parts of its four rows together, and lengths and notes
@@ -708,29 +836,49 @@ __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(const Params p) {
   }
 }
 
-struct Plan { int grid, smem; int64_t items, rows, steps; };
+struct Plan { int grid, smem, ready_tiles; int64_t items, rows, steps, ready_bytes; };   // ready_tiles 0: operands are made beside the products
 
-Plan make_plan(int64_t batch, int64_t total, int G, int Hkv, int D, int64_t max_len) {
+// Row blocks of the longest portion from which on operands are made ready.  1 x 256 / 320 / 384 / 512 tokens (4 to 8 blocks) over 7500:
+// 66.5 / 73.6 / 77.6 / 90.6 us ready, 66.2 / 74.9 / 82.2 / 100.8 converted beside the products; 6 x 200 / 290 / 400 over 1200:
+// 58.5 / 77.8 / 87.4 and 56.8 / 80.3 / 94.0.
+constexpr int kReadyBlocks = 5;
+// Their room in the workspace at most: 65536 keys of 8 heads.  It grows with batch * max_seq_len, of which ragged steps use a part.
+constexpr int64_t kReadyMost = 256ll << 20;
+
+Plan make_plan(int64_t batch, int64_t total, int64_t max_new, int G, int Hkv, int D, int64_t max_len) {
   Plan pl;
   const int DP = D < 64 ? 64 : D;
-  const int64_t rows = batch < kMaxBatch ? batch : kMaxBatch;
-  pl.smem = 1024 + (2 + kKStages + kVStages) * kBN * DP * 2 + kUnits * kUnitKeys * kUnitPitch +
-            (2 * kMaxBatch + 1) * 4 + kMaxBatch * (int)sizeof(Seq);
+  const int64_t rows = batch < kMaxBatch ? batch : kMaxBatch, tiles = cdiv64(max_len > 0 ? max_len : 1, kBN);
+  const int lists = (2 * kMaxBatch + 1) * 4 + kMaxBatch * (int)sizeof(Seq);
   pl.items = (cdiv64(total * G, kRows) + rows) * Hkv;
-  pl.steps = pl.items * cdiv64(max_len > 0 ? max_len : 1, kBN);
+  pl.steps = pl.items * tiles;
   const int64_t worth = cdiv64(pl.steps, kMinSteps);
   pl.grid = (int)(worth < b2l_num_sms() ? worth : b2l_num_sms());
   if (pl.grid < 1) pl.grid = 1;
   pl.rows = 2ll * pl.grid * kRows;
+  // A tile is read by every row block that sees it: converted once for all of them where they are several, with room for the tiles
+  // of the bounds.
+  const int64_t tile = 2ll * kBN * DP * 2, blocks = cdiv64((max_new < total ? max_new : total) * G, kRows);
+  const bool ready = blocks >= kReadyBlocks && rows * Hkv * tiles <= kReadyMost / tile;
+  pl.ready_tiles = ready ? (int)tiles : 0;
+  pl.ready_bytes = ready ? rows * Hkv * tiles * (tile + 16) : 0;
+  pl.smem = 1024 + (2 + kKStages + kVStages) * kBN * DP * 2 + (ready ? 0 : kUnits * kUnitKeys * kUnitPitch) + lists;
   return pl;
 }
+// partial rows, notes, sequences, each from a multiple of 16 bytes on; the ready operands first
+int64_t workspace_for(const Plan& pl, int D) { return pl.ready_bytes + pl.rows * (D + 2) * 4 + (pl.items + 1) / 2 * 16 + (int64_t)kMaxBatch * 16; }
 
 template <typename T, int D, int GS>
 int launch(const Params& p, const Plan& pl, cudaStream_t st) {
-  static int configured[64] = {0};
-  auto kern = kv4_prompt_kernel<T, D, GS>;
-  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured));
-  b2l_launch(kern, dim3((unsigned)pl.grid), dim3(kThreads), (size_t)pl.smem, st, p);
+  static int configured[2][64] = {{0}};
+  const bool ready = pl.ready_tiles > 0;
+  auto kern = ready ? kv4_prompt_kernel<T, D, GS, true> : kv4_prompt_kernel<T, D, GS, false>;
+  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured[ready]));
+  if (ready) {
+    b2l_launch(kv4_prompt_ready_kernel<T, D, GS>, dim3(2u * (unsigned)pl.ready_tiles, (unsigned)p.Hkv, (unsigned)p.batch), dim3(256), (size_t)0, st, p);
+    B2L_LAUNCH_CHECK();
+  }
+  b2l_launch(kern, dim3((unsigned)pl.grid), dim3(ready ? kReadyThreads : kThreads), (size_t)pl.smem, st, p);
   B2L_LAUNCH_CHECK();
   const int64_t x = cdiv64(p.max_new * p.G, 32);
   b2l_launch(kv4_prompt_merge_kernel<T, D>, dim3((unsigned)x, (unsigned)p.Hkv, (unsigned)p.batch), dim3(256), (size_t)0, st, p);
@@ -740,12 +888,11 @@ int launch(const Params& p, const Plan& pl, cudaStream_t st) {
 
 }  // namespace kv4p
 
-extern "C" int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64_t total_tokens, int num_q_heads, int num_kv_heads,
+extern "C" int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64_t total_tokens, int64_t max_new_len, int num_q_heads, int num_kv_heads,
                                                             int head_dim, int group, int64_t max_seq_len) {
   if (batch <= 0 || total_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || !kv4::shape_ok(head_dim, group))
     return 0;
-  const kv4p::Plan pl = kv4p::make_plan(batch, total_tokens, num_q_heads / num_kv_heads, num_kv_heads, head_dim, max_seq_len);
-  return pl.rows * (head_dim + 2) * 4 + pl.items * 8 + (int64_t)kv4p::kMaxBatch * 16 + 16;
+  return kv4p::workspace_for(kv4p::make_plan(batch, total_tokens, max_new_len, num_q_heads / num_kv_heads, num_kv_heads, head_dim, max_seq_len), head_dim);
 }
 
 extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* cache, int64_t cache_row_stride, int64_t max_tokens,
@@ -772,10 +919,11 @@ extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* ca
                   max_new_len >= 0 && max_new_len < (1ll << 30) && max_seq_len < (1ll << 30), "%s: bad shape", what);
   if (batch == 0 || total_tokens == 0 || max_new_len == 0) return B2L_OK;
   const int G = num_q_heads / num_kv_heads;
-  const Plan pl = make_plan(batch, total_tokens, G, num_kv_heads, head_dim, max_seq_len);
+  const int64_t most = max_seq_len < table_width ? max_seq_len : table_width;
+  const Plan pl = make_plan(batch, total_tokens, max_new_len, G, num_kv_heads, head_dim, max_seq_len);
   B2L_REQUIRE(pl.steps < (1ll << 31) && total_tokens * G < (1ll << 31), "%s: too many tokens", what);
   B2L_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
-                  workspace_bytes >= b2l_flash_attention_int4_workspace_bytes(batch, total_tokens, num_q_heads, num_kv_heads, head_dim, group, max_seq_len),
+                  workspace_bytes >= workspace_for(pl, head_dim),
               "%s: workspace too small", what);
   Params p;
   p.q = q; p.q_ts = q_tok_stride; p.q_hs = q_head_stride;
@@ -787,13 +935,16 @@ extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* ca
   p.start_w = start_width; p.fresh_w = new_width; p.req_w = req_width; p.len_w = len_width;
   p.Hkv = num_kv_heads; p.G = G; p.by_G = G > 1 ? ~0ull / G + 1 : 0;
   p.total = total_tokens; p.max_new = max_new_len < total_tokens ? max_new_len : total_tokens;
-  p.most = max_seq_len < table_width ? max_seq_len : table_width;
-  if (p.most < 0) p.most = 0;
+  p.most = most < 0 ? 0 : most;
   p.scale_log2 = qk_scale * 1.4426950408889634f;
-  p.ws_o = (float*)workspace;
+  char* ws = (char*)workspace;
+  p.ready = (uint8_t*)ws;
+  p.ready_tiles = pl.ready_tiles;
+  p.ready_nan = (int4*)(ws + pl.ready_bytes / (2ll * kBN * (head_dim < 64 ? 64 : head_dim) * 2 + 16) * (2ll * kBN * (head_dim < 64 ? 64 : head_dim) * 2));
+  p.ws_o = (float*)(ws + pl.ready_bytes);
   p.ws_ml = (float2*)(p.ws_o + pl.rows * head_dim);
   p.ws_info = (int2*)(p.ws_ml + pl.rows);
-  p.ws_item = (int4*)(((uintptr_t)(p.ws_info + pl.items) + 15) & ~(uintptr_t)15);
+  p.ws_item = (int4*)((char*)p.ws_info + (pl.items + 1) / 2 * 16);
   cudaStream_t st = (cudaStream_t)stream;
   for (int64_t b0 = 0; b0 < batch; b0 += kMaxBatch) {
     p.batch = (int)(batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch);

@@ -242,7 +242,7 @@ def _flash_attention_int4(q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_
     if batch == 0 or tokens == 0:
         return out
     max_len = int(max_actual_seq_len)
-    nbytes = lib().b2l_flash_attention_int4_workspace_bytes(batch, tokens, hq, num_kv_heads, d, group_size, max_len)
+    nbytes = lib().b2l_flash_attention_int4_workspace_bytes(batch, tokens, int(max_new_len), hq, num_kv_heads, d, group_size, max_len)
     ws = workspace(max(nbytes, 16), q.device)
     check(lib().b2l_flash_attention_int4(
         out.data_ptr(), q.data_ptr(), address, stride, rows, b_start_loc.data_ptr(), index_width(b_start_loc, "b_start_loc"),

@@ -105,9 +105,10 @@ def test_large_and_small_values(dtype, scale_q, scale_k, scale_v):
     _check(_call(step, 2, 64, 0.088), step, 2, 64, 0.088)
 
 
-def test_elements_past_the_range_of_halves():
-    """Of a bf16 cache: as 65504; of an fp16 cache, a group whose rounded steps end past it, as its largest."""
-    step = _run([4], [40], 2, 1, 64, 64, torch.bfloat16)
+@pytest.mark.parametrize("wide", [False, True])
+def test_elements_past_the_range_of_halves(wide):
+    """Of a bf16 cache: as 65504.  wide: beside a long portion, whose operands are made before."""
+    step = _run([4, 600] if wide else [4], [40, 700] if wide else [40], 2, 1, 64, 64, torch.bfloat16)
     q, rows, start, new, table, req, n = step
     k, v, _, _ = O.values(rows, 1, 64, 64, torch.bfloat16)
     v = v.bfloat16()
@@ -116,15 +117,17 @@ def test_elements_past_the_range_of_halves():
     step = (q, O.rows_of(k.bfloat16(), v, 64), start, new, table, req, n)
     out = _call(step, 1, 64, 0.1)
     assert torch.isfinite(out).all()
+    q, out = q[:4], out[:4]
     v[at, 0] = v[at, 0].clamp(-65504, 65504)
     w = torch.softmax(torch.einsum("mhd,nd->hmn", q.double(), O.values(step[1], 1, 64, 64, torch.bfloat16)[0][table[int(req[0]), :40].long(), 0]) * 0.1 +
                       torch.full((4, 40), -math.inf, device="cuda", dtype=torch.float64).triu(37), -1)
     assert ((out.double().abs().amax(-1) - w[:, :, 3].T * 65504).abs() <= 0.02 * w[:, :, 3].T * 65504 + 5).all()
 
 
-def test_a_value_that_is_nan_reaches_only_the_rows_that_see_it():
-    for where in (3, 60, 97):                       # before the new tokens, among them, the last one
-        q, rows, start, new, table, req, n = _run([48, 5], [98, 20], 8, 2, 128, 64, torch.float16)
+@pytest.mark.parametrize("count", [48, 200])             # a row block, and several with operands made before
+def test_a_value_that_is_nan_reaches_only_the_rows_that_see_it(count):
+    for where in (3, 60, count + 49):               # before the new tokens, among them, the last one
+        q, rows, start, new, table, req, n = _run([count, 5], [count + 50, 20], 8, 2, 128, 64, torch.float16)
         k, v, _, _ = O.values(rows, 2, 128, 64, torch.float16)
         k, v = k.half(), v.half()
         fine = _call((q, O.rows_of(k, v, 64), start, new, table, req, n), 2, 64, 0.1)
@@ -132,14 +135,15 @@ def test_a_value_that_is_nan_reaches_only_the_rows_that_see_it():
         out = _call((q, O.rows_of(k, v, 64), start, new, table, req, n), 2, 64, 0.1)
         nan = torch.zeros_like(out, dtype=torch.bool)
         first = max(0, where - 50)
-        nan[first:48, 4:, 64:] = True
+        nan[first:count, 4:, 64:] = True
         assert torch.equal(out.isnan(), nan), where
         # the NaN's group of the others is as before
         assert torch.equal(out[~nan], fine[~nan])
 
 
-def test_a_key_that_is_nan_reaches_only_the_rows_that_see_it():
-    q, rows, start, new, table, req, n = _run([48], [98], 8, 2, 128, 64, torch.bfloat16)
+@pytest.mark.parametrize("count", [48, 200])
+def test_a_key_that_is_nan_reaches_only_the_rows_that_see_it(count):
+    q, rows, start, new, table, req, n = _run([count], [count + 50], 8, 2, 128, 64, torch.bfloat16)
     k, v, _, _ = O.values(rows, 2, 128, 64, torch.bfloat16)
     k, v = k.bfloat16(), v.bfloat16()
     fine = _call((q, O.rows_of(k, v, 64), start, new, table, req, n), 2, 64, 0.1)
@@ -221,3 +225,29 @@ def test_a_single_token_meets_decode_attention():
     for i, (r, c) in enumerate(zip(req.tolist(), n.tolist())):
         _, error = O.prompt_attention(q[i:i + 1], rows[table[r, :c].long()], 4, 64, 0.088)
         assert O.within(b[i:i + 1], a[i:i + 1].double(), error + a[i:i + 1].double().abs() * 2.0**-11).all()
+
+
+def test_scales_that_are_not_positive_are_refused():
+    step = _run([2], [9], 2, 1, 64, 64, torch.float16)
+    for scale in (0.0, -0.1, math.inf, math.nan):
+        with pytest.raises(ValueError, match="qk_scale must be positive"):
+            _call(step, 1, 64, scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,heads,d,group", SHAPES)
+def test_long_portions_of_every_shape(hq, heads, d, group, dtype):
+    """Several row blocks to a sequence, whose operands are made before, beside short ones."""
+    new, lens = [300, 3, 0, 520], [301, 400, 9, 1111]
+    step = _run(new, lens, hq, heads, d, group, dtype, gap=1)
+    keep = _normal(*step[0].shape, dtype=dtype)
+    _check(_call(step, heads, group, d**-0.5, out=keep.clone(), max_len=1200), step, heads, group, d**-0.5, keep)
+
+
+def test_ready_operands_do_not_outgrow_their_limit():
+    """The same step under bounds that leave room for ready operands, and under bounds that do not."""
+    step = _run([300, 250], [1300, 600], 8, 2, 128, 64, torch.float16)
+    a = _call(step, 2, 64, 0.1)
+    b = _call(step, 2, 64, 0.1, max_len=1 << 20)
+    _check(a, step, 2, 64, 0.1)
+    _check(b, step, 2, 64, 0.1)
