@@ -7,7 +7,9 @@ while slots are free, prefill, then decode the running set every step) on top of
   token of every running request plus prompt PORTIONS of the requests still reading their prompt, under a token
   budget per step, so a long prompt never stalls the decoding requests;
 * the uniform rotary decoders keep the reference's scheme on the slot layout (``SlotBatch``): a new request's whole
-  prompt is one prefill step, the running set decodes together.
+  prompt is one prefill step, the running set decodes together;
+* over a 4-bit pool (``kv_cache_dtype="int4"``) they too read prompts in portions, in flat steps with the decoding
+  requests' tokens, while any prompt is left to read.
 
 Sampling is greedy through the library's ``argmax_rows`` kernel (the temperature-0 branch of
 lite_llama/engine/sampler.py).  Admission reserves a request's worst case (prompt + new tokens) against the KV pool,
@@ -132,13 +134,15 @@ class Engine:
         self.steps += 1
         return self._step_ragged() if self.runner.ragged_steps else self._step_slots()
 
-    def _step_ragged(self) -> list[tuple[int, int]]:
+    def _schedule(self) -> tuple[list[tuple[GenerationRequest, int, list[int]]], list[GenerationRequest], list[int]]:
+        """A flat step: ``(request, tokens it has cached, its next tokens)``, the requests to sample for and where in the
+        flat batch."""
         budget = self.max_step_tokens
         entries, samplers, want, at = [], [], [], 0
         # one token of every decoding request first, then prompt portions with what is left of the budget
         for req in self.running:
             if req.fed == len(req.prompt) and budget > 0:
-                entries.append((req.state, [req.output[-1]]))
+                entries.append((req, len(req.prompt) + len(req.output) - 1, [req.output[-1]]))
                 at += 1
                 budget -= 1
                 want.append(at - 1)
@@ -146,14 +150,16 @@ class Engine:
         for req in self.running:
             if req.fed < len(req.prompt) and budget > 0:
                 n = min(len(req.prompt) - req.fed, self.max_portion, budget)
-                entries.append((req.state, req.prompt[req.fed:req.fed + n]))
+                entries.append((req, req.fed, req.prompt[req.fed:req.fed + n]))
                 req.fed += n
                 at += n
                 budget -= n
                 if req.fed == len(req.prompt):
                     want.append(at - 1)
                     samplers.append(req)
-        logits = self.runner.forward_ragged(entries, want)
+        return entries, samplers, want
+
+    def _sample(self, logits: torch.Tensor, samplers: list[GenerationRequest]) -> list[tuple[int, int]]:
         produced: list[tuple[int, int]] = []
         if samplers:
             tokens = argmax_rows(logits).tolist()
@@ -161,8 +167,24 @@ class Engine:
                 self._accept(req, tok, produced)
         return produced
 
+    def _step_ragged(self) -> list[tuple[int, int]]:
+        entries, samplers, want = self._schedule()
+        return self._sample(self.runner.forward_ragged([(r.state, t) for r, _, t in entries], want), samplers)
+
+    def _step_portions(self) -> list[tuple[int, int]]:
+        entries, samplers, want = self._schedule()
+        dev = self.runner.device
+        pos = self._sb.begin_portions([r.slot for r, _, _ in entries], [c for _, c, _ in entries],
+                                      [len(t) for _, _, t in entries])
+        ids = torch.tensor([[t for _, _, toks in entries for t in toks]], dtype=torch.int64, device=dev)
+        # without anything to sample one position still ends the forward
+        logits = self.runner.forward(ids, pos, last_token_index=torch.tensor(want or [0], device=dev))
+        return self._sample(logits[:, -1, :].contiguous(), samplers)
+
     def _step_slots(self) -> list[tuple[int, int]]:
         runner, dev = self.runner, self.runner.device
+        if getattr(runner, "kv_group_size", 0) and any(r.fed < len(r.prompt) for r in self.running):
+            return self._step_portions()
         produced: list[tuple[int, int]] = []
         fresh = next((r for r in self.running if r.fed == 0), None)
         if fresh is not None:                      # whole prompt of one new request

@@ -24,12 +24,15 @@ import torch
 from ..distributed import divide, get_tp_rank, get_tp_world_size
 from ..kernels import (
     flash_attention2_no_pad,
+    flash_attention_int4,
     flash_decoding,
+    flash_decoding_int4,
     fused_moe,
     linear,
     route_topk,
     rope_emb_inplace,
     rope_kv_write,
+    rope_kv_write_int4,
     skip_rmsnorm,
     swiglu_forward,
     update_kv_buffer,
@@ -218,9 +221,11 @@ class Decoder:
     """Forward skeleton (reference: CausalLM.forward, lite_llama/models/base.py:447-489)."""
 
     def __init__(self, cfg: ModelConfig, weights: DecoderWeights, max_pos: int, device: str = "cuda",
-                 dtype: torch.dtype = torch.float16) -> None:
+                 dtype: torch.dtype = torch.float16, kv_group_size: int = 0) -> None:
+        """``kv_group_size``: elements that share a scale in a 4-bit KV pool; 0: the pool holds ``dtype``."""
         cfg.validate()
         self.cfg = cfg
+        self.kv_group_size = kv_group_size
         self.w = weights
         tp = get_tp_world_size()
         self.num_heads = divide(cfg.num_heads, tp, "attention heads")
@@ -248,7 +253,10 @@ class Decoder:
             xq, _ = skip_rmsnorm(xq, None, lw.q_norm, eps)
             xk, _ = skip_rmsnorm(xk, None, lw.k_norm, eps)
         kv_buffer = atten_info.kv_buffer[li]
-        if self.head_dim % 4 == 0:
+        group = self.kv_group_size
+        if group:
+            rope_kv_write_int4(xq, xk, xv, cos, sin, atten_info.cur_select_index, kv_buffer, batch, seq_len, group)
+        elif self.head_dim % 4 == 0:
             # rope (base.py:228) + cat + cache write (base.py:76-79) in one launch; q/k rotate where they lie
             rope_kv_write(xq, xk, xv, cos, sin, atten_info.cur_select_index, kv_buffer, batch, seq_len)
         else:
@@ -256,9 +264,16 @@ class Decoder:
             from ..kernels import update_kv_buffer_split
 
             update_kv_buffer_split(xk, xv, atten_info.cur_select_index, kv_buffer)
-        if seq_len > 1:                                                                 # base.py:95-103
+        if group and atten_info.b_new_len is not None:                                  # portions, one flat batch
+            attn = flash_attention_int4(xq, kv_buffer, self.scale, atten_info.b_start_loc, atten_info.b_new_len,
+                                        atten_info.b_req_tokens_table, atten_info.b_req_idx, atten_info.b_seq_len,
+                                        atten_info.max_new_len, atten_info.max_actual_seq_len, self.num_kv_heads, group)
+        elif seq_len > 1:                                                               # base.py:95-103
             attn = flash_attention2_no_pad(xq, xk, xv, self.scale * _LOG2E, atten_info.b_start_loc,
                                            atten_info.b_seq_len, atten_info.max_actual_seq_len)
+        elif group:
+            attn = flash_decoding_int4(xq, kv_buffer, self.scale, atten_info.b_req_tokens_table, atten_info.b_req_idx,
+                                       atten_info.b_seq_len, atten_info.max_actual_seq_len, self.num_kv_heads, group)
         else:                                                                           # base.py:120-129
             attn = flash_decoding(xq, kv_buffer[:, : self.num_kv_heads], kv_buffer[:, self.num_kv_heads :],
                                   self.scale, atten_info.b_req_tokens_table, atten_info.b_req_idx,
@@ -306,7 +321,8 @@ class Decoder:
     def forward(self, input_ids: torch.Tensor, position_ids: torch.Tensor, atten_info,
                 last_token_index: torch.Tensor | None = None) -> torch.Tensor:
         """``[batch, seq_len]`` ids -> ``[batch, seq_len, vocab]`` logits (all positions, like the
-        reference); with ``last_token_index [batch]`` only those positions are projected."""
+        reference); with ``last_token_index [batch]`` only those positions are projected (a flat batch of portions is
+        one row, of which any number of positions may be named)."""
         batch, seq_len = input_ids.shape
         hidden = torch.nn.functional.embedding(input_ids, self.w.embed)                 # base.py:470-472
         cos = self.cos_table[position_ids]                                              # base.py:473

@@ -20,7 +20,7 @@ from typing import Any
 import torch
 
 from ..distributed import all_reduce_min, divide, get_tp_world_size
-from ..kernels import argmax_rows, update_kv_index
+from ..kernels import argmax_rows, kv_int4_row_bytes, update_kv_index
 from ..kernels._common import counters
 from .attention_metadata import AttentionMetadata
 from .decoder import Decoder, DecoderWeights, random_weights
@@ -251,11 +251,20 @@ class RequestState:
 class ModelRunner:
     def __init__(self, config: ModelConfig | LayeredConfig, weights, max_gpu_num_blocks: int,
                  device: str = "cuda", dtype: torch.dtype = torch.float16, max_requests: int | None = None,
-                 max_seq_len: int | None = None) -> None:
+                 max_seq_len: int | None = None, kv_cache_dtype: str | None = None, kv_group_size: int | None = None) -> None:
+        """``kv_cache_dtype="int4"``: the uniform decoders' pool holds K and V in 4 bits with a scale and a minimum per
+        ``kv_group_size`` elements of a head (default: 64, or the head's size below that); ``None``: in ``dtype``."""
+        if kv_cache_dtype not in (None, "int4"):
+            raise ValueError(f"kv_cache_dtype is None or 'int4', got {kv_cache_dtype!r}")
+        if kv_cache_dtype is None and kv_group_size is not None:
+            raise ValueError("kv_group_size belongs to kv_cache_dtype='int4'")
+        if kv_cache_dtype is not None and isinstance(config, LayeredConfig):
+            raise ValueError("layer-list models keep their pool in the activation type")
         self.config = config
         self.device = device
         self.dtype = dtype
         self.ragged_steps = isinstance(config, LayeredConfig)
+        self.kv_group_size = 0                         # 4-bit pool: elements that share a scale
         self._slot_batch: SlotBatch | None = None
         self._graphs: dict[tuple[int, int], _CapturedDecode] = {}
         self._graph_batches: tuple[int, ...] = ()
@@ -271,15 +280,22 @@ class ModelRunner:
         self.max_seq_len = config.max_seq_len
         # every rank must agree on the pool size (model_runner.py:84-89)
         max_gpu_num_blocks = all_reduce_min(max_gpu_num_blocks, device)
-        self.kv_cache_manager = KVCacheManager(self.num_layers, self.num_kv_heads, self.head_dim,
-                                               max_gpu_num_blocks, dtype=dtype, device=device)
+        if kv_cache_dtype == "int4":
+            self.kv_group_size = min(64, self.head_dim) if kv_group_size is None else kv_group_size
+            row = kv_int4_row_bytes(self.num_kv_heads, self.head_dim, self.kv_group_size)
+            self.kv_cache_manager = KVCacheManager(self.num_layers, self.num_kv_heads, self.head_dim, max_gpu_num_blocks,
+                                                   dtype=torch.uint8, device=device, row_widths=[row] * self.num_layers)
+        else:
+            self.kv_cache_manager = KVCacheManager(self.num_layers, self.num_kv_heads, self.head_dim,
+                                                   max_gpu_num_blocks, dtype=dtype, device=device)
         self.max_request_num = max(1, max_gpu_num_blocks // self.max_seq_len)
         self.b_req_tokens_table = torch.zeros((self.max_request_num, self.max_seq_len), dtype=torch.int32,
                                               device=device)
         self.atten_info = AttentionMetadata()
         self.atten_info.kv_buffer = self.kv_cache_manager.gpu_kv_buffer
         self.atten_info.b_req_tokens_table = self.b_req_tokens_table
-        self.model = Decoder(config, weights, max_pos=self.max_seq_len, device=device, dtype=dtype)
+        self.model = Decoder(config, weights, max_pos=self.max_seq_len, device=device, dtype=dtype,
+                             kv_group_size=self.kv_group_size)
         self.spec = ModelSpec(config.name)
         counters(torch.device(device))  # allocate the split-K ticket buffer outside any capture
 
@@ -455,10 +471,11 @@ class ModelRunner:
     def build(cls, model: str | ModelConfig, max_seq_len: int, max_gpu_num_blocks: int | None = None,
               device: str = "cuda", quantization: str | None = None, seed: int = 0,
               dtype: torch.dtype = torch.float16, num_layers: int | None = None,
-              draw_device: str | None = None) -> "ModelRunner":
+              draw_device: str | None = None, kv_cache_dtype: str | None = None,
+              kv_group_size: int | None = None) -> "ModelRunner":
         """``model`` is a preset name (see ``PRESETS``) or a ModelConfig; ``quantization`` one of
         ``None | "int4" | "int8" | "fp8" | "smoothquant"`` (the reference's ``--quantization`` values,
-        models/quantization/config.py:39-54)."""
+        models/quantization/config.py:39-54), of the weights; ``kv_cache_dtype`` and ``kv_group_size`` as in ``__init__``."""
         cfg = PRESETS[model] if isinstance(model, str) else model
         cfg = cfg.with_(max_seq_len=max_seq_len)
         if num_layers is not None:
@@ -467,7 +484,8 @@ class ModelRunner:
                                  draw_device=draw_device)
         if max_gpu_num_blocks is None:
             max_gpu_num_blocks = 32 * max_seq_len
-        return cls(cfg, weights, max_gpu_num_blocks, device=device, dtype=dtype)
+        return cls(cfg, weights, max_gpu_num_blocks, device=device, dtype=dtype, kv_cache_dtype=kv_cache_dtype,
+                   kv_group_size=kv_group_size)
 
     # --------------------------------------------------------- kv allocation #
     def _init_req_tokens_table(self, b_req_idx, b_seq_len, alloc_index, max_prompt_len) -> torch.Tensor:
@@ -484,6 +502,7 @@ class ModelRunner:
     def prefill_alloc_kv_cache(self, max_prompt_len, actual_prompt_lens, b_req_idx) -> torch.Tensor:
         batch_size = len(actual_prompt_lens)
         self.atten_info.b_req_idx = b_req_idx
+        self.atten_info.b_new_len = None
         self.atten_info.cur_select_index = self.kv_cache_manager.alloc_kvcache_index(max_prompt_len * batch_size)
         if self.atten_info.cur_select_index is None:
             raise RuntimeError("KV cache exhausted during prefill allocation")
@@ -500,6 +519,7 @@ class ModelRunner:
         if self.atten_info.cur_select_index is None:
             raise RuntimeError("KV cache exhausted during decode allocation")
         self.atten_info.b_seq_len += 1
+        self.atten_info.b_new_len = None
         self.atten_info.max_actual_seq_len += 1
         update_kv_index(self.atten_info.b_req_tokens_table, self.atten_info.b_req_idx,
                         self.atten_info.b_seq_len, self.atten_info.cur_select_index)

@@ -16,6 +16,8 @@ from typing import TYPE_CHECKING
 
 import torch
 
+from ..kernels import build_slot_maps
+
 if TYPE_CHECKING:  # pragma: no cover
     from .model_runner import ModelRunner
 
@@ -58,6 +60,7 @@ class SlotBatch:
         at.max_actual_seq_len = longest
         at.cur_select_index = at.b_req_tokens_table[idx, :longest].reshape(-1)
         at.b_start_loc = self._grid_rows[: len(slots)] * longest
+        at.b_new_len = None
         self.reset()            # the running set changed: the next decode rebuilds its metadata
 
     def begin_decode(self, slots: Sequence[int], seq_lens: Sequence[int]) -> int:
@@ -77,8 +80,29 @@ class SlotBatch:
         at.b_seq_len = self._dev_lens
         at.max_actual_seq_len = max(seq_lens)
         at.cur_select_index = at.b_req_tokens_table[self._dev_slots, self._dev_lens - 1]
-        at.b_start_loc = None
+        at.b_start_loc = at.b_new_len = None
         return len(slots_p)
+
+    def begin_portions(self, slots: Sequence[int], cached_lens: Sequence[int], new_lens: Sequence[int]) -> torch.Tensor:
+        """Attention metadata for one flat step over a 4-bit pool: sequence ``i`` (its own slot) has ``cached_lens[i]`` tokens
+        cached and brings ``new_lens[i] >= 1``, behind those of the sequences before it.  Returns the tokens' positions
+        ``[1, total]`` for a forward of one row of ``total`` tokens."""
+        if not self._runner.kv_group_size:
+            raise RuntimeError("portions are read from a 4-bit pool (kv_cache_dtype='int4')")
+        if not slots or not len(slots) == len(cached_lens) == len(new_lens) or min(new_lens) < 1 or min(cached_lens) < 0:
+            raise ValueError("begin_portions: every sequence brings at least one token")
+        if len(set(slots)) != len(slots) or min(slots) < 0 or max(slots) >= self.num_slots:
+            raise ValueError(f"begin_portions: slots are different numbers below {self.num_slots}")
+        longest = max(c + n for c, n in zip(cached_lens, new_lens))
+        if longest > self.max_seq_len:
+            raise ValueError(f"sequence of {longest} tokens exceeds max_seq_len {self.max_seq_len}")
+        at = self._atten
+        at.b_req_idx, cached, at.b_new_len = self._upload([*slots, *cached_lens, *new_lens]).view(3, -1).unbind()
+        maps = build_slot_maps(at.b_req_idx, cached, at.b_new_len, at.b_req_tokens_table, sum(new_lens))
+        at.cur_select_index, positions, at.b_start_loc, at.b_seq_len = maps
+        at.max_new_len, at.max_actual_seq_len = max(new_lens), longest
+        self.reset()
+        return positions.view(1, -1)
 
     def reset(self) -> None:
         self._cur_slots, self._cur_lens = [], []
