@@ -12,7 +12,7 @@
 // columns that up to four heads leave free, else in a second product -- since a code's products are larger than its value's.
 //
 // Work: tiles of 16 * TS or 32 * TS tokens of all rows, in equal shares over one wave of CTAs, whatever rows they belong to (the lengths are device
-// data).  Whole token rows come by asynchronous copies into a ring (of the working warps: with a warp of its own for that, two CTAs to
+// data).  Whole token rows come by bulk copies into a ring (of the working warps: with a warp of its own for that, two CTAs to
 // an SM leave a thread 96 registers, and spill); a warp takes 16 or 32 tokens of one kv head.  A row
 // that lies in one share is written out; else its parts go to the workspace and a second kernel adds them up.
 #include "kv_int4.cuh"
@@ -20,8 +20,11 @@
 
 namespace {
 
-constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kCluster = 8, kRowCost = 1, kFirst = 3;
-constexpr int kMinLog2 = 6, kMinTokens = 1 << kMinLog2;   // of a share: below that the merge costs more than the share
+constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kCluster = 8, kFirst = 3;
+// a row's start and end in tiles (150 rows of 200 - 400 tokens, 2 kv heads of 64: 13.6 us; 0 tiles 15.9, 2 tiles 15.0)
+constexpr int kRowCost = 1;
+// tokens of a share, at least a tile (one row of 1500 / 3900 tokens, 8 kv heads of 128: 11.2 / 12.2 us; of 64 tokens 13.5 / 14.1, 128: 15.3 / 17.4)
+constexpr int kMinLog2 = 5, kMinTokens = 1 << kMinLog2;
 
 struct Int4DecodeParams {
   const void* q; int64_t q_bs, q_hs; int q_vec;   // q_vec: heads on 16-byte boundaries
@@ -30,7 +33,7 @@ struct Int4DecodeParams {
   const int32_t* table; int64_t tab_rs, tab_cs, requests, width;
   const void* req_idx; int req_w;
   const void* seq_len; int len_w;
-  int batch, Hq, Hkv, G, HB, nblk, qblocks, TS, TS_log2, stages, pitch, bulk;
+  int batch, Hq, Hkv, G, HB, nblk, qblocks, TS, TS_log2, stages, pitch;
   int64_t most;                                   // tokens of a row that the call's bound lets count
   float scale_log2;
   float* ws_o; float* ws_ml; int2* ws_info;       // parts [cta][2][HB * G]: rows, (largest score, sum); first and last CTA of a row
@@ -391,14 +394,6 @@ struct Int4Consumer {
 
 struct Segment { int b, blk, first, last, tiles; };   // tiles [first, last) of a row of `tiles`
 
-// 16 bytes to shared memory
-__device__ __forceinline__ void copy16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-// the barrier's arrival of this thread, once its copies so far are done
-__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -440,7 +435,7 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
   };
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full_bar[s], p.bulk ? nwarps : nwarps * 32);
+      mbar_init(&full_bar[s], nwarps);
       mbar_init(&empty_bar[s], nwarps);
     }
     mbar_fence_init();
@@ -530,10 +525,9 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     return any;
   };
 
-  // ---- the ring's copies: each warp brings its part of a tile's token rows, whose table entries are read a tile ahead.  One bulk copy to
-  // a row costs the warp least, but the engine ~40 cycles: 32 rows 1400, which a cluster's few tiles wait for, and rows of 160 bytes
-  // limited the whole kernel (150 sequences of 200 - 400 tokens, 2 kv heads of 64: 20.5 us, this 18.0).  Else 16 bytes a lane (32 of
-  // 1000 - 2000, 8 kv heads of 128: 34 us, bulk 31). ----
+  // ---- the ring's copies: each warp brings its part of a tile's token rows, whose table entries are read a tile ahead, one bulk copy to
+  // a row.  (16 bytes a lane instead: 32 rows of 1000 - 2000 tokens, 8 kv heads of 128: 32 us, bulk 29; one row of 201: 7.2 and 6.6; rows
+  // of 160 bytes, 150 of 200 - 400 tokens: 13.6 and 13.4.) ----
   const int hb = kv4::head_bytes(D, GS), mine = nwarps == 8 ? tile >> 3 : (tile + nwarps - 1) / nwarps;   // token rows of this warp, at most 32
   struct Place { Segment s; int item, t; bool more; };   // a tile of the share
   auto start_of = [&](Place& x) {
@@ -562,28 +556,9 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     const uint8_t* src = p.cache + (from - shift);
     uint8_t* dst = ring + s * stage_bytes + first * p.pitch;
     const int at = row < 0 || row >= p.max_tokens ? 0 : row;
-    if (p.bulk) {
-      if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], (uint32_t)((mine_here > 0 ? mine_here : 0) * pieces * 16));
-      __syncwarp();
-      if (lane < mine_here) bulk_g2s(dst + lane * p.pitch, src + (int64_t)at * p.row_stride, (uint32_t)pieces * 16u, &full_bar[s]);
-      return;
-    }
-    if (pieces >= 32) {                           // a row at a time
-#pragma unroll 1
-      for (int i = 0; i < mine_here; ++i) {
-        const uint8_t* x = src + (int64_t)__shfl_sync(0xffffffffu, at, i) * p.row_stride;
-        uint8_t* y = dst + i * p.pitch;
-        for (int c = lane; c < pieces; c += 32) copy16(y + c * 16, x + c * 16);
-      }
-    } else {                                      // several rows at a time
-      const int rows = 32 / pieces, i0 = lane / pieces, c = lane - i0 * pieces;
-#pragma unroll 1
-      for (int i = 0; i < mine_here; i += rows) {
-        const int64_t r = __shfl_sync(0xffffffffu, at, (i + i0) & 31);
-        if (i0 < rows && i + i0 < mine_here) copy16(dst + (i + i0) * p.pitch + c * 16, src + r * p.row_stride + c * 16);
-      }
-    }
-    copies_arrive(&full_bar[s]);
+    if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], (uint32_t)((mine_here > 0 ? mine_here : 0) * pieces * 16));
+    __syncwarp();
+    if (lane < mine_here) bulk_g2s(dst + lane * p.pitch, src + (int64_t)at * p.row_stride, (uint32_t)pieces * 16u, &full_bar[s]);
   };
 
   // ===================== a warp: (kv head, block of query heads, unit of the tile) =====================
@@ -854,7 +829,9 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) kv4_decode_merge_kernel
 }
 
 constexpr int kMaxBatch = 4096;                   // rows of one launch (their lengths lie in shared memory)
-constexpr int kClusterMost = 1024;                // tokens of a row that a cluster takes
+// Tokens of a row that a cluster takes.  One row of 201 / 650 / 1000 / 1400 tokens, 8 kv heads of 128: 6.6 / 9.4 / 11.1 / 14.2 us, in shares
+// 9.6 / 11.9 / 11.0 / 11.2; 18 rows of 900: 14.9 and 18.3; 4 kv heads, 2 rows of 1000 / 1900: 8.5 / 11.8 and 11.2 / 10.2.
+constexpr int kClusterMost = 1024;
 
 struct Int4Plan { int HB, qblocks, TS, pitch, stages, smem, grid; bool cluster; };
 
@@ -881,7 +858,8 @@ Int4Plan make_plan(int64_t batch, int G, int Hkv, int D, int group, int64_t max_
   if (pl.stages > kMaxStages) pl.stages = kMaxStages;
   if (pl.stages < 2) pl.stages = 2;
   pl.smem = fixed + pl.stages * stage;
-  const int64_t most = (int64_t)rows * cdiv64(max_len > 0 ? max_len : 1, kMinTokens) * (Hkv / pl.HB);
+  const int tile = pl.TS * units * kUnit;
+  const int64_t most = (int64_t)rows * cdiv64(max_len > 0 ? max_len : 1, tile > kMinTokens ? tile : kMinTokens) * (Hkv / pl.HB);
   const int64_t wave = (int64_t)per_sm * b2l_num_sms();
   pl.grid = (int)(most < wave ? most : wave);
   pl.cluster = batch * (Hkv / pl.HB) * kCluster <= wave && max_len <= kClusterMost && pl.HB * G * (D + 2) * 4 <= pl.stages * stage;
@@ -919,7 +897,7 @@ int launch_int4_decode(const Int4DecodeParams& p, const Int4Plan& pl, cudaStream
   B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured[p.G <= 4]));
   b2l_launch(kern, grid, block, (size_t)pl.smem, st, p);
   B2L_LAUNCH_CHECK();
-  // many parts to a row, or few
+  // many parts to a row, or few: 16 warps to a head, or one (2 rows of 30000 tokens: 18.9 and 37.8 us; 32 rows of 1000 - 2000: 38.0 and 29.5)
   if ((int64_t)pl.grid > 24 * (int64_t)p.batch)
     b2l_launch(kv4_decode_merge_kernel<T, D, 16>, dim3((unsigned)p.batch, (unsigned)p.Hq), dim3(512), (size_t)0, st, p);
   else
@@ -980,7 +958,6 @@ extern "C" int b2l_flash_decoding_int4(void* out, const void* q, const void* cac
   p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = G; p.HB = pl.HB; p.qblocks = pl.qblocks; p.TS = pl.TS;
   p.stages = pl.stages; p.pitch = pl.pitch; p.nblk = num_kv_heads / pl.HB;
   for (p.TS_log2 = 0; 1 << p.TS_log2 < pl.TS;) ++p.TS_log2;     // a power of two
-  p.bulk = !pl.cluster && pl.HB * kv4::head_bytes(head_dim, group) >= 512;   // rows that take all lanes a piece
   p.most = max_seq_len < table_width ? max_seq_len : table_width;
   if (p.most < 0) p.most = 0;
   B2L_REQUIRE((batch < kMaxBatch ? batch : kMaxBatch) * cdiv64(p.most, kUnit) * num_kv_heads < (1ll << 31), "flash_decoding_int4: too many tokens");
