@@ -33,13 +33,16 @@ def _ids(*shape, seed=0):
 @pytest.fixture
 def calls(monkeypatch):
     """Checks each call of the decoder's three operators as it is made; counts them."""
-    count = dict(write=0, decode=0, portions=0)
+    count = dict(write=0, decode=0, portions=0, real=0)
     write, decode, portions = D.rope_kv_write_int4, D.flash_decoding_int4, D.flash_attention_int4
 
     def checked_write(q, k, v, cos, sin, index, pool, batch, seq, group):
         out = write(q, k, v, cos, sin, index, pool, batch, seq, group)
         used = k.shape[1] * (k.shape[2] + 8 * (k.shape[2] // group))
-        assert torch.equal(pool[index.long()][:, :used], O.rows_of(k, v, group)[:, :used])
+        # a padded prompt's tokens behind its length come from what no kernel wrote (NaN maybe, whose bytes may be any)
+        real = torch.isfinite(k).flatten(1).all(1) & torch.isfinite(v).flatten(1).all(1)
+        count["real"] += int(real.sum())
+        assert torch.equal(pool[index.long()][real, :used], O.rows_of(k, v, group)[real, :used])
         count["write"] += 1
         return out
 
@@ -77,6 +80,7 @@ def test_engine(name, dtype, kw, calls):
     outs = engine.generate(prompts, 6)
     assert [len(o) for o in outs] == [6] * 5
     assert calls["portions"] > 0 and calls["decode"] > 0 and calls["write"] == calls["portions"] + calls["decode"]
+    assert calls["real"] >= runner.num_layers * sum(len(p) + 5 for p in prompts)
 
 
 @pytest.mark.parametrize("name,dtype,kw", MODELS[:2], ids=str)
@@ -85,13 +89,14 @@ def test_padded_prompts_then_decode(name, dtype, kw, calls):
     lens = torch.tensor([12, 7, 9], device="cuda")
     runner.prefill_alloc_kv_cache(12, lens.clone(), torch.arange(3, device="cuda"))
     logits = runner.forward(_ids(3, 12).cuda(), torch.arange(12, device="cuda").repeat(3, 1))
-    assert torch.isfinite(logits).all()
+    assert all(torch.isfinite(logits[b, :n]).all() for b, n in enumerate(lens.tolist()))
     for _ in range(3):
         runner.decode_alloc_kv_cache(3)
         pos = (runner.atten_info.b_seq_len - 1).view(3, 1)
         assert torch.isfinite(runner.forward(_ids(3, 1).cuda(), pos)).all()
     layers = runner.num_layers
-    assert calls == dict(write=4 * layers, decode=3 * layers, portions=0)
+    assert calls["real"] >= layers * (12 + 7 + 9 + 3 * 3)
+    assert (calls["write"], calls["decode"], calls["portions"]) == (4 * layers, 3 * layers, 0)
 
 
 def test_a_captured_decode_step_is_the_eager_one():
