@@ -78,7 +78,8 @@ template <typename T>
 struct Grid {
   uint32_t stored;
   float lo16, step16, inv;
-  int way;                                        // 0 codes are zero, 1 by the reciprocal, 2 by division (steps near the end of the range)
+  int way;                                        // 0 codes are zero, 1 by the reciprocal, 2 by division (steps near the ends of the range; one that was
+                                                  // rounded to few bits may lead past 15, else 15.06 is the most)
   __device__ __forceinline__ void from(float lo, float hi) {
     lo16 = lo * 0.0625f;
     const float range16 = hi * 0.0625f - lo16;
@@ -90,7 +91,7 @@ struct Grid {
     }
     stored = pack2<T>(__fdiv_rn(range16, 0.9375f), lo);
     step16 = kv4::scale_min<T>(stored).x * 0.0625f;
-    way = step16 == 0.f ? 0 : step16 > 1e-30f && step16 < 1e30f ? 1 : 2;
+    way = step16 == 0.f ? 0 : step16 > (std::is_same<T, __half>::value ? 0x1p-18f : 1e-30f) && step16 < 1e30f ? 1 : 2;
     inv = __frcp_rn(step16);
   }
   // Quotient by the correctly rounded reciprocal and one correction with the remainder, which gives the correctly rounded quotient
@@ -103,9 +104,17 @@ struct Grid {
       c = t * inv;
       c = fmaf(fmaf(-c, step16, t), inv, c);
     } else {
-      c = way == 0 ? 0.f : __fdiv_rn(t, step16);
+      c = way == 0 ? 0.f : fminf(__fdiv_rn(t, step16), 15.f);
     }
-    return __float_as_uint(fminf(c, 15.f) + 12582912.f) & 15u;   // 1.5 * 2^23: the sum's last bits are the nearest whole number
+    const float near = c + 12582912.f;                           // 1.5 * 2^23: the sum's last bits are the nearest whole number
+    uint32_t code = __float_as_uint(near);
+    if (fabsf(c - (near - 12582912.f)) == 0.5f) {
+      // Half a step of the difference that 32 bits hold.  What they do not (of an element some 2^13 times smaller than the minimum, or the
+      // other way round) decides.
+      const float x16 = x * 0.0625f, part = t + lo16, rest = (x16 - part) - (lo16 - (part - t));
+      if (rest != 0.f) code = (uint32_t)(c + (rest > 0.f ? 0.5f : -0.5f));
+    }
+    return code & 15u;
   }
   __device__ __forceinline__ uint32_t codes(const uint32_t (&w)[4]) const {
     using T2 = typename Ext<T>::T2;
@@ -122,7 +131,7 @@ struct Grid {
 // A thread holds eight elements of a head's lower half and the eight that rotate with them of its upper half; a head's threads are
 // neighbours in a warp and find their groups' ends with one to four shuffles.  All of a token's heads -- q rotated, k rotated and
 // stored, v stored -- are units of one grid: a decode step is one trip through L2, not one per head.  (8000 tokens of 28 + 4 + 4 heads of
-// 128, bf16, 147 MB: blocks of 96 threads 29 us, of 288, a token's all heads, 33, with two tokens to a thread 42.)
+// 128, bf16, 147 MB: blocks of 96 threads 29 us, of 288, a token's all heads, 33, with two tokens to a thread 42; deciding half steps exactly 2 more.)
 template <typename T, int D, int GS, bool VEC>
 __global__ void __launch_bounds__(128) kv4_write_kernel(const WriteParams p) {
   pdl_prologue();

@@ -78,6 +78,21 @@ def test_values_with_every_scale_and_ties(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_half_steps_that_a_tiny_element_leaves(dtype):
+    """Elements of +-2^-24 .. 2^-8 in groups whose minimum lies exactly k + 1/2 steps below zero: their sign decides the code."""
+    groups = []
+    for k in range(15):
+        for base in (1.0, 3.0, 1024.0):                      # scale 2 base; the range is 15 of it, so that it is stored exactly (fp16: 29 * 1024 is finite)
+            lo = -(2 * k + 1) * base
+            tiny = [s * 2.0**-e for e in (8, 12, 14, 18, 24) for s in (1, -1)]
+            groups.append([lo, lo + 30 * base] + tiny + [0.0] * 20)
+    k = torch.tensor(groups, device="cuda", dtype=torch.float64).to(dtype).view(-1, 1, 32)
+    cache = _cache(k.shape[0], 1, 32, 32)
+    K.update_kv_buffer_int4(k, k.flip(0).contiguous(), torch.arange(k.shape[0], device="cuda"), cache, 32)
+    _same_rows(cache, O.rows_of(k, k.flip(0), 32), _used(1, 32, 32))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 def test_a_group_that_is_not_finite_reads_as_nan(dtype, bad):
     k, v = _normal(5, 2, 128, dtype=dtype), _normal(5, 2, 128, dtype=dtype)
@@ -320,6 +335,20 @@ def test_decode_with_strides():
               _normal(2, 128, 4, dtype=torch.bfloat16).transpose(1, 2)):
         out = K.flash_decoding_int4(q, wide[:, 16:16 + rows.shape[1]], 0.1, turned, req, n, 70, 2, 32)
         _check(out, q, rows, table, req, n, 2, 32, 0.1)
+
+
+@pytest.mark.parametrize("lens", [[201, 17], [1500, 3000]], ids=str)
+def test_decode_into_a_tensor(lens):
+    """A part of a larger tensor; the query itself."""
+    rows, table, req, n = _step(lens, 4, 128, 64, torch.float16)
+    q, keep = _normal(2, 8, 128, dtype=torch.float16), _normal(5, 10, 136, dtype=torch.float16)
+    want = K.flash_decoding_int4(q, rows, 0.1, table, req, n, max(lens), 4, 64)
+    to = keep.clone()
+    view = to[1:3, 2:, 4:132]
+    assert K.flash_decoding_int4(q, rows, 0.1, table, req, n, max(lens), 4, 64, view) is view and torch.equal(view, want)
+    keep[1:3, 2:, 4:132] = want
+    assert torch.equal(to, keep)
+    assert K.flash_decoding_int4(q, rows, 0.1, table, req, n, max(lens), 4, 64, out=q) is q and torch.equal(q, want)
 
 
 def test_decode_of_rows_past_32_bits():
