@@ -175,7 +175,7 @@ int b2l_flash_decoding_int4(void* out, const void* q, const void* cache, int64_t
 /* Portions of prompts over that cache, causal: the new_len[b] rows of q [total_tokens, Hq, D] from start_loc[b] on stand at the positions
  * seq_len[b] - new_len[b], ... and see the cached tokens up to their own.  Rows of no sequence are not written, a row that sees
  * nothing is zero; rows past total_tokens, new tokens past max_new_len and keys past max_seq_len or the table's width do not count. */
-int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64_t total_tokens, int64_t max_new_len, int num_q_heads,
+int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64_t total_tokens, int num_q_heads,
                                                  int num_kv_heads, int head_dim, int group, int64_t max_seq_len);
 int b2l_flash_attention_int4(void* out, const void* q, const void* cache, int64_t cache_row_stride, int64_t max_tokens,
                              const void* b_start_loc, int start_width, const void* b_new_len, int new_width,

@@ -44,7 +44,7 @@ struct {
   int64_t (*kv4_decode_workspace)(i64, int, int, int, int, i64);
   int (*kv4_decode)(void*, const void*, const void*, i64, i64, const void*, i64, i64, i64, i64, const void*, int, const void*, int, i64, int,
                     int, int, int, i64, float, i64, i64, i64, i64, void*, i64, int, void*);
-  int64_t (*kv4_prompt_workspace)(i64, i64, i64, int, int, int, int, i64);
+  int64_t (*kv4_prompt_workspace)(i64, i64, int, int, int, int, i64);
   int (*kv4_prompt)(void*, const void*, const void*, i64, i64, const void*, int, const void*, int, const void*, i64, i64, i64, i64, const void*,
                     int, const void*, int, i64, i64, i64, int, int, int, int, i64, float, i64, i64, i64, i64, void*, i64, int, void*);
   int (*slot_maps)(void*, void*, void*, void*, const void*, int, const void*, int, const void*, int, const void*, int, void*, i64, i64, i64,
@@ -477,12 +477,13 @@ PyObject* kv4_read(PyObject*, PyObject* const* a, Py_ssize_t count) {
   FAST_END
 }
 
-// (q, kv_buffer, scale, table, req_idx, seq_len, max_len, kv heads, group) -> out
+// (q, kv_buffer, scale, table, req_idx, seq_len, max_len, kv heads, group, out or None) -> out
 PyObject* kv4_decode(PyObject*, PyObject* const* a, Py_ssize_t count) {
-  ARGS(9)
+  ARGS(10)
   FAST_BEGIN
   const at::Tensor *q = plain(a[0]), *kv = plain(a[1]), *table = plain(a[3]), *req = plain(a[4]), *len = plain(a[5]);
-  const int device = device_for(abi.kv4_decode, {q, kv, table, req, len});
+  const at::Tensor* given = a[9] == Py_None ? q : plain(a[9]);
+  const int device = device_for(abi.kv4_decode, {q, kv, table, req, len, given});
   i64 n[3];
   if (device < 0 || !PyFloat_CheckExact(a[2]) || !numbers(a, {6, 7, 8}, n)) return none();
   const int code = half_code(*q);
@@ -490,19 +491,21 @@ PyObject* kv4_decode(PyObject*, PyObject* const* a, Py_ssize_t count) {
   const i64 batch = q->size(0), hq = q->size(1), d = q->size(2);
   const int rw = indices(*req, batch), lw = indices(*len, batch);
   if (!rw || !lw || !cache4(*kv, n[1], d, n[2]) || hq % n[1] != 0) return none();
+  if (given != q && (given->scalar_type() != q->scalar_type() || given->sizes() != q->sizes() || given->stride(2) != 1)) return none();
   const i64 bytes = abi.kv4_decode_workspace(batch, (int)hq, (int)n[1], (int)d, (int)n[2], n[0]);
   at::Tensor out, ws;
   int rc;
   {
     const Unlocked unlocked;
-    out = at::empty({batch, hq, d}, q->options());
+    out = a[9] == Py_None ? at::empty({batch, hq, d}, q->options()) : *given;
     ws = at::empty({bytes > 16 ? bytes : 16}, q->options().dtype(at::kByte));
     rc = abi.kv4_decode(out.data_ptr(), q->data_ptr(), kv->data_ptr(), kv->stride(0), kv->size(0), table->data_ptr(), table->stride(0),
                         table->stride(1), table->size(0), table->size(1), req->data_ptr(), rw, len->data_ptr(), lw, batch, (int)hq, (int)n[1],
-                        (int)d, (int)n[2], n[0], (float)PyFloat_AS_DOUBLE(a[2]), q->stride(0), q->stride(1), hq * d, d, ws.data_ptr(), bytes,
+                        (int)d, (int)n[2], n[0], (float)PyFloat_AS_DOUBLE(a[2]), q->stride(0), q->stride(1), out.stride(0), out.stride(1), ws.data_ptr(), bytes,
                         code, stream(device));
   }
-  return rc ? failed(rc) : THPVariable_Wrap(std::move(out));
+  if (rc) return failed(rc);
+  return a[9] == Py_None ? THPVariable_Wrap(std::move(out)) : Py_NewRef(a[9]);
   FAST_END
 }
 
@@ -522,7 +525,7 @@ PyObject* kv4_prompt(PyObject*, PyObject* const* a, Py_ssize_t count) {
   const int sw = indices(*start, batch), fw = indices(*fresh, batch), rw = indices(*req, batch), lw = indices(*len, batch);
   if (!sw || !fw || !rw || !lw || !cache4(*kv, n[2], d, n[3]) || hq % n[2] != 0) return none();
   if (given != q && (given->scalar_type() != q->scalar_type() || given->sizes() != q->sizes() || given->stride(2) != 1)) return none();
-  const i64 bytes = abi.kv4_prompt_workspace(batch, tokens, n[0], (int)hq, (int)n[2], (int)d, (int)n[3], n[1]);
+  const i64 bytes = abi.kv4_prompt_workspace(batch, tokens, (int)hq, (int)n[2], (int)d, (int)n[3], n[1]);
   at::Tensor out, ws;
   int rc;
   {

@@ -17,11 +17,11 @@
 // (a key tile of both row tiles) takes about 5000 cycles, bound by the conversion's and the softmax's instructions together; its four
 // products would take 2050.
 //
-// READY: where five row blocks or more read a key tile, a kernel before this one converts each tile once into the workspace, as the
+// READY: where five row blocks or more read a key tile on average, a kernel before this one converts each tile once into the workspace, as the
 // tensor cores read it, and one warp fetches whole operands; the softmax warps then have registers for a whole row of 128 scores
 // (S for both tiles in turn | P0 P1 | O0 | O1), which they free before the exponentials.  A step takes 2800 cycles, of which 2050 are
 // the exponentials' issue alone.  The kernel before takes 6 us for 8000 keys of 8 heads.
-// 512 tokens over 7500, 32 / 8 heads: 89 us (101 the other way), 256: 66 both ways, 128: 59 (54).
+// 512 tokens over 7500, 32 / 8 heads: 90 us (98 the other way).
 // The operands are halves for both activation types: elements are rounded to 11 bits (as the 16-bit cache of an fp16 model rounds
 // them), which for bf16 models are three bits more than reading the cache into their type would leave; elements of those beyond 65504
 // count as 65504.  Queries of bf16 models are scaled by a power of two per row.  Probabilities are rounded to 11 bits, as in
@@ -838,14 +838,14 @@ __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(const Params p) {
 
 struct Plan { int grid, smem, ready_tiles; int64_t items, rows, steps, ready_bytes; };   // ready_tiles 0: operands are made beside the products
 
-// Row blocks of the longest portion from which on operands are made ready.  1 x 256 / 320 / 384 / 512 tokens (4 to 8 blocks) over 7500:
-// 66.5 / 73.6 / 77.6 / 90.6 us ready, 66.2 / 74.9 / 82.2 / 100.8 converted beside the products; 6 x 200 / 290 / 400 over 1200:
-// 58.5 / 77.8 / 87.4 and 56.8 / 80.3 / 94.0.
+// Row blocks of a portion, on average, from which on operands are made ready.  1 x 320 / 384 / 512 tokens (5 to 8 blocks) over 7500: 72.0 /
+// 76.1 / 89.6 us ready, 72.7 / 80.2 / 98.5 converted beside the products; 256 (4 blocks): 66.5 and 64.6; 6 x 290 / 400 at most over 1200:
+// 73.2 / 82.3 and 76.2 / 90.0; 6 x 200: 58.5 and 54.2.
 constexpr int kReadyBlocks = 5;
 // Their room in the workspace at most: 65536 keys of 8 heads.  It grows with batch * max_seq_len, of which ragged steps use a part.
 constexpr int64_t kReadyMost = 256ll << 20;
 
-Plan make_plan(int64_t batch, int64_t total, int64_t max_new, int G, int Hkv, int D, int64_t max_len) {
+Plan make_plan(int64_t batch, int64_t total, int G, int Hkv, int D, int64_t max_len) {
   Plan pl;
   const int DP = D < 64 ? 64 : D;
   const int64_t rows = batch < kMaxBatch ? batch : kMaxBatch, tiles = cdiv64(max_len > 0 ? max_len : 1, kBN);
@@ -858,8 +858,8 @@ Plan make_plan(int64_t batch, int64_t total, int64_t max_new, int G, int Hkv, in
   pl.rows = 2ll * pl.grid * kRows;
   // A tile is read by every row block that sees it: converted once for all of them where they are several, with room for the tiles
   // of the bounds.
-  const int64_t tile = 2ll * kBN * DP * 2, blocks = cdiv64((max_new < total ? max_new : total) * G, kRows);
-  const bool ready = blocks >= kReadyBlocks && rows * Hkv * tiles <= kReadyMost / tile;
+  const int64_t tile = 2ll * kBN * DP * 2;
+  const bool ready = total * G > (kReadyBlocks - 1) * kRows * batch && rows * Hkv * tiles <= kReadyMost / tile;
   pl.ready_tiles = ready ? (int)tiles : 0;
   pl.ready_bytes = ready ? rows * Hkv * tiles * (tile + 16) : 0;
   pl.smem = 1024 + (2 + kKStages + kVStages) * kBN * DP * 2 + (ready ? 0 : kUnits * kUnitKeys * kUnitPitch) + lists;
@@ -888,11 +888,11 @@ int launch(const Params& p, const Plan& pl, cudaStream_t st) {
 
 }  // namespace kv4p
 
-extern "C" int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64_t total_tokens, int64_t max_new_len, int num_q_heads, int num_kv_heads,
+extern "C" int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64_t total_tokens, int num_q_heads, int num_kv_heads,
                                                             int head_dim, int group, int64_t max_seq_len) {
   if (batch <= 0 || total_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || !kv4::shape_ok(head_dim, group))
     return 0;
-  return kv4p::workspace_for(kv4p::make_plan(batch, total_tokens, max_new_len, num_q_heads / num_kv_heads, num_kv_heads, head_dim, max_seq_len), head_dim);
+  return kv4p::workspace_for(kv4p::make_plan(batch, total_tokens, num_q_heads / num_kv_heads, num_kv_heads, head_dim, max_seq_len), head_dim);
 }
 
 extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* cache, int64_t cache_row_stride, int64_t max_tokens,
@@ -920,7 +920,7 @@ extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* ca
   if (batch == 0 || total_tokens == 0 || max_new_len == 0) return B2L_OK;
   const int G = num_q_heads / num_kv_heads;
   const int64_t most = max_seq_len < table_width ? max_seq_len : table_width;
-  const Plan pl = make_plan(batch, total_tokens, max_new_len, G, num_kv_heads, head_dim, max_seq_len);
+  const Plan pl = make_plan(batch, total_tokens, G, num_kv_heads, head_dim, max_seq_len);
   B2L_REQUIRE(pl.steps < (1ll << 31) && total_tokens * G < (1ll << 31), "%s: too many tokens", what);
   B2L_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
                   workspace_bytes >= workspace_for(pl, head_dim),

@@ -23,3 +23,5 @@ class AttentionMetadata:
     max_actual_seq_len: int = 0                                   # host int, sizes the split grid
     b_new_len: torch.Tensor | None = None                         # portions: tokens each sequence brings this step (flat batch)
     max_new_len: int = 0                                          # portions: host int, the longest of them
+    num_singles: int = 0                                          # sequences in front that bring one token each
+    max_single_len: int = 0                                       # host int, the longest history of those

@@ -265,9 +265,14 @@ class Decoder:
 
             update_kv_buffer_split(xk, xv, atten_info.cur_select_index, kv_buffer)
         if group and atten_info.b_new_len is not None:                                  # portions, one flat batch
-            attn = flash_attention_int4(xq, kv_buffer, self.scale, atten_info.b_start_loc, atten_info.b_new_len,
-                                        atten_info.b_req_tokens_table, atten_info.b_req_idx, atten_info.b_seq_len,
-                                        atten_info.max_new_len, atten_info.max_actual_seq_len, self.num_kv_heads, group)
+            attn, n, table = torch.empty_like(xq, memory_format=torch.contiguous_format), atten_info.num_singles, atten_info.b_req_tokens_table
+            if n:
+                flash_decoding_int4(xq[:n], kv_buffer, self.scale, table, atten_info.b_req_idx[:n], atten_info.b_seq_len[:n],
+                                    atten_info.max_single_len, self.num_kv_heads, group, attn[:n])
+            if n < atten_info.b_req_idx.shape[0]:
+                flash_attention_int4(xq, kv_buffer, self.scale, atten_info.b_start_loc[n:], atten_info.b_new_len[n:], table,
+                                     atten_info.b_req_idx[n:], atten_info.b_seq_len[n:], atten_info.max_new_len,
+                                     atten_info.max_actual_seq_len, self.num_kv_heads, group, attn)
         elif seq_len > 1:                                                               # base.py:95-103
             attn = flash_attention2_no_pad(xq, xk, xv, self.scale * _LOG2E, atten_info.b_start_loc,
                                            atten_info.b_seq_len, atten_info.max_actual_seq_len)

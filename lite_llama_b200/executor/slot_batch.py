@@ -101,6 +101,9 @@ class SlotBatch:
         maps = build_slot_maps(at.b_req_idx, cached, at.b_new_len, at.b_req_tokens_table, sum(new_lens))
         at.cur_select_index, positions, at.b_start_loc, at.b_seq_len = maps
         at.max_new_len, at.max_actual_seq_len = max(new_lens), longest
+        # sequences of one token in front (the engine's decoding requests) take decode attention
+        at.num_singles = next((i for i, n in enumerate(new_lens) if n > 1), len(new_lens))
+        at.max_single_len = max(cached_lens[:at.num_singles], default=0) + 1
         self.reset()
         return positions.view(1, -1)
 

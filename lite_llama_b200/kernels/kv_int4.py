@@ -154,8 +154,9 @@ def _vector(t: torch.Tensor, n: int, name: str, what: str) -> None:
 
 
 def flash_decoding_int4(q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b_seq_len, max_actual_seq_len, num_kv_heads: int,
-                        group_size: int = 64) -> torch.Tensor:
-    """``flash_decoding`` over a 4-bit cache: one query ``q [B, Hq, D]`` per sequence against its cached tokens, ``qk_scale = 1/sqrt(D)``.
+                        group_size: int = 64, out=None) -> torch.Tensor:
+    """``flash_decoding`` over a 4-bit cache: one query ``q [B, Hq, D]`` per sequence against its cached tokens, ``qk_scale = 1/sqrt(D)``;
+    into ``out``, by default a new tensor.
 
     Scores, softmax and sums are held in 32 bits and the cached elements enter as they are, so the result is that of 32-bit attention
     over ``read_kv_buffer_int4``'s values before their rounding, rounded once.  A row of length 0, or of a request outside the table, is
@@ -164,14 +165,14 @@ def flash_decoding_int4(q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b
 
     The same arguments give the same bits.  Where a row's tokens are parted for the sum follows from the lengths of all rows, so a
     sequence's last bits may change with what stands beside it."""
-    args = (q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b_seq_len, max_actual_seq_len, num_kv_heads, group_size)
-    out = _native.kv4_decode(*args)
-    return _flash_decoding_int4(*args) if out is None else out
+    args = (q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b_seq_len, max_actual_seq_len, num_kv_heads, group_size, out)
+    got = _native.kv4_decode(*args)
+    return _flash_decoding_int4(*args) if got is None else got
 
 
 @no_grad
 def _flash_decoding_int4(q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, b_seq_len, max_actual_seq_len, num_kv_heads: int,
-                        group_size: int = 64) -> torch.Tensor:
+                        group_size: int = 64, out=None) -> torch.Tensor:
     what = "flash_decoding_int4"
     code = dtype_code(q, "q")
     if q.dim() != 3:
@@ -185,8 +186,11 @@ def _flash_decoding_int4(q, kv_buffer, qk_scale, b_req_tokens_table, b_req_idx, 
     _vector(b_seq_len, batch, "b_seq_len", what)
     address, stride, rows = _cache_rows(kv_buffer, num_kv_heads, d, group_size, what)
     table = _table(b_req_tokens_table, what)
-    _same_device(what, q, kv_buffer, b_req_tokens_table, b_req_idx, b_seq_len)
-    out = torch.empty((batch, hq, d), dtype=q.dtype, device=q.device)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
+        raise ValueError(f"{what}: out has the shape and type of q and a contiguous head_dim")
+    _same_device(what, q, kv_buffer, b_req_tokens_table, b_req_idx, b_seq_len, out)
+    if out is None:
+        out = torch.empty((batch, hq, d), dtype=q.dtype, device=q.device)
     if batch == 0:
         return out
     max_len = int(max_actual_seq_len)
@@ -242,7 +246,7 @@ def _flash_attention_int4(q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_
     if batch == 0 or tokens == 0:
         return out
     max_len = int(max_actual_seq_len)
-    nbytes = lib().b2l_flash_attention_int4_workspace_bytes(batch, tokens, int(max_new_len), hq, num_kv_heads, d, group_size, max_len)
+    nbytes = lib().b2l_flash_attention_int4_workspace_bytes(batch, tokens, hq, num_kv_heads, d, group_size, max_len)
     ws = workspace(max(nbytes, 16), q.device)
     check(lib().b2l_flash_attention_int4(
         out.data_ptr(), q.data_ptr(), address, stride, rows, b_start_loc.data_ptr(), index_width(b_start_loc, "b_start_loc"),

@@ -92,6 +92,8 @@ def test_attention_and_maps_refuse_what_does_not_fit():
         (lambda: K.flash_decoding_int4(q, cache, 0.1, table.long(), idx, idx, 8, 2), "int32 matrix"),
         (lambda: K.flash_decoding_int4(q, cache, 0.1, table, idx[:2], idx, 8, 2), "one entry per sequence"),
         (lambda: K.flash_decoding_int4(q, cache, 0.1, table, idx, idx, 8, 4), "takes 288 bytes"),
+        (lambda: K.flash_decoding_int4(q, cache, 0.1, table, idx, idx, 8, 2, out=q[:2]), "shape and type of q"),
+        (lambda: K.flash_decoding_int4(q, cache, 0.1, table, idx, idx, 8, 2, out=q.bfloat16()), "shape and type of q"),
         (lambda: K.flash_attention_int4(q, cache, 0.1, idx, idx, table, idx, idx, 2, 8, 3), "no multiple"),
         (lambda: K.flash_attention_int4(q, cache, 0.1, idx[:2], idx, table, idx, idx, 2, 8, 2), "one entry per sequence"),
         (lambda: K.flash_attention_int4(q, cache, 0.1, idx, idx, table, idx, idx, 2, 8, 2, out=q[:2]), "shape and type of q"),

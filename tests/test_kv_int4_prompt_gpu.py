@@ -105,10 +105,10 @@ def test_large_and_small_values(dtype, scale_q, scale_k, scale_v):
     _check(_call(step, 2, 64, 0.088), step, 2, 64, 0.088)
 
 
-@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("wide", [0, 600, 1100])
 def test_elements_past_the_range_of_halves(wide):
-    """Of a bf16 cache: as 65504.  wide: beside a long portion, whose operands are made before."""
-    step = _run([4, 600] if wide else [4], [40, 700] if wide else [40], 2, 1, 64, 64, torch.bfloat16)
+    """Of a bf16 cache: as 65504.  wide: beside a long portion, at 1100 tokens with operands that are made before."""
+    step = _run([4, wide] if wide else [4], [40, wide + 100] if wide else [40], 2, 1, 64, 64, torch.bfloat16)
     q, rows, start, new, table, req, n = step
     k, v, _, _ = O.values(rows, 1, 64, 64, torch.bfloat16)
     v = v.bfloat16()
@@ -124,7 +124,7 @@ def test_elements_past_the_range_of_halves(wide):
     assert ((out.double().abs().amax(-1) - w[:, :, 3].T * 65504).abs() <= 0.02 * w[:, :, 3].T * 65504 + 5).all()
 
 
-@pytest.mark.parametrize("count", [48, 200])             # a row block, and several with operands made before
+@pytest.mark.parametrize("count", [48, 200, 600])        # a row block, several, and more than four on average: operands made before
 def test_a_value_that_is_nan_reaches_only_the_rows_that_see_it(count):
     for where in (3, 60, count + 49):               # before the new tokens, among them, the last one
         q, rows, start, new, table, req, n = _run([count, 5], [count + 50, 20], 8, 2, 128, 64, torch.float16)
@@ -141,7 +141,7 @@ def test_a_value_that_is_nan_reaches_only_the_rows_that_see_it(count):
         assert torch.equal(out[~nan], fine[~nan])
 
 
-@pytest.mark.parametrize("count", [48, 200])
+@pytest.mark.parametrize("count", [48, 200, 300])
 def test_a_key_that_is_nan_reaches_only_the_rows_that_see_it(count):
     q, rows, start, new, table, req, n = _run([count], [count + 50], 8, 2, 128, 64, torch.bfloat16)
     k, v, _, _ = O.values(rows, 2, 128, 64, torch.bfloat16)
@@ -237,11 +237,29 @@ def test_scales_that_are_not_positive_are_refused():
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("hq,heads,d,group", SHAPES)
 def test_long_portions_of_every_shape(hq, heads, d, group, dtype):
-    """Several row blocks to a sequence, whose operands are made before, beside short ones."""
+    """Several row blocks to a sequence beside short ones."""
     new, lens = [300, 3, 0, 520], [301, 400, 9, 1111]
     step = _run(new, lens, hq, heads, d, group, dtype, gap=1)
     keep = _normal(*step[0].shape, dtype=dtype)
     _check(_call(step, heads, group, d**-0.5, out=keep.clone(), max_len=1200), step, heads, group, d**-0.5, keep)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,heads,d,group", SHAPES)
+def test_ready_operands_of_every_shape(hq, heads, d, group, dtype):
+    """More than four row blocks to a sequence on average, of which one has none and sees nothing."""
+    new, lens = [2000, 0, 1301], [2001, 40, 1500]
+    step = _run(new, lens, hq, heads, d, group, dtype, gap=1)
+    keep = _normal(*step[0].shape, dtype=dtype)
+    _check(_call(step, heads, group, d**-0.5, out=keep.clone(), max_len=2300), step, heads, group, d**-0.5, keep)
+
+
+def test_ready_operands_of_a_sequence_that_sees_nothing():
+    q, rows, start, new, table, req, n = _run([600, 600], [700, 600], 8, 2, 64, 32, torch.float16)
+    n = n * torch.tensor([1, 0], device="cuda", dtype=n.dtype)
+    out = _call((q, rows, start, new, table, req, n), 2, 32, 0.1, max_len=800)
+    assert not out[600:].any()
+    _check(out[:600], (q[:600], rows, start[:1], new[:1], table, req[:1], n[:1]), 2, 32, 0.1)
 
 
 def test_ready_operands_do_not_outgrow_their_limit():

