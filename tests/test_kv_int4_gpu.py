@@ -337,6 +337,13 @@ def test_decode_with_strides():
         _check(out, q, rows, table, req, n, 2, 32, 0.1)
 
 
+@pytest.mark.parametrize("batch,max_len", [(1, 0), (1, 5), (3, 1), (3, 2000), (200, 64), (70, 3000)])
+def test_decode_of_rows_that_see_nothing(batch, max_len):
+    rows, table, req, n = _step([1] * batch, 2, 64, 32, torch.float16, width=1)
+    q = _normal(batch, 4, 64, dtype=torch.float16)
+    assert not K.flash_decoding_int4(q, rows, 0.1, table, req, torch.zeros_like(n) if max_len else n, max_len, 2, 32).any()
+
+
 @pytest.mark.parametrize("lens", [[201, 17], [1500, 3000]], ids=str)
 def test_decode_into_a_tensor(lens):
     """A part of a larger tensor; the query itself."""

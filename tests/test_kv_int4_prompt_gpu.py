@@ -9,6 +9,8 @@ import torch
 
 import kv_int4_oracle as O
 from lite_llama_b200 import kernels as K
+from lite_llama_b200.kernels import kv_int4 as KV
+from lite_llama_b200.kernels import slot_maps as SM
 from test_kv_int4_gpu import DTYPES, SHAPES, _normal, _step
 
 pytestmark = pytest.mark.gpu
@@ -269,3 +271,47 @@ def test_ready_operands_do_not_outgrow_their_limit():
     b = _call(step, 2, 64, 0.1, max_len=1 << 20)
     _check(a, step, 2, 64, 0.1)
     _check(b, step, 2, 64, 0.1)
+
+
+def test_two_streams_and_a_graph_at_once():
+    """Two long portions on streams of their own beside a replayed one: each has its own workspace."""
+    steps = [_run([1400], [2000 + 100 * i], 8, 2, 128, 64, torch.float16) for i in range(3)]
+    want = [_call(s, 2, 64, 0.1) for s in steps]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = _call(steps[2], 2, 64, 0.1, max_new=1400, max_len=2200)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    outs = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(_call(steps[i], 2, 64, 0.1, max_new=1400, max_len=2000 + 100 * i))
+        with torch.cuda.stream(streams[2]):
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i]) and torch.equal(replayed, want[2])
+
+
+@pytest.mark.parametrize("new,lens", [([5, 1, 40], [90, 300, 40]), ([2000], [2500])], ids=str)
+def test_native_and_python_forms(new, lens):
+    """Both make the same call."""
+    step = _run(new, lens, 8, 2, 128, 64, torch.bfloat16, gap=1)
+    q, rows, start, fresh, table, req, n = step
+    keep = _normal(*q.shape, dtype=torch.bfloat16)
+    args = (q, rows, 0.1, start, fresh, table, req, n, max(new), max(lens), 2, 64)
+    assert torch.equal(KV._flash_attention_int4(*args, keep.clone()), K.flash_attention_int4(*args, out=keep.clone()))
+    args = (q[:len(new)], rows, 0.1, table, req, n, max(lens), 2, 64)
+    assert torch.equal(KV._flash_decoding_int4(*args), K.flash_decoding_int4(*args))
+    index = table[req[0].long(), :lens[0]].contiguous()
+    assert torch.equal(KV._read_kv_buffer_int4(rows, index, 2, 128, torch.bfloat16, 64), K.read_kv_buffer_int4(rows, index, 2, 128, torch.bfloat16, 64))
+    caches = [torch.zeros_like(rows) for _ in range(2)]
+    for write, cache in zip((KV._rope_kv_write_int4, K.rope_kv_write_int4), caches):
+        g = torch.Generator(device="cuda").manual_seed(1)
+        a, b, c, cos = (torch.randn(m, x, 128, device="cuda", generator=g).bfloat16() for m, x in ((lens[0], 8), (lens[0], 2), (lens[0], 2), (1, lens[0])))
+        write(a, b, c, cos.view(1, lens[0], 128), cos.view(1, lens[0], 128), index, cache, 1, lens[0], 64)
+    assert torch.equal(*caches) and caches[0].any()
+    total = sum(new)
+    maps = [f(req, n - fresh, fresh, t, total, None) for f, t in ((SM._build_slot_maps, table.clone()), (K.build_slot_maps, table.clone()))]
+    assert all(torch.equal(x, y) for x, y in zip(*maps))
