@@ -21,7 +21,7 @@
 // tensor cores read it, and one warp fetches whole operands; the softmax warps then have registers for a whole row of 128 scores
 // (S for both tiles in turn | P0 P1 | O0 | O1), which they free before the exponentials.  A step takes 2800 cycles, of which 2050 are
 // the exponentials' issue alone.  The kernel before takes 6 us for 8000 keys of 8 heads.
-// 512 tokens over 7500, 32 / 8 heads: 90 us (98 the other way).
+// 512 tokens over 7500, 32 / 8 heads: 86 us (98 the other way).
 // The operands are halves for both activation types: elements are rounded to 11 bits (as the 16-bit cache of an fp16 model rounds
 // them), which for bf16 models are three bits more than reading the cache into their type would leave; elements of those beyond 65504
 // count as 65504.  Queries of bf16 models are scaled by a power of two per row.  Probabilities are rounded to 11 bits, as in
@@ -769,70 +769,87 @@ __global__ void __launch_bounds__(256, 6) kv4_prompt_ready_kernel(const Params p
   if (tid < 4) reinterpret_cast<int*>(p.ready_nan + at)[tid] = nan_at[tid];
 }
 
-// Row blocks that several CTAs met in.  Bound by latency: a warp asks for the parts of its four rows together, and lengths and notes
-// were left in the workspace by the first CTA.
-template <typename T, int D>
+// Row blocks that several CTAs met in.  Bound by latency, or by the parts' bytes: a warp asks for the parts of its R rows together, before
+// their weights are known, and lanes share the largest scores and sums.
+template <typename T, int D, int R>
 __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(const Params p) {
   pdl_prologue();
-  constexpr int E = D / 32, kR = 4, kRowsHere = 8 * kR;
+  constexpr int E = D / 32, kTogether = 16 / R, kLook = 32 / R;      // parts of a row asked for together; lanes that look at one row's
   const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r0 = blockIdx.x * kRowsHere;
-  const int4 s = __ldcg(p.ws_item + b);           // row blocks before, m, start
+  const int r0 = blockIdx.x * 8 * R;
+  const int4 s = __ldcg(p.ws_item + b);           // row blocks before, m, start: left in the workspace by the first CTA
   const int rows = s.y * p.G;
   if (r0 >= rows) return;
   const int rb = r0 / kRows, nb = (rows + kRows - 1) / kRows;
   const int2 who = __ldcg(p.ws_info + s.x + kvh * nb + rb);
   const int n = who.y - who.x + 1;
   if (n < 2) return;                              // written by its only CTA
-  const int in_block = r0 - rb * kRows + warp * kR;
-  float acc[kR][E], M[kR], L[kR];
+  const int in_block = r0 - rb * kRows + warp * R, here = rows - (r0 + warp * R);
+  auto part_of = [&](int i) { return ((int64_t)(who.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + in_block; };
+  float x[kTogether][R][E], acc[R][E];
+  auto ask = [&](int from) {
 #pragma unroll
-  for (int k = 0; k < kR; ++k) {
-    M[k] = -INFINITY;
-    L[k] = 0.f;
+    for (int i = 0; i < kTogether; ++i) {
+      if (from + i >= n) continue;
+      const float* row = p.ws_o + part_of(from + i) * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[k][e] = 0.f;
-  }
-#pragma unroll 1
-  for (int i0 = 0; i0 < n; i0 += 2) {
-    float x[2][kR][E];
-    float2 ml[2][kR];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (i0 + i >= n) {
-#pragma unroll
-        for (int k = 0; k < kR; ++k) ml[i][k] = make_float2(-INFINITY, 0.f);
-        continue;
-      }
-      const int64_t part = ((int64_t)(who.x + i0 + i) * 2 + (i0 + i == 0 ? 1 : 0)) * kRows + in_block;
-#pragma unroll
-      for (int k = 0; k < kR; ++k) {
-        ml[i][k] = __ldcg(p.ws_ml + part + k);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[i][k][e] = __ldcg(p.ws_o + (part + k) * D + e * 32 + lane);
+      for (int k = 0; k < R; ++k) {
+        if (E == 4) *reinterpret_cast<float4*>(x[i][k]) = __ldcg(reinterpret_cast<const float4*>(row + k * D));
+        else if (E == 2) *reinterpret_cast<float2*>(x[i][k]) = __ldcg(reinterpret_cast<const float2*>(row + k * D));
+        else x[i][k][0] = __ldcg(row + k * D);
       }
     }
+  };
+  auto look = [&](int from) -> float2 {           // lane (row, part): its largest score and its sum
+    const int i = from + lane % kLook;
+    return i < n ? __ldcg(p.ws_ml + part_of(i) + lane / kLook) : make_float2(-INFINITY, 0.f);
+  };
+  ask(0);
+  const float2 first = look(0);
+  float M = first.x;
+#pragma unroll 1
+  for (int from = kLook; from < n; from += kLook) M = fmaxf(M, look(from).x);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+  for (int o = 1; o < kLook; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float base = M == -INFINITY ? 0.f : M;
+  float L = 0.f, w = 0.f;
 #pragma unroll
-      for (int k = 0; k < kR; ++k) {
-        if (ml[i][k].y == 0.f) continue;          // a part of keys that the row does not see: nothing was stored
-        const float mm = fmaxf(M[k], ml[i][k].x), base = mm == -INFINITY ? 0.f : mm;
-        const float a = fast_exp2(M[k] - base), w = fast_exp2(ml[i][k].x - base);
-        M[k] = mm;
-        L[k] = L[k] * a + ml[i][k].y * w;
+  for (int k = 0; k < R; ++k)
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[k][e] = acc[k][e] * a + x[i][k][e] * w;
+    for (int e = 0; e < E; ++e) acc[k][e] = 0.f;
+#pragma unroll 1
+  for (int from = 0; from < n; from += kTogether) {
+    if (from % kLook == 0) {
+      const float2 ml = from == 0 ? first : look(from);
+      w = ml.y == 0.f ? 0.f : fast_exp2(ml.x - base);      // 0: of keys that the row does not see, nothing was stored
+      if (w != 0.f) L += ml.y * w;
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i)
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const float wi = __shfl_sync(0xffffffffu, w, k * kLook + from % kLook + i);
+        if (wi != 0.f) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[k][e] = fmaf(x[i][k][e], wi, acc[k][e]);
+        }
       }
+    ask(from + kTogether);
   }
 #pragma unroll
-  for (int k = 0; k < kR; ++k) {
-    const int r = r0 + warp * kR + k;
-    if (r >= rows) return;
-    const int token = over_G(p, r), head = kvh * p.G + r - token * p.G;
-    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(s.z + token) * p.o_ts + (int64_t)head * p.o_hs;
+  for (int o = 1; o < kLook; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[e * 32 + lane] = from_f32<T>(L[k] == 0.f ? 0.f : acc[k][e] / L[k]);
+  for (int k = 0; k < R; ++k) {
+    const float sum = __shfl_sync(0xffffffffu, L, k * kLook), inv = sum == 0.f ? 0.f : 1.0f / sum;
+    if (k >= here) continue;
+    const int r = r0 + warp * R + k, token = over_G(p, r), head = kvh * p.G + r - token * p.G;
+    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(s.z + token) * p.o_ts + (int64_t)head * p.o_hs + lane * E;
+    if (p.o_vec && E == 4) {
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(acc[k][0] * inv, acc[k][1 % E] * inv), pack2<T>(acc[k][2 % E] * inv, acc[k][3 % E] * inv));
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) out[e] = from_f32<T>(acc[k][e] * inv);
+    }
   }
 }
 
@@ -844,6 +861,9 @@ struct Plan { int grid, smem, ready_tiles; int64_t items, rows, steps, ready_byt
 constexpr int kReadyBlocks = 5;
 // Their room in the workspace at most: 65536 keys of 8 heads.  It grows with batch * max_seq_len, of which ragged steps use a part.
 constexpr int64_t kReadyMost = 256ll << 20;
+// Parts of a row block from which on a warp merges one row at a time, sixteen parts together, instead of four rows, four parts together:
+// 64 tokens over 7500 (9 parts, 8 kv heads) 34.7 us and 39.4, 128 tokens (6 parts) 48.8 and 48.1, 256 tokens 67.5 and 61.7.
+constexpr int kManyParts = 8;
 
 Plan make_plan(int64_t batch, int64_t total, int G, int Hkv, int D, int64_t max_len) {
   Plan pl;
@@ -880,8 +900,11 @@ int launch(const Params& p, const Plan& pl, cudaStream_t st) {
   }
   b2l_launch(kern, dim3((unsigned)pl.grid), dim3(ready ? kReadyThreads : kThreads), (size_t)pl.smem, st, p);
   B2L_LAUNCH_CHECK();
-  const int64_t x = cdiv64(p.max_new * p.G, 32);
-  b2l_launch(kv4_prompt_merge_kernel<T, D>, dim3((unsigned)x, (unsigned)p.Hkv, (unsigned)p.batch), dim3(256), (size_t)0, st, p);
+  // many parts to a row block, or few: a row to a warp, or four
+  if (pl.grid > kManyParts * pl.items)
+    b2l_launch(kv4_prompt_merge_kernel<T, D, 1>, dim3((unsigned)cdiv64(p.max_new * p.G, 8), (unsigned)p.Hkv, (unsigned)p.batch), dim3(256), (size_t)0, st, p);
+  else
+    b2l_launch(kv4_prompt_merge_kernel<T, D, 4>, dim3((unsigned)cdiv64(p.max_new * p.G, 32), (unsigned)p.Hkv, (unsigned)p.batch), dim3(256), (size_t)0, st, p);
   B2L_LAUNCH_CHECK();
   return B2L_OK;
 }
