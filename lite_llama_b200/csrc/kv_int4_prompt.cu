@@ -28,8 +28,8 @@
 // flash_attention_tc.cu; sums, maxima and outputs are held in 32.
 // A value that is NaN enters as 0 and makes NaN of the rows that see it at the end, since 0 * NaN would reach the rows that do not.
 //
-// Work: key tiles of all row blocks of all sequences, in equal shares over one wave of CTAs (lengths are device data).  A row block in
-// several shares leaves parts in the workspace, which a second kernel adds up.
+// Work: key tiles of all row blocks of all sequences, in equal shares over one wave of CTAs (lengths are device data), down to one
+// (5 tokens over 300, 8 kv heads: 11.7 us, two tiles at least 17.2; 64 over 500: 19.6 and 30.9).  A row block in several shares leaves parts in the workspace, which a second kernel adds up.
 #include "kv_int4.cuh"
 #include "attention_tmem.cuh"
 #include <climits>
@@ -41,7 +41,6 @@ constexpr int kBM = 128, kBN = 128, kRows = 2 * kBM;
 constexpr int kThreads = 640, kConvert = 256, kReadyThreads = 384, kKStages = 2, kVStages = 2, kSegs = 4;
 constexpr int kUnits = 5, kUnitKeys = 64, kUnitPitch = 96;   // pitch: rows of four neighbours in different banks
 constexpr int kMaxBatch = 128;                    // sequences of a launch (their sizes lie in shared memory)
-constexpr int kMinSteps = 2;                      // key tiles of a share: below that the parts cost more than the tiles
 
 struct Params {
   const void* q; int64_t q_ts, q_hs; int q_vec;
@@ -240,8 +239,7 @@ __global__ void __launch_bounds__(READY ? kReadyThreads : kThreads, 1) kv4_promp
   __syncthreads();
   const uint32_t tmem_base = ctl->tmem_base;
 
-  const int total = prefix[p.batch], worth = (total + kMinSteps - 1) / kMinSteps;
-  const int shares = worth < (int)gridDim.x ? worth : (int)gridDim.x;
+  const int total = prefix[p.batch], shares = total < (int)gridDim.x ? total : (int)gridDim.x;
   int step = 0, step_end = 0;
   if ((int)blockIdx.x < shares) {
     step = (int)((int64_t)blockIdx.x * total / shares);
@@ -872,8 +870,7 @@ Plan make_plan(int64_t batch, int64_t total, int G, int Hkv, int D, int64_t max_
   const int lists = (2 * kMaxBatch + 1) * 4 + kMaxBatch * (int)sizeof(Seq);
   pl.items = (cdiv64(total * G, kRows) + rows) * Hkv;
   pl.steps = pl.items * tiles;
-  const int64_t worth = cdiv64(pl.steps, kMinSteps);
-  pl.grid = (int)(worth < b2l_num_sms() ? worth : b2l_num_sms());
+  pl.grid = (int)(pl.steps < b2l_num_sms() ? pl.steps : b2l_num_sms());
   if (pl.grid < 1) pl.grid = 1;
   pl.rows = 2ll * pl.grid * kRows;
   // A tile is read by every row block that sees it: converted once for all of them where they are several, with room for the tiles
