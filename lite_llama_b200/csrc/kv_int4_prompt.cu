@@ -857,6 +857,9 @@ struct Plan { int grid, smem, ready_tiles; int64_t items, rows, steps, ready_byt
 // 76.1 / 89.6 us ready, 72.7 / 80.2 / 98.5 converted beside the products; 256 (4 blocks): 66.5 and 64.6; 6 x 290 / 400 at most over 1200:
 // 73.2 / 82.3 and 76.2 / 90.0; 6 x 200: 58.5 and 54.2.
 constexpr int kReadyBlocks = 5;
+// And steps of a CTA, by the bounds.  One portion of 1000 tokens over none / 1000 (7 / 15 steps): 52.6 / 61.0 us ready, 49.9 / 64.2 the other
+// way; 500 over 1000 / 2000 / 4000 (6 / 10 / 17): 45.5 / 51.9 / 64.7 and 44.7 / 51.4 / 68.1; 2000 over 6000: 215 and 279.
+constexpr int kReadySteps = 10;
 // Their room in the workspace at most: 65536 keys of 8 heads.  It grows with batch * max_seq_len, of which ragged steps use a part.
 constexpr int64_t kReadyMost = 256ll << 20;
 // Parts of a row block from which on a warp merges one row at a time, sixteen parts together, instead of four rows, four parts together:
@@ -876,7 +879,8 @@ Plan make_plan(int64_t batch, int64_t total, int G, int Hkv, int D, int64_t max_
   // A tile is read by every row block that sees it: converted once for all of them where they are several, with room for the tiles
   // of the bounds.
   const int64_t tile = 2ll * kBN * DP * 2;
-  const bool ready = total * G > (kReadyBlocks - 1) * kRows * batch && rows * Hkv * tiles <= kReadyMost / tile;
+  const bool ready = total * G > (kReadyBlocks - 1) * kRows * batch && rows * Hkv * tiles <= kReadyMost / tile &&
+                     pl.steps >= (int64_t)kReadySteps * b2l_num_sms();
   pl.ready_tiles = ready ? (int)tiles : 0;
   pl.ready_bytes = ready ? rows * Hkv * tiles * (tile + 16) : 0;
   pl.smem = 1024 + (2 + kKStages + kVStages) * kBN * DP * 2 + (ready ? 0 : kUnits * kUnitKeys * kUnitPitch) + lists;
