@@ -485,6 +485,8 @@ __global__ void __launch_bounds__(READY ? kReadyThreads : kThreads, 1) kv4_promp
     uint32_t par = 0;                             // of the key tiles
     int nseg = 0;
     for (; next(seg, seq); ++nseg) {
+      // A row tile without keys here has nothing to wait for: it must not arrive for a segment before all have left the slot's last one.
+      if (nseg >= kSegs) kv4_wait(&ctl->seg_done[nseg % kSegs], (uint32_t)(nseg / kSegs - 1) & 1u);
       const int nt = key_tiles(p, seq, seg.rb, t), j_end = nt < seg.j1 ? nt : seg.j1;
       const int r = seg.rb * kRows + t * kBM + row;
       const int token = over_G(p, r), head = seg.kvh * G + r - token * G;

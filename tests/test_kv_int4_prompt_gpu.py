@@ -320,3 +320,20 @@ def test_native_and_python_forms(new, lens):
     total = sum(new)
     maps = [f(req, n - fresh, fresh, t, total, None) for f, t in ((SM._build_slot_maps, table.clone()), (K.build_slot_maps, table.clone()))]
     assert all(torch.equal(x, y) for x, y in zip(*maps))
+
+
+def test_many_row_blocks_of_one_tile_to_a_cta():
+    """More short sequences and heads than CTAs, by a factor: a CTA's second row tile has nothing to do in any of them."""
+    new = [1 + i % 7 for i in range(128)]
+    lens = [m + i % 50 for i, m in enumerate(new)]
+    for d, group in ((64, 32), (128, 64)):
+        step = _run(new, lens, 32, 16, d, group, torch.float16)
+        _check(_call(step, 16, group, 0.1), step, 16, group, 0.1)
+
+
+def test_a_short_sequence_of_many_heads_behind_long_portions():
+    """The last CTA has the short one's eight heads, a row block of one tile each; operands are made ready."""
+    new, lens = [512, 388, 512, 118, 512, 3], [1024, 900, 1024, 512, 512, 3]
+    step = _run(new, lens, 32, 8, 128, 64, torch.float16)
+    _check(_call(step, 8, 64, 0.088, max_len=LOOSE), step, 8, 64, 0.088)
+    _check(_call(step, 8, 64, 0.088), step, 8, 64, 0.088)
