@@ -174,7 +174,10 @@ int b2l_flash_decoding_int4(void* out, const void* q, const void* cache, int64_t
                             int64_t workspace_bytes, int dtype, void* stream);
 /* Portions of prompts over that cache, causal: the new_len[b] rows of q [total_tokens, Hq, D] from start_loc[b] on stand at the positions
  * seq_len[b] - new_len[b], ... and see the cached tokens up to their own.  Rows of no sequence are not written, a row that sees
- * nothing is zero; rows past total_tokens, new tokens past max_new_len and keys past max_seq_len or the table's width do not count. */
+ * nothing is zero; rows past total_tokens, new tokens past max_new_len and keys past max_seq_len or the table's width do not count.
+ * A row of q belongs to one sequence.  Where ranges overlap, a row holds what one of its sequences gives, and sequences past the
+ * row blocks of 256 (token, head of a kv head's group) pairs that disjoint ranges make at most (ceil(total_tokens * Hq / Hkv / 256)
+ * + the smaller of batch and 128, for every 128 sequences) are left out: their rows are not written. */
 int64_t b2l_flash_attention_int4_workspace_bytes(int64_t batch, int64_t total_tokens, int num_q_heads,
                                                  int num_kv_heads, int head_dim, int group, int64_t max_seq_len);
 int b2l_flash_attention_int4(void* out, const void* q, const void* cache, int64_t cache_row_stride, int64_t max_tokens,

@@ -52,6 +52,7 @@ struct Params {
   int batch, Hkv, G;
   uint64_t by_G;                                  // 2^64 / G, rounded up: n / G is the high half of n * by_G for n < 2^32 (G > 1)
   int64_t total, max_new, most;
+  uint32_t items;                                 // row blocks (of all kv heads) that the workspace has notes for
   float scale_log2;
   float* ws_o; float2* ws_ml; int2* ws_info; int4* ws_item;
   uint8_t* ready; int4* ready_nan; int ready_tiles;   // operands made before: tiles [sequence][kv head][ready_tiles], K's image and V's
@@ -216,6 +217,7 @@ __global__ void __launch_bounds__(READY ? kReadyThreads : kThreads, 1) kv4_promp
   tc_fence_after();
   if (warp == 0) {
     int steps = 0, blocks = 0;
+    bool full = false;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       const int b = b0 + lane;
       int s = b < p.batch ? prefix[b + 1] : 0;
@@ -226,10 +228,25 @@ __global__ void __launch_bounds__(READY ? kReadyThreads : kThreads, 1) kv4_promp
         const int x = __shfl_up_sync(0xffffffffu, s, o), y = __shfl_up_sync(0xffffffffu, k, o);
         if (lane >= o) { s += x; k += y; }
       }
+      // Disjoint ranges of q fit into the workspace by its size.  Of others (stale starts), the sequences from the first on that does not fit
+      // are left out.  (The sum up to it is below 2^32; what stands behind it in the scan is not used.)
+      const unsigned past = __ballot_sync(0xffffffffu, full || (uint32_t)blocks + (uint32_t)k > p.items);
+      bool out = false;
+      if (past != 0u) {
+        const int first = __ffs(past) - 1, from = first > 0 ? first - 1 : 0;
+        const int s_kept = __shfl_sync(0xffffffffu, s, from), k_kept = __shfl_sync(0xffffffffu, k, from);
+        full = true;
+        out = lane >= first;
+        if (out) {
+          s = first > 0 ? s_kept : 0;
+          k = first > 0 ? k_kept : 0;
+        }
+      }
       if (b < p.batch) {
+        const int before = blocks + k - (out ? 0 : own);
         prefix[b + 1] = steps + s;
-        items[b] = blocks + k - own;
-        if (blockIdx.x == 0) p.ws_item[b] = make_int4(blocks + k - own, seqs[b].m, seqs[b].start, 0);
+        items[b] = before;
+        if (blockIdx.x == 0) p.ws_item[b] = make_int4(before, out ? 0 : seqs[b].m, seqs[b].start, 0);
       }
       steps += __shfl_sync(0xffffffffu, s, 31);
       blocks += __shfl_sync(0xffffffffu, k, 31);
@@ -873,7 +890,7 @@ Plan make_plan(int64_t batch, int64_t total, int G, int Hkv, int D, int64_t max_
   const int DP = D < 64 ? 64 : D;
   const int64_t rows = batch < kMaxBatch ? batch : kMaxBatch, tiles = cdiv64(max_len > 0 ? max_len : 1, kBN);
   const int lists = (2 * kMaxBatch + 1) * 4 + kMaxBatch * (int)sizeof(Seq);
-  pl.items = (cdiv64(total * G, kRows) + rows) * Hkv;
+  pl.items = (cdiv64(total * G, kRows) + rows) * Hkv;   // of disjoint ranges of q at most; the kernel takes no more
   pl.steps = pl.items * tiles;
   pl.grid = (int)(pl.steps < b2l_num_sms() ? pl.steps : b2l_num_sms());
   if (pl.grid < 1) pl.grid = 1;
@@ -962,6 +979,7 @@ extern "C" int b2l_flash_attention_int4(void* out, const void* q, const void* ca
   p.Hkv = num_kv_heads; p.G = G; p.by_G = G > 1 ? ~0ull / G + 1 : 0;
   p.total = total_tokens; p.max_new = max_new_len < total_tokens ? max_new_len : total_tokens;
   p.most = most < 0 ? 0 : most;
+  p.items = (uint32_t)pl.items;
   p.scale_log2 = qk_scale * 1.4426950408889634f;
   char* ws = (char*)workspace;
   p.ready = (uint8_t*)ws;

@@ -213,6 +213,8 @@ def flash_attention_int4(q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_t
     65504), and so are the probabilities; sums and the softmax are held in 32 bits.  ``max_new_len`` and ``max_actual_seq_len`` are
     bounds that the host knows: new tokens and keys past them do not count.  A row that sees nothing is zero; rows of ``q`` that belong to no
     sequence are not written (``out``, by default a new tensor, keeps what it held there); a table entry outside the cache reads row 0.
+    A row belongs to one sequence: where the ranges overlap (starts of an earlier step), it holds what one of its sequences gives, and
+    sequences past the row blocks that disjoint ranges could make are left out, their rows not written.
 
     The same arguments give the same bits; where a row's keys are parted for the sum follows from all lengths of the step."""
     args = (q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_tokens_table, b_req_idx, b_seq_len, max_new_len, max_actual_seq_len,
