@@ -191,7 +191,8 @@ int b2l_flash_attention_int4(void* out, const void* q, const void* cache, int64_
 /* Slot maps of a ragged step: start[b] = sum of new_len over the requests before b, length[b] = ctx_len[b] + new_len[b] (int32 [batch]);
  * for token t of the flat batch, the j-th new one of request b: position[t] = ctx_len[b] + j (int64), rows[t] (int32) =
  * table[req_idx[b], position], or, with pool_rows, pool_rows[t], which is entered there.  Tokens behind the last request: row -1,
- * position 0; a request or position outside the table: row -1.  Negative lengths count as 0. */
+ * position 0; a request or position outside the table: row -1.  Negative lengths count as 0, those past 2^31 - 1 as that, which start and
+ * length do not pass either. */
 int b2l_slot_maps(void* rows, void* position, void* start, void* length, const void* req_idx, int req_width, const void* ctx_len,
                   int ctx_width, const void* new_len, int new_width, const void* pool_rows, int pool_width, void* table,
                   int64_t table_req_stride, int64_t table_seq_stride, int64_t requests, int64_t width, int64_t batch,

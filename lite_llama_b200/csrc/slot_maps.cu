@@ -5,6 +5,7 @@
 // start(b) = sum of new(b') over b' < b.  Token t belongs to the last b with start(b) <= t and new(b) > 0.  Every block adds up the
 // lengths by itself, 1024 at a time, instead of a scan with a second launch: latency is the bound (a step's lengths are a few KB in L2).
 #include "common.cuh"
+#include <cstdint>
 
 namespace {
 
@@ -19,6 +20,13 @@ struct MapParams {
   int64_t batch, total;
 };
 
+// a length as it counts: 64-bit ones too fit into 32 bits, so that no sum of them leaves 64
+__device__ __forceinline__ int64_t length_of(const void* lens, int64_t b, int width) {
+  const int64_t n = load_index(lens, b, width);
+  return n < 0 ? 0 : n > INT32_MAX ? INT32_MAX : n;
+}
+__device__ __forceinline__ int32_t int32_at_most(int64_t n) { return n > INT32_MAX ? INT32_MAX : (int32_t)n; }
+
 __global__ void __launch_bounds__(kThreads) slot_maps_kernel(const MapParams p) {
   pdl_prologue();
   __shared__ int64_t ends[kChunk];                 // of the requests in hand, in the flat batch
@@ -32,8 +40,7 @@ __global__ void __launch_bounds__(kThreads) slot_maps_kernel(const MapParams p) 
     int64_t n[kPer], own = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int64_t x = b + i < p.batch ? load_index(p.fresh, b + i, p.fresh_w) : 0;
-      n[i] = x > 0 ? x : 0;
+      n[i] = b + i < p.batch ? length_of(p.fresh, b + i, p.fresh_w) : 0;
       own += n[i];
     }
     int64_t upto = own;
@@ -50,9 +57,8 @@ __global__ void __launch_bounds__(kThreads) slot_maps_kernel(const MapParams p) 
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       if (heads && b + i < p.batch) {
-        p.start[b + i] = (int32_t)at;
-        const int64_t c = load_index(p.ctx, b + i, p.ctx_w);
-        p.length[b + i] = (int32_t)((c > 0 ? c : 0) + n[i]);
+        p.start[b + i] = int32_at_most(at);
+        p.length[b + i] = int32_at_most(length_of(p.ctx, b + i, p.ctx_w) + n[i]);
       }
       at += n[i];
       ends[threadIdx.x * kPer + i] = at;
@@ -69,8 +75,7 @@ __global__ void __launch_bounds__(kThreads) slot_maps_kernel(const MapParams p) 
         else count = half;
       }
       const int64_t begin = first > 0 ? ends[first - 1] : base;
-      const int64_t c = load_index(p.ctx, b0 + first, p.ctx_w), r = load_index(p.req, b0 + first, p.req_w);
-      const int64_t pos = (c > 0 ? c : 0) + t - begin;
+      const int64_t r = load_index(p.req, b0 + first, p.req_w), pos = length_of(p.ctx, b0 + first, p.ctx_w) + t - begin;
       int32_t row = -1;
       if (r >= 0 && r < p.requests && pos < p.width) {
         int32_t* entry = p.table + r * p.tab_rs + pos * p.tab_cs;
