@@ -4,10 +4,14 @@
 //
 // Elements are not formed.  With codes c, q . k = sum over groups (s q . c + m sum(q)), so a key's scales meet the finished sums of
 // its codes; and out = sum_t (p s) c + sum_t p m, so a value's scale is multiplied into the probability.  What is left of unpacking is
-// a mask: the four bits of a code, in a half's lowest bits, ARE the subnormal half 2^-24 c (one place higher 2^-20 c), and a product
-// of it is exact.  Five integer instructions turn a word of eight key codes into operands, six one of value codes.
+// a shift and a mask: four bits inside a half's fraction ARE a subnormal half, 2^-24 c in the lowest places, and a product of it is exact.
+// The SUM of products is not: a tensor core lines products up by their operands' exponents, a subnormal's being 2^-14 however small it is,
+// and drops what lies 24 bits or so below the largest.  Measured against the largest product of 16: 2^-15.9 with codes in the lowest places,
+// 2^-20.4 four places higher, 2^-21.9 six.  So keys' codes go to bits 4 - 7 (seven integer instructions for a word of eight), values', which
+// all add up with one sign, to the top of the fraction, bits 6 - 9 (eight).  (With the codes in the lowest places, five: 32 rows of 1000 - 2000
+// tokens take 29.0 us instead of 30.2, and a query with one large element is off by 2^-14 of its score's parts.)
 // The tokens are the 16 rows of an mma.sync tile and the group's query heads its 8 columns: the cache is the operand that fills the
-// tile.  Queries are scaled by a power of two per head to the middle of the range of halves, which is exact down to 2^-29 of the
+// tile.  Queries are scaled by a power of two per head to the middle of the range of halves, which is exact down to 2^-32 of the
 // head's largest element.  Probabilities are not rounded to 11 bits: what rounding leaves of p s is multiplied as well -- in the
 // columns that up to four heads leave free, else in a second product -- since a code's products are larger than its value's.
 //
@@ -67,9 +71,9 @@ template <typename T, int D, int GS, bool DUP>
 struct Int4Consumer {
   static constexpr int NG = D / GS, NW = D / 32, MT = D / 16, U = units_of(D, GS);
   uint4 raw[NW];                                  // the query as it is in memory, between ask() and begin()
-  uint32_t qb[NW][4];                             // a key word's query elements: nibbles (0, 4), (2, 6), (1, 5) / 16, (3, 7) / 16
+  uint32_t qb[NW][4];                             // a key word's query elements: nibbles (0, 4), (2, 6), (1, 5), (3, 7)
   float f[2], sq[2][NG];                          // per column: what a sum of codes is multiplied by; scaled sums of the query
-  float O[MT][4], z[2][NG];                       // sums of p s c (rows r + 8 hold 16 times theirs) and of p m
+  float O[MT][4], z[2][NG];                       // sums of p s c and of p m
   float m[2], base[2], l[2], m_lim[2];            // the maximum (base: 0 instead of -inf) that sums are relative to; above m_lim it is raised
   float v_scale, v_lim;                           // value scales are multiplied by v_scale = 2^-e before p s is rounded
   int r, c;
@@ -126,24 +130,23 @@ struct Int4Consumer {
     if (!(big < INFINITY) || big == 0.f) e = 0;
     constexpr int kMost = std::is_same<T, __half>::value ? 15 : 100;
     e = e < -kMost ? -kMost : e > kMost ? kMost : e;
-    const float up = exp2i(e);
-    const T2 lo = pair2(up), hi = pair2(up * 0.0625f);
+    const T2 by = pair2(exp2i(e));
     float sums[NG][4];
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
       for (int i = 0; i < 4; ++i) sums[g][i] = 0.f;
-    const uint32_t one[4] = {0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u}, one16[4] = {0x00100010u, 0x00100010u, 0x00100010u, 0x00100010u};
+    const uint32_t one[4] = {0x00100010u, 0x00100010u, 0x00100010u, 0x00100010u};
 #pragma unroll
     for (int k = 0; k < NW; ++k) {
-      qb[k][0] = to_half2(__hmul2(as2(__byte_perm(raw[k].x, raw[k].z, 0x5410)), lo));
-      qb[k][1] = to_half2(__hmul2(as2(__byte_perm(raw[k].y, raw[k].w, 0x5410)), lo));
-      qb[k][2] = to_half2(__hmul2(as2(__byte_perm(raw[k].x, raw[k].z, 0x7632)), hi));
-      qb[k][3] = to_half2(__hmul2(as2(__byte_perm(raw[k].y, raw[k].w, 0x7632)), hi));
+      qb[k][0] = to_half2(__hmul2(as2(__byte_perm(raw[k].x, raw[k].z, 0x5410)), by));
+      qb[k][1] = to_half2(__hmul2(as2(__byte_perm(raw[k].y, raw[k].w, 0x5410)), by));
+      qb[k][2] = to_half2(__hmul2(as2(__byte_perm(raw[k].x, raw[k].z, 0x7632)), by));
+      qb[k][3] = to_half2(__hmul2(as2(__byte_perm(raw[k].y, raw[k].w, 0x7632)), by));
       mma(sums[group_of(k)], one, qb[k][0], qb[k][1]);
-      mma(sums[group_of(k)], one16, qb[k][2], qb[k][3]);
+      mma(sums[group_of(k)], one, qb[k][2], qb[k][3]);
     }
-    const float back = p.scale_log2 * exp2i(-e) * 16777216.f;
+    const float back = p.scale_log2 * exp2i(-e) * 1048576.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       f[j] = __shfl_sync(0xffffffffu, back, (2 * c + j) * 4);
@@ -211,7 +214,7 @@ struct Int4Consumer {
 
   // 16 U tokens at `at` (the head's bytes of the first), of which `valid` count
   __device__ __forceinline__ void tile(const uint8_t* at, int valid) {
-    constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+    constexpr uint32_t kKey = 0x00f000f0u, kValue = 0x03c003c0u;   // 2^-20 code and 2^-18 code as halves
     // ---- scores: 16 tokens (rows) and 8 heads (columns) to a unit ----
     float acc[U][NG][4];
     uint32_t vg[U][2][NG];                        // the values' groups
@@ -237,9 +240,8 @@ struct Int4Consumer {
         for (int i = 0; i < 4; ++i) acc[n][g][i] = 0.f;
 #pragma unroll
       for (int k = 0; k < NW; ++k) {
-        const uint32_t x0 = w0[k] >> 8, x1 = w1[k] >> 8;
-        const uint32_t lo[4] = {w0[k] & kLow, w1[k] & kLow, x0 & kLow, x1 & kLow};
-        const uint32_t hi[4] = {w0[k] & kHigh, w1[k] & kHigh, x0 & kHigh, x1 & kHigh};
+        const uint32_t lo[4] = {w0[k] << 4 & kKey, w1[k] << 4 & kKey, w0[k] >> 4 & kKey, w1[k] >> 4 & kKey};
+        const uint32_t hi[4] = {w0[k] & kKey, w1[k] & kKey, w0[k] >> 8 & kKey, w1[k] >> 8 & kKey};
         mma(acc[n][group_of(k)], lo, qb[k][0], qb[k][1]);
         mma(acc[n][group_of(k)], hi, qb[k][2], qb[k][3]);
       }
@@ -336,9 +338,8 @@ struct Int4Consumer {
         for (int g = 0; g < NG; ++g) {
           auto word = [&](int o) { return *reinterpret_cast<const uint32_t*>(u + o + g * 16); };
           const uint32_t x = __byte_perm(word(v_at[0]), word(v_at[1]), pick), y = __byte_perm(word(v_at[0] + step), word(v_at[1] + step), pick);
-          const uint32_t a0[4] = {x & kLow, x & kHigh, y & kLow, y & kHigh};
-          const uint32_t x8 = x >> 8, y8 = y >> 8;
-          const uint32_t a1[4] = {x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh};
+          const uint32_t a0[4] = {x << 6 & kValue, x << 2 & kValue, y << 6 & kValue, y << 2 & kValue};
+          const uint32_t a1[4] = {x >> 2 & kValue, x >> 6 & kValue, y >> 2 & kValue, y >> 6 & kValue};
           add(g * 2, g, a0);
           add(g * 2 + 1, g, a1);
         }
@@ -351,9 +352,8 @@ struct Int4Consumer {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t x = __byte_perm(e0, e1, h ? 0x7632 : 0x5410), y = __byte_perm(e2, e3, h ? 0x7632 : 0x5410);
-            const uint32_t a0[4] = {x & kLow, x & kHigh, y & kLow, y & kHigh};
-            const uint32_t x8 = x >> 8, y8 = y >> 8;
-            const uint32_t a1[4] = {x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh};
+            const uint32_t a0[4] = {x << 6 & kValue, x << 2 & kValue, y << 6 & kValue, y << 2 & kValue};
+            const uint32_t a1[4] = {x >> 2 & kValue, x >> 6 & kValue, y >> 2 & kValue, y >> 6 & kValue};
             add(b * 4 + h * 2, g, a0);
             add(b * 4 + h * 2 + 1, g, a1);
           }
@@ -368,7 +368,7 @@ struct Int4Consumer {
   }
   // sums in true units, complete over the lanes
   __device__ __forceinline__ void finish() {
-    const float by = 16777216.f / v_scale;
+    const float by = 262144.f / v_scale;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -386,7 +386,7 @@ struct Int4Consumer {
         }
         const int g = GS == 32 ? t >> 1 : (t >> 2) * 64 / GS;
         O[t][j] = fmaf(lo, by, z[j][g]);
-        O[t][2 + j] = fmaf(hi, by * 0.0625f, z[j][g]);
+        O[t][2 + j] = fmaf(hi, by, z[j][g]);
       }
     }
   }
