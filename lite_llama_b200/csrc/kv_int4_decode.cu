@@ -20,6 +20,7 @@
 // an SM leave a thread 96 registers, and spill); a warp takes 16 or 32 tokens of one kv head.  A row
 // that lies in one share is written out; else its parts go to the workspace and a second kernel adds them up.
 #include "kv_int4.cuh"
+#include "attention_tmem.cuh"
 #include <type_traits>
 
 namespace {
@@ -75,7 +76,8 @@ struct Int4Consumer {
   float f[2], sq[2][NG];                          // per column: what a sum of codes is multiplied by; scaled sums of the query
   float O[MT][4], z[2][NG];                       // sums of p s c and of p m
   float m[2], base[2], l[2], m_lim[2];            // the maximum (base: 0 instead of -inf) that sums are relative to; above m_lim it is raised
-  float v_scale, v_lim;                           // value scales are multiplied by v_scale = 2^-e before p s is rounded
+  float v_scale[2][NG];                           // powers of two that p s is multiplied by before it is rounded
+  static constexpr int kMostUp = 118;             // 2^kMostUp at most: times 2^8, a number
   int r, c;
   int k_at, g_at, v_at[2], step;                   // bytes from a unit's first row: key words, groups, value words of two tokens; eight rows
 
@@ -162,14 +164,15 @@ struct Int4Consumer {
       m[j] = m_lim[j] = -INFINITY;
       l[j] = base[j] = 0.f;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) z[j][g] = 0.f;
+      for (int g = 0; g < NG; ++g) {
+        z[j][g] = 0.f;
+        v_scale[j][g] = exp2i(kMostUp);
+      }
     }
-    v_scale = 1.f;
-    v_lim = -1.f;
   }
 
-  // a score above what the sums are scaled for, or a value scale: raise either
-  __device__ __forceinline__ void raise(const float (&v)[U][2][2], float vs) {
+  // a score above what the sums are scaled for: the maximum rises, and the sums so far are worth `fell` of what they were (O is left to rescale())
+  __device__ __forceinline__ void raise(const float (&v)[U][2][2], float (&fell)[2]) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       float mx = v[0][0][j];
@@ -183,23 +186,51 @@ struct Int4Consumer {
         l[j] *= a;
 #pragma unroll
         for (int g = 0; g < NG; ++g) z[j][g] *= a;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) { O[t][j] *= a; O[t][2 + j] *= a; }
+        fell[j] = a;
       }
       m_lim[j] = m[j] + 8.f;
     }
-    const uint32_t top = __reduce_max_sync(0xffffffffu, vs > v_lim && vs < INFINITY ? __float_as_uint(vs) : 0u);
-    if (v_lim < 0.f || top != 0u) {
-      int e = (int)(top >> 23) - 127;
-      e = e < -100 ? -100 : e > 120 ? 120 : e;
-      const float next = exp2i(-e), by = v_lim < 0.f ? 1.f : next / v_scale;
-      v_scale = next;
-      v_lim = exp2i(e + 6);
+  }
+
+  // The power of two that a head's products with a group's scales are multiplied by before they are rounded to two halves, whose least
+  // step is 2^-24: the largest p s so far -- of the sums as they are worth now, and of these tokens -- comes to 2^7 or above.  By the products,
+  // per head and group, and not by the scales, which may lie any range apart: a wide token of little weight, or a wide group, must not take
+  // the digits of the others.  A larger power than the last one is allowed by as much as the sums have fallen.  (One power for a warp, by
+  // the largest scale: one row of 201 tokens 6.6 us instead of 6.85, the larger cases level; a value 2^-20 of a scale seen before was off by 1 %.)
+  __device__ __forceinline__ void rescale(const float (&pr)[U][2][2], const uint32_t (&vg)[U][2][NG], const float (&fell)[2], bool fresh) {
+    // powers of two by their exponents alone: what `fell` leaves room for (2^127 where nothing is left)
+    float up[2];
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+    for (int j = 0; j < 2; ++j) up[j] = __uint_as_float(0x7f000000u - (__float_as_uint(fell[j]) & 0x7f800000u));
+    float by[2][NG];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) O[t][i] *= by;
+    for (int g = 0; g < NG; ++g) {
+      float top[2] = {0.f, 0.f};                  // of what is a number
+#pragma unroll
+      for (int n = 0; n < U; ++n) {
+        const float s0 = kv4::scale_min<T>(vg[n][0][g]).x, s1 = kv4::scale_min<T>(vg[n][1][g]).x;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) top[j] = max3(top[j], pr[n][0][j] * s0, pr[n][1][j] * s1);
+      }
+      uint32_t e = __float_as_uint(top[0]) >> 23 | __float_as_uint(top[1]) >> 23 << 16;      // of both heads
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) e = __vmaxu2(e, __shfl_xor_sync(0xffffffffu, e, o));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int want = 134 + 127 - (int)(j ? e >> 16 : e & 0xffffu);
+        const float next = fminf(__int_as_float((want < 127 + kMostUp ? want : 127 + kMostUp) << 23), v_scale[j][g] * up[j]);
+        by[j][g] = fell[j] * next * __uint_as_float(0x7f000000u - __float_as_uint(v_scale[j][g]));
+        v_scale[j][g] = next;
+      }
     }
+    if (fresh) return;                            // O is zero
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        O[t][j] *= by[j][t * 16 / GS];
+        O[t][2 + j] *= by[j][t * 16 / GS];
+      }
   }
 
   __device__ __forceinline__ Int4Consumer(int lane, int pitch) {
@@ -212,8 +243,8 @@ struct Int4Consumer {
     v_at[1] = place(2 * c + 1) * pitch + D / 2 + (GS == 32 ? r >> 1 : r) * 4;
   }
 
-  // 16 U tokens at `at` (the head's bytes of the first), of which `valid` count
-  __device__ __forceinline__ void tile(const uint8_t* at, int valid) {
+  // 16 U tokens at `at` (the head's bytes of the first), of which `valid` count; fresh: the first of a part
+  __device__ __forceinline__ void tile(const uint8_t* at, int valid, bool fresh) {
     constexpr uint32_t kKey = 0x00f000f0u, kValue = 0x03c003c0u;   // 2^-20 code and 2^-18 code as halves
     // ---- scores: 16 tokens (rows) and 8 heads (columns) to a unit ----
     float acc[U][NG][4];
@@ -246,7 +277,6 @@ struct Int4Consumer {
         mma(acc[n][group_of(k)], hi, qb[k][2], qb[k][3]);
       }
     }
-    float top = 0.f;
 #pragma unroll
     for (int n = 0; n < U; ++n)
 #pragma unroll
@@ -264,6 +294,7 @@ struct Int4Consumer {
           ks[g] = kv4::scale_min<T>(word[g]);
           vg[n][i][g] = word[NG + g];
         }
+        float tu[2], uu[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float t = ks[0].x * acc[n][0][2 * i + j], u = ks[0].y * sq[j][0];
@@ -272,8 +303,10 @@ struct Int4Consumer {
             t = fmaf(ks[g].x, acc[n][g][2 * i + j], t);
             u = fmaf(ks[g].y, sq[j][g], u);
           }
-          v[n][i][j] = fmaf(t, f[j], u);
+          tu[j] = t;
+          uu[j] = u;
         }
+        f32x2_split(f32x2_fma(f32x2(tu[0], tu[1]), f32x2(f[0], f[1]), f32x2(uu[0], uu[1])), v[n][i][0], v[n][i][1]);
       }
     if (valid < 16 * U) {                         // a row's last tokens
 #pragma unroll
@@ -286,27 +319,40 @@ struct Int4Consumer {
             for (int g = 0; g < NG; ++g) vg[n][i][g] = 0u;
           }
     }
-    bool over = false;
+    // the largest of a thread's 2 U values of either head
+    auto largest = [](const float (&x)[U][2][2], int j) {
+      const float y = fmaxf(x[0][0][j], x[0][1][j]);
+      return U == 1 ? y : max3(y, x[U - 1][0][j], x[U - 1][1][j]);
+    };
+    float fell[2] = {1.f, 1.f};
+    const bool risen = __any_sync(0xffffffffu, largest(v, 0) > m_lim[0] || largest(v, 1) > m_lim[1]);
+    if (risen) raise(v, fell);
+    // ---- probabilities; whether a product with a scale may be past the range of halves ----
+    float pr[U][2][2];
 #pragma unroll
-    for (int n = 0; n < U; ++n) {
+    for (int n = 0; n < U; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) over |= fmaxf(v[n][0][j], v[n][1][j]) > m_lim[j];
+      for (int i = 0; i < 2; ++i) {
+        f32x2_split(f32x2_add(f32x2(v[n][i][0], v[n][i][1]), f32x2(-base[0], -base[1])), pr[n][i][0], pr[n][i][1]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2; ++j) pr[n][i][j] = fast_exp2(pr[n][i][j]);
+        f32x2_split(f32x2_add(f32x2(l[0], l[1]), f32x2(pr[n][i][0], pr[n][i][1])), l[0], l[1]);
+      }
+    const uint64_t p_top = f32x2(largest(pr, 0), largest(pr, 1));
+    float product = 0.f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) top = fmaxf(top, kv4::scale_min<T>(vg[n][i][g]).x);
+    for (int g = 0; g < NG; ++g) {
+      using T2 = typename Vec2<T>::type;
+      T2 s = __hmax2(as2(vg[0][0][g]), as2(vg[0][1][g]));
+      if (U == 2) s = __hmax2(s, __hmax2(as2(vg[U - 1][0][g]), as2(vg[U - 1][1][g])));
+      float a, b;
+      f32x2_split(f32x2_mul(p_top, f32x2(v_scale[0][g], v_scale[1][g])), a, b);
+      product = fmaxf(product, fmaxf(a, b) * kv4::scale_min<T>(*reinterpret_cast<uint32_t*>(&s)).x);
     }
-    if (__any_sync(0xffffffffu, over || top > v_lim)) raise(v, top);
+    if (__any_sync(0xffffffffu, risen || product > 32768.f)) rescale(pr, vg, fell, fresh);
 #pragma unroll
     for (int n = 0; n < U; ++n) {
       // ---- probabilities, times the values' scales, as the second product's columns ----
-      float pr[2][2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) pr[i][j] = fast_exp2(v[n][i][j] - base[j]);
-        l[j] += pr[0][j] + pr[1][j];
-      }
       uint32_t pb[NG][2], rest[NG][2];
 #pragma unroll
       for (int g = 0; g < NG; ++g)
@@ -314,11 +360,15 @@ struct Int4Consumer {
         for (int i = 0; i < 2; ++i) {
           const float2 vs = kv4::scale_min<T>(vg[n][i][g]);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) z[j][g] = fmaf(pr[i][j], vs.y, z[j][g]);
-          const float s = vs.x * v_scale, x = pr[i][0] * s, y = pr[i][1] * s;
+          for (int j = 0; j < 2; ++j) z[j][g] = fmaf(pr[n][i][j], vs.y, z[j][g]);
+          float x, y, dx, dy;
+          f32x2_split(f32x2_mul(f32x2(pr[n][i][0], pr[n][i][1]), f32x2(v_scale[0][g], v_scale[1][g])), x, y);
+          x *= vs.x;
+          y *= vs.x;
           const uint32_t near = pack2<__half>(x, y);
           const float2 back = halves(near);
-          const uint32_t left = pack2<__half>(x - back.x, y - back.y);
+          f32x2_split(f32x2_fma(f32x2(back.x, back.y), f32x2(-1.f, -1.f), f32x2(x, y)), dx, dy);
+          const uint32_t left = pack2<__half>(dx, dy);
           if (DUP) {
             pb[g][i] = trans8x8(c < 2 ? near : left);
           } else {
@@ -368,7 +418,6 @@ struct Int4Consumer {
   }
   // sums in true units, complete over the lanes
   __device__ __forceinline__ void finish() {
-    const float by = 262144.f / v_scale;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -385,8 +434,9 @@ struct Int4Consumer {
           hi += __shfl_xor_sync(0xffffffffu, hi, 2);
         }
         const int g = GS == 32 ? t >> 1 : (t >> 2) * 64 / GS;
-        O[t][j] = fmaf(lo, by, z[j][g]);
-        O[t][2 + j] = fmaf(hi, by, z[j][g]);
+        const float by = exp2i(127 - (int)(__float_as_uint(v_scale[j][g]) >> 23));
+        O[t][j] = fmaf(lo * 262144.f, by, z[j][g]);
+        O[t][2 + j] = fmaf(hi * 262144.f, by, z[j][g]);
       }
     }
   }
@@ -603,7 +653,7 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
     for (int t = seg.first; t < seg.last; ++t, ++at_tile) {
       mbar_wait(&full_bar[s], phase);
       const int valid = len - t * tile - ts * kWarpTokens;
-      if (valid > 0) c.tile(ring + s * stage_bytes + off, valid);
+      if (valid > 0) c.tile(ring + s * stage_bytes + off, valid, t == seg.first);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[s]);
       if (at_tile > 0 && ahead.more) {            // into the stage of the tile before this one, which the others have left by now
