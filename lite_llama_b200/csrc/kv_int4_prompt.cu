@@ -24,7 +24,7 @@
 // 512 tokens over 7500, 32 / 8 heads: 86 us (98 the other way).
 // The operands are halves for both activation types: elements are rounded to 11 bits (as the 16-bit cache of an fp16 model rounds
 // them), which for bf16 models are three bits more than reading the cache into their type would leave; elements of those beyond 65504
-// count as 65504.  Queries of bf16 models are scaled by a power of two per row.  Probabilities are rounded to 11 bits, as in
+// count as 65504, and below 2^-14 they come in steps of 2^-24.  Queries of bf16 models are scaled by a power of two per row.  Probabilities are rounded to 11 bits, as in
 // flash_attention_tc.cu; sums, maxima and outputs are held in 32.
 // A value that is NaN enters as 0 and makes NaN of the rows that see it at the end, since 0 * NaN would reach the rows that do not.
 //
@@ -133,7 +133,7 @@ __device__ __forceinline__ uint4 to_halves(uint32_t w, __half2 s, __half2 m) {
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
-// the same for scales or minima that may lead past the halves' range, or NaN
+// the same for scales or minima that may lead past the halves' range or are too small for it, or NaN: rounded once
 __device__ __forceinline__ uint4 to_halves_wide(uint32_t w, float s, float m) {
   uint32_t r[4];
 #pragma unroll
@@ -145,16 +145,21 @@ __device__ __forceinline__ uint4 to_halves_wide(uint32_t w, float s, float m) {
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
+// A group's (scale, minimum) as halves; wide(): the top bit of either place is set where the fast conversion does not serve
 template <typename T> struct Group;
 template <> struct Group<__half> {
-  static constexpr uint32_t kAdd = 0x18001800u;   // carries into the top bit from 2048 on
+  static __device__ __forceinline__ uint32_t wide(uint32_t g) { return (g & 0x7fff7fffu) + 0x18001800u; }   // from 2048 on
   static __device__ __forceinline__ __half2 both(uint32_t g, int which) {
     const uint32_t x = __byte_perm(g, g, which ? 0x3232 : 0x1010);
     return *reinterpret_cast<const __half2*>(&x);
   }
 };
 template <> struct Group<__nv_bfloat16> {
-  static constexpr uint32_t kAdd = 0x3b003b00u;
+  // from 2048 on, and, but for zero, below 2^-17, from where on a half holds all digits of a bf16 number
+  static __device__ __forceinline__ uint32_t wide(uint32_t g) {
+    const uint32_t x = g & 0x7fff7fffu;
+    return (x + 0x3b003b00u) | ((x + 0x7fff7fffu) & ~(x + 0x49004900u));
+  }
   static __device__ __forceinline__ __half2 both(uint32_t g, int which) {
     const float2 f = kv4::scale_min<__nv_bfloat16>(g);
     return __float2half2_rn(which ? f.y : f.x);
@@ -448,7 +453,7 @@ __global__ void __launch_bounds__(READY ? kReadyThreads : kThreads, 1) kv4_promp
           kv4_wait(&ctl->raw_full[us], up);
           const uint8_t* unit = raw_ring + us * kUnitKeys * kUnitPitch + kq * kUnitPitch;
           constexpr int kPass = kConvert / 8, NI = kUnitKeys / kPass;   // rows of all threads; rows of a thread and unit
-          uint32_t w[NI][NWD], g[NI][NWD], large = 0u;
+          uint32_t w[NI][NWD], g[NI][NWD], wide = 0u;
 #pragma unroll
           for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -456,15 +461,15 @@ __global__ void __launch_bounds__(READY ? kReadyThreads : kThreads, 1) kv4_promp
               const uint32_t* row = reinterpret_cast<const uint32_t*>(unit + i * kPass * kUnitPitch);
               w[i][k] = on ? row[k * 8 + l] : 0u;
               g[i][k] = on ? row[D / 8 + (k * 8 + l) * 8 / GS] : 0u;
-              large |= (g[i][k] & 0x7fff7fffu) + Group<T>::kAdd;
+              wide |= Group<T>::wide(g[i][k]);
             }
-          if ((large & 0x80008000u) == 0u) {
+          if ((wide & 0x80008000u) == 0u) {
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
               for (int k = 0; k < NWD; ++k)
                 *reinterpret_cast<uint4*>(to + k * kHalf + i * kPass * 128) = to_halves(w[i][k], Group<T>::both(g[i][k], 0), Group<T>::both(g[i][k], 1));
-          } else {                                // past the range of halves somewhere, or NaN
+          } else {                                // outside the range of halves somewhere, or NaN
 #pragma unroll 1
             for (int x = 0; x < NI * NWD; ++x) {
               const int i = x / NWD, k = x % NWD, group = (k * 8 + l) * 8 / GS;
@@ -769,7 +774,7 @@ __global__ void __launch_bounds__(256, 6) kv4_prompt_ready_kernel(const Params p
     for (int k = 0; k < NWD; ++k) {
       const uint32_t x = g[i][k];
       uint4 v;
-      if ((((x & 0x7fff7fffu) + Group<T>::kAdd) & 0x80008000u) == 0u) {
+      if ((Group<T>::wide(x) & 0x80008000u) == 0u) {
         v = to_halves(w[i][k], Group<T>::both(x, 0), Group<T>::both(x, 1));
       } else {
         float2 f = kv4::scale_min<T>(x);

@@ -209,8 +209,8 @@ def flash_attention_int4(q, kv_buffer, qk_scale, b_start_loc, b_new_len, b_req_t
     """Portions of prompts over a 4-bit cache that already holds them: sequence ``b`` brings the ``b_new_len[b]`` rows of ``q [T, Hq, D]``
     from ``b_start_loc[b]`` on, its last tokens of ``b_seq_len[b]`` cached ones; each sees the cached tokens up to itself.
 
-    The products are of 16-bit operands: cached elements are rounded to halves (for bf16 models too, whose elements beyond 65504 count as
-    65504), and so are the probabilities; sums and the softmax are held in 32 bits.  ``max_new_len`` and ``max_actual_seq_len`` are
+    The products are of 16-bit operands: cached elements are rounded to halves, by 2^-11 of themselves or by 2^-25 (for bf16 models too, whose
+    elements beyond 65504 count as 65504), and so are the probabilities; sums and the softmax are held in 32 bits.  ``max_new_len`` and ``max_actual_seq_len`` are
     bounds that the host knows: new tokens and keys past them do not count.  A row that sees nothing is zero; rows of ``q`` that belong to no
     sequence are not written (``out``, by default a new tensor, keeps what it held there); a table entry outside the cache reads row 0.
     A row belongs to one sequence: where the ranges overlap (starts of an earlier step), it holds what one of its sequences gives, and
