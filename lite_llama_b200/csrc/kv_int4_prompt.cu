@@ -843,15 +843,16 @@ __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(const Params p) {
   for (int from = 0; from < n; from += kTogether) {
     if (from % kLook == 0) {
       const float2 ml = from == 0 ? first : look(from);
-      w = ml.y == 0.f ? 0.f : fast_exp2(ml.x - base);      // 0: of keys that the row does not see, nothing was stored
-      if (w != 0.f) L += ml.y * w;
+      // A sum of zero: of keys that the row does not see, nothing was stored.  A weight that is zero counts: the part may hold a NaN.
+      w = ml.y == 0.f ? -1.f : fast_exp2(ml.x - base);
+      if (!(w < 0.f)) L = fmaf(ml.y, w, L);
     }
 #pragma unroll
     for (int i = 0; i < kTogether; ++i)
 #pragma unroll
       for (int k = 0; k < R; ++k) {
         const float wi = __shfl_sync(0xffffffffu, w, k * kLook + from % kLook + i);
-        if (wi != 0.f) {
+        if (!(wi < 0.f)) {
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[k][e] = fmaf(x[i][k][e], wi, acc[k][e]);
         }
