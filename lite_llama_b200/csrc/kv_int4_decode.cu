@@ -1010,7 +1010,9 @@ extern "C" int b2l_flash_decoding_int4(void* out, const void* q, const void* cac
   for (p.TS_log2 = 0; 1 << p.TS_log2 < pl.TS;) ++p.TS_log2;     // a power of two
   p.most = max_seq_len < table_width ? max_seq_len : table_width;
   if (p.most < 0) p.most = 0;
-  B2L_REQUIRE((batch < kMaxBatch ? batch : kMaxBatch) * cdiv64(p.most, kUnit) * num_kv_heads < (1ll << 31), "flash_decoding_int4: too many tokens");
+  // the shares' sums, each row's kRowCost among them
+  B2L_REQUIRE((batch < kMaxBatch ? batch : kMaxBatch) * (cdiv64(p.most, kUnit) + kRowCost) * num_kv_heads < (1ll << 31),
+              "flash_decoding_int4: too many tokens");
   p.q_vec = (uintptr_t)q % 16 == 0 && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0;
   p.scale_log2 = qk_scale * 1.4426950408889634f;
   p.ws_o = (float*)workspace;
