@@ -316,7 +316,10 @@ extern "C" int b2l_kv_int4_read(void* out, const void* cache, int64_t cache_row_
   if (tokens == 0) return B2L_OK;
   const Blocks bl = blocks_of(2 * (int64_t)n_kh * (head_dim / 8), 256);
   B2L_REQUIRE(bl.parts <= 65535, "kv_int4_read: too many heads");
-  const bool four = tokens * bl.parts * bl.threads > 2ll * 2048 * b2l_num_sms();   // as above
+  // Four tokens a thread, whose loads are on their way together, from eight blocks of one token to an SM on (one and four, us; 8 kv heads of 128:
+  // 1000 tokens 2.3 and 3.0, 2000 3.7 and 4.0, 4000 5.9 and 5.3, 16000 23.8 and 16.4; 4 of 128: 1000 2.0 and 2.0, 4000 4.6 and 3.7; 2 of 64, blocks
+  // of a warp, which start one after the other: 500 1.4 and 1.6, 1500 2.0 and 1.7, 8000 8.7 and 2.6).
+  const bool four = tokens * bl.parts > 8ll * b2l_num_sms();
   const dim3 grid((unsigned)cdiv64(tokens, four ? 4 : 1), bl.parts);
   cudaStream_t st = (cudaStream_t)stream;
 #define KV4_READ(TT)                                                                                                             \
