@@ -26,9 +26,9 @@
 namespace {
 
 constexpr int kMaxConsumers = 8, kMaxStages = 8, kUnit = 16, kCluster = 8, kFirst = 3;
-// a row's start and end in tiles (150 rows of 200 - 400 tokens, 2 kv heads of 64: 13.6 us; 0 tiles 15.9, 2 tiles 15.0)
+// a row's start and end in tiles (150 rows of 200 - 400 tokens, 2 kv heads of 64: 13.5 us; 0 tiles 16.0, 2 tiles 15.0)
 constexpr int kRowCost = 1;
-// tokens of a share, at least a tile (one row of 1500 / 3900 tokens, 8 kv heads of 128: 11.2 / 12.2 us; of 64 tokens 13.5 / 14.1, 128: 15.3 / 17.4)
+// tokens of a share, at least a tile (one row of 1500 / 3900 tokens, 8 kv heads of 128: 11.5 / 12.4 us; of 64 tokens 13.3 / 14.2, 128: 15.5 / 16.9)
 constexpr int kMinLog2 = 5, kMinTokens = 1 << kMinLog2;
 
 struct Int4DecodeParams {
@@ -576,8 +576,8 @@ __global__ void __launch_bounds__(kMaxConsumers * 32, 2) kv4_decode_kernel(const
   };
 
   // ---- the ring's copies: each warp brings its part of a tile's token rows, whose table entries are read a tile ahead, one bulk copy to
-  // a row.  (16 bytes a lane instead: 32 rows of 1000 - 2000 tokens, 8 kv heads of 128: 32 us, bulk 29; one row of 201: 7.2 and 6.6; rows
-  // of 160 bytes, 150 of 200 - 400 tokens: 13.6 and 13.4.) ----
+  // a row.  (16 bytes a lane instead, measured when a code cost fewer instructions: 32 rows of 1000 - 2000 tokens, 8 kv heads of 128: 32 us, bulk
+  // 29; one row of 201: 7.2 and 6.6; rows of 160 bytes, 150 of 200 - 400 tokens: 13.6 and 13.4.) ----
   const int hb = kv4::head_bytes(D, GS), mine = nwarps == 8 ? tile >> 3 : (tile + nwarps - 1) / nwarps;   // token rows of this warp, at most 32
   struct Place { Segment s; int item, t; bool more; };   // a tile of the share
   auto start_of = [&](Place& x) {
@@ -879,8 +879,8 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) kv4_decode_merge_kernel
 }
 
 constexpr int kMaxBatch = 4096;                   // rows of one launch (their lengths lie in shared memory)
-// Tokens of a row that a cluster takes.  One row of 201 / 650 / 1000 / 1400 tokens, 8 kv heads of 128: 6.6 / 9.4 / 11.1 / 14.2 us, in shares
-// 9.6 / 11.9 / 11.0 / 11.2; 18 rows of 900: 14.9 and 18.3; 4 kv heads, 2 rows of 1000 / 1900: 8.5 / 11.8 and 11.2 / 10.2.
+// Tokens of a row that a cluster takes.  One row of 201 / 650 / 1000 / 1400 tokens, 8 kv heads of 128: 6.9 / 10.3 / 12.3 / 16.0 us, in shares
+// 9.4 / 11.7 / 11.0 / 11.4; 18 rows of 900: 16.1 and 18.4; 4 kv heads, 2 rows of 1000 / 1900: 9.2 / 13.1 and 11.8 / 10.9.
 constexpr int kClusterMost = 1024;
 
 struct Int4Plan { int HB, qblocks, TS, pitch, stages, smem, grid; bool cluster; };
@@ -947,7 +947,7 @@ int launch_int4_decode(const Int4DecodeParams& p, const Int4Plan& pl, cudaStream
   B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, pl.smem, configured[p.G <= 4]));
   b2l_launch(kern, grid, block, (size_t)pl.smem, st, p);
   B2L_LAUNCH_CHECK();
-  // many parts to a row, or few: 16 warps to a head, or one (2 rows of 30000 tokens: 18.9 and 37.8 us; 32 rows of 1000 - 2000: 38.0 and 29.5)
+  // many parts to a row, or few: 16 warps to a head, or one (2 rows of 30000 tokens: 19.4 and 38.7 us; 32 rows of 1000 - 2000: 39.0 and 30.3)
   if ((int64_t)pl.grid > 24 * (int64_t)p.batch)
     b2l_launch(kv4_decode_merge_kernel<T, D, 16>, dim3((unsigned)p.batch, (unsigned)p.Hq), dim3(512), (size_t)0, st, p);
   else

@@ -14,14 +14,14 @@
 //                 where the running maximum rises by more than 2^8 (both by one factor, hence exact)
 // Tensor memory: two buffers of 64 keys' scores for either tile, whose place the probabilities take | O0 | O1.  A softmax thread works on
 // one half of a key tile (its registers suffice for that beside eight converting warps) while the products of the other run.  A step
-// (a key tile of both row tiles) takes about 5000 cycles, bound by the conversion's and the softmax's instructions together; its four
+// (a key tile of both row tiles) takes 4500 to 4900 cycles, bound by the conversion's and the softmax's instructions together; its four
 // products would take 2050.
 //
 // READY: where five row blocks or more read a key tile on average and a CTA has ten steps or more, a kernel before this one converts
 // each tile once into the workspace, as the tensor cores read it, and one warp fetches whole operands; the softmax warps then have
 // registers for a whole row of 128 scores (S for both tiles in turn | P0 P1 | O0 | O1), which they free before the exponentials.  A
-// step takes 2800 cycles, of which 2050 are the exponentials' issue alone.  The kernel before takes 8 - 12 us for 8000 keys of 8 heads.
-// 512 tokens over 7500, 32 / 8 heads: 86 us (98 the other way).
+// step takes 2750 cycles, of which 2050 are the exponentials' issue alone.  The kernel before takes 8 - 12 us for 8000 keys of 8 heads.
+// 512 tokens over 7500, 32 / 8 heads: 85 us (98 the other way).
 // The operands are halves for both activation types: elements are rounded to 11 bits (as the 16-bit cache of an fp16 model rounds
 // them), which for bf16 models are three bits more than reading the cache into their type would leave; elements of those beyond 65504
 // count as 65504, and below 2^-14 they come in steps of 2^-24.  Queries of bf16 models are scaled by a power of two per row.  Probabilities are rounded to 11 bits, as in

@@ -17,7 +17,9 @@ def build_slot_maps(b_req_idx, b_ctx_len, b_new_len, b_req_tokens_table, total_t
     pool and its position, each request's first token, and its length with the new tokens.  The rows come from the table (fixed slots),
     or from ``rows`` (at least ``total`` entries, int32 or int64), which are then entered into the table.  ``total_tokens`` may exceed the sum of the
     lengths (a captured size): the tokens behind it get row -1, which ``update_kv_buffer_int4`` skips, and position 0, and take nothing from
-    ``rows``.  A position or request outside the table gets row -1; lengths, starts and their sums count up to 2^31 - 1.  Nothing is read by the host, so the call can be captured."""
+    ``rows``.  A position or request outside the table gets row -1; lengths, starts and their sums count up to 2^31 - 1.  Requests are
+    different rows of the table: where two tokens with ``rows`` have one request and position, it holds the row of either.  Nothing is
+    read by the host, so the call can be captured."""
     maps = _native.slot_maps(b_req_idx, b_ctx_len, b_new_len, b_req_tokens_table, total_tokens, rows)
     return _build_slot_maps(b_req_idx, b_ctx_len, b_new_len, b_req_tokens_table, total_tokens, rows) if maps is None else maps
 
