@@ -320,6 +320,27 @@ int b2l_moe_sum(void* out, const void* in, const void* addend, int64_t tokens, i
 int b2l_moe_route_topk(void* topk_weights, void* topk_ids_i64, const void* router_logits, int64_t row_stride,
                        int64_t tokens, int num_experts, int top_k, int renormalize, int dtype, void* stream);
 
+/* ---- microscaled 4-bit floating point (csrc/mxfp4*.cu; no reference counterpart) ----
+ * Format and layout: csrc/mxfp4.cuh.  codes: rows of k / 2 bytes; scales: b2l_mxfp4_scale_bytes(rows, k) bytes per matrix, in tiles
+ * of 128 rows x 128 elements.  k is a multiple of 32; rows start on 16 bytes.  Strides of codes are in bytes.
+ * b2l_mxfp4_quantize / _dequantize: `matrices` stacked matrices of `rows` rows; fp16, bf16 or fp32.
+ * b2l_skip_rmsnorm_mxfp4: sum = x + residual (sum may be residual; residual null: sum is not written), then the RMS norm of it
+ * times weight, quantised; n <= 16384.
+ * b2l_mxfp4_matmul: y[t, n] = x . w (+ bias), 16-bit; gated: silu(gate) * up quantised into y (codes, row stride in bytes)
+ * and y_scales, rows of w in runs of 64 gate and 64 up rows.  weights_ready: nothing still running writes w, so that it is requested
+ * before the previous kernel has ended. */
+int64_t b2l_mxfp4_scale_bytes(int64_t rows, int64_t k);
+int b2l_mxfp4_quantize(void* codes, void* scales, const void* x, int64_t matrices, int64_t rows, int64_t k,
+                       int64_t x_row_stride, int dtype, void* stream);
+int b2l_mxfp4_dequantize(void* y, const void* codes, const void* scales, int64_t matrices, int64_t rows, int64_t k,
+                         int64_t codes_row_stride, int dtype, void* stream);
+int b2l_skip_rmsnorm_mxfp4(void* codes, void* scales, void* sum, const void* x, const void* residual, const void* weight,
+                           int64_t rows, int64_t n, int64_t x_row_stride, int64_t r_row_stride, int64_t s_row_stride,
+                           float eps, int dtype, void* stream);
+int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w, const void* w_scales,
+                     const void* bias, int64_t t, int64_t n, int64_t k, int64_t x_row_stride, int64_t w_row_stride,
+                     int64_t y_row_stride, int gated, int weights_ready, int dtype, void* stream);
+
 /* ---- tensor-parallel exchange over NVLink peer memory (csrc/tp_comm.cu) ----
  * Replaces all_reduce_tp (lite_llama/distributed/parallel_state.py:208-213: in-place NCCL SUM of the [tokens, hidden]
  * partial after every row-parallel projection, lite_llama/models/linear.py:160-161, models/qwen3_moe.py:110) TOGETHER

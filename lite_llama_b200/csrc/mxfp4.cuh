@@ -1,0 +1,109 @@
+// Microscaled 4-bit floating point: rows of e2m1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), 32 consecutive
+// ones of which share a power of two (the OCP microscaling format MXFP4).
+//
+//   scale byte   b = max(exponent field of the block's largest magnitude - 2, 0), the scale is 2^(b - 127): the largest power of
+//                two not above that magnitude, over 4 (the largest power of two of an element).  255: the block is NaN, which is
+//                what a block with an infinity or a NaN becomes.
+//   element      the value over the scale, rounded to the nearest element (ties to the even code), at most 6 in magnitude
+//   codes        uint8 [rows, k / 2], element 2i in the low half of byte i
+//   scales       uint8 [ceil(rows / 128)][ceil(k / 128)][32][4][4], indices row % 32, row % 128 / 32, block % 4: tiles of 512 bytes
+//                for 128 rows x 128 elements.  It is the order in which the tensor cores want their scales (a tile fills 32
+//                lanes x 4 columns of tensor memory by one tcgen05.cp), so no product rearranges them.  Blocks behind k are 0;
+//                rows behind the last one hold anything.
+//
+// Scaling by a power of two is exact, so an element depends on its value alone: what is quantised from 16 bits is the same
+// bits wherever it is quantised.  Kernels that quantise what they computed in 32 bits (norm) look whether the value lies so near
+// a border that its own error could decide, and compute those blocks again in 64 bits.
+#pragma once
+#include "common.cuh"
+
+namespace mx4 {
+
+constexpr int kBlock = 32;             // elements that share a scale
+constexpr int kTileBytes = 512;        // scales of 128 rows x 128 elements
+
+static inline int64_t k_tiles(int64_t k) { return cdiv64(k, 128); }
+
+#ifdef __CUDACC__
+
+// byte offset of the scale word (4 blocks = 128 elements) `kt` of a row
+__device__ __forceinline__ int64_t scale_word(int64_t row, int kt, int64_t ktiles) {
+  return ((row >> 7) * ktiles + kt) * kTileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+}
+
+// bits of a magnitude -> scale byte (monotonic: infinities and NaN have the exponent field 255)
+__device__ __forceinline__ uint32_t scale_byte(uint32_t abs_bits) {
+  const uint32_t field = abs_bits >> 23;
+  return field == 255u ? 255u : (field > 2u ? field - 2u : 0u);
+}
+// 2^(127 - byte), exactly representable for every byte of a finite block (at most 252)
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - (byte > 253u ? 253u : byte)) << 23); }
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 0u ? 0x00400000u : (byte == 255u ? 0x7fc00000u : byte << 23));
+}
+
+// eight scaled values -> eight codes, the first in the lowest half byte
+__device__ __forceinline__ uint32_t codes8(const float (&t)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r) : "f"(t[0]), "f"(t[1]), "f"(t[2]), "f"(t[3]), "f"(t[4]), "f"(t[5]), "f"(t[6]), "f"(t[7]));
+  return r;
+}
+// eight codes -> eight elements (exact)
+__device__ __forceinline__ void elements8(uint32_t c, float (&t)[8]) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(c));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    t[2 * i] = f.x;
+    t[2 * i + 1] = f.y;
+  }
+}
+// the code of a scaled value in 64 bits
+__device__ __forceinline__ uint32_t code_of(double t) {
+  const double m = fabs(t);
+  const uint32_t c = (m > 0.25) + (m >= 0.75) + (m > 1.25) + (m >= 1.75) + (m > 2.5) + (m >= 3.5) + (m > 5.0);
+  return c | (signbit(t) ? 8u : 0u);
+}
+
+// Four neighbouring lanes hold a block, 16 a scale word.  All lanes of the warp take part; `abs_bits` is the lane's largest magnitude.
+__device__ __forceinline__ uint32_t block_max(uint32_t abs_bits) {
+  uint32_t m = abs_bits;
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+}
+__device__ __forceinline__ uint32_t word_of(uint32_t byte, int lane) {
+  uint32_t w = byte << (8 * ((lane >> 2) & 3));
+  w |= __shfl_xor_sync(0xffffffffu, w, 4);
+  return w | __shfl_xor_sync(0xffffffffu, w, 8);
+}
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// eight consecutive elements in 32 bits
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  const uint4 q = ldg_stream_128(p);
+  const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+  const uint4 q[2] = {ldg_stream_128(p), ldg_stream_128(p + 4)};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = reinterpret_cast<const float*>(q)[i];
+}
+
+#endif  // __CUDACC__
+
+}  // namespace mx4

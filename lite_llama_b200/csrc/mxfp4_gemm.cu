@@ -1,0 +1,326 @@
+// Y = X W^T with both operands in microscaled 4-bit floating point, for up to 128 tokens (and for what the pair kernel leaves).
+//
+//   Y[t, n] = sum over blocks b of 2^(sx[t, b] + sw[n, b] - 254) * sum_i ex[t, 32 b + i] * ew[n, 32 b + i]
+//
+// The products of elements are exact, scales are powers of two, sums are in 32 bits on the tensor cores; rounded once.
+//
+// Bound: with few tokens the weights (17/32 bytes an element) are what streams.  128 weight rows are the rows of the MMA (they are
+// most of the bytes), 32, 64 or 128 tokens its columns, so the tensor pipe is idle nearly always and the kernel is a ring of TMA copies: a CTA has
+// four stages of 256 k (90 - 105 KiB) in flight and two CTAs share an SM.  A tile whose n leaves SMs idle is parted along k
+// over a cluster of 2, 4 or 8 CTAs, which leave their sums in shared memory and add them up there, each a share of the tile, in
+// the order of the parts: nothing outlives the launch, so calls on several streams and captured graphs share nothing.
+#include "gemm_tc.cuh"
+#include "mxfp4_mma.cuh"
+#include "pair.cuh"
+
+namespace mx4 {
+
+constexpr int kThreads = 6 * 32;       // TMA producer, MMA issuer, four warps that read the accumulator
+
+struct Params {
+  void* y; int64_t ldy;                // [T, N] 16-bit, or the codes [T, N / 4] of silu(gate) * up
+  uint8_t* y_scales; int64_t y_ktiles;
+  const void* bias;                    // [N] in the output's type, or null
+  const uint8_t* x_scales; const uint8_t* w_scales;
+  int64_t ktiles;                      // scale tiles along k
+  int T, N, K, num_kb;
+  int early;                           // weights may be requested before the previous kernel has ended
+  int vec;                             // 8-byte stores of y
+};
+
+template <int BT> struct Ring {
+  static constexpr int kStages = BT == 128 ? 5 : 4;
+  static constexpr int kStage = 16384 + kSfBytes + BT * 128 + kSfBytes;   // W, its scales, X, its scales
+  static constexpr int kX = 16384 + kSfBytes;
+  static constexpr int kCols = BT + kStages * 16;                         // accumulator, then 16 columns of scales a stage
+  static constexpr int kAlloc = kCols <= 128 ? 128 : 256;
+  static constexpr int kSmem = 1024 + 1024 + kStages * kStage;
+};
+
+struct __align__(8) Control {
+  uint64_t full[8], empty[8], done;
+  uint32_t tmem;
+};
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+
+template <typename T, int BT, bool GATED>
+__global__ void __launch_bounds__(kThreads, BT == 128 ? 1 : 2)
+stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Params p) {
+  using R = Ring<BT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  Control* ctl = reinterpret_cast<Control*>(smem);
+  uint8_t* ring = smem + 1024;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t S = cluster_size(), rank = pair_rank();
+  const int tile = blockIdx.x / S, m0 = blockIdx.y * BT;
+  const int kb0 = (int)((int64_t)p.num_kb * rank / S), kb1 = (int)((int64_t)p.num_kb * (rank + 1) / S);
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_x);
+    tma_prefetch_desc(&tmap_w);
+    for (int s = 0; s < R::kStages; ++s) {
+      mbar_init(&ctl->full[s], 1);
+      mbar_init(&ctl->empty[s], 1);
+    }
+    mbar_init(&ctl->done, 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl->tmem, R::kAlloc);
+    tmem_relinquish();
+    pdl_launch_dependents();           // after the allocation: the next kernel's waits for this one's columns otherwise
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+
+  if (warp == 0) {
+    // ===================== TMA producer =====================
+    const uint8_t* ws = p.w_scales + (int64_t)tile * p.ktiles * kTileBytes;
+    const uint8_t* xs = p.x_scales + (int64_t)(m0 >> 7) * p.ktiles * kTileBytes;
+    auto sf_bytes = [&](int kb) { return (uint32_t)(2 * kb + 2 <= p.ktiles ? 2 : 1) * kTileBytes; };
+    auto load_w = [&](int s, int kb) {
+      uint8_t* st = ring + s * R::kStage;
+      mbar_arrive_expect_tx(&ctl->full[s], 16384 + BT * 128 + 2 * sf_bytes(kb));
+      tma_load_2d_hint(st, &tmap_w, kb * 128, tile * 128, &ctl->full[s], kEvictFirst);
+      bulk_g2s(st + 16384, ws + (int64_t)2 * kb * kTileBytes, sf_bytes(kb), &ctl->full[s]);
+    };
+    auto load_x = [&](int s, int kb) {
+      uint8_t* st = ring + s * R::kStage + R::kX;
+      tma_load_2d_hint(st, &tmap_x, kb * 128, m0, &ctl->full[s], kEvictLast);
+      bulk_g2s(st + BT * 128, xs + (int64_t)2 * kb * kTileBytes, sf_bytes(kb), &ctl->full[s]);
+    };
+    const int pre = kb1 - kb0 < R::kStages ? kb1 - kb0 : R::kStages;
+    if (!p.early) pdl_wait_prior();
+    if (elect_one())
+      for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);
+    __syncwarp();
+    pdl_wait_prior();
+    if (elect_one())
+      for (int i = 0; i < pre; ++i) load_x(i, kb0 + i);
+    __syncwarp();
+    gemm::PipeState ps(R::kStages);
+    for (int i = 0; i < pre; ++i) ps.advance();
+    for (int kb = kb0 + pre; kb < kb1; ++kb) {
+      mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
+      if (elect_one()) {
+        load_w(ps.stage, kb);
+        load_x(ps.stage, kb);
+      }
+      __syncwarp();
+      ps.advance();
+    }
+  } else if (warp == 1) {
+    // ===================== MMA issuer =====================
+    const uint64_t desc0 = umma_desc_sw128_kmajor(smem_u32(ring)), sf0 = scale_desc(smem_u32(ring));
+    gemm::PipeState ps(R::kStages);
+    for (int kb = kb0; kb < kb1; ++kb) {
+      mbar_wait(&ctl->full[ps.stage], ps.phase);
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t base = (uint64_t)(ps.stage * R::kStage) >> 4;
+        const uint64_t wd = desc0 + base, xd = wd + (R::kX >> 4);
+        const uint64_t wsf = sf0 + base + (16384 >> 4), xsf = sf0 + base + ((R::kX + BT * 128) >> 4);
+        const uint32_t sf = tmem + BT + ps.stage * 16;
+        const int steps = (p.K - kb * kStageK + 63) >> 6;      // MMAs of 64 k that hold anything
+        copy_scales<1>(sf, wsf);
+        copy_scales<1>(sf + 8, xsf);
+        if (steps > 2) {
+          copy_scales<1>(sf + 4, wsf + (kTileBytes >> 4));
+          copy_scales<1>(sf + 12, xsf + (kTileBytes >> 4));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < steps)
+            mma<1>(tmem, wd + 2 * j, xd + 2 * j, idesc(128, BT, j & 1), sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 4,
+                   (kb - kb0) | j ? 1u : 0u);
+        tc_commit(&ctl->empty[ps.stage]);
+        if (kb + 1 == kb1) tc_commit(&ctl->done);
+      }
+      __syncwarp();
+      ps.advance();
+    }
+  } else {
+    // ===================== this CTA's sums to shared memory, [token][128] =====================
+    // done covers every MMA, and with it every copy into the ring: its memory is free
+    const int quad = warp & 3;
+    float* part = reinterpret_cast<float*>(ring) + quad * 32 + lane;
+    mbar_wait(&ctl->done, 0);
+    tc_fence_after();
+#pragma unroll 1
+    for (int c = 0; c < BT; c += 32) {
+      if (m0 + c >= p.T) break;
+      uint32_t v[32];
+      tmem_ld_32x32b_x32(tmem + ((uint32_t)(quad * 32) << 16) + c, v);
+      tc_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) part[(c + j) * 128] = __uint_as_float(v[j]);
+    }
+  }
+  tc_fence_before();
+  pair_sync();                         // all sums of the cluster are in place
+  pdl_wait_prior();                    // y may still be read upstream
+  const int tokens = p.T - m0 < BT ? p.T - m0 : BT;
+  if (!GATED) {
+    // four outputs a thread, over the parts of k in their order
+    for (int i = threadIdx.x + kThreads * rank; i < tokens * 32; i += kThreads * S) {
+      const int t = i >> 5, n = tile * 128 + (i & 31) * 4;
+      const uint8_t* src = ring + (size_t)i * 16;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      for (uint32_t s = 0; s < S; ++s) {
+        const uint4 q = ld_cluster_128(cluster_addr(src, s));
+        v[0] += __uint_as_float(q.x);
+        v[1] += __uint_as_float(q.y);
+        v[2] += __uint_as_float(q.z);
+        v[3] += __uint_as_float(q.w);
+      }
+      T* out = reinterpret_cast<T*>(p.y) + (int64_t)(m0 + t) * p.ldy + n;
+      const T* bias = reinterpret_cast<const T*>(p.bias);
+      if (bias)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) v[j] += to_f32(bias[n + j]);
+      if (p.vec && n < p.N) {          // N is a multiple of four
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) out[j] = from_f32<T>(v[j]);
+      }
+    }
+  } else {
+    // eight outputs a lane, four lanes a block, two blocks a tile: 64 gate rows, then their up rows
+    const int tasks = tokens * 8;
+    for (int base = (int)(threadIdx.x & ~31u) + kThreads * (int)rank; base < tasks; base += kThreads * (int)S) {
+      const int i = base + lane, t = i >> 3, e = (i & 7) * 8;
+      const bool in = i < tasks;
+      float g[8], u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = u[j] = 0.f;
+      if (in) {
+        const uint8_t* src = ring + ((size_t)t * 128 + e) * 4;
+        for (uint32_t s = 0; s < S; ++s) {
+          const uint32_t a = cluster_addr(src, s);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 q = ld_cluster_128(a + 16 * h), r = ld_cluster_128(a + 256 + 16 * h);
+            g[4 * h] += __uint_as_float(q.x); g[4 * h + 1] += __uint_as_float(q.y);
+            g[4 * h + 2] += __uint_as_float(q.z); g[4 * h + 3] += __uint_as_float(q.w);
+            u[4 * h] += __uint_as_float(r.x); u[4 * h + 1] += __uint_as_float(r.y);
+            u[4 * h + 2] += __uint_as_float(r.z); u[4 * h + 3] += __uint_as_float(r.w);
+          }
+        }
+        if (p.bias) {
+          const T* bias = reinterpret_cast<const T*>(p.bias) + (int64_t)tile * 128 + e;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            g[j] += to_f32(bias[j]);
+            u[j] += to_f32(bias[64 + j]);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = gated(g[j], u[j]);
+      uint32_t byte;
+      const uint32_t code = quantise8(g, byte);
+      if (in) {
+        const int64_t row = m0 + t;
+        const int k = tile * 64 + e;
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.y) + row * p.ldy + k / 2) = code;
+        if ((lane & 3) == 0) {
+          uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles);
+          word[(k >> 5) & 3] = (uint8_t)byte;
+          // an odd number of tiles: the second half of the last word lies behind the end
+          if (tile * 128 + 128 >= p.N && (tile & 1) == 0) word[((k >> 5) & 3) + 2] = 0;
+        }
+      }
+    }
+  }
+  pair_sync();                         // the peers have read this CTA's sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, R::kAlloc);
+  }
+}
+
+// Parts of k: as many CTAs as keep every SM with two of them busy, each with two stages at least.
+static int parts(int64_t tiles, int num_kb) {
+  const int64_t room = 2 * b2l_num_sms();
+  int s = 1;
+  while (s < 8 && tiles * s * 2 <= room && num_kb >= 4 * s) s *= 2;
+  return s;
+}
+
+template <typename T, int BT, bool GATED>
+static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const Params& p, cudaStream_t st) {
+  auto kern = stream_kernel<T, BT, GATED>;
+  static int configured[64] = {0};
+  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, Ring<BT>::kSmem, configured));
+  const int64_t n_tiles = cdiv64(p.N, 128), m_tiles = cdiv64(p.T, BT);
+  const int s = parts(n_tiles * m_tiles, p.num_kb);
+  b2l_hang_arm(st);
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)(n_tiles * s), (unsigned)m_tiles);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Ring<BT>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)s;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = b2l_pdl_enabled() ? 2 : 1;
+  B2L_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tx, tw, p));
+  B2L_LAUNCH_CHECK();
+  return B2L_OK;
+}
+
+template <typename T>
+static int stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const Params& p, bool gated, cudaStream_t st) {
+  const int bt = p.T <= 32 ? 32 : (p.T <= 64 ? 64 : 128);
+  CUtensorMap tx, tw;
+  int rc = b2l_make_tmap_2d(&tx, x, TMA_U8, (uint64_t)p.T, (uint64_t)p.K / 2, (uint64_t)x_stride, (uint32_t)bt, 128, true);
+  if (rc != B2L_OK) return rc;
+  rc = b2l_make_tmap_2d(&tw, w, TMA_U8, (uint64_t)p.N, (uint64_t)p.K / 2, (uint64_t)w_stride, 128, 128, true);
+  if (rc != B2L_OK) return rc;
+#define STREAM(BT) (gated ? launch<T, BT, true>(tx, tw, p, st) : launch<T, BT, false>(tx, tw, p, st))
+  return bt == 32 ? STREAM(32) : (bt == 64 ? STREAM(64) : STREAM(128));
+#undef STREAM
+}
+
+}  // namespace mx4
+
+extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w, const void* w_scales,
+                                const void* bias, int64_t t, int64_t n, int64_t k, int64_t x_row_stride, int64_t w_row_stride,
+                                int64_t y_row_stride, int gated, int weights_ready, int dtype, void* stream) {
+  B2L_REQUIRE(t >= 0 && n > 0 && k > 0 && k % 32 == 0 && t < (1ll << 30) && n < (1ll << 30) && k < (1ll << 30),
+              "mxfp4_matmul: t=%lld n=%lld k=%lld (k a multiple of 32)", (long long)t, (long long)n, (long long)k);
+  if (t == 0) return B2L_OK;
+  B2L_REQUIRE(y && x && x_scales && w && w_scales && (!gated || y_scales), "mxfp4_matmul: null pointer");
+  B2L_REQUIRE(!gated || n % 128 == 0, "mxfp4_matmul: gate and up rows come in runs of 64 (n=%lld)", (long long)n);
+  B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales) % 16 == 0 && (x_row_stride | w_row_stride) % 16 == 0 &&
+                  (!gated || ((uintptr_t)y % 4 == 0 && y_row_stride % 4 == 0)),
+              "mxfp4_matmul: rows of codes must start on 16 bytes");
+  mx4::Params p;
+  p.y = y; p.ldy = y_row_stride;
+  p.y_scales = (uint8_t*)y_scales; p.y_ktiles = mx4::k_tiles(n / 2);
+  p.bias = bias;
+  p.x_scales = (const uint8_t*)x_scales; p.w_scales = (const uint8_t*)w_scales;
+  p.ktiles = mx4::k_tiles(k);
+  p.T = (int)t; p.N = (int)n; p.K = (int)k; p.num_kb = (int)cdiv64(k, mx4::kStageK);
+  p.early = weights_ready;
+  p.vec = n % 4 == 0 && y_row_stride % 4 == 0 && (uintptr_t)y % 8 == 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == B2L_F16) return mx4::stream_gemm<__half>(x, x_row_stride, w, w_row_stride, p, gated != 0, st);
+  if (dtype == B2L_BF16) return mx4::stream_gemm<__nv_bfloat16>(x, x_row_stride, w, w_row_stride, p, gated != 0, st);
+  B2L_UNSUPPORTED("mxfp4_matmul: dtype %d", dtype);
+}

@@ -1,0 +1,181 @@
+"""Microscaled 4-bit operators against their definition in 64 bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import mxfp4_oracle as O
+from lite_llama_b200 import kernels as K
+
+pytestmark = pytest.mark.gpu
+HALVES = (torch.float16, torch.bfloat16)
+
+
+def same_codes(q: K.MXFP4, want) -> None:
+    code, byte = want
+    got = O.unpack_codes(q.codes)
+    assert torch.equal(O.scale_rows(q.scales, q.rows, q.k), byte)
+    assert torch.equal(got, code)
+
+
+# ------------------------------------------------------------------------------------------------- the format
+@pytest.mark.parametrize("dtype", (*HALVES, torch.float32))
+@pytest.mark.parametrize("rows,k", ((1, 32), (1, 4096), (3, 96), (5, 160), (31, 224), (129, 256), (200, 1056), (7, 18944)))
+def test_quantised_like_the_definition(dtype, rows, k):
+    x = (torch.randn(rows, k, device="cuda") * torch.randn(rows, 1, device="cuda").exp()).to(dtype)
+    x[0, :32] = 0
+    q = K.mxfp4_quantize(x)
+    same_codes(q, O.quantise(x))
+    y = K.mxfp4_dequantize(q, torch.float32)
+    assert torch.equal(y.double(), O.rounded(x))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+def test_every_16_bit_value_in_every_place_of_a_scale(dtype):
+    """All 65536 patterns, alone in their block (infinities, NaN, subnormals), beside a block maximum that makes them small, and
+    ties between elements."""
+    bits = torch.arange(65536, device="cuda", dtype=torch.int32).to(torch.int16).view(dtype)
+    alone = torch.zeros(65536, 32, dtype=dtype, device="cuda")
+    alone[:, 5] = bits
+    same_codes(K.mxfp4_quantize(alone), O.quantise(alone))
+    for top in (1.0, 7.5, 2.0 ** -14):
+        beside = alone.clone()
+        beside[:, 30] = top
+        same_codes(K.mxfp4_quantize(beside), O.quantise(beside))
+
+
+def test_borders_of_32_bit_values():
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0], device="cuda")
+    near = torch.stack([torch.nextafter(ties, torch.zeros_like(ties)), ties, torch.nextafter(ties, ties + 9)]).flatten()
+    x = torch.zeros(64, 64, device="cuda")
+    x[:, 0], x[:, 32] = 4.0, -7.9
+    x[:, 1:28], x[:, 33:60] = near, -near
+    x *= torch.exp2(torch.arange(64, device="cuda") - 32.0)[:, None]
+    same_codes(K.mxfp4_quantize(x), O.quantise(x))
+
+
+def test_smallest_and_largest_scales():
+    x = torch.zeros(4, 64, device="cuda")
+    x[0, 0], x[0, 33] = 2.0 ** -149, 2.0 ** -127
+    x[1, 3], x[1, 40] = 2.0 ** -126, 3 * 2.0 ** -125
+    x[2, 3], x[2, 40] = torch.finfo(torch.float32).max, -(2.0 ** 127)
+    x[3, 0], x[3, 32] = float("inf"), float("nan")
+    q = K.mxfp4_quantize(x)
+    same_codes(q, O.quantise(x))
+    y = K.mxfp4_dequantize(q, torch.float32)
+    assert y[3].isnan().all() and torch.equal(y[:3].double(), O.rounded(x)[:3])
+
+
+def test_rows_of_any_stride_and_stacks():
+    wide = torch.randn(9, 400, device="cuda").half()
+    for x in (wide[:, 8:72], wide[:, 3:67], wide[:, ::2][:, :160], wide.t()[:96].t(), wide[::3, 32:64], wide[4:5, 1:33]):
+        assert x.shape[1] % 32 == 0
+        same_codes(K.mxfp4_quantize(x), O.quantise(x))
+    stack = torch.randn(3, 130, 96, device="cuda").bfloat16()
+    q = K.mxfp4_quantize(stack)
+    same_codes(q, O.quantise(stack))
+    assert torch.equal(K.mxfp4_dequantize(q, torch.float32).double(), O.rounded(stack))
+    packed = K.mxfp4_pack(q.codes, O.scale_rows(q.scales, 130, 96))
+    rows_behind = torch.zeros_like(packed.scales)
+    assert torch.equal(O.scale_rows(packed.scales, 130, 96), O.scale_rows(q.scales, 130, 96)) and rows_behind.shape == q.scales.shape
+    empty = K.mxfp4_quantize(stack[:, :0])
+    assert empty.rows == 0 and K.mxfp4_dequantize(empty).shape == (3, 0, 96)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+def test_values_come_back_rounded_once(dtype):
+    code = torch.randint(0, 16, (40, 96), device="cuda", dtype=torch.uint8)
+    byte = torch.randint(100, 140, (40, 3), device="cuda", dtype=torch.uint8)
+    byte[0], byte[1, 0] = 255, 0
+    y = K.mxfp4_dequantize(K.mxfp4_pack(O.pack_codes(code), byte), dtype)
+    want = O.values(code, byte).float().to(dtype)
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y[1:], want[1:])
+
+
+# ------------------------------------------------------------------------------------------------- the norm
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("rows,n", ((1, 32), (3, 96), (33, 896), (130, 4096), (5, 5120), (2, 16384)))
+@pytest.mark.parametrize("with_residual", (True, False))
+def test_norm_decides_as_exact_arithmetic(dtype, rows, n, with_residual):
+    x = (torch.randn(rows, n, device="cuda") * 2).to(dtype)
+    r = (torch.randn(rows, n, device="cuda") * 3).to(dtype) if with_residual else None
+    w = (1 + 0.2 * torch.randn(n, device="cuda")).to(dtype)
+    y, total = O.norm(x, r, w, 1e-5)
+    kept = None if r is None else r.clone()
+    q, out = K.skip_rmsnorm_mxfp4(x, r, w, 1e-5)
+    same_codes(q, O.quantise(y))
+    if with_residual:
+        assert out is r and torch.equal(out, (x.float() + kept.float()).to(dtype))
+        sums, again = torch.empty_like(kept), kept.clone()
+        q2, out2 = K.skip_rmsnorm_mxfp4(x, again, w, 1e-5, out_residual=sums)
+        assert out2 is sums and torch.equal(sums, out) and torch.equal(again, kept)
+        assert torch.equal(q2.codes, q.codes)
+    else:
+        assert out is x
+
+
+def test_norm_of_rows_that_lie_on_borders():
+    """All elements alike, so that the norm is just below 1 (a power of two) and the weight puts it on ties; rows of zeros; tiny rows."""
+    n = 256
+    x = torch.ones(6, n, device="cuda")
+    x[1] *= 2.0 ** -8
+    x[2] *= 1000
+    x[3] = 0
+    x[4] *= 1e-7
+    x[5, ::2] *= -1
+    x = x.half()
+    for weights in (1.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0):
+        w = torch.full((n,), weights, device="cuda").half()
+        w[::32] = 4.0
+        q, _ = K.skip_rmsnorm_mxfp4(x, None, w, 1e-6)
+        same_codes(q, O.quantise(O.norm(x, None, w, float(torch.tensor(1e-6, dtype=torch.float32)))[0]))
+
+
+def test_norm_keeps_other_rows_from_a_bad_one():
+    x = torch.randn(4, 128, device="cuda").bfloat16()
+    good, _ = K.skip_rmsnorm_mxfp4(x, None, torch.ones(128, device="cuda").bfloat16())
+    x[2, 7] = float("inf")
+    q, _ = K.skip_rmsnorm_mxfp4(x, None, torch.ones(128, device="cuda").bfloat16())
+    y, z = K.mxfp4_dequantize(q, torch.float32), K.mxfp4_dequantize(good, torch.float32)
+    assert y[2, :32].isnan().all() and torch.equal(y[[0, 1, 3]], z[[0, 1, 3]])
+
+
+# ------------------------------------------------------------------------------------------------- products
+def weights(n, k, spread=0.02):
+    w = torch.randn(n, k, device="cuda") * spread
+    q = K.mxfp4_quantize_weight(w)
+    return q, O.values(O.unpack_codes(q.codes), O.scale_rows(q.scales, n, k))
+
+
+@pytest.mark.parametrize("t,n,k", ((1, 128, 64), (1, 128, 256), (3, 5, 32), (32, 256, 512), (33, 130, 96), (17, 384, 1120), (64, 200, 2048),
+                                   (65, 640, 992), (128, 129, 4096), (100, 1000, 352)))
+def test_products_of_whole_numbers_are_exact(t, n, k):
+    """Elements and scales whose products add up to whole numbers below 2^11: any order of exact sums gives the same bits, and one
+    element, scale, row or block in a wrong place gives others."""
+    gen = torch.Generator(device="cuda").manual_seed(t * 7 + n)
+    few = lambda rows: torch.where(torch.rand(rows, k, device="cuda", generator=gen) < 16 / k,  # noqa: E731
+                                   torch.randint(0, 16, (rows, k), device="cuda", generator=gen), 0).to(torch.uint8)
+    xc, wc = few(t), few(n)
+    xb, wb = (torch.randint(128, 130, (rows, k // 32), device="cuda", generator=gen, dtype=torch.uint8) for rows in (t, n))
+    x, w = K.mxfp4_pack(O.pack_codes(xc), xb), K.mxfp4_pack(O.pack_codes(wc), wb)
+    want = O.values(xc, xb) @ O.values(wc, wb).t()
+    assert want.abs().max() > 0
+    for dtype in HALVES:
+        assert torch.equal(K.mxfp4_matmul(x, w, out_dtype=dtype), want.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,n,k", ((1, 6144, 4096), (2, 896, 4864), (7, 4096, 14336), (31, 77, 3584), (40, 4608, 3584), (128, 1152, 896),
+                                   (5, 33, 32)))
+@pytest.mark.parametrize("with_bias", (False, True))
+def test_products_against_64_bits(dtype, t, n, k, with_bias):
+    x = torch.randn(t, k, device="cuda").to(dtype)
+    w, wv = weights(n, k)
+    b = torch.randn(n, device="cuda").to(dtype) if with_bias else None
+    y = K.mxfp4_matmul(x, w, bias=b)
+    xv = O.rounded(x)
+    want = xv @ wv.t()
+    bound = O.product_bound(xv, wv, want + (0 if b is None else b.double()), dtype)
+    want = want if b is None else want + b.double()
+    assert y.dtype == dtype and ((y.double() - want).abs() <= bound).all()
