@@ -341,6 +341,22 @@ int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scale
                      const void* bias, int64_t t, int64_t n, int64_t k, int64_t x_row_stride, int64_t w_row_stride,
                      int64_t y_row_stride, int gated, int weights_ready, int dtype, void* stream);
 
+/* Routed experts: every slot (token, choice) gets row place[slot] (int32; -1: its id names no expert), the rows of an expert fill tiles of
+ * tile_rows (32, 64 or 128), row r of tile i is row i * tile_rows + r; scales of a tile start on a tile of 128 rows.
+ * table int32 [1 + 2 * max_tiles] = {tiles, {expert, rows} per tile}.
+ * _scatter: x quantised into the rows of its slots.  _grouped_matmul: w [experts, n, k], buffers of max_tiles * tile_rows rows
+ * (scales: 128 max_tiles); gated as in b2l_mxfp4_matmul.  _combine: out[t] = sum_j weights[t, j] * y[place[t, j]]. */
+int64_t b2l_mxfp4_moe_max_tiles(int64_t slots, int tile_rows, int experts);
+int b2l_mxfp4_moe_sort(void* place, void* table, const void* topk_ids, int id_width, int64_t slots, int tile_rows, int experts,
+                       void* stream);
+int b2l_mxfp4_moe_scatter(void* codes, void* scales, const void* x, const void* place, int64_t tokens, int top_k,
+                          int tile_rows, int64_t k, int64_t x_row_stride, int dtype, void* stream);
+int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w,
+                             const void* w_scales, const void* table, int64_t max_tiles, int tile_rows, int experts,
+                             int64_t n, int64_t k, int gated, int dtype, void* stream);
+int b2l_mxfp4_moe_combine(void* out, const void* y, const void* place, const void* weights, int weights_f32, int64_t tokens,
+                          int top_k, int64_t n, int dtype, void* stream);
+
 /* ---- tensor-parallel exchange over NVLink peer memory (csrc/tp_comm.cu) ----
  * Replaces all_reduce_tp (lite_llama/distributed/parallel_state.py:208-213: in-place NCCL SUM of the [tokens, hidden]
  * partial after every row-parallel projection, lite_llama/models/linear.py:160-161, models/qwen3_moe.py:110) TOGETHER

@@ -140,8 +140,7 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
           if (j < steps)
             mma<1>(tmem, wd + 2 * j, xd + 2 * j, idesc(128, BT, j & 1), sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 4,
                    (kb - kb0) | j ? 1u : 0u);
-        tc_commit(&ctl->empty[ps.stage]);
-        if (kb + 1 == kb1) tc_commit(&ctl->done);
+        tc_commit(kb + 1 == kb1 ? &ctl->done : &ctl->empty[ps.stage]);
       }
       __syncwarp();
       ps.advance();
@@ -297,6 +296,239 @@ static int stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w
 #undef STREAM
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// The same product for routed experts: tiles of up to BT rows of one expert, {expert, rows} in a table on the device
+// (mxfp4_moe.cu), row r of tile i in row i BT + r of x and y and in row 128 i + r of their scales.
+//
+// Bound: the experts' weights, each read from memory once (further tiles of an expert find them in L2).  Persistent, one CTA to
+// an SM with 180 KiB of copies in flight, the accumulator in two buffers: a tile's end overlaps the next one's products.
+// ---------------------------------------------------------------------------------------------------------------
+template <int BT> struct GroupedRing {
+  static constexpr int kStage = 16384 + kSfBytes + BT * 128 + kSfBytes;
+  static constexpr int kX = 16384 + kSfBytes;
+  static constexpr int kStages = BT == 32 ? 8 : (BT == 64 ? 7 : 5);
+  static constexpr int kCols = 2 * BT + kStages * 16;
+  static constexpr int kAlloc = kCols <= 256 ? 256 : 512;
+  static constexpr int kOut = 32 * 128 * 4;
+  static constexpr int kSmem = 1024 + 1024 + kStages * kStage + kOut;
+};
+
+struct GroupedParams {
+  void* y; int64_t ldy;                // rows of 16-bit outputs (elements) or of codes (bytes)
+  uint8_t* y_scales; int64_t y_ktiles;
+  const uint8_t* x_scales; const uint8_t* w_scales;
+  const int32_t* table;                // tiles, then {expert, rows} of each
+  int64_t ktiles;
+  int N, K, num_kb, n_tiles;
+  int vec;
+};
+
+struct __align__(8) GroupedControl {
+  uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+};
+
+template <typename T, int BT, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1)
+grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const GroupedParams p) {
+  using R = GroupedRing<BT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  GroupedControl* ctl = reinterpret_cast<GroupedControl*>(smem);
+  uint8_t* ring = smem + 1024;
+  float* out_stage = reinterpret_cast<float*>(ring + R::kStages * R::kStage);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_x);
+    tma_prefetch_desc(&tmap_w);
+    for (int s = 0; s < R::kStages; ++s) {
+      mbar_init(&ctl->full[s], 1);
+      mbar_init(&ctl->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&ctl->acc_full[b], 1);
+      mbar_init(&ctl->acc_empty[b], 4);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl->tmem, R::kAlloc);
+    tmem_relinquish();
+    pdl_launch_dependents();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+  pdl_wait_prior();                    // the table and the rows are upstream data
+  const int items = ld_upstream(p.table) * p.n_tiles;
+
+  if (warp == 0) {
+    // ===================== TMA producer =====================
+    gemm::PipeState ps(R::kStages);
+    for (int it = blockIdx.x; it < items; it += gridDim.x) {
+      const int tile = it / p.n_tiles, nt = it - tile * p.n_tiles;
+      const int expert = ld_upstream(p.table + 1 + 2 * tile);
+      const int64_t w_tile = (int64_t)expert * p.n_tiles + nt;
+      const uint8_t* ws = p.w_scales + w_tile * p.ktiles * kTileBytes;
+      const uint8_t* xs = p.x_scales + (int64_t)tile * p.ktiles * kTileBytes;
+      const int w_row = expert * p.N + nt * 128;
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
+        if (elect_one()) {
+          uint8_t* st = ring + ps.stage * R::kStage;
+          const uint32_t sf = (uint32_t)(2 * kb + 2 <= p.ktiles ? 2 : 1) * kTileBytes;
+          uint64_t* full = &ctl->full[ps.stage];
+          mbar_arrive_expect_tx(full, 16384 + BT * 128 + 2 * sf);
+          tma_load_2d_hint(st, &tmap_w, kb * 128, w_row, full, kEvictNormal);
+          bulk_g2s(st + 16384, ws + (int64_t)2 * kb * kTileBytes, sf, full);
+          tma_load_2d_hint(st + R::kX, &tmap_x, kb * 128, tile * BT, full, kEvictLast);
+          bulk_g2s(st + R::kX + BT * 128, xs + (int64_t)2 * kb * kTileBytes, sf, full);
+        }
+        __syncwarp();
+        ps.advance();
+      }
+    }
+  } else if (warp == 1) {
+    // ===================== MMA issuer =====================
+    const uint64_t desc0 = umma_desc_sw128_kmajor(smem_u32(ring)), sf0 = scale_desc(smem_u32(ring));
+    gemm::PipeState ps(R::kStages);
+    int turn = 0;
+    for (int it = blockIdx.x; it < items; it += gridDim.x, ++turn) {
+      const int buf = turn & 1;
+      mbar_wait(&ctl->acc_empty[buf], ((turn >> 1) & 1) ^ 1);
+      tc_fence_after();
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        mbar_wait(&ctl->full[ps.stage], ps.phase);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t base = (uint64_t)(ps.stage * R::kStage) >> 4;
+          const uint64_t wd = desc0 + base, xd = wd + (R::kX >> 4);
+          const uint64_t wsf = sf0 + base + (16384 >> 4), xsf = sf0 + base + ((R::kX + BT * 128) >> 4);
+          const uint32_t sf = tmem + 2 * BT + ps.stage * 16;
+          const int steps = (p.K - kb * kStageK + 63) >> 6;
+          copy_scales<1>(sf, wsf);
+          copy_scales<1>(sf + 8, xsf);
+          if (steps > 2) {
+            copy_scales<1>(sf + 4, wsf + (kTileBytes >> 4));
+            copy_scales<1>(sf + 12, xsf + (kTileBytes >> 4));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < steps)
+              mma<1>(tmem + buf * BT, wd + 2 * j, xd + 2 * j, idesc(128, BT, j & 1), sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 4,
+                     kb | j ? 1u : 0u);
+          // nobody waits for the last stage of all, and no arrival may be on its way when the CTA leaves
+          if (kb + 1 < p.num_kb || it + (int)gridDim.x < items) tc_commit(&ctl->empty[ps.stage]);
+          if (kb + 1 == p.num_kb) tc_commit(&ctl->acc_full[buf]);
+        }
+        __syncwarp();
+        ps.advance();
+      }
+    }
+  } else {
+    // ===================== four warps: 32 rows at a time through shared memory, [row][128] =====================
+    const int quad = warp & 3, tid = quad * 32 + lane;
+    float* mine = out_stage + quad * 32 + lane;
+    int turn = 0;
+    for (int it = blockIdx.x; it < items; it += gridDim.x, ++turn) {
+      const int tile = it / p.n_tiles, nt = it - tile * p.n_tiles, buf = turn & 1;
+      const int rows = ld_upstream(p.table + 2 + 2 * tile);
+      mbar_wait(&ctl->acc_full[buf], (turn >> 1) & 1);
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < BT; c += 32) {
+        if (c < rows) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(tmem + ((uint32_t)(quad * 32) << 16) + buf * BT + c, v);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mine[j * 128] = __uint_as_float(v[j]);
+        }
+        if (c + 32 == BT) {            // every row is on its way out: the accumulator is free
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->acc_empty[buf]);
+        }
+        if (c >= rows) continue;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const int here = rows - c < 32 ? rows - c : 32;
+        if (!GATED) {
+          for (int i = tid; i < here * 32; i += 128) {
+            const int r = i >> 5, n = nt * 128 + (i & 31) * 4;
+            const float4 v = *reinterpret_cast<const float4*>(out_stage + i * 4);
+            T* out = reinterpret_cast<T*>(p.y) + ((int64_t)tile * BT + c + r) * p.ldy + n;
+            if (p.vec && n < p.N) {
+              *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+            } else {
+              if (n < p.N) out[0] = from_f32<T>(v.x);
+              if (n + 1 < p.N) out[1] = from_f32<T>(v.y);
+              if (n + 2 < p.N) out[2] = from_f32<T>(v.z);
+              if (n + 3 < p.N) out[3] = from_f32<T>(v.w);
+            }
+          }
+        } else {
+          for (int base = quad * 32; base < here * 8; base += 128) {
+            const int i = base + lane, r = i >> 3, e = (i & 7) * 8;
+            const bool in = i < here * 8;
+            float g[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] = 0.f;
+            if (in) {
+              const float* src = out_stage + r * 128 + e;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) g[j] = gated(src[j], src[64 + j]);
+            }
+            uint32_t byte;
+            const uint32_t code = quantise8(g, byte);
+            if (in) {
+              const int k = nt * 64 + e;
+              *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.y) + ((int64_t)tile * BT + c + r) * p.ldy + k / 2) = code;
+              if ((lane & 3) == 0) {
+                uint8_t* word = p.y_scales + scale_word((int64_t)tile * 128 + c + r, k >> 7, p.y_ktiles);
+                word[(k >> 5) & 3] = (uint8_t)byte;
+                if (nt + 1 == p.n_tiles && (nt & 1) == 0) word[((k >> 5) & 3) + 2] = 0;
+              }
+            }
+          }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, R::kAlloc);
+  }
+}
+
+template <typename T, int BT, bool GATED>
+static int launch_grouped(const CUtensorMap& tx, const CUtensorMap& tw, const GroupedParams& p, int64_t max_tiles, cudaStream_t st) {
+  auto kern = grouped_kernel<T, BT, GATED>;
+  static int configured[64] = {0};
+  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, GroupedRing<BT>::kSmem, configured));
+  const int64_t items = max_tiles * p.n_tiles;
+  const int grid = (int)(items < b2l_num_sms() ? items : b2l_num_sms());
+  b2l_launch(kern, dim3((unsigned)grid), dim3(kThreads), (size_t)GroupedRing<BT>::kSmem, st, tx, tw, p);
+  B2L_LAUNCH_CHECK();
+  return B2L_OK;
+}
+
+template <typename T>
+static int grouped_gemm(const void* x, const void* w, const GroupedParams& p, int64_t max_tiles, int tile_rows, int experts, bool is_gated,
+                        cudaStream_t st) {
+  CUtensorMap tx, tw;
+  int rc = b2l_make_tmap_2d(&tx, x, TMA_U8, (uint64_t)(max_tiles * tile_rows), (uint64_t)p.K / 2, (uint64_t)p.K / 2, (uint32_t)tile_rows, 128, true);
+  if (rc != B2L_OK) return rc;
+  rc = b2l_make_tmap_2d(&tw, w, TMA_U8, (uint64_t)experts * p.N, (uint64_t)p.K / 2, (uint64_t)p.K / 2, 128, 128, true);
+  if (rc != B2L_OK) return rc;
+#define GROUPED(BT) (is_gated ? launch_grouped<T, BT, true>(tx, tw, p, max_tiles, st) : launch_grouped<T, BT, false>(tx, tw, p, max_tiles, st))
+  return tile_rows == 32 ? GROUPED(32) : (tile_rows == 64 ? GROUPED(64) : GROUPED(128));
+#undef GROUPED
+}
+
 }  // namespace mx4
 
 extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w, const void* w_scales,
@@ -323,4 +555,30 @@ extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const vo
   if (dtype == B2L_F16) return mx4::stream_gemm<__half>(x, x_row_stride, w, w_row_stride, p, gated != 0, st);
   if (dtype == B2L_BF16) return mx4::stream_gemm<__nv_bfloat16>(x, x_row_stride, w, w_row_stride, p, gated != 0, st);
   B2L_UNSUPPORTED("mxfp4_matmul: dtype %d", dtype);
+}
+
+extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w,
+                                        const void* w_scales, const void* table, int64_t max_tiles, int tile_rows, int experts,
+                                        int64_t n, int64_t k, int gated, int dtype, void* stream) {
+  B2L_REQUIRE(max_tiles >= 0 && experts > 0 && n > 0 && k > 0 && k % 32 == 0 && k < (1ll << 30) && n * experts < (1ll << 31) &&
+                  max_tiles * cdiv64(n, 128) < (1ll << 31) && max_tiles * 128 < (1ll << 31),
+              "mxfp4_grouped_matmul: experts=%d n=%lld k=%lld (a multiple of 32) tiles=%lld", experts, (long long)n, (long long)k, (long long)max_tiles);
+  B2L_REQUIRE(tile_rows == 32 || tile_rows == 64 || tile_rows == 128, "mxfp4_grouped_matmul: tiles of %d rows", tile_rows);
+  if (max_tiles == 0) return B2L_OK;
+  B2L_REQUIRE(y && x && x_scales && w && w_scales && table && (!gated || y_scales), "mxfp4_grouped_matmul: null pointer");
+  B2L_REQUIRE(!gated || n % 128 == 0, "mxfp4_grouped_matmul: gate and up rows come in runs of 64 (n=%lld)", (long long)n);
+  B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales) % 16 == 0 && (uintptr_t)y % 8 == 0,
+              "mxfp4_grouped_matmul: rows of codes must start on 16 bytes");
+  mx4::GroupedParams p;
+  p.y = y; p.ldy = gated ? n / 4 : n;
+  p.y_scales = (uint8_t*)y_scales; p.y_ktiles = mx4::k_tiles(n / 2);
+  p.x_scales = (const uint8_t*)x_scales; p.w_scales = (const uint8_t*)w_scales;
+  p.table = (const int32_t*)table;
+  p.ktiles = mx4::k_tiles(k);
+  p.N = (int)n; p.K = (int)k; p.num_kb = (int)cdiv64(k, mx4::kStageK); p.n_tiles = (int)cdiv64(n, 128);
+  p.vec = n % 4 == 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == B2L_F16) return mx4::grouped_gemm<__half>(x, w, p, max_tiles, tile_rows, experts, gated != 0, st);
+  if (dtype == B2L_BF16) return mx4::grouped_gemm<__nv_bfloat16>(x, w, p, max_tiles, tile_rows, experts, gated != 0, st);
+  B2L_UNSUPPORTED("mxfp4_grouped_matmul: dtype %d", dtype);
 }

@@ -1,0 +1,203 @@
+// Routed experts in microscaled 4-bit floating point: tokens sorted by expert and back (the products: mxfp4_gemm.cu).
+//
+//   out[t] = sum_j weight[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])),  e = ids[t, j]
+//
+// A slot (t, j) gets a row among its expert's; every expert's rows fill tiles of `tile` rows, and row r of tile i is row i tile + r of
+// all buffers (row 128 i + r of their scales, so that a tile's scales start on a tile of their own).  Ids that name no expert get no
+// row and add nothing.  A row's results do not depend on its place, so places are given out by atomics.
+#include "mxfp4.cuh"
+
+namespace mx4 {
+
+constexpr int kSortThreads = 1024;
+
+// One CTA: ranks by counters in shared memory, tiles by a scan over experts.
+__global__ void __launch_bounds__(kSortThreads)
+sort_kernel(int32_t* __restrict__ place, int32_t* __restrict__ table, const void* __restrict__ ids, int id_width, int slots, int tile,
+            int experts) {
+  extern __shared__ int counts[];      // per expert, then the first tile of each
+  int* first = counts + experts;
+  __shared__ int warp_sum[32], carry;
+  pdl_prologue();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int e = tid; e < experts; e += kSortThreads) counts[e] = 0;
+  if (tid == 0) carry = 0;
+  __syncthreads();
+  for (int s = tid; s < slots; s += kSortThreads) {
+    const int64_t e = load_index(ids, s, id_width);
+    place[s] = e >= 0 && e < experts ? atomicAdd(&counts[e], 1) : -1;
+  }
+  __syncthreads();
+  for (int base = 0; base < experts; base += kSortThreads) {
+    const int e = base + tid;
+    const int tiles = e < experts ? (counts[e] + tile - 1) / tile : 0;
+    int sum = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (lane == 31) warp_sum[warp] = sum;
+    __syncthreads();
+    if (warp == 0) {
+      int w = warp_sum[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += up;
+      }
+      warp_sum[lane] = w;
+    }
+    __syncthreads();
+    const int before = carry + (warp ? warp_sum[warp - 1] : 0) + sum - tiles;
+    if (e < experts) first[e] = before;
+    __syncthreads();
+    if (tid == 0) carry += warp_sum[31];
+    __syncthreads();
+  }
+  if (tid == 0) table[0] = carry;
+  for (int e = tid; e < experts; e += kSortThreads) {
+    const int n = counts[e];
+    for (int i = 0; i * tile < n; ++i) {
+      table[1 + 2 * (first[e] + i)] = e;
+      table[2 + 2 * (first[e] + i)] = n - i * tile < tile ? n - i * tile : tile;
+    }
+  }
+  for (int s = tid; s < slots; s += kSortThreads) {
+    const int64_t e = load_index(ids, s, id_width);
+    if (e >= 0 && e < experts) place[s] += first[e] * tile;
+  }
+}
+
+// A token's row quantised once and written to the rows of all its slots (quantize_kernel in mxfp4_quant.cu).
+template <typename T>
+__global__ void __launch_bounds__(256)
+scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, const int32_t* __restrict__ place,
+               int64_t tokens, int top_k, int tile, int64_t k, int64_t x_stride, int64_t ktiles, int units) {
+  pdl_prologue();
+  const int lane = threadIdx.x & 31;
+  const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t row = u / units;
+  if (row >= tokens) return;
+  const int64_t c = (u - row * units) * 32 + lane;
+  const bool in = c * 8 < k;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (in) load8(x + row * x_stride + c * 8, v);
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+  const uint32_t byte = scale_byte(block_max(m));
+  const float inv = inverse_scale(byte);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] *= inv;
+  const uint32_t word = word_of(in ? byte : 0u, lane);
+  const uint32_t code = byte == 255u ? 0u : codes8(v);
+  for (int j = 0; j < top_k; ++j) {
+    const int to = ld_upstream(place + row * top_k + j);
+    if (to < 0 || !in) continue;
+    *reinterpret_cast<uint32_t*>(codes + to * (k / 2) + c * 4) = code;
+    if ((lane & 15) == 0)
+      *reinterpret_cast<uint32_t*>(scales + scale_word((int64_t)(to / tile) * 128 + to % tile, (int)(c >> 4), ktiles)) = word;
+  }
+}
+
+// A token's expert rows, weighted, added up in the order of its choices in 32 bits; eight outputs a thread.
+template <typename T, typename W>
+__global__ void __launch_bounds__(256)
+combine_kernel(T* __restrict__ out, const T* __restrict__ y, const int32_t* __restrict__ place, const W* __restrict__ weights,
+               int64_t tokens, int top_k, int64_t n) {
+  pdl_prologue();
+  const int64_t chunks = n / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= tokens * chunks) return;
+  const int64_t t = i / chunks, c = i - t * chunks;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 < top_k; j0 += 4) {              // four rows requested together
+    uint4 q[4];
+    float w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int from = j0 + j < top_k ? ld_upstream(place + t * top_k + j0 + j) : -1;
+      q[j] = make_uint4(0u, 0u, 0u, 0u);
+      w[j] = 0.f;
+      if (from >= 0) {
+        q[j] = ldg_stream_128(y + (int64_t)from * n + c * 8);
+        w[j] = to_f32(weights[t * top_k + j0 + j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const T* e = reinterpret_cast<const T*>(&q[j]);
+#pragma unroll
+      for (int h = 0; h < 8; ++h) sum[h] = fmaf(w[j], to_f32(e[h]), sum[h]);
+    }
+  }
+  stg_128(out + t * n + c * 8, make_uint4(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]), pack2<T>(sum[6], sum[7])));
+}
+
+template <typename T>
+static int combine(void* out, const void* y, const void* place, const void* weights, int wide, int64_t tokens, int top_k, int64_t n,
+                   cudaStream_t st) {
+  const dim3 grid((unsigned)cdiv64(tokens * (n / 8), 256));
+  if (wide)
+    b2l_launch(combine_kernel<T, float>, grid, dim3(256), (size_t)0, st, (T*)out, (const T*)y, (const int32_t*)place, (const float*)weights,
+               tokens, top_k, n);
+  else
+    b2l_launch(combine_kernel<T, T>, grid, dim3(256), (size_t)0, st, (T*)out, (const T*)y, (const int32_t*)place, (const T*)weights, tokens,
+               top_k, n);
+  B2L_LAUNCH_CHECK();
+  return B2L_OK;
+}
+
+}  // namespace mx4
+
+extern "C" int64_t b2l_mxfp4_moe_max_tiles(int64_t slots, int tile_rows, int experts) {
+  if (slots <= 0 || tile_rows <= 0 || experts <= 0) return 0;
+  return slots / tile_rows + (slots < experts ? slots : experts);
+}
+
+extern "C" int b2l_mxfp4_moe_sort(void* place, void* table, const void* topk_ids, int id_width, int64_t slots, int tile_rows, int experts,
+                                  void* stream) {
+  B2L_REQUIRE(id_width == 4 || id_width == 8, "mxfp4_moe_sort: topk_ids must be int32 or int64");
+  B2L_REQUIRE(tile_rows > 0 && experts > 0 && experts <= 4096 && slots >= 0 && slots < (1ll << 24),
+              "mxfp4_moe_sort: bad sizes (slots=%lld tile=%d experts=%d)", (long long)slots, tile_rows, experts);
+  B2L_REQUIRE(table && (slots == 0 || (place && topk_ids)), "mxfp4_moe_sort: null pointer");
+  b2l_launch(mx4::sort_kernel, dim3(1), dim3(mx4::kSortThreads), (size_t)experts * 8, (cudaStream_t)stream, (int32_t*)place, (int32_t*)table,
+             topk_ids, id_width, (int)slots, tile_rows, experts);
+  B2L_LAUNCH_CHECK();
+  return B2L_OK;
+}
+
+extern "C" int b2l_mxfp4_moe_scatter(void* codes, void* scales, const void* x, const void* place, int64_t tokens, int top_k, int tile_rows,
+                                     int64_t k, int64_t x_row_stride, int dtype, void* stream) {
+  B2L_REQUIRE(tokens >= 0 && top_k > 0 && tile_rows > 0 && tile_rows <= 128 && k > 0 && k % 32 == 0 && k < (1ll << 30),
+              "mxfp4_moe_scatter: tokens=%lld top_k=%d k=%lld (a multiple of 32)", (long long)tokens, top_k, (long long)k);
+  if (tokens == 0) return B2L_OK;
+  B2L_REQUIRE(codes && scales && x && place, "mxfp4_moe_scatter: null pointer");
+  B2L_REQUIRE((uintptr_t)x % 16 == 0 && x_row_stride % 8 == 0 && (uintptr_t)codes % 4 == 0 && (uintptr_t)scales % 4 == 0,
+              "mxfp4_moe_scatter: rows must start on 16 bytes");
+  const int units = (int)cdiv64(k, 256);
+  const int64_t grid = cdiv64(tokens * units, 8);
+  B2L_REQUIRE(grid < (1ll << 31), "mxfp4_moe_scatter: too many tokens");
+#define SCATTER(T)                                                                                                                  \
+  b2l_launch(mx4::scatter_kernel<T>, dim3((unsigned)grid), dim3(256), (size_t)0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, \
+             (const T*)x, (const int32_t*)place, tokens, top_k, tile_rows, k, x_row_stride, mx4::k_tiles(k), units)
+  if (dtype == B2L_F16) SCATTER(__half);
+  else if (dtype == B2L_BF16) SCATTER(__nv_bfloat16);
+  else B2L_UNSUPPORTED("mxfp4_moe_scatter: dtype %d", dtype);
+#undef SCATTER
+  B2L_LAUNCH_CHECK();
+  return B2L_OK;
+}
+
+extern "C" int b2l_mxfp4_moe_combine(void* out, const void* y, const void* place, const void* weights, int weights_f32, int64_t tokens,
+                                     int top_k, int64_t n, int dtype, void* stream) {
+  B2L_REQUIRE(tokens >= 0 && top_k > 0 && n > 0 && n % 8 == 0 && tokens * (n / 8) < (1ll << 38), "mxfp4_moe_combine: tokens=%lld n=%lld (a multiple of 8)",
+              (long long)tokens, (long long)n);
+  if (tokens == 0) return B2L_OK;
+  B2L_REQUIRE(out && y && place && weights && ((uintptr_t)out | (uintptr_t)y) % 16 == 0, "mxfp4_moe_combine: null or misaligned pointer");
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == B2L_F16) return mx4::combine<__half>(out, y, place, weights, weights_f32, tokens, top_k, n, st);
+  if (dtype == B2L_BF16) return mx4::combine<__nv_bfloat16>(out, y, place, weights, weights_f32, tokens, top_k, n, st);
+  B2L_UNSUPPORTED("mxfp4_moe_combine: dtype %d", dtype);
+}

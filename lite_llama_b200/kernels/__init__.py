@@ -28,7 +28,7 @@ from .skip_rmsnorm import can_fuse_int8_quant, skip_rmsnorm, skip_rmsnorm_quant_
 from .swiglu import swiglu_forward
 from .update_kv_buffer import update_kv_buffer, update_kv_buffer_split
 from .update_kv_index import update_kv_index
-from .quantization import MXFP4, PackedW4, mxfp4_dequantize, mxfp4_gate_up, mxfp4_matmul, mxfp4_pack, mxfp4_quantize, mxfp4_quantize_weight, skip_rmsnorm_mxfp4
+from .quantization import MXFP4, PackedW4, fused_moe_mxfp4, mxfp4_dequantize, mxfp4_gate_up, mxfp4_matmul, mxfp4_pack, mxfp4_quantize, mxfp4_quantize_weight, skip_rmsnorm_mxfp4
 from .quantization import quantize_activations_int8, smoothquant_matmul, smoothquant_matmul_prequant, w4a16_matmul, w4a16_matmul_packed, w4a16_pack, w8a16_matmul
 
 __all__ = [
@@ -113,4 +113,5 @@ __all__ = [
     "mxfp4_gate_up",
     "mxfp4_matmul",
     "skip_rmsnorm_mxfp4",
+    "fused_moe_mxfp4",
 ]

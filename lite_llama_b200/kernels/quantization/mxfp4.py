@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .._common import as_rows, check, current_device, dtype_code, float_code, lib, no_grad, ptr, require_cuda, stream_handle, weights_written
+from .._common import as_rows, check, current_device, dtype_code, float_code, index_width, lib, no_grad, ptr, require_cuda, stream_handle, weights_written
 
 BLOCK = 32          # elements that share a scale
 GATE_RUN = 64       # gate rows, then as many up rows
@@ -244,3 +244,68 @@ def mxfp4_matmul(x: torch.Tensor | MXFP4, w: MXFP4, bias: torch.Tensor | None = 
     if swiglu:
         return MXFP4(y, ys, ready=False)
     return y if lead is None or len(lead) == 1 else y.view(*lead, n)
+
+
+def _tile_rows(slots: int, experts: int) -> int:
+    """Rows of an expert's tile: the MMA's columns.  More than an expert's rows are copies of nothing, fewer read its weights again."""
+    per = slots / experts
+    return 32 if per <= 24 else (64 if per <= 48 else 128)
+
+
+@no_grad
+def fused_moe_mxfp4(hidden_states: torch.Tensor, w1: MXFP4, w2: MXFP4, topk_weights: torch.Tensor, topk_ids: torch.Tensor) -> torch.Tensor:
+    """``sum_k w_k * (silu(x @ W1g.T) * (x @ W1u.T)) @ W2.T`` over the routed experts, both products with 4-bit operands.
+
+    ``hidden_states`` 16-bit ``[tokens, h]``; ``w1`` ``[experts, 2 inner, h]`` with rows as ``mxfp4_gate_up`` orders them, ``w2``
+    ``[experts, h, inner]``; ``topk_weights`` (fp32 or the activations' type) and ``topk_ids`` (int32 or int64) ``[tokens, k]``.  Tokens are
+    quantised once and sorted by expert, the activation is quantised from the first product's sums, a slot's output is
+    rounded to 16 bits before it is weighted, and the weighted sum is held in 32 bits.  Ids that name no expert add nothing."""
+    for w, what in ((w1, "w1"), (w2, "w2")):
+        if not isinstance(w, MXFP4):
+            raise ValueError(f"fused_moe_mxfp4: {what} must be MXFP4, got {type(w).__name__}")
+        _check(w, f"fused_moe_mxfp4: {what}", 3)
+    x, dtype = hidden_states, hidden_states.dtype
+    _together("fused_moe_mxfp4", x, w1.codes, w2.codes, topk_weights, topk_ids)
+    code = dtype_code(x, "hidden_states")
+    experts, rows1, hidden, inner = w1.codes.shape[0], w1.rows, w1.k, w2.k
+    if x.dim() != 2 or x.shape[1] != hidden:
+        raise ValueError(f"fused_moe_mxfp4: hidden_states of shape {tuple(x.shape)} under experts of {hidden} inputs")
+    if w2.codes.shape[0] != experts or w2.rows != hidden or rows1 != 2 * inner or inner % GATE_RUN != 0:
+        raise ValueError(f"fused_moe_mxfp4: w1 [{experts}, {rows1}, {hidden}] and w2 {[*w2.codes.shape[:2], inner]} do not belong together")
+    tokens = x.shape[0]
+    if topk_ids.dim() != 2 or topk_ids.shape[0] != tokens or topk_ids.shape != topk_weights.shape or topk_ids.shape[1] == 0:
+        raise ValueError(f"fused_moe_mxfp4: ids {tuple(topk_ids.shape)} and weights {tuple(topk_weights.shape)} for {tokens} tokens")
+    if topk_weights.dtype not in (torch.float32, dtype):
+        raise ValueError(f"fused_moe_mxfp4: weights must be float32 or {dtype}, got {topk_weights.dtype}")
+    width = index_width(topk_ids, "topk_ids")
+    top_k = topk_ids.shape[1]
+    slots = tokens * top_k
+    out = torch.empty((tokens, hidden), dtype=dtype, device=x.device)
+    if tokens == 0:
+        return out
+    x, ids, weights = _aligned(x), topk_ids.contiguous(), topk_weights.contiguous()
+    with _on(x):
+        L, dev, st = lib(), x.device, stream_handle()
+        tile = _tile_rows(slots, experts)
+        tiles = L.b2l_mxfp4_moe_max_tiles(slots, tile, experts)
+        if not (w1.ready and w2.ready):
+            weights_written()
+
+        def buffer(*shape):
+            return torch.empty(shape, dtype=torch.uint8, device=dev)
+
+        plan = torch.empty(slots + 1 + 2 * tiles, dtype=torch.int32, device=dev)
+        place, table = plan.data_ptr(), plan.data_ptr() + 4 * slots
+        check(L.b2l_mxfp4_moe_sort(place, table, ids.data_ptr(), width, slots, tile, experts, st))
+        xq, xs = buffer(tiles * tile, hidden // 2), buffer(*_tiles(128 * tiles, hidden))
+        check(L.b2l_mxfp4_moe_scatter(xq.data_ptr(), xs.data_ptr(), x.data_ptr(), place, tokens, top_k, tile, hidden, _row_stride(x),
+                                      code, st))
+        aq, as_ = buffer(tiles * tile, inner // 2), buffer(*_tiles(128 * tiles, inner))
+        check(L.b2l_mxfp4_grouped_matmul(aq.data_ptr(), as_.data_ptr(), xq.data_ptr(), xs.data_ptr(), w1.codes.data_ptr(),
+                                         w1.scales.data_ptr(), table, tiles, tile, experts, rows1, hidden, 1, code, st))
+        y = torch.empty((tiles * tile, hidden), dtype=dtype, device=dev)
+        check(L.b2l_mxfp4_grouped_matmul(y.data_ptr(), None, aq.data_ptr(), as_.data_ptr(), w2.codes.data_ptr(), w2.scales.data_ptr(),
+                                         table, tiles, tile, experts, hidden, inner, 0, code, st))
+        check(L.b2l_mxfp4_moe_combine(out.data_ptr(), y.data_ptr(), place, weights.data_ptr(), int(weights.dtype == torch.float32),
+                                      tokens, top_k, hidden, code, st))
+    return out

@@ -179,3 +179,109 @@ def test_products_against_64_bits(dtype, t, n, k, with_bias):
     bound = O.product_bound(xv, wv, want + (0 if b is None else b.double()), dtype)
     want = want if b is None else want + b.double()
     assert y.dtype == dtype and ((y.double() - want).abs() <= bound).all()
+
+
+# ------------------------------------------------------------------------------------------------- the gated feed-forward
+def gated_weights(inner, k, lead=()):
+    gate, up = (torch.randn(*lead, inner, k, device="cuda") * 0.05 for _ in range(2))
+    q = K.mxfp4_quantize_weight(K.mxfp4_gate_up(gate, up))
+    return q, O.rounded(gate), O.rounded(up)
+
+
+def act_errors(g, u, sums_g, sums_u, k):
+    """How far silu(g) u may be off before it is quantised: each product as ``product_bound`` without the rounding, the activation's
+    slope in g is at most 1.1, and 2^-20 of it for the exponential and the quotient."""
+    e = k * 2.0 ** -23
+    act = torch.nn.functional.silu(g) * u
+    return act, 1.1 * e * sums_g * u.abs() + e * sums_u * torch.nn.functional.silu(g).abs() + 2.0 ** -20 * act.abs()
+
+
+def quantised_near(q, act, off):
+    """Every value is what some value within `off` of `act` is quantised to: rounding and scales grow with the value, so it lies
+    between the quantised ends; a block whose largest magnitude may be on either side of a power of two has either scale."""
+    got = K.mxfp4_dequantize(q, torch.float32).double().unflatten(-1, (-1, 32))
+    byte = O.scale_rows(q.scales, q.rows, q.k)
+    a, o = act.unflatten(-1, (-1, 32)), off.unflatten(-1, (-1, 32))
+    high, low = (a.abs() + o).amax(-1), (a.abs() - o).amax(-1).clamp(min=0)
+    top = [torch.where(m > 0, (torch.frexp(m)[1] - 3 + 127).clamp(0, 254), 0) for m in (low, high)]
+    assert ((byte >= top[0]) & (byte <= top[1])).all()
+    scale = torch.exp2(byte.double() - 127)[..., None]
+
+    def grid(v):
+        t = (v / scale).abs()
+        step = torch.where(t < 2, 0.5, torch.where(t < 4, 1.0, 2.0))
+        return torch.sign(v) * (torch.round(t / step) * step).clamp(max=6) * scale
+    assert ((got >= grid(a - o)) & (got <= grid(a + o))).all()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,inner,k", ((1, 64, 64), (3, 128, 96), (32, 192, 256), (20, 4864, 896), (50, 320, 1120), (100, 448, 512), (128, 64, 2048)))
+@pytest.mark.parametrize("with_bias", (False, True))
+def test_feed_forward_quantises_its_own_sums(dtype, t, inner, k, with_bias):
+    x = torch.randn(t, k, device="cuda").to(dtype)
+    w, gate, up = gated_weights(inner, k)
+    bias = None
+    xv = O.rounded(x)
+    g, u = xv @ gate.t(), xv @ up.t()
+    if with_bias:
+        bg, bu = (torch.randn(inner, 1, device="cuda").to(dtype) for _ in range(2))
+        bias = K.mxfp4_gate_up(bg, bu).flatten()
+        g, u = g + bg.double().t(), u + bu.double().t()
+    q = K.mxfp4_matmul(x, w, bias=bias, swiglu=True)
+    assert (q.rows, q.k) == (t, inner)
+    act, off = act_errors(g, u, xv.abs() @ gate.abs().t() + g.abs(), xv.abs() @ up.abs().t() + u.abs(), k)
+    quantised_near(q, act, off)
+    behind = q.scales.permute(0, 3, 2, 1, 4).flatten(-2).flatten(0, 2)[:t, inner // 32:]
+    assert not behind.any()                                              # blocks behind the end are zero
+
+
+# ------------------------------------------------------------------------------------------------- routed experts
+def experts_reference(x, w1, gate, up, down, weights, ids, dtype):
+    """The operator step by step with the framework's own quantised activations in the middle: (out, how far off)."""
+    tokens = x.shape[0]
+    out, off = torch.zeros(tokens, down.shape[1], dtype=torch.float64, device="cuda"), torch.zeros(tokens, down.shape[1], dtype=torch.float64, device="cuda")
+    for e in range(gate.shape[0]):
+        t, j = torch.nonzero(ids == e, as_tuple=True)
+        if not t.numel():
+            continue
+        q = K.mxfp4_matmul(x[t], K.MXFP4(w1.codes[e], w1.scales[e]), swiglu=True)
+        act = O.values(O.unpack_codes(q.codes), O.scale_rows(q.scales, q.rows, q.k))
+        y = act @ down[e].t()
+        w = weights[t, j].double()[:, None]
+        out.index_add_(0, t, w * y)
+        off.index_add_(0, t, w.abs() * O.product_bound(act, down[e], y, dtype))
+    k = ids.shape[1]
+    return out, off * (1 + k * 2.0 ** -23) + k * 2.0 ** -23 * off.new_tensor(1) * out.abs() + out.abs() * torch.finfo(dtype).eps / 2 + 1e-7
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("experts,top_k,hidden,inner,tokens", ((4, 2, 64, 64, 1), (8, 2, 256, 128, 5), (8, 3, 96, 192, 40), (16, 2, 256, 64, 300), (3, 2, 160, 128, 129),
+                                                               (4, 4, 128, 320, 200)))
+def test_experts_step_by_step(dtype, experts, top_k, hidden, inner, tokens):
+    x = torch.randn(tokens, hidden, device="cuda").to(dtype)
+    w1, gate, up = gated_weights(inner, hidden, (experts,))
+    down = torch.randn(experts, hidden, inner, device="cuda") * 0.05
+    w2 = K.mxfp4_quantize_weight(down)
+    top = torch.softmax(torch.randn(tokens, experts, device="cuda"), -1).topk(top_k, -1)
+    for weights, ids in ((top.values.to(dtype), top.indices), (top.values, top.indices.int())):
+        want, off = experts_reference(x, w1, gate, up, O.rounded(down), weights, ids, dtype)
+        got = K.fused_moe_mxfp4(x, w1, w2, weights, ids)
+        assert ((got.double() - want).abs() <= off).all()
+        assert torch.equal(got, K.fused_moe_mxfp4(x, w1, w2, weights, ids))
+
+
+def test_experts_without_tokens_the_same_twice_and_ids_of_none():
+    experts, hidden, inner = 8, 128, 64
+    x = torch.randn(70, hidden, device="cuda").half()
+    w1, gate, up = gated_weights(inner, hidden, (experts,))
+    down = torch.randn(experts, hidden, inner, device="cuda") * 0.05
+    w2 = K.mxfp4_quantize_weight(down)
+    weights = torch.rand(70, 3, device="cuda")
+    ids = torch.randint(0, 2, (70, 3), device="cuda")                    # six experts see nobody, some tokens one expert twice
+    ids[5], ids[6, 1], ids[7, 2], ids[9, 0] = -1, 8, 2 ** 40, -7
+    want, off = experts_reference(x, w1, gate, up, O.rounded(down), weights, ids, torch.float16)
+    got = K.fused_moe_mxfp4(x, w1, w2, weights, ids)
+    assert ((got.double() - want).abs() <= off).all() and not got[5].any()
+    none = K.fused_moe_mxfp4(x, w1, w2, weights, torch.full_like(ids, -1))
+    assert not none.any()
+    assert K.fused_moe_mxfp4(x[:0], w1, w2, weights[:0], ids[:0]).shape == (0, hidden)
