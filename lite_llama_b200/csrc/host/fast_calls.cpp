@@ -49,6 +49,19 @@ struct {
                     int, const void*, int, i64, i64, i64, int, int, int, int, i64, float, i64, i64, i64, i64, void*, i64, int, void*);
   int (*slot_maps)(void*, void*, void*, void*, const void*, int, const void*, int, const void*, int, const void*, int, void*, i64, i64, i64,
                    i64, i64, i64, void*);
+  int (*weights_written)(void*);
+  i64 (*mx4_scale_bytes)(i64, i64);
+  int (*mx4_quantize)(void*, void*, const void*, i64, i64, i64, i64, int, void*);
+  int (*mx4_dequantize)(void*, const void*, const void*, i64, i64, i64, i64, int, void*);
+  int (*mx4_norm)(void*, void*, void*, const void*, const void*, const void*, i64, i64, i64, i64, i64, float, int, void*);
+  int (*mx4_matmul)(void*, void*, const void*, const void*, const void*, const void*, const void*, i64, i64, i64, i64, i64, i64, int, int, int,
+                    void*);
+  i64 (*mx4_tile_rows)(i64, int);
+  i64 (*mx4_max_tiles)(i64, int, int);
+  int (*mx4_sort)(void*, void*, const void*, int, i64, int, int, void*);
+  int (*mx4_scatter)(void*, void*, const void*, const void*, i64, int, int, i64, i64, int, void*);
+  int (*mx4_grouped)(void*, void*, const void*, const void*, const void*, const void*, const void*, i64, int, int, i64, i64, int, int, void*);
+  int (*mx4_combine)(void*, const void*, const void*, const void*, int, i64, int, i64, int, void*);
   const char* (*last_error)();
 } abi;
 PyObject* py_zeroed = nullptr;      // kernels._common.zeroed_workspace(bytes, device)
@@ -578,6 +591,207 @@ PyObject* slot_maps(PyObject*, PyObject* const* a, Py_ssize_t count) {
   FAST_END
 }
 
+// ---- microscaled 4-bit operands (kernels/quantization/mxfp4.py) ----
+// An MXFP4 (a named tuple) of one matrix or a stack: the tensors as the class describes them.
+struct Mx4 { const at::Tensor *codes = nullptr, *scales = nullptr; bool ready = false; i64 lead = 1, rows = 0, k = 0; };
+i64 up(i64 n, i64 to) { return (n + to - 1) / to; }
+bool mx4(PyObject* o, i64 dims, Mx4& m) {
+  if (!PyTuple_Check(o) || PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 3) return false;
+  const at::Tensor *c = plain(PyTuple_GET_ITEM(o, 0)), *s = plain(PyTuple_GET_ITEM(o, 1));
+  if (!c || !s || c->scalar_type() != at::kByte || s->scalar_type() != at::kByte || c->dim() != dims || s->dim() != dims + 3) return false;
+  if (!c->is_contiguous() || !s->is_contiguous() || c->numel() == 0 || (uintptr_t)c->data_ptr() % 16 || (uintptr_t)s->data_ptr() % 16) return false;
+  m.rows = c->size(dims - 2);
+  m.k = 2 * c->size(dims - 1);
+  m.lead = dims == 3 ? c->size(0) : 1;
+  if (m.k % 32 != 0 || (dims == 3 && s->size(0) != m.lead)) return false;
+  const i64 want[5] = {up(m.rows, 128), up(m.k, 128), 32, 4, 4};
+  for (int i = 0; i < 5; ++i)
+    if (s->size(dims - 2 + i) != want[i]) return false;
+  m.codes = c;
+  m.scales = s;
+  m.ready = PyTuple_GET_ITEM(o, 2) == Py_True;
+  return true;
+}
+// rows of activations that the quantiser reads as they are
+bool mx4_rows(const at::Tensor& x, bool wide) {
+  if (!matrix(x) || x.size(1) % 32 != 0 || (half_code(x) < 0 && !(wide && x.scalar_type() == at::kFloat))) return false;
+  return (uintptr_t)x.data_ptr() % 16 == 0 && x.stride(0) >= 0 && x.stride(0) * x.element_size() % 16 == 0;
+}
+at::Tensor mx4_tiles(const at::Tensor& like, i64 rows, i64 k) {
+  return at::empty({up(rows, 128), up(k, 128), 32, 4, 4}, like.options().dtype(at::kByte));
+}
+at::Tensor bytes_of(const at::Tensor& like, i64 n) { return at::empty({n}, like.options().dtype(at::kByte)); }
+
+// x -> (codes, scales)
+PyObject* mx4_quantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(1)
+  FAST_BEGIN
+  const at::Tensor* x = plain(a[0]);
+  const int device = device_for(abi.mx4_quantize, {x});
+  if (device < 0 || !mx4_rows(*x, true)) return none();
+  const i64 m = x->size(0), k = x->size(1);
+  at::Tensor c, s;
+  int rc;
+  {
+    const Unlocked unlocked;
+    c = at::empty({m, k / 2}, x->options().dtype(at::kByte));
+    s = mx4_tiles(*x, m, k);
+    rc = abi.mx4_quantize(c.data_ptr(), s.data_ptr(), x->data_ptr(), 1, m, k, x->stride(0), x->scalar_type() == at::kFloat ? 2 : half_code(*x),
+                          stream(device));
+  }
+  return rc ? failed(rc) : pair_of(std::move(c), std::move(s));
+  FAST_END
+}
+
+// (MXFP4, dtype) -> values
+PyObject* mx4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(2)
+  FAST_BEGIN
+  Mx4 q;
+  if (!mx4(a[0], 2, q) || !THPDtype_Check(a[1])) return none();
+  const int device = device_for(abi.mx4_dequantize, {q.codes, q.scales});
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[1])->scalar_type;
+  if (device < 0 || (type != at::kHalf && type != at::kBFloat16)) return none();
+  at::Tensor y;
+  int rc;
+  {
+    const Unlocked unlocked;
+    y = at::empty({q.rows, q.k}, q.codes->options().dtype(type));
+    rc = abi.mx4_dequantize(y.data_ptr(), q.codes->data_ptr(), q.scales->data_ptr(), 1, q.rows, q.k, q.k / 2, half_code(y), stream(device));
+  }
+  return rc ? failed(rc) : THPVariable_Wrap(std::move(y));
+  FAST_END
+}
+
+// (X, residual or None, weight, eps, out_residual or None) -> (codes, scales)
+PyObject* mx4_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(5)
+  FAST_BEGIN
+  const at::Tensor *x = plain(a[0]), *r = a[1] == Py_None ? nullptr : plain(a[1]), *w = plain(a[2]), *o = a[4] == Py_None ? r : plain(a[4]);
+  const int device = a[1] == Py_None ? device_for(abi.mx4_norm, {x, w}) : device_for(abi.mx4_norm, {x, w, r, o});
+  if (device < 0 || !PyFloat_CheckExact(a[3]) || (a[1] == Py_None && a[4] != Py_None)) return none();
+  const i64 n = x->dim() > 1 ? x->size(-1) : 0;
+  if (n == 0 || n % 32 != 0 || n > 16384 || x->numel() == 0 || half_code(*x) < 0 || w->dim() != 1 || w->size(0) != n) return none();
+  for (const at::Tensor* t : {x, w, r, o}) {
+    if (!t) continue;
+    if (t->scalar_type() != x->scalar_type() || !t->is_contiguous() || (uintptr_t)t->data_ptr() % 16) return none();
+    if (t != w && t->sizes() != x->sizes()) return none();
+  }
+  const i64 rows = x->numel() / n;
+  at::Tensor c, s;
+  int rc;
+  {
+    const Unlocked unlocked;
+    c = at::empty({rows, n / 2}, x->options().dtype(at::kByte));
+    s = mx4_tiles(*x, rows, n);
+    rc = abi.mx4_norm(c.data_ptr(), s.data_ptr(), o ? o->data_ptr() : nullptr, x->data_ptr(), r ? r->data_ptr() : nullptr, w->data_ptr(), rows, n,
+                      n, n, n, (float)PyFloat_AS_DOUBLE(a[3]), half_code(*x), stream(device));
+  }
+  return rc ? failed(rc) : pair_of(std::move(c), std::move(s));
+  FAST_END
+}
+
+// (x or MXFP4, MXFP4, bias or None, swiglu, out_dtype or None) -> y, with swiglu (codes, scales)
+PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(5)
+  FAST_BEGIN
+  Mx4 w, q;
+  if (!mx4(a[1], 2, w)) return none();
+  const at::Tensor *x = plain(a[0]), *bias = a[2] == Py_None ? w.codes : plain(a[2]);
+  if (!x && !mx4(a[0], 2, q)) return none();
+  const int device = device_for(abi.mx4_matmul, {x ? x : q.codes, x ? x : q.scales, w.codes, w.scales, bias});
+  if (device < 0 || (a[4] != Py_None && !THPDtype_Check(a[4])) || !PyBool_Check(a[3])) return none();
+  const bool gated = a[3] == Py_True;
+  if (x && (!mx4_rows(*x, false) || x->size(1) != w.k)) return none();
+  if (!x && q.k != w.k) return none();
+  at::ScalarType type = x ? x->scalar_type() : bias != w.codes ? bias->scalar_type() : at::kHalf;
+  if (a[4] != Py_None) {
+    const at::ScalarType wanted = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+    if (x && wanted != type) return none();
+    type = wanted;
+  }
+  if (type != at::kHalf && type != at::kBFloat16) return none();
+  if (bias != w.codes && (bias->dim() != 1 || bias->size(0) != w.rows || !bias->is_contiguous() || bias->scalar_type() != type)) return none();
+  if (gated && w.rows % 128 != 0) return none();
+  const i64 t = x ? x->size(0) : q.rows, n = w.rows, k = w.k;
+  const int code = type == at::kHalf ? 0 : 1;
+  at::Tensor y, ys, held;
+  int rc = 0;
+  {
+    const Unlocked unlocked;
+    const void *xc, *xs;
+    void* st = stream(device);
+    if (x) {
+      const i64 at = up(t * k / 2, 256) * 256;
+      held = bytes_of(*x, at + abi.mx4_scale_bytes(t, k));
+      xc = held.data_ptr();
+      xs = (const char*)xc + at;
+      rc = abi.mx4_quantize((void*)xc, (void*)xs, x->data_ptr(), 1, t, k, x->stride(0), code, st);
+    } else {
+      xc = q.codes->data_ptr();
+      xs = q.scales->data_ptr();
+    }
+    if (!rc && !w.ready) rc = abi.weights_written(st);
+    y = at::empty({t, gated ? n / 4 : n}, w.codes->options().dtype(gated ? at::kByte : type));
+    if (gated) ys = mx4_tiles(*w.codes, t, n / 2);
+    if (!rc)
+      rc = abi.mx4_matmul(y.data_ptr(), gated ? ys.data_ptr() : nullptr, xc, xs, w.codes->data_ptr(), w.scales->data_ptr(),
+                          bias == w.codes ? nullptr : bias->data_ptr(), t, n, k, k / 2, k / 2, gated ? n / 4 : n, gated ? 1 : 0, 1, code, st);
+  }
+  if (rc) return failed(rc);
+  return gated ? pair_of(std::move(y), std::move(ys)) : THPVariable_Wrap(std::move(y));
+  FAST_END
+}
+
+// (hidden_states, w1, w2, topk_weights, topk_ids) -> out
+PyObject* mx4_moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(5)
+  FAST_BEGIN
+  Mx4 w1, w2;
+  if (!mx4(a[1], 3, w1) || !mx4(a[2], 3, w2)) return none();
+  const at::Tensor *x = plain(a[0]), *weights = plain(a[3]), *ids = plain(a[4]);
+  const int device = device_for(abi.mx4_grouped, {x, weights, ids, w1.codes, w1.scales, w2.codes, w2.scales});
+  if (device < 0 || !mx4_rows(*x, false) || x->size(1) != w1.k) return none();
+  const i64 tokens = x->size(0), hidden = w1.k, inner = w2.k, experts = w1.lead;
+  if (w2.lead != experts || w2.rows != hidden || w1.rows != 2 * inner || inner % 64 != 0 || experts > 4096) return none();
+  if (ids->dim() != 2 || ids->size(0) != tokens || ids->size(1) < 1 || ids->size(1) > 65536 || weights->sizes() != ids->sizes() ||
+      !ids->is_contiguous() || !weights->is_contiguous())
+    return none();
+  const int width = ids->scalar_type() == at::kInt ? 4 : ids->scalar_type() == at::kLong ? 8 : 0;
+  const bool wide = weights->scalar_type() == at::kFloat;
+  if (!width || (!wide && weights->scalar_type() != x->scalar_type())) return none();
+  const int top_k = (int)ids->size(1), code = half_code(*x), e = (int)experts;
+  const i64 slots = tokens * top_k;
+  const int tile = (int)abi.mx4_tile_rows(slots, e);
+  const i64 tiles = abi.mx4_max_tiles(slots, tile, e), rows = tiles * tile;
+  // one buffer for what lives within the call
+  i64 size = 0;
+  auto part = [&](i64 n) { const i64 at = size; size += up(n, 256) * 256; return at; };
+  const i64 place = part(4 * slots), table = part(4 + 8 * tiles), xc = part(rows * (hidden / 2)), xs = part(abi.mx4_scale_bytes(128 * tiles, hidden)),
+            ac = part(rows * (inner / 2)), as = part(abi.mx4_scale_bytes(128 * tiles, inner)), y = part(2 * rows * hidden);
+  at::Tensor out, held;
+  int rc = 0;
+  {
+    const Unlocked unlocked;
+    held = bytes_of(*x, size);
+    out = at::empty({tokens, hidden}, x->options());
+    char* p = (char*)held.data_ptr();
+    void* st = stream(device);
+    if (!w1.ready || !w2.ready) rc = abi.weights_written(st);
+    if (!rc) rc = abi.mx4_sort(p + place, p + table, ids->data_ptr(), width, slots, tile, e, st);
+    if (!rc) rc = abi.mx4_scatter(p + xc, p + xs, x->data_ptr(), p + place, tokens, top_k, tile, hidden, x->stride(0), code, st);
+    if (!rc)
+      rc = abi.mx4_grouped(p + ac, p + as, p + xc, p + xs, w1.codes->data_ptr(), w1.scales->data_ptr(), p + table, tiles, tile, e, w1.rows, hidden, 1,
+                           code, st);
+    if (!rc)
+      rc = abi.mx4_grouped(p + y, nullptr, p + ac, p + as, w2.codes->data_ptr(), w2.scales->data_ptr(), p + table, tiles, tile, e, hidden, inner, 0,
+                           code, st);
+    if (!rc) rc = abi.mx4_combine(out.data_ptr(), p + y, p + place, weights->data_ptr(), wide ? 1 : 0, tokens, top_k, hidden, code, st);
+  }
+  return rc ? failed(rc) : THPVariable_Wrap(std::move(out));
+  FAST_END
+}
+
 // (addresses of the C functions in the order of `abi`, zeroed_workspace, counters)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t count) {
   constexpr Py_ssize_t n = sizeof(abi) / sizeof(void*);
@@ -595,7 +809,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t count) {
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(init), FAST(w8a16), FAST(w4a16_packed), FAST(linear), FAST(w8a8), FAST(quantize), FAST(norm),
                          FAST(norm_quant), FAST(swiglu), FAST(kv4_rope_write), FAST(kv4_read), FAST(kv4_decode), FAST(kv4_prompt),
-                         FAST(slot_maps), {nullptr, nullptr, 0, nullptr}};
+                         FAST(slot_maps), FAST(mx4_quantize), FAST(mx4_dequantize), FAST(mx4_norm), FAST(mx4_matmul), FAST(mx4_moe),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods};
 
 }  // namespace

@@ -11,6 +11,7 @@
 // the order of the parts: nothing outlives the launch, so calls on several streams and captured graphs share nothing.
 #include "gemm_tc.cuh"
 #include "mxfp4_mma.cuh"
+#include "mxfp4_gemm.cuh"
 #include "pair.cuh"
 
 namespace mx4 {
@@ -542,6 +543,10 @@ extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const vo
   B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales) % 16 == 0 && (x_row_stride | w_row_stride) % 16 == 0 &&
                   (!gated || ((uintptr_t)y % 4 == 0 && y_row_stride % 4 == 0)),
               "mxfp4_matmul: rows of codes must start on 16 bytes");
+  B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "mxfp4_matmul: dtype %d", dtype);
+  cudaStream_t st = (cudaStream_t)stream;
+  mx4::PairCall g = {y, y_row_stride, y_scales, bias, x, x_scales, w, w_scales, t, n, k, x_row_stride, w_row_stride, gated != 0};
+  if (mx4::pair_wanted(g)) return mx4::pair_gemm(g, dtype, st);
   mx4::Params p;
   p.y = y; p.ldy = y_row_stride;
   p.y_scales = (uint8_t*)y_scales; p.y_ktiles = mx4::k_tiles(n / 2);
@@ -551,10 +556,8 @@ extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const vo
   p.T = (int)t; p.N = (int)n; p.K = (int)k; p.num_kb = (int)cdiv64(k, mx4::kStageK);
   p.early = weights_ready;
   p.vec = n % 4 == 0 && y_row_stride % 4 == 0 && (uintptr_t)y % 8 == 0;
-  cudaStream_t st = (cudaStream_t)stream;
   if (dtype == B2L_F16) return mx4::stream_gemm<__half>(x, x_row_stride, w, w_row_stride, p, gated != 0, st);
-  if (dtype == B2L_BF16) return mx4::stream_gemm<__nv_bfloat16>(x, x_row_stride, w, w_row_stride, p, gated != 0, st);
-  B2L_UNSUPPORTED("mxfp4_matmul: dtype %d", dtype);
+  return mx4::stream_gemm<__nv_bfloat16>(x, x_row_stride, w, w_row_stride, p, gated != 0, st);
 }
 
 extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w,

@@ -1,0 +1,335 @@
+// Y = X W^T with both operands in microscaled 4-bit floating point, for prompt-sized batches, on CTA pairs.
+//
+// Bound: the tensor pipe (four times the rate of 16-bit operands), and right behind it what L2 can bring: a pair multiplies 256
+// tokens x 256 outputs, 35 KiB per SM for 256 k.  As in gemm_pair.cu, with what the rate and the scales ask for:
+//   * tokens are the MMA's rows, so a thread holds consecutive outputs of one token: 16-byte stores to shared memory and one TMA
+//     store per 32 tokens x 64 outputs, or, for the gated unit, a token's 32 activations, which it quantises alone;
+//   * 512 columns of tensor memory hold two accumulators of 256 only if the scales have none.  The accumulators overlap by 48 columns:
+//     [0, 256) and [208, 464), scales behind them.  The shared columns are read out first and handed on at once, so a tile's products
+//     start when a quarter of the tile before has been read, and the rest is written out under them;
+//   * scales are TMA copies of whole tiles into every stage; both CTAs hold those of all 256 outputs.  Two sets of 24 columns take turns:
+//     a set is written again when the MMAs of two stages ago have retired.
+#include "gemm_tc.cuh"
+#include "mxfp4_mma.cuh"
+#include "mxfp4_gemm.cuh"
+#include "pair.cuh"
+
+namespace mx4 {
+
+constexpr int kPairThreads = 6 * 32;   // TMA producer, MMA issuer, four warps that read the accumulator
+constexpr int kPairStages = 5;
+constexpr int kPairRows = 128;         // tokens per CTA
+constexpr int kPairBand = 16;          // token tiles per band: 16 x 256 rows x 4096 / 2 bytes = 8 MiB of L2
+
+template <int BN> struct PairRing {
+  static constexpr int kX = 16384, kW = BN / 2 * 128;
+  static constexpr int kXs = kX + kW, kWs = kXs + kSfBytes;
+  static constexpr int kBytes = kWs + BN / 128 * kSfBytes;
+  static constexpr int kSmem = 1024 + 1024 + kPairStages * kBytes + 4 * 2 * 4096;
+  static constexpr int kAcc1 = BN == 256 ? 208 : 128;                     // first column of the second accumulator
+  static constexpr int kSf = BN == 256 ? 464 : 256;
+  static constexpr int kSfSet = 8 + BN / 128 * 8;
+};
+
+struct PairParams {
+  const void* bias;
+  uint8_t* y; uint8_t* y_scales; int64_t ldy, y_ktiles;                   // gated: codes and scales
+  int T, N, K, num_kb, m_tiles, n_tiles, ktiles;
+};
+
+struct __align__(8) PairControl {
+  uint64_t full[kPairStages];          // leader: both CTAs' operands and scales of a stage have landed
+  uint64_t empty[kPairStages];         // both: the MMAs of a stage have retired
+  uint64_t acc_full[2];                // both: a tile's accumulator is complete
+  uint64_t freed[2];                   // leader: all eight warps have read what the next tile's products overwrite
+  uint32_t tmem;
+};
+
+// 32 values of one row: scale byte and codes
+__device__ __forceinline__ uint32_t quantise32(float (&v)[32], uint4& codes) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) m = max(m, abs_bits(v[j]));
+  const uint32_t byte = scale_byte(m);
+  const float inv = inverse_scale(byte);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] *= inv;
+  uint32_t c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c[j] = byte == 255u ? 0u : codes8(*reinterpret_cast<float(*)[8]>(v + 8 * j));
+  codes = make_uint4(c[0], c[1], c[2], c[3]);
+  return byte;
+}
+
+template <typename T, int BN, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_xs,
+            const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_y, const PairParams p) {
+  using R = PairRing<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  PairControl* ctl = reinterpret_cast<PairControl*>(smem);
+  uint8_t* ring = smem + 1024;
+  uint8_t* out_stage = ring + kPairStages * R::kBytes;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = pair_rank();
+  const int pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
+  const int tiles = p.m_tiles * p.n_tiles;
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_x);
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_xs);
+    tma_prefetch_desc(&tmap_ws);
+    if (!GATED) tma_prefetch_desc(&tmap_y);
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&ctl->full[s], 1);
+      mbar_init(&ctl->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&ctl->acc_full[b], 1);
+      mbar_init(&ctl->freed[b], 8);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&ctl->tmem, 512);
+    tmem_relinquish_pair();
+    pdl_launch_dependents();           // after the allocation (gemm_dense.cu)
+  }
+  tc_fence_before();
+  pair_sync();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+
+  if (warp == 0) {
+    // ===================== TMA producer: this CTA's halves of both operands, its tokens' scales, all outputs' scales =====================
+    pdl_wait_prior();
+    gemm::PipeState ps(kPairStages);
+    for (int t = pair; t < tiles; t += pairs) {
+      const PairTile pt = pair_tile(t, p.m_tiles, p.n_tiles, kPairBand);
+      const int row_x = (pt.m * 2 + (int)rank) * kPairRows, row_w = pt.n * BN + (int)rank * (BN / 2);
+      const int xs = (pt.m * 2 + (int)rank) * p.ktiles * 4, ws = pt.n * (BN / 128) * p.ktiles * 4;      // rows of 128 bytes
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(&ctl->full[ps.stage], 2 * R::kBytes);
+          uint8_t* st = ring + (size_t)ps.stage * R::kBytes;
+          const uint32_t bar = leader_addr(&ctl->full[ps.stage]);
+          tma_load_2d_pair(st, &tmap_x, kb * 128, row_x, bar, kEvictNormal);
+          tma_load_2d_pair(st + R::kX, &tmap_w, kb * 128, row_w, bar, kEvictNormal);
+          tma_load_2d_pair(st + R::kXs, &tmap_xs, 0, xs + kb * 8, bar, kEvictNormal);
+#pragma unroll
+          for (int h = 0; h < BN / 128; ++h)
+            tma_load_2d_pair(st + R::kWs + h * kSfBytes, &tmap_ws, 0, ws + h * p.ktiles * 4 + kb * 8, bar, kEvictNormal);
+        }
+        __syncwarp();
+        ps.advance();
+      }
+    }
+    // every stage handed back: no commit is still on its way to this CTA's barriers when it leaves
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
+      ps.advance();
+    }
+  } else if (warp == 1) {
+    // ===================== MMA issuer (leader only) =====================
+    if (rank == 0) {
+      const uint64_t desc0 = umma_desc_sw128_kmajor(smem_u32(ring)), sf0 = scale_desc(smem_u32(ring));
+      gemm::PipeState ps(kPairStages), back(kPairStages);      // back: the stage two before
+      int it = 0, i = 0;
+      for (int t = pair; t < tiles; t += pairs, ++it) {
+        const uint32_t acc = tmem + (it & 1) * R::kAcc1;
+        if (BN == 256) {
+          if (it >= 1) mbar_wait(&ctl->freed[(it - 1) & 1], ((it - 1) >> 1) & 1);
+        } else {
+          if (it >= 2) mbar_wait(&ctl->freed[it & 1], ((it - 2) >> 1) & 1);
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < p.num_kb; ++kb, ++i) {
+          if (i >= 2) {
+            mbar_wait(&ctl->empty[back.stage], back.phase);
+            back.advance();
+          }
+          mbar_wait(&ctl->full[ps.stage], ps.phase);
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t base = (uint64_t)(ps.stage * R::kBytes) >> 4;
+            const uint64_t xd = desc0 + base, wd = xd + (R::kX >> 4);
+            const uint64_t xsf = sf0 + base + (R::kXs >> 4), wsf = sf0 + base + (R::kWs >> 4);
+            const uint32_t sfa = tmem + R::kSf + (i & 1) * R::kSfSet, sfb = sfa + 8;
+            const int steps = (p.K - kb * kStageK + 63) >> 6;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (2 * j < steps) {
+                copy_scales<2>(sfa + 4 * j, xsf + j * (kTileBytes >> 4));
+#pragma unroll
+                for (int h = 0; h < BN / 128; ++h)
+                  copy_scales<2>(sfb + j * (BN / 32) + 4 * h, wsf + h * (kSfBytes >> 4) + j * (kTileBytes >> 4));
+              }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < steps)
+                mma<2>(acc, xd + 2 * j, wd + 2 * j, idesc(256, BN, j & 1), sfa + (j >> 1) * 4, sfb + (j >> 1) * (BN / 32), kb | j ? 1u : 0u);
+            tc_commit_pair(&ctl->empty[ps.stage]);
+            if (kb + 1 == p.num_kb) tc_commit_pair(&ctl->acc_full[it & 1]);
+          }
+          __syncwarp();
+          ps.advance();
+        }
+      }
+    }
+  } else {
+    // ===================== one thread per token =====================
+    const int quad = warp & 3;
+    const uint32_t freed0 = leader_addr(&ctl->freed[0]), freed1 = leader_addr(&ctl->freed[1]);
+    auto hand_on = [&](int buf) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(buf ? freed1 : freed0);
+    };
+    pdl_wait_prior();                  // y may still be read upstream
+    int it = 0, box = 0;
+    for (int t = pair; t < tiles; t += pairs, ++it) {
+      const PairTile pt = pair_tile(t, p.m_tiles, p.n_tiles, kPairBand);
+      const int buf = it & 1;
+      const int m_warp = (pt.m * 2 + (int)rank) * kPairRows + quad * 32;
+      const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * R::kAcc1;
+      mbar_wait(&ctl->acc_full[buf], (it >> 1) & 1);
+      tc_fence_after();
+      if (!GATED) {
+#pragma unroll 1
+        for (int j = 0; j < BN / 64; ++j) {
+          // the shared columns first: the first accumulator's last, the second one's first
+          const int c = (BN == 256 && buf == 0 ? BN / 64 - 1 - j : j) * 64;
+          uint32_t v[64];
+          tmem_ld_32x32b_x32(acc + c, *reinterpret_cast<uint32_t(*)[32]>(v));
+          tmem_ld_32x32b_x32(acc + c + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+          tc_wait_ld();
+          if (j == (BN == 256 ? 0 : BN / 64 - 1)) hand_on(buf);
+          const int n0 = pt.n * BN + c;
+          if (n0 >= p.N || m_warp >= p.T) continue;     // uniform over the warp
+          uint8_t* dst = out_stage + (quad * 2 + (box & 1)) * 4096;
+          if (lane == 0) bulk_wait_read<1>();           // the store that used this box two boxes ago has read it
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            uint32_t o[4];
+            const int n = n0 + 8 * q;
+            uint4 b4 = make_uint4(0u, 0u, 0u, 0u);
+            if (p.bias && n < p.N) b4 = ldg_128(reinterpret_cast<const T*>(p.bias) + n);      // N is a multiple of 8
+            const T* b = reinterpret_cast<const T*>(&b4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[e] = pack2<T>(__uint_as_float(v[8 * q + 2 * e]) + to_f32(b[2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]) + to_f32(b[2 * e + 1]));
+            *reinterpret_cast<uint4*>(dst + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmap_y, dst, n0, m_warp);
+            bulk_commit();
+          }
+          ++box;
+        }
+      } else {
+        // runs of 64 gate and 64 up columns; a run's half that lies on the shared columns is read whole before anything else
+        const int row = m_warp + lane;
+#pragma unroll 1
+        for (int j = 0; j < BN / 128; ++j) {
+          const bool back = BN == 256 && buf == 0;
+          const int c = (back ? BN / 128 - 1 - j : j) * 128;
+          uint32_t held[64];           // the up half of the first accumulator's runs, the gate half of the second's
+          tmem_ld_32x32b_x32(acc + c + (back ? 64 : 0), *reinterpret_cast<uint32_t(*)[32]>(held));
+          tmem_ld_32x32b_x32(acc + c + (back ? 96 : 32), *reinterpret_cast<uint32_t(*)[32]>(held + 32));
+          tc_wait_ld();
+          if (BN == 256 && j == 0) hand_on(buf);
+          const int n0 = pt.n * BN + c;
+          uint32_t bytes = 0;
+          uint4 codes[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t other[32];
+            tmem_ld_32x32b_x32(acc + c + (back ? 0 : 64) + 32 * h, other);
+            tc_wait_ld();
+            if (BN != 256 && j + 1 == BN / 128 && h == 1) hand_on(buf);
+            float v[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float g = __uint_as_float(back ? other[e] : held[32 * h + e]), u = __uint_as_float(back ? held[32 * h + e] : other[e]);
+              if (p.bias && n0 < p.N) {
+                g += to_f32(reinterpret_cast<const T*>(p.bias)[n0 + 32 * h + e]);
+                u += to_f32(reinterpret_cast<const T*>(p.bias)[n0 + 64 + 32 * h + e]);
+              }
+              v[e] = gated(g, u);
+            }
+            bytes |= quantise32(v, codes[h]) << (8 * h);
+          }
+          if (n0 < p.N && row < p.T) {                  // N is a multiple of 128
+            uint8_t* y = p.y + row * p.ldy + n0 / 4;
+            stg_128(y, codes[0]);
+            stg_128(y + 16, codes[1]);
+            const int k = n0 / 2;                       // first activation: a multiple of 64
+            uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles) + ((k >> 5) & 3);
+            if (n0 + 128 == p.N && (k & 64) == 0) *reinterpret_cast<uint32_t*>(word) = bytes;   // nothing behind: zeros
+            else *reinterpret_cast<uint16_t*>(word) = (uint16_t)bytes;
+          }
+        }
+      }
+    }
+    if (!GATED && lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  pair_sync();                         // the peer's MMAs, commits and arrivals are over
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+template <typename T, int BN, bool GATED>
+static int launch_pair(const PairCall& g, cudaStream_t st) {
+  using R = PairRing<BN>;
+  const int pairs = b2l_num_sms() / 2;
+  PairParams p;
+  p.bias = g.bias;
+  p.y = (uint8_t*)g.y; p.y_scales = (uint8_t*)g.y_scales; p.ldy = g.ldy; p.y_ktiles = k_tiles(g.N / 2);
+  p.T = (int)g.T; p.N = (int)g.N; p.K = (int)g.K; p.num_kb = (int)cdiv64(g.K, kStageK); p.ktiles = (int)k_tiles(g.K);
+  p.m_tiles = (int)cdiv64(g.T, 2 * kPairRows);
+  p.n_tiles = (int)cdiv64(g.N, BN);
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  const int grid = 2 * (int)(tiles < pairs ? tiles : pairs);
+  CUtensorMap tx, tw, txs, tws, ty;
+  int rc = b2l_make_tmap_2d(&tx, g.x, TMA_U8, (uint64_t)g.T, (uint64_t)g.K / 2, (uint64_t)g.ldx, kPairRows, 128, true);
+  if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tw, g.w, TMA_U8, (uint64_t)g.N, (uint64_t)g.K / 2, (uint64_t)g.ldw, BN / 2, 128, true);
+  if (rc == B2L_OK) rc = b2l_make_tmap_2d(&txs, g.x_scales, TMA_U8, (uint64_t)(cdiv64(g.T, 128) * p.ktiles * 4), 128, 128, 8, 128, false);
+  if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tws, g.w_scales, TMA_U8, (uint64_t)(cdiv64(g.N, 128) * p.ktiles * 4), 128, 128, 8, 128, false);
+  if (rc == B2L_OK && !GATED)
+    rc = b2l_make_tmap_2d(&ty, g.y, std::is_same<T, __half>::value ? TMA_F16 : TMA_BF16, (uint64_t)g.T, (uint64_t)g.N, (uint64_t)g.ldy * 2, 32, 64, true);
+  if (rc != B2L_OK) return rc;
+  if (GATED) ty = tx;
+  auto kern = pair_kernel<T, BN, GATED>;
+  static int configured[64] = {0};
+  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, R::kSmem, configured));
+  b2l_launch(kern, dim3((unsigned)grid), dim3(kPairThreads), (size_t)R::kSmem, st, tx, tw, txs, tws, ty, p);
+  B2L_LAUNCH_CHECK();
+  return B2L_OK;
+}
+
+bool pair_wanted(const PairCall& g) {
+  if (g.T <= 128) return false;
+  return g.gated ? (uintptr_t)g.y % 16 == 0 && g.ldy % 16 == 0
+                 : g.N % 8 == 0 && g.ldy % 8 == 0 && (uintptr_t)g.y % 16 == 0 && (uintptr_t)g.bias % 16 == 0;
+}
+
+int pair_gemm(const PairCall& g, int dtype, cudaStream_t st) {
+  const int64_t m_tiles = cdiv64(g.T, 2 * kPairRows), pairs = b2l_num_sms() / 2;
+  // waves x tile width is what the grid spends on the tensor pipe
+  const int64_t w256 = cdiv64(m_tiles * cdiv64(g.N, 256), pairs) * 256, w128 = cdiv64(m_tiles * cdiv64(g.N, 128), pairs) * 128;
+  const bool narrow = w128 * 130 < w256 * 100;
+#define PAIR(T) (narrow ? (g.gated ? launch_pair<T, 128, true>(g, st) : launch_pair<T, 128, false>(g, st)) \
+                        : (g.gated ? launch_pair<T, 256, true>(g, st) : launch_pair<T, 256, false>(g, st)))
+  if (dtype == B2L_F16) return PAIR(__half);
+  return PAIR(__nv_bfloat16);
+#undef PAIR
+}
+
+}  // namespace mx4

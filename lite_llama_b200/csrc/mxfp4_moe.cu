@@ -151,6 +151,12 @@ static int combine(void* out, const void* y, const void* place, const void* weig
 
 }  // namespace mx4
 
+// Rows of an expert's tile, the MMA's columns: more than an expert's rows are products of nothing, fewer read its weights again.
+extern "C" int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts) {
+  const int64_t e = experts > 0 ? experts : 1;
+  return slots <= 24 * e ? 32 : (slots <= 48 * e ? 64 : 128);
+}
+
 extern "C" int64_t b2l_mxfp4_moe_max_tiles(int64_t slots, int tile_rows, int experts) {
   if (slots <= 0 || tile_rows <= 0 || experts <= 0) return 0;
   return slots / tile_rows + (slots < experts ? slots : experts);

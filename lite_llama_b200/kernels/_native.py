@@ -18,9 +18,11 @@ _ABI = ("b2l_quant_gemm_workspace_bytes", "b2l_linear_workspace_bytes", "b2l_w8a
         "b2l_linear", "b2l_w8a8_gemm", "b2l_quantize_activations_int8", "b2l_skip_rmsnorm", "b2l_skip_rmsnorm_quant_int8",
         "b2l_swiglu", "b2l_kv_int4_row_bytes", "b2l_kv_int4_write", "b2l_kv_int4_read", "b2l_flash_decoding_int4_workspace_bytes",
         "b2l_flash_decoding_int4", "b2l_flash_attention_int4_workspace_bytes", "b2l_flash_attention_int4", "b2l_slot_maps",
-        "b2l_last_error")
+        "b2l_weights_written", "b2l_mxfp4_scale_bytes", "b2l_mxfp4_quantize", "b2l_mxfp4_dequantize", "b2l_skip_rmsnorm_mxfp4",
+        "b2l_mxfp4_matmul", "b2l_mxfp4_moe_tile_rows", "b2l_mxfp4_moe_max_tiles", "b2l_mxfp4_moe_sort", "b2l_mxfp4_moe_scatter",
+        "b2l_mxfp4_grouped_matmul", "b2l_mxfp4_moe_combine", "b2l_last_error")
 NAMES = ("w8a16", "w4a16_packed", "linear", "w8a8", "quantize", "norm", "norm_quant", "swiglu", "kv4_rope_write", "kv4_read",
-         "kv4_decode", "kv4_prompt", "slot_maps")
+         "kv4_decode", "kv4_prompt", "slot_maps", "mx4_quantize", "mx4_dequantize", "mx4_norm", "mx4_matmul", "mx4_moe")
 
 
 def _address(name: str) -> int:
@@ -47,7 +49,8 @@ def _table() -> dict:
 def _first(name: str):
     """Stands in for ``name`` until the first call on the GPU, which needs the library loaded in any case."""
     def call(*args):
-        if not args[0].is_cuda:
+        first = args[0] if isinstance(args[0], torch.Tensor) else args[0][0]      # an MXFP4 begins with its codes
+        if not first.is_cuda:
             return None
         table = _table()
         globals().update({n: table.get(n, _python) for n in NAMES})
@@ -56,4 +59,4 @@ def _first(name: str):
 
 
 (w8a16, w4a16_packed, linear, w8a8, quantize, norm, norm_quant, swiglu, kv4_rope_write, kv4_read, kv4_decode, kv4_prompt,
- slot_maps) = map(_first, NAMES)
+ slot_maps, mx4_quantize, mx4_dequantize, mx4_norm, mx4_matmul, mx4_moe) = map(_first, NAMES)

@@ -8,18 +8,18 @@ kernels: csrc/mxfp4.cuh, mxfp4_quant.cu, mxfp4_gemm.cu.
 from __future__ import annotations
 
 from contextlib import nullcontext
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
+from .. import _native
 from .._common import as_rows, check, current_device, dtype_code, float_code, index_width, lib, no_grad, ptr, require_cuda, stream_handle, weights_written
 
 BLOCK = 32          # elements that share a scale
 GATE_RUN = 64       # gate rows, then as many up rows
 
 
-@dataclass(frozen=True, eq=False)
-class MXFP4:
+class MXFP4(NamedTuple):
     """A matrix ``[..., rows, k]`` in the format (or a stack of them).
 
     ``codes`` uint8 ``[..., rows, k / 2]``, element 2i in the low half of byte i; ``scales`` uint8
@@ -91,11 +91,16 @@ def _check(q: MXFP4, what: str, dims: int | None = None) -> None:
         raise ValueError(f"{what}: codes and scales must be contiguous and start on 16 bytes")
 
 
-@no_grad
 def mxfp4_quantize(x: torch.Tensor) -> MXFP4:
     """``x [..., rows, k]`` (fp16, bf16 or fp32; k a multiple of 32) in the format.  A block's scale is the largest power of two not
     above its largest magnitude, over 4; elements are rounded to the nearest, ties to the even code, and end at 6 scales.  A block
     that holds an infinity or a NaN becomes NaN."""
+    out = _native.mx4_quantize(x)
+    return _mxfp4_quantize(x) if out is None else MXFP4(*out, False)
+
+
+@no_grad
+def _mxfp4_quantize(x: torch.Tensor) -> MXFP4:
     require_cuda(x)
     code = float_code(x, "x")
     if x.dim() < 2:
@@ -113,9 +118,16 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4:
     return MXFP4(codes, scales, ready=False)
 
 
-@no_grad
 def mxfp4_dequantize(q: MXFP4, dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """The values that ``q`` stands for, rounded to ``dtype`` (fp16, bf16 or fp32): ``[..., rows, k]``."""
+    y = _native.mx4_dequantize(q, dtype) if isinstance(q, MXFP4) else None
+    return _mxfp4_dequantize(q, dtype) if y is None else y
+
+
+@no_grad
+def _mxfp4_dequantize(q: MXFP4, dtype: torch.dtype) -> torch.Tensor:
+    if not isinstance(q, MXFP4):
+        raise ValueError(f"mxfp4_dequantize: q must be MXFP4, got {type(q).__name__}")
     _check(q, "mxfp4_dequantize")
     with _on(q.codes):
         y = torch.empty((*q.codes.shape[:-1], q.k), dtype=dtype, device=q.device)
@@ -157,7 +169,6 @@ def mxfp4_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return torch.stack((gate.unflatten(-2, (-1, GATE_RUN)), up.unflatten(-2, (-1, GATE_RUN))), -3).flatten(-4, -2)
 
 
-@no_grad
 def skip_rmsnorm_mxfp4(X: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-5, *,
                        out_residual: torch.Tensor | None = None) -> tuple[MXFP4, torch.Tensor]:
     """``(q, residual)``: ``residual += X`` in place (or into ``out_residual``), ``q`` the RMS norm of it times ``weight`` in the
@@ -165,6 +176,14 @@ def skip_rmsnorm_mxfp4(X: torch.Tensor, residual: torch.Tensor | None, weight: t
 
     The norm is not rounded to 16 bits before it is quantised (:func:`~lite_llama_b200.kernels.skip_rmsnorm` rounds twice), and
     decides borders as exact arithmetic does.  n: a multiple of 32, at most 16384."""
+    out = _native.mx4_norm(X, residual, weight, eps, out_residual)
+    if out is None:
+        return _skip_rmsnorm_mxfp4(X, residual, weight, eps, out_residual)
+    return MXFP4(*out, False), X if residual is None else residual if out_residual is None else out_residual
+
+
+@no_grad
+def _skip_rmsnorm_mxfp4(X, residual, weight, eps, out_residual) -> tuple[MXFP4, torch.Tensor]:
     _together("skip_rmsnorm_mxfp4", X, residual, weight, out_residual)
     n = X.shape[-1]
     code = dtype_code(X, "X")
@@ -192,7 +211,6 @@ def skip_rmsnorm_mxfp4(X: torch.Tensor, residual: torch.Tensor | None, weight: t
     return MXFP4(codes, scales, ready=False), X if total is None else total
 
 
-@no_grad
 def mxfp4_matmul(x: torch.Tensor | MXFP4, w: MXFP4, bias: torch.Tensor | None = None, *, swiglu: bool = False,
                  out_dtype: torch.dtype | None = None) -> torch.Tensor | MXFP4:
     """``x @ w.T (+ bias)`` with both operands in the format, sums in 32 bits.
@@ -201,6 +219,15 @@ def mxfp4_matmul(x: torch.Tensor | MXFP4, w: MXFP4, bias: torch.Tensor | None = 
     type.  The output is of ``x``'s type, for quantised ``x`` of ``out_dtype`` (default fp16).  ``swiglu``: the rows of ``w`` (and
     ``bias``) alternate as ``mxfp4_gate_up`` orders them, and ``silu(gate) * up`` comes back in the format, ``[rows, n / 2]``,
     quantised from the sums themselves."""
+    if isinstance(w, MXFP4) and isinstance(x, (torch.Tensor, MXFP4)):
+        y = _native.mx4_matmul(x, w, bias, swiglu, out_dtype)
+        if y is not None:
+            return MXFP4(*y, False) if swiglu else y
+    return _mxfp4_matmul(x, w, bias, swiglu, out_dtype)
+
+
+@no_grad
+def _mxfp4_matmul(x, w, bias, swiglu, out_dtype) -> torch.Tensor | MXFP4:
     if not isinstance(w, MXFP4):
         raise ValueError(f"mxfp4_matmul: w must be MXFP4, got {type(w).__name__}")
     _check(w, "mxfp4_matmul: w", 2)
@@ -209,6 +236,8 @@ def mxfp4_matmul(x: torch.Tensor | MXFP4, w: MXFP4, bias: torch.Tensor | None = 
         _check(x, "mxfp4_matmul: x", 2)
         dtype = out_dtype or (torch.float16 if bias is None else bias.dtype)
     else:
+        if not isinstance(x, torch.Tensor):
+            raise ValueError(f"mxfp4_matmul: x must be a tensor or MXFP4, got {type(x).__name__}")
         require_cuda(x)
         dtype_code(x, "x")
         if out_dtype not in (None, x.dtype):
@@ -246,13 +275,6 @@ def mxfp4_matmul(x: torch.Tensor | MXFP4, w: MXFP4, bias: torch.Tensor | None = 
     return y if lead is None or len(lead) == 1 else y.view(*lead, n)
 
 
-def _tile_rows(slots: int, experts: int) -> int:
-    """Rows of an expert's tile: the MMA's columns.  More than an expert's rows are copies of nothing, fewer read its weights again."""
-    per = slots / experts
-    return 32 if per <= 24 else (64 if per <= 48 else 128)
-
-
-@no_grad
 def fused_moe_mxfp4(hidden_states: torch.Tensor, w1: MXFP4, w2: MXFP4, topk_weights: torch.Tensor, topk_ids: torch.Tensor) -> torch.Tensor:
     """``sum_k w_k * (silu(x @ W1g.T) * (x @ W1u.T)) @ W2.T`` over the routed experts, both products with 4-bit operands.
 
@@ -260,6 +282,15 @@ def fused_moe_mxfp4(hidden_states: torch.Tensor, w1: MXFP4, w2: MXFP4, topk_weig
     ``[experts, h, inner]``; ``topk_weights`` (fp32 or the activations' type) and ``topk_ids`` (int32 or int64) ``[tokens, k]``.  Tokens are
     quantised once and sorted by expert, the activation is quantised from the first product's sums, a slot's output is
     rounded to 16 bits before it is weighted, and the weighted sum is held in 32 bits.  Ids that name no expert add nothing."""
+    if isinstance(w1, MXFP4) and isinstance(w2, MXFP4):
+        out = _native.mx4_moe(hidden_states, w1, w2, topk_weights, topk_ids)
+        if out is not None:
+            return out
+    return _fused_moe_mxfp4(hidden_states, w1, w2, topk_weights, topk_ids)
+
+
+@no_grad
+def _fused_moe_mxfp4(hidden_states, w1, w2, topk_weights, topk_ids) -> torch.Tensor:
     for w, what in ((w1, "w1"), (w2, "w2")):
         if not isinstance(w, MXFP4):
             raise ValueError(f"fused_moe_mxfp4: {what} must be MXFP4, got {type(w).__name__}")
@@ -286,7 +317,7 @@ def fused_moe_mxfp4(hidden_states: torch.Tensor, w1: MXFP4, w2: MXFP4, topk_weig
     x, ids, weights = _aligned(x), topk_ids.contiguous(), topk_weights.contiguous()
     with _on(x):
         L, dev, st = lib(), x.device, stream_handle()
-        tile = _tile_rows(slots, experts)
+        tile = L.b2l_mxfp4_moe_tile_rows(slots, experts)
         tiles = L.b2l_mxfp4_moe_max_tiles(slots, tile, experts)
         if not (w1.ready and w2.ready):
             weights_written()

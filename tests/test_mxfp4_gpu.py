@@ -149,7 +149,10 @@ def weights(n, k, spread=0.02):
 
 
 @pytest.mark.parametrize("t,n,k", ((1, 128, 64), (1, 128, 256), (3, 5, 32), (32, 256, 512), (33, 130, 96), (17, 384, 1120), (64, 200, 2048),
-                                   (65, 640, 992), (128, 129, 4096), (100, 1000, 352)))
+                                   (65, 640, 992), (128, 129, 4096), (100, 1000, 352),
+                                   # pairs: one tile, both widths, ragged edges, several tiles to a pair; what they leave (odd n)
+                                   (129, 8, 32), (256, 256, 256), (200, 264, 96), (385, 1000, 736), (300, 20488, 256), (1000, 9000, 1312),
+                                   (2048, 4096, 512), (140, 131, 256), (300, 33, 1024)))
 def test_products_of_whole_numbers_are_exact(t, n, k):
     """Elements and scales whose products add up to whole numbers below 2^11: any order of exact sums gives the same bits, and one
     element, scale, row or block in a wrong place gives others."""
@@ -167,7 +170,7 @@ def test_products_of_whole_numbers_are_exact(t, n, k):
 
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("t,n,k", ((1, 6144, 4096), (2, 896, 4864), (7, 4096, 14336), (31, 77, 3584), (40, 4608, 3584), (128, 1152, 896),
-                                   (5, 33, 32)))
+                                   (5, 33, 32), (777, 4608, 3584), (129, 896, 4864), (513, 9728, 896), (200, 77, 1024)))
 @pytest.mark.parametrize("with_bias", (False, True))
 def test_products_against_64_bits(dtype, t, n, k, with_bias):
     x = torch.randn(t, k, device="cuda").to(dtype)
@@ -215,7 +218,8 @@ def quantised_near(q, act, off):
 
 
 @pytest.mark.parametrize("dtype", HALVES)
-@pytest.mark.parametrize("t,inner,k", ((1, 64, 64), (3, 128, 96), (32, 192, 256), (20, 4864, 896), (50, 320, 1120), (100, 448, 512), (128, 64, 2048)))
+@pytest.mark.parametrize("t,inner,k", ((1, 64, 64), (3, 128, 96), (32, 192, 256), (20, 4864, 896), (50, 320, 1120), (100, 448, 512), (128, 64, 2048),
+                                        (129, 64, 64), (300, 320, 256), (260, 4864, 896), (1000, 5056, 352)))
 @pytest.mark.parametrize("with_bias", (False, True))
 def test_feed_forward_quantises_its_own_sums(dtype, t, inner, k, with_bias):
     x = torch.randn(t, k, device="cuda").to(dtype)
