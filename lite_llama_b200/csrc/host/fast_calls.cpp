@@ -699,6 +699,7 @@ PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
   if (!mx4(a[1], 2, w)) return none();
   const at::Tensor *x = plain(a[0]), *bias = a[2] == Py_None ? w.codes : plain(a[2]);
   if (!x && !mx4(a[0], 2, q)) return none();
+  if (!abi.mx4_quantize || !abi.mx4_scale_bytes) return none();      // of a library that holds another file's functions alone
   const int device = device_for(abi.mx4_matmul, {x ? x : q.codes, x ? x : q.scales, w.codes, w.scales, bias});
   if (device < 0 || (a[4] != Py_None && !THPDtype_Check(a[4])) || !PyBool_Check(a[3])) return none();
   const bool gated = a[3] == Py_True;
@@ -750,6 +751,7 @@ PyObject* mx4_moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
   Mx4 w1, w2;
   if (!mx4(a[1], 3, w1) || !mx4(a[2], 3, w2)) return none();
   const at::Tensor *x = plain(a[0]), *weights = plain(a[3]), *ids = plain(a[4]);
+  if (!abi.mx4_sort || !abi.mx4_scatter || !abi.mx4_combine || !abi.mx4_tile_rows || !abi.mx4_max_tiles || !abi.mx4_scale_bytes) return none();
   const int device = device_for(abi.mx4_grouped, {x, weights, ids, w1.codes, w1.scales, w2.codes, w2.scales});
   if (device < 0 || !mx4_rows(*x, false) || x->size(1) != w1.k) return none();
   const i64 tokens = x->size(0), hidden = w1.k, inner = w2.k, experts = w1.lead;

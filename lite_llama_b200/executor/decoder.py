@@ -23,17 +23,23 @@ import torch
 
 from ..distributed import divide, get_tp_rank, get_tp_world_size
 from ..kernels import (
+    MXFP4,
     flash_attention2_no_pad,
     flash_attention_int4,
     flash_decoding,
     flash_decoding_int4,
     fused_moe,
+    fused_moe_mxfp4,
     linear,
+    mxfp4_gate_up,
+    mxfp4_matmul,
+    mxfp4_quantize_weight,
     route_topk,
     rope_emb_inplace,
     rope_kv_write,
     rope_kv_write_int4,
     skip_rmsnorm,
+    skip_rmsnorm_mxfp4,
     swiglu_forward,
     update_kv_buffer,
 )
@@ -56,8 +62,8 @@ class MoeWeights:
     columns of EVERY expert (models/weights.py:129-130); the router is replicated and never quantised."""
 
     router: torch.Tensor                  # [E, hidden], activation dtype
-    w1: torch.Tensor                      # [E, 2 * I_local, hidden]  fp16 | uint8 (e4m3 bits)
-    w2: torch.Tensor                      # [E, hidden, I_local]
+    w1: torch.Tensor | MXFP4              # [E, 2 * I_local, hidden]  fp16 | uint8 (e4m3 bits) | 4-bit floats (rows in runs of 64)
+    w2: torch.Tensor | MXFP4              # [E, hidden, I_local]
     w1_scale: torch.Tensor | None = None  # fp32 [E, ceil(2 I_local / group_n), ceil(hidden / group_k)]
     w2_scale: torch.Tensor | None = None  # fp32 [E, ceil(hidden / group_n), ceil(I_local / group_k)]
     group_n: int = 0
@@ -65,9 +71,13 @@ class MoeWeights:
     top_k: int = 8
     norm_topk_prob: bool = True
 
+    @property
+    def num_experts(self) -> int:
+        return self.router.shape[0]
+
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.router, self.w1, self.w2, self.w1_scale, self.w2_scale)
-                   if t is not None)
+        return sum(t.nbytes() if isinstance(t, MXFP4) else t.numel() * t.element_size()
+                   for t in (self.router, self.w1, self.w2, self.w1_scale, self.w2_scale) if t is not None)
 
 
 @dataclass
@@ -108,7 +118,7 @@ class DecoderWeights:
         if not moe:
             return 0
         m = moe[0]
-        e = m.w1.shape[0]
+        e = m.num_experts
         return (m.nbytes() - m.router.numel() * m.router.element_size()) // e
 
 
@@ -122,6 +132,9 @@ def make_moe_weights(cfg: ModelConfig, router, gate, up, down, method: str, tp: 
     il = divide(inter, tp, "MoE intermediate")
     lo, hi = rank * il, (rank + 1) * il
     kw = dict(top_k=cfg.num_experts_per_tok, norm_topk_prob=cfg.norm_topk_prob)
+    if method == "mxfp4":
+        w1 = mxfp4_quantize_weight(mxfp4_gate_up(gate[:, lo:hi], up[:, lo:hi]).to(dtype))
+        return MoeWeights(router.to(dtype), w1, mxfp4_quantize_weight(down[:, :, lo:hi].to(dtype)), **kw)
     if method != "fp8":
         w1 = torch.cat([gate[:, lo:hi], up[:, lo:hi]], dim=1).to(dtype).contiguous()
         return MoeWeights(router.to(dtype), w1, down[:, :, lo:hi].to(dtype).contiguous(), **kw)
@@ -290,9 +303,9 @@ class Decoder:
             down = self._moe(hidden.view(tokens, -1), lw.moe)                           # qwen3_moe.py:102-111 (partial)
             return down.view(batch, seq_len, -1), residual
         gu, residual = self._norm_linear(o.view(batch, seq_len, -1), residual, lw.post_norm, lw.gate_up, eps, tokens)  # base.py:263-264
-        # W4A16: the activation already ran in the GEMM epilogue (row-interleaved gate|up), gu is [tokens, inter]
+        # W4A16, MXFP4: the activation already ran in the GEMM epilogue (row-interleaved gate|up), gu is [tokens, inter]
         act = gu if lw.gate_up.swiglu else swiglu_forward(gu[:, : self.inter], gu[:, self.inter :])
-        down = apply_linear(act, lw.down)                                               # partial: reduced by the next norm
+        down = apply_linear(act, lw.down, out_dtype=o.dtype)                            # partial: reduced by the next norm
         return down.view(batch, seq_len, -1), residual
 
     @staticmethod
@@ -306,6 +319,9 @@ class Decoder:
                 and hidden.dtype == torch.float16):
             q, s, residual = skip_rmsnorm_quant_int8(hidden, residual, norm_weight, eps)
             return smoothquant_matmul_prequant(q, s, w.qweight, w.scales, bias=w.bias, out_dtype=hidden.dtype), residual
+        if w.method == "mxfp4" and (residual is None or get_tp_world_size() <= 1) and n <= 16384:
+            q, residual = skip_rmsnorm_mxfp4(hidden, residual, norm_weight, eps)
+            return mxfp4_matmul(q, w.mx4, w.bias, swiglu=w.swiglu, out_dtype=hidden.dtype), residual
         if residual is None:
             hidden, residual = skip_rmsnorm(hidden, residual, norm_weight, eps)
         else:
@@ -319,6 +335,8 @@ class Decoder:
         dimension; its all-reduce (qwen3_moe.py:110) is fused into the next norm like the dense MLP's."""
         logits = linear(x, m.router)
         weights, ids = route_topk(logits, m.top_k, m.norm_topk_prob)
+        if isinstance(m.w1, MXFP4):
+            return fused_moe_mxfp4(x, m.w1, m.w2, weights, ids)
         return fused_moe(x, m.w1, m.w2, weights, ids, w1_scale=m.w1_scale, w2_scale=m.w2_scale,
                          group_n=m.group_n, group_k=m.group_k)
 

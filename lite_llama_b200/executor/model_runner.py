@@ -475,7 +475,7 @@ class ModelRunner:
               kv_group_size: int | None = None) -> "ModelRunner":
         """``model`` is a preset name (see ``PRESETS``) or a ModelConfig; ``quantization`` one of
         ``None | "int4" | "int8" | "fp8" | "smoothquant"`` (the reference's ``--quantization`` values,
-        models/quantization/config.py:39-54), of the weights; ``kv_cache_dtype`` and ``kv_group_size`` as in ``__init__``."""
+        models/quantization/config.py:39-54) or ``"mxfp4"``, of the weights (mxfp4: and of the activations in front of them); ``kv_cache_dtype`` and ``kv_group_size`` as in ``__init__``."""
         cfg = PRESETS[model] if isinstance(model, str) else model
         cfg = cfg.with_(max_seq_len=max_seq_len)
         if num_layers is not None:

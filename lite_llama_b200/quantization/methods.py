@@ -2,7 +2,8 @@
 
 Mirrors the reference's strategy registry (lite_llama/models/quantization/methods/__init__.py:21-63):
 ``fp16`` -> dense GEMM (unquantized.py:21-22), ``int4`` -> w4a16 (w4a16.py:15-43), ``int8`` / ``fp8``
--> w8a16 (w8a16.py:37-112), ``smoothquant`` -> w8a8 (w8a8.py:15-37).
+-> w8a16 (w8a16.py:37-112), ``smoothquant`` -> w8a8 (w8a8.py:15-37); and ``mxfp4``, weights and activations in microscaled
+4-bit floating point, which the reference has not.
 """
 
 from __future__ import annotations
@@ -12,11 +13,11 @@ from dataclasses import dataclass
 
 import torch
 
-from ..kernels import PackedW4, linear, smoothquant_matmul, w4a16_matmul, w4a16_matmul_packed, w4a16_pack, w8a16_matmul
+from ..kernels import MXFP4, PackedW4, linear, mxfp4_gate_up, mxfp4_matmul, mxfp4_quantize_weight, smoothquant_matmul, w4a16_matmul, w4a16_matmul_packed, w4a16_pack, w8a16_matmul
 from ..kernels.quantization import interleave_gate_up
 from .params import quantize_fp8_per_channel, quantize_int4_groupwise, quantize_int8_per_channel
 
-LINEAR_METHODS = ("fp16", "int4", "int8", "fp8", "smoothquant")
+LINEAR_METHODS = ("fp16", "int4", "int8", "fp8", "smoothquant", "mxfp4")
 
 
 @dataclass
@@ -34,6 +35,7 @@ class LinearWeights:
     group_size: int = 128
     packed: PackedW4 | None = None          # int4: kernel-native repack (replaces qweight/scales/zeros)
     swiglu: bool = False                    # gate|up projection stored row-interleaved: the GEMM applies silu(gate) * up
+    mx4: MXFP4 | None = None
 
     def nbytes(self) -> int:
         total = 0
@@ -42,6 +44,8 @@ class LinearWeights:
                 total += t.numel() * t.element_size()
         if self.packed is not None:
             total += self.packed.nbytes()
+        if self.mx4 is not None:
+            total += self.mx4.nbytes()
         return total
 
 
@@ -70,11 +74,19 @@ def make_linear_weights(weight: torch.Tensor, method: str, bias: torch.Tensor | 
     if method == "fp8":
         q, s = quantize_fp8_per_channel(weight)
         return LinearWeights(method, n, k, qweight=q, scales=s, bias=bias)
+    if method == "mxfp4":
+        # [gate | up] rows in runs of 64: the GEMM applies the activation and quantises it for the next one
+        fuse = fuse_swiglu and n % 128 == 0
+        if fuse:
+            weight = mxfp4_gate_up(weight[:n // 2], weight[n // 2:])
+            bias = mxfp4_gate_up(bias[:n // 2, None], bias[n // 2:, None]).flatten() if bias is not None else None
+        return LinearWeights(method, n, k, bias=bias, swiglu=fuse, mx4=mxfp4_quantize_weight(weight))
     raise ValueError(f"unknown linear method {method!r}; expected one of {LINEAR_METHODS}")
 
 
-def apply_linear(x: torch.Tensor, w: LinearWeights) -> torch.Tensor:
-    """``x @ W.T (+ bias)`` through the GEMM that matches ``w.method``."""
+def apply_linear(x: torch.Tensor | MXFP4, w: LinearWeights, out_dtype: torch.dtype | None = None) -> torch.Tensor | MXFP4:
+    """``x @ W.T (+ bias)`` through the GEMM that matches ``w.method``; with ``w.swiglu`` the activation of the two halves (for
+    ``mxfp4`` in that format, which it also takes: the result is of ``out_dtype`` then)."""
     if w.method == "fp16":
         return linear(x, w.weight, w.bias)
     if w.method == "int4":
@@ -85,4 +97,6 @@ def apply_linear(x: torch.Tensor, w: LinearWeights) -> torch.Tensor:
         return w8a16_matmul(x, w.qweight, w.scales, group_n=1, group_k=w.in_features, bias=w.bias)
     if w.method == "smoothquant":
         return smoothquant_matmul(x, w.qweight, w.scales, bias=w.bias)
+    if w.method == "mxfp4":
+        return mxfp4_matmul(x, w.mx4, w.bias, swiglu=w.swiglu, out_dtype=out_dtype)
     raise ValueError(f"unknown linear method {w.method!r}")
