@@ -91,6 +91,24 @@ __device__ __forceinline__ uint32_t word_of(uint32_t byte, int lane) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// A lane's eight of a block's 32 values (four neighbouring lanes; the whole warp takes part): the codes, and the block's scale byte.
+__device__ __forceinline__ uint32_t quantise8(float (&v)[8], uint32_t& byte) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+  byte = scale_byte(block_max(m));
+  const float inv = inverse_scale(byte);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] *= inv;
+  const uint32_t c = codes8(v);
+  return byte == 255u ? 0u : c;
+}
+
+__device__ __forceinline__ uint32_t ld_once(const uint8_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
 // eight consecutive elements in 32 bits
 template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
   const uint4 q = ldg_stream_128(p);

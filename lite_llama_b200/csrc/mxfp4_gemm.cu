@@ -301,15 +301,18 @@ static int stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w
 // The same product for routed experts: tiles of up to BT rows of one expert, {expert, rows} in a table on the device
 // (mxfp4_moe.cu), row r of tile i in row i BT + r of x and y and in row 128 i + r of their scales.
 //
+// Tiles of 32 or 64 rows; those of 128 are multiplied with the rows as the MMA's (mxfp4_gemm_pair.cu), where a thread holds a row's
+// outputs: here its lane is an output, and bringing 128 columns out through shared memory took longer than the products (2000 tokens,
+// 128 experts of 2048 x 768, both products 137 us -> see there).
 // Bound: the experts' weights, each read from memory once (further tiles of an expert find them in L2).  Persistent, one CTA to
 // an SM with 180 KiB of copies in flight, the accumulator in two buffers: a tile's end overlaps the next one's products.
 // ---------------------------------------------------------------------------------------------------------------
 template <int BT> struct GroupedRing {
   static constexpr int kStage = 16384 + kSfBytes + BT * 128 + kSfBytes;
   static constexpr int kX = 16384 + kSfBytes;
-  static constexpr int kStages = BT == 32 ? 8 : (BT == 64 ? 7 : 5);
+  static constexpr int kStages = BT == 32 ? 8 : 7;
   static constexpr int kCols = 2 * BT + kStages * 16;
-  static constexpr int kAlloc = kCols <= 256 ? 256 : 512;
+  static constexpr int kAlloc = 256;
   static constexpr int kOut = 32 * 128 * 4;
   static constexpr int kSmem = 1024 + 1024 + kStages * kStage + kOut;
 };
@@ -526,7 +529,7 @@ static int grouped_gemm(const void* x, const void* w, const GroupedParams& p, in
   rc = b2l_make_tmap_2d(&tw, w, TMA_U8, (uint64_t)experts * p.N, (uint64_t)p.K / 2, (uint64_t)p.K / 2, 128, 128, true);
   if (rc != B2L_OK) return rc;
 #define GROUPED(BT) (is_gated ? launch_grouped<T, BT, true>(tx, tw, p, max_tiles, st) : launch_grouped<T, BT, false>(tx, tw, p, max_tiles, st))
-  return tile_rows == 32 ? GROUPED(32) : (tile_rows == 64 ? GROUPED(64) : GROUPED(128));
+  return tile_rows == 32 ? GROUPED(32) : GROUPED(64);
 #undef GROUPED
 }
 
@@ -564,7 +567,8 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
                                         const void* w_scales, const void* table, int64_t max_tiles, int tile_rows, int experts,
                                         int64_t n, int64_t k, int gated, int dtype, void* stream) {
   B2L_REQUIRE(max_tiles >= 0 && experts > 0 && n > 0 && k > 0 && k % 32 == 0 && k < (1ll << 30) && n * experts < (1ll << 31) &&
-                  max_tiles * cdiv64(n, 128) < (1ll << 31) && max_tiles * 128 < (1ll << 31),
+                  max_tiles * cdiv64(n, 128) < (1ll << 31) && max_tiles * 128 < (1ll << 31) &&
+                  (experts * cdiv64(n, 128) + max_tiles) * mx4::k_tiles(k) < (1ll << 29),
               "mxfp4_grouped_matmul: experts=%d n=%lld k=%lld (a multiple of 32) tiles=%lld", experts, (long long)n, (long long)k, (long long)max_tiles);
   B2L_REQUIRE(tile_rows == 32 || tile_rows == 64 || tile_rows == 128, "mxfp4_grouped_matmul: tiles of %d rows", tile_rows);
   if (max_tiles == 0) return B2L_OK;
@@ -572,6 +576,14 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
   B2L_REQUIRE(!gated || n % 128 == 0, "mxfp4_grouped_matmul: gate and up rows come in runs of 64 (n=%lld)", (long long)n);
   B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales) % 16 == 0 && (uintptr_t)y % 8 == 0,
               "mxfp4_grouped_matmul: rows of codes must start on 16 bytes");
+  B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "mxfp4_grouped_matmul: dtype %d", dtype);
+  cudaStream_t st = (cudaStream_t)stream;
+  mx4::PairCall g = {y, gated ? n / 4 : n, y_scales, nullptr, x, x_scales, w, w_scales, max_tiles, n, k, k / 2, k / 2, gated != 0};
+  if (tile_rows == 128) {
+    B2L_REQUIRE(gated || (n % 8 == 0 && (uintptr_t)y % 16 == 0), "mxfp4_grouped_matmul: tiles of 128 rows are written in units of 8 outputs (n=%lld)", (long long)n);
+    B2L_REQUIRE(!gated || (uintptr_t)y % 16 == 0, "mxfp4_grouped_matmul: rows of codes must start on 16 bytes");
+    return mx4::rows_gemm(g, table, experts, dtype, st);
+  }
   mx4::GroupedParams p;
   p.y = y; p.ldy = gated ? n / 4 : n;
   p.y_scales = (uint8_t*)y_scales; p.y_ktiles = mx4::k_tiles(n / 2);
@@ -580,8 +592,6 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
   p.ktiles = mx4::k_tiles(k);
   p.N = (int)n; p.K = (int)k; p.num_kb = (int)cdiv64(k, mx4::kStageK); p.n_tiles = (int)cdiv64(n, 128);
   p.vec = n % 4 == 0;
-  cudaStream_t st = (cudaStream_t)stream;
   if (dtype == B2L_F16) return mx4::grouped_gemm<__half>(x, w, p, max_tiles, tile_rows, experts, gated != 0, st);
-  if (dtype == B2L_BF16) return mx4::grouped_gemm<__nv_bfloat16>(x, w, p, max_tiles, tile_rows, experts, gated != 0, st);
-  B2L_UNSUPPORTED("mxfp4_grouped_matmul: dtype %d", dtype);
+  return mx4::grouped_gemm<__nv_bfloat16>(x, w, p, max_tiles, tile_rows, experts, gated != 0, st);
 }

@@ -9,6 +9,8 @@
 //     start when a quarter of the tile before has been read, and the rest is written out under them;
 //   * scales are TMA copies of whole tiles into every stage; both CTAs hold those of all 256 outputs.  Two sets of 24 columns take turns:
 //     a set is written again when the MMAs of two stages ago have retired.
+// The same kernel on single CTAs (CTAS = 1) multiplies the rows of routed experts: tiles of up to 128 rows of one expert, from a table on
+// the device, by 256 of its weight rows (a pair's 256 tokens would be half empty).
 #include "gemm_tc.cuh"
 #include "mxfp4_mma.cuh"
 #include "mxfp4_gemm.cuh"
@@ -17,15 +19,15 @@
 namespace mx4 {
 
 constexpr int kPairThreads = 6 * 32;   // TMA producer, MMA issuer, four warps that read the accumulator
-constexpr int kPairStages = 5;
 constexpr int kPairRows = 128;         // tokens per CTA
 constexpr int kPairBand = 16;          // token tiles per band: 16 x 256 rows x 4096 / 2 bytes = 8 MiB of L2
 
-template <int BN> struct PairRing {
-  static constexpr int kX = 16384, kW = BN / 2 * 128;
+template <int BN, int CTAS> struct PairRing {
+  static constexpr int kStages = CTAS == 2 ? 5 : 4, kBoxes = CTAS == 2 ? 2 : 1;      // boxes of 32 rows x 64 outputs on their way out, per warp
+  static constexpr int kX = 16384, kW = BN / CTAS * 128;
   static constexpr int kXs = kX + kW, kWs = kXs + kSfBytes;
   static constexpr int kBytes = kWs + BN / 128 * kSfBytes;
-  static constexpr int kSmem = 1024 + 1024 + kPairStages * kBytes + 4 * 2 * 4096;
+  static constexpr int kSmem = 1024 + 1024 + kStages * kBytes + 4 * kBoxes * 4096;
   static constexpr int kAcc1 = BN == 256 ? 208 : 128;                     // first column of the second accumulator
   static constexpr int kSf = BN == 256 ? 464 : 256;
   static constexpr int kSfSet = 8 + BN / 128 * 8;
@@ -34,14 +36,15 @@ template <int BN> struct PairRing {
 struct PairParams {
   const void* bias;
   uint8_t* y; uint8_t* y_scales; int64_t ldy, y_ktiles;                   // gated: codes and scales
+  const int32_t* table;                // experts: tiles, then {expert, rows} of each
   int T, N, K, num_kb, m_tiles, n_tiles, ktiles;
 };
 
 struct __align__(8) PairControl {
-  uint64_t full[kPairStages];          // leader: both CTAs' operands and scales of a stage have landed
-  uint64_t empty[kPairStages];         // both: the MMAs of a stage have retired
+  uint64_t full[5];                    // leader: both CTAs' operands and scales of a stage have landed
+  uint64_t empty[5];                   // both: the MMAs of a stage have retired
   uint64_t acc_full[2];                // both: a tile's accumulator is complete
-  uint64_t freed[2];                   // leader: all eight warps have read what the next tile's products overwrite
+  uint64_t freed[2];                   // leader: all warps have read what the next tile's products overwrite
   uint32_t tmem;
 };
 
@@ -61,74 +64,106 @@ __device__ __forceinline__ uint32_t quantise32(float (&v)[32], uint4& codes) {
   return byte;
 }
 
-template <typename T, int BN, bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+// What differs between a pair and a single CTA
+template <int CTAS> __device__ __forceinline__ void sync_all() {
+  if (CTAS == 2) pair_sync();
+  else __syncthreads();
+}
+template <int CTAS> __device__ __forceinline__ void load_2d(void* dst, const void* map, int c0, int c1, uint64_t* bar) {
+  if (CTAS == 2) tma_load_2d_pair(dst, map, c0, c1, leader_addr(bar), kEvictNormal);
+  else tma_load_2d_hint(dst, map, c0, c1, bar, kEvictNormal);
+}
+template <int CTAS> __device__ __forceinline__ void commit(uint64_t* bar) {
+  if (CTAS == 2) tc_commit_pair(bar);
+  else tc_commit(bar);
+}
+// A tile of outputs: token tile (index of 128 rows for each CTA), output tile, rows that hold anything, expert
+struct Work { int m, n, rows, expert; };
+template <int CTAS> __device__ __forceinline__ Work work_of(const PairParams& p, int t, int rank) {
+  Work o;
+  if (CTAS == 2) {
+    const PairTile pt = pair_tile(t, p.m_tiles, p.n_tiles, kPairBand);
+    o.m = pt.m * 2 + rank;
+    o.n = pt.n;
+    o.rows = p.T - o.m * kPairRows;
+    o.expert = 0;
+  } else {
+    o.m = t / p.n_tiles;
+    o.n = t - o.m * p.n_tiles;
+    o.expert = ld_upstream(p.table + 1 + 2 * o.m);
+    o.rows = ld_upstream(p.table + 2 + 2 * o.m);
+  }
+  return o;
+}
+
+template <typename T, int BN, bool GATED, int CTAS>
+__global__ void __launch_bounds__(kPairThreads, 1)
 pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_xs,
             const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_y, const PairParams p) {
-  using R = PairRing<BN>;
+  using R = PairRing<BN, CTAS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   PairControl* ctl = reinterpret_cast<PairControl*>(smem);
   uint8_t* ring = smem + 1024;
-  uint8_t* out_stage = ring + kPairStages * R::kBytes;
+  uint8_t* out_stage = ring + R::kStages * R::kBytes;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = pair_rank();
-  const int pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
-  const int tiles = p.m_tiles * p.n_tiles;
+  const uint32_t rank = CTAS == 2 ? pair_rank() : 0u;
+  const int pairs = gridDim.x / CTAS, pair = blockIdx.x / CTAS;
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmap_x);
     tma_prefetch_desc(&tmap_w);
     tma_prefetch_desc(&tmap_xs);
     tma_prefetch_desc(&tmap_ws);
     if (!GATED) tma_prefetch_desc(&tmap_y);
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < R::kStages; ++s) {
       mbar_init(&ctl->full[s], 1);
       mbar_init(&ctl->empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&ctl->acc_full[b], 1);
-      mbar_init(&ctl->freed[b], 8);
+      mbar_init(&ctl->freed[b], 4 * CTAS);
     }
     mbar_fence_init();
   }
   if (warp == 1) {
-    tmem_alloc_pair(&ctl->tmem, 512);
-    tmem_relinquish_pair();
+    if (CTAS == 2) { tmem_alloc_pair(&ctl->tmem, 512); tmem_relinquish_pair(); }
+    else { tmem_alloc(&ctl->tmem, 512); tmem_relinquish(); }
     pdl_launch_dependents();           // after the allocation (gemm_dense.cu)
   }
   tc_fence_before();
-  pair_sync();
+  sync_all<CTAS>();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
+  if (CTAS == 1) pdl_wait_prior();     // the table is upstream data
+  const int tiles = (CTAS == 2 ? p.m_tiles : ld_upstream(p.table)) * p.n_tiles;
 
   if (warp == 0) {
     // ===================== TMA producer: this CTA's halves of both operands, its tokens' scales, all outputs' scales =====================
     pdl_wait_prior();
-    gemm::PipeState ps(kPairStages);
+    gemm::PipeState ps(R::kStages);
     for (int t = pair; t < tiles; t += pairs) {
-      const PairTile pt = pair_tile(t, p.m_tiles, p.n_tiles, kPairBand);
-      const int row_x = (pt.m * 2 + (int)rank) * kPairRows, row_w = pt.n * BN + (int)rank * (BN / 2);
-      const int xs = (pt.m * 2 + (int)rank) * p.ktiles * 4, ws = pt.n * (BN / 128) * p.ktiles * 4;      // rows of 128 bytes
+      const Work wk = work_of<CTAS>(p, t, (int)rank);
+      const int row_x = wk.m * kPairRows, row_w = wk.expert * p.N + wk.n * BN + (int)rank * (BN / CTAS);
+      const int xs = wk.m * p.ktiles * 4, ws = (wk.expert * ((p.N + 127) / 128) + wk.n * (BN / 128)) * p.ktiles * 4;      // rows of 128 bytes
       for (int kb = 0; kb < p.num_kb; ++kb) {
         mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
         if (elect_one()) {
-          if (rank == 0) mbar_arrive_expect_tx(&ctl->full[ps.stage], 2 * R::kBytes);
+          if (rank == 0) mbar_arrive_expect_tx(&ctl->full[ps.stage], CTAS * R::kBytes);
           uint8_t* st = ring + (size_t)ps.stage * R::kBytes;
-          const uint32_t bar = leader_addr(&ctl->full[ps.stage]);
-          tma_load_2d_pair(st, &tmap_x, kb * 128, row_x, bar, kEvictNormal);
-          tma_load_2d_pair(st + R::kX, &tmap_w, kb * 128, row_w, bar, kEvictNormal);
-          tma_load_2d_pair(st + R::kXs, &tmap_xs, 0, xs + kb * 8, bar, kEvictNormal);
+          uint64_t* bar = &ctl->full[ps.stage];
+          load_2d<CTAS>(st, &tmap_x, kb * 128, row_x, bar);
+          load_2d<CTAS>(st + R::kX, &tmap_w, kb * 128, row_w, bar);
+          load_2d<CTAS>(st + R::kXs, &tmap_xs, 0, xs + kb * 8, bar);
 #pragma unroll
-          for (int h = 0; h < BN / 128; ++h)
-            tma_load_2d_pair(st + R::kWs + h * kSfBytes, &tmap_ws, 0, ws + h * p.ktiles * 4 + kb * 8, bar, kEvictNormal);
+          for (int h = 0; h < BN / 128; ++h) load_2d<CTAS>(st + R::kWs + h * kSfBytes, &tmap_ws, 0, ws + h * p.ktiles * 4 + kb * 8, bar);
         }
         __syncwarp();
         ps.advance();
       }
     }
     // every stage handed back: no commit is still on its way to this CTA's barriers when it leaves
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < R::kStages; ++s) {
       mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
       ps.advance();
     }
@@ -136,7 +171,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     // ===================== MMA issuer (leader only) =====================
     if (rank == 0) {
       const uint64_t desc0 = umma_desc_sw128_kmajor(smem_u32(ring)), sf0 = scale_desc(smem_u32(ring));
-      gemm::PipeState ps(kPairStages), back(kPairStages);      // back: the stage two before
+      gemm::PipeState ps(R::kStages), back(R::kStages);      // back: the stage two before
       int it = 0, i = 0;
       for (int t = pair; t < tiles; t += pairs, ++it) {
         const uint32_t acc = tmem + (it & 1) * R::kAcc1;
@@ -162,17 +197,17 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
 #pragma unroll
             for (int j = 0; j < 2; ++j)
               if (2 * j < steps) {
-                copy_scales<2>(sfa + 4 * j, xsf + j * (kTileBytes >> 4));
+                copy_scales<CTAS>(sfa + 4 * j, xsf + j * (kTileBytes >> 4));
 #pragma unroll
                 for (int h = 0; h < BN / 128; ++h)
-                  copy_scales<2>(sfb + j * (BN / 32) + 4 * h, wsf + h * (kSfBytes >> 4) + j * (kTileBytes >> 4));
+                  copy_scales<CTAS>(sfb + j * (BN / 32) + 4 * h, wsf + h * (kSfBytes >> 4) + j * (kTileBytes >> 4));
               }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               if (j < steps)
-                mma<2>(acc, xd + 2 * j, wd + 2 * j, idesc(256, BN, j & 1), sfa + (j >> 1) * 4, sfb + (j >> 1) * (BN / 32), kb | j ? 1u : 0u);
-            tc_commit_pair(&ctl->empty[ps.stage]);
-            if (kb + 1 == p.num_kb) tc_commit_pair(&ctl->acc_full[it & 1]);
+                mma<CTAS>(acc, xd + 2 * j, wd + 2 * j, idesc(128 * CTAS, BN, j & 1), sfa + (j >> 1) * 4, sfb + (j >> 1) * (BN / 32), kb | j ? 1u : 0u);
+            commit<CTAS>(&ctl->empty[ps.stage]);
+            if (kb + 1 == p.num_kb) commit<CTAS>(&ctl->acc_full[it & 1]);
           }
           __syncwarp();
           ps.advance();
@@ -182,18 +217,20 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
   } else {
     // ===================== one thread per token =====================
     const int quad = warp & 3;
-    const uint32_t freed0 = leader_addr(&ctl->freed[0]), freed1 = leader_addr(&ctl->freed[1]);
     auto hand_on = [&](int buf) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(buf ? freed1 : freed0);
+      if (lane == 0) {
+        if (CTAS == 2) mbar_arrive_cluster(leader_addr(&ctl->freed[buf]));
+        else mbar_arrive(&ctl->freed[buf]);
+      }
     };
     pdl_wait_prior();                  // y may still be read upstream
     int it = 0, box = 0;
     for (int t = pair; t < tiles; t += pairs, ++it) {
-      const PairTile pt = pair_tile(t, p.m_tiles, p.n_tiles, kPairBand);
-      const int buf = it & 1;
-      const int m_warp = (pt.m * 2 + (int)rank) * kPairRows + quad * 32;
+      const Work wk = work_of<CTAS>(p, t, (int)rank);
+      const int buf = it & 1, m_warp = wk.m * kPairRows + quad * 32;
+      const bool any = quad * 32 < wk.rows;             // uniform over the warp
       const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * R::kAcc1;
       mbar_wait(&ctl->acc_full[buf], (it >> 1) & 1);
       tc_fence_after();
@@ -207,10 +244,10 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           tmem_ld_32x32b_x32(acc + c + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
           tc_wait_ld();
           if (j == (BN == 256 ? 0 : BN / 64 - 1)) hand_on(buf);
-          const int n0 = pt.n * BN + c;
-          if (n0 >= p.N || m_warp >= p.T) continue;     // uniform over the warp
-          uint8_t* dst = out_stage + (quad * 2 + (box & 1)) * 4096;
-          if (lane == 0) bulk_wait_read<1>();           // the store that used this box two boxes ago has read it
+          const int n0 = wk.n * BN + c;
+          if (n0 >= p.N || !any) continue;
+          uint8_t* dst = out_stage + (quad * R::kBoxes + box % R::kBoxes) * 4096;
+          if (lane == 0) bulk_wait_read<R::kBoxes - 1>();      // the store that used this box before has read it
           __syncwarp();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
@@ -244,7 +281,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           tmem_ld_32x32b_x32(acc + c + (back ? 96 : 32), *reinterpret_cast<uint32_t(*)[32]>(held + 32));
           tc_wait_ld();
           if (BN == 256 && j == 0) hand_on(buf);
-          const int n0 = pt.n * BN + c;
+          const int n0 = wk.n * BN + c;
           uint32_t bytes = 0;
           uint4 codes[2];
 #pragma unroll
@@ -265,8 +302,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
             }
             bytes |= quantise32(v, codes[h]) << (8 * h);
           }
-          if (n0 < p.N && row < p.T) {                  // N is a multiple of 128
-            uint8_t* y = p.y + row * p.ldy + n0 / 4;
+          if (n0 < p.N && quad * 32 + lane < wk.rows) {                  // N is a multiple of 128
+            uint8_t* y = p.y + (int64_t)row * p.ldy + n0 / 4;
             stg_128(y, codes[0]);
             stg_128(y + 16, codes[1]);
             const int k = n0 / 2;                       // first activation: a multiple of 64
@@ -281,37 +318,63 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
   }
 
   tc_fence_before();
-  pair_sync();                         // the peer's MMAs, commits and arrivals are over
-  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+  sync_all<CTAS>();                    // the peer's MMAs, commits and arrivals are over
+  if (warp == 1) {
+    if (CTAS == 2) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
+  }
+}
+
+// Maps and launch, for `rows` rows of x and y in tiles of 128 and `weight_rows` rows of w
+template <typename T, int BN, bool GATED, int CTAS>
+static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t experts, int64_t tiles, cudaStream_t st) {
+  using R = PairRing<BN, CTAS>;
+  const int sms = b2l_num_sms();
+  p.bias = g.bias;
+  p.y = (uint8_t*)g.y; p.y_scales = (uint8_t*)g.y_scales; p.ldy = g.ldy; p.y_ktiles = k_tiles(g.N / 2);
+  p.N = (int)g.N; p.K = (int)g.K; p.num_kb = (int)cdiv64(g.K, kStageK); p.ktiles = (int)k_tiles(g.K);
+  p.n_tiles = (int)cdiv64(g.N, BN);
+  tiles *= p.n_tiles;
+  const int grid = CTAS * (int)(tiles < sms / CTAS ? tiles : sms / CTAS);
+  CUtensorMap tx, tw, txs, tws, ty;
+  int rc = b2l_make_tmap_2d(&tx, g.x, TMA_U8, (uint64_t)rows, (uint64_t)g.K / 2, (uint64_t)g.ldx, kPairRows, 128, true);
+  if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tw, g.w, TMA_U8, (uint64_t)(experts * g.N), (uint64_t)g.K / 2, (uint64_t)g.ldw, BN / CTAS, 128, true);
+  if (rc == B2L_OK) rc = b2l_make_tmap_2d(&txs, g.x_scales, TMA_U8, (uint64_t)(cdiv64(rows, 128) * p.ktiles * 4), 128, 128, 8, 128, false);
+  if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tws, g.w_scales, TMA_U8, (uint64_t)(experts * cdiv64(g.N, 128) * p.ktiles * 4), 128, 128, 8, 128, false);
+  if (rc == B2L_OK && !GATED)
+    rc = b2l_make_tmap_2d(&ty, g.y, std::is_same<T, __half>::value ? TMA_F16 : TMA_BF16, (uint64_t)rows, (uint64_t)g.N, (uint64_t)g.ldy * 2, 32, 64, true);
+  if (rc != B2L_OK) return rc;
+  if (GATED) ty = tx;
+  auto kern = pair_kernel<T, BN, GATED, CTAS>;
+  static int configured[64] = {0};
+  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, R::kSmem, configured));
+  b2l_hang_arm(st);
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = R::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CTAS;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = b2l_pdl_enabled() ? 2 : 1;
+  B2L_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tx, tw, txs, tws, ty, p));
+  B2L_LAUNCH_CHECK();
+  return B2L_OK;
 }
 
 template <typename T, int BN, bool GATED>
 static int launch_pair(const PairCall& g, cudaStream_t st) {
-  using R = PairRing<BN>;
-  const int pairs = b2l_num_sms() / 2;
   PairParams p;
-  p.bias = g.bias;
-  p.y = (uint8_t*)g.y; p.y_scales = (uint8_t*)g.y_scales; p.ldy = g.ldy; p.y_ktiles = k_tiles(g.N / 2);
-  p.T = (int)g.T; p.N = (int)g.N; p.K = (int)g.K; p.num_kb = (int)cdiv64(g.K, kStageK); p.ktiles = (int)k_tiles(g.K);
+  p.table = nullptr;
+  p.T = (int)g.T;
   p.m_tiles = (int)cdiv64(g.T, 2 * kPairRows);
-  p.n_tiles = (int)cdiv64(g.N, BN);
-  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-  const int grid = 2 * (int)(tiles < pairs ? tiles : pairs);
-  CUtensorMap tx, tw, txs, tws, ty;
-  int rc = b2l_make_tmap_2d(&tx, g.x, TMA_U8, (uint64_t)g.T, (uint64_t)g.K / 2, (uint64_t)g.ldx, kPairRows, 128, true);
-  if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tw, g.w, TMA_U8, (uint64_t)g.N, (uint64_t)g.K / 2, (uint64_t)g.ldw, BN / 2, 128, true);
-  if (rc == B2L_OK) rc = b2l_make_tmap_2d(&txs, g.x_scales, TMA_U8, (uint64_t)(cdiv64(g.T, 128) * p.ktiles * 4), 128, 128, 8, 128, false);
-  if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tws, g.w_scales, TMA_U8, (uint64_t)(cdiv64(g.N, 128) * p.ktiles * 4), 128, 128, 8, 128, false);
-  if (rc == B2L_OK && !GATED)
-    rc = b2l_make_tmap_2d(&ty, g.y, std::is_same<T, __half>::value ? TMA_F16 : TMA_BF16, (uint64_t)g.T, (uint64_t)g.N, (uint64_t)g.ldy * 2, 32, 64, true);
-  if (rc != B2L_OK) return rc;
-  if (GATED) ty = tx;
-  auto kern = pair_kernel<T, BN, GATED>;
-  static int configured[64] = {0};
-  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, R::kSmem, configured));
-  b2l_launch(kern, dim3((unsigned)grid), dim3(kPairThreads), (size_t)R::kSmem, st, tx, tw, txs, tws, ty, p);
-  B2L_LAUNCH_CHECK();
-  return B2L_OK;
+  return launch_rows<T, BN, GATED, 2>(g, p, g.T, 1, p.m_tiles, st);
 }
 
 bool pair_wanted(const PairCall& g) {
@@ -330,6 +393,17 @@ int pair_gemm(const PairCall& g, int dtype, cudaStream_t st) {
   if (dtype == B2L_F16) return PAIR(__half);
   return PAIR(__nv_bfloat16);
 #undef PAIR
+}
+
+// Routed experts: g.T tiles of 128 rows at most, w of `experts` stacked matrices
+int rows_gemm(const PairCall& g, const void* table, int experts, int dtype, cudaStream_t st) {
+  PairParams p;
+  p.table = (const int32_t*)table;
+  p.T = p.m_tiles = 0;
+  if (dtype == B2L_F16)
+    return g.gated ? launch_rows<__half, 256, true, 1>(g, p, g.T * 128, experts, g.T, st) : launch_rows<__half, 256, false, 1>(g, p, g.T * 128, experts, g.T, st);
+  return g.gated ? launch_rows<__nv_bfloat16, 256, true, 1>(g, p, g.T * 128, experts, g.T, st)
+                 : launch_rows<__nv_bfloat16, 256, false, 1>(g, p, g.T * 128, experts, g.T, st);
 }
 
 }  // namespace mx4

@@ -49,19 +49,6 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 // silu(g) * u in 32 bits
 __device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
 
-// A lane's eight of a block's 32 values (four neighbouring lanes; the whole warp takes part): the codes, and the block's scale byte.
-__device__ __forceinline__ uint32_t quantise8(float (&v)[8], uint32_t& byte) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
-  byte = scale_byte(block_max(m));
-  const float inv = inverse_scale(byte);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] *= inv;
-  const uint32_t c = codes8(v);
-  return byte == 255u ? 0u : c;
-}
-
 #endif  // __CUDACC__
 
 }  // namespace mx4

@@ -11,7 +11,9 @@ namespace mx4 {
 
 constexpr int kSortThreads = 1024;
 
-// One CTA: ranks by counters in shared memory, tiles by a scan over experts.
+// One CTA: ranks by counters in shared memory, tiles by a scan over experts.  Up to HELD slots a thread, whose ids are asked for together and
+// stay in registers with their ranks; what is left goes through `place`.
+template <int HELD>
 __global__ void __launch_bounds__(kSortThreads)
 sort_kernel(int32_t* __restrict__ place, int32_t* __restrict__ table, const void* __restrict__ ids, int id_width, int slots, int tile,
             int experts) {
@@ -23,9 +25,18 @@ sort_kernel(int32_t* __restrict__ place, int32_t* __restrict__ table, const void
   for (int e = tid; e < experts; e += kSortThreads) counts[e] = 0;
   if (tid == 0) carry = 0;
   __syncthreads();
-  for (int s = tid; s < slots; s += kSortThreads) {
+  auto expert_of = [&](int s) {
     const int64_t e = load_index(ids, s, id_width);
-    place[s] = e >= 0 && e < experts ? atomicAdd(&counts[e], 1) : -1;
+    return e >= 0 && e < experts ? (int)e : -1;
+  };
+  int held[HELD], rank[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) held[i] = tid + i * kSortThreads < slots ? expert_of(tid + i * kSortThreads) : -1;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) rank[i] = held[i] >= 0 ? atomicAdd(&counts[held[i]], 1) : -1;
+  for (int s = tid + HELD * kSortThreads; s < slots; s += kSortThreads) {
+    const int e = expert_of(s);
+    place[s] = e >= 0 ? atomicAdd(&counts[e], 1) : -1;
   }
   __syncthreads();
   for (int base = 0; base < experts; base += kSortThreads) {
@@ -63,41 +74,39 @@ sort_kernel(int32_t* __restrict__ place, int32_t* __restrict__ table, const void
       table[2 + 2 * (first[e] + i)] = n - i * tile < tile ? n - i * tile : tile;
     }
   }
-  for (int s = tid; s < slots; s += kSortThreads) {
-    const int64_t e = load_index(ids, s, id_width);
-    if (e >= 0 && e < experts) place[s] += first[e] * tile;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i)
+    if (tid + i * kSortThreads < slots) place[tid + i * kSortThreads] = held[i] >= 0 ? rank[i] + first[held[i]] * tile : -1;
+  for (int s = tid + HELD * kSortThreads; s < slots; s += kSortThreads) {
+    const int e = expert_of(s);
+    if (e >= 0) place[s] += first[e] * tile;
   }
 }
 
-// A token's row quantised once and written to the rows of all its slots (quantize_kernel in mxfp4_quant.cu).
+// A token's row quantised once (quantize_kernel in mxfp4_quant.cu) and written to the rows of all its slots.
 template <typename T>
 __global__ void __launch_bounds__(256)
 scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, const int32_t* __restrict__ place,
-               int64_t tokens, int top_k, int tile, int64_t k, int64_t x_stride, int64_t ktiles, int units) {
+               uint32_t tokens, int top_k, uint32_t tile, uint32_t k, int64_t x_stride, int64_t ktiles, uint32_t units) {
   pdl_prologue();
   const int lane = threadIdx.x & 31;
-  const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t row = u / units;
-  if (row >= tokens) return;
-  const int64_t c = (u - row * units) * 32 + lane;
+  const uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 5), row = u / units;
+  if (row >= tokens) return;                           // whole warps
+  const uint32_t c = (u - row * units) * 32 + lane;
   const bool in = c * 8 < k;
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  int mine = lane < top_k ? ld_upstream(place + (int64_t)row * top_k + lane) : -1;      // the first 32 slots, a lane each
   if (in) load8(x + row * x_stride + c * 8, v);
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
-  const uint32_t byte = scale_byte(block_max(m));
-  const float inv = inverse_scale(byte);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] *= inv;
+  uint32_t byte;
+  const uint32_t code = quantise8(v, byte);
   const uint32_t word = word_of(in ? byte : 0u, lane);
-  const uint32_t code = byte == 255u ? 0u : codes8(v);
   for (int j = 0; j < top_k; ++j) {
-    const int to = ld_upstream(place + row * top_k + j);
+    if (j > 0 && (j & 31) == 0) mine = j + lane < top_k ? ld_upstream(place + (int64_t)row * top_k + j + lane) : -1;
+    const int to = __shfl_sync(0xffffffffu, mine, j & 31);
     if (to < 0 || !in) continue;
-    *reinterpret_cast<uint32_t*>(codes + to * (k / 2) + c * 4) = code;
+    *reinterpret_cast<uint32_t*>(codes + (int64_t)to * (k / 2) + c * 4) = code;
     if ((lane & 15) == 0)
-      *reinterpret_cast<uint32_t*>(scales + scale_word((int64_t)(to / tile) * 128 + to % tile, (int)(c >> 4), ktiles)) = word;
+      *reinterpret_cast<uint32_t*>(scales + scale_word((int64_t)(to / (int)tile) * 128 + to % (int)tile, (int)(c >> 4), ktiles)) = word;
   }
 }
 
@@ -107,16 +116,15 @@ __global__ void __launch_bounds__(256)
 combine_kernel(T* __restrict__ out, const T* __restrict__ y, const int32_t* __restrict__ place, const W* __restrict__ weights,
                int64_t tokens, int top_k, int64_t n) {
   pdl_prologue();
-  const int64_t chunks = n / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t chunks = (uint32_t)(n / 8), i = blockIdx.x * 256 + threadIdx.x;
   if (i >= tokens * chunks) return;
-  const int64_t t = i / chunks, c = i - t * chunks;
+  const int64_t t = i / chunks, c = i % chunks;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int j0 = 0; j0 < top_k; j0 += 4) {              // four rows requested together
-    uint4 q[4];
-    float w[4];
+  for (int j0 = 0; j0 < top_k; j0 += 8) {              // eight rows requested together
+    uint4 q[8];
+    float w[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 8; ++j) {
       const int from = j0 + j < top_k ? ld_upstream(place + t * top_k + j0 + j) : -1;
       q[j] = make_uint4(0u, 0u, 0u, 0u);
       w[j] = 0.f;
@@ -126,7 +134,7 @@ combine_kernel(T* __restrict__ out, const T* __restrict__ y, const int32_t* __re
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 8; ++j) {
       const T* e = reinterpret_cast<const T*>(&q[j]);
 #pragma unroll
       for (int h = 0; h < 8; ++h) sum[h] = fmaf(w[j], to_f32(e[h]), sum[h]);
@@ -168,7 +176,7 @@ extern "C" int b2l_mxfp4_moe_sort(void* place, void* table, const void* topk_ids
   B2L_REQUIRE(tile_rows > 0 && experts > 0 && experts <= 4096 && slots >= 0 && slots < (1ll << 24),
               "mxfp4_moe_sort: bad sizes (slots=%lld tile=%d experts=%d)", (long long)slots, tile_rows, experts);
   B2L_REQUIRE(table && (slots == 0 || (place && topk_ids)), "mxfp4_moe_sort: null pointer");
-  b2l_launch(mx4::sort_kernel, dim3(1), dim3(mx4::kSortThreads), (size_t)experts * 8, (cudaStream_t)stream, (int32_t*)place, (int32_t*)table,
+  b2l_launch(slots <= mx4::kSortThreads ? mx4::sort_kernel<1> : mx4::sort_kernel<16>, dim3(1), dim3(mx4::kSortThreads), (size_t)experts * 8, (cudaStream_t)stream, (int32_t*)place, (int32_t*)table,
              topk_ids, id_width, (int)slots, tile_rows, experts);
   B2L_LAUNCH_CHECK();
   return B2L_OK;
@@ -182,12 +190,11 @@ extern "C" int b2l_mxfp4_moe_scatter(void* codes, void* scales, const void* x, c
   B2L_REQUIRE(codes && scales && x && place, "mxfp4_moe_scatter: null pointer");
   B2L_REQUIRE((uintptr_t)x % 16 == 0 && x_row_stride % 8 == 0 && (uintptr_t)codes % 4 == 0 && (uintptr_t)scales % 4 == 0,
               "mxfp4_moe_scatter: rows must start on 16 bytes");
-  const int units = (int)cdiv64(k, 256);
-  const int64_t grid = cdiv64(tokens * units, 8);
-  B2L_REQUIRE(grid < (1ll << 31), "mxfp4_moe_scatter: too many tokens");
+  const int64_t units = cdiv64(k, 256), grid = cdiv64(tokens * units, 8);
+  B2L_REQUIRE(tokens * units < (1ll << 31), "mxfp4_moe_scatter: too many tokens");
 #define SCATTER(T)                                                                                                                  \
   b2l_launch(mx4::scatter_kernel<T>, dim3((unsigned)grid), dim3(256), (size_t)0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, \
-             (const T*)x, (const int32_t*)place, tokens, top_k, tile_rows, k, x_row_stride, mx4::k_tiles(k), units)
+             (const T*)x, (const int32_t*)place, (uint32_t)tokens, top_k, (uint32_t)tile_rows, (uint32_t)k, x_row_stride, mx4::k_tiles(k), (uint32_t)units)
   if (dtype == B2L_F16) SCATTER(__half);
   else if (dtype == B2L_BF16) SCATTER(__nv_bfloat16);
   else B2L_UNSUPPORTED("mxfp4_moe_scatter: dtype %d", dtype);
@@ -198,7 +205,7 @@ extern "C" int b2l_mxfp4_moe_scatter(void* codes, void* scales, const void* x, c
 
 extern "C" int b2l_mxfp4_moe_combine(void* out, const void* y, const void* place, const void* weights, int weights_f32, int64_t tokens,
                                      int top_k, int64_t n, int dtype, void* stream) {
-  B2L_REQUIRE(tokens >= 0 && top_k > 0 && n > 0 && n % 8 == 0 && tokens * (n / 8) < (1ll << 38), "mxfp4_moe_combine: tokens=%lld n=%lld (a multiple of 8)",
+  B2L_REQUIRE(tokens >= 0 && top_k > 0 && n > 0 && n % 8 == 0 && tokens * (n / 8) < (1ll << 31), "mxfp4_moe_combine: tokens=%lld n=%lld (a multiple of 8)",
               (long long)tokens, (long long)n);
   if (tokens == 0) return B2L_OK;
   B2L_REQUIRE(out && y && place && weights && ((uintptr_t)out | (uintptr_t)y) % 16 == 0, "mxfp4_moe_combine: null or misaligned pointer");

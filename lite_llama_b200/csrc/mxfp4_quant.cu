@@ -6,115 +6,162 @@ namespace mx4 {
 
 constexpr int kWarps = 8;
 
-// A warp takes 256 consecutive elements of a row: 16 bytes a lane (512 a warp) in, four bytes a lane out, one scale word per 16 lanes.
-// Rows are `per` to a matrix; a matrix starts on a tile of scales of its own.
-template <typename T>
+// A warp takes U x 256 consecutive elements of a row and asks for all of them before it uses the first: 16 bytes a lane (512 a warp) in,
+// four bytes a lane out, one scale word per 16 lanes.  Rows are `per` to a matrix; a matrix starts on a tile of scales of its own.
+template <typename T, int U>
 __global__ void __launch_bounds__(kWarps * 32)
-quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, int64_t rows, int64_t per,
-                int64_t k, int64_t x_stride, int64_t ktiles, int units) {
+quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, uint32_t rows, uint32_t per,
+                uint32_t k, int64_t x_stride, int64_t ktiles, uint32_t units) {
   pdl_prologue();
   const int lane = threadIdx.x & 31;
-  const int64_t u = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int64_t row = u / units;
+  const uint32_t u = blockIdx.x * kWarps + (threadIdx.x >> 5), row = u / units;
   if (row >= rows) return;                             // whole warps
-  const int64_t c = (u - row * units) * 32 + lane;     // chunk of eight elements
-  const bool in = c * 8 < k;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (in) load8(x + row * x_stride + c * 8, v);
-  uint32_t m = 0;
+  const uint32_t first = (u - row * units) * (32 * U) + lane, chunks = k / 8;      // chunks of eight elements
+  float v[U][8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
-  const uint32_t byte = scale_byte(block_max(m));
-  const float inv = inverse_scale(byte);
+  for (int i = 0; i < U; ++i) {
+    if (first + 32 * i < chunks) {
+      load8(x + row * x_stride + (first + 32 * i) * 8, v[i]);
+    } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] *= inv;
-  const uint32_t word = word_of(in ? byte : 0u, lane);
-  if (in) *reinterpret_cast<uint32_t*>(codes + row * (k / 2) + c * 4) = byte == 255u ? 0u : codes8(v);
-  if (in && (lane & 15) == 0) {
-    const int64_t matrix = row / per;
-    const int64_t padded = matrix * ((per + 127) / 128 * 128) + (row - matrix * per);
-    *reinterpret_cast<uint32_t*>(scales + scale_word(padded, (int)(c >> 4), ktiles)) = word;
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    }
+  }
+  const uint32_t matrix = row / per;
+  const int64_t padded = (int64_t)matrix * ((per + 127) / 128 * 128) + (row - matrix * per);
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint32_t c = first + 32 * i;
+    if (c - lane >= chunks) break;                     // whole warps
+    const bool in = c < chunks;
+    uint32_t byte;
+    const uint32_t code = quantise8(v[i], byte);
+    const uint32_t word = word_of(in ? byte : 0u, lane);
+    if (in) *reinterpret_cast<uint32_t*>(codes + (int64_t)row * (k / 2) + c * 4) = code;
+    if (in && (lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(padded, (int)(c >> 4), ktiles)) = word;
   }
 }
 
-template <typename T>
+// The same cut; a lane reads four bytes of codes and its block's byte and writes eight values.
+template <typename T, int U>
 __global__ void __launch_bounds__(kWarps * 32)
-dequantize_kernel(T* __restrict__ y, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
-                  int64_t per, int64_t k, int64_t codes_stride, int64_t ktiles, int units) {
+dequantize_kernel(T* __restrict__ y, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t rows, uint32_t per,
+                  uint32_t k, int64_t codes_stride, int64_t ktiles, uint32_t units) {
   pdl_prologue();
   const int lane = threadIdx.x & 31;
-  const int64_t u = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int64_t row = u / units;
-  const int64_t c = (u - row * units) * 32 + lane;
-  if (row >= rows || c * 8 >= k) return;
-  const int64_t matrix = row / per;
-  const int64_t padded = matrix * ((per + 127) / 128 * 128) + (row - matrix * per);
-  const uint32_t word = *reinterpret_cast<const uint32_t*>(scales + scale_word(padded, (int)(c >> 4), ktiles));
-  const uint32_t q = *reinterpret_cast<const uint32_t*>(codes + row * codes_stride + c * 4);
-  const float s = scale_value((word >> (8 * ((c >> 2) & 3))) & 255u);
-  float t[8];
-  elements8(q, t);
-  T* out = y + row * k + c * 8;
-  if constexpr (sizeof(T) == 4) {
-    stg_128(out, make_uint4(__float_as_uint(t[0] * s), __float_as_uint(t[1] * s), __float_as_uint(t[2] * s), __float_as_uint(t[3] * s)));
-    stg_128(out + 4, make_uint4(__float_as_uint(t[4] * s), __float_as_uint(t[5] * s), __float_as_uint(t[6] * s), __float_as_uint(t[7] * s)));
-  } else {
-    stg_128(out, make_uint4(pack2<T>(t[0] * s, t[1] * s), pack2<T>(t[2] * s, t[3] * s), pack2<T>(t[4] * s, t[5] * s),
-                            pack2<T>(t[6] * s, t[7] * s)));
+  const uint32_t u = blockIdx.x * kWarps + (threadIdx.x >> 5), row = u / units;
+  if (row >= rows) return;
+  const uint32_t first = (u - row * units) * (32 * U) + lane, chunks = k / 8;
+  const uint32_t matrix = row / per;
+  const int64_t padded = (int64_t)matrix * ((per + 127) / 128 * 128) + (row - matrix * per);
+  uint32_t q[U], b[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint32_t c = first + 32 * i;
+    q[i] = b[i] = 0;
+    if (c < chunks) {
+      q[i] = ld_once(codes + row * codes_stride + c * 4);
+      b[i] = scales[scale_word(padded, (int)(c >> 4), ktiles) + ((c >> 2) & 3)];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint32_t c = first + 32 * i;
+    if (c >= chunks) break;
+    const float s = scale_value(b[i]);
+    float t[8];
+    elements8(q[i], t);
+    T* out = y + (int64_t)row * k + c * 8;
+    if constexpr (sizeof(T) == 4) {
+      stg_128(out, make_uint4(__float_as_uint(t[0] * s), __float_as_uint(t[1] * s), __float_as_uint(t[2] * s), __float_as_uint(t[3] * s)));
+      stg_128(out + 4, make_uint4(__float_as_uint(t[4] * s), __float_as_uint(t[5] * s), __float_as_uint(t[6] * s), __float_as_uint(t[7] * s)));
+    } else {
+      stg_128(out, make_uint4(pack2<T>(t[0] * s, t[1] * s), pack2<T>(t[2] * s, t[3] * s), pack2<T>(t[4] * s, t[5] * s),
+                              pack2<T>(t[6] * s, t[7] * s)));
+    }
   }
 }
+
+// Units of 256 elements to a warp: one where the warps of all would not fill the SMs twice over, else four.
+static int units_of(int64_t rows, int64_t k) { return rows * cdiv64(k, 256) < 128LL * b2l_num_sms() ? 1 : 4; }
 
 // ---------------------------------------------------------------------------------------------------------------
 // s = x + r (stored over r, or to `sum`, in the activations' type), y = s / sqrt(mean s^2 + eps) * w, quantised.
 //
 // y is not rounded to 16 bits on the way: the 16-bit norm would round it twice (before and behind the weight), and elements that
-// lie next to a border would then go by those roundings.  It is computed in 32 bits, at most 2^-21.5 off; where that could change an
-// element or the scale (values within 2^-20 of a border, one element in 10^5), the warp computes its blocks again in 64 bits, so
-// the codes are those of exact arithmetic.  The sum of squares is in 64 bits for them from the start.
+// lie next to a border would then go by those roundings.  It is computed in 32 bits.  The sum of squares, in four sums to a thread that
+// a tree joins, is off by at most (2 VPT + 23) 2^-24, its root by half of that, root and products by 2^-21.6 more: below 2^-19.  A value that
+// lies nearer to a border, and a largest magnitude nearer to a power of two, is decided in 64 bits: where a row has one (a twentieth
+// of the rows of 4096), the CTA adds up the squares again and its threads redo the blocks in question, so the codes are those of exact
+// arithmetic.
+// Bound: instructions (with the sum of squares in 64 bits from the start and integer maxima 42 an element, 1999 x 3584 20.6 us); with
+// few rows latency, of which a row's second turn is 1.8 us (32 x 4096: 4.2): there (FEW) the sum is in 64 bits from the start, and a warp
+// redoes its blocks by itself.
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T, int VPT>
-__global__ void __launch_bounds__(512)
-norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, T* __restrict__ sum, const T* __restrict__ x,
-                     const T* __restrict__ res, const T* __restrict__ w, int64_t n, int64_t x_stride, int64_t r_stride,
-                     int64_t s_stride, int64_t ktiles, float eps) {
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+template <typename T, int VPT, bool FEW>
+__global__ void __launch_bounds__(512, 2)
+norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, T* sum, const T* __restrict__ x, const T* res,
+                     const T* __restrict__ w, int n, int64_t x_stride, int64_t r_stride, int64_t s_stride, int64_t ktiles, double inv_n,
+                     float eps) {
   pdl_prologue();
   const int64_t row = blockIdx.x;
-  const int chunks = (int)(n / 8), lane = threadIdx.x & 31;
-  uint4 xv[VPT], rv[VPT];
-  double ss = 0.0;
+  const int chunks = n / 8, lane = threadIdx.x & 31;
+  x += row * x_stride;
+  res = res ? res + row * r_stride : nullptr;
+  float s[VPT][8];
+  float ss[4] = {0.f, 0.f, 0.f, 0.f};
+  double sq = 0.0;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
-    xv[i] = rv[i] = make_uint4(0u, 0u, 0u, 0u);
+    uint4 xv = make_uint4(0u, 0u, 0u, 0u), rv = xv;
     if (c < chunks) {
-      xv[i] = ldg_128(x + row * x_stride + c * 8);
-      if (res) rv[i] = ldg_128(res + row * r_stride + c * 8);
+      xv = ldg_128(x + c * 8);
+      if (res) rv = ldg_128(res + c * 8);
+    }
+    const T *xe = reinterpret_cast<const T*>(&xv), *re = reinterpret_cast<const T*>(&rv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      s[i][j] = to_f32(xe[j]) + to_f32(re[j]);
+      if (FEW) {
+        const double p = (double)to_f32(xe[j]) + (double)to_f32(re[j]);
+        sq = fma(p, p, sq);
+      } else {
+        ss[j & 3] = fmaf(s[i][j], s[i][j], ss[j & 3]);
+      }
     }
   }
+  __shared__ float red[16];
+  __shared__ double wide[16];
+  auto add_up = [&]() {                // of all threads, in 64 bits
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = threadIdx.x + i * blockDim.x;
-    const T *xe = reinterpret_cast<const T*>(&xv[i]), *re = reinterpret_cast<const T*>(&rv[i]);
-    uint32_t o[4];
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const float a = to_f32(xe[j]), b = to_f32(xe[j + 1]), d = to_f32(re[j]), e = to_f32(re[j + 1]);
-      o[j / 2] = pack2<T>(a + d, b + e);
-      const double p = (double)a + (double)d, q = (double)b + (double)e;
-      ss = fma(p, p, ss);
-      ss = fma(q, q, ss);
-    }
-    if (res && c < chunks) stg_128(sum + row * s_stride + c * 8, make_uint4(o[0], o[1], o[2], o[3]));
+    for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    if (lane == 0) wide[threadIdx.x >> 5] = sq;
+    __syncthreads();
+    double all = 0.0;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) all += wide[i];
+    return rsqrt(fma(all, inv_n, (double)eps));
+  };
+  double root = 0.0;
+  float rrms;
+  if (FEW) {
+    root = add_up();
+    rrms = (float)root;
+  } else {
+    const float mine = warp_reduce_sum((ss[0] + ss[1]) + (ss[2] + ss[3]));
+    if (lane == 0) red[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    float tot = 0.f;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) tot += red[i];
+    rrms = rsqrtf(fmaf(tot, (float)inv_n, eps));
   }
-  __shared__ double red[16];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (lane == 0) red[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  double tot = 0.0;
-  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) tot += red[i];
-  const double rrms = 1.0 / sqrt(tot / (double)n + (double)eps);
-  const float r32 = (float)rrms;
+  uint32_t near = 0;                   // chunks that 64 bits decide
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
@@ -122,48 +169,77 @@ norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, 
     const bool in = c < chunks;
     uint4 wv = make_uint4(0u, 0u, 0u, 0u);
     if (in) wv = ldg_128(w + c * 8);
-    const T *xe = reinterpret_cast<const T*>(&xv[i]), *re = reinterpret_cast<const T*>(&rv[i]), *we = reinterpret_cast<const T*>(&wv);
-    float v[8];
-    uint32_t m = 0;
+    const T* we = reinterpret_cast<const T*>(&wv);
+    float v[8], m = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      v[j] = (to_f32(xe[j]) + to_f32(re[j])) * r32 * to_f32(we[j]);
-      m = max(m, abs_bits(v[j]));
+      v[j] = s[i][j] * rrms * to_f32(we[j]);
+      m = max_nan(m, fabsf(v[j]));
     }
-    m = block_max(m);
-    uint32_t byte = scale_byte(m);
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const uint32_t top = __float_as_uint(m) & 0x7fffffffu, byte = scale_byte(top);
     const float inv = inverse_scale(byte);
-    float lo[8], hi[8];
+    float end[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float t = v[j] * inv;
-      lo[j] = fmaf(t, -0x1p-20f, t);
-      hi[j] = fmaf(t, 0x1p-20f, t);
+      v[j] *= inv;
+      end[j] = fmaf(v[j], -0x1p-19f, v[j]);
     }
-    uint32_t code = codes8(lo);
-    // a value next to a border, a maximum next to a power of two (8 steps of 2^-23), or so small that 32 bits lose digits
-    const bool near = m != 0u && byte != 255u && (code != codes8(hi) || ((m - 8u) >> 23) != ((m + 8u) >> 23) || m < 0x0d000000u);
-    if (__any_sync(0xffffffffu, near)) {
-      double d[8], top = 0.0;
+    const uint32_t code = codes8(end);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        d[j] = ((double)to_f32(xe[j]) + (double)to_f32(re[j])) * rrms * (double)to_f32(we[j]);
-        top = fmax(top, fabs(d[j]));
-      }
+    for (int j = 0; j < 8; ++j) end[j] = fmaf(v[j], 0x1p-19f, v[j]);
+    // next to a border, the largest next to a power of two (16 steps of 2^-23), or so small that 32 bits lose digits
+    bool unsure = top != 0u && byte != 255u && (code != codes8(end) || ((top - 16u) >> 23) != ((top + 16u) >> 23) || top < 0x0d000000u);
+    unsure |= __shfl_xor_sync(0xffffffffu, (int)unsure, 1) != 0;
+    unsure |= __shfl_xor_sync(0xffffffffu, (int)unsure, 2) != 0;
+    near |= (uint32_t)unsure << i;
+    const uint32_t word = word_of(in ? byte : 0u, lane);
+    if (in) *reinterpret_cast<uint32_t*>(codes + row * (n / 2) + c * 4) = byte == 255u ? 0u : code;
+    if (in && (lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(row, c >> 4, ktiles)) = word;
+  }
+  if (FEW ? __any_sync(0xffffffffu, (int)near) : __syncthreads_or((int)near)) {
+    __syncwarp();                      // behind the words of scales above
+    // again in 64 bits, from memory (a thread's own chunks, whose sums are stored below); blocks that were sure keep their codes
+    if (!FEW) {
+      for (int c = threadIdx.x; c < chunks; c += blockDim.x)
+        for (int j = 0; j < 8; ++j) {
+          const double p = (double)to_f32(x[c * 8 + j]) + (res ? (double)to_f32(res[c * 8 + j]) : 0.0);
+          sq = fma(p, p, sq);
+        }
+      root = add_up();
+    }
+#pragma unroll 1
+    for (int i = 0; i < VPT; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (c - lane >= chunks || __ballot_sync(0xffffffffu, (near >> i) & 1u) == 0u) continue;      // whole warps
+      auto exact = [&](int j) {
+        return c >= chunks ? 0.0 : ((double)to_f32(x[c * 8 + j]) + (res ? (double)to_f32(res[c * 8 + j]) : 0.0)) * root * (double)to_f32(w[c * 8 + j]);
+      };
+      double top = 0.0;
+      for (int j = 0; j < 8; ++j) top = fmax(top, fabs(exact(j)));
       top = fmax(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmax(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (byte != 255u) {                              // infinities and NaN are those of 32 bits
+      if ((near >> i) & 1u) {
         const int field = (int)((__double_as_longlong(top) >> 52) & 2047) - 1023 + 127;
-        byte = field > 254 ? 255u : (field > 2 ? (uint32_t)(field - 2) : 0u);
+        const uint32_t byte = field > 254 ? 255u : (field > 2 ? (uint32_t)(field - 2) : 0u);
         const double scale = __longlong_as_double((long long)(1023 + 127 - (int)byte) << 52);
-        code = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) code |= code_of(d[j] * scale) << (4 * j);
+        uint32_t code = 0;
+        if (byte != 255u)
+          for (int j = 0; j < 8; ++j) code |= code_of(exact(j) * scale) << (4 * j);
+        *reinterpret_cast<uint32_t*>(codes + row * (n / 2) + c * 4) = code;
+        if ((lane & 3) == 0) scales[scale_word(row, c >> 4, ktiles) + ((c >> 2) & 3)] = (uint8_t)byte;
       }
     }
-    const uint32_t word = word_of(in ? byte : 0u, lane);
-    if (in) *reinterpret_cast<uint32_t*>(codes + row * (n / 2) + (int64_t)c * 4) = byte == 255u ? 0u : code;
-    if (in && (lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(row, c >> 4, ktiles)) = word;
+  }
+  if (res) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (c < chunks)
+        stg_128(sum + row * s_stride + c * 8, make_uint4(pack2<T>(s[i][0], s[i][1]), pack2<T>(s[i][2], s[i][3]), pack2<T>(s[i][4], s[i][5]),
+                                                         pack2<T>(s[i][6], s[i][7])));
+    }
   }
 }
 
@@ -171,15 +247,17 @@ template <typename T>
 static int launch_norm(void* codes, void* scales, void* sum, const void* x, const void* res, const void* w, int64_t rows,
                        int64_t n, int64_t xs, int64_t rs, int64_t ss, float eps, cudaStream_t st) {
   const int64_t chunks = n / 8;
-#define NORM(V)                                                                                                                \
+#define NORM(V, F)                                                                                                                \
   {                                                                                                                            \
     const int threads = (int)(cdiv64(cdiv64(chunks, V), 32) * 32);                                                             \
-    b2l_launch(norm_quantize_kernel<T, V>, dim3((unsigned)rows), dim3(threads), (size_t)0, st, (uint8_t*)codes, (uint8_t*)scales, \
-               (T*)sum, (const T*)x, (const T*)res, (const T*)w, n, xs, rs, ss, k_tiles(n), eps);                               \
+    b2l_launch(norm_quantize_kernel<T, V, F>, dim3((unsigned)rows), dim3(threads), (size_t)0, st, (uint8_t*)codes, (uint8_t*)scales, \
+               (T*)sum, (const T*)x, (const T*)res, (const T*)w, (int)n, xs, rs, ss, k_tiles(n), 1.0 / (double)n, eps);               \
   }
-  if (chunks <= 512) NORM(1)
-  else if (chunks <= 1024) NORM(2)
-  else NORM(4)
+  // rows that come two or more to an SM are read by fewer threads each, so that more of them are in flight
+  const bool many = rows > 2LL * b2l_num_sms();
+  if (many) NORM(4, false)
+  else if (chunks <= 512) NORM(1, true)
+  else NORM(4, true)
 #undef NORM
   B2L_LAUNCH_CHECK();
   return B2L_OK;
@@ -201,12 +279,14 @@ extern "C" int b2l_mxfp4_quantize(void* codes, void* scales, const void* x, int6
   const int esz = dtype == B2L_F32 ? 4 : 2;
   B2L_REQUIRE((uintptr_t)x % 16 == 0 && x_row_stride * esz % 16 == 0 && (uintptr_t)codes % 4 == 0 && (uintptr_t)scales % 4 == 0,
               "mxfp4_quantize: rows must start on 16 bytes");
-  const int units = (int)cdiv64(k, 256);
-  const int64_t grid = cdiv64(all * units, mx4::kWarps);
-  B2L_REQUIRE(grid < (1ll << 31), "mxfp4_quantize: too many rows");
+  const int per_warp = mx4::units_of(all, k);
+  const int64_t units = cdiv64(k, 256 * per_warp);
+  B2L_REQUIRE(all * units < (1ll << 31), "mxfp4_quantize: too many rows");
+  const dim3 grid((unsigned)cdiv64(all * units, mx4::kWarps));
   B2L_DISPATCH_FLOAT(dtype, "mxfp4_quantize", {
-    b2l_launch(mx4::quantize_kernel<T>, dim3((unsigned)grid), dim3(mx4::kWarps * 32), (size_t)0, (cudaStream_t)stream,
-               (uint8_t*)codes, (uint8_t*)scales, (const T*)x, all, rows, k, x_row_stride, mx4::k_tiles(k), units);
+    b2l_launch(per_warp == 1 ? mx4::quantize_kernel<T, 1> : mx4::quantize_kernel<T, 4>, grid, dim3(mx4::kWarps * 32), (size_t)0,
+               (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const T*)x, (uint32_t)all, (uint32_t)rows, (uint32_t)k,
+               x_row_stride, mx4::k_tiles(k), (uint32_t)units);
   });
   B2L_LAUNCH_CHECK();
   return B2L_OK;
@@ -221,12 +301,14 @@ extern "C" int b2l_mxfp4_dequantize(void* y, const void* codes, const void* scal
   B2L_REQUIRE(y && codes && scales, "mxfp4_dequantize: null pointer");
   B2L_REQUIRE((uintptr_t)y % 16 == 0 && (uintptr_t)codes % 4 == 0 && codes_row_stride % 4 == 0 && (uintptr_t)scales % 4 == 0,
               "mxfp4_dequantize: misaligned rows");
-  const int units = (int)cdiv64(k, 256);
-  const int64_t grid = cdiv64(all * units, mx4::kWarps);
-  B2L_REQUIRE(grid < (1ll << 31), "mxfp4_dequantize: too many rows");
+  const int per_warp = mx4::units_of(all, k);
+  const int64_t units = cdiv64(k, 256 * per_warp);
+  B2L_REQUIRE(all * units < (1ll << 31), "mxfp4_dequantize: too many rows");
+  const dim3 grid((unsigned)cdiv64(all * units, mx4::kWarps));
   B2L_DISPATCH_FLOAT(dtype, "mxfp4_dequantize", {
-    b2l_launch(mx4::dequantize_kernel<T>, dim3((unsigned)grid), dim3(mx4::kWarps * 32), (size_t)0, (cudaStream_t)stream, (T*)y,
-               (const uint8_t*)codes, (const uint8_t*)scales, all, rows, k, codes_row_stride, mx4::k_tiles(k), units);
+    b2l_launch(per_warp == 1 ? mx4::dequantize_kernel<T, 1> : mx4::dequantize_kernel<T, 4>, grid, dim3(mx4::kWarps * 32), (size_t)0,
+               (cudaStream_t)stream, (T*)y, (const uint8_t*)codes, (const uint8_t*)scales, (uint32_t)all, (uint32_t)rows, (uint32_t)k,
+               codes_row_stride, mx4::k_tiles(k), (uint32_t)units);
   });
   B2L_LAUNCH_CHECK();
   return B2L_OK;
