@@ -57,7 +57,7 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   Control* ctl = reinterpret_cast<Control*>(smem);
   uint8_t* ring = smem + 1024;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;      // uniform (mxfp4_gemm_pair.cu)
   const uint32_t S = cluster_size(), rank = pair_rank();
   const int tile = blockIdx.x / S, m0 = blockIdx.y * BT;
   const int kb0 = (int)((int64_t)p.num_kb * rank / S), kb1 = (int)((int64_t)p.num_kb * (rank + 1) / S);
@@ -79,7 +79,7 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl->tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
 
   if (warp == 0) {
     // ===================== TMA producer =====================
@@ -341,7 +341,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   GroupedControl* ctl = reinterpret_cast<GroupedControl*>(smem);
   uint8_t* ring = smem + 1024;
   float* out_stage = reinterpret_cast<float*>(ring + R::kStages * R::kStage);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;      // uniform (mxfp4_gemm_pair.cu)
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmap_x);
     tma_prefetch_desc(&tmap_w);
@@ -363,7 +363,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl->tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
   pdl_wait_prior();                    // the table and the rows are upstream data
   const int items = ld_upstream(p.table) * p.n_tiles;
 
@@ -548,7 +548,7 @@ extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const vo
               "mxfp4_matmul: rows of codes must start on 16 bytes");
   B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "mxfp4_matmul: dtype %d", dtype);
   cudaStream_t st = (cudaStream_t)stream;
-  mx4::PairCall g = {y, y_row_stride, y_scales, bias, x, x_scales, w, w_scales, t, n, k, x_row_stride, w_row_stride, gated != 0};
+  mx4::PairCall g = {y, y_row_stride, y_scales, bias, x, x_scales, w, w_scales, t, n, k, x_row_stride, w_row_stride, gated != 0, weights_ready != 0};
   if (mx4::pair_wanted(g)) return mx4::pair_gemm(g, dtype, st);
   mx4::Params p;
   p.y = y; p.ldy = y_row_stride;
@@ -578,7 +578,7 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
               "mxfp4_grouped_matmul: rows of codes must start on 16 bytes");
   B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "mxfp4_grouped_matmul: dtype %d", dtype);
   cudaStream_t st = (cudaStream_t)stream;
-  mx4::PairCall g = {y, gated ? n / 4 : n, y_scales, nullptr, x, x_scales, w, w_scales, max_tiles, n, k, k / 2, k / 2, gated != 0};
+  mx4::PairCall g = {y, gated ? n / 4 : n, y_scales, nullptr, x, x_scales, w, w_scales, max_tiles, n, k, k / 2, k / 2, gated != 0, false};
   if (tile_rows == 128) {
     B2L_REQUIRE(gated || (n % 8 == 0 && (uintptr_t)y % 16 == 0), "mxfp4_grouped_matmul: tiles of 128 rows are written in units of 8 outputs (n=%lld)", (long long)n);
     B2L_REQUIRE(!gated || (uintptr_t)y % 16 == 0, "mxfp4_grouped_matmul: rows of codes must start on 16 bytes");

@@ -11,6 +11,7 @@ struct PairCall {
   const void *x, *x_scales, *w, *w_scales;
   int64_t T, N, K, ldx, ldw;           // row strides of codes in bytes
   bool gated;
+  bool early;                          // weights may be requested before the previous kernel has ended
 };
 
 // whether the pair kernel takes the call and is the faster one (mxfp4_gemm_pair.cu)

@@ -18,16 +18,16 @@
 
 namespace mx4 {
 
-constexpr int kPairThreads = 6 * 32;   // TMA producer, MMA issuer, four warps that read the accumulator
+constexpr int kPairThreads = 10 * 32;  // TMA producer, MMA issuer, eight warps that read the accumulator
 constexpr int kPairRows = 128;         // tokens per CTA
 constexpr int kPairBand = 16;          // token tiles per band: 16 x 256 rows x 4096 / 2 bytes = 8 MiB of L2
 
 template <int BN, int CTAS> struct PairRing {
-  static constexpr int kStages = CTAS == 2 ? 5 : 4, kBoxes = CTAS == 2 ? 2 : 1;      // boxes of 32 rows x 64 outputs on their way out, per warp
+  static constexpr int kStages = CTAS == 2 ? 5 : 3;
   static constexpr int kX = 16384, kW = BN / CTAS * 128;
   static constexpr int kXs = kX + kW, kWs = kXs + kSfBytes;
   static constexpr int kBytes = kWs + BN / 128 * kSfBytes;
-  static constexpr int kSmem = 1024 + 1024 + kStages * kBytes + 4 * kBoxes * 4096;
+  static constexpr int kSmem = 1024 + 1024 + kStages * kBytes + 8 * 4096;
   static constexpr int kAcc1 = BN == 256 ? 208 : 128;                     // first column of the second accumulator
   static constexpr int kSf = BN == 256 ? 464 : 256;
   static constexpr int kSfSet = 8 + BN / 128 * 8;
@@ -38,6 +38,7 @@ struct PairParams {
   uint8_t* y; uint8_t* y_scales; int64_t ldy, y_ktiles;                   // gated: codes and scales
   const int32_t* table;                // experts: tiles, then {expert, rows} of each
   int T, N, K, num_kb, m_tiles, n_tiles, ktiles;
+  int early;                           // weights may be requested before the previous kernel has ended
 };
 
 struct __align__(8) PairControl {
@@ -107,7 +108,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
   uint8_t* ring = smem + 1024;
   uint8_t* out_stage = ring + R::kStages * R::kBytes;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // one value for the warp, as far as the compiler can see: roles and addresses then live in uniform registers
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = CTAS == 2 ? pair_rank() : 0u;
   const int pairs = gridDim.x / CTAS, pair = blockIdx.x / CTAS;
   if (warp == 0 && lane == 0) {
@@ -122,7 +124,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&ctl->acc_full[b], 1);
-      mbar_init(&ctl->freed[b], 4 * CTAS);
+      mbar_init(&ctl->freed[b], 8 * CTAS);
     }
     mbar_fence_init();
   }
@@ -134,30 +136,48 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
   tc_fence_before();
   sync_all<CTAS>();
   tc_fence_after();
-  const uint32_t tmem = ctl->tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
   if (CTAS == 1) pdl_wait_prior();     // the table is upstream data
   const int tiles = (CTAS == 2 ? p.m_tiles : ld_upstream(p.table)) * p.n_tiles;
 
   if (warp == 0) {
     // ===================== TMA producer: this CTA's halves of both operands, its tokens' scales, all outputs' scales =====================
-    pdl_wait_prior();
+    auto expect = [&](int s) {
+      if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], CTAS * R::kBytes);
+    };
+    auto load_w = [&](int s, int kb, const Work& wk) {
+      uint8_t* st = ring + (size_t)s * R::kBytes;
+      const int row = wk.expert * p.N + wk.n * BN + (int)rank * (BN / CTAS);
+      const int ws = (wk.expert * ((p.N + 127) / 128) + wk.n * (BN / 128)) * p.ktiles * 4;      // rows of 128 bytes
+      load_2d<CTAS>(st + R::kX, &tmap_w, kb * 128, row, &ctl->full[s]);
+#pragma unroll
+      for (int h = 0; h < BN / 128; ++h) load_2d<CTAS>(st + R::kWs + h * kSfBytes, &tmap_ws, 0, ws + h * p.ktiles * 4 + kb * 8, &ctl->full[s]);
+    };
+    auto load_x = [&](int s, int kb, const Work& wk) {
+      uint8_t* st = ring + (size_t)s * R::kBytes;
+      load_2d<CTAS>(st, &tmap_x, kb * 128, wk.m * kPairRows, &ctl->full[s]);
+      load_2d<CTAS>(st + R::kXs, &tmap_xs, 0, (wk.m * p.ktiles + kb * 2) * 4, &ctl->full[s]);
+    };
     gemm::PipeState ps(R::kStages);
+    int ahead = 0;                     // stages whose weights were requested before the previous kernel has ended
+    if (CTAS == 2 && p.early && pair < tiles) {
+      const Work wk = work_of<CTAS>(p, pair, (int)rank);
+      ahead = p.num_kb < R::kStages ? p.num_kb : R::kStages;
+      if (elect_one())
+        for (int s = 0; s < ahead; ++s) { expect(s); load_w(s, s, wk); }
+      __syncwarp();
+    }
+    pdl_wait_prior();
     for (int t = pair; t < tiles; t += pairs) {
       const Work wk = work_of<CTAS>(p, t, (int)rank);
-      const int row_x = wk.m * kPairRows, row_w = wk.expert * p.N + wk.n * BN + (int)rank * (BN / CTAS);
-      const int xs = wk.m * p.ktiles * 4, ws = (wk.expert * ((p.N + 127) / 128) + wk.n * (BN / 128)) * p.ktiles * 4;      // rows of 128 bytes
+#pragma unroll 1
       for (int kb = 0; kb < p.num_kb; ++kb) {
         mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
         if (elect_one()) {
-          if (rank == 0) mbar_arrive_expect_tx(&ctl->full[ps.stage], CTAS * R::kBytes);
-          uint8_t* st = ring + (size_t)ps.stage * R::kBytes;
-          uint64_t* bar = &ctl->full[ps.stage];
-          load_2d<CTAS>(st, &tmap_x, kb * 128, row_x, bar);
-          load_2d<CTAS>(st + R::kX, &tmap_w, kb * 128, row_w, bar);
-          load_2d<CTAS>(st + R::kXs, &tmap_xs, 0, xs + kb * 8, bar);
-#pragma unroll
-          for (int h = 0; h < BN / 128; ++h) load_2d<CTAS>(st + R::kWs + h * kSfBytes, &tmap_ws, 0, ws + h * p.ktiles * 4 + kb * 8, bar);
+          if (ahead == 0) { expect(ps.stage); load_w(ps.stage, kb, wk); }
+          load_x(ps.stage, kb, wk);
         }
+        if (ahead > 0) --ahead;
         __syncwarp();
         ps.advance();
       }
@@ -169,6 +189,9 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     }
   } else if (warp == 1) {
     // ===================== MMA issuer (leader only) =====================
+    // A step of 256 k is 512 cycles of the tensor pipe, and the issuer's own instructions take nearly as long: they bound the kernel
+    // until warp index and column base were uniform to the compiler (1000 x 4096 x 14336 29.9 -> 24 us).  The loop unrolled over the
+    // ring is slower (256 x 4096 x 4096 7.7 -> 8.8: instruction cache), a second elected region costs 120 ns a step.
     if (rank == 0) {
       const uint64_t desc0 = umma_desc_sw128_kmajor(smem_u32(ring)), sf0 = scale_desc(smem_u32(ring));
       gemm::PipeState ps(R::kStages), back(R::kStages);      // back: the stage two before
@@ -176,22 +199,23 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       for (int t = pair; t < tiles; t += pairs, ++it) {
         const uint32_t acc = tmem + (it & 1) * R::kAcc1;
         if (BN == 256) {
-          if (it >= 1) mbar_wait(&ctl->freed[(it - 1) & 1], ((it - 1) >> 1) & 1);
+          if (it >= 1) mbar_wait_spin(&ctl->freed[(it - 1) & 1], ((it - 1) >> 1) & 1);
         } else {
-          if (it >= 2) mbar_wait(&ctl->freed[it & 1], ((it - 2) >> 1) & 1);
+          if (it >= 2) mbar_wait_spin(&ctl->freed[it & 1], ((it - 2) >> 1) & 1);
         }
         tc_fence_after();
+#pragma unroll 1
         for (int kb = 0; kb < p.num_kb; ++kb, ++i) {
           if (i >= 2) {
-            mbar_wait(&ctl->empty[back.stage], back.phase);
+            mbar_wait_spin(&ctl->empty[back.stage], back.phase);
             back.advance();
           }
-          mbar_wait(&ctl->full[ps.stage], ps.phase);
+          mbar_wait_spin(&ctl->full[ps.stage], ps.phase);
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t base = (uint64_t)(ps.stage * R::kBytes) >> 4;
+            const uint32_t base = (uint32_t)(ps.stage * R::kBytes) >> 4;
             const uint64_t xd = desc0 + base, wd = xd + (R::kX >> 4);
-            const uint64_t xsf = sf0 + base + (R::kXs >> 4), wsf = sf0 + base + (R::kWs >> 4);
+            const uint64_t xsf = sf0 + base + (R::kXs >> 4), wsf = xsf + (kSfBytes >> 4);
             const uint32_t sfa = tmem + R::kSf + (i & 1) * R::kSfSet, sfb = sfa + 8;
             const int steps = (p.K - kb * kStageK + 63) >> 6;
 #pragma unroll
@@ -201,11 +225,11 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
 #pragma unroll
                 for (int h = 0; h < BN / 128; ++h)
                   copy_scales<CTAS>(sfb + j * (BN / 32) + 4 * h, wsf + h * (kSfBytes >> 4) + j * (kTileBytes >> 4));
-              }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (j < steps)
-                mma<CTAS>(acc, xd + 2 * j, wd + 2 * j, idesc(128 * CTAS, BN, j & 1), sfa + (j >> 1) * 4, sfb + (j >> 1) * (BN / 32), kb | j ? 1u : 0u);
+                for (int q = 2 * j; q < 2 * j + 2; ++q)
+                  if (q < steps)
+                    mma<CTAS>(acc, xd + 2 * q, wd + 2 * q, idesc(128 * CTAS, BN, q & 1), sfa + j * 4, sfb + j * (BN / 32), kb | q ? 1u : 0u);
+              }
             commit<CTAS>(&ctl->empty[ps.stage]);
             if (kb + 1 == p.num_kb) commit<CTAS>(&ctl->acc_full[it & 1]);
           }
@@ -215,8 +239,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       }
     }
   } else {
-    // ===================== one thread per token =====================
-    const int quad = warp & 3;
+    // ===================== one thread per token, two warps to its columns =====================
+    const int quad = warp & 3, half = (warp - 2) >> 2;
     auto hand_on = [&](int buf) {
       tc_fence_before();
       __syncwarp();
@@ -226,28 +250,31 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       }
     };
     pdl_wait_prior();                  // y may still be read upstream
-    int it = 0, box = 0;
+    uint8_t* dst = out_stage + (quad + 4 * half) * 4096;
+    int it = 0;
     for (int t = pair; t < tiles; t += pairs, ++it) {
       const Work wk = work_of<CTAS>(p, t, (int)rank);
       const int buf = it & 1, m_warp = wk.m * kPairRows + quad * 32;
       const bool any = quad * 32 < wk.rows;             // uniform over the warp
       const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * R::kAcc1;
-      mbar_wait(&ctl->acc_full[buf], (it >> 1) & 1);
+      // the columns that both accumulators have: the first one's last, read by the second half's warps, the second one's first.  The other
+      // half's warps are done with the tile before, which is what their arrival says.
+      const bool shared = BN == 256 && half == 1 - buf;
+      mbar_wait_spin(&ctl->acc_full[buf], (it >> 1) & 1);
       tc_fence_after();
+      if (BN == 256 && !shared) hand_on(buf);
       if (!GATED) {
 #pragma unroll 1
-        for (int j = 0; j < BN / 64; ++j) {
-          // the shared columns first: the first accumulator's last, the second one's first
-          const int c = (BN == 256 && buf == 0 ? BN / 64 - 1 - j : j) * 64;
+        for (int j = 0; j < BN / 128; ++j) {
+          const int c = half * (BN / 2) + (BN == 256 && buf == 0 ? 1 - j : j) * 64;
           uint32_t v[64];
           tmem_ld_32x32b_x32(acc + c, *reinterpret_cast<uint32_t(*)[32]>(v));
           tmem_ld_32x32b_x32(acc + c + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
           tc_wait_ld();
-          if (j == (BN == 256 ? 0 : BN / 64 - 1)) hand_on(buf);
+          if (BN == 256 ? shared && j == 0 : true) hand_on(buf);
           const int n0 = wk.n * BN + c;
           if (n0 >= p.N || !any) continue;
-          uint8_t* dst = out_stage + (quad * R::kBoxes + box % R::kBoxes) * 4096;
-          if (lane == 0) bulk_wait_read<R::kBoxes - 1>();      // the store that used this box before has read it
+          if (lane == 0) bulk_wait_read<0>();           // the store before has read the box
           __syncwarp();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
@@ -267,49 +294,53 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
             tma_store_2d(&tmap_y, dst, n0, m_warp);
             bulk_commit();
           }
-          ++box;
         }
       } else {
-        // runs of 64 gate and 64 up columns; a run's half that lies on the shared columns is read whole before anything else
-        const int row = m_warp + lane;
-#pragma unroll 1
-        for (int j = 0; j < BN / 128; ++j) {
-          const bool back = BN == 256 && buf == 0;
-          const int c = (back ? BN / 128 - 1 - j : j) * 128;
-          uint32_t held[64];           // the up half of the first accumulator's runs, the gate half of the second's
-          tmem_ld_32x32b_x32(acc + c + (back ? 64 : 0), *reinterpret_cast<uint32_t(*)[32]>(held));
-          tmem_ld_32x32b_x32(acc + c + (back ? 96 : 32), *reinterpret_cast<uint32_t(*)[32]>(held + 32));
+        // A run of 64 gate and 64 up columns to each half (of the narrow tile's only run: a block of 32).  What lies on the shared columns is
+        // read before anything else: the up columns of the first accumulator's second run, the gate columns of the second's first.
+        constexpr int kBlocks = BN / 128;               // blocks of 32 activations to a warp
+        const bool up_first = BN == 256 && buf == 0;
+        const int c = BN == 256 ? half * 128 : half * 32;
+        uint32_t held[32 * kBlocks];
+#pragma unroll
+        for (int h = 0; h < kBlocks; ++h)
+          tmem_ld_32x32b_x32(acc + c + (up_first ? 64 : 0) + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(held + 32 * h));
+        tc_wait_ld();
+        if (shared) hand_on(buf);
+        const int n0 = wk.n * BN + (BN == 256 ? c : 0), k = n0 / 2 + (BN == 256 ? 0 : half * 32), row = m_warp + lane;
+        uint32_t bytes = 0;
+        uint4 codes[kBlocks];
+#pragma unroll
+        for (int h = 0; h < kBlocks; ++h) {
+          uint32_t other[32];
+          tmem_ld_32x32b_x32(acc + c + (up_first ? 0 : 64) + 32 * h, other);
           tc_wait_ld();
-          if (BN == 256 && j == 0) hand_on(buf);
-          const int n0 = wk.n * BN + c;
-          uint32_t bytes = 0;
-          uint4 codes[2];
+          if (BN != 256) hand_on(buf);
+          const int n = n0 + (BN == 256 ? 32 * h : 32 * half);      // the block's gate rows
+          float v[32];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t other[32];
-            tmem_ld_32x32b_x32(acc + c + (back ? 0 : 64) + 32 * h, other);
-            tc_wait_ld();
-            if (BN != 256 && j + 1 == BN / 128 && h == 1) hand_on(buf);
-            float v[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              float g = __uint_as_float(back ? other[e] : held[32 * h + e]), u = __uint_as_float(back ? held[32 * h + e] : other[e]);
-              if (p.bias && n0 < p.N) {
-                g += to_f32(reinterpret_cast<const T*>(p.bias)[n0 + 32 * h + e]);
-                u += to_f32(reinterpret_cast<const T*>(p.bias)[n0 + 64 + 32 * h + e]);
-              }
-              v[e] = gated(g, u);
+          for (int e = 0; e < 32; ++e) {
+            float g = __uint_as_float(up_first ? other[e] : held[32 * h + e]), u = __uint_as_float(up_first ? held[32 * h + e] : other[e]);
+            if (p.bias && n < p.N) {
+              g += to_f32(reinterpret_cast<const T*>(p.bias)[n + e]);
+              u += to_f32(reinterpret_cast<const T*>(p.bias)[n + 64 + e]);
             }
-            bytes |= quantise32(v, codes[h]) << (8 * h);
+            v[e] = gated(g, u);
           }
-          if (n0 < p.N && quad * 32 + lane < wk.rows) {                  // N is a multiple of 128
-            uint8_t* y = p.y + (int64_t)row * p.ldy + n0 / 4;
-            stg_128(y, codes[0]);
-            stg_128(y + 16, codes[1]);
-            const int k = n0 / 2;                       // first activation: a multiple of 64
-            uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles) + ((k >> 5) & 3);
-            if (n0 + 128 == p.N && (k & 64) == 0) *reinterpret_cast<uint32_t*>(word) = bytes;   // nothing behind: zeros
+          bytes |= quantise32(v, codes[h]) << (8 * h);
+        }
+        if (n0 < p.N && quad * 32 + lane < wk.rows) {   // N is a multiple of 128
+          uint8_t* y = p.y + (int64_t)row * p.ldy + k / 2;
+#pragma unroll
+          for (int h = 0; h < kBlocks; ++h) stg_128(y + 16 * h, codes[h]);
+          uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles) + ((k >> 5) & 3);
+          const bool last = n0 + 128 == p.N && (k & 64) == 0;      // an odd number of runs: zeros behind the end
+          if (BN == 256) {
+            if (last) *reinterpret_cast<uint32_t*>(word) = bytes;
             else *reinterpret_cast<uint16_t*>(word) = (uint16_t)bytes;
+          } else {
+            word[0] = (uint8_t)bytes;
+            if (last) word[2] = 0;
           }
         }
       }
@@ -373,6 +404,7 @@ static int launch_pair(const PairCall& g, cudaStream_t st) {
   PairParams p;
   p.table = nullptr;
   p.T = (int)g.T;
+  p.early = g.early ? 1 : 0;
   p.m_tiles = (int)cdiv64(g.T, 2 * kPairRows);
   return launch_rows<T, BN, GATED, 2>(g, p, g.T, 1, p.m_tiles, st);
 }
@@ -399,7 +431,7 @@ int pair_gemm(const PairCall& g, int dtype, cudaStream_t st) {
 int rows_gemm(const PairCall& g, const void* table, int experts, int dtype, cudaStream_t st) {
   PairParams p;
   p.table = (const int32_t*)table;
-  p.T = p.m_tiles = 0;
+  p.T = p.m_tiles = p.early = 0;
   if (dtype == B2L_F16)
     return g.gated ? launch_rows<__half, 256, true, 1>(g, p, g.T * 128, experts, g.T, st) : launch_rows<__half, 256, false, 1>(g, p, g.T * 128, experts, g.T, st);
   return g.gated ? launch_rows<__nv_bfloat16, 256, true, 1>(g, p, g.T * 128, experts, g.T, st)
