@@ -7,7 +7,7 @@ namespace mx4 {
 constexpr int kWarps = 8;
 
 // A warp takes U x 256 consecutive elements of a row and asks for all of them before it uses the first: 16 bytes a lane (512 a warp) in,
-// four bytes a lane out, one scale word per 16 lanes.  Rows are `per` to a matrix; a matrix starts on a tile of scales of its own.
+// four bytes a lane out, and a scale byte per four lanes.  Rows are `per` to a matrix; a matrix starts on a tile of scales of its own.
 template <typename T, int U>
 __global__ void __launch_bounds__(kWarps * 32)
 quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, uint32_t rows, uint32_t per,
@@ -17,29 +17,56 @@ quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const
   const uint32_t u = blockIdx.x * kWarps + (threadIdx.x >> 5), row = u / units;
   if (row >= rows) return;                             // whole warps
   const uint32_t first = (u - row * units) * (32 * U) + lane, chunks = k / 8;      // chunks of eight elements
-  float v[U][8];
+  const T* src = x + row * x_stride + (int64_t)first * 8;
+  Raw8<T> v[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    if (first + 32 * i < chunks) {
-      load8(x + row * x_stride + (first + 32 * i) * 8, v[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    }
+    zero_raw(v[i]);
+    if (first + 32 * i < chunks) load_raw(src + 256 * i, v[i]);
   }
   const uint32_t matrix = row / per;
   const int64_t padded = (int64_t)matrix * ((per + 127) / 128 * 128) + (row - matrix * per);
+  uint8_t* out = codes + (int64_t)row * (k / 2) + first * 4;
+  uint8_t* scale = scales + scale_word(padded, (int)(first >> 4), ktiles) + ((first >> 2) & 3);
+  const uint32_t behind = (chunks + 15) & ~15u;        // blocks up to here are filled up with zeros
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const uint32_t c = first + 32 * i;
-    if (c - lane >= chunks) break;                     // whole warps
-    const bool in = c < chunks;
-    uint32_t byte;
-    const uint32_t code = quantise8(v[i], byte);
-    const uint32_t word = word_of(in ? byte : 0u, lane);
-    if (in) *reinterpret_cast<uint32_t*>(codes + (int64_t)row * (k / 2) + c * 4) = code;
-    if (in && (lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(padded, (int)(c >> 4), ktiles)) = word;
+    uint32_t byte;                                     // of a block behind the end: 0
+    const uint32_t code = quantise_raw(v[i], byte);
+    if (first + 32 * i < chunks) *reinterpret_cast<uint32_t*>(out + 128 * i) = code;
+    if ((lane & 3) == 0 && first + 32 * i < behind) scale[2 * kTileBytes * i] = (uint8_t)byte;
   }
+}
+
+// Eight codes and their block's scale byte -> eight values, rounded once
+template <typename T> __device__ __forceinline__ uint4 values8(uint32_t c, uint32_t byte) {
+  uint32_t o[4];
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    // The elements' bf16 bits from two tables of eight bytes; the scale is a bf16 for every byte.
+    const uint32_t s = byte == 0u ? 0x00400040u : (byte == 255u ? 0x7fc07fc0u : byte * 0x00800080u);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t q = (c >> (16 * h)) & 0xffffu, index = q & 0x7777u;
+      const uint32_t high = __byte_perm(0x3f3f3f00u, 0x40404040u, index), low = __byte_perm(0xc0800000u, 0xc0804000u, index);
+      const uint32_t a = __byte_perm(low, high, 0x5140) | ((q << 12) & 0x8000u) | ((q << 24) & 0x80000000u);
+      const uint32_t b = __byte_perm(low, high, 0x7362) | ((q << 4) & 0x8000u) | ((q << 16) & 0x80000000u);
+      const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162*>(&s);
+      const __nv_bfloat162 y0 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), s2), y1 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), s2);
+      o[2 * h] = *reinterpret_cast<const uint32_t*>(&y0);
+      o[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&y1);
+    }
+  } else {
+    float t[8];
+    elements8(c, t);
+    const float s = scale_value(byte);
+    const f32x2 s2 = pair_of(s, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 y = mul2(pair_of(t[2 * i], t[2 * i + 1]), s2);
+      o[i] = pack2<__half>(first_of(y), second_of(y));
+    }
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // The same cut; a lane reads four bytes of codes and its block's byte and writes eight values.
@@ -54,30 +81,29 @@ dequantize_kernel(T* __restrict__ y, const uint8_t* __restrict__ codes, const ui
   const uint32_t first = (u - row * units) * (32 * U) + lane, chunks = k / 8;
   const uint32_t matrix = row / per;
   const int64_t padded = (int64_t)matrix * ((per + 127) / 128 * 128) + (row - matrix * per);
+  const uint8_t* src = codes + row * codes_stride + first * 4;
+  const uint8_t* scale = scales + scale_word(padded, (int)(first >> 4), ktiles) + ((first >> 2) & 3);
+  T* out = y + (int64_t)row * k + (int64_t)first * 8;
   uint32_t q[U], b[U];
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const uint32_t c = first + 32 * i;
-    q[i] = b[i] = 0;
-    if (c < chunks) {
-      q[i] = ld_once(codes + row * codes_stride + c * 4);
-      b[i] = scales[scale_word(padded, (int)(c >> 4), ktiles) + ((c >> 2) & 3)];
+  for (int i = 0; i < U; ++i)
+    if (first + 32 * i < chunks) {
+      q[i] = ld_once(src + 128 * i);
+      b[i] = scale[2 * kTileBytes * i];
     }
-  }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const uint32_t c = first + 32 * i;
-    if (c >= chunks) break;
-    const float s = scale_value(b[i]);
-    float t[8];
-    elements8(q[i], t);
-    T* out = y + (int64_t)row * k + c * 8;
+    if (first + 32 * i >= chunks) break;
     if constexpr (sizeof(T) == 4) {
-      stg_128(out, make_uint4(__float_as_uint(t[0] * s), __float_as_uint(t[1] * s), __float_as_uint(t[2] * s), __float_as_uint(t[3] * s)));
-      stg_128(out + 4, make_uint4(__float_as_uint(t[4] * s), __float_as_uint(t[5] * s), __float_as_uint(t[6] * s), __float_as_uint(t[7] * s)));
+      float t[8];
+      elements8(q[i], t);
+      const float s = scale_value(b[i]);
+#pragma unroll
+      for (int j = 0; j < 8; j += 4)
+        stg_128(out + 256 * i + j, make_uint4(__float_as_uint(t[j] * s), __float_as_uint(t[j + 1] * s), __float_as_uint(t[j + 2] * s),
+                                              __float_as_uint(t[j + 3] * s)));
     } else {
-      stg_128(out, make_uint4(pack2<T>(t[0] * s, t[1] * s), pack2<T>(t[2] * s, t[3] * s), pack2<T>(t[4] * s, t[5] * s),
-                              pack2<T>(t[6] * s, t[7] * s)));
+      stg_128(out + 256 * i, values8<T>(q[i], b[i]));
     }
   }
 }
@@ -89,8 +115,8 @@ static int units_of(int64_t rows, int64_t k) { return rows * cdiv64(k, 256) < 12
 // s = x + r (stored over r, or to `sum`, in the activations' type), y = s / sqrt(mean s^2 + eps) * w, quantised.
 //
 // y is not rounded to 16 bits on the way: the 16-bit norm would round it twice (before and behind the weight), and elements that
-// lie next to a border would then go by those roundings.  It is computed in 32 bits.  The sum of squares, in four sums to a thread that
-// a tree joins, is off by at most (2 VPT + 23) 2^-24, its root by half of that, root and products by 2^-21.6 more: below 2^-19.  A value that
+// lie next to a border would then go by those roundings.  It is computed in 32 bits.  The sum of squares, in eight sums to a thread that
+// a tree joins, is off by at most (VPT + 24) 2^-24, its root by half of that, root and products by 2^-21.6 more: below 2^-19.  A value that
 // lies nearer to a border, and a largest magnitude nearer to a power of two, is decided in 64 bits: where a row has one (a twentieth
 // of the rows of 4096), the CTA adds up the squares again and its threads redo the blocks in question, so the codes are those of exact
 // arithmetic.
@@ -98,9 +124,10 @@ static int units_of(int64_t rows, int64_t k) { return rows * cdiv64(k, 256) < 12
 // few rows latency, of which a row's second turn is 1.8 us (32 x 4096: 4.2): there (FEW) the sum is in 64 bits from the start, and a warp
 // redoes its blocks by itself.
 // ---------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float max_nan(float a, float b) {
+// the larger magnitude; NaN if one of them is
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -114,29 +141,31 @@ norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, 
   const int chunks = n / 8, lane = threadIdx.x & 31;
   x += row * x_stride;
   res = res ? res + row * r_stride : nullptr;
-  float s[VPT][8];
-  float ss[4] = {0.f, 0.f, 0.f, 0.f};
+  f32x2 s[VPT][4], ss[4] = {0ull, 0ull, 0ull, 0ull};
   double sq = 0.0;
+  uint4 xv[VPT], rv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
-    uint4 xv = make_uint4(0u, 0u, 0u, 0u), rv = xv;
+    xv[i] = rv[i] = make_uint4(0u, 0u, 0u, 0u);
     if (c < chunks) {
-      xv = ldg_128(x + c * 8);
-      if (res) rv = ldg_128(res + c * 8);
-    }
-    const T *xe = reinterpret_cast<const T*>(&xv), *re = reinterpret_cast<const T*>(&rv);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      s[i][j] = to_f32(xe[j]) + to_f32(re[j]);
-      if (FEW) {
-        const double p = (double)to_f32(xe[j]) + (double)to_f32(re[j]);
-        sq = fma(p, p, sq);
-      } else {
-        ss[j & 3] = fmaf(s[i][j], s[i][j], ss[j & 3]);
-      }
+      xv[i] = ldg_128(x + c * 8);
+      if (res) rv[i] = ldg_128(res + c * 8);
     }
   }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 a = widen<T>(reinterpret_cast<const uint32_t*>(&xv[i])[j]), b = widen<T>(reinterpret_cast<const uint32_t*>(&rv[i])[j]);
+      s[i][j] = add2(a, b);
+      if (FEW) {
+        const double p = (double)first_of(a) + (double)first_of(b), q = (double)second_of(a) + (double)second_of(b);
+        sq = fma(q, q, fma(p, p, sq));
+      } else {
+        ss[j] = fma2(s[i][j], s[i][j], ss[j]);
+      }
+    }
   __shared__ float red[16];
   __shared__ double wide[16];
   auto add_up = [&]() {                // of all threads, in 64 bits
@@ -154,13 +183,16 @@ norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, 
     root = add_up();
     rrms = (float)root;
   } else {
-    const float mine = warp_reduce_sum((ss[0] + ss[1]) + (ss[2] + ss[3]));
+    const f32x2 all = add2(add2(ss[0], ss[1]), add2(ss[2], ss[3]));
+    const float mine = warp_reduce_sum(first_of(all) + second_of(all));
     if (lane == 0) red[threadIdx.x >> 5] = mine;
     __syncthreads();
     float tot = 0.f;
     for (int i = 0; i < (int)(blockDim.x >> 5); ++i) tot += red[i];
     rrms = rsqrtf(fmaf(tot, (float)inv_n, eps));
   }
+  const f32x2 r2 = pair_of(rrms, rrms), below = pair_of(-0x1p-19f, -0x1p-19f), above = pair_of(0x1p-19f, 0x1p-19f);
+  const uint32_t behind = ((uint32_t)chunks + 15u) & ~15u;
   uint32_t near = 0;                   // chunks that 64 bits decide
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -169,37 +201,36 @@ norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, 
     const bool in = c < chunks;
     uint4 wv = make_uint4(0u, 0u, 0u, 0u);
     if (in) wv = ldg_128(w + c * 8);
-    const T* we = reinterpret_cast<const T*>(&wv);
-    float v[8], m = 0.f;
+    f32x2 v[4];
+    float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = s[i][j] * rrms * to_f32(we[j]);
-      m = max_nan(m, fabsf(v[j]));
+    for (int j = 0; j < 4; ++j) {
+      v[j] = mul2(mul2(s[i][j], r2), widen<T>(reinterpret_cast<const uint32_t*>(&wv)[j]));
+      m = max_abs(m, first_of(v[j]), second_of(v[j]));
     }
-    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, 1), 0.f);
+    m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, 2), 0.f);
     const uint32_t top = __float_as_uint(m) & 0x7fffffffu, byte = scale_byte(top);
     const float inv = inverse_scale(byte);
-    float end[8];
+    const f32x2 inv2 = pair_of(inv, inv);
+    f32x2 end[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] *= inv;
-      end[j] = fmaf(v[j], -0x1p-19f, v[j]);
+    for (int j = 0; j < 4; ++j) {
+      v[j] = mul2(v[j], inv2);
+      end[j] = fma2(v[j], below, v[j]);
     }
     const uint32_t code = codes8(end);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) end[j] = fmaf(v[j], 0x1p-19f, v[j]);
+    for (int j = 0; j < 4; ++j) end[j] = fma2(v[j], above, v[j]);
     // next to a border, the largest next to a power of two (16 steps of 2^-23), or so small that 32 bits lose digits
-    bool unsure = top != 0u && byte != 255u && (code != codes8(end) || ((top - 16u) >> 23) != ((top + 16u) >> 23) || top < 0x0d000000u);
-    unsure |= __shfl_xor_sync(0xffffffffu, (int)unsure, 1) != 0;
-    unsure |= __shfl_xor_sync(0xffffffffu, (int)unsure, 2) != 0;
-    near |= (uint32_t)unsure << i;
-    const uint32_t word = word_of(in ? byte : 0u, lane);
+    const bool unsure = byte != 255u && (code != codes8(end) || ((top - 16u) ^ (top + 16u)) >> 23 != 0u || top < 0x0d000000u) && top != 0u;
+    const uint32_t group = __ballot_sync(0xffffffffu, unsure) >> (lane & 28) & 15u;      // of the block's four lanes
+    near |= (group != 0u ? 1u : 0u) << i;
     if (in) *reinterpret_cast<uint32_t*>(codes + row * (n / 2) + c * 4) = byte == 255u ? 0u : code;
-    if (in && (lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(row, c >> 4, ktiles)) = word;
+    if ((lane & 3) == 0 && (uint32_t)c < behind) scales[scale_word(row, c >> 4, ktiles) + ((c >> 2) & 3)] = (uint8_t)byte;
   }
   if (FEW ? __any_sync(0xffffffffu, (int)near) : __syncthreads_or((int)near)) {
-    __syncwarp();                      // behind the words of scales above
+    __syncwarp();                      // behind the stores above
     // again in 64 bits, from memory (a thread's own chunks, whose sums are stored below); blocks that were sure keep their codes
     if (!FEW) {
       for (int c = threadIdx.x; c < chunks; c += blockDim.x)
@@ -237,8 +268,8 @@ norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, 
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < chunks)
-        stg_128(sum + row * s_stride + c * 8, make_uint4(pack2<T>(s[i][0], s[i][1]), pack2<T>(s[i][2], s[i][3]), pack2<T>(s[i][4], s[i][5]),
-                                                         pack2<T>(s[i][6], s[i][7])));
+        stg_128(sum + row * s_stride + c * 8, make_uint4(pack2<T>(first_of(s[i][0]), second_of(s[i][0])), pack2<T>(first_of(s[i][1]), second_of(s[i][1])),
+                                                         pack2<T>(first_of(s[i][2]), second_of(s[i][2])), pack2<T>(first_of(s[i][3]), second_of(s[i][3]))));
     }
   }
 }

@@ -80,6 +80,11 @@ __device__ __forceinline__ uint4 ld_cluster_128(uint32_t a) {
   asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
 }
+__device__ __forceinline__ uint32_t ld_cluster_32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
 // one arrival in both CTAs of the pair whose even rank is `first`
 __device__ __forceinline__ void tc_commit_pair_at(uint64_t* bar, uint32_t first) {
   asm volatile(
