@@ -115,14 +115,12 @@ static int units_of(int64_t rows, int64_t k) { return rows * cdiv64(k, 256) < 12
 // s = x + r (stored over r, or to `sum`, in the activations' type), y = s / sqrt(mean s^2 + eps) * w, quantised.
 //
 // y is not rounded to 16 bits on the way: the 16-bit norm would round it twice (before and behind the weight), and elements that
-// lie next to a border would then go by those roundings.  It is computed in 32 bits.  The sum of squares, in eight sums to a thread that
-// a tree joins, is off by at most (VPT + 24) 2^-24, its root by half of that, root and products by 2^-21.6 more: below 2^-19.  A value that
-// lies nearer to a border, and a largest magnitude nearer to a power of two, is decided in 64 bits: where a row has one (a twentieth
-// of the rows of 4096), the CTA adds up the squares again and its threads redo the blocks in question, so the codes are those of exact
-// arithmetic.
-// Bound: instructions (with the sum of squares in 64 bits from the start and integer maxima 42 an element, 1999 x 3584 20.6 us); with
-// few rows latency, of which a row's second turn is 1.8 us (32 x 4096: 4.2): there (FEW) the sum is in 64 bits from the start, and a warp
-// redoes its blocks by itself.
+// lie next to a border would then go by those roundings.  The sum of squares is in 64 bits, y in 32, four roundings of 2^-24.  A value that
+// lies within 2^-21 of a border, or a largest magnitude that near to a power of two, is decided in 64 bits: the warp computes the blocks
+// in question again (one element in 10^5), so the codes are those of exact arithmetic.
+// Bound: instructions.  1999 x 3584, us with the reader behind it: 25.8 with all in 64 bits and integer maxima, 20.8 with the sum in 32 bits,
+// wider margins and rows with a doubtful block added up again by their CTA, 18.5 so; 17.8 without any decision in 64 bits.
+// Two chunks a thread 18.5, four 19.0, one 22.3.
 // ---------------------------------------------------------------------------------------------------------------
 // the larger magnitude; NaN if one of them is
 __device__ __forceinline__ float max_abs(float a, float b, float c) {
@@ -131,7 +129,7 @@ __device__ __forceinline__ float max_abs(float a, float b, float c) {
   return r;
 }
 
-template <typename T, int VPT, bool FEW>
+template <typename T, int VPT>
 __global__ void __launch_bounds__(512, 2)
 norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, T* sum, const T* __restrict__ x, const T* res,
                      const T* __restrict__ w, int n, int64_t x_stride, int64_t r_stride, int64_t s_stride, int64_t ktiles, double inv_n,
@@ -141,7 +139,7 @@ norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, 
   const int chunks = n / 8, lane = threadIdx.x & 31;
   x += row * x_stride;
   res = res ? res + row * r_stride : nullptr;
-  f32x2 s[VPT][4], ss[4] = {0ull, 0ull, 0ull, 0ull};
+  f32x2 s[VPT][4];
   double sq = 0.0;
   uint4 xv[VPT], rv[VPT];
 #pragma unroll
@@ -159,39 +157,19 @@ norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, 
     for (int j = 0; j < 4; ++j) {
       const f32x2 a = widen<T>(reinterpret_cast<const uint32_t*>(&xv[i])[j]), b = widen<T>(reinterpret_cast<const uint32_t*>(&rv[i])[j]);
       s[i][j] = add2(a, b);
-      if (FEW) {
-        const double p = (double)first_of(a) + (double)first_of(b), q = (double)second_of(a) + (double)second_of(b);
-        sq = fma(q, q, fma(p, p, sq));
-      } else {
-        ss[j] = fma2(s[i][j], s[i][j], ss[j]);
-      }
+      const double p = (double)first_of(a) + (double)first_of(b), q = (double)second_of(a) + (double)second_of(b);
+      sq = fma(q, q, fma(p, p, sq));
     }
-  __shared__ float red[16];
   __shared__ double wide[16];
-  auto add_up = [&]() {                // of all threads, in 64 bits
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-    if (lane == 0) wide[threadIdx.x >> 5] = sq;
-    __syncthreads();
-    double all = 0.0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) all += wide[i];
-    return rsqrt(fma(all, inv_n, (double)eps));
-  };
-  double root = 0.0;
-  float rrms;
-  if (FEW) {
-    root = add_up();
-    rrms = (float)root;
-  } else {
-    const f32x2 all = add2(add2(ss[0], ss[1]), add2(ss[2], ss[3]));
-    const float mine = warp_reduce_sum(first_of(all) + second_of(all));
-    if (lane == 0) red[threadIdx.x >> 5] = mine;
-    __syncthreads();
-    float tot = 0.f;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) tot += red[i];
-    rrms = rsqrtf(fmaf(tot, (float)inv_n, eps));
-  }
-  const f32x2 r2 = pair_of(rrms, rrms), below = pair_of(-0x1p-19f, -0x1p-19f), above = pair_of(0x1p-19f, 0x1p-19f);
+  for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+  if (lane == 0) wide[threadIdx.x >> 5] = sq;
+  __syncthreads();
+  double all = 0.0;
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) all += wide[i];
+  const double root = rsqrt(fma(all, inv_n, (double)eps));
+  const float rrms = (float)root;
+  const f32x2 r2 = pair_of(rrms, rrms), below = pair_of(-0x1p-21f, -0x1p-21f), above = pair_of(0x1p-21f, 0x1p-21f);
   const uint32_t behind = ((uint32_t)chunks + 15u) & ~15u;
   uint32_t near = 0;                   // chunks that 64 bits decide
 #pragma unroll
@@ -222,24 +200,16 @@ norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, 
     const uint32_t code = codes8(end);
 #pragma unroll
     for (int j = 0; j < 4; ++j) end[j] = fma2(v[j], above, v[j]);
-    // next to a border, the largest next to a power of two (16 steps of 2^-23), or so small that 32 bits lose digits
-    const bool unsure = byte != 255u && (code != codes8(end) || ((top - 16u) ^ (top + 16u)) >> 23 != 0u || top < 0x0d000000u) && top != 0u;
+    // next to a border, the largest next to a power of two (4 steps of 2^-23), or so small that 32 bits lose digits
+    const bool unsure = byte != 255u && (code != codes8(end) || ((top - 4u) ^ (top + 4u)) >> 23 != 0u || top < 0x0d000000u) && top != 0u;
     const uint32_t group = __ballot_sync(0xffffffffu, unsure) >> (lane & 28) & 15u;      // of the block's four lanes
     near |= (group != 0u ? 1u : 0u) << i;
     if (in) *reinterpret_cast<uint32_t*>(codes + row * (n / 2) + c * 4) = byte == 255u ? 0u : code;
     if ((lane & 3) == 0 && (uint32_t)c < behind) scales[scale_word(row, c >> 4, ktiles) + ((c >> 2) & 3)] = (uint8_t)byte;
   }
-  if (FEW ? __any_sync(0xffffffffu, (int)near) : __syncthreads_or((int)near)) {
+  if (__any_sync(0xffffffffu, (int)near)) {
     __syncwarp();                      // behind the stores above
     // again in 64 bits, from memory (a thread's own chunks, whose sums are stored below); blocks that were sure keep their codes
-    if (!FEW) {
-      for (int c = threadIdx.x; c < chunks; c += blockDim.x)
-        for (int j = 0; j < 8; ++j) {
-          const double p = (double)to_f32(x[c * 8 + j]) + (res ? (double)to_f32(res[c * 8 + j]) : 0.0);
-          sq = fma(p, p, sq);
-        }
-      root = add_up();
-    }
 #pragma unroll 1
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
@@ -278,17 +248,17 @@ template <typename T>
 static int launch_norm(void* codes, void* scales, void* sum, const void* x, const void* res, const void* w, int64_t rows,
                        int64_t n, int64_t xs, int64_t rs, int64_t ss, float eps, cudaStream_t st) {
   const int64_t chunks = n / 8;
-#define NORM(V, F)                                                                                                                \
+#define NORM(V)                                                                                                                \
   {                                                                                                                            \
     const int threads = (int)(cdiv64(cdiv64(chunks, V), 32) * 32);                                                             \
-    b2l_launch(norm_quantize_kernel<T, V, F>, dim3((unsigned)rows), dim3(threads), (size_t)0, st, (uint8_t*)codes, (uint8_t*)scales, \
+    b2l_launch(norm_quantize_kernel<T, V>, dim3((unsigned)rows), dim3(threads), (size_t)0, st, (uint8_t*)codes, (uint8_t*)scales, \
                (T*)sum, (const T*)x, (const T*)res, (const T*)w, (int)n, xs, rs, ss, k_tiles(n), 1.0 / (double)n, eps);               \
   }
-  // rows that come two or more to an SM are read by fewer threads each, so that more of them are in flight
+  // rows that come two or more to an SM are read by fewer threads each, so that more of them are in flight (figures above)
   const bool many = rows > 2LL * b2l_num_sms();
-  if (many) NORM(4, false)
-  else if (chunks <= 512) NORM(1, true)
-  else NORM(4, true)
+  if (chunks <= 512 && !many) NORM(1)
+  else if (chunks <= 1024) NORM(2)
+  else NORM(4)
 #undef NORM
   B2L_LAUNCH_CHECK();
   return B2L_OK;
