@@ -136,6 +136,15 @@ __device__ __forceinline__ uint32_t quantise8(float (&v)[8], uint32_t& byte) {
   return byte == 255u ? 0u : c;
 }
 
+// A lane's four of a block's 32 values (eight neighbouring lanes)
+__device__ __forceinline__ uint32_t quantise4(float a, float b, float c, float d, uint32_t& byte) {
+  uint32_t m = block_max(max(max(abs_bits(a), abs_bits(b)), max(abs_bits(c), abs_bits(d))));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+  byte = scale_byte(m);
+  const float inv = inverse_scale(byte), v[8] = {a * inv, b * inv, c * inv, d * inv, 0.f, 0.f, 0.f, 0.f};
+  return byte == 255u ? 0u : codes8(v);
+}
+
 // The same of eight values as they lie in memory.  16 bits: magnitudes are compared two at a time as the whole numbers that their bits are,
 // bf16 is scaled in pairs (exact but for what is far below the smallest element): 6 instructions an element, 14 by way of 32 bits.
 template <typename T> struct Raw8 { uint4 q; };

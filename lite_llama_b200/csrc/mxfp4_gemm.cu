@@ -30,7 +30,7 @@ struct Params {
 };
 
 template <int BT> struct Ring {
-  static constexpr int kStages = BT == 128 ? 5 : 4;
+  static constexpr int kStages = BT == 128 ? 3 : 4;
   static constexpr int kStage = 16384 + kSfBytes + BT * 128 + kSfBytes;   // W, its scales, X, its scales
   static constexpr int kX = 16384 + kSfBytes;
   static constexpr int kCols = BT + kStages * 16;                         // accumulator, then 16 columns of scales a stage
@@ -49,8 +49,90 @@ __device__ __forceinline__ uint32_t cluster_size() {
   return r;
 }
 
+// This CTA's share of a tile: sums over the S parts of k in their order, all parts of an output asked for together (one after another
+// they cost a trip to the other SM each: 128 tokens, 4096 x 4096, gated 13.1 us).  `sums`: [token][128] in every CTA of the cluster.
+template <typename T, bool GATED, int S>
+__device__ __forceinline__ void add_up(const Params& p, const uint8_t* sums, int tile, int m0, int tokens, uint32_t rank) {
+  const int lane = threadIdx.x & 31;
+  uint32_t base[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) base[s] = cluster_addr(sums, (uint32_t)s);
+  if (!GATED) {
+    // four outputs a thread
+    for (int i = threadIdx.x + kThreads * rank; i < tokens * 32; i += kThreads * S) {
+      const int t = i >> 5, n = tile * 128 + (i & 31) * 4;
+      uint4 q[S];
+#pragma unroll
+      for (int s = 0; s < S; ++s) q[s] = ld_cluster_128(base[s] + i * 16);
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        v[0] += __uint_as_float(q[s].x);
+        v[1] += __uint_as_float(q[s].y);
+        v[2] += __uint_as_float(q[s].z);
+        v[3] += __uint_as_float(q[s].w);
+      }
+      T* out = reinterpret_cast<T*>(p.y) + (int64_t)(m0 + t) * p.ldy + n;
+      const T* bias = reinterpret_cast<const T*>(p.bias);
+      if (bias)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) v[j] += to_f32(bias[n + j]);
+      if (p.vec && n < p.N) {          // N is a multiple of four
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) out[j] = from_f32<T>(v[j]);
+      }
+    }
+  } else {
+    // four activations a lane, eight lanes a block, two blocks a tile: 64 gate rows, then their up rows
+    const int tasks = tokens * 16;
+    for (int first = (int)(threadIdx.x & ~31u) + kThreads * (int)rank; first < tasks; first += kThreads * S) {
+      const int i = first + lane, t = i >> 4, e = (i & 15) * 4;
+      const bool in = i < tasks;
+      float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+      if (in) {
+        uint4 q[S], r[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          q[s] = ld_cluster_128(base[s] + (t * 128 + e) * 4);
+          r[s] = ld_cluster_128(base[s] + (t * 128 + 64 + e) * 4);
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          g[0] += __uint_as_float(q[s].x); g[1] += __uint_as_float(q[s].y); g[2] += __uint_as_float(q[s].z); g[3] += __uint_as_float(q[s].w);
+          u[0] += __uint_as_float(r[s].x); u[1] += __uint_as_float(r[s].y); u[2] += __uint_as_float(r[s].z); u[3] += __uint_as_float(r[s].w);
+        }
+        if (p.bias) {
+          const T* bias = reinterpret_cast<const T*>(p.bias) + (int64_t)tile * 128 + e;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            g[j] += to_f32(bias[j]);
+            u[j] += to_f32(bias[64 + j]);
+          }
+        }
+      }
+      uint32_t byte;
+      const uint32_t code = quantise4(gated(g[0], u[0]), gated(g[1], u[1]), gated(g[2], u[2]), gated(g[3], u[3]), byte);
+      if (in) {
+        const int64_t row = m0 + t;
+        const int k = tile * 64 + e;
+        *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p.y) + row * p.ldy + k / 2) = (uint16_t)code;
+        if ((lane & 7) == 0) {
+          uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles);
+          word[(k >> 5) & 3] = (uint8_t)byte;
+          // an odd number of tiles: the second half of the last word lies behind the end
+          if (tile * 128 + 128 >= p.N && (tile & 1) == 0) word[((k >> 5) & 3) + 2] = 0;
+        }
+      }
+    }
+  }
+}
+
 template <typename T, int BT, bool GATED>
-__global__ void __launch_bounds__(kThreads, BT == 128 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, 2)
 stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Params p) {
   using R = Ring<BT>;
   extern __shared__ uint8_t smem_raw[];
@@ -167,81 +249,10 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
   pair_sync();                         // all sums of the cluster are in place
   pdl_wait_prior();                    // y may still be read upstream
   const int tokens = p.T - m0 < BT ? p.T - m0 : BT;
-  if (!GATED) {
-    // four outputs a thread, over the parts of k in their order
-    for (int i = threadIdx.x + kThreads * rank; i < tokens * 32; i += kThreads * S) {
-      const int t = i >> 5, n = tile * 128 + (i & 31) * 4;
-      const uint8_t* src = ring + (size_t)i * 16;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      for (uint32_t s = 0; s < S; ++s) {
-        const uint4 q = ld_cluster_128(cluster_addr(src, s));
-        v[0] += __uint_as_float(q.x);
-        v[1] += __uint_as_float(q.y);
-        v[2] += __uint_as_float(q.z);
-        v[3] += __uint_as_float(q.w);
-      }
-      T* out = reinterpret_cast<T*>(p.y) + (int64_t)(m0 + t) * p.ldy + n;
-      const T* bias = reinterpret_cast<const T*>(p.bias);
-      if (bias)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.N) v[j] += to_f32(bias[n + j]);
-      if (p.vec && n < p.N) {          // N is a multiple of four
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.N) out[j] = from_f32<T>(v[j]);
-      }
-    }
-  } else {
-    // eight outputs a lane, four lanes a block, two blocks a tile: 64 gate rows, then their up rows
-    const int tasks = tokens * 8;
-    for (int base = (int)(threadIdx.x & ~31u) + kThreads * (int)rank; base < tasks; base += kThreads * (int)S) {
-      const int i = base + lane, t = i >> 3, e = (i & 7) * 8;
-      const bool in = i < tasks;
-      float g[8], u[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = u[j] = 0.f;
-      if (in) {
-        const uint8_t* src = ring + ((size_t)t * 128 + e) * 4;
-        for (uint32_t s = 0; s < S; ++s) {
-          const uint32_t a = cluster_addr(src, s);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 q = ld_cluster_128(a + 16 * h), r = ld_cluster_128(a + 256 + 16 * h);
-            g[4 * h] += __uint_as_float(q.x); g[4 * h + 1] += __uint_as_float(q.y);
-            g[4 * h + 2] += __uint_as_float(q.z); g[4 * h + 3] += __uint_as_float(q.w);
-            u[4 * h] += __uint_as_float(r.x); u[4 * h + 1] += __uint_as_float(r.y);
-            u[4 * h + 2] += __uint_as_float(r.z); u[4 * h + 3] += __uint_as_float(r.w);
-          }
-        }
-        if (p.bias) {
-          const T* bias = reinterpret_cast<const T*>(p.bias) + (int64_t)tile * 128 + e;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            g[j] += to_f32(bias[j]);
-            u[j] += to_f32(bias[64 + j]);
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = gated(g[j], u[j]);
-      uint32_t byte;
-      const uint32_t code = quantise8(g, byte);
-      if (in) {
-        const int64_t row = m0 + t;
-        const int k = tile * 64 + e;
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.y) + row * p.ldy + k / 2) = code;
-        if ((lane & 3) == 0) {
-          uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles);
-          word[(k >> 5) & 3] = (uint8_t)byte;
-          // an odd number of tiles: the second half of the last word lies behind the end
-          if (tile * 128 + 128 >= p.N && (tile & 1) == 0) word[((k >> 5) & 3) + 2] = 0;
-        }
-      }
-    }
-  }
+  if (S == 1) add_up<T, GATED, 1>(p, ring, tile, m0, tokens, rank);
+  else if (S == 2) add_up<T, GATED, 2>(p, ring, tile, m0, tokens, rank);
+  else if (S == 4) add_up<T, GATED, 4>(p, ring, tile, m0, tokens, rank);
+  else add_up<T, GATED, 8>(p, ring, tile, m0, tokens, rank);
   pair_sync();                         // the peers have read this CTA's sums
   if (warp == 1) {
     tc_fence_after();
@@ -249,11 +260,13 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
   }
 }
 
-// Parts of k: as many CTAs as keep every SM with two of them busy, each with two stages at least.
+// Parts of k: as many CTAs as keep every SM with two of them busy, two of two stages or more of four stages at least (one token,
+// 4096 x 4096, us: eight parts of two stages 5.1, four of four 4.1; 6144 x 4096 four 5.0, two 5.6, eight 8.5 in two waves; 4096 x 14336 eight 7.6,
+// four 8.2; 9728 x 896 two of two stages 3.7, one 3.9).
 static int parts(int64_t tiles, int num_kb) {
   const int64_t room = 2 * b2l_num_sms();
   int s = 1;
-  while (s < 8 && tiles * s * 2 <= room && num_kb >= 4 * s) s *= 2;
+  while (s < 8 && tiles * s * 2 <= room && num_kb >= (s == 1 ? 4 : 8 * s)) s *= 2;
   return s;
 }
 
