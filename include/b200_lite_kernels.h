@@ -326,7 +326,8 @@ int b2l_moe_route_topk(void* topk_weights, void* topk_ids_i64, const void* route
  * b2l_mxfp4_quantize / _dequantize: `matrices` stacked matrices of `rows` rows; fp16, bf16 or fp32.
  * b2l_skip_rmsnorm_mxfp4: sum = x + residual (sum may be residual; residual null: sum is not written), then the RMS norm of it
  * times weight, quantised; n <= 16384.
- * b2l_mxfp4_matmul: y[t, n] = x . w (+ bias), 16-bit; gated: silu(gate) * up quantised into y (codes, row stride in bytes)
+ * b2l_mxfp4_matmul: y[t, n] = x . w (+ bias), 16-bit; x_scales null (where b2l_mxfp4_matmul_takes_16bit says so): x holds elements of
+ * dtype, its stride counts them, and the product quantises them itself; gated: silu(gate) * up quantised into y (codes, row stride in bytes)
  * and y_scales, rows of w in runs of 64 gate and 64 up rows.  weights_ready: nothing still running writes w, so that it is requested
  * before the previous kernel has ended. */
 int64_t b2l_mxfp4_scale_bytes(int64_t rows, int64_t k);
@@ -337,6 +338,7 @@ int b2l_mxfp4_dequantize(void* y, const void* codes, const void* scales, int64_t
 int b2l_skip_rmsnorm_mxfp4(void* codes, void* scales, void* sum, const void* x, const void* residual, const void* weight,
                            int64_t rows, int64_t n, int64_t x_row_stride, int64_t r_row_stride, int64_t s_row_stride,
                            float eps, int dtype, void* stream);
+int64_t b2l_mxfp4_matmul_takes_16bit(int64_t t, int64_t n, int64_t k);
 int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w, const void* w_scales,
                      const void* bias, int64_t t, int64_t n, int64_t k, int64_t x_row_stride, int64_t w_row_stride,
                      int64_t y_row_stride, int gated, int weights_ready, int dtype, void* stream);

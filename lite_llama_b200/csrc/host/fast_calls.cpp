@@ -58,6 +58,7 @@ struct {
   int (*mx4_norm)(void*, void*, void*, const void*, const void*, const void*, i64, i64, i64, i64, i64, float, int, void*);
   int (*mx4_matmul)(void*, void*, const void*, const void*, const void*, const void*, const void*, i64, i64, i64, i64, i64, i64, int, int, int,
                     void*);
+  i64 (*mx4_takes_16bit)(i64, i64, i64);
   i64 (*mx4_tile_rows)(i64, int);
   i64 (*mx4_max_tiles)(i64, int, int);
   int (*mx4_sort)(void*, void*, const void*, int, i64, int, int, void*);
@@ -702,7 +703,7 @@ PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
   if (!mx4(a[1], 2, w)) return none();
   const at::Tensor *x = plain(a[0]), *bias = a[2] == Py_None ? w.codes : plain(a[2]);
   if (!x && !mx4(a[0], 2, q)) return none();
-  if (!abi.mx4_quantize || !abi.mx4_scale_bytes) return none();      // of a library that holds another file's functions alone
+  if (!abi.mx4_quantize || !abi.mx4_scale_bytes || !abi.mx4_takes_16bit) return none();      // of a library that holds another file's functions alone
   const int device = device_for(abi.mx4_matmul, {x ? x : q.codes, x ? x : q.scales, w.codes, w.scales, bias});
   if (device < 0 || (a[4] != Py_None && !THPDtype_Check(a[4])) || !PyBool_Check(a[3])) return none();
   const bool gated = a[3] == Py_True;
@@ -725,7 +726,12 @@ PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const Unlocked unlocked;
     const void *xc, *xs;
     void* st = stream(device);
-    if (x) {
+    i64 stride = k / 2;
+    if (x && abi.mx4_takes_16bit(t, n, k)) {
+      xc = x->data_ptr();
+      xs = nullptr;
+      stride = t > 1 ? x->stride(0) : k;
+    } else if (x) {
       const i64 at = up(t * k / 2, 256) * 256;
       held = fresh({at + abi.mx4_scale_bytes(t, k)}, at::kByte);
       xc = held.data_ptr();
@@ -740,7 +746,7 @@ PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (gated) ys = mx4_tiles(t, n / 2);
     if (!rc)
       rc = abi.mx4_matmul(y.data_ptr(), gated ? ys.data_ptr() : nullptr, xc, xs, w.codes->data_ptr(), w.scales->data_ptr(),
-                          bias == w.codes ? nullptr : bias->data_ptr(), t, n, k, k / 2, k / 2, gated ? n / 4 : n, gated ? 1 : 0, 1, code, st);
+                          bias == w.codes ? nullptr : bias->data_ptr(), t, n, k, stride, k / 2, gated ? n / 4 : n, gated ? 1 : 0, 1, code, st);
   }
   if (rc) return failed(rc);
   return gated ? pair_of(std::move(y), std::move(ys)) : THPVariable_Wrap(std::move(y));

@@ -87,6 +87,13 @@ __device__ __forceinline__ uint32_t block_max(uint32_t abs_bits) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// the largest magnitude; NaN if one of them is
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // pairs of 32-bit values (one instruction for both)
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair_of(float a, float b) {

@@ -23,23 +23,30 @@ struct Params {
   uint8_t* y_scales; int64_t y_ktiles;
   const void* bias;                    // [N] in the output's type, or null
   const uint8_t* x_scales; const uint8_t* w_scales;
+  const void* x16; int64_t ldx16;      // activations that the kernel quantises itself
   int64_t ktiles;                      // scale tiles along k
   int T, N, K, num_kb;
   int early;                           // weights may be requested before the previous kernel has ended
   int vec;                             // 8-byte stores of y
 };
 
-template <int BT> struct Ring {
+constexpr int kRawTokens = 8;          // activations that the kernel quantises itself: up to so many rows,
+constexpr int kRawStages = 24;         // so many stages of 256 k of a CTA's part
+
+template <int BT, bool RAW> struct Ring {
   static constexpr int kStages = BT == 128 ? 3 : 4;
-  static constexpr int kStage = 16384 + kSfBytes + BT * 128 + kSfBytes;   // W, its scales, X, its scales
+  static constexpr int kStage = 16384 + kSfBytes + (RAW ? 0 : BT * 128 + kSfBytes);   // W, its scales, X, its scales
+  // RAW: X of all stages stays, eight rows of 128 bytes each and for every scale tile eight rows of 16; the MMA's columns from 8 on read
+  // what follows, whatever it is, and are not looked at
+  static constexpr int kRaw = kStages * kStage, kRawScales = kRaw + (kRawStages + 3) * 1024;
   static constexpr int kX = 16384 + kSfBytes;
   static constexpr int kCols = BT + kStages * 16;                         // accumulator, then 16 columns of scales a stage
   static constexpr int kAlloc = kCols <= 128 ? 128 : 256;
-  static constexpr int kSmem = 1024 + 1024 + kStages * kStage;
+  static constexpr int kSmem = 1024 + 1024 + (RAW ? kRawScales + (2 * kRawStages + 3) * 128 : kStages * kStage);
 };
 
 struct __align__(8) Control {
-  uint64_t full[8], empty[8], done;
+  uint64_t full[8], empty[8], done, raw;
   uint32_t tmem;
 };
 
@@ -131,10 +138,38 @@ __device__ __forceinline__ void add_up(const Params& p, const uint8_t* sums, int
   }
 }
 
-template <typename T, int BT, bool GATED>
+// The rows of x in this CTA's part of k, quantised by the four warps that wait for the accumulator anyway: one launch less than with the quantiser
+// by itself, and the same codes (one token, 6144 x 4096, us on the device 5.8 -> 5.1, a call among others 8.1 -> 5.0).
+template <typename T, int BT>
+__device__ __forceinline__ void quantise_rows(const Params& p, uint8_t* ring, int kb0, int stages, int warp, int lane) {
+  using R = Ring<BT, true>;
+  const T* x = reinterpret_cast<const T*>(p.x16);
+  const int units = stages * p.T;
+#pragma unroll 1
+  for (int first = warp; first < units; first += 16) {           // four units of 256 k asked for together
+    Raw8<T> v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int u = first + 4 * i, t = u / stages, k = (kb0 + u - t * stages) * kStageK + lane * 8;
+      zero_raw(v[i]);
+      if (u < units && k < p.K) load_raw(x + t * p.ldx16 + k, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int u = first + 4 * i, t = u / stages, s = u - t * stages;
+      uint32_t byte;
+      const uint32_t code = quantise_raw(v[i], byte);
+      if (u >= units) break;                                     // whole warps
+      *reinterpret_cast<uint32_t*>(ring + R::kRaw + s * 1024 + t * 128 + (((lane >> 2) ^ t) << 4) + (lane & 3) * 4) = code;
+      if ((lane & 3) == 0) ring[R::kRawScales + (2 * s + (lane >> 4)) * 128 + t * 16 + ((lane >> 2) & 3)] = (uint8_t)byte;
+    }
+  }
+}
+
+template <typename T, int BT, bool GATED, bool RAW>
 __global__ void __launch_bounds__(kThreads, 2)
 stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Params p) {
-  using R = Ring<BT>;
+  using R = Ring<BT, RAW>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   Control* ctl = reinterpret_cast<Control*>(smem);
@@ -144,13 +179,14 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
   const int tile = blockIdx.x / S, m0 = blockIdx.y * BT;
   const int kb0 = (int)((int64_t)p.num_kb * rank / S), kb1 = (int)((int64_t)p.num_kb * (rank + 1) / S);
   if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmap_x);
+    if (!RAW) tma_prefetch_desc(&tmap_x);
     tma_prefetch_desc(&tmap_w);
     for (int s = 0; s < R::kStages; ++s) {
       mbar_init(&ctl->full[s], 1);
       mbar_init(&ctl->empty[s], 1);
     }
     mbar_init(&ctl->done, 1);
+    mbar_init(&ctl->raw, 128);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -170,11 +206,12 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
     auto sf_bytes = [&](int kb) { return (uint32_t)(2 * kb + 2 <= p.ktiles ? 2 : 1) * kTileBytes; };
     auto load_w = [&](int s, int kb) {
       uint8_t* st = ring + s * R::kStage;
-      mbar_arrive_expect_tx(&ctl->full[s], 16384 + BT * 128 + 2 * sf_bytes(kb));
+      mbar_arrive_expect_tx(&ctl->full[s], RAW ? 16384 + sf_bytes(kb) : 16384 + BT * 128 + 2 * sf_bytes(kb));
       tma_load_2d_hint(st, &tmap_w, kb * 128, tile * 128, &ctl->full[s], kEvictFirst);
       bulk_g2s(st + 16384, ws + (int64_t)2 * kb * kTileBytes, sf_bytes(kb), &ctl->full[s]);
     };
     auto load_x = [&](int s, int kb) {
+      if (RAW) return;
       uint8_t* st = ring + s * R::kStage + R::kX;
       tma_load_2d_hint(st, &tmap_x, kb * 128, m0, &ctl->full[s], kEvictLast);
       bulk_g2s(st + BT * 128, xs + (int64_t)2 * kb * kTileBytes, sf_bytes(kb), &ctl->full[s]);
@@ -203,20 +240,22 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
     // ===================== MMA issuer =====================
     const uint64_t desc0 = umma_desc_sw128_kmajor(smem_u32(ring)), sf0 = scale_desc(smem_u32(ring));
     gemm::PipeState ps(R::kStages);
+    if (RAW) mbar_wait(&ctl->raw, 0);
     for (int kb = kb0; kb < kb1; ++kb) {
       mbar_wait(&ctl->full[ps.stage], ps.phase);
       tc_fence_after();
       if (elect_one()) {
         const uint64_t base = (uint64_t)(ps.stage * R::kStage) >> 4;
-        const uint64_t wd = desc0 + base, xd = wd + (R::kX >> 4);
-        const uint64_t wsf = sf0 + base + (16384 >> 4), xsf = sf0 + base + ((R::kX + BT * 128) >> 4);
+        const uint64_t wd = desc0 + base, xd = RAW ? desc0 + ((R::kRaw + (kb - kb0) * 1024) >> 4) : wd + (R::kX >> 4);
+        const uint64_t wsf = sf0 + base + (16384 >> 4);
+        const uint64_t xsf = RAW ? sf0 + ((R::kRawScales + (kb - kb0) * 256) >> 4) : sf0 + base + ((R::kX + BT * 128) >> 4);
         const uint32_t sf = tmem + BT + ps.stage * 16;
         const int steps = (p.K - kb * kStageK + 63) >> 6;      // MMAs of 64 k that hold anything
         copy_scales<1>(sf, wsf);
         copy_scales<1>(sf + 8, xsf);
         if (steps > 2) {
           copy_scales<1>(sf + 4, wsf + (kTileBytes >> 4));
-          copy_scales<1>(sf + 12, xsf + (kTileBytes >> 4));
+          copy_scales<1>(sf + 12, xsf + ((RAW ? 128 : kTileBytes) >> 4));
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -233,6 +272,12 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
     // done covers every MMA, and with it every copy into the ring: its memory is free
     const int quad = warp & 3;
     float* part = reinterpret_cast<float*>(ring) + quad * 32 + lane;
+    if (RAW) {
+      pdl_wait_prior();
+      quantise_rows<T, BT>(p, ring, kb0, kb1 - kb0, quad, lane);
+      fence_proxy_async_smem();
+      mbar_arrive(&ctl->raw);
+    }
     mbar_wait(&ctl->done, 0);
     tc_fence_after();
 #pragma unroll 1
@@ -270,11 +315,12 @@ static int parts(int64_t tiles, int num_kb) {
   return s;
 }
 
-template <typename T, int BT, bool GATED>
+template <typename T, int BT, bool GATED, bool RAW>
 static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const Params& p, cudaStream_t st) {
-  auto kern = stream_kernel<T, BT, GATED>;
+  using R = Ring<BT, RAW>;
+  auto kern = stream_kernel<T, BT, GATED, RAW>;
   static int configured[64] = {0};
-  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, Ring<BT>::kSmem, configured));
+  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, R::kSmem, configured));
   const int64_t n_tiles = cdiv64(p.N, 128), m_tiles = cdiv64(p.T, BT);
   const int s = parts(n_tiles * m_tiles, p.num_kb);
   b2l_hang_arm(st);
@@ -282,7 +328,7 @@ static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const Params& p,
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)(n_tiles * s), (unsigned)m_tiles);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Ring<BT>::kSmem;
+  cfg.dynamicSmemBytes = R::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -301,11 +347,12 @@ template <typename T>
 static int stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const Params& p, bool gated, cudaStream_t st) {
   const int bt = p.T <= 32 ? 32 : (p.T <= 64 ? 64 : 128);
   CUtensorMap tx, tw;
-  int rc = b2l_make_tmap_2d(&tx, x, TMA_U8, (uint64_t)p.T, (uint64_t)p.K / 2, (uint64_t)x_stride, (uint32_t)bt, 128, true);
+  int rc = b2l_make_tmap_2d(&tw, w, TMA_U8, (uint64_t)p.N, (uint64_t)p.K / 2, (uint64_t)w_stride, 128, 128, true);
   if (rc != B2L_OK) return rc;
-  rc = b2l_make_tmap_2d(&tw, w, TMA_U8, (uint64_t)p.N, (uint64_t)p.K / 2, (uint64_t)w_stride, 128, 128, true);
+  if (p.x16) return gated ? launch<T, 32, true, true>(tw, tw, p, st) : launch<T, 32, false, true>(tw, tw, p, st);
+  rc = b2l_make_tmap_2d(&tx, x, TMA_U8, (uint64_t)p.T, (uint64_t)p.K / 2, (uint64_t)x_stride, (uint32_t)bt, 128, true);
   if (rc != B2L_OK) return rc;
-#define STREAM(BT) (gated ? launch<T, BT, true>(tx, tw, p, st) : launch<T, BT, false>(tx, tw, p, st))
+#define STREAM(BT) (gated ? launch<T, BT, true, false>(tx, tw, p, st) : launch<T, BT, false, false>(tx, tw, p, st))
   return bt == 32 ? STREAM(32) : (bt == 64 ? STREAM(64) : STREAM(128));
 #undef STREAM
 }
@@ -548,26 +595,37 @@ static int grouped_gemm(const void* x, const void* w, const GroupedParams& p, in
 
 }  // namespace mx4
 
+// whether the product quantises 16-bit activations itself
+extern "C" int64_t b2l_mxfp4_matmul_takes_16bit(int64_t t, int64_t n, int64_t k) {
+  if (t < 1 || t > mx4::kRawTokens || n < 1 || k < 1) return 0;
+  const int num_kb = (int)cdiv64(k, mx4::kStageK), s = mx4::parts(cdiv64(n, 128), num_kb);
+  return (num_kb + s - 1) / s <= mx4::kRawStages;
+}
+
 extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w, const void* w_scales,
                                 const void* bias, int64_t t, int64_t n, int64_t k, int64_t x_row_stride, int64_t w_row_stride,
                                 int64_t y_row_stride, int gated, int weights_ready, int dtype, void* stream) {
   B2L_REQUIRE(t >= 0 && n > 0 && k > 0 && k % 32 == 0 && t < (1ll << 30) && n < (1ll << 30) && k < (1ll << 30),
               "mxfp4_matmul: t=%lld n=%lld k=%lld (k a multiple of 32)", (long long)t, (long long)n, (long long)k);
   if (t == 0) return B2L_OK;
-  B2L_REQUIRE(y && x && x_scales && w && w_scales && (!gated || y_scales), "mxfp4_matmul: null pointer");
+  const bool raw = x_scales == nullptr;
+  B2L_REQUIRE(y && x && w && w_scales && (!gated || y_scales), "mxfp4_matmul: null pointer");
+  B2L_REQUIRE(!raw || b2l_mxfp4_matmul_takes_16bit(t, n, k), "mxfp4_matmul: %lld rows of 16-bit activations want the quantiser first", (long long)t);
   B2L_REQUIRE(!gated || n % 128 == 0, "mxfp4_matmul: gate and up rows come in runs of 64 (n=%lld)", (long long)n);
-  B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales) % 16 == 0 && (x_row_stride | w_row_stride) % 16 == 0 &&
-                  (!gated || ((uintptr_t)y % 4 == 0 && y_row_stride % 4 == 0)),
+  B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales) % 16 == 0 &&
+                  ((raw ? 2 * x_row_stride : x_row_stride) | w_row_stride) % 16 == 0 && (!gated || ((uintptr_t)y % 4 == 0 && y_row_stride % 4 == 0)),
               "mxfp4_matmul: rows of codes must start on 16 bytes");
   B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "mxfp4_matmul: dtype %d", dtype);
+  B2L_REQUIRE((cdiv64(t, 128) + cdiv64(n, 128)) * mx4::k_tiles(k) < (1ll << 29), "mxfp4_matmul: t=%lld n=%lld k=%lld", (long long)t, (long long)n, (long long)k);
   cudaStream_t st = (cudaStream_t)stream;
   mx4::PairCall g = {y, y_row_stride, y_scales, bias, x, x_scales, w, w_scales, t, n, k, x_row_stride, w_row_stride, gated != 0, weights_ready != 0};
-  if (mx4::pair_wanted(g)) return mx4::pair_gemm(g, dtype, st);
+  if (!raw && mx4::pair_wanted(g)) return mx4::pair_gemm(g, dtype, st);
   mx4::Params p;
   p.y = y; p.ldy = y_row_stride;
   p.y_scales = (uint8_t*)y_scales; p.y_ktiles = mx4::k_tiles(n / 2);
   p.bias = bias;
   p.x_scales = (const uint8_t*)x_scales; p.w_scales = (const uint8_t*)w_scales;
+  p.x16 = raw ? x : nullptr; p.ldx16 = x_row_stride;
   p.ktiles = mx4::k_tiles(k);
   p.T = (int)t; p.N = (int)n; p.K = (int)k; p.num_kb = (int)cdiv64(k, mx4::kStageK);
   p.early = weights_ready;

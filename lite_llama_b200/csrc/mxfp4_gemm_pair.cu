@@ -22,12 +22,12 @@ constexpr int kPairThreads = 10 * 32;  // TMA producer, MMA issuer, eight warps 
 constexpr int kPairRows = 128;         // tokens per CTA
 constexpr int kPairBand = 16;          // token tiles per band: 16 x 256 rows x 4096 / 2 bytes = 8 MiB of L2
 
-template <int BN, int CTAS> struct PairRing {
-  static constexpr int kStages = CTAS == 2 ? 5 : 3;
+template <int BN, int CTAS, bool GATED> struct PairRing {
+  static constexpr int kStages = CTAS == 2 ? (GATED ? 6 : 5) : (GATED ? 4 : 3);
   static constexpr int kX = 16384, kW = BN / CTAS * 128;
   static constexpr int kXs = kX + kW, kWs = kXs + kSfBytes;
   static constexpr int kBytes = kWs + BN / 128 * kSfBytes;
-  static constexpr int kSmem = 1024 + 1024 + kStages * kBytes + 8 * 4096;
+  static constexpr int kSmem = 1024 + 1024 + kStages * kBytes + (GATED ? 0 : 8 * 4096);
   static constexpr int kAcc1 = BN == 256 ? 208 : 128;                     // first column of the second accumulator
   static constexpr int kSf = BN == 256 ? 464 : 256;
   static constexpr int kSfSet = 8 + BN / 128 * 8;
@@ -42,8 +42,8 @@ struct PairParams {
 };
 
 struct __align__(8) PairControl {
-  uint64_t full[5];                    // leader: both CTAs' operands and scales of a stage have landed
-  uint64_t empty[5];                   // both: the MMAs of a stage have retired
+  uint64_t full[6];                    // leader: both CTAs' operands and scales of a stage have landed
+  uint64_t empty[6];                   // both: the MMAs of a stage have retired
   uint64_t acc_full[2];                // both: a tile's accumulator is complete
   uint64_t freed[2];                   // leader: all warps have read what the next tile's products overwrite
   uint32_t tmem;
@@ -51,10 +51,10 @@ struct __align__(8) PairControl {
 
 // 32 values of one row: scale byte and codes
 __device__ __forceinline__ uint32_t quantise32(float (&v)[32], uint4& codes) {
-  uint32_t m = 0;
+  float m = 0.f;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) m = max(m, abs_bits(v[j]));
-  const uint32_t byte = scale_byte(m);
+  for (int j = 0; j < 32; j += 2) m = max_abs(m, v[j], v[j + 1]);
+  const uint32_t byte = scale_byte(abs_bits(m));
   const float inv = inverse_scale(byte);
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] *= inv;
@@ -101,7 +101,7 @@ template <typename T, int BN, bool GATED, int CTAS>
 __global__ void __launch_bounds__(kPairThreads, 1)
 pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_xs,
             const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_y, const PairParams p) {
-  using R = PairRing<BN, CTAS>;
+  using R = PairRing<BN, CTAS, GATED>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   PairControl* ctl = reinterpret_cast<PairControl*>(smem);
@@ -276,16 +276,21 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           if (n0 >= p.N || !any) continue;
           if (lane == 0) bulk_wait_read<0>();           // the store before has read the box
           __syncwarp();
+          if (p.bias) {                                 // a branch of its own: without a bias nothing of it is issued
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const int n = n0 + 8 * q;                 // N is a multiple of 8
+              const uint4 b4 = n < p.N ? ldg_128(reinterpret_cast<const T*>(p.bias) + n) : make_uint4(0u, 0u, 0u, 0u);
+              const T* b = reinterpret_cast<const T*>(&b4);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[8 * q + e] = __float_as_uint(__uint_as_float(v[8 * q + e]) + to_f32(b[e]));
+            }
+          }
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             uint32_t o[4];
-            const int n = n0 + 8 * q;
-            uint4 b4 = make_uint4(0u, 0u, 0u, 0u);
-            if (p.bias && n < p.N) b4 = ldg_128(reinterpret_cast<const T*>(p.bias) + n);      // N is a multiple of 8
-            const T* b = reinterpret_cast<const T*>(&b4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              o[e] = pack2<T>(__uint_as_float(v[8 * q + 2 * e]) + to_f32(b[2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]) + to_f32(b[2 * e + 1]));
+            for (int e = 0; e < 4; ++e) o[e] = pack2<T>(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
             *reinterpret_cast<uint4*>(dst + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
           }
           fence_proxy_async_smem();
@@ -317,16 +322,21 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           tc_wait_ld();
           if (BN != 256) hand_on(buf);
           const int n = n0 + (BN == 256 ? 32 * h : 32 * half);      // the block's gate rows
-          float v[32];
+          float v[32], u[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            float g = __uint_as_float(up_first ? other[e] : held[32 * h + e]), u = __uint_as_float(up_first ? held[32 * h + e] : other[e]);
-            if (p.bias && n < p.N) {
-              g += to_f32(reinterpret_cast<const T*>(p.bias)[n + e]);
-              u += to_f32(reinterpret_cast<const T*>(p.bias)[n + 64 + e]);
-            }
-            v[e] = gated(g, u);
+            v[e] = __uint_as_float(up_first ? other[e] : held[32 * h + e]);
+            u[e] = __uint_as_float(up_first ? held[32 * h + e] : other[e]);
           }
+          if (p.bias && n < p.N) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              v[e] += to_f32(reinterpret_cast<const T*>(p.bias)[n + e]);
+              u[e] += to_f32(reinterpret_cast<const T*>(p.bias)[n + 64 + e]);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = gated(v[e], u[e]);
           bytes |= quantise32(v, codes[h]) << (8 * h);
         }
         if (n0 < p.N && quad * 32 + lane < wk.rows) {   // N is a multiple of 128
@@ -359,7 +369,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
 // Maps and launch, for `rows` rows of x and y in tiles of 128 and `weight_rows` rows of w
 template <typename T, int BN, bool GATED, int CTAS>
 static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t experts, int64_t tiles, cudaStream_t st) {
-  using R = PairRing<BN, CTAS>;
+  using R = PairRing<BN, CTAS, GATED>;
   const int sms = b2l_num_sms();
   p.bias = g.bias;
   p.y = (uint8_t*)g.y; p.y_scales = (uint8_t*)g.y_scales; p.ldy = g.ldy; p.y_ktiles = k_tiles(g.N / 2);
@@ -409,8 +419,11 @@ static int launch_pair(const PairCall& g, cudaStream_t st) {
   return launch_rows<T, BN, GATED, 2>(g, p, g.T, 1, p.m_tiles, st);
 }
 
+// Up to 128 tokens half of a pair's rows are padding, and the streaming kernel is as fast or faster (65 - 128 tokens, us, streaming / pairs:
+// 28672 x 4096 14.0 - 15.2 / 16.7, 4096 x 14336 13.1 / 17.6; 2048 x 2048 5.5 / 5.2).  With few tiles and a long k it parts k over more SMs, up to 256
+// tokens: 256 x 4096 x 14336 14.3 / 17.7, 200 x 896 x 4864 6.6 / 7.8; but 256 x 4096 x 4096 9.4 / 8.1, 400 x 4096 x 14336 18.5 / 18.4.
 bool pair_wanted(const PairCall& g) {
-  if (g.T <= 128) return false;
+  if (g.T <= 128 || (g.T <= 256 && cdiv64(g.N, 128) * 4 <= b2l_num_sms() && g.K > 16 * kStageK)) return false;
   return g.gated ? (uintptr_t)g.y % 16 == 0 && g.ldy % 16 == 0
                  : g.N % 8 == 0 && g.ldy % 8 == 0 && (uintptr_t)g.y % 16 == 0 && (uintptr_t)g.bias % 16 == 0;
 }

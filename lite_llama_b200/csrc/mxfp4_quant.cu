@@ -122,13 +122,6 @@ static int units_of(int64_t rows, int64_t k) { return rows * cdiv64(k, 256) < 12
 // wider margins and rows with a doubtful block added up again by their CTA, 18.5 so; 17.8 without any decision in 64 bits.
 // Two chunks a thread 18.5, four 19.0, one 22.3.
 // ---------------------------------------------------------------------------------------------------------------
-// the larger magnitude; NaN if one of them is
-__device__ __forceinline__ float max_abs(float a, float b, float c) {
-  float r;
-  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
 template <typename T, int VPT>
 __global__ void __launch_bounds__(512, 2)
 norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, T* sum, const T* __restrict__ x, const T* res,

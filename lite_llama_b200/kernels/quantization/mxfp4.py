@@ -245,13 +245,19 @@ def _mxfp4_matmul(x, w, bias, swiglu, out_dtype) -> torch.Tensor | MXFP4:
         dtype, lead = x.dtype, x.shape[:-1]
         if x.shape[-1] != w.k:
             raise ValueError(f"x has {x.shape[-1]} cols but weight expects {w.k}")
-        x = mxfp4_quantize(as_rows(x) if x.dim() != 2 else x)
+        x = _aligned(as_rows(x))
+        if not lib().b2l_mxfp4_matmul_takes_16bit(x.shape[0], w.rows, w.k):
+            x = mxfp4_quantize(x)
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"mxfp4_matmul: unsupported output dtype {dtype}")
-    if x.k != w.k:
-        raise ValueError(f"x has {x.k} cols but weight expects {w.k}")
-    _together("mxfp4_matmul", x.codes, w.codes, bias)
-    n, t = w.rows, x.rows
+    if isinstance(x, MXFP4):
+        if x.k != w.k:
+            raise ValueError(f"x has {x.k} cols but weight expects {w.k}")
+        xc, xs, t, stride = x.codes, x.scales, x.rows, w.k // 2
+    else:                                                 # few rows: the product quantises them itself
+        xc, xs, t, stride = x, None, x.shape[0], _row_stride(x)
+    _together("mxfp4_matmul", xc, w.codes, bias)
+    n = w.rows
     if swiglu and n % (2 * GATE_RUN) != 0:
         raise ValueError(f"mxfp4_matmul: gate and up rows come in runs of {GATE_RUN}, got {n} rows")
     if bias is not None:
@@ -267,9 +273,8 @@ def _mxfp4_matmul(x, w, bias, swiglu, out_dtype) -> torch.Tensor | MXFP4:
         else:
             y, ys = torch.empty((t, n), dtype=dtype, device=w.device), None
         code = {torch.float16: 0, torch.bfloat16: 1}[dtype]
-        check(lib().b2l_mxfp4_matmul(y.data_ptr(), ptr(ys), x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(),
-                                     w.scales.data_ptr(), ptr(bias), t, n, w.k, w.k // 2, w.k // 2, y.shape[1], int(swiglu), 1, code,
-                                     stream_handle()))
+        check(lib().b2l_mxfp4_matmul(y.data_ptr(), ptr(ys), xc.data_ptr(), ptr(xs), w.codes.data_ptr(), w.scales.data_ptr(), ptr(bias), t, n,
+                                     w.k, stride, w.k // 2, y.shape[1], int(swiglu), 1, code, stream_handle()))
     if swiglu:
         return MXFP4(y, ys, ready=False)
     return y if lead is None or len(lead) == 1 else y.view(*lead, n)

@@ -152,7 +152,7 @@ def weights(n, k, spread=0.02):
                                    (65, 640, 992), (128, 129, 4096), (100, 1000, 352),
                                    # pairs: one tile, both widths, ragged edges, several tiles to a pair; what they leave (odd n)
                                    (129, 8, 32), (256, 256, 256), (200, 264, 96), (385, 1000, 736), (300, 20488, 256), (1000, 9000, 1312),
-                                   (2048, 4096, 512), (140, 131, 256), (300, 33, 1024)))
+                                   (2048, 4096, 512), (140, 131, 256), (300, 33, 1024), (256, 1200, 8192), (150, 40, 4384)))
 def test_products_of_whole_numbers_are_exact(t, n, k):
     """Elements and scales whose products add up to whole numbers below 2^11: any order of exact sums gives the same bits, and one
     element, scale, row or block in a wrong place gives others."""
@@ -182,6 +182,22 @@ def test_products_against_64_bits(dtype, t, n, k, with_bias):
     bound = O.product_bound(xv, wv, want + (0 if b is None else b.double()), dtype)
     want = want if b is None else want + b.double()
     assert y.dtype == dtype and ((y.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t", (1, 2, 5, 8, 9))
+@pytest.mark.parametrize("n,k", ((128, 32), (384, 96), (256, 4096), (6144, 4096), (4096, 14336), (19200, 6144), (19200, 6400), (130, 992)))
+def test_activations_in_16_bits_give_the_quantised_ones_bits(dtype, t, n, k):
+    """Few rows are quantised inside the product: the codes are those of the quantiser, the sums are in the same order."""
+    wide = torch.randn(t, k + 64, device="cuda").to(dtype)
+    wide[0, 8] = float("nan")
+    w, _ = weights(n, k)
+    for x in (wide[:, :k], wide[:, 16:16 + k], wide[:, 3:3 + k]):
+        want = K.mxfp4_matmul(K.mxfp4_quantize(x), w, out_dtype=dtype)
+        assert torch.equal(K.mxfp4_matmul(x, w).view(torch.int16), want.view(torch.int16))
+        if n % 128 == 0:
+            a, b = K.mxfp4_matmul(K.mxfp4_quantize(x), w, swiglu=True, out_dtype=dtype), K.mxfp4_matmul(x, w, swiglu=True)
+            same_codes(a, (O.unpack_codes(b.codes), O.scale_rows(b.scales, b.rows, b.k)))
 
 
 # ------------------------------------------------------------------------------------------------- the gated feed-forward
