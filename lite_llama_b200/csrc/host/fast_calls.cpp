@@ -788,8 +788,7 @@ PyObject* mx4_moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
     out = fresh({tokens, hidden}, x->scalar_type());
     char* p = (char*)held.data_ptr();
     void* st = stream(device);
-    if (!w1.ready || !w2.ready) rc = abi.weights_written(st);
-    if (!rc) rc = abi.mx4_sort(p + place, p + table, ids->data_ptr(), width, slots, tile, e, st);
+    rc = abi.mx4_sort(p + place, p + table, ids->data_ptr(), width, slots, tile, e, st);
     if (!rc) rc = abi.mx4_scatter(p + xc, p + xs, x->data_ptr(), p + place, tokens, top_k, tile, hidden, x->stride(0), code, st);
     if (!rc)
       rc = abi.mx4_grouped(p + ac, p + as, p + xc, p + xs, w1.codes->data_ptr(), w1.scales->data_ptr(), p + table, tiles, tile, e, w1.rows, hidden, 1,

@@ -430,9 +430,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   if (warp == 0) {
     // ===================== TMA producer =====================
     gemm::PipeState ps(R::kStages);
+    int next = (int)blockIdx.x < items ? ld_upstream(p.table + 1 + 2 * (blockIdx.x / p.n_tiles)) : 0;
     for (int it = blockIdx.x; it < items; it += gridDim.x) {
       const int tile = it / p.n_tiles, nt = it - tile * p.n_tiles;
-      const int expert = ld_upstream(p.table + 1 + 2 * tile);
+      const int expert = next;
+      if (it + (int)gridDim.x < items) next = ld_upstream(p.table + 1 + 2 * ((it + gridDim.x) / p.n_tiles));      // a tile ahead
       const int64_t w_tile = (int64_t)expert * p.n_tiles + nt;
       const uint8_t* ws = p.w_scales + w_tile * p.ktiles * kTileBytes;
       const uint8_t* xs = p.x_scales + (int64_t)tile * p.ktiles * kTileBytes;
@@ -495,9 +497,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     const int quad = warp & 3, tid = quad * 32 + lane;
     float* mine = out_stage + quad * 32 + lane;
     int turn = 0;
+    int next = (int)blockIdx.x < items ? ld_upstream(p.table + 2 + 2 * (blockIdx.x / p.n_tiles)) : 0;
     for (int it = blockIdx.x; it < items; it += gridDim.x, ++turn) {
       const int tile = it / p.n_tiles, nt = it - tile * p.n_tiles, buf = turn & 1;
-      const int rows = ld_upstream(p.table + 2 + 2 * tile);
+      const int rows = next;
+      if (it + (int)gridDim.x < items) next = ld_upstream(p.table + 2 + 2 * ((it + gridDim.x) / p.n_tiles));
       mbar_wait(&ctl->acc_full[buf], (turn >> 1) & 1);
       tc_fence_after();
 #pragma unroll 1

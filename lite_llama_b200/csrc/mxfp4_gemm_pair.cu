@@ -168,8 +168,10 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       __syncwarp();
     }
     pdl_wait_prior();
+    Work next = pair < tiles ? work_of<CTAS>(p, pair, (int)rank) : Work{0, 0, 0, 0};
     for (int t = pair; t < tiles; t += pairs) {
-      const Work wk = work_of<CTAS>(p, t, (int)rank);
+      const Work wk = next;
+      if (t + pairs < tiles) next = work_of<CTAS>(p, t + pairs, (int)rank);      // table entries are asked for a tile ahead
 #pragma unroll 1
       for (int kb = 0; kb < p.num_kb; ++kb) {
         mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
@@ -252,15 +254,17 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     pdl_wait_prior();                  // y may still be read upstream
     uint8_t* dst = out_stage + (quad + 4 * half) * 4096;
     int it = 0;
+    Work next = pair < tiles ? work_of<CTAS>(p, pair, (int)rank) : Work{0, 0, 0, 0};
     for (int t = pair; t < tiles; t += pairs, ++it) {
-      const Work wk = work_of<CTAS>(p, t, (int)rank);
+      const Work wk = next;
+      if (t + pairs < tiles) next = work_of<CTAS>(p, t + pairs, (int)rank);
       const int buf = it & 1, m_warp = wk.m * kPairRows + quad * 32;
       const bool any = quad * 32 < wk.rows;             // uniform over the warp
       const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * R::kAcc1;
       // the columns that both accumulators have: the first one's last, read by the second half's warps, the second one's first.  The other
       // half's warps are done with the tile before, which is what their arrival says.
       const bool shared = BN == 256 && half == 1 - buf;
-      mbar_wait_spin(&ctl->acc_full[buf], (it >> 1) & 1);
+      mbar_wait(&ctl->acc_full[buf], (it >> 1) & 1);
       tc_fence_after();
       if (BN == 256 && !shared) hand_on(buf);
       if (!GATED) {

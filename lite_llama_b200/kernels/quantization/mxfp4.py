@@ -324,9 +324,6 @@ def _fused_moe_mxfp4(hidden_states, w1, w2, topk_weights, topk_ids) -> torch.Ten
         L, dev, st = lib(), x.device, stream_handle()
         tile = L.b2l_mxfp4_moe_tile_rows(slots, experts)
         tiles = L.b2l_mxfp4_moe_max_tiles(slots, tile, experts)
-        if not (w1.ready and w2.ready):
-            weights_written()
-
         def buffer(*shape):
             return torch.empty(shape, dtype=torch.uint8, device=dev)
 
