@@ -298,7 +298,7 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
   else if (S == 2) add_up<T, GATED, 2>(p, ring, tile, m0, tokens, rank);
   else if (S == 4) add_up<T, GATED, 4>(p, ring, tile, m0, tokens, rank);
   else add_up<T, GATED, 8>(p, ring, tile, m0, tokens, rank);
-  pair_sync();                         // the peers have read this CTA's sums
+  pair_sync_relaxed();                 // the peers have read this CTA's sums
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, R::kAlloc);

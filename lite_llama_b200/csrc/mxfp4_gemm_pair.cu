@@ -67,7 +67,7 @@ __device__ __forceinline__ uint32_t quantise32(float (&v)[32], uint4& codes) {
 
 // What differs between a pair and a single CTA
 template <int CTAS> __device__ __forceinline__ void sync_all() {
-  if (CTAS == 2) pair_sync();
+  if (CTAS == 2) pair_sync_relaxed();
   else __syncthreads();
 }
 template <int CTAS> __device__ __forceinline__ void load_2d(void* dst, const void* map, int c0, int c1, uint64_t* bar) {
@@ -359,7 +359,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
         }
       }
     }
-    if (!GATED && lane == 0) bulk_wait_all();
+    if (!GATED && lane == 0) bulk_wait_read<0>();       // the boxes have been read; the stores end with the kernel
   }
 
   tc_fence_before();

@@ -27,6 +27,12 @@ __device__ __forceinline__ uint32_t leader_addr(const void* p) {
 __device__ __forceinline__ void pair_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same without a release: for what needs no ordinary store to be seen (barriers initialised behind mbar_fence_init, tensor memory, peers
+// that have read their last word of this CTA's shared memory).  A release waits for the CTA's stores to global memory, 1500 cycles at
+// the end of a kernel.
+__device__ __forceinline__ void pair_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // Arrival on a barrier of either CTA.  What the pair's barriers order is tensor memory (by the tcgen05 fences around them)
 // and shared memory written by the TMA unit, never ordinary stores, so neither side asks for cluster-scope release or
 // acquire: with them every hand-off cost microseconds (quantised pair GEMM, 4096 x 28672 x 4096: 1802 us, without: 977 us).
