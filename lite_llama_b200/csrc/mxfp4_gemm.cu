@@ -7,8 +7,10 @@
 // Bound: with few tokens the weights (17/32 bytes an element) are what streams.  128 weight rows are the rows of the MMA (they are
 // most of the bytes), 32, 64 or 128 tokens its columns, so the tensor pipe is idle nearly always and the kernel is a ring of TMA copies: a CTA has
 // four stages of 256 k (90 - 105 KiB) in flight and two CTAs share an SM.  A tile whose n leaves SMs idle is parted along k
-// over a cluster of 2, 4 or 8 CTAs, which leave their sums in shared memory and add them up there, each a share of the tile, in
-// the order of the parts: nothing outlives the launch, so calls on several streams and captured graphs share nothing.
+// over a cluster of 2, 4 or 8 CTAs, whose sums are added up in shared memory in the order of the parts: nothing outlives the
+// launch, so calls on several streams and captured graphs share nothing.  Up to 32 tokens every CTA sends its sums of a token to the CTA that
+// owns it (st.async, counted by the owner's barrier), which is one way through the cluster; with more they lie where they are, between
+// two barriers of the cluster, and each CTA fetches a share of the tile (one token, 4096 x 4096, us: 3.6 that way, 3.3 so).
 #include "gemm_tc.cuh"
 #include "mxfp4_mma.cuh"
 #include "mxfp4_gemm.cuh"
@@ -40,13 +42,16 @@ template <int BT, bool RAW> struct Ring {
   // what follows, whatever it is, and are not looked at
   static constexpr int kRaw = kStages * kStage, kRawScales = kRaw + (kRawStages + 3) * 1024;
   static constexpr int kX = 16384 + kSfBytes;
+  // Up to 32 tokens: [token of this CTA][part of k][128] sums
+  static constexpr int kSums = RAW ? kRawScales + (2 * kRawStages + 3) * 128 : kStages * kStage;
+  static constexpr int kSumBytes = BT == 32 ? (RAW ? kRawTokens : 32) * 512 : 0;
   static constexpr int kCols = BT + kStages * 16;                         // accumulator, then 16 columns of scales a stage
   static constexpr int kAlloc = kCols <= 128 ? 128 : 256;
-  static constexpr int kSmem = 1024 + 1024 + (RAW ? kRawScales + (2 * kRawStages + 3) * 128 : kStages * kStage);
+  static constexpr int kSmem = 1024 + 1024 + kSums + kSumBytes;
 };
 
 struct __align__(8) Control {
-  uint64_t full[8], empty[8], done, raw;
+  uint64_t full[8], empty[8], done, raw, sums;
   uint32_t tmem;
 };
 
@@ -54,6 +59,46 @@ __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
   return r;
+}
+
+// Four outputs of a token from their sums
+template <typename T> __device__ __forceinline__ void store4(const Params& p, int64_t row, int n, float (&v)[4]) {
+  T* out = reinterpret_cast<T*>(p.y) + row * p.ldy + n;
+  const T* bias = reinterpret_cast<const T*>(p.bias);
+  if (bias)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < p.N) v[j] += to_f32(bias[n + j]);
+  if (p.vec && n < p.N) {              // N is a multiple of four
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < p.N) out[j] = from_f32<T>(v[j]);
+  }
+}
+// Four activations of a token from the sums of their gate and up rows, e to e + 3 of the tile's 64; eight lanes hold a block (whole warps)
+template <typename T>
+__device__ __forceinline__ void store_unit4(const Params& p, bool in, int64_t row, int tile, int e, float (&g)[4], float (&u)[4], int lane) {
+  if (in && p.bias) {
+    const T* bias = reinterpret_cast<const T*>(p.bias) + (int64_t)tile * 128 + e;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      g[j] += to_f32(bias[j]);
+      u[j] += to_f32(bias[64 + j]);
+    }
+  }
+  uint32_t byte;
+  const uint32_t code = quantise4(gated(g[0], u[0]), gated(g[1], u[1]), gated(g[2], u[2]), gated(g[3], u[3]), byte);
+  if (!in) return;
+  const int k = tile * 64 + e;
+  *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p.y) + row * p.ldy + k / 2) = (uint16_t)code;
+  if ((lane & 7) == 0) {
+    uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles);
+    word[(k >> 5) & 3] = (uint8_t)byte;
+    // an odd number of tiles: the second half of the last word lies behind the end
+    if (tile * 128 + 128 >= p.N && (tile & 1) == 0) word[((k >> 5) & 3) + 2] = 0;
+  }
 }
 
 // This CTA's share of a tile: sums over the S parts of k in their order, all parts of an output asked for together (one after another
@@ -79,19 +124,7 @@ __device__ __forceinline__ void add_up(const Params& p, const uint8_t* sums, int
         v[2] += __uint_as_float(q[s].z);
         v[3] += __uint_as_float(q[s].w);
       }
-      T* out = reinterpret_cast<T*>(p.y) + (int64_t)(m0 + t) * p.ldy + n;
-      const T* bias = reinterpret_cast<const T*>(p.bias);
-      if (bias)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.N) v[j] += to_f32(bias[n + j]);
-      if (p.vec && n < p.N) {          // N is a multiple of four
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.N) out[j] = from_f32<T>(v[j]);
-      }
+      store4<T>(p, m0 + t, n, v);
     }
   } else {
     // four activations a lane, eight lanes a block, two blocks a tile: 64 gate rows, then their up rows
@@ -112,30 +145,73 @@ __device__ __forceinline__ void add_up(const Params& p, const uint8_t* sums, int
           g[0] += __uint_as_float(q[s].x); g[1] += __uint_as_float(q[s].y); g[2] += __uint_as_float(q[s].z); g[3] += __uint_as_float(q[s].w);
           u[0] += __uint_as_float(r[s].x); u[1] += __uint_as_float(r[s].y); u[2] += __uint_as_float(r[s].z); u[3] += __uint_as_float(r[s].w);
         }
-        if (p.bias) {
-          const T* bias = reinterpret_cast<const T*>(p.bias) + (int64_t)tile * 128 + e;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            g[j] += to_f32(bias[j]);
-            u[j] += to_f32(bias[64 + j]);
-          }
-        }
       }
-      uint32_t byte;
-      const uint32_t code = quantise4(gated(g[0], u[0]), gated(g[1], u[1]), gated(g[2], u[2]), gated(g[3], u[3]), byte);
-      if (in) {
-        const int64_t row = m0 + t;
-        const int k = tile * 64 + e;
-        *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p.y) + row * p.ldy + k / 2) = (uint16_t)code;
-        if ((lane & 7) == 0) {
-          uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles);
-          word[(k >> 5) & 3] = (uint8_t)byte;
-          // an odd number of tiles: the second half of the last word lies behind the end
-          if (tile * 128 + 128 >= p.N && (tile & 1) == 0) word[((k >> 5) & 3) + 2] = 0;
-        }
-      }
+      store_unit4<T>(p, in, m0 + t, tile, e, g, u, lane);
     }
   }
+}
+
+// The tokens rank, rank + S, ... of a tile from their parts, [token][part][128] in this CTA: as add_up, by the 128 threads of four warps.
+template <typename T, bool GATED, int S>
+__device__ __forceinline__ void add_own(const Params& p, const float* sums, int tile, int rank, int tid) {
+  const int lane = tid & 31, owned = p.T > rank ? (p.T - rank + S - 1) / S : 0;
+  if (!GATED) {
+    for (int i = tid; i < owned * 32; i += 128) {
+      const int slot = i >> 5, n = tile * 128 + (i & 31) * 4;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const float4 q = *reinterpret_cast<const float4*>(sums + (slot * S + s) * 128 + (i & 31) * 4);
+        v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+      }
+      store4<T>(p, rank + slot * S, n, v);
+    }
+  } else {
+    const int tasks = owned * 16;
+    for (int first = tid & ~31; first < tasks; first += 128) {
+      const int i = first + lane, slot = i >> 4, e = (i & 15) * 4;
+      float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+      if (i < tasks) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const float* src = sums + (slot * S + s) * 128 + e;
+          const float4 q = *reinterpret_cast<const float4*>(src), r = *reinterpret_cast<const float4*>(src + 64);
+          g[0] += q.x; g[1] += q.y; g[2] += q.z; g[3] += q.w;
+          u[0] += r.x; u[1] += r.y; u[2] += r.z; u[3] += r.w;
+        }
+      }
+      store_unit4<T>(p, i < tasks, rank + slot * S, tile, e, g, u, lane);
+    }
+  }
+}
+
+__device__ __forceinline__ void send_f32(uint32_t to, float v, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to), "r"(__float_as_uint(v)), "r"(bar) : "memory");
+}
+
+// A thread's output row over all tokens, each to the CTA that owns the token; then this CTA's tokens.
+template <typename T, bool GATED, int S>
+__device__ __forceinline__ void send_and_add(const Params& p, const uint32_t (&v)[32], float* sums, uint64_t* bar, int tile, int rank, int tid) {
+  if (S == 1) {
+#pragma unroll
+    for (int t = 0; t < 32; ++t)
+      if (t < p.T) sums[t * 128 + tid] = __uint_as_float(v[t]);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+  } else {
+    uint32_t to[S], done[S];
+#pragma unroll
+    for (int c = 0; c < S; ++c) {
+      to[c] = cluster_addr(sums, (uint32_t)c) + (rank * 128 + tid) * 4;
+      done[c] = cluster_addr(bar, (uint32_t)c);
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");        // every CTA of the cluster runs and expects its sums
+#pragma unroll
+    for (int t = 0; t < 32; ++t)
+      if (t < p.T) send_f32(to[t % S] + (t / S) * S * 512, __uint_as_float(v[t]), done[t % S]);
+    if (rank < p.T) mbar_wait(bar, 0);
+  }
+  pdl_wait_prior();                    // y may still be read upstream
+  add_own<T, GATED, S>(p, sums, tile, rank, tid);
 }
 
 // The rows of x in this CTA's part of k, quantised by the four warps that wait for the accumulator anyway: one launch less than with the quantiser
@@ -187,8 +263,12 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
     }
     mbar_init(&ctl->done, 1);
     mbar_init(&ctl->raw, 128);
+    mbar_init(&ctl->sums, 1);
     mbar_fence_init();
+    if (BT == 32 && S > 1 && (int)rank < p.T) mbar_arrive_expect_tx(&ctl->sums, (p.T - rank + S - 1) / S * S * 512);
   }
+  __syncwarp();
+  if (BT == 32 && S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // waited for before the sums travel
   if (warp == 1) {
     tmem_alloc(&ctl->tmem, R::kAlloc);
     tmem_relinquish();
@@ -280,8 +360,19 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
     }
     mbar_wait(&ctl->done, 0);
     tc_fence_after();
+    if constexpr (BT == 32) {
+      uint32_t v[32];
+      tmem_ld_32x32b_x32(tmem + ((uint32_t)(quad * 32) << 16), v);
+      tc_wait_ld();
+      float* sums = reinterpret_cast<float*>(ring + R::kSums);
+      const int tid = quad * 32 + lane;
+      if (S == 1) send_and_add<T, GATED, 1>(p, v, sums, &ctl->sums, tile, (int)rank, tid);
+      else if (S == 2) send_and_add<T, GATED, 2>(p, v, sums, &ctl->sums, tile, (int)rank, tid);
+      else if (S == 4) send_and_add<T, GATED, 4>(p, v, sums, &ctl->sums, tile, (int)rank, tid);
+      else send_and_add<T, GATED, 8>(p, v, sums, &ctl->sums, tile, (int)rank, tid);
+    }
 #pragma unroll 1
-    for (int c = 0; c < BT; c += 32) {
+    for (int c = 0; BT != 32 && c < BT; c += 32) {
       if (m0 + c >= p.T) break;
       uint32_t v[32];
       tmem_ld_32x32b_x32(tmem + ((uint32_t)(quad * 32) << 16) + c, v);
@@ -291,6 +382,15 @@ stream_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
     }
   }
   tc_fence_before();
+  if (BT == 32) {
+    if (warp < 2 && S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncthreads();                   // the accumulator has been read
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, R::kAlloc);
+    }
+    return;
+  }
   pair_sync();                         // all sums of the cluster are in place
   pdl_wait_prior();                    // y may still be read upstream
   const int tokens = p.T - m0 < BT ? p.T - m0 : BT;

@@ -168,6 +168,26 @@ def test_products_of_whole_numbers_are_exact(t, n, k):
         assert torch.equal(K.mxfp4_matmul(x, w, out_dtype=dtype), want.to(dtype))
 
 
+@pytest.mark.parametrize("k", (512, 1024, 4096, 8192))
+@pytest.mark.parametrize("n", (256, 200))
+def test_every_number_of_tokens_that_shares_its_sums(n, k):
+    """One to eight parts of k, by any number of tokens: which CTA of a cluster adds up a token follows from both."""
+    gen = torch.Generator(device="cuda").manual_seed(n + k)
+    few = lambda rows: torch.where(torch.rand(rows, k, device="cuda", generator=gen) < 16 / k,  # noqa: E731
+                                   torch.randint(0, 16, (rows, k), device="cuda", generator=gen), 0).to(torch.uint8)
+    xc, wc = few(130), few(n)
+    xb, wb = (torch.randint(128, 130, (rows, k // 32), device="cuda", generator=gen, dtype=torch.uint8) for rows in (130, n))
+    w, want = K.mxfp4_pack(O.pack_codes(wc), wb), (O.values(xc, xb) @ O.values(wc, wb).t()).half()
+    for t in (*range(1, 34), 63, 64, 65, 96, 127, 128, 129):
+        x = K.mxfp4_pack(O.pack_codes(xc[:t]), xb[:t])
+        assert torch.equal(K.mxfp4_matmul(x, w), want[:t])
+        if n == 256 and t <= 40:
+            a = K.mxfp4_matmul(x, w, swiglu=True)
+            one = K.mxfp4_matmul(K.mxfp4_pack(O.pack_codes(xc[:130]), xb[:130]), w, swiglu=True)      # all rows at once
+            assert torch.equal(a.codes, one.codes[:t])
+            assert torch.equal(O.scale_rows(a.scales, t, 128), O.scale_rows(one.scales, 130, 128)[:t])
+
+
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("t,n,k", ((1, 6144, 4096), (2, 896, 4864), (7, 4096, 14336), (31, 77, 3584), (40, 4608, 3584), (128, 1152, 896),
                                    (5, 33, 32), (777, 4608, 3584), (129, 896, 4864), (513, 9728, 896), (200, 77, 1024)))
