@@ -136,24 +136,26 @@ scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const 
 
 // A token's expert rows, weighted, added up in the order of its choices in 32 bits; eight outputs a thread.
 template <typename T, typename W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 combine_kernel(T* __restrict__ out, const T* __restrict__ y, const int32_t* __restrict__ place, const W* __restrict__ weights,
                int64_t tokens, int top_k, int64_t n) {
   pdl_prologue();
-  const uint32_t chunks = (uint32_t)(n / 8), i = blockIdx.x * 256 + threadIdx.x;
+  const uint32_t chunks = (uint32_t)(n / 8), i = blockIdx.x * 128 + threadIdx.x;
   if (i >= tokens * chunks) return;
   const int64_t t = i / chunks, c = i % chunks;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int j0 = 0; j0 < top_k; j0 += 8) {              // eight rows requested together
     uint4 q[8];
     float w[8];
+    int from[8];                       // all places first: one after another each would wait for the row before
+#pragma unroll
+    for (int j = 0; j < 8; ++j) from[j] = j0 + j < top_k ? ld_upstream(place + t * top_k + j0 + j) : -1;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int from = j0 + j < top_k ? ld_upstream(place + t * top_k + j0 + j) : -1;
       q[j] = make_uint4(0u, 0u, 0u, 0u);
       w[j] = 0.f;
-      if (from >= 0) {
-        q[j] = ldg_stream_128(y + (int64_t)from * n + c * 8);
+      if (from[j] >= 0) {
+        q[j] = ldg_stream_128(y + (int64_t)from[j] * n + c * 8);
         w[j] = to_f32(weights[t * top_k + j0 + j]);
       }
     }
@@ -170,12 +172,12 @@ combine_kernel(T* __restrict__ out, const T* __restrict__ y, const int32_t* __re
 template <typename T>
 static int combine(void* out, const void* y, const void* place, const void* weights, int wide, int64_t tokens, int top_k, int64_t n,
                    cudaStream_t st) {
-  const dim3 grid((unsigned)cdiv64(tokens * (n / 8), 256));
+  const dim3 grid((unsigned)cdiv64(tokens * (n / 8), 128));
   if (wide)
-    b2l_launch(combine_kernel<T, float>, grid, dim3(256), (size_t)0, st, (T*)out, (const T*)y, (const int32_t*)place, (const float*)weights,
+    b2l_launch(combine_kernel<T, float>, grid, dim3(128), (size_t)0, st, (T*)out, (const T*)y, (const int32_t*)place, (const float*)weights,
                tokens, top_k, n);
   else
-    b2l_launch(combine_kernel<T, T>, grid, dim3(256), (size_t)0, st, (T*)out, (const T*)y, (const int32_t*)place, (const T*)weights, tokens,
+    b2l_launch(combine_kernel<T, T>, grid, dim3(128), (size_t)0, st, (T*)out, (const T*)y, (const int32_t*)place, (const T*)weights, tokens,
                top_k, n);
   B2L_LAUNCH_CHECK();
   return B2L_OK;
