@@ -33,7 +33,7 @@ struct Params {
 };
 
 constexpr int kRawTokens = 8;          // activations that the kernel quantises itself: up to so many rows,
-constexpr int kRawStages = 24;         // so many stages of 256 k of a CTA's part
+constexpr int kRawStages = 24;         // so many stages of 256 k of a CTA's part, and so many of both together
 
 template <int BT, bool RAW> struct Ring {
   static constexpr int kStages = BT == 128 ? 3 : 4;
@@ -215,7 +215,9 @@ __device__ __forceinline__ void send_and_add(const Params& p, const uint32_t (&v
 }
 
 // The rows of x in this CTA's part of k, quantised by the four warps that wait for the accumulator anyway: one launch less than with the quantiser
-// by itself, and the same codes (one token, 6144 x 4096, us on the device 5.8 -> 5.1, a call among others 8.1 -> 5.0).
+// by itself, and the same codes.  It pays while a warp has few units of 256 elements to do (quantiser and product -> this, us: one token, 6144 x
+// 4096 5.1 -> 4.5, 4096 x 14336 8.2 -> 7.6; four tokens, 6144 x 4096, 16 units to a CTA, 5.3 -> 4.8; eight, 32 units, 5.4 -> 5.6; eight, 28672 x 4096,
+// 128 units, 12.5 -> 17.9).
 template <typename T, int BT>
 __device__ __forceinline__ void quantise_rows(const Params& p, uint8_t* ring, int kb0, int stages, int warp, int lane) {
   using R = Ring<BT, true>;
@@ -458,19 +460,20 @@ static int stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// The same product for routed experts: tiles of up to BT rows of one expert, {expert, rows} in a table on the device
-// (mxfp4_moe.cu), row r of tile i in row i BT + r of x and y and in row 128 i + r of their scales.
+// The same product for routed experts: tiles of up to 64 rows of one expert, {expert, rows} in a table on the device
+// (mxfp4_moe.cu), row r of tile i in row 64 i + r of x and y and in row 128 i + r of their scales.
 //
-// Tiles of 32 or 64 rows; those of 128 are multiplied with the rows as the MMA's (mxfp4_gemm_pair.cu), where a thread holds a row's
+// Tiles of 128 rows are multiplied with the rows as the MMA's (mxfp4_gemm_pair.cu), where a thread holds a row's
 // outputs: here its lane is an output, and bringing 128 columns out through shared memory took longer than the products (2000 tokens,
-// 128 experts of 2048 x 768, both products 137 us -> see there).
+// 128 experts of 2048 x 768, both products 137 us, there 82).  Tiles of 32 rows were no faster at two rows an expert (58.7 against 56.1 us).
 // Bound: the experts' weights, each read from memory once (further tiles of an expert find them in L2).  Persistent, one CTA to
 // an SM with 180 KiB of copies in flight, the accumulator in two buffers: a tile's end overlaps the next one's products.
 // ---------------------------------------------------------------------------------------------------------------
-template <int BT> struct GroupedRing {
+struct GroupedRing {
+  static constexpr int BT = 64;        // rows of a tile
   static constexpr int kStage = 16384 + kSfBytes + BT * 128 + kSfBytes;
   static constexpr int kX = 16384 + kSfBytes;
-  static constexpr int kStages = BT == 32 ? 8 : 7;
+  static constexpr int kStages = 7;
   static constexpr int kCols = 2 * BT + kStages * 16;
   static constexpr int kAlloc = 256;
   static constexpr int kOut = 32 * 128 * 4;
@@ -492,10 +495,11 @@ struct __align__(8) GroupedControl {
   uint32_t tmem;
 };
 
-template <typename T, int BT, bool GATED>
+template <typename T, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const GroupedParams p) {
-  using R = GroupedRing<BT>;
+  using R = GroupedRing;
+  constexpr int BT = R::BT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   GroupedControl* ctl = reinterpret_cast<GroupedControl*>(smem);
@@ -672,29 +676,27 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   }
 }
 
-template <typename T, int BT, bool GATED>
+template <typename T, bool GATED>
 static int launch_grouped(const CUtensorMap& tx, const CUtensorMap& tw, const GroupedParams& p, int64_t max_tiles, cudaStream_t st) {
-  auto kern = grouped_kernel<T, BT, GATED>;
+  auto kern = grouped_kernel<T, GATED>;
   static int configured[64] = {0};
-  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, GroupedRing<BT>::kSmem, configured));
+  B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, GroupedRing::kSmem, configured));
   const int64_t items = max_tiles * p.n_tiles;
   const int grid = (int)(items < b2l_num_sms() ? items : b2l_num_sms());
-  b2l_launch(kern, dim3((unsigned)grid), dim3(kThreads), (size_t)GroupedRing<BT>::kSmem, st, tx, tw, p);
+  b2l_launch(kern, dim3((unsigned)grid), dim3(kThreads), (size_t)GroupedRing::kSmem, st, tx, tw, p);
   B2L_LAUNCH_CHECK();
   return B2L_OK;
 }
 
 template <typename T>
-static int grouped_gemm(const void* x, const void* w, const GroupedParams& p, int64_t max_tiles, int tile_rows, int experts, bool is_gated,
+static int grouped_gemm(const void* x, const void* w, const GroupedParams& p, int64_t max_tiles, int experts, bool is_gated,
                         cudaStream_t st) {
   CUtensorMap tx, tw;
-  int rc = b2l_make_tmap_2d(&tx, x, TMA_U8, (uint64_t)(max_tiles * tile_rows), (uint64_t)p.K / 2, (uint64_t)p.K / 2, (uint32_t)tile_rows, 128, true);
+  int rc = b2l_make_tmap_2d(&tx, x, TMA_U8, (uint64_t)(max_tiles * GroupedRing::BT), (uint64_t)p.K / 2, (uint64_t)p.K / 2, (uint32_t)GroupedRing::BT, 128, true);
   if (rc != B2L_OK) return rc;
   rc = b2l_make_tmap_2d(&tw, w, TMA_U8, (uint64_t)experts * p.N, (uint64_t)p.K / 2, (uint64_t)p.K / 2, 128, 128, true);
   if (rc != B2L_OK) return rc;
-#define GROUPED(BT) (is_gated ? launch_grouped<T, BT, true>(tx, tw, p, max_tiles, st) : launch_grouped<T, BT, false>(tx, tw, p, max_tiles, st))
-  return tile_rows == 32 ? GROUPED(32) : GROUPED(64);
-#undef GROUPED
+  return is_gated ? launch_grouped<T, true>(tx, tw, p, max_tiles, st) : launch_grouped<T, false>(tx, tw, p, max_tiles, st);
 }
 
 }  // namespace mx4
@@ -703,7 +705,7 @@ static int grouped_gemm(const void* x, const void* w, const GroupedParams& p, in
 extern "C" int64_t b2l_mxfp4_matmul_takes_16bit(int64_t t, int64_t n, int64_t k) {
   if (t < 1 || t > mx4::kRawTokens || n < 1 || k < 1) return 0;
   const int num_kb = (int)cdiv64(k, mx4::kStageK), s = mx4::parts(cdiv64(n, 128), num_kb);
-  return (num_kb + s - 1) / s <= mx4::kRawStages;
+  return (num_kb + s - 1) / s * t <= mx4::kRawStages;
 }
 
 extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w, const void* w_scales,
@@ -745,7 +747,7 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
                   max_tiles * cdiv64(n, 128) < (1ll << 31) && max_tiles * 128 < (1ll << 31) &&
                   (experts * cdiv64(n, 128) + max_tiles) * mx4::k_tiles(k) < (1ll << 29),
               "mxfp4_grouped_matmul: experts=%d n=%lld k=%lld (a multiple of 32) tiles=%lld", experts, (long long)n, (long long)k, (long long)max_tiles);
-  B2L_REQUIRE(tile_rows == 32 || tile_rows == 64 || tile_rows == 128, "mxfp4_grouped_matmul: tiles of %d rows", tile_rows);
+  B2L_REQUIRE(tile_rows == 64 || tile_rows == 128, "mxfp4_grouped_matmul: tiles of %d rows", tile_rows);
   if (max_tiles == 0) return B2L_OK;
   B2L_REQUIRE(y && x && x_scales && w && w_scales && table && (!gated || y_scales), "mxfp4_grouped_matmul: null pointer");
   B2L_REQUIRE(!gated || n % 128 == 0, "mxfp4_grouped_matmul: gate and up rows come in runs of 64 (n=%lld)", (long long)n);
@@ -767,6 +769,6 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
   p.ktiles = mx4::k_tiles(k);
   p.N = (int)n; p.K = (int)k; p.num_kb = (int)cdiv64(k, mx4::kStageK); p.n_tiles = (int)cdiv64(n, 128);
   p.vec = n % 4 == 0;
-  if (dtype == B2L_F16) return mx4::grouped_gemm<__half>(x, w, p, max_tiles, tile_rows, experts, gated != 0, st);
-  return mx4::grouped_gemm<__nv_bfloat16>(x, w, p, max_tiles, tile_rows, experts, gated != 0, st);
+  if (dtype == B2L_F16) return mx4::grouped_gemm<__half>(x, w, p, max_tiles, experts, gated != 0, st);
+  return mx4::grouped_gemm<__nv_bfloat16>(x, w, p, max_tiles, experts, gated != 0, st);
 }

@@ -121,7 +121,7 @@ scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const 
   if (in) load_raw(x + row * x_stride + c * 8, v);
   uint32_t byte;
   const uint32_t code = quantise_raw(v, byte);
-  const uint32_t behind = (k / 8 + 15) & ~15u, shift = 31 - __clz((int)tile);          // a tile is 32, 64 or 128 rows
+  const uint32_t behind = (k / 8 + 15) & ~15u, shift = 31 - __clz((int)tile);          // a tile is 64 or 128 rows
   const bool scaled = (lane & 3) == 0 && c < behind;
   uint8_t* out = codes + c * 4;
   uint8_t* scale = scales + (c >> 4) * kTileBytes + ((c >> 2) & 3);
@@ -185,11 +185,9 @@ static int combine(void* out, const void* y, const void* place, const void* weig
 
 }  // namespace mx4
 
-// Rows of an expert's tile, the MMA's columns: more than an expert's rows are products of nothing, fewer read its weights again.
-extern "C" int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts) {
-  const int64_t e = experts > 0 ? experts : 1;
-  return slots <= 24 * e ? 32 : (slots <= 48 * e ? 64 : 128);
-}
+// Rows of an expert's tile.  64: the weights are the MMA's rows, for few rows an expert; 128: the tokens are (whole call, 128 experts of 2048 x
+// 768, 64 / 128, us: two rows each 56 / 65, 24 71 / 79, 48 83 / 85, 64 95 / 89; 8 experts, 64 rows each 20.6 / 22.8, 100 23.3 / 23.2).
+extern "C" int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts) { return slots <= 800 || slots <= 48LL * experts ? 64 : 128; }
 
 extern "C" int64_t b2l_mxfp4_moe_max_tiles(int64_t slots, int tile_rows, int experts) {
   if (slots <= 0 || tile_rows <= 0 || experts <= 0) return 0;
@@ -212,7 +210,7 @@ extern "C" int b2l_mxfp4_moe_sort(void* place, void* table, const void* topk_ids
 
 extern "C" int b2l_mxfp4_moe_scatter(void* codes, void* scales, const void* x, const void* place, int64_t tokens, int top_k, int tile_rows,
                                      int64_t k, int64_t x_row_stride, int dtype, void* stream) {
-  B2L_REQUIRE(tokens >= 0 && top_k > 0 && (tile_rows == 32 || tile_rows == 64 || tile_rows == 128) && k > 0 && k % 32 == 0 && k < (1ll << 30),
+  B2L_REQUIRE(tokens >= 0 && top_k > 0 && (tile_rows == 64 || tile_rows == 128) && k > 0 && k % 32 == 0 && k < (1ll << 30),
               "mxfp4_moe_scatter: tokens=%lld top_k=%d k=%lld (a multiple of 32)", (long long)tokens, top_k, (long long)k);
   if (tokens == 0) return B2L_OK;
   B2L_REQUIRE(codes && scales && x && place, "mxfp4_moe_scatter: null pointer");

@@ -108,8 +108,9 @@ dequantize_kernel(T* __restrict__ y, const uint8_t* __restrict__ codes, const ui
   }
 }
 
-// Units of 256 elements to a warp: one where the warps of all would not fill the SMs twice over, else four.
-static int units_of(int64_t rows, int64_t k) { return rows * cdiv64(k, 256) < 128LL * b2l_num_sms() ? 1 : 4; }
+// Units of 256 elements to a warp: one where there are few, for latency, else four (quantiser / reader, one -> four, us: 32 x 4096 1.31 / 1.33 ->
+// 1.70 / 1.59; 256 x 4096 2.1 / 2.1 -> 2.0 / 1.7; 1000 x 4096 3.7 / 3.5 -> 3.4 / 3.2; 4000 x 4096 12.2 / 10.6 -> 7.8 / 6.6).
+static int units_of(int64_t rows, int64_t k) { return rows * cdiv64(k, 256) < 24LL * b2l_num_sms() ? 1 : 4; }
 
 // ---------------------------------------------------------------------------------------------------------------
 // s = x + r (stored over r, or to `sum`, in the activations' type), y = s / sqrt(mean s^2 + eps) * w, quantised.
@@ -247,8 +248,9 @@ static int launch_norm(void* codes, void* scales, void* sum, const void* x, cons
     b2l_launch(norm_quantize_kernel<T, V>, dim3((unsigned)rows), dim3(threads), (size_t)0, st, (uint8_t*)codes, (uint8_t*)scales, \
                (T*)sum, (const T*)x, (const T*)res, (const T*)w, (int)n, xs, rs, ss, k_tiles(n), 1.0 / (double)n, eps);               \
   }
-  // rows that come two or more to an SM are read by fewer threads each, so that more of them are in flight (figures above)
-  const bool many = rows > 2LL * b2l_num_sms();
+  // many rows are read by fewer threads each, so that more of them are in flight (one -> two chunks a thread, us: 32 x 4096 2.6 -> 2.9, 400 x
+  // 4096 4.9 -> 5.2, 800 x 4096 7.7 -> 7.0, 1999 x 3584 with the reader 22.3 -> 18.5)
+  const bool many = rows > 4LL * b2l_num_sms();
   if (chunks <= 512 && !many) NORM(1)
   else if (chunks <= 1024) NORM(2)
   else NORM(4)

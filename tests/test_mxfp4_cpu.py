@@ -125,7 +125,7 @@ def test_tiles_of_experts_hold_every_split_of_the_slots():
     gen = torch.Generator().manual_seed(0)
     for slots, experts in ((1, 1), (5, 128), (256, 128), (1000, 7), (16000, 128), (33, 32)):
         tile = lib.b2l_mxfp4_moe_tile_rows(slots, experts)
-        assert tile in (32, 64, 128)
+        assert tile in (64, 128)
         most = lib.b2l_mxfp4_moe_max_tiles(slots, tile, experts)
         for _ in range(20):
             skew = torch.rand(experts, generator=gen) ** 4 + 1e-9
@@ -134,8 +134,9 @@ def test_tiles_of_experts_hold_every_split_of_the_slots():
 
 
 def test_products_that_quantise_their_rows_have_room_for_them():
-    """A CTA's part of k is at most 24 stages of 256, by the same division as the launch."""
+    """A CTA's part is at most 24 rows of 256 elements, by the same division as the launch."""
     lib = _lib.load()
-    assert lib.b2l_mxfp4_matmul_takes_16bit(1, 6144, 4096) and lib.b2l_mxfp4_matmul_takes_16bit(8, 4096, 14336)
+    assert lib.b2l_mxfp4_matmul_takes_16bit(1, 6144, 4096) and lib.b2l_mxfp4_matmul_takes_16bit(3, 4096, 14336)
+    assert not lib.b2l_mxfp4_matmul_takes_16bit(4, 4096, 14336) and lib.b2l_mxfp4_matmul_takes_16bit(8, 9728, 896)
     assert not lib.b2l_mxfp4_matmul_takes_16bit(9, 6144, 4096) and not lib.b2l_mxfp4_matmul_takes_16bit(0, 6144, 4096)
     assert lib.b2l_mxfp4_matmul_takes_16bit(1, 40000, 24 * 256) and not lib.b2l_mxfp4_matmul_takes_16bit(1, 40000, 24 * 256 + 32)
