@@ -38,6 +38,7 @@ struct PairParams {
   uint8_t* y; uint8_t* y_scales; int64_t ldy, y_ktiles;                   // gated: codes and scales
   const int32_t* table;                // experts: tiles, then {expert, rows} of each
   int T, N, K, num_kb, m_tiles, n_tiles, ktiles;
+  int wide, tiles;                     // tiles of BN outputs; those and the halves behind them
   int early;                           // weights may be requested before the previous kernel has ended
 };
 
@@ -78,19 +79,26 @@ template <int CTAS> __device__ __forceinline__ void commit(uint64_t* bar) {
   if (CTAS == 2) tc_commit_pair(bar);
   else tc_commit(bar);
 }
-// A tile of outputs: token tile (index of 128 rows for each CTA), output tile, rows that hold anything, expert
-struct Work { int m, n, rows, expert; };
-template <int CTAS> __device__ __forceinline__ Work work_of(const PairParams& p, int t, int rank) {
+// A tile of outputs: token tile (index of 128 rows for each CTA), first 128 outputs and how many of those, rows that hold anything, expert
+struct Work { int m, n, width, rows, expert; };
+template <int BN, int CTAS> __device__ __forceinline__ Work work_of(const PairParams& p, int t, int rank) {
   Work o;
+  o.width = BN / 128;
   if (CTAS == 2) {
-    const PairTile pt = pair_tile(t, p.m_tiles, p.n_tiles, kPairBand);
+    // the tiles that would make a last wave of less than half of the pairs come in halves
+    const int behind = t - p.wide;
+    const PairTile pt = pair_tile(behind < 0 ? t : p.wide + (behind >> 1), p.m_tiles, p.n_tiles, kPairBand);
     o.m = pt.m * 2 + rank;
-    o.n = pt.n;
+    o.n = pt.n * (BN / 128);
+    if (behind >= 0) {
+      o.n += behind & 1;
+      o.width = 1;
+    }
     o.rows = p.T - o.m * kPairRows;
     o.expert = 0;
   } else {
     o.m = t / p.n_tiles;
-    o.n = t - o.m * p.n_tiles;
+    o.n = (t - o.m * p.n_tiles) * (BN / 128);
     o.expert = ld_upstream(p.table + 1 + 2 * o.m);
     o.rows = ld_upstream(p.table + 2 + 2 * o.m);
   }
@@ -138,7 +146,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
   if (CTAS == 1) pdl_wait_prior();     // the table is upstream data
-  const int tiles = (CTAS == 2 ? p.m_tiles : ld_upstream(p.table)) * p.n_tiles;
+  const int tiles = CTAS == 2 ? p.tiles : ld_upstream(p.table) * p.n_tiles;
 
   if (warp == 0) {
     // ===================== TMA producer: this CTA's halves of both operands, its tokens' scales, all outputs' scales =====================
@@ -147,8 +155,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     };
     auto load_w = [&](int s, int kb, const Work& wk) {
       uint8_t* st = ring + (size_t)s * R::kBytes;
-      const int row = wk.expert * p.N + wk.n * BN + (int)rank * (BN / CTAS);
-      const int ws = (wk.expert * ((p.N + 127) / 128) + wk.n * (BN / 128)) * p.ktiles * 4;      // rows of 128 bytes
+      const int row = wk.expert * p.N + wk.n * 128 + (int)rank * (wk.width * (128 / CTAS));      // of half a tile the box holds twice as much
+      const int ws = (wk.expert * ((p.N + 127) / 128) + wk.n) * p.ktiles * 4;                     // rows of 128 bytes
       load_2d<CTAS>(st + R::kX, &tmap_w, kb * 128, row, &ctl->full[s]);
 #pragma unroll
       for (int h = 0; h < BN / 128; ++h) load_2d<CTAS>(st + R::kWs + h * kSfBytes, &tmap_ws, 0, ws + h * p.ktiles * 4 + kb * 8, &ctl->full[s]);
@@ -161,17 +169,17 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     gemm::PipeState ps(R::kStages);
     int ahead = 0;                     // stages whose weights were requested before the previous kernel has ended
     if (CTAS == 2 && p.early && pair < tiles) {
-      const Work wk = work_of<CTAS>(p, pair, (int)rank);
+      const Work wk = work_of<BN, CTAS>(p, pair, (int)rank);
       ahead = p.num_kb < R::kStages ? p.num_kb : R::kStages;
       if (elect_one())
         for (int s = 0; s < ahead; ++s) { expect(s); load_w(s, s, wk); }
       __syncwarp();
     }
     pdl_wait_prior();
-    Work next = pair < tiles ? work_of<CTAS>(p, pair, (int)rank) : Work{0, 0, 0, 0};
+    Work next = pair < tiles ? work_of<BN, CTAS>(p, pair, (int)rank) : Work{0, 0, 0, 0, 0};
     for (int t = pair; t < tiles; t += pairs) {
       const Work wk = next;
-      if (t + pairs < tiles) next = work_of<CTAS>(p, t + pairs, (int)rank);      // table entries are asked for a tile ahead
+      if (t + pairs < tiles) next = work_of<BN, CTAS>(p, t + pairs, (int)rank);      // table entries are asked for a tile ahead
 #pragma unroll 1
       for (int kb = 0; kb < p.num_kb; ++kb) {
         mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
@@ -200,6 +208,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       int it = 0, i = 0;
       for (int t = pair; t < tiles; t += pairs, ++it) {
         const uint32_t acc = tmem + (it & 1) * R::kAcc1;
+        const uint32_t id = BN == 256 && CTAS == 2 && t >= p.wide ? idesc(128 * CTAS, 128, 0) : idesc(128 * CTAS, BN, 0);
         if (BN == 256) {
           if (it >= 1) mbar_wait_spin(&ctl->freed[(it - 1) & 1], ((it - 1) >> 1) & 1);
         } else {
@@ -230,7 +239,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
 #pragma unroll
                 for (int q = 2 * j; q < 2 * j + 2; ++q)
                   if (q < steps)
-                    mma<CTAS>(acc, xd + 2 * q, wd + 2 * q, idesc(128 * CTAS, BN, q & 1), sfa + j * 4, sfb + j * (BN / 32), kb | q ? 1u : 0u);
+                    mma<CTAS>(acc, xd + 2 * q, wd + 2 * q, id | ((q & 1) ? kSecondHalf : 0u), sfa + j * 4, sfb + j * (BN / 32), kb | q ? 1u : 0u);
               }
             commit<CTAS>(&ctl->empty[ps.stage]);
             if (kb + 1 == p.num_kb) commit<CTAS>(&ctl->acc_full[it & 1]);
@@ -254,12 +263,13 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     pdl_wait_prior();                  // y may still be read upstream
     uint8_t* dst = out_stage + (quad + 4 * half) * 4096;
     int it = 0;
-    Work next = pair < tiles ? work_of<CTAS>(p, pair, (int)rank) : Work{0, 0, 0, 0};
+    Work next = pair < tiles ? work_of<BN, CTAS>(p, pair, (int)rank) : Work{0, 0, 0, 0, 0};
     for (int t = pair; t < tiles; t += pairs, ++it) {
       const Work wk = next;
-      if (t + pairs < tiles) next = work_of<CTAS>(p, t + pairs, (int)rank);
+      if (t + pairs < tiles) next = work_of<BN, CTAS>(p, t + pairs, (int)rank);
       const int buf = it & 1, m_warp = wk.m * kPairRows + quad * 32;
       const bool any = quad * 32 < wk.rows;             // uniform over the warp
+      const int end = (wk.n + wk.width) * 128 < p.N ? (wk.n + wk.width) * 128 : p.N;
       const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * R::kAcc1;
       // the columns that both accumulators have: the first one's last, read by the second half's warps, the second one's first.  The other
       // half's warps are done with the tile before, which is what their arrival says.
@@ -276,8 +286,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           tmem_ld_32x32b_x32(acc + c + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
           tc_wait_ld();
           if (BN == 256 ? shared && j == 0 : true) hand_on(buf);
-          const int n0 = wk.n * BN + c;
-          if (n0 >= p.N || !any) continue;
+          const int n0 = wk.n * 128 + c;
+          if (n0 >= end || !any) continue;
           if (lane == 0) bulk_wait_read<0>();           // the store before has read the box
           __syncwarp();
           if (p.bias) {                                 // a branch of its own: without a bias nothing of it is issued
@@ -316,7 +326,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           tmem_ld_32x32b_x32(acc + c + (up_first ? 64 : 0) + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(held + 32 * h));
         tc_wait_ld();
         if (shared) hand_on(buf);
-        const int n0 = wk.n * BN + (BN == 256 ? c : 0), k = n0 / 2 + (BN == 256 ? 0 : half * 32), row = m_warp + lane;
+        const int n0 = wk.n * 128 + (BN == 256 ? c : 0), k = n0 / 2 + (BN == 256 ? 0 : half * 32), row = m_warp + lane;
         uint32_t bytes = 0;
         uint4 codes[kBlocks];
 #pragma unroll
@@ -343,7 +353,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           for (int e = 0; e < 32; ++e) v[e] = gated(v[e], u[e]);
           bytes |= quantise32(v, codes[h]) << (8 * h);
         }
-        if (n0 < p.N && quad * 32 + lane < wk.rows) {   // N is a multiple of 128
+        if (n0 < end && quad * 32 + lane < wk.rows) {   // N is a multiple of 128
           uint8_t* y = p.y + (int64_t)row * p.ldy + k / 2;
 #pragma unroll
           for (int h = 0; h < kBlocks; ++h) stg_128(y + 16 * h, codes[h]);
@@ -380,7 +390,12 @@ static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t e
   p.N = (int)g.N; p.K = (int)g.K; p.num_kb = (int)cdiv64(g.K, kStageK); p.ktiles = (int)k_tiles(g.K);
   p.n_tiles = (int)cdiv64(g.N, BN);
   tiles *= p.n_tiles;
-  const int grid = CTAS * (int)(tiles < sms / CTAS ? tiles : sms / CTAS);
+  // Halves for what is left of the last wave if that is at most half of one (us: 1000 x 28672 x 4096, 448 tiles
+  // for 74 pairs, 54 -> 52; 300 x 28672 x 4096 32.5 -> 29.3)
+  const int64_t pairs = sms / CTAS, rest = tiles % pairs;
+  p.wide = (int)(CTAS == 2 && BN == 256 && tiles > pairs && 2 * rest <= pairs ? tiles - rest : tiles);
+  p.tiles = (int)(p.wide + 2 * (tiles - p.wide));
+  const int grid = CTAS * (int)(tiles < pairs ? tiles : pairs);
   CUtensorMap tx, tw, txs, tws, ty;
   int rc = b2l_make_tmap_2d(&tx, g.x, TMA_U8, (uint64_t)rows, (uint64_t)g.K / 2, (uint64_t)g.ldx, kPairRows, 128, true);
   if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tw, g.w, TMA_U8, (uint64_t)(experts * g.N), (uint64_t)g.K / 2, (uint64_t)g.ldw, BN / CTAS, 128, true);

@@ -20,6 +20,9 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t M, uint32_t N, uint32_t ha
   return ((2u * half) << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | (1u << 23) | ((M >> 4) << 24) | ((2u * half) << 29);
 }
 
+constexpr uint32_t kSecondHalf = (2u << 4) | (2u << 29);      // idesc(M, N, 1) is idesc(M, N, 0) with these bits
+static_assert(idesc(256, 256, 1) == (idesc(256, 256, 0) | kSecondHalf), "scale ids");
+
 // 32 rows of 16 bytes, rows in groups of eight one after another
 __device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
   return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128u >> 4) << 16) | ((uint64_t)(128u >> 4) << 32) | ((uint64_t)1 << 46);
