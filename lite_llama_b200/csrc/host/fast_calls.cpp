@@ -701,7 +701,8 @@ PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
   FAST_BEGIN
   Mx4 w, q;
   if (!mx4(a[1], 2, w)) return none();
-  const at::Tensor *x = plain(a[0]), *bias = a[2] == Py_None ? w.codes : plain(a[2]);
+  const bool biased = a[2] != Py_None;
+  const at::Tensor *x = plain(a[0]), *bias = biased ? plain(a[2]) : w.codes;      // w.codes: none
   if (!x && !mx4(a[0], 2, q)) return none();
   if (!abi.mx4_quantize || !abi.mx4_scale_bytes || !abi.mx4_takes_16bit) return none();      // of a library that holds another file's functions alone
   const int device = device_for(abi.mx4_matmul, {x ? x : q.codes, x ? x : q.scales, w.codes, w.scales, bias});
@@ -709,14 +710,14 @@ PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
   const bool gated = a[3] == Py_True;
   if (x && (!mx4_rows(*x, false) || x->size(1) != w.k)) return none();
   if (!x && q.k != w.k) return none();
-  at::ScalarType type = x ? x->scalar_type() : bias != w.codes ? bias->scalar_type() : at::kHalf;
+  at::ScalarType type = x ? x->scalar_type() : biased ? bias->scalar_type() : at::kHalf;
   if (a[4] != Py_None) {
     const at::ScalarType wanted = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
     if (x && wanted != type) return none();
     type = wanted;
   }
   if (type != at::kHalf && type != at::kBFloat16) return none();
-  if (bias != w.codes && (bias->dim() != 1 || bias->size(0) != w.rows || !bias->is_contiguous() || bias->scalar_type() != type)) return none();
+  if (biased && (bias->dim() != 1 || bias->size(0) != w.rows || !bias->is_contiguous() || bias->scalar_type() != type)) return none();
   if (gated && w.rows % 128 != 0) return none();
   const i64 t = x ? x->size(0) : q.rows, n = w.rows, k = w.k;
   const int code = type == at::kHalf ? 0 : 1;
@@ -746,7 +747,7 @@ PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (gated) ys = mx4_tiles(t, n / 2);
     if (!rc)
       rc = abi.mx4_matmul(y.data_ptr(), gated ? ys.data_ptr() : nullptr, xc, xs, w.codes->data_ptr(), w.scales->data_ptr(),
-                          bias == w.codes ? nullptr : bias->data_ptr(), t, n, k, stride, k / 2, gated ? n / 4 : n, gated ? 1 : 0, 1, code, st);
+                          biased ? bias->data_ptr() : nullptr, t, n, k, stride, k / 2, gated ? n / 4 : n, gated ? 1 : 0, 1, code, st);
   }
   if (rc) return failed(rc);
   return gated ? pair_of(std::move(y), std::move(ys)) : THPVariable_Wrap(std::move(y));
