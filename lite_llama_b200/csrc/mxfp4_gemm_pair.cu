@@ -252,10 +252,13 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
   } else {
     // ===================== one thread per token, two warps to its columns =====================
     const int quad = warp & 3, half = (warp - 2) >> 2;
+    // Only where a later tile's products wait for it: an arrival that nobody waits for could still be on its way to the leader when that
+    // has left.
+    bool awaited = false;
     auto hand_on = [&](int buf) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
+      if (lane == 0 && awaited) {
         if (CTAS == 2) mbar_arrive_cluster(leader_addr(&ctl->freed[buf]));
         else mbar_arrive(&ctl->freed[buf]);
       }
@@ -268,6 +271,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       const Work wk = next;
       if (t + pairs < tiles) next = work_of<BN, CTAS>(p, t + pairs, (int)rank);
       const int buf = it & 1, m_warp = wk.m * kPairRows + quad * 32;
+      awaited = t + (BN == 256 ? 1 : 2) * pairs < tiles;
       const bool any = quad * 32 < wk.rows;             // uniform over the warp
       const int end = (wk.n + wk.width) * 128 < p.N ? (wk.n + wk.width) * 128 : p.N;
       const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * R::kAcc1;
