@@ -487,7 +487,6 @@ struct GroupedParams {
   const int32_t* table;                // tiles, then {expert, rows} of each
   int64_t ktiles;
   int N, K, num_kb, n_tiles;
-  int vec;
 };
 
 struct __align__(8) GroupedControl {
@@ -630,14 +629,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
             const int r = i >> 5, n = nt * 128 + (i & 31) * 4;
             const float4 v = *reinterpret_cast<const float4*>(out_stage + i * 4);
             T* out = reinterpret_cast<T*>(p.y) + ((int64_t)tile * BT + c + r) * p.ldy + n;
-            if (p.vec && n < p.N) {
-              *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
-            } else {
-              if (n < p.N) out[0] = from_f32<T>(v.x);
-              if (n + 1 < p.N) out[1] = from_f32<T>(v.y);
-              if (n + 2 < p.N) out[2] = from_f32<T>(v.z);
-              if (n + 3 < p.N) out[3] = from_f32<T>(v.w);
-            }
+            if (n < p.N) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));      // N: a multiple of 8
           }
         } else {
           for (int base = quad * 32; base < here * 8; base += 128) {
@@ -726,6 +718,7 @@ extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const vo
   cudaStream_t st = (cudaStream_t)stream;
   mx4::PairCall g = {y, y_row_stride, y_scales, bias, x, x_scales, w, w_scales, t, n, k, x_row_stride, w_row_stride, gated != 0, weights_ready != 0};
   if (!raw && mx4::pair_wanted(g)) return mx4::pair_gemm(g, dtype, st);
+  B2L_REQUIRE(cdiv64(t, 128) < 65536, "mxfp4_matmul: %lld tokens of outputs that start off 16 bytes", (long long)t);
   mx4::Params p;
   p.y = y; p.ldy = y_row_stride;
   p.y_scales = (uint8_t*)y_scales; p.y_ktiles = mx4::k_tiles(n / 2);
@@ -751,16 +744,13 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
   if (max_tiles == 0) return B2L_OK;
   B2L_REQUIRE(y && x && x_scales && w && w_scales && table && (!gated || y_scales), "mxfp4_grouped_matmul: null pointer");
   B2L_REQUIRE(!gated || n % 128 == 0, "mxfp4_grouped_matmul: gate and up rows come in runs of 64 (n=%lld)", (long long)n);
-  B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales) % 16 == 0 && (uintptr_t)y % 8 == 0,
-              "mxfp4_grouped_matmul: rows of codes must start on 16 bytes");
+  B2L_REQUIRE(n % 8 == 0, "mxfp4_grouped_matmul: outputs are written in units of 8 (n=%lld)", (long long)n);
+  B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales | (uintptr_t)y) % 16 == 0,
+              "mxfp4_grouped_matmul: rows must start on 16 bytes");
   B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "mxfp4_grouped_matmul: dtype %d", dtype);
   cudaStream_t st = (cudaStream_t)stream;
   mx4::PairCall g = {y, gated ? n / 4 : n, y_scales, nullptr, x, x_scales, w, w_scales, max_tiles, n, k, k / 2, k / 2, gated != 0, false};
-  if (tile_rows == 128) {
-    B2L_REQUIRE(gated || (n % 8 == 0 && (uintptr_t)y % 16 == 0), "mxfp4_grouped_matmul: tiles of 128 rows are written in units of 8 outputs (n=%lld)", (long long)n);
-    B2L_REQUIRE(!gated || (uintptr_t)y % 16 == 0, "mxfp4_grouped_matmul: rows of codes must start on 16 bytes");
-    return mx4::rows_gemm(g, table, experts, dtype, st);
-  }
+  if (tile_rows == 128) return mx4::rows_gemm(g, table, experts, dtype, st);
   mx4::GroupedParams p;
   p.y = y; p.ldy = gated ? n / 4 : n;
   p.y_scales = (uint8_t*)y_scales; p.y_ktiles = mx4::k_tiles(n / 2);
@@ -768,7 +758,6 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
   p.table = (const int32_t*)table;
   p.ktiles = mx4::k_tiles(k);
   p.N = (int)n; p.K = (int)k; p.num_kb = (int)cdiv64(k, mx4::kStageK); p.n_tiles = (int)cdiv64(n, 128);
-  p.vec = n % 4 == 0;
   if (dtype == B2L_F16) return mx4::grouped_gemm<__half>(x, w, p, max_tiles, experts, gated != 0, st);
   return mx4::grouped_gemm<__nv_bfloat16>(x, w, p, max_tiles, experts, gated != 0, st);
 }

@@ -125,7 +125,7 @@ static int units_of(int64_t rows, int64_t k) { return rows * cdiv64(k, 256) < 24
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int VPT>
 __global__ void __launch_bounds__(512, 2)
-norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, T* sum, const T* __restrict__ x, const T* res,
+norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, T* sum, const T* x, const T* res,      // sum: may be x or res
                      const T* __restrict__ w, int n, int64_t x_stride, int64_t r_stride, int64_t s_stride, int64_t ktiles, double inv_n,
                      float eps) {
   pdl_prologue();

@@ -25,8 +25,9 @@ class MXFP4(NamedTuple):
     ``codes`` uint8 ``[..., rows, k / 2]``, element 2i in the low half of byte i; ``scales`` uint8
     ``[..., ceil(rows / 128), ceil(k / 128), 32, 4, 4]``, indices row % 32, row % 128 / 32, block % 4: the order the tensor cores read
     (``mxfp4_pack`` makes it from scales in rows).  ``ready``: nothing that is still running on the GPU writes it, so that a product
-    may request it as its weight while the kernel before is at work.  What the operators here return is not ready in this sense;
-    ``mxfp4_pack`` and ``mxfp4_quantize_weight`` return weights that are, and a pair of tensors that other code wrote is."""
+    may request it as its weight while the kernel before is at work.  What the operators here return is not ready in this sense, nor
+    are pieces of it (``MXFP4(q.codes[e], q.scales[e], q.ready)``); ``mxfp4_pack`` and ``mxfp4_quantize_weight`` return weights that
+    are, and a pair of tensors that other code wrote is."""
 
     codes: torch.Tensor
     scales: torch.Tensor

@@ -122,6 +122,33 @@ def test_weights_of_the_kernel_before():
             same(K.mxfp4_matmul(x, K.MXFP4(codes, scales, ready=False)), y)
 
 
+def test_pieces_of_a_stack_just_quantised_and_a_matrix_by_itself():
+    for _ in range(5):
+        w, x = randn(3, 4096, 1024), randn(4, 1024)
+        want = [K.mxfp4_matmul(x, K.mxfp4_quantize_weight(m)) for m in w]
+        for e in range(3):
+            q = K.mxfp4_quantize(w)
+            same(K.mxfp4_matmul(x, K.MXFP4(q.codes[e], q.scales[e], q.ready)), want[e])
+    for t in (24, 200):
+        m = randn(t, 1024)
+        q = K.mxfp4_quantize(m)
+        same(K.mxfp4_matmul(q, q), K.mxfp4_matmul(m, K.mxfp4_quantize_weight(m)))
+
+
+@pytest.mark.parametrize("rows,n", ((3, 4096), (700, 256)))
+def test_norm_in_the_place_of_its_inputs(rows, n):
+    x, r, w = randn(rows, n), randn(rows, n), randn(n)
+    q, total = K.skip_rmsnorm_mxfp4(x, r, w, out_residual=torch.empty_like(r))
+    over = x.clone()
+    p, s = K.skip_rmsnorm_mxfp4(over, r, w, out_residual=over)
+    same(p, q)
+    assert s is over and torch.equal(s, total)
+    twice = x.clone()
+    p, s = K.skip_rmsnorm_mxfp4(twice, twice, w)
+    same(p, K.skip_rmsnorm_mxfp4(x, x.clone(), w)[0])
+    assert s is twice and torch.equal(s, x + x)
+
+
 # ------------------------------------------------------------------------------------------------- rows and columns behind the end
 @pytest.mark.parametrize("t,n", ((1, 33), (5, 130), (70, 128), (300, 264), (300, 250)))
 def test_nothing_is_written_behind_the_outputs(t, n):
