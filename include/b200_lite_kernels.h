@@ -344,11 +344,12 @@ int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scale
                      int64_t y_row_stride, int gated, int weights_ready, int dtype, void* stream);
 
 /* Routed experts: every slot (token, choice) gets row place[slot] (int32; -1: its id names no expert), the rows of an expert fill tiles of
- * tile_rows (64 or 128), row r of tile i is row i * tile_rows + r; scales of a tile start on a tile of 128 rows.
+ * tile_rows (64, 128 or 256), row r of tile i is row i * tile_rows + r; scales of a tile start on a tile of 128
+ * rows.
  * table int32 [1 + 2 * max_tiles] = {tiles, {expert, rows} per tile}.
- * _tile_rows: the tile for so many slots.  _scatter: x quantised into the rows of its slots.  _grouped_matmul: w [experts, n, k], buffers of max_tiles * tile_rows rows
- * (scales: 128 max_tiles); gated as in b2l_mxfp4_matmul.  _combine: out[t] = sum_j weights[t, j] * y[place[t, j]]. */
-int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts);
+ * _tile_rows: the tile for so many slots, n: outputs of the first product.  _scatter: x quantised into the rows of its slots.
+ * _grouped_matmul: w [experts, n, k], buffers of max_tiles * tile_rows rows (scales: max_tiles * 128 at least); gated as in b2l_mxfp4_matmul.  _combine: out[t] = sum_j weights[t, j] * y[place[t, j]]. */
+int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts, int64_t n);
 int64_t b2l_mxfp4_moe_max_tiles(int64_t slots, int tile_rows, int experts);
 int b2l_mxfp4_moe_sort(void* place, void* table, const void* topk_ids, int id_width, int64_t slots, int tile_rows, int experts,
                        void* stream);

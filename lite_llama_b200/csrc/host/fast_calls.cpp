@@ -59,7 +59,7 @@ struct {
   int (*mx4_matmul)(void*, void*, const void*, const void*, const void*, const void*, const void*, i64, i64, i64, i64, i64, i64, int, int, int,
                     void*);
   i64 (*mx4_takes_16bit)(i64, i64, i64);
-  i64 (*mx4_tile_rows)(i64, int);
+  i64 (*mx4_tile_rows)(i64, int, i64);
   i64 (*mx4_max_tiles)(i64, int, int);
   int (*mx4_sort)(void*, void*, const void*, int, i64, int, int, void*);
   int (*mx4_scatter)(void*, void*, const void*, const void*, i64, int, int, i64, i64, int, void*);
@@ -774,13 +774,13 @@ PyObject* mx4_moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
   if (!width || (!wide && weights->scalar_type() != x->scalar_type())) return none();
   const int top_k = (int)ids->size(1), code = half_code(*x), e = (int)experts;
   const i64 slots = tokens * top_k;
-  const int tile = (int)abi.mx4_tile_rows(slots, e);
+  const int tile = (int)abi.mx4_tile_rows(slots, e, w1.rows);
   const i64 tiles = abi.mx4_max_tiles(slots, tile, e), rows = tiles * tile;
   // one buffer for what lives within the call
   i64 size = 0;
   auto part = [&](i64 n) { const i64 at = size; size += up(n, 256) * 256; return at; };
-  const i64 place = part(4 * slots), table = part(4 + 8 * tiles), xc = part(rows * (hidden / 2)), xs = part(abi.mx4_scale_bytes(128 * tiles, hidden)),
-            ac = part(rows * (inner / 2)), as = part(abi.mx4_scale_bytes(128 * tiles, inner)), y = part(2 * rows * hidden);
+  const i64 place = part(4 * slots), table = part(4 + 8 * tiles), xc = part(rows * (hidden / 2)), xs = part(abi.mx4_scale_bytes(std::max<i64>(128, tile) * tiles, hidden)),
+            ac = part(rows * (inner / 2)), as = part(abi.mx4_scale_bytes(std::max<i64>(128, tile) * tiles, inner)), y = part(2 * rows * hidden);
   at::Tensor out, held;
   int rc = 0;
   {

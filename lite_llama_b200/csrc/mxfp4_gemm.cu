@@ -463,7 +463,7 @@ static int stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w
 // The same product for routed experts: tiles of up to 64 rows of one expert, {expert, rows} in a table on the device
 // (mxfp4_moe.cu), row r of tile i in row 64 i + r of x and y and in row 128 i + r of their scales.
 //
-// Tiles of 128 rows are multiplied with the rows as the MMA's (mxfp4_gemm_pair.cu), where a thread holds a row's
+// Tiles of 128 rows or more are multiplied with the rows as the MMA's (mxfp4_gemm_pair.cu), where a thread holds a row's
 // outputs: here its lane is an output, and bringing 128 columns out through shared memory took longer than the products (2000 tokens,
 // 128 experts of 2048 x 768, both products 137 us, there 82).  Tiles of 32 rows were no faster at two rows an expert (58.7 against 56.1 us).
 // Bound: the experts' weights, each read from memory once (further tiles of an expert find them in L2).  Persistent, one CTA to
@@ -737,10 +737,10 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
                                         const void* w_scales, const void* table, int64_t max_tiles, int tile_rows, int experts,
                                         int64_t n, int64_t k, int gated, int dtype, void* stream) {
   B2L_REQUIRE(max_tiles >= 0 && experts > 0 && n > 0 && k > 0 && k % 32 == 0 && k < (1ll << 30) && n * experts < (1ll << 31) &&
-                  max_tiles * cdiv64(n, 128) < (1ll << 31) && max_tiles * 128 < (1ll << 31) &&
-                  (experts * cdiv64(n, 128) + max_tiles) * mx4::k_tiles(k) < (1ll << 29),
+                  max_tiles * cdiv64(n, 128) < (1ll << 31) && max_tiles * 256 < (1ll << 31) &&
+                  (experts * cdiv64(n, 128) + 2 * max_tiles) * mx4::k_tiles(k) < (1ll << 29),
               "mxfp4_grouped_matmul: experts=%d n=%lld k=%lld (a multiple of 32) tiles=%lld", experts, (long long)n, (long long)k, (long long)max_tiles);
-  B2L_REQUIRE(tile_rows == 64 || tile_rows == 128, "mxfp4_grouped_matmul: tiles of %d rows", tile_rows);
+  B2L_REQUIRE(tile_rows == 64 || tile_rows == 128 || tile_rows == 256, "mxfp4_grouped_matmul: tiles of %d rows", tile_rows);
   if (max_tiles == 0) return B2L_OK;
   B2L_REQUIRE(y && x && x_scales && w && w_scales && table && (!gated || y_scales), "mxfp4_grouped_matmul: null pointer");
   B2L_REQUIRE(!gated || n % 128 == 0, "mxfp4_grouped_matmul: gate and up rows come in runs of 64 (n=%lld)", (long long)n);
@@ -750,7 +750,7 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
   B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "mxfp4_grouped_matmul: dtype %d", dtype);
   cudaStream_t st = (cudaStream_t)stream;
   mx4::PairCall g = {y, gated ? n / 4 : n, y_scales, nullptr, x, x_scales, w, w_scales, max_tiles, n, k, k / 2, k / 2, gated != 0, false};
-  if (tile_rows == 128) return mx4::rows_gemm(g, table, experts, dtype, st);
+  if (tile_rows != 64) return mx4::rows_gemm(g, table, tile_rows, experts, dtype, st);
   mx4::GroupedParams p;
   p.y = y; p.ldy = gated ? n / 4 : n;
   p.y_scales = (uint8_t*)y_scales; p.y_ktiles = mx4::k_tiles(n / 2);

@@ -9,8 +9,8 @@
 //     start when a quarter of the tile before has been read, and the rest is written out under them;
 //   * scales are TMA copies of whole tiles into every stage; both CTAs hold those of all 256 outputs.  Two sets of 24 columns take turns:
 //     a set is written again when the MMAs of two stages ago have retired.
-// The same kernel on single CTAs (CTAS = 1) multiplies the rows of routed experts: tiles of up to 128 rows of one expert, from a table on
-// the device, by 256 of its weight rows (a pair's 256 tokens would be half empty).
+// ROUTED: the rows of routed experts, tiles of up to 128 rows of one expert by 256 of its weight rows, from a table on the device, on single
+// CTAs (CTAS = 1); up to 256 rows on pairs, which fetch the weights once for both, where experts have so many.
 #include "gemm_tc.cuh"
 #include "mxfp4_mma.cuh"
 #include "mxfp4_gemm.cuh"
@@ -81,10 +81,10 @@ template <int CTAS> __device__ __forceinline__ void commit(uint64_t* bar) {
 }
 // A tile of outputs: token tile (index of 128 rows for each CTA), first 128 outputs and how many of those, rows that hold anything, expert
 struct Work { int m, n, width, rows, expert; };
-template <int BN, int CTAS> __device__ __forceinline__ Work work_of(const PairParams& p, int t, int rank) {
+template <int BN, int CTAS, bool ROUTED> __device__ __forceinline__ Work work_of(const PairParams& p, int t, int rank) {
   Work o;
   o.width = BN / 128;
-  if (CTAS == 2) {
+  if (!ROUTED) {
     // the tiles that would make a last wave of less than half of the pairs come in halves
     const int behind = t - p.wide;
     const PairTile pt = pair_tile(behind < 0 ? t : p.wide + (behind >> 1), p.m_tiles, p.n_tiles, kPairBand);
@@ -97,15 +97,16 @@ template <int BN, int CTAS> __device__ __forceinline__ Work work_of(const PairPa
     o.rows = p.T - o.m * kPairRows;
     o.expert = 0;
   } else {
-    o.m = t / p.n_tiles;
-    o.n = (t - o.m * p.n_tiles) * (BN / 128);
-    o.expert = ld_upstream(p.table + 1 + 2 * o.m);
-    o.rows = ld_upstream(p.table + 2 + 2 * o.m);
+    const int tile = t / p.n_tiles;
+    o.m = tile * CTAS + rank;
+    o.n = (t - tile * p.n_tiles) * (BN / 128);
+    o.expert = ld_upstream(p.table + 1 + 2 * tile);
+    o.rows = ld_upstream(p.table + 2 + 2 * tile) - rank * kPairRows;
   }
   return o;
 }
 
-template <typename T, int BN, bool GATED, int CTAS>
+template <typename T, int BN, bool GATED, int CTAS, bool ROUTED>
 __global__ void __launch_bounds__(kPairThreads, 1)
 pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_xs,
             const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_y, const PairParams p) {
@@ -145,8 +146,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
   sync_all<CTAS>();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
-  if (CTAS == 1) pdl_wait_prior();     // the table is upstream data
-  const int tiles = CTAS == 2 ? p.tiles : ld_upstream(p.table) * p.n_tiles;
+  if (ROUTED) pdl_wait_prior();        // the table is upstream data
+  const int tiles = ROUTED ? ld_upstream(p.table) * p.n_tiles : p.tiles;
 
   if (warp == 0) {
     // ===================== TMA producer: this CTA's halves of both operands, its tokens' scales, all outputs' scales =====================
@@ -168,18 +169,18 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     };
     gemm::PipeState ps(R::kStages);
     int ahead = 0;                     // stages whose weights were requested before the previous kernel has ended
-    if (CTAS == 2 && p.early && pair < tiles) {
-      const Work wk = work_of<BN, CTAS>(p, pair, (int)rank);
+    if (!ROUTED && p.early && pair < tiles) {
+      const Work wk = work_of<BN, CTAS, ROUTED>(p, pair, (int)rank);
       ahead = p.num_kb < R::kStages ? p.num_kb : R::kStages;
       if (elect_one())
         for (int s = 0; s < ahead; ++s) { expect(s); load_w(s, s, wk); }
       __syncwarp();
     }
     pdl_wait_prior();
-    Work next = pair < tiles ? work_of<BN, CTAS>(p, pair, (int)rank) : Work{0, 0, 0, 0, 0};
+    Work next = pair < tiles ? work_of<BN, CTAS, ROUTED>(p, pair, (int)rank) : Work{0, 0, 0, 0, 0};
     for (int t = pair; t < tiles; t += pairs) {
       const Work wk = next;
-      if (t + pairs < tiles) next = work_of<BN, CTAS>(p, t + pairs, (int)rank);      // table entries are asked for a tile ahead
+      if (t + pairs < tiles) next = work_of<BN, CTAS, ROUTED>(p, t + pairs, (int)rank);      // table entries are asked for a tile ahead
 #pragma unroll 1
       for (int kb = 0; kb < p.num_kb; ++kb) {
         mbar_wait(&ctl->empty[ps.stage], ps.phase ^ 1);
@@ -208,7 +209,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       int it = 0, i = 0;
       for (int t = pair; t < tiles; t += pairs, ++it) {
         const uint32_t acc = tmem + (it & 1) * R::kAcc1;
-        const uint32_t id = BN == 256 && CTAS == 2 && t >= p.wide ? idesc(128 * CTAS, 128, 0) : idesc(128 * CTAS, BN, 0);
+        const uint32_t id = BN == 256 && !ROUTED && t >= p.wide ? idesc(128 * CTAS, 128, 0) : idesc(128 * CTAS, BN, 0);
         if (BN == 256) {
           if (it >= 1) mbar_wait_spin(&ctl->freed[(it - 1) & 1], ((it - 1) >> 1) & 1);
         } else {
@@ -266,10 +267,10 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     pdl_wait_prior();                  // y may still be read upstream
     uint8_t* dst = out_stage + (quad + 4 * half) * 4096;
     int it = 0;
-    Work next = pair < tiles ? work_of<BN, CTAS>(p, pair, (int)rank) : Work{0, 0, 0, 0, 0};
+    Work next = pair < tiles ? work_of<BN, CTAS, ROUTED>(p, pair, (int)rank) : Work{0, 0, 0, 0, 0};
     for (int t = pair; t < tiles; t += pairs, ++it) {
       const Work wk = next;
-      if (t + pairs < tiles) next = work_of<BN, CTAS>(p, t + pairs, (int)rank);
+      if (t + pairs < tiles) next = work_of<BN, CTAS, ROUTED>(p, t + pairs, (int)rank);
       const int buf = it & 1, m_warp = wk.m * kPairRows + quad * 32;
       awaited = t + (BN == 256 ? 1 : 2) * pairs < tiles;
       const bool any = quad * 32 < wk.rows;             // uniform over the warp
@@ -385,7 +386,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
 }
 
 // Maps and launch, for `rows` rows of x and y in tiles of 128 and `weight_rows` rows of w
-template <typename T, int BN, bool GATED, int CTAS>
+template <typename T, int BN, bool GATED, int CTAS, bool ROUTED>
 static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t experts, int64_t tiles, cudaStream_t st) {
   using R = PairRing<BN, CTAS, GATED>;
   const int sms = b2l_num_sms();
@@ -397,7 +398,7 @@ static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t e
   // Halves for what is left of the last wave if that is at most half of one (us: 1000 x 28672 x 4096, 448 tiles
   // for 74 pairs, 54 -> 52; 300 x 28672 x 4096 32.5 -> 29.3)
   const int64_t pairs = sms / CTAS, rest = tiles % pairs;
-  p.wide = (int)(CTAS == 2 && BN == 256 && tiles > pairs && 2 * rest <= pairs ? tiles - rest : tiles);
+  p.wide = (int)(!ROUTED && BN == 256 && tiles > pairs && 2 * rest <= pairs ? tiles - rest : tiles);
   p.tiles = (int)(p.wide + 2 * (tiles - p.wide));
   const int grid = CTAS * (int)(tiles < pairs ? tiles : pairs);
   CUtensorMap tx, tw, txs, tws, ty;
@@ -409,7 +410,7 @@ static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t e
     rc = b2l_make_tmap_2d(&ty, g.y, std::is_same<T, __half>::value ? TMA_F16 : TMA_BF16, (uint64_t)rows, (uint64_t)g.N, (uint64_t)g.ldy * 2, 32, 64, true);
   if (rc != B2L_OK) return rc;
   if (GATED) ty = tx;
-  auto kern = pair_kernel<T, BN, GATED, CTAS>;
+  auto kern = pair_kernel<T, BN, GATED, CTAS, ROUTED>;
   static int configured[64] = {0};
   B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, R::kSmem, configured));
   b2l_hang_arm(st);
@@ -439,7 +440,7 @@ static int launch_pair(const PairCall& g, cudaStream_t st) {
   p.T = (int)g.T;
   p.early = g.early ? 1 : 0;
   p.m_tiles = (int)cdiv64(g.T, 2 * kPairRows);
-  return launch_rows<T, BN, GATED, 2>(g, p, g.T, 1, p.m_tiles, st);
+  return launch_rows<T, BN, GATED, 2, false>(g, p, g.T, 1, p.m_tiles, st);
 }
 
 // Up to 128 tokens half of a pair's rows are padding, and the streaming kernel is as fast or faster (65 - 128 tokens, us, streaming / pairs:
@@ -464,15 +465,20 @@ int pair_gemm(const PairCall& g, int dtype, cudaStream_t st) {
 #undef PAIR
 }
 
-// Routed experts: g.T tiles of 128 rows at most, w of `experts` stacked matrices
-int rows_gemm(const PairCall& g, const void* table, int experts, int dtype, cudaStream_t st) {
+// Routed experts: g.T tiles of 128 or 256 rows at most, w of `experts` stacked matrices
+template <int CTAS>
+static int routed(const PairCall& g, PairParams& p, int experts, int dtype, cudaStream_t st) {
+  const int64_t rows = g.T * CTAS * kPairRows;
+  if (dtype == B2L_F16)
+    return g.gated ? launch_rows<__half, 256, true, CTAS, true>(g, p, rows, experts, g.T, st) : launch_rows<__half, 256, false, CTAS, true>(g, p, rows, experts, g.T, st);
+  return g.gated ? launch_rows<__nv_bfloat16, 256, true, CTAS, true>(g, p, rows, experts, g.T, st)
+                 : launch_rows<__nv_bfloat16, 256, false, CTAS, true>(g, p, rows, experts, g.T, st);
+}
+int rows_gemm(const PairCall& g, const void* table, int tile_rows, int experts, int dtype, cudaStream_t st) {
   PairParams p;
   p.table = (const int32_t*)table;
   p.T = p.m_tiles = p.early = 0;
-  if (dtype == B2L_F16)
-    return g.gated ? launch_rows<__half, 256, true, 1>(g, p, g.T * 128, experts, g.T, st) : launch_rows<__half, 256, false, 1>(g, p, g.T * 128, experts, g.T, st);
-  return g.gated ? launch_rows<__nv_bfloat16, 256, true, 1>(g, p, g.T * 128, experts, g.T, st)
-                 : launch_rows<__nv_bfloat16, 256, false, 1>(g, p, g.T * 128, experts, g.T, st);
+  return tile_rows == 128 ? routed<1>(g, p, experts, dtype, st) : routed<2>(g, p, experts, dtype, st);
 }
 
 }  // namespace mx4

@@ -3,7 +3,7 @@
 //   out[t] = sum_j weight[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])),  e = ids[t, j]
 //
 // A slot (t, j) gets a row among its expert's; every expert's rows fill tiles of `tile` rows, and row r of tile i is row i tile + r of
-// all buffers (row 128 i + r of their scales, so that a tile's scales start on a tile of their own).  Ids that name no expert get no
+// all buffers (with 64 rows to a tile row 128 i + r of their scales, so that a tile's scales start on a tile of their own).  Ids that name no expert get no
 // row and add nothing.  A row's results do not depend on its place, so places are given out by atomics.
 #include "mxfp4.cuh"
 #include "pair.cuh"
@@ -121,7 +121,7 @@ scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const 
   if (in) load_raw(x + row * x_stride + c * 8, v);
   uint32_t byte;
   const uint32_t code = quantise_raw(v, byte);
-  const uint32_t behind = (k / 8 + 15) & ~15u, shift = 31 - __clz((int)tile);          // a tile is 64 or 128 rows
+  const uint32_t behind = (k / 8 + 15) & ~15u, half = tile == 64 ? ~63u : 0u;      // of tiles of 64 rows each has a tile of scales
   const bool scaled = (lane & 3) == 0 && c < behind;
   uint8_t* out = codes + c * 4;
   uint8_t* scale = scales + (c >> 4) * kTileBytes + ((c >> 2) & 3);
@@ -130,7 +130,7 @@ scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const 
     const int to = __shfl_sync(0xffffffffu, mine, j & 31);
     if (to < 0) continue;                              // whole warps
     if (in) *reinterpret_cast<uint32_t*>(out + (int64_t)to * (k / 2)) = code;
-    if (scaled) scale[scale_word(((int64_t)(to >> shift) << 7) + (to & ((int)tile - 1)), 0, ktiles)] = (uint8_t)byte;
+    if (scaled) scale[scale_word((int64_t)to + (to & half), 0, ktiles)] = (uint8_t)byte;
   }
 }
 
@@ -185,9 +185,14 @@ static int combine(void* out, const void* y, const void* place, const void* weig
 
 }  // namespace mx4
 
-// Rows of an expert's tile.  64: the weights are the MMA's rows, for few rows an expert; 128: the tokens are (whole call, 128 experts of 2048 x
-// 768, 64 / 128, us: two rows each 56 / 65, 24 71 / 79, 48 83 / 85, 64 95 / 89; 8 experts, 64 rows each 20.6 / 22.8, 100 23.3 / 23.2).
-extern "C" int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts) { return slots <= 800 || slots <= 48LL * experts ? 64 : 128; }
+// Rows of an expert's tile.  64: the weights are the MMA's rows, for few rows an expert (or of few outputs, n of them in the first product); 128: the
+// tokens are, in 256: on a pair of CTAs that share the weights (whole call, us, 64 / 128 / 256; 128 experts of 2048 x 768: two rows each 56 /
+// 65, 24 71 / 79, 48 83 / 85, 64 93 / 88 / 96, 256 257 / 163 / 163, 320 314 / 191 / 188, 1024 949 / 534 / 494; 8 of 4096 x 1792: 320
+// 82 / 65 / 61, 1024 208 / 139 / 132; 8 of 256 x 128, a quarter as many tiles as SMs: 512 16.5 / 19.2, half as many: 1024 22.7 / 20.0).
+extern "C" int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts, int64_t n) {
+  if (slots <= 800 || slots <= 48LL * experts || cdiv64(slots, 128) * cdiv64(n, 256) * 4 <= b2l_num_sms()) return 64;
+  return slots < 320LL * experts ? 128 : 256;
+}
 
 extern "C" int64_t b2l_mxfp4_moe_max_tiles(int64_t slots, int tile_rows, int experts) {
   if (slots <= 0 || tile_rows <= 0 || experts <= 0) return 0;
@@ -210,7 +215,7 @@ extern "C" int b2l_mxfp4_moe_sort(void* place, void* table, const void* topk_ids
 
 extern "C" int b2l_mxfp4_moe_scatter(void* codes, void* scales, const void* x, const void* place, int64_t tokens, int top_k, int tile_rows,
                                      int64_t k, int64_t x_row_stride, int dtype, void* stream) {
-  B2L_REQUIRE(tokens >= 0 && top_k > 0 && (tile_rows == 64 || tile_rows == 128) && k > 0 && k % 32 == 0 && k < (1ll << 30),
+  B2L_REQUIRE(tokens >= 0 && top_k > 0 && (tile_rows == 64 || tile_rows == 128 || tile_rows == 256) && k > 0 && k % 32 == 0 && k < (1ll << 30),
               "mxfp4_moe_scatter: tokens=%lld top_k=%d k=%lld (a multiple of 32)", (long long)tokens, top_k, (long long)k);
   if (tokens == 0) return B2L_OK;
   B2L_REQUIRE(codes && scales && x && place, "mxfp4_moe_scatter: null pointer");

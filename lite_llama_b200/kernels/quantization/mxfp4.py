@@ -323,7 +323,7 @@ def _fused_moe_mxfp4(hidden_states, w1, w2, topk_weights, topk_ids) -> torch.Ten
     x, ids, weights = _aligned(x), topk_ids.contiguous(), topk_weights.contiguous()
     with _on(x):
         L, dev, st = lib(), x.device, stream_handle()
-        tile = L.b2l_mxfp4_moe_tile_rows(slots, experts)
+        tile = L.b2l_mxfp4_moe_tile_rows(slots, experts, rows1)
         tiles = L.b2l_mxfp4_moe_max_tiles(slots, tile, experts)
         def buffer(*shape):
             return torch.empty(shape, dtype=torch.uint8, device=dev)
@@ -331,10 +331,10 @@ def _fused_moe_mxfp4(hidden_states, w1, w2, topk_weights, topk_ids) -> torch.Ten
         plan = torch.empty(slots + 1 + 2 * tiles, dtype=torch.int32, device=dev)
         place, table = plan.data_ptr(), plan.data_ptr() + 4 * slots
         check(L.b2l_mxfp4_moe_sort(place, table, ids.data_ptr(), width, slots, tile, experts, st))
-        xq, xs = buffer(tiles * tile, hidden // 2), buffer(*_tiles(128 * tiles, hidden))
+        xq, xs = buffer(tiles * tile, hidden // 2), buffer(*_tiles(max(tile, 128) * tiles, hidden))
         check(L.b2l_mxfp4_moe_scatter(xq.data_ptr(), xs.data_ptr(), x.data_ptr(), place, tokens, top_k, tile, hidden, _row_stride(x),
                                       code, st))
-        aq, as_ = buffer(tiles * tile, inner // 2), buffer(*_tiles(128 * tiles, inner))
+        aq, as_ = buffer(tiles * tile, inner // 2), buffer(*_tiles(max(tile, 128) * tiles, inner))
         check(L.b2l_mxfp4_grouped_matmul(aq.data_ptr(), as_.data_ptr(), xq.data_ptr(), xs.data_ptr(), w1.codes.data_ptr(),
                                          w1.scales.data_ptr(), table, tiles, tile, experts, rows1, hidden, 1, code, st))
         y = torch.empty((tiles * tile, hidden), dtype=dtype, device=dev)

@@ -123,9 +123,9 @@ def test_host_entries_refuse_before_any_launch():
 def test_tiles_of_experts_hold_every_split_of_the_slots():
     lib = _lib.load()
     gen = torch.Generator().manual_seed(0)
-    for slots, experts in ((1, 1), (5, 128), (256, 128), (1000, 7), (16000, 128), (33, 32)):
-        tile = lib.b2l_mxfp4_moe_tile_rows(slots, experts)
-        assert tile in (64, 128)
+    for slots, experts, rows in ((1, 1, 64), (5, 128, 64), (256, 128, 64), (6000, 150, 64), (1000, 7, 128), (16000, 128, 128), (33, 32, 64), (50000, 128, 256)):
+        tile = lib.b2l_mxfp4_moe_tile_rows(slots, experts, 1536)
+        assert tile == rows
         most = lib.b2l_mxfp4_moe_max_tiles(slots, tile, experts)
         for _ in range(20):
             skew = torch.rand(experts, generator=gen) ** 4 + 1e-9
