@@ -66,6 +66,9 @@ __device__ __forceinline__ uint32_t quantise32(float (&v)[32], uint4& codes) {
   return byte;
 }
 
+// Outputs in boxes by TMA, in rows that start anywhere, or of routed experts (in boxes)
+enum Kind { kBoxes, kRagged, kRouted };
+
 // What differs between a pair and a single CTA
 template <int CTAS> __device__ __forceinline__ void sync_all() {
   if (CTAS == 2) pair_sync_relaxed();
@@ -106,11 +109,12 @@ template <int BN, int CTAS, bool ROUTED> __device__ __forceinline__ Work work_of
   return o;
 }
 
-template <typename T, int BN, bool GATED, int CTAS, bool ROUTED>
+template <typename T, int BN, bool GATED, int CTAS, Kind KIND>
 __global__ void __launch_bounds__(kPairThreads, 1)
 pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_xs,
             const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_y, const PairParams p) {
   using R = PairRing<BN, CTAS, GATED>;
+  constexpr bool ROUTED = KIND == kRouted;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   PairControl* ctl = reinterpret_cast<PairControl*>(smem);
@@ -295,7 +299,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           if (n0 >= end || !any) continue;
           if (lane == 0) bulk_wait_read<0>();           // the store before has read the box
           __syncwarp();
-          if (p.bias) {                                 // a branch of its own: without a bias nothing of it is issued
+          if (p.bias && KIND == kBoxes) {               // a branch of its own: without a bias nothing of it is issued
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               const int n = n0 + 8 * q;                 // N is a multiple of 8
@@ -305,6 +309,15 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
               for (int e = 0; e < 8; ++e) v[8 * q + e] = __float_as_uint(__uint_as_float(v[8 * q + e]) + to_f32(b[e]));
             }
           }
+          if (p.bias && KIND == kRagged) {
+            const T* bias = reinterpret_cast<const T*>(p.bias) + n0;
+            const float b0 = n0 + lane < p.N ? to_f32(bias[lane]) : 0.f, b1 = n0 + 32 + lane < p.N ? to_f32(bias[32 + lane]) : 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              v[e] = __float_as_uint(__uint_as_float(v[e]) + __shfl_sync(0xffffffffu, b0, e));
+              v[32 + e] = __float_as_uint(__uint_as_float(v[32 + e]) + __shfl_sync(0xffffffffu, b1, e));
+            }
+          }
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             uint32_t o[4];
@@ -312,11 +325,26 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
             for (int e = 0; e < 4; ++e) o[e] = pack2<T>(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
             *reinterpret_cast<uint4*>(dst + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&tmap_y, dst, n0, m_warp);
-            bulk_commit();
+          if (KIND != kRagged) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmap_y, dst, n0, m_warp);
+              bulk_commit();
+            }
+          } else {                                      // two outputs a lane and row
+            __syncwarp();
+            const int rows = wk.rows - quad * 32, n = n0 + 2 * lane;
+            T* y = reinterpret_cast<T*>(p.y) + (int64_t)m_warp * p.ldy + n;
+            const uint8_t* src = dst + (lane & 3) * 4;
+#pragma unroll 4
+            for (int r = 0; r < 32 && r < rows; ++r, y += p.ldy) {
+              const uint32_t two = *reinterpret_cast<const uint32_t*>(src + r * 128 + (((lane >> 2) ^ (r & 7)) << 4));
+              const T* o = reinterpret_cast<const T*>(&two);
+              if (n < end) y[0] = o[0];
+              if (n + 1 < end) y[1] = o[1];
+            }
+            __syncwarp();
           }
         }
       } else {
@@ -386,7 +414,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
 }
 
 // Maps and launch, for `rows` rows of x and y in tiles of 128 and `weight_rows` rows of w
-template <typename T, int BN, bool GATED, int CTAS, bool ROUTED>
+template <typename T, int BN, bool GATED, int CTAS, Kind KIND>
 static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t experts, int64_t tiles, cudaStream_t st) {
   using R = PairRing<BN, CTAS, GATED>;
   const int sms = b2l_num_sms();
@@ -398,7 +426,7 @@ static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t e
   // Halves for what is left of the last wave if that is at most half of one (us: 1000 x 28672 x 4096, 448 tiles
   // for 74 pairs, 54 -> 52; 300 x 28672 x 4096 32.5 -> 29.3)
   const int64_t pairs = sms / CTAS, rest = tiles % pairs;
-  p.wide = (int)(!ROUTED && BN == 256 && tiles > pairs && 2 * rest <= pairs ? tiles - rest : tiles);
+  p.wide = (int)(KIND != kRouted && BN == 256 && tiles > pairs && 2 * rest <= pairs ? tiles - rest : tiles);
   p.tiles = (int)(p.wide + 2 * (tiles - p.wide));
   const int grid = CTAS * (int)(tiles < pairs ? tiles : pairs);
   CUtensorMap tx, tw, txs, tws, ty;
@@ -406,11 +434,12 @@ static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t e
   if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tw, g.w, TMA_U8, (uint64_t)(experts * g.N), (uint64_t)g.K / 2, (uint64_t)g.ldw, BN / CTAS, 128, true);
   if (rc == B2L_OK) rc = b2l_make_tmap_2d(&txs, g.x_scales, TMA_U8, (uint64_t)(cdiv64(rows, 128) * p.ktiles * 4), 128, 128, 8, 128, false);
   if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tws, g.w_scales, TMA_U8, (uint64_t)(experts * cdiv64(g.N, 128) * p.ktiles * 4), 128, 128, 8, 128, false);
-  if (rc == B2L_OK && !GATED)
+  const bool boxes = !GATED && KIND != kRagged;
+  if (rc == B2L_OK && boxes)
     rc = b2l_make_tmap_2d(&ty, g.y, std::is_same<T, __half>::value ? TMA_F16 : TMA_BF16, (uint64_t)rows, (uint64_t)g.N, (uint64_t)g.ldy * 2, 32, 64, true);
   if (rc != B2L_OK) return rc;
-  if (GATED) ty = tx;
-  auto kern = pair_kernel<T, BN, GATED, CTAS, ROUTED>;
+  if (!boxes) ty = tx;
+  auto kern = pair_kernel<T, BN, GATED, CTAS, KIND>;
   static int configured[64] = {0};
   B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, R::kSmem, configured));
   b2l_hang_arm(st);
@@ -440,16 +469,19 @@ static int launch_pair(const PairCall& g, cudaStream_t st) {
   p.T = (int)g.T;
   p.early = g.early ? 1 : 0;
   p.m_tiles = (int)cdiv64(g.T, 2 * kPairRows);
-  return launch_rows<T, BN, GATED, 2, false>(g, p, g.T, 1, p.m_tiles, st);
+  if constexpr (!GATED) {
+    // two bytes at a time: 2881 x 4563 x 7808 43 us, 63 with the streaming kernel; 2881 x 4560 x 7808 in boxes 39
+    if (g.N % 8 != 0 || g.ldy % 8 != 0 || (uintptr_t)g.y % 16 != 0 || (uintptr_t)g.bias % 16 != 0)
+      return launch_rows<T, BN, false, 2, kRagged>(g, p, g.T, 1, p.m_tiles, st);
+  }
+  return launch_rows<T, BN, GATED, 2, kBoxes>(g, p, g.T, 1, p.m_tiles, st);
 }
 
 // Up to 128 tokens half of a pair's rows are padding, and the streaming kernel is as fast or faster (65 - 128 tokens, us, streaming / pairs:
 // 28672 x 4096 14.0 - 15.2 / 16.7, 4096 x 14336 13.1 / 17.6; 2048 x 2048 5.5 / 5.2).  With few tiles and a long k it parts k over more SMs, up to 256
 // tokens: 256 x 4096 x 14336 14.3 / 17.7, 200 x 896 x 4864 6.6 / 7.8; but 256 x 4096 x 4096 9.4 / 8.1, 400 x 4096 x 14336 18.5 / 18.4.
 bool pair_wanted(const PairCall& g) {
-  if (g.T <= 128 || (g.T <= 256 && cdiv64(g.N, 128) * 4 <= b2l_num_sms() && g.K > 16 * kStageK)) return false;
-  return g.gated ? (uintptr_t)g.y % 16 == 0 && g.ldy % 16 == 0
-                 : g.N % 8 == 0 && g.ldy % 8 == 0 && (uintptr_t)g.y % 16 == 0 && (uintptr_t)g.bias % 16 == 0;
+  return g.T > 128 && !(g.T <= 256 && cdiv64(g.N, 128) * 4 <= b2l_num_sms() && g.K > 16 * kStageK);
 }
 
 int pair_gemm(const PairCall& g, int dtype, cudaStream_t st) {
@@ -470,9 +502,9 @@ template <int CTAS>
 static int routed(const PairCall& g, PairParams& p, int experts, int dtype, cudaStream_t st) {
   const int64_t rows = g.T * CTAS * kPairRows;
   if (dtype == B2L_F16)
-    return g.gated ? launch_rows<__half, 256, true, CTAS, true>(g, p, rows, experts, g.T, st) : launch_rows<__half, 256, false, CTAS, true>(g, p, rows, experts, g.T, st);
-  return g.gated ? launch_rows<__nv_bfloat16, 256, true, CTAS, true>(g, p, rows, experts, g.T, st)
-                 : launch_rows<__nv_bfloat16, 256, false, CTAS, true>(g, p, rows, experts, g.T, st);
+    return g.gated ? launch_rows<__half, 256, true, CTAS, kRouted>(g, p, rows, experts, g.T, st) : launch_rows<__half, 256, false, CTAS, kRouted>(g, p, rows, experts, g.T, st);
+  return g.gated ? launch_rows<__nv_bfloat16, 256, true, CTAS, kRouted>(g, p, rows, experts, g.T, st)
+                 : launch_rows<__nv_bfloat16, 256, false, CTAS, kRouted>(g, p, rows, experts, g.T, st);
 }
 int rows_gemm(const PairCall& g, const void* table, int tile_rows, int experts, int dtype, cudaStream_t st) {
   PairParams p;

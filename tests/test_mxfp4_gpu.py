@@ -254,6 +254,21 @@ def quantised_near(q, act, off):
 
 
 @pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t", (129, 300, 777))
+def test_outputs_of_any_number_and_place(dtype, t):
+    """Rows that start anywhere have the bits of those that start on 16 bytes, with and without a bias, wherever that lies."""
+    x, w = K.mxfp4_quantize(torch.randn(t, 512, device="cuda")), torch.randn(1024, 512, device="cuda") * 0.05
+    bias = torch.randn(1025, device="cuda").to(dtype)
+    q = K.mxfp4_quantize_weight(w)
+    for b in (None, bias[1:]):
+        want = K.mxfp4_matmul(x, q, None if b is None else b.clone(), out_dtype=dtype)
+        assert torch.equal(K.mxfp4_matmul(x, q, b, out_dtype=dtype), want)
+        for n in (1023, 1002, 700, 513, 250, 129):
+            part = K.mxfp4_quantize_weight(w[:n])
+            assert torch.equal(K.mxfp4_matmul(x, part, None if b is None else b[:n], out_dtype=dtype), want[:, :n])
+
+
+@pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("t,inner,k", ((1, 64, 64), (3, 128, 96), (32, 192, 256), (20, 4864, 896), (50, 320, 1120), (100, 448, 512), (128, 64, 2048),
                                         (129, 64, 64), (300, 320, 256), (260, 4864, 896), (1000, 5056, 352)))
 @pytest.mark.parametrize("with_bias", (False, True))
