@@ -104,8 +104,9 @@ sort_kernel(int32_t* __restrict__ place, int32_t* __restrict__ table, const void
   if (CTAS > 1) pair_sync();           // the peers have read this CTA's counters
 }
 
-// A token's row quantised once (quantize_kernel in mxfp4_quant.cu) and written to the rows of all its slots.
-template <typename T>
+// A token's row quantised once, as quantize_kernel does (mxfp4_quant.cu), and written to the rows of all its slots.
+// Two units of 256 elements to a warp (U): the lanes of a block exchange codes, so that two of them have each unit's, 8 bytes a lane.
+template <typename T, int U>
 __global__ void __launch_bounds__(256)
 scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, const int32_t* __restrict__ place,
                uint32_t tokens, int top_k, uint32_t tile, uint32_t k, int64_t x_stride, int64_t ktiles, uint32_t units) {
@@ -113,24 +114,47 @@ scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const 
   const int lane = threadIdx.x & 31;
   const uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 5), row = u / units;
   if (row >= tokens) return;                           // whole warps
-  const uint32_t c = (u - row * units) * 32 + lane;
-  const bool in = c * 8 < k;
-  Raw8<T> v;
-  zero_raw(v);
+  const uint32_t first = (u - row * units) * (32 * U), chunks = k / 8;      // chunks of eight elements
+  const T* src = x + row * x_stride + (int64_t)(first + lane) * 8;
+  Raw8<T> v[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    zero_raw(v[i]);
+    if (first + lane + 32 * i < chunks) load_raw(src + 256 * i, v[i]);
+  }
   int mine = lane < top_k ? ld_upstream(place + (int64_t)row * top_k + lane) : -1;      // the first 32 slots, a lane each
-  if (in) load_raw(x + row * x_stride + c * 8, v);
-  uint32_t byte;
-  const uint32_t code = quantise_raw(v, byte);
-  const uint32_t behind = (k / 8 + 15) & ~15u, half = tile == 64 ? ~63u : 0u;      // of tiles of 64 rows each has a tile of scales
-  const bool scaled = (lane & 3) == 0 && c < behind;
-  uint8_t* out = codes + c * 4;
-  uint8_t* scale = scales + (c >> 4) * kTileBytes + ((c >> 2) & 3);
+  uint32_t code[U], byte[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) code[i] = quantise_raw(v[i], byte[i]);
+  uint32_t block = (first + lane) >> 2;
+  uint2 both = make_uint2(code[0], 0u);
+  bool scaled = (lane & 3) == 0, in = first + lane < chunks;
+  uint32_t at = (first + lane) * 4;
+  if constexpr (U == 2) {
+    // lane 4 b + j: bytes 8 (j & 1) of block b of unit j / 2, the codes of lanes 4 b + 2 (j & 1) and the next
+    const int from = (lane & 28) | ((lane & 1) << 1);
+    const uint32_t a0 = __shfl_sync(0xffffffffu, code[0], from), a1 = __shfl_sync(0xffffffffu, code[1], from);
+    const uint32_t b0 = __shfl_sync(0xffffffffu, code[0], from + 1), b1 = __shfl_sync(0xffffffffu, code[1], from + 1);
+    const bool second = (lane & 2) != 0;
+    both = second ? make_uint2(a1, b1) : make_uint2(a0, b0);
+    if (second) { byte[0] = byte[1]; block += 8; }
+    scaled = (lane & 1) == 0;
+    in = block < k / 32;
+    at = block * 16 + (lane & 1) * 8;
+  }
+  const uint32_t half = tile == 64 ? ~63u : 0u;        // of tiles of 64 rows each has a tile of scales
+  scaled = scaled && block < ((k / 32 + 3) & ~3u);
+  uint8_t* out = codes + at;
+  uint8_t* scale = scales + (block >> 2) * kTileBytes + (block & 3);
   for (int j = 0; j < top_k; ++j) {
     if (j > 0 && (j & 31) == 0) mine = j + lane < top_k ? ld_upstream(place + (int64_t)row * top_k + j + lane) : -1;
     const int to = __shfl_sync(0xffffffffu, mine, j & 31);
     if (to < 0) continue;                              // whole warps
-    if (in) *reinterpret_cast<uint32_t*>(out + (int64_t)to * (k / 2)) = code;
-    if (scaled) scale[scale_word((int64_t)to + (to & half), 0, ktiles)] = (uint8_t)byte;
+    if (in) {
+      if (U == 2) *reinterpret_cast<uint2*>(out + (int64_t)to * (k / 2)) = both;
+      else *reinterpret_cast<uint32_t*>(out + (int64_t)to * (k / 2)) = code[0];
+    }
+    if (scaled) scale[scale_word((int64_t)to + (to & half), 0, ktiles)] = (uint8_t)byte[0];
   }
 }
 
@@ -219,12 +243,15 @@ extern "C" int b2l_mxfp4_moe_scatter(void* codes, void* scales, const void* x, c
               "mxfp4_moe_scatter: tokens=%lld top_k=%d k=%lld (a multiple of 32)", (long long)tokens, top_k, (long long)k);
   if (tokens == 0) return B2L_OK;
   B2L_REQUIRE(codes && scales && x && place, "mxfp4_moe_scatter: null pointer");
-  B2L_REQUIRE((uintptr_t)x % 16 == 0 && x_row_stride % 8 == 0 && (uintptr_t)codes % 4 == 0 && (uintptr_t)scales % 4 == 0,
+  B2L_REQUIRE((uintptr_t)x % 16 == 0 && x_row_stride % 8 == 0 && (uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0,
               "mxfp4_moe_scatter: rows must start on 16 bytes");
-  const int64_t units = cdiv64(k, 256), grid = cdiv64(tokens * units, 8);
+  // one unit a warp where there are few, or one to a row (one / two, us, 8 slots a token: 32 x 2048 2.1 / 2.2, 200 2.7 / 2.4, 2000 8.6 / 6.5, 8000
+  // 29 / 22; two slots: 2000 x 4096 8.6 / 6.2, 4000 x 256 2.5 / 2.9)
+  const int per_warp = k <= 256 || tokens * cdiv64(k, 256) < 8LL * b2l_num_sms() ? 1 : 2;
+  const int64_t units = cdiv64(k, 256 * per_warp), grid = cdiv64(tokens * units, 8);
   B2L_REQUIRE(tokens * units < (1ll << 31), "mxfp4_moe_scatter: too many tokens");
 #define SCATTER(T)                                                                                                                  \
-  b2l_launch(mx4::scatter_kernel<T>, dim3((unsigned)grid), dim3(256), (size_t)0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, \
+  b2l_launch(per_warp == 1 ? mx4::scatter_kernel<T, 1> : mx4::scatter_kernel<T, 2>, dim3((unsigned)grid), dim3(256), (size_t)0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, \
              (const T*)x, (const int32_t*)place, (uint32_t)tokens, top_k, (uint32_t)tile_rows, (uint32_t)k, x_row_stride, mx4::k_tiles(k), (uint32_t)units)
   if (dtype == B2L_F16) SCATTER(__half);
   else if (dtype == B2L_BF16) SCATTER(__nv_bfloat16);

@@ -311,7 +311,8 @@ def experts_reference(x, w1, gate, up, down, weights, ids, dtype):
 
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("experts,top_k,hidden,inner,tokens", ((4, 2, 64, 64, 1), (8, 2, 256, 128, 5), (8, 3, 96, 192, 40), (16, 2, 256, 64, 300), (3, 2, 160, 128, 129),
-                                                               (4, 4, 128, 320, 200), (5, 2, 160, 576, 700), (3, 2, 160, 576, 700)))
+                                                               (4, 4, 128, 320, 200), (5, 2, 160, 576, 700), (3, 2, 160, 576, 700),
+                                                               (8, 2, 800, 64, 400), (5, 3, 416, 576, 700)))
 def test_experts_step_by_step(dtype, experts, top_k, hidden, inner, tokens):
     x = torch.randn(tokens, hidden, device="cuda").to(dtype)
     w1, gate, up = gated_weights(inner, hidden, (experts,))
