@@ -347,14 +347,12 @@ int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scale
  * tile_rows (64, 128 or 256), row r of tile i is row i * tile_rows + r; scales of a tile start on a tile of 128
  * rows.
  * table int32 [1 + 2 * max_tiles] = {tiles, {expert, rows} per tile}.
- * _tile_rows: the tile for so many slots, n: outputs of the first product.  _scatter: x quantised into the rows of its slots.
+ * _tile_rows: the tile for so many slots, n: outputs of the first product.  _scatter: place, table, and x quantised into the rows of its slots.
  * _grouped_matmul: w [experts, n, k], buffers of max_tiles * tile_rows rows (scales: max_tiles * 128 at least); gated as in b2l_mxfp4_matmul.  _combine: out[t] = sum_j weights[t, j] * y[place[t, j]]. */
 int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts, int64_t n);
 int64_t b2l_mxfp4_moe_max_tiles(int64_t slots, int tile_rows, int experts);
-int b2l_mxfp4_moe_sort(void* place, void* table, const void* topk_ids, int id_width, int64_t slots, int tile_rows, int experts,
-                       void* stream);
-int b2l_mxfp4_moe_scatter(void* codes, void* scales, const void* x, const void* place, int64_t tokens, int top_k,
-                          int tile_rows, int64_t k, int64_t x_row_stride, int dtype, void* stream);
+int b2l_mxfp4_moe_scatter(void* place, void* table, void* codes, void* scales, const void* x, const void* topk_ids, int id_width,
+                          int64_t tokens, int top_k, int tile_rows, int experts, int64_t k, int64_t x_row_stride, int dtype, void* stream);
 int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w,
                              const void* w_scales, const void* table, int64_t max_tiles, int tile_rows, int experts,
                              int64_t n, int64_t k, int gated, int dtype, void* stream);

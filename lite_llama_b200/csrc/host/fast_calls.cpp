@@ -61,8 +61,7 @@ struct {
   i64 (*mx4_takes_16bit)(i64, i64, i64);
   i64 (*mx4_tile_rows)(i64, int, i64);
   i64 (*mx4_max_tiles)(i64, int, int);
-  int (*mx4_sort)(void*, void*, const void*, int, i64, int, int, void*);
-  int (*mx4_scatter)(void*, void*, const void*, const void*, i64, int, int, i64, i64, int, void*);
+  int (*mx4_scatter)(void*, void*, void*, void*, const void*, const void*, int, i64, int, int, int, i64, i64, int, void*);
   int (*mx4_grouped)(void*, void*, const void*, const void*, const void*, const void*, const void*, i64, int, int, i64, i64, int, int, void*);
   int (*mx4_combine)(void*, const void*, const void*, const void*, int, i64, int, i64, int, void*);
   const char* (*last_error)();
@@ -761,7 +760,7 @@ PyObject* mx4_moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
   Mx4 w1, w2;
   if (!mx4(a[1], 3, w1) || !mx4(a[2], 3, w2)) return none();
   const at::Tensor *x = plain(a[0]), *weights = plain(a[3]), *ids = plain(a[4]);
-  if (!abi.mx4_sort || !abi.mx4_scatter || !abi.mx4_combine || !abi.mx4_tile_rows || !abi.mx4_max_tiles || !abi.mx4_scale_bytes) return none();
+  if (!abi.mx4_scatter || !abi.mx4_combine || !abi.mx4_tile_rows || !abi.mx4_max_tiles || !abi.mx4_scale_bytes) return none();
   const int device = device_for(abi.mx4_grouped, {x, weights, ids, w1.codes, w1.scales, w2.codes, w2.scales});
   if (device < 0 || !mx4_rows(*x, false) || x->size(1) != w1.k) return none();
   const i64 tokens = x->size(0), hidden = w1.k, inner = w2.k, experts = w1.lead;
@@ -789,8 +788,7 @@ PyObject* mx4_moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
     out = fresh({tokens, hidden}, x->scalar_type());
     char* p = (char*)held.data_ptr();
     void* st = stream(device);
-    rc = abi.mx4_sort(p + place, p + table, ids->data_ptr(), width, slots, tile, e, st);
-    if (!rc) rc = abi.mx4_scatter(p + xc, p + xs, x->data_ptr(), p + place, tokens, top_k, tile, hidden, x->stride(0), code, st);
+    rc = abi.mx4_scatter(p + place, p + table, p + xc, p + xs, x->data_ptr(), ids->data_ptr(), width, tokens, top_k, tile, e, hidden, x->stride(0), code, st);
     if (!rc)
       rc = abi.mx4_grouped(p + ac, p + as, p + xc, p + xs, w1.codes->data_ptr(), w1.scales->data_ptr(), p + table, tiles, tile, e, w1.rows, hidden, 1,
                            code, st);

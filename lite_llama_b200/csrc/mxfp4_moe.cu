@@ -104,12 +104,36 @@ sort_kernel(int32_t* __restrict__ place, int32_t* __restrict__ table, const void
   if (CTAS > 1) pair_sync();           // the peers have read this CTA's counters
 }
 
+// What sort_kernel gives for up to 32 slots, a lane each, by one warp: the lane's place.  An expert has one tile; `write`: place and table, too.
+__device__ __forceinline__ int place_of_few(int32_t* place, int32_t* table, const void* ids, int id_width, int slots, int tile, int experts, bool write) {
+  const int lane = threadIdx.x & 31;
+  int64_t id = -1;
+  if (lane < slots) id = load_index(ids, lane, id_width);
+  const int e = id >= 0 && id < experts ? (int)id : -1;
+  const uint32_t same = __match_any_sync(0xffffffffu, e), below = (1u << lane) - 1u;
+  const uint32_t firsts = __ballot_sync(0xffffffffu, e >= 0 && (same & below) == 0u);
+  int before = 0;                      // experts with a smaller number
+  for (uint32_t left = firsts; left; left &= left - 1u) before += __shfl_sync(0xffffffffu, e, __ffs((int)left) - 1) < e;
+  const int to = e >= 0 ? before * tile + __popc(same & below) : -1;
+  if (write) {
+    if (lane < slots) place[lane] = to;
+    if (firsts >> lane & 1u) {
+      table[1 + 2 * before] = e;
+      table[2 + 2 * before] = __popc(same);
+    }
+    if (lane == 0) table[0] = __popc(firsts);
+  }
+  return to;
+}
+
 // A token's row quantised once, as quantize_kernel does (mxfp4_quant.cu), and written to the rows of all its slots.
 // Two units of 256 elements to a warp (U): the lanes of a block exchange codes, so that two of them have each unit's, 8 bytes a lane.
-template <typename T, int U>
+// FEW: every warp finds the places itself.
+template <typename T, int U, bool FEW>
 __global__ void __launch_bounds__(256)
-scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, const int32_t* __restrict__ place,
-               uint32_t tokens, int top_k, uint32_t tile, uint32_t k, int64_t x_stride, int64_t ktiles, uint32_t units) {
+scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, int32_t* __restrict__ place,
+               int32_t* __restrict__ table, const void* __restrict__ ids, int id_width, int experts, uint32_t tokens, int top_k, uint32_t tile,
+               uint32_t k, int64_t x_stride, int64_t ktiles, uint32_t units) {
   pdl_prologue();
   const int lane = threadIdx.x & 31;
   const uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 5), row = u / units;
@@ -122,7 +146,9 @@ scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const 
     zero_raw(v[i]);
     if (first + lane + 32 * i < chunks) load_raw(src + 256 * i, v[i]);
   }
-  int mine = lane < top_k ? ld_upstream(place + (int64_t)row * top_k + lane) : -1;      // the first 32 slots, a lane each
+  int mine;                            // the row's first 32 slots, a lane each; FEW: all slots
+  if (FEW) mine = place_of_few(place, table, ids, id_width, (int)tokens * top_k, (int)tile, experts, u == 0);
+  else mine = lane < top_k ? ld_upstream(place + (int64_t)row * top_k + lane) : -1;
   uint32_t code[U], byte[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) code[i] = quantise_raw(v[i], byte[i]);
@@ -147,8 +173,8 @@ scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const 
   uint8_t* out = codes + at;
   uint8_t* scale = scales + (block >> 2) * kTileBytes + (block & 3);
   for (int j = 0; j < top_k; ++j) {
-    if (j > 0 && (j & 31) == 0) mine = j + lane < top_k ? ld_upstream(place + (int64_t)row * top_k + j + lane) : -1;
-    const int to = __shfl_sync(0xffffffffu, mine, j & 31);
+    if (!FEW && j > 0 && (j & 31) == 0) mine = j + lane < top_k ? ld_upstream(place + (int64_t)row * top_k + j + lane) : -1;
+    const int to = __shfl_sync(0xffffffffu, mine, FEW ? (int)row * top_k + j : j & 31);
     if (to < 0) continue;                              // whole warps
     if (in) {
       if (U == 2) *reinterpret_cast<uint2*>(out + (int64_t)to * (k / 2)) = both;
@@ -223,39 +249,41 @@ extern "C" int64_t b2l_mxfp4_moe_max_tiles(int64_t slots, int tile_rows, int exp
   return slots / tile_rows + (slots < experts ? slots : experts);
 }
 
-extern "C" int b2l_mxfp4_moe_sort(void* place, void* table, const void* topk_ids, int id_width, int64_t slots, int tile_rows, int experts,
-                                  void* stream) {
-  B2L_REQUIRE(id_width == 4 || id_width == 8, "mxfp4_moe_sort: topk_ids must be int32 or int64");
-  B2L_REQUIRE(tile_rows > 0 && experts > 0 && experts <= 4096 && slots >= 0 && slots < (1ll << 24),
-              "mxfp4_moe_sort: bad sizes (slots=%lld tile=%d experts=%d)", (long long)slots, tile_rows, experts);
-  B2L_REQUIRE(table && (slots == 0 || (place && topk_ids)), "mxfp4_moe_sort: null pointer");
-  const bool many = slots > 4 * mx4::kSortThreads;
-  auto kern = many ? mx4::sort_kernel<4, 8> : (slots <= mx4::kSortThreads ? mx4::sort_kernel<1, 1> : mx4::sort_kernel<4, 1>);
-  b2l_launch(kern, dim3(many ? 8 : 1), dim3(mx4::kSortThreads), (size_t)experts * 8, (cudaStream_t)stream, (int32_t*)place, (int32_t*)table,
-             topk_ids, id_width, (int)slots, tile_rows, experts);
-  B2L_LAUNCH_CHECK();
-  return B2L_OK;
-}
-
-extern "C" int b2l_mxfp4_moe_scatter(void* codes, void* scales, const void* x, const void* place, int64_t tokens, int top_k, int tile_rows,
-                                     int64_t k, int64_t x_row_stride, int dtype, void* stream) {
-  B2L_REQUIRE(tokens >= 0 && top_k > 0 && (tile_rows == 64 || tile_rows == 128 || tile_rows == 256) && k > 0 && k % 32 == 0 && k < (1ll << 30),
-              "mxfp4_moe_scatter: tokens=%lld top_k=%d k=%lld (a multiple of 32)", (long long)tokens, top_k, (long long)k);
+extern "C" int b2l_mxfp4_moe_scatter(void* place, void* table, void* codes, void* scales, const void* x, const void* topk_ids, int id_width,
+                                     int64_t tokens, int top_k, int tile_rows, int experts, int64_t k, int64_t x_row_stride, int dtype,
+                                     void* stream) {
+  B2L_REQUIRE(id_width == 4 || id_width == 8, "mxfp4_moe_scatter: topk_ids must be int32 or int64");
+  B2L_REQUIRE(tokens >= 0 && top_k > 0 && top_k < (1 << 24) && tokens < (1ll << 24) && tokens * top_k < (1ll << 24) && experts > 0 && experts <= 4096,
+              "mxfp4_moe_scatter: %lld tokens of %d slots over %d experts", (long long)tokens, top_k, experts);
+  B2L_REQUIRE((tile_rows == 64 || tile_rows == 128 || tile_rows == 256) && k > 0 && k % 32 == 0 && k < (1ll << 30),
+              "mxfp4_moe_scatter: tiles of %d rows, k=%lld (a multiple of 32)", tile_rows, (long long)k);
   if (tokens == 0) return B2L_OK;
-  B2L_REQUIRE(codes && scales && x && place, "mxfp4_moe_scatter: null pointer");
+  B2L_REQUIRE(place && table && topk_ids && codes && scales && x, "mxfp4_moe_scatter: null pointer");
   B2L_REQUIRE((uintptr_t)x % 16 == 0 && x_row_stride % 8 == 0 && (uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0,
               "mxfp4_moe_scatter: rows must start on 16 bytes");
+  B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "mxfp4_moe_scatter: dtype %d", dtype);
+  const int slots = (int)(tokens * top_k);
+  // up to 32 slots in one launch (whole call, one token, two -> one, us: 8 of 128 experts of 2048 x 768 16.4 -> 14.6, 2 of 8 of 4096 x 1792 17.6 -> 15.5)
+  const bool few = slots <= 32;
   // one unit a warp where there are few, or one to a row (one / two, us, 8 slots a token: 32 x 2048 2.1 / 2.2, 200 2.7 / 2.4, 2000 8.6 / 6.5, 8000
   // 29 / 22; two slots: 2000 x 4096 8.6 / 6.2, 4000 x 256 2.5 / 2.9)
-  const int per_warp = k <= 256 || tokens * cdiv64(k, 256) < 8LL * b2l_num_sms() ? 1 : 2;
+  const int per_warp = few || k <= 256 || tokens * cdiv64(k, 256) < 8LL * b2l_num_sms() ? 1 : 2;
   const int64_t units = cdiv64(k, 256 * per_warp), grid = cdiv64(tokens * units, 8);
   B2L_REQUIRE(tokens * units < (1ll << 31), "mxfp4_moe_scatter: too many tokens");
-#define SCATTER(T)                                                                                                                  \
-  b2l_launch(per_warp == 1 ? mx4::scatter_kernel<T, 1> : mx4::scatter_kernel<T, 2>, dim3((unsigned)grid), dim3(256), (size_t)0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, \
-             (const T*)x, (const int32_t*)place, (uint32_t)tokens, top_k, (uint32_t)tile_rows, (uint32_t)k, x_row_stride, mx4::k_tiles(k), (uint32_t)units)
+  if (!few) {
+    const bool many = slots > 4 * mx4::kSortThreads;
+    auto kern = many ? mx4::sort_kernel<4, 8> : (slots <= mx4::kSortThreads ? mx4::sort_kernel<1, 1> : mx4::sort_kernel<4, 1>);
+    b2l_launch(kern, dim3(many ? 8 : 1), dim3(mx4::kSortThreads), (size_t)experts * 8, (cudaStream_t)stream, (int32_t*)place, (int32_t*)table,
+               topk_ids, id_width, slots, tile_rows, experts);
+    B2L_LAUNCH_CHECK();
+  }
+#define SCATTER(T)                                                                                                                       \
+  b2l_launch(few ? mx4::scatter_kernel<T, 1, true> : (per_warp == 1 ? mx4::scatter_kernel<T, 1, false> : mx4::scatter_kernel<T, 2, false>), \
+             dim3((unsigned)grid), dim3(256), (size_t)0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const T*)x, (int32_t*)place, \
+             (int32_t*)table, topk_ids, id_width, experts, (uint32_t)tokens, top_k, (uint32_t)tile_rows, (uint32_t)k, x_row_stride,           \
+             mx4::k_tiles(k), (uint32_t)units)
   if (dtype == B2L_F16) SCATTER(__half);
-  else if (dtype == B2L_BF16) SCATTER(__nv_bfloat16);
-  else B2L_UNSUPPORTED("mxfp4_moe_scatter: dtype %d", dtype);
+  else SCATTER(__nv_bfloat16);
 #undef SCATTER
   B2L_LAUNCH_CHECK();
   return B2L_OK;

@@ -19,7 +19,7 @@ _ABI = ("b2l_quant_gemm_workspace_bytes", "b2l_linear_workspace_bytes", "b2l_w8a
         "b2l_swiglu", "b2l_kv_int4_row_bytes", "b2l_kv_int4_write", "b2l_kv_int4_read", "b2l_flash_decoding_int4_workspace_bytes",
         "b2l_flash_decoding_int4", "b2l_flash_attention_int4_workspace_bytes", "b2l_flash_attention_int4", "b2l_slot_maps",
         "b2l_weights_written", "b2l_mxfp4_scale_bytes", "b2l_mxfp4_quantize", "b2l_mxfp4_dequantize", "b2l_skip_rmsnorm_mxfp4",
-        "b2l_mxfp4_matmul", "b2l_mxfp4_matmul_takes_16bit", "b2l_mxfp4_moe_tile_rows", "b2l_mxfp4_moe_max_tiles", "b2l_mxfp4_moe_sort", "b2l_mxfp4_moe_scatter",
+        "b2l_mxfp4_matmul", "b2l_mxfp4_matmul_takes_16bit", "b2l_mxfp4_moe_tile_rows", "b2l_mxfp4_moe_max_tiles", "b2l_mxfp4_moe_scatter",
         "b2l_mxfp4_grouped_matmul", "b2l_mxfp4_moe_combine", "b2l_last_error")
 NAMES = ("w8a16", "w4a16_packed", "linear", "w8a8", "quantize", "norm", "norm_quant", "swiglu", "kv4_rope_write", "kv4_read",
          "kv4_decode", "kv4_prompt", "slot_maps", "mx4_quantize", "mx4_dequantize", "mx4_norm", "mx4_matmul", "mx4_moe")

@@ -330,10 +330,9 @@ def _fused_moe_mxfp4(hidden_states, w1, w2, topk_weights, topk_ids) -> torch.Ten
 
         plan = torch.empty(slots + 1 + 2 * tiles, dtype=torch.int32, device=dev)
         place, table = plan.data_ptr(), plan.data_ptr() + 4 * slots
-        check(L.b2l_mxfp4_moe_sort(place, table, ids.data_ptr(), width, slots, tile, experts, st))
         xq, xs = buffer(tiles * tile, hidden // 2), buffer(*_tiles(max(tile, 128) * tiles, hidden))
-        check(L.b2l_mxfp4_moe_scatter(xq.data_ptr(), xs.data_ptr(), x.data_ptr(), place, tokens, top_k, tile, hidden, _row_stride(x),
-                                      code, st))
+        check(L.b2l_mxfp4_moe_scatter(place, table, xq.data_ptr(), xs.data_ptr(), x.data_ptr(), ids.data_ptr(), width, tokens, top_k, tile, experts,
+                                      hidden, _row_stride(x), code, st))
         aq, as_ = buffer(tiles * tile, inner // 2), buffer(*_tiles(max(tile, 128) * tiles, inner))
         check(L.b2l_mxfp4_grouped_matmul(aq.data_ptr(), as_.data_ptr(), xq.data_ptr(), xs.data_ptr(), w1.codes.data_ptr(),
                                          w1.scales.data_ptr(), table, tiles, tile, experts, rows1, hidden, 1, code, st))

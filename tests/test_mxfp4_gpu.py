@@ -338,6 +338,9 @@ def test_experts_without_tokens_the_same_twice_and_ids_of_none():
     want, off = experts_reference(x, w1, gate, up, O.rounded(down), weights, ids, torch.float16)
     got = K.fused_moe_mxfp4(x, w1, w2, weights, ids)
     assert ((got.double() - want).abs() <= off).all() and not got[5].any()
-    none = K.fused_moe_mxfp4(x, w1, w2, weights, torch.full_like(ids, -1))
-    assert not none.any()
+    for n in (1, 4, 10, 11, 70):                                         # up to 32 slots in one launch: the same rows
+        s = slice(0, n)
+        for a in (ids, ids.int()) if n < 8 else (ids,):
+            assert torch.equal(K.fused_moe_mxfp4(x[s], w1, w2, weights[s], a[s]), got[s])
+        assert not K.fused_moe_mxfp4(x[s], w1, w2, weights[s], torch.full_like(ids[s], -1)).any()
     assert K.fused_moe_mxfp4(x[:0], w1, w2, weights[:0], ids[:0]).shape == (0, hidden)

@@ -237,7 +237,7 @@ def test_two_captured_graphs_replayed_together(t):
 
 
 # ------------------------------------------------------------------------------------------------- many slots
-@pytest.mark.parametrize("tokens,top_k,experts,skew", ((1, 40, 64, False), (700, 8, 16, False), (700, 8, 16, True), (5000, 8, 300, False), (9000, 4, 5, True)))
+@pytest.mark.parametrize("tokens,top_k,experts,skew", ((1, 1, 3, False), (1, 32, 8, False), (4, 8, 128, False), (31, 1, 5, False), (2, 16, 4096, False), (1, 40, 64, False), (700, 8, 16, False), (700, 8, 16, True), (5000, 8, 300, False), (9000, 4, 5, True)))
 def test_slots_of_any_number_reach_their_experts(tokens, top_k, experts, skew):
     """Expert e multiplies by e + 1 (its weights are that many times one pattern that sums are exact for), so that a row in a wrong place shows."""
     hidden, inner = 64, 64
