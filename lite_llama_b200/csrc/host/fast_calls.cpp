@@ -68,6 +68,7 @@ struct {
 } abi;
 PyObject* py_zeroed = nullptr;      // kernels._common.zeroed_workspace(bytes, device)
 PyObject* py_counters = nullptr;    // kernels._common.counters(device)
+PyObject* py_mxfp4 = nullptr;       // kernels.quantization.mxfp4.MXFP4
 
 // ---- which calls are plain ----
 constexpr c10::DispatchKeySet kPlainKeys({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA, c10::DispatchKey::AutocastCUDA,
@@ -623,9 +624,19 @@ bool mx4_rows(const at::Tensor& x, bool wide) {
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
   return at::detail::empty_generic(sizes, c10::cuda::CUDACachingAllocator::get(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, c10::nullopt);
 }
+// MXFP4(codes, scales, False), without the class's own constructor
+PyObject* mx4_of(at::Tensor codes, at::Tensor scales) {
+  PyTypeObject* type = reinterpret_cast<PyTypeObject*>(py_mxfp4);
+  PyObject* r = type->tp_alloc(type, 3);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(codes)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(scales)));
+  PyTuple_SET_ITEM(r, 2, Py_NewRef(Py_False));
+  return r;
+}
 at::Tensor mx4_tiles(i64 rows, i64 k) { return fresh({up(rows, 128), up(k, 128), 32, 4, 4}, at::kByte); }
 
-// x -> (codes, scales)
+// x -> MXFP4
 PyObject* mx4_quantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
   ARGS(1)
   FAST_BEGIN
@@ -642,7 +653,7 @@ PyObject* mx4_quantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
     rc = abi.mx4_quantize(c.data_ptr(), s.data_ptr(), x->data_ptr(), 1, m, k, x->stride(0), x->scalar_type() == at::kFloat ? 2 : half_code(*x),
                           stream(device));
   }
-  return rc ? failed(rc) : pair_of(std::move(c), std::move(s));
+  return rc ? failed(rc) : mx4_of(std::move(c), std::move(s));
   FAST_END
 }
 
@@ -666,7 +677,7 @@ PyObject* mx4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
   FAST_END
 }
 
-// (X, residual or None, weight, eps, out_residual or None) -> (codes, scales)
+// (X, residual or None, weight, eps, out_residual or None) -> MXFP4
 PyObject* mx4_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
   ARGS(5)
   FAST_BEGIN
@@ -690,11 +701,11 @@ PyObject* mx4_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
     rc = abi.mx4_norm(c.data_ptr(), s.data_ptr(), o ? o->data_ptr() : nullptr, x->data_ptr(), r ? r->data_ptr() : nullptr, w->data_ptr(), rows, n,
                       n, n, n, (float)PyFloat_AS_DOUBLE(a[3]), half_code(*x), stream(device));
   }
-  return rc ? failed(rc) : pair_of(std::move(c), std::move(s));
+  return rc ? failed(rc) : mx4_of(std::move(c), std::move(s));
   FAST_END
 }
 
-// (x or MXFP4, MXFP4, bias or None, swiglu, out_dtype or None) -> y, with swiglu (codes, scales)
+// (x or MXFP4, MXFP4, bias or None, swiglu, out_dtype or None) -> y, with swiglu an MXFP4
 PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
   ARGS(5)
   FAST_BEGIN
@@ -749,7 +760,7 @@ PyObject* mx4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
                           biased ? bias->data_ptr() : nullptr, t, n, k, stride, k / 2, gated ? n / 4 : n, gated ? 1 : 0, 1, code, st);
   }
   if (rc) return failed(rc);
-  return gated ? pair_of(std::move(y), std::move(ys)) : THPVariable_Wrap(std::move(y));
+  return gated ? mx4_of(std::move(y), std::move(ys)) : THPVariable_Wrap(std::move(y));
   FAST_END
 }
 
@@ -801,10 +812,10 @@ PyObject* mx4_moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
   FAST_END
 }
 
-// (addresses of the C functions in the order of `abi`, zeroed_workspace, counters)
+// (addresses of the C functions in the order of `abi`, zeroed_workspace, counters, MXFP4)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t count) {
   constexpr Py_ssize_t n = sizeof(abi) / sizeof(void*);
-  if (count != n + 2) { PyErr_SetString(PyExc_TypeError, "wrong number of arguments"); return nullptr; }
+  if (count != n + 3 || !PyType_Check(a[n + 2]) || !PyType_IsSubtype((PyTypeObject*)a[n + 2], &PyTuple_Type)) { PyErr_SetString(PyExc_TypeError, "wrong number of arguments"); return nullptr; }
   for (Py_ssize_t i = 0; i < n; ++i) {
     void* p = PyLong_AsVoidPtr(a[i]);      // 0: not in this library
     if (!p && PyErr_Occurred()) return nullptr;
@@ -812,6 +823,7 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t count) {
   }
   py_zeroed = Py_NewRef(a[n]);
   py_counters = Py_NewRef(a[n + 1]);
+  py_mxfp4 = Py_NewRef(a[n + 2]);
   Py_RETURN_NONE;
 }
 

@@ -42,7 +42,8 @@ def _table() -> dict:
         return {}
     if getattr(_fast, "built_for", None) != wanted:
         return {}
-    _fast.init(*map(_address, _ABI), _common.zeroed_workspace, _common.counters)
+    from .quantization.mxfp4 import MXFP4
+    _fast.init(*map(_address, _ABI), _common.zeroed_workspace, _common.counters, MXFP4)
     return {name: getattr(_fast, name) for name in NAMES}
 
 

@@ -97,7 +97,7 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4:
     above its largest magnitude, over 4; elements are rounded to the nearest, ties to the even code, and end at 6 scales.  A block
     that holds an infinity or a NaN becomes NaN."""
     out = _native.mx4_quantize(x)
-    return _mxfp4_quantize(x) if out is None else MXFP4(*out, False)
+    return _mxfp4_quantize(x) if out is None else out
 
 
 @no_grad
@@ -180,7 +180,7 @@ def skip_rmsnorm_mxfp4(X: torch.Tensor, residual: torch.Tensor | None, weight: t
     out = _native.mx4_norm(X, residual, weight, eps, out_residual)
     if out is None:
         return _skip_rmsnorm_mxfp4(X, residual, weight, eps, out_residual)
-    return MXFP4(*out, False), X if residual is None else residual if out_residual is None else out_residual
+    return out, X if residual is None else residual if out_residual is None else out_residual
 
 
 @no_grad
@@ -223,7 +223,7 @@ def mxfp4_matmul(x: torch.Tensor | MXFP4, w: MXFP4, bias: torch.Tensor | None = 
     if isinstance(w, MXFP4) and isinstance(x, (torch.Tensor, MXFP4)):
         y = _native.mx4_matmul(x, w, bias, swiglu, out_dtype)
         if y is not None:
-            return MXFP4(*y, False) if swiglu else y
+            return y
     return _mxfp4_matmul(x, w, bias, swiglu, out_dtype)
 
 
