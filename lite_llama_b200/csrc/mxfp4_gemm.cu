@@ -481,7 +481,7 @@ struct GroupedRing {
 };
 
 struct GroupedParams {
-  void* y; int64_t ldy;                // rows of 16-bit outputs (elements) or of codes (bytes)
+  void* y; int64_t ldy;                // rows of 32-bit outputs (elements) or of codes (bytes)
   uint8_t* y_scales; int64_t y_ktiles;
   const uint8_t* x_scales; const uint8_t* w_scales;
   const int32_t* table;                // tiles, then {expert, rows} of each
@@ -494,7 +494,7 @@ struct __align__(8) GroupedControl {
   uint32_t tmem;
 };
 
-template <typename T, bool GATED>
+template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const GroupedParams p) {
   using R = GroupedRing;
@@ -627,9 +627,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         if (!GATED) {
           for (int i = tid; i < here * 32; i += 128) {
             const int r = i >> 5, n = nt * 128 + (i & 31) * 4;
-            const float4 v = *reinterpret_cast<const float4*>(out_stage + i * 4);
-            T* out = reinterpret_cast<T*>(p.y) + ((int64_t)tile * BT + c + r) * p.ldy + n;
-            if (n < p.N) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));      // N: a multiple of 8
+            if (n < p.N) stg_128(reinterpret_cast<float*>(p.y) + ((int64_t)tile * BT + c + r) * p.ldy + n, *reinterpret_cast<const uint4*>(out_stage + i * 4));
           }
         } else {
           for (int base = quad * 32; base < here * 8; base += 128) {
@@ -668,9 +666,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   }
 }
 
-template <typename T, bool GATED>
+template <bool GATED>
 static int launch_grouped(const CUtensorMap& tx, const CUtensorMap& tw, const GroupedParams& p, int64_t max_tiles, cudaStream_t st) {
-  auto kern = grouped_kernel<T, GATED>;
+  auto kern = grouped_kernel<GATED>;
   static int configured[64] = {0};
   B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, GroupedRing::kSmem, configured));
   const int64_t items = max_tiles * p.n_tiles;
@@ -680,7 +678,6 @@ static int launch_grouped(const CUtensorMap& tx, const CUtensorMap& tw, const Gr
   return B2L_OK;
 }
 
-template <typename T>
 static int grouped_gemm(const void* x, const void* w, const GroupedParams& p, int64_t max_tiles, int experts, bool is_gated,
                         cudaStream_t st) {
   CUtensorMap tx, tw;
@@ -688,7 +685,7 @@ static int grouped_gemm(const void* x, const void* w, const GroupedParams& p, in
   if (rc != B2L_OK) return rc;
   rc = b2l_make_tmap_2d(&tw, w, TMA_U8, (uint64_t)experts * p.N, (uint64_t)p.K / 2, (uint64_t)p.K / 2, 128, 128, true);
   if (rc != B2L_OK) return rc;
-  return is_gated ? launch_grouped<T, true>(tx, tw, p, max_tiles, st) : launch_grouped<T, false>(tx, tw, p, max_tiles, st);
+  return is_gated ? launch_grouped<true>(tx, tw, p, max_tiles, st) : launch_grouped<false>(tx, tw, p, max_tiles, st);
 }
 
 }  // namespace mx4
@@ -734,22 +731,21 @@ extern "C" int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const vo
 
 extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w,
                                         const void* w_scales, const void* table, int64_t max_tiles, int tile_rows, int experts,
-                                        int64_t n, int64_t k, int gated, int dtype, void* stream) {
+                                        int64_t n, int64_t k, int gated, void* stream) {
   B2L_REQUIRE(max_tiles >= 0 && experts > 0 && n > 0 && k > 0 && k % 32 == 0 && k < (1ll << 30) && n * experts < (1ll << 31) &&
                   max_tiles * cdiv64(n, 128) < (1ll << 31) && max_tiles * 256 < (1ll << 31) &&
                   (experts * cdiv64(n, 128) + 2 * max_tiles) * mx4::k_tiles(k) < (1ll << 29),
               "mxfp4_grouped_matmul: experts=%d n=%lld k=%lld (a multiple of 32) tiles=%lld", experts, (long long)n, (long long)k, (long long)max_tiles);
   B2L_REQUIRE(tile_rows == 64 || tile_rows == 128 || tile_rows == 256, "mxfp4_grouped_matmul: tiles of %d rows", tile_rows);
   if (max_tiles == 0) return B2L_OK;
-  B2L_REQUIRE(y && x && x_scales && w && w_scales && table && (!gated || y_scales), "mxfp4_grouped_matmul: null pointer");
+  B2L_REQUIRE(y && x && x_scales && w && w_scales && table && (y_scales || (!gated && tile_rows == 64)), "mxfp4_grouped_matmul: null pointer");
   B2L_REQUIRE(!gated || n % 128 == 0, "mxfp4_grouped_matmul: gate and up rows come in runs of 64 (n=%lld)", (long long)n);
-  B2L_REQUIRE(n % 8 == 0, "mxfp4_grouped_matmul: outputs are written in units of 8 (n=%lld)", (long long)n);
+  B2L_REQUIRE(n % 32 == 0, "mxfp4_grouped_matmul: outputs come in units of 32 (n=%lld)", (long long)n);
   B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales | (uintptr_t)y) % 16 == 0,
               "mxfp4_grouped_matmul: rows must start on 16 bytes");
-  B2L_REQUIRE(dtype == B2L_F16 || dtype == B2L_BF16, "mxfp4_grouped_matmul: dtype %d", dtype);
   cudaStream_t st = (cudaStream_t)stream;
   mx4::PairCall g = {y, gated ? n / 4 : n, y_scales, nullptr, x, x_scales, w, w_scales, max_tiles, n, k, k / 2, k / 2, gated != 0, false};
-  if (tile_rows != 64) return mx4::rows_gemm(g, table, tile_rows, experts, dtype, st);
+  if (tile_rows != 64) return mx4::rows_gemm(g, table, tile_rows, experts, st);
   mx4::GroupedParams p;
   p.y = y; p.ldy = gated ? n / 4 : n;
   p.y_scales = (uint8_t*)y_scales; p.y_ktiles = mx4::k_tiles(n / 2);
@@ -757,6 +753,5 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
   p.table = (const int32_t*)table;
   p.ktiles = mx4::k_tiles(k);
   p.N = (int)n; p.K = (int)k; p.num_kb = (int)cdiv64(k, mx4::kStageK); p.n_tiles = (int)cdiv64(n, 128);
-  if (dtype == B2L_F16) return mx4::grouped_gemm<__half>(x, w, p, max_tiles, experts, gated != 0, st);
-  return mx4::grouped_gemm<__nv_bfloat16>(x, w, p, max_tiles, experts, gated != 0, st);
+  return mx4::grouped_gemm(x, w, p, max_tiles, experts, gated != 0, st);
 }

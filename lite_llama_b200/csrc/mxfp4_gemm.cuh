@@ -19,6 +19,6 @@ bool pair_wanted(const PairCall& g);
 int pair_gemm(const PairCall& g, int dtype, cudaStream_t st);
 
 // the same for routed experts (T: tiles of 128 or 256 rows, N: rows of one expert's weights)
-int rows_gemm(const PairCall& g, const void* table, int tile_rows, int experts, int dtype, cudaStream_t st);
+int rows_gemm(const PairCall& g, const void* table, int tile_rows, int experts, cudaStream_t st);
 
 }  // namespace mx4

@@ -35,7 +35,7 @@ template <int BN, int CTAS, bool GATED> struct PairRing {
 
 struct PairParams {
   const void* bias;
-  uint8_t* y; uint8_t* y_scales; int64_t ldy, y_ktiles;                   // gated: codes and scales
+  uint8_t* y; uint8_t* y_scales; int64_t ldy, y_ktiles;                   // gated: codes and scales; routed: whole numbers and theirs, for 64
   const int32_t* table;                // experts: tiles, then {expert, rows} of each
   int T, N, K, num_kb, m_tiles, n_tiles, ktiles;
   int wide, tiles;                     // tiles of BN outputs; those and the halves behind them
@@ -287,6 +287,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       tc_fence_after();
       if (BN == 256 && !shared) hand_on(buf);
       if (!GATED) {
+        float2 steps = make_float2(0.f, 0.f);      // ROUTED: the scales of the two runs of 64
 #pragma unroll 1
         for (int j = 0; j < BN / 128; ++j) {
           const int c = half * (BN / 2) + (BN == 256 && buf == 0 ? 1 - j : j) * 64;
@@ -318,11 +319,39 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
               v[32 + e] = __float_as_uint(__uint_as_float(v[32 + e]) + __shfl_sync(0xffffffffu, b1, e));
             }
           }
+          float factor = 0.f;
+          if (ROUTED) {                                 // whole numbers; behind the end (N is a multiple of 32) lie other experts' sums
+            const bool full = n0 + 64 <= end;
+            float parts[8];                             // eight short chains
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              parts[e] = 0.f;
+#pragma unroll
+              for (int h = 0; h < 8; h += 2)
+                if (e < 4 || full) parts[e] = max_abs(parts[e], __uint_as_float(v[8 * e + h]), __uint_as_float(v[8 * e + h + 1]));
+            }
+            float m = max_abs(max_abs(parts[0], parts[1], parts[2]), max_abs(parts[3], parts[4], parts[5]), max_abs(parts[6], parts[7], 0.f));
+            const bool bad = !(m < INFINITY) && quad * 32 + lane < wk.rows;      // rows behind the last hold anything
+            if (bad) {
+              m = 0.f;
+#pragma unroll
+              for (int e = 0; e < 64; ++e)
+                if ((e < 32 || full) && abs_bits(__uint_as_float(v[e])) < 0x7f800000u) m = fmaxf(m, fabsf(__uint_as_float(v[e])));
+              if (m <= 0x1p-110f) m = 1.f;
+#pragma unroll
+              for (int e = 0; e < 64; ++e) v[e] = __float_as_uint(not_finite_as(__uint_as_float(v[e]), m));
+            }
+            factor = whole_factor(m);
+            ((c & 64) ? steps.y : steps.x) = m * (bad ? -1.f / kWholeMax : 1.f / kWholeMax);
+          }
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = pack2<T>(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
+            for (int e = 0; e < 4; ++e) {
+              const float a = __uint_as_float(v[8 * q + 2 * e]), b = __uint_as_float(v[8 * q + 2 * e + 1]);
+              o[e] = ROUTED ? whole2(a, b, factor) : pack2<T>(a, b);
+            }
             *reinterpret_cast<uint4*>(dst + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
           }
           if (KIND != kRagged) {
@@ -345,6 +374,18 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
               if (n + 1 < end) y[1] = o[1];
             }
             __syncwarp();
+          }
+        }
+        if (ROUTED) {
+          const int n0 = wk.n * 128 + half * 128;
+          if (n0 < end && quad * 32 + lane < wk.rows) {
+            float* out = reinterpret_cast<float*>(p.y_scales) + (int64_t)(m_warp + lane) * p.y_ktiles + (n0 >> 6);
+            if ((p.y_ktiles & 1) == 0) {
+              *reinterpret_cast<float2*>(out) = steps;
+            } else {
+              out[0] = steps.x;
+              if (n0 + 64 < end) out[1] = steps.y;
+            }
           }
         }
       } else {
@@ -419,7 +460,7 @@ static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t e
   using R = PairRing<BN, CTAS, GATED>;
   const int sms = b2l_num_sms();
   p.bias = g.bias;
-  p.y = (uint8_t*)g.y; p.y_scales = (uint8_t*)g.y_scales; p.ldy = g.ldy; p.y_ktiles = k_tiles(g.N / 2);
+  p.y = (uint8_t*)g.y; p.y_scales = (uint8_t*)g.y_scales; p.ldy = g.ldy; p.y_ktiles = KIND == kRouted && !GATED ? cdiv64(g.N, 64) : k_tiles(g.N / 2);
   p.N = (int)g.N; p.K = (int)g.K; p.num_kb = (int)cdiv64(g.K, kStageK); p.ktiles = (int)k_tiles(g.K);
   p.n_tiles = (int)cdiv64(g.N, BN);
   tiles *= p.n_tiles;
@@ -498,19 +539,14 @@ int pair_gemm(const PairCall& g, int dtype, cudaStream_t st) {
 }
 
 // Routed experts: g.T tiles of 128 or 256 rows at most, w of `experts` stacked matrices
-template <int CTAS>
-static int routed(const PairCall& g, PairParams& p, int experts, int dtype, cudaStream_t st) {
-  const int64_t rows = g.T * CTAS * kPairRows;
-  if (dtype == B2L_F16)
-    return g.gated ? launch_rows<__half, 256, true, CTAS, kRouted>(g, p, rows, experts, g.T, st) : launch_rows<__half, 256, false, CTAS, kRouted>(g, p, rows, experts, g.T, st);
-  return g.gated ? launch_rows<__nv_bfloat16, 256, true, CTAS, kRouted>(g, p, rows, experts, g.T, st)
-                 : launch_rows<__nv_bfloat16, 256, false, CTAS, kRouted>(g, p, rows, experts, g.T, st);
-}
-int rows_gemm(const PairCall& g, const void* table, int tile_rows, int experts, int dtype, cudaStream_t st) {
+int rows_gemm(const PairCall& g, const void* table, int tile_rows, int experts, cudaStream_t st) {
   PairParams p;
   p.table = (const int32_t*)table;
   p.T = p.m_tiles = p.early = 0;
-  return tile_rows == 128 ? routed<1>(g, p, experts, dtype, st) : routed<2>(g, p, experts, dtype, st);
+  const int64_t rows = g.T * tile_rows;
+  if (tile_rows == 128)
+    return g.gated ? launch_rows<__half, 256, true, 1, kRouted>(g, p, rows, experts, g.T, st) : launch_rows<__half, 256, false, 1, kRouted>(g, p, rows, experts, g.T, st);
+  return g.gated ? launch_rows<__half, 256, true, 2, kRouted>(g, p, rows, experts, g.T, st) : launch_rows<__half, 256, false, 2, kRouted>(g, p, rows, experts, g.T, st);
 }
 
 }  // namespace mx4

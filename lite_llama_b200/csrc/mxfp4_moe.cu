@@ -188,51 +188,98 @@ scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const 
   }
 }
 
-// A token's expert rows, weighted, added up in the order of its choices in 32 bits; eight outputs a thread.
-template <typename T, typename W>
+// A token's expert rows (32 bits, or WHOLE numbers and scales for 64, mxfp4.cuh), weighted, added up in the order of its choices in 32 bits; eight
+// outputs a thread.
+template <typename T, typename W, bool WHOLE>
 __global__ void __launch_bounds__(128)
-combine_kernel(T* __restrict__ out, const T* __restrict__ y, const int32_t* __restrict__ place, const W* __restrict__ weights,
-               int64_t tokens, int top_k, int64_t n) {
+combine_kernel(T* __restrict__ out, const void* __restrict__ y, const float* y_scales, const int32_t* __restrict__ place,
+               const W* __restrict__ weights, int64_t tokens, int top_k, int64_t n) {
   pdl_prologue();
   const uint32_t chunks = (uint32_t)(n / 8), i = blockIdx.x * 128 + threadIdx.x;
   if (i >= tokens * chunks) return;
-  const int64_t t = i / chunks, c = i % chunks;
+  const uint32_t t = i / chunks, c = i - t * chunks, groups = (uint32_t)((n + 63) / 64);
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int j0 = 0; j0 < top_k; j0 += 8) {              // eight rows requested together
-    uint4 q[8];
-    float w[8];
+    uint4 q[8], q2[WHOLE ? 1 : 8];
+    float w[8], s[8];
+    bool bad = false;
     int from[8];                       // all places first: one after another each would wait for the row before
 #pragma unroll
-    for (int j = 0; j < 8; ++j) from[j] = j0 + j < top_k ? ld_upstream(place + t * top_k + j0 + j) : -1;
+    for (int j = 0; j < 8; ++j) from[j] = j0 + j < top_k ? ld_upstream(place + (int64_t)t * top_k + j0 + j) : -1;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       q[j] = make_uint4(0u, 0u, 0u, 0u);
-      w[j] = 0.f;
+      w[j] = s[j] = 0.f;
+      if (!WHOLE) q2[j] = q[j];
       if (from[j] >= 0) {
-        q[j] = ldg_stream_128(y + (int64_t)from[j] * n + c * 8);
-        w[j] = to_f32(weights[t * top_k + j0 + j]);
+        const int64_t at = (int64_t)from[j] * n + c * 8;
+        if (WHOLE) {
+          q[j] = ldg_stream_128(reinterpret_cast<const int16_t*>(y) + at);
+          s[j] = y_scales[(int64_t)from[j] * groups + c / 8];
+        } else {
+          q[j] = ldg_stream_128(reinterpret_cast<const float*>(y) + at);
+          q2[j] = ldg_stream_128(reinterpret_cast<const float*>(y) + at + 4);
+        }
+        w[j] = to_f32(weights[(int64_t)t * top_k + j0 + j]);
       }
     }
+    auto add = [&](int j) {
+      const uint32_t* e = reinterpret_cast<const uint32_t*>(&q[j]);
+      if (WHOLE) {
+        const float f = w[j] * fabsf(s[j]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const T* e = reinterpret_cast<const T*>(&q[j]);
+        for (int h = 0; h < 8; ++h) {
+          // behind the exponent of 2^23 the bits are the number and 32768
+          const uint32_t b = __byte_perm(e[h / 2] ^ 0x80008000u, 0x4b004b00u, h & 1 ? 0x5432 : 0x5410);
+          sum[h] = fmaf(f, __uint_as_float(b) - 8421376.f, sum[h]);
+        }
+        bad = bad || s[j] < 0.f;
+      } else {
+        const uint32_t* e2 = reinterpret_cast<const uint32_t*>(&q2[WHOLE ? 0 : j]);
 #pragma unroll
-      for (int h = 0; h < 8; ++h) sum[h] = fmaf(w[j], to_f32(e[h]), sum[h]);
+        for (int h = 0; h < 4; ++h) {
+          sum[h] = fmaf(w[j], __uint_as_float(e[h]), sum[h]);
+          sum[4 + h] = fmaf(w[j], __uint_as_float(e2[h]), sum[4 + h]);
+        }
+      }
+    };
+    // by fours where issue is the bound, one by one where latency is
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (WHOLE || j0 + j < top_k) add(j);
+    if (j0 + 4 < top_k) {
+#pragma unroll
+      for (int j = 4; j < 8; ++j)
+        if (WHOLE || j0 + j < top_k) add(j);
+    }
+    if (WHOLE && bad) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t* e = reinterpret_cast<const uint32_t*>(&q[j]);
+#pragma unroll
+        for (int h = 0; h < 8; ++h)
+          if (s[j] < 0.f && (e[h / 2] >> (h & 1) * 16 & 0xffffu) == 0x8000u) sum[h] = NAN;
+      }
     }
   }
-  stg_128(out + t * n + c * 8, make_uint4(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]), pack2<T>(sum[6], sum[7])));
+  stg_128(out + (int64_t)t * n + c * 8, make_uint4(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]), pack2<T>(sum[6], sum[7])));
 }
 
 template <typename T>
-static int combine(void* out, const void* y, const void* place, const void* weights, int wide, int64_t tokens, int top_k, int64_t n,
-                   cudaStream_t st) {
+static int combine(void* out, const void* y, const void* y_scales, const void* place, const void* weights, int wide, int64_t tokens, int top_k,
+                   int64_t n, cudaStream_t st) {
   const dim3 grid((unsigned)cdiv64(tokens * (n / 8), 128));
-  if (wide)
-    b2l_launch(combine_kernel<T, float>, grid, dim3(128), (size_t)0, st, (T*)out, (const T*)y, (const int32_t*)place, (const float*)weights,
-               tokens, top_k, n);
-  else
-    b2l_launch(combine_kernel<T, T>, grid, dim3(128), (size_t)0, st, (T*)out, (const T*)y, (const int32_t*)place, (const T*)weights, tokens,
-               top_k, n);
+#define COMBINE(W, WHOLE)                                                                                                              \
+  b2l_launch(combine_kernel<T, W, WHOLE>, grid, dim3(128), (size_t)0, st, (T*)out, y, (const float*)y_scales, (const int32_t*)place,    \
+             (const W*)weights, tokens, top_k, n)
+  if (y_scales) {
+    if (wide) COMBINE(float, true);
+    else COMBINE(T, true);
+  } else {
+    if (wide) COMBINE(float, false);
+    else COMBINE(T, false);
+  }
+#undef COMBINE
   B2L_LAUNCH_CHECK();
   return B2L_OK;
 }
@@ -294,14 +341,14 @@ extern "C" int b2l_mxfp4_moe_scatter(void* place, void* table, void* codes, void
   return B2L_OK;
 }
 
-extern "C" int b2l_mxfp4_moe_combine(void* out, const void* y, const void* place, const void* weights, int weights_f32, int64_t tokens,
+extern "C" int b2l_mxfp4_moe_combine(void* out, const void* y, const void* y_scales, const void* place, const void* weights, int weights_f32, int64_t tokens,
                                      int top_k, int64_t n, int dtype, void* stream) {
   B2L_REQUIRE(tokens >= 0 && top_k > 0 && n > 0 && n % 8 == 0 && tokens * (n / 8) < (1ll << 31), "mxfp4_moe_combine: tokens=%lld n=%lld (a multiple of 8)",
               (long long)tokens, (long long)n);
   if (tokens == 0) return B2L_OK;
   B2L_REQUIRE(out && y && place && weights && ((uintptr_t)out | (uintptr_t)y) % 16 == 0, "mxfp4_moe_combine: null or misaligned pointer");
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == B2L_F16) return mx4::combine<__half>(out, y, place, weights, weights_f32, tokens, top_k, n, st);
-  if (dtype == B2L_BF16) return mx4::combine<__nv_bfloat16>(out, y, place, weights, weights_f32, tokens, top_k, n, st);
+  if (dtype == B2L_F16) return mx4::combine<__half>(out, y, y_scales, place, weights, weights_f32, tokens, top_k, n, st);
+  if (dtype == B2L_BF16) return mx4::combine<__nv_bfloat16>(out, y, y_scales, place, weights, weights_f32, tokens, top_k, n, st);
   B2L_UNSUPPORTED("mxfp4_moe_combine: dtype %d", dtype);
 }

@@ -287,7 +287,8 @@ def fused_moe_mxfp4(hidden_states: torch.Tensor, w1: MXFP4, w2: MXFP4, topk_weig
     ``hidden_states`` 16-bit ``[tokens, h]``; ``w1`` ``[experts, 2 inner, h]`` with rows as ``mxfp4_gate_up`` orders them, ``w2``
     ``[experts, h, inner]``; ``topk_weights`` (fp32 or the activations' type) and ``topk_ids`` (int32 or int64) ``[tokens, k]``.  Tokens are
     quantised once and sorted by expert, the activation is quantised from the first product's sums, a slot's output is
-    rounded to 16 bits before it is weighted, and the weighted sum is held in 32 bits.  Ids that name no expert add nothing."""
+    held in 32 bits, for many tokens in whole numbers up to 32767 with a 32-bit scale for 64 of them (half a step: 2^-16 of the largest), and
+    the weighted sum in 32 bits.  Ids that name no expert add nothing."""
     if isinstance(w1, MXFP4) and isinstance(w2, MXFP4):
         out = _native.mx4_moe(hidden_states, w1, w2, topk_weights, topk_ids)
         if out is not None:
@@ -335,10 +336,11 @@ def _fused_moe_mxfp4(hidden_states, w1, w2, topk_weights, topk_ids) -> torch.Ten
                                       hidden, _row_stride(x), code, st))
         aq, as_ = buffer(tiles * tile, inner // 2), buffer(*_tiles(max(tile, 128) * tiles, inner))
         check(L.b2l_mxfp4_grouped_matmul(aq.data_ptr(), as_.data_ptr(), xq.data_ptr(), xs.data_ptr(), w1.codes.data_ptr(),
-                                         w1.scales.data_ptr(), table, tiles, tile, experts, rows1, hidden, 1, code, st))
-        y = torch.empty((tiles * tile, hidden), dtype=dtype, device=dev)
-        check(L.b2l_mxfp4_grouped_matmul(y.data_ptr(), None, aq.data_ptr(), as_.data_ptr(), w2.codes.data_ptr(), w2.scales.data_ptr(),
-                                         table, tiles, tile, experts, hidden, inner, 0, code, st))
-        check(L.b2l_mxfp4_moe_combine(out.data_ptr(), y.data_ptr(), place, weights.data_ptr(), int(weights.dtype == torch.float32),
+                                         w1.scales.data_ptr(), table, tiles, tile, experts, rows1, hidden, 1, st))
+        y = torch.empty((tiles * tile, hidden), dtype=torch.float32 if tile == 64 else torch.int16, device=dev)
+        ys = None if tile == 64 else torch.empty((tiles * tile, -(-hidden // 64)), dtype=torch.float32, device=dev)
+        check(L.b2l_mxfp4_grouped_matmul(y.data_ptr(), ptr(ys), aq.data_ptr(), as_.data_ptr(), w2.codes.data_ptr(), w2.scales.data_ptr(),
+                                         table, tiles, tile, experts, hidden, inner, 0, st))
+        check(L.b2l_mxfp4_moe_combine(out.data_ptr(), y.data_ptr(), ptr(ys), place, weights.data_ptr(), int(weights.dtype == torch.float32),
                                       tokens, top_k, hidden, code, st))
     return out

@@ -67,3 +67,13 @@ def product_bound(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, dtype: torc
     sums = x.double().abs() @ w.double().abs().transpose(-1, -2)
     info = torch.finfo(dtype)
     return x.shape[-1] * 2.0 ** -23 * sums + y.abs() * info.eps / 2 + info.smallest_normal * info.eps / 2
+
+
+def slot_bound(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+    """The same for an expert's output that is held as a whole number of up to 32767 with a scale for 64: the sums' error; half a step of
+    the block's largest / 32767, which may itself be off by its sum's error; and five roundings in 32 bits on the way there and back (the
+    factor by a division of two units, the scale, its product with a weight)."""
+    sums = x.shape[-1] * 2.0 ** -23 * (x.double().abs() @ w.double().abs().transpose(-1, -2))
+    n = y.shape[-1]
+    high = torch.nn.functional.pad(y.abs() + sums, (0, -n % 64)).unflatten(-1, (-1, 64)).amax(-1).repeat_interleave(64, -1)[..., :n]
+    return sums + high / 65534 + (y.abs() + high / 65534) * 2.0 ** -20 + 2.0 ** -110

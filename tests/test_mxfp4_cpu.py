@@ -105,14 +105,15 @@ def test_host_entries_refuse_before_any_launch():
         ("16 bytes", lib.b2l_mxfp4_matmul, (p, None, p, p, p, p, None, 2, 8, 64, 24, 32, 8, 0, 0, 0, None)),
         ("quantiser first", lib.b2l_mxfp4_matmul, (p, None, p, None, p, p, None, 9, 8, 64, 64, 32, 8, 0, 0, 0, None)),
         ("dtype", lib.b2l_mxfp4_matmul, (p, None, p, p, p, p, None, 1, 8, 64, 32, 32, 8, 0, 0, 2, None)),
-        ("tiles of", lib.b2l_mxfp4_grouped_matmul, (p, None, p, p, p, p, p, 1, 16, 1, 8, 64, 0, 0, None)),
-        ("units of 8", lib.b2l_mxfp4_grouped_matmul, (p, None, p, p, p, p, p, 1, 128, 1, 12, 64, 0, 0, None)),
+        ("tiles of", lib.b2l_mxfp4_grouped_matmul, (p, p, p, p, p, p, p, 1, 16, 1, 32, 64, 0, None)),
+        ("units of 32", lib.b2l_mxfp4_grouped_matmul, (p, p, p, p, p, p, p, 1, 128, 1, 40, 64, 0, None)),
+        ("null", lib.b2l_mxfp4_grouped_matmul, (p, None, p, p, p, p, p, 1, 128, 1, 32, 64, 0, None)),
         ("over 5000 experts", lib.b2l_mxfp4_moe_scatter, (p, p, p, p, p, p, 8, 1, 1, 64, 5000, 64, 64, 0, None)),
         ("int32 or int64", lib.b2l_mxfp4_moe_scatter, (p, p, p, p, p, p, 2, 1, 1, 64, 8, 64, 64, 0, None)),
         ("16777216 tokens", lib.b2l_mxfp4_moe_scatter, (p, p, p, p, p, p, 8, 1 << 24, 1, 64, 8, 64, 64, 0, None)),
         ("tiles of 48", lib.b2l_mxfp4_moe_scatter, (p, p, p, p, p, p, 8, 1, 1, 48, 8, 64, 64, 0, None)),
         ("null", lib.b2l_mxfp4_moe_scatter, (p, p, p, p, p, None, 8, 1, 1, 64, 8, 64, 64, 0, None)),
-        ("multiple of 8", lib.b2l_mxfp4_moe_combine, (p, p, p, p, 0, 1, 1, 12, 0, None)),
+        ("multiple of 8", lib.b2l_mxfp4_moe_combine, (p, p, p, p, p, 0, 1, 1, 12, 0, None)),
     ]
     for what, entry, args in refused:
         rc = entry(*args)

@@ -304,7 +304,7 @@ def experts_reference(x, w1, gate, up, down, weights, ids, dtype):
         y = act @ down[e].t()
         w = weights[t, j].double()[:, None]
         out.index_add_(0, t, w * y)
-        off.index_add_(0, t, w.abs() * O.product_bound(act, down[e], y, dtype))
+        off.index_add_(0, t, w.abs() * O.slot_bound(act, down[e], y))
     k = ids.shape[1]
     return out, off * (1 + k * 2.0 ** -23) + k * 2.0 ** -23 * off.new_tensor(1) * out.abs() + out.abs() * torch.finfo(dtype).eps / 2 + 1e-7
 
@@ -344,3 +344,33 @@ def test_experts_without_tokens_the_same_twice_and_ids_of_none():
             assert torch.equal(K.fused_moe_mxfp4(x[s], w1, w2, weights[s], a[s]), got[s])
         assert not K.fused_moe_mxfp4(x[s], w1, w2, weights[s], torch.full_like(ids[s], -1)).any()
     assert K.fused_moe_mxfp4(x[:0], w1, w2, weights[:0], ids[:0]).shape == (0, hidden)
+
+
+@pytest.mark.parametrize("tokens,experts", ((3, 4), (70, 4), (700, 5), (700, 3)))      # tiles of 64 (one launch and two), 128 and 256 rows
+def test_bad_weights_and_tokens_reach_their_own_outputs_alone(tokens, experts):
+    hidden, inner = 160, 576
+    x = torch.randn(tokens, hidden, device="cuda").half()
+    w1, _, _ = gated_weights(inner, hidden, (experts,))
+    down = torch.randn(experts, hidden, inner, device="cuda") * 0.05
+    ids = torch.stack([torch.randperm(experts, device="cuda")[:2] for _ in range(tokens)])
+    weights = torch.rand(tokens, 2, device="cuda") + 0.1
+    ids[0] = torch.tensor([0, 1], device="cuda")
+    want = K.fused_moe_mxfp4(x, w1, K.mxfp4_quantize_weight(down), weights, ids)
+    down[1, 130, 40], down[1, 7, 3] = float("nan"), float("inf")
+    zero = torch.zeros(64, inner, device="cuda")
+    down[2, 64:128] = zero
+    down[2, 70, 5] = float("nan")                                       # nothing else in its 64 outputs
+    got = K.fused_moe_mxfp4(x, w1, K.mxfp4_quantize_weight(down), weights, ids)
+    one, two = (ids == 1).any(1), (ids == 2).any(1)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[:, 130] |= one
+    bad[:, 7] |= one
+    bad[:, 70] |= two
+    assert torch.equal(got.isnan(), bad)
+    other = ~bad
+    other[two, 64:128] = False                                          # those weights are others
+    near = (got.double() - want.double()).abs() <= 2.0 ** -9 * want.double().abs().amax()      # without the bad one a block's steps are others
+    assert near[other].all()
+    x[0, 3] = float("nan")
+    got = K.fused_moe_mxfp4(x, w1, K.mxfp4_quantize_weight(down), weights, ids)
+    assert got[0].isnan().all() and torch.equal(got[1:].isnan(), bad[1:])

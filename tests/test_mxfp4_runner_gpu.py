@@ -71,7 +71,7 @@ def checked(monkeypatch):
                 y = act @ down.t()
                 w = weights[t, j].double()[:, None]
                 want.index_add_(0, t, w * y)
-                off.index_add_(0, t, w * O.product_bound(act, down, y, out.dtype))
+                off.index_add_(0, t, w * O.slot_bound(act, down, y))
         eps = torch.finfo(out.dtype).eps
         assert ((out.double() - want).abs() <= off * 1.001 + want.abs() * eps / 2 + 1e-6 * want.abs() + torch.finfo(out.dtype).smallest_normal * eps).all()
         seen["moe"] += 1
