@@ -287,8 +287,8 @@ def fused_moe_mxfp4(hidden_states: torch.Tensor, w1: MXFP4, w2: MXFP4, topk_weig
     ``hidden_states`` 16-bit ``[tokens, h]``; ``w1`` ``[experts, 2 inner, h]`` with rows as ``mxfp4_gate_up`` orders them, ``w2``
     ``[experts, h, inner]``; ``topk_weights`` (fp32 or the activations' type) and ``topk_ids`` (int32 or int64) ``[tokens, k]``.  Tokens are
     quantised once and sorted by expert, the activation is quantised from the first product's sums, a slot's output is
-    held in 32 bits, for many tokens in whole numbers up to 32767 with a 32-bit scale for 64 of them (half a step: 2^-16 of the largest), and
-    the weighted sum in 32 bits.  Ids that name no expert add nothing."""
+    held in 32 bits, for many tokens in whole numbers up to 32767 with a 32-bit scale for 64 of them (half a step: 2^-16 of the largest; one
+    that is not finite reads as NaN), and the weighted sum in 32 bits.  Ids that name no expert add nothing."""
     if isinstance(w1, MXFP4) and isinstance(w2, MXFP4):
         out = _native.mx4_moe(hidden_states, w1, w2, topk_weights, topk_ids)
         if out is not None:
