@@ -12,8 +12,8 @@
 //                rows behind the last one hold anything.
 //
 // Scaling by a power of two is exact, so an element depends on its value alone: what is quantised from 16 bits is the same
-// bits wherever it is quantised.  Kernels that quantise what they computed in 32 bits (norm) look whether the value lies so near
-// a border that its own error could decide, and compute those blocks again in 64 bits.
+// bits wherever it is quantised.  Kernels that quantise what they computed in 32 bits (the norm, the gated unit) look whether the value lies
+// so near a border that its own error could decide, and compute those blocks again in 64 bits.
 #pragma once
 #include "common.cuh"
 #include <type_traits>
@@ -72,7 +72,12 @@ __device__ __forceinline__ void elements8(uint32_t c, float (&t)[8]) {
     t[2 * i + 1] = f.y;
   }
 }
-// the code of a scaled value in 64 bits
+// scale byte of a block by its largest magnitude in 64 bits, 2^(127 - byte), and the code of a scaled value
+__device__ __forceinline__ uint32_t scale_byte(double top) {
+  const int field = (int)((__double_as_longlong(top) >> 52) & 2047) - 1023 + 127;
+  return field > 254 ? 255u : (field > 2 ? (uint32_t)(field - 2) : 0u);
+}
+__device__ __forceinline__ double inverse_scale_64(uint32_t byte) { return __longlong_as_double((long long)(1023 + 127 - (int)byte) << 52); }
 __device__ __forceinline__ uint32_t code_of(double t) {
   const double m = fabs(t);
   const uint32_t c = (m > 0.25) + (m >= 0.75) + (m > 1.25) + (m >= 1.75) + (m > 2.5) + (m >= 3.5) + (m > 5.0);
@@ -143,16 +148,7 @@ __device__ __forceinline__ uint32_t quantise8(float (&v)[8], uint32_t& byte) {
   return byte == 255u ? 0u : c;
 }
 
-// A lane's four of a block's 32 values (eight neighbouring lanes)
-__device__ __forceinline__ uint32_t quantise4(float a, float b, float c, float d, uint32_t& byte) {
-  uint32_t m = block_max(max(max(abs_bits(a), abs_bits(b)), max(abs_bits(c), abs_bits(d))));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-  byte = scale_byte(m);
-  const float inv = inverse_scale(byte), v[8] = {a * inv, b * inv, c * inv, d * inv, 0.f, 0.f, 0.f, 0.f};
-  return byte == 255u ? 0u : codes8(v);
-}
-
-// The same of eight values as they lie in memory.  16 bits: magnitudes are compared two at a time as the whole numbers that their bits are,
+// The same of a lane's eight values as they lie in memory.  16 bits: magnitudes are compared two at a time as the whole numbers that their bits are,
 // bf16 is scaled in pairs (exact but for what is far below the smallest element): 6 instructions an element, 14 by way of 32 bits.
 template <typename T> struct Raw8 { uint4 q; };
 template <> struct Raw8<float> { uint4 q, r; };

@@ -80,19 +80,12 @@ template <typename T> __device__ __forceinline__ void store4(const Params& p, in
 // Four activations of a token from the sums of their gate and up rows, e to e + 3 of the tile's 64; eight lanes hold a block (whole warps)
 template <typename T>
 __device__ __forceinline__ void store_unit4(const Params& p, bool in, int64_t row, int tile, int e, float (&g)[4], float (&u)[4], int lane) {
-  if (in && p.bias) {
-    const T* bias = reinterpret_cast<const T*>(p.bias) + (int64_t)tile * 128 + e;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      g[j] += to_f32(bias[j]);
-      u[j] += to_f32(bias[64 + j]);
-    }
-  }
-  uint32_t byte;
-  const uint32_t code = quantise4(gated(g[0], u[0]), gated(g[1], u[1]), gated(g[2], u[2]), gated(g[3], u[3]), byte);
+  const T* bias = p.bias ? reinterpret_cast<const T*>(p.bias) + (int64_t)tile * 128 + e : nullptr;
+  uint32_t byte, code[1];
+  quantise_unit<4, T>(g, u, bias, in, code, byte);
   if (!in) return;
   const int k = tile * 64 + e;
-  *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p.y) + row * p.ldy + k / 2) = (uint16_t)code;
+  *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p.y) + row * p.ldy + k / 2) = (uint16_t)code[0];
   if ((lane & 7) == 0) {
     uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles);
     word[(k >> 5) & 3] = (uint8_t)byte;
@@ -633,19 +626,22 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
           for (int base = quad * 32; base < here * 8; base += 128) {
             const int i = base + lane, r = i >> 3, e = (i & 7) * 8;
             const bool in = i < here * 8;
-            float g[8];
+            float g[8], u[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = 0.f;
+            for (int j = 0; j < 8; ++j) g[j] = u[j] = 0.f;
             if (in) {
               const float* src = out_stage + r * 128 + e;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) g[j] = gated(src[j], src[64 + j]);
+              for (int j = 0; j < 8; ++j) {
+                g[j] = src[j];
+                u[j] = src[64 + j];
+              }
             }
-            uint32_t byte;
-            const uint32_t code = quantise8(g, byte);
+            uint32_t byte, code[1];
+            quantise_unit<8, __half>(g, u, nullptr, in, code, byte);
             if (in) {
               const int k = nt * 64 + e;
-              *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.y) + ((int64_t)tile * BT + c + r) * p.ldy + k / 2) = code;
+              *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.y) + ((int64_t)tile * BT + c + r) * p.ldy + k / 2) = code[0];
               if ((lane & 3) == 0) {
                 uint8_t* word = p.y_scales + scale_word((int64_t)tile * 128 + c + r, k >> 7, p.y_ktiles);
                 word[(k >> 5) & 3] = (uint8_t)byte;

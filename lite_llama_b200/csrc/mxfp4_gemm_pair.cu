@@ -50,22 +50,6 @@ struct __align__(8) PairControl {
   uint32_t tmem;
 };
 
-// 32 values of one row: scale byte and codes
-__device__ __forceinline__ uint32_t quantise32(float (&v)[32], uint4& codes) {
-  float m = 0.f;
-#pragma unroll
-  for (int j = 0; j < 32; j += 2) m = max_abs(m, v[j], v[j + 1]);
-  const uint32_t byte = scale_byte(abs_bits(m));
-  const float inv = inverse_scale(byte);
-#pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] *= inv;
-  uint32_t c[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) c[j] = byte == 255u ? 0u : codes8(*reinterpret_cast<float(*)[8]>(v + 8 * j));
-  codes = make_uint4(c[0], c[1], c[2], c[3]);
-  return byte;
-}
-
 // Outputs in boxes by TMA, in rows that start anywhere, or of routed experts (in boxes)
 enum Kind { kBoxes, kRagged, kRouted };
 
@@ -402,7 +386,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
         if (shared) hand_on(buf);
         const int n0 = wk.n * 128 + (BN == 256 ? c : 0), k = n0 / 2 + (BN == 256 ? 0 : half * 32), row = m_warp + lane;
         uint32_t bytes = 0;
-        uint4 codes[kBlocks];
+        uint32_t codes[kBlocks][4];
 #pragma unroll
         for (int h = 0; h < kBlocks; ++h) {
           uint32_t other[32];
@@ -416,21 +400,15 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
             v[e] = __uint_as_float(up_first ? other[e] : held[32 * h + e]);
             u[e] = __uint_as_float(up_first ? held[32 * h + e] : other[e]);
           }
-          if (p.bias && n < p.N) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              v[e] += to_f32(reinterpret_cast<const T*>(p.bias)[n + e]);
-              u[e] += to_f32(reinterpret_cast<const T*>(p.bias)[n + 64 + e]);
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = gated(v[e], u[e]);
-          bytes |= quantise32(v, codes[h]) << (8 * h);
+          const T* bias = p.bias && n < p.N ? reinterpret_cast<const T*>(p.bias) + n : nullptr;
+          uint32_t byte;
+          quantise_unit<32, T>(v, u, bias, quad * 32 + lane < wk.rows, codes[h], byte);
+          bytes |= byte << (8 * h);
         }
         if (n0 < end && quad * 32 + lane < wk.rows) {   // N is a multiple of 128
           uint8_t* y = p.y + (int64_t)row * p.ldy + k / 2;
 #pragma unroll
-          for (int h = 0; h < kBlocks; ++h) stg_128(y + 16 * h, codes[h]);
+          for (int h = 0; h < kBlocks; ++h) stg_128(y + 16 * h, make_uint4(codes[h][0], codes[h][1], codes[h][2], codes[h][3]));
           uint8_t* word = p.y_scales + scale_word(row, k >> 7, p.y_ktiles) + ((k >> 5) & 3);
           const bool last = n0 + 128 == p.N && (k & 64) == 0;      // an odd number of runs: zeros behind the end
           if (BN == 256) {

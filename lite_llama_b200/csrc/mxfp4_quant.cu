@@ -216,9 +216,8 @@ norm_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, 
       top = fmax(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmax(top, __shfl_xor_sync(0xffffffffu, top, 2));
       if ((near >> i) & 1u) {
-        const int field = (int)((__double_as_longlong(top) >> 52) & 2047) - 1023 + 127;
-        const uint32_t byte = field > 254 ? 255u : (field > 2 ? (uint32_t)(field - 2) : 0u);
-        const double scale = __longlong_as_double((long long)(1023 + 127 - (int)byte) << 52);
+        const uint32_t byte = scale_byte(top);
+        const double scale = inverse_scale_64(byte);
         uint32_t code = 0;
         if (byte != 255u)
           for (int j = 0; j < 8; ++j) code |= code_of(exact(j) * scale) << (4 * j);
