@@ -348,8 +348,9 @@ int b2l_mxfp4_matmul(void* y, void* y_scales, const void* x, const void* x_scale
  * rows.
  * table int32 [1 + 2 * max_tiles] = {tiles, {expert, rows} per tile}.
  * _tile_rows: the tile for so many slots, n: outputs of the first product.  _scatter: place, table, and x quantised into the rows of its slots.
- * _grouped_matmul: w [experts, n, k], buffers of max_tiles * tile_rows rows (scales: max_tiles * 128 at least); gated as in b2l_mxfp4_matmul, else y as
- * _combine reads it: fp32 in tiles of 64 rows (y_scales null), in others int16 with y_scales (fp32, ceil(n / 64) a row) for 64 of them; n % 32 = 0.  _combine: out[t] = sum_j weights[t, j] * y[place[t, j]]. */
+ * _grouped_matmul: w [experts, n, k], buffers of max_tiles * tile_rows rows (scales: max_tiles * 128 at least); gated as in b2l_mxfp4_matmul, else fp32
+ * sums as _combine reads them: in y in tiles of 64 rows (y_scales null), in others their upper 16 bits in y and their lower 16 in y_scales, n a row in
+ * both; n % 32 = 0.  _combine: out[t] = sum_j weights[t, j] * y[place[t, j]]; y_low: the lower 16 bits, or null. */
 int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts, int64_t n);
 int64_t b2l_mxfp4_moe_max_tiles(int64_t slots, int tile_rows, int experts);
 int b2l_mxfp4_moe_scatter(void* place, void* table, void* codes, void* scales, const void* x, const void* topk_ids, int id_width,
@@ -357,7 +358,7 @@ int b2l_mxfp4_moe_scatter(void* place, void* table, void* codes, void* scales, c
 int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, const void* x_scales, const void* w,
                              const void* w_scales, const void* table, int64_t max_tiles, int tile_rows, int experts,
                              int64_t n, int64_t k, int gated, void* stream);
-int b2l_mxfp4_moe_combine(void* out, const void* y, const void* y_scales, const void* place, const void* weights, int weights_f32, int64_t tokens,
+int b2l_mxfp4_moe_combine(void* out, const void* y, const void* y_low, const void* place, const void* weights, int weights_f32, int64_t tokens,
                           int top_k, int64_t n, int dtype, void* stream);
 
 /* ---- tensor-parallel exchange over NVLink peer memory (csrc/tp_comm.cu) ----

@@ -790,7 +790,7 @@ PyObject* mx4_moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
   i64 size = 0;
   auto part = [&](i64 n) { const i64 at = size; size += up(n, 256) * 256; return at; };
   const i64 place = part(4 * slots), table = part(4 + 8 * tiles), xc = part(rows * (hidden / 2)), xs = part(abi.mx4_scale_bytes(std::max<i64>(128, tile) * tiles, hidden)),
-            ac = part(rows * (inner / 2)), as = part(abi.mx4_scale_bytes(std::max<i64>(128, tile) * tiles, inner)), y = part((tile == 64 ? 4 : 2) * rows * hidden), ys = tile == 64 ? 0 : part(4 * rows * up(hidden, 64));
+            ac = part(rows * (inner / 2)), as = part(abi.mx4_scale_bytes(std::max<i64>(128, tile) * tiles, inner)), y = part((tile == 64 ? 4 : 2) * rows * hidden), low = tile == 64 ? 0 : part(2 * rows * hidden);
   at::Tensor out, held;
   int rc = 0;
   {
@@ -804,9 +804,9 @@ PyObject* mx4_moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
       rc = abi.mx4_grouped(p + ac, p + as, p + xc, p + xs, w1.codes->data_ptr(), w1.scales->data_ptr(), p + table, tiles, tile, e, w1.rows, hidden, 1,
                            st);
     if (!rc)
-      rc = abi.mx4_grouped(p + y, tile == 64 ? nullptr : p + ys, p + ac, p + as, w2.codes->data_ptr(), w2.scales->data_ptr(), p + table, tiles, tile, e, hidden, inner, 0,
+      rc = abi.mx4_grouped(p + y, tile == 64 ? nullptr : p + low, p + ac, p + as, w2.codes->data_ptr(), w2.scales->data_ptr(), p + table, tiles, tile, e, hidden, inner, 0,
                            st);
-    if (!rc) rc = abi.mx4_combine(out.data_ptr(), p + y, tile == 64 ? nullptr : p + ys, p + place, weights->data_ptr(), wide ? 1 : 0, tokens, top_k, hidden, code, st);
+    if (!rc) rc = abi.mx4_combine(out.data_ptr(), p + y, tile == 64 ? nullptr : p + low, p + place, weights->data_ptr(), wide ? 1 : 0, tokens, top_k, hidden, code, st);
   }
   return rc ? failed(rc) : THPVariable_Wrap(std::move(out));
   FAST_END

@@ -187,18 +187,6 @@ template <> __device__ __forceinline__ uint32_t quantise_raw<float>(const Raw8<f
   }
   return quantise8(v, byte);
 }
-// An expert row's outputs between its product and the weighted sum: whole numbers of 16 bits and a 32-bit scale for 64 of them, the largest over
-// 32767.  Half a step is 2^-16 of the largest (a tenth of what fp16 would lose on average, a hundredth of bf16) in as many bytes and a 32nd.
-// Blocks that hold an infinity or a NaN have the scale's sign set, and -32768 in those places, which are read as NaN.
-constexpr float kWholeMax = 32767.f;
-// the factor from values to whole numbers; m: the largest magnitude, finite
-__device__ __forceinline__ float whole_factor(float m) { return m > 0x1p-110f ? __fdividef(kWholeMax, m) : 0.f; }
-// two values, rounded to the nearest: the low bits behind 1.5 x 2^23
-__device__ __forceinline__ uint32_t whole2(float a, float b, float factor) {
-  return __byte_perm(__float_as_uint(fmaf(a, factor, 12582912.f)), __float_as_uint(fmaf(b, factor, 12582912.f)), 0x5410);
-}
-__device__ __forceinline__ float not_finite_as(float v, float m) { return abs_bits(v) < 0x7f800000u ? v : m * -(32768.f / kWholeMax); }
-
 template <typename T> __device__ __forceinline__ void load_raw(const T* p, Raw8<T>& x) { x.q = ldg_stream_128(p); }
 template <> __device__ __forceinline__ void load_raw<float>(const float* p, Raw8<float>& x) {
   x.q = ldg_stream_128(p);

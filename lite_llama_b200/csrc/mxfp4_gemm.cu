@@ -737,7 +737,7 @@ extern "C" int b2l_mxfp4_grouped_matmul(void* y, void* y_scales, const void* x, 
   B2L_REQUIRE(y && x && x_scales && w && w_scales && table && (y_scales || (!gated && tile_rows == 64)), "mxfp4_grouped_matmul: null pointer");
   B2L_REQUIRE(!gated || n % 128 == 0, "mxfp4_grouped_matmul: gate and up rows come in runs of 64 (n=%lld)", (long long)n);
   B2L_REQUIRE(n % 32 == 0, "mxfp4_grouped_matmul: outputs come in units of 32 (n=%lld)", (long long)n);
-  B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales | (uintptr_t)y) % 16 == 0,
+  B2L_REQUIRE(((uintptr_t)x | (uintptr_t)x_scales | (uintptr_t)w | (uintptr_t)w_scales | (uintptr_t)y | (uintptr_t)y_scales) % 16 == 0,
               "mxfp4_grouped_matmul: rows must start on 16 bytes");
   cudaStream_t st = (cudaStream_t)stream;
   mx4::PairCall g = {y, gated ? n / 4 : n, y_scales, nullptr, x, x_scales, w, w_scales, max_tiles, n, k, k / 2, k / 2, gated != 0, false};

@@ -22,12 +22,16 @@ constexpr int kPairThreads = 10 * 32;  // TMA producer, MMA issuer, eight warps 
 constexpr int kPairRows = 128;         // tokens per CTA
 constexpr int kPairBand = 16;          // token tiles per band: 16 x 256 rows x 4096 / 2 bytes = 8 MiB of L2
 
-template <int BN, int CTAS, bool GATED> struct PairRing {
-  static constexpr int kStages = CTAS == 2 ? (GATED ? 6 : 5) : (GATED ? 4 : 3);
+// Outputs in boxes by TMA, in rows that start anywhere, or of routed experts (in boxes)
+enum Kind { kBoxes, kRagged, kRouted };
+
+template <int BN, int CTAS, bool GATED, Kind KIND> struct PairRing {
+  static constexpr int kStages = CTAS == 2 ? (GATED ? 6 : (KIND == kRouted ? 4 : 5)) : (GATED ? 4 : 3);
   static constexpr int kX = 16384, kW = BN / CTAS * 128;
   static constexpr int kXs = kX + kW, kWs = kXs + kSfBytes;
   static constexpr int kBytes = kWs + BN / 128 * kSfBytes;
-  static constexpr int kSmem = 1024 + 1024 + kStages * kBytes + (GATED ? 0 : 8 * 4096);
+  static constexpr int kOut = KIND == kRouted ? 8192 : 4096;               // boxes of a warp: 32 rows of 64 outputs, 16 bits of each
+  static constexpr int kSmem = 1024 + 1024 + kStages * kBytes + (GATED ? 0 : 8 * kOut);
   static constexpr int kAcc1 = BN == 256 ? 208 : 128;                     // first column of the second accumulator
   static constexpr int kSf = BN == 256 ? 464 : 256;
   static constexpr int kSfSet = 8 + BN / 128 * 8;
@@ -35,7 +39,7 @@ template <int BN, int CTAS, bool GATED> struct PairRing {
 
 struct PairParams {
   const void* bias;
-  uint8_t* y; uint8_t* y_scales; int64_t ldy, y_ktiles;                   // gated: codes and scales; routed: whole numbers and theirs, for 64
+  uint8_t* y; uint8_t* y_scales; int64_t ldy, y_ktiles;                   // gated: codes and scales
   const int32_t* table;                // experts: tiles, then {expert, rows} of each
   int T, N, K, num_kb, m_tiles, n_tiles, ktiles;
   int wide, tiles;                     // tiles of BN outputs; those and the halves behind them
@@ -49,9 +53,6 @@ struct __align__(8) PairControl {
   uint64_t freed[2];                   // leader: all warps have read what the next tile's products overwrite
   uint32_t tmem;
 };
-
-// Outputs in boxes by TMA, in rows that start anywhere, or of routed experts (in boxes)
-enum Kind { kBoxes, kRagged, kRouted };
 
 // What differs between a pair and a single CTA
 template <int CTAS> __device__ __forceinline__ void sync_all() {
@@ -96,8 +97,9 @@ template <int BN, int CTAS, bool ROUTED> __device__ __forceinline__ Work work_of
 template <typename T, int BN, bool GATED, int CTAS, Kind KIND>
 __global__ void __launch_bounds__(kPairThreads, 1)
 pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_xs,
-            const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_y, const PairParams p) {
-  using R = PairRing<BN, CTAS, GATED>;
+            const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ CUtensorMap tmap_low,
+            const PairParams p) {
+  using R = PairRing<BN, CTAS, GATED, KIND>;
   constexpr bool ROUTED = KIND == kRouted;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -115,6 +117,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     tma_prefetch_desc(&tmap_xs);
     tma_prefetch_desc(&tmap_ws);
     if (!GATED) tma_prefetch_desc(&tmap_y);
+    if (!GATED && ROUTED) tma_prefetch_desc(&tmap_low);
     for (int s = 0; s < R::kStages; ++s) {
       mbar_init(&ctl->full[s], 1);
       mbar_init(&ctl->empty[s], 1);
@@ -253,7 +256,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       }
     };
     pdl_wait_prior();                  // y may still be read upstream
-    uint8_t* dst = out_stage + (quad + 4 * half) * 4096;
+    uint8_t* dst = out_stage + (quad + 4 * half) * R::kOut;
     int it = 0;
     Work next = pair < tiles ? work_of<BN, CTAS, ROUTED>(p, pair, (int)rank) : Work{0, 0, 0, 0, 0};
     for (int t = pair; t < tiles; t += pairs, ++it) {
@@ -271,7 +274,6 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       tc_fence_after();
       if (BN == 256 && !shared) hand_on(buf);
       if (!GATED) {
-        float2 steps = make_float2(0.f, 0.f);      // ROUTED: the scales of the two runs of 64
 #pragma unroll 1
         for (int j = 0; j < BN / 128; ++j) {
           const int c = half * (BN / 2) + (BN == 256 && buf == 0 ? 1 - j : j) * 64;
@@ -282,6 +284,31 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           if (BN == 256 ? shared && j == 0 : true) hand_on(buf);
           const int n0 = wk.n * 128 + c;
           if (n0 >= end || !any) continue;
+          if (ROUTED) {
+            // Sums stay in 32 bits, in two planes of 16 (boxes of 64 outputs, as 16-bit ones have): the upper halves, then the lower.  In 16
+            // bits, as whole numbers with a scale for 64 of them, 2000 tokens over 128 experts took 113 us instead of 133 (16000 slots written
+            // and read), but an output a thousand times its neighbours cost them all but six bits.  Two boxes and four stages on
+            // pairs, or one box and five, us: 131072 slots of 2048 x 768 706 / 722, 8192 of 4096 x 1792 143 / 138.
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (lane == 0) bulk_wait_read<1>();       // the box's store before, which is the last but one, has read it
+              __syncwarp();
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __byte_perm(v[8 * q + 2 * e], v[8 * q + 2 * e + 1], h ? 0x5410 : 0x7632);
+                *reinterpret_cast<uint4*>(dst + h * 4096 + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(h ? &tmap_low : &tmap_y, dst + h * 4096, n0, m_warp);
+                bulk_commit();
+              }
+            }
+            continue;
+          }
           if (lane == 0) bulk_wait_read<0>();           // the store before has read the box
           __syncwarp();
           if (p.bias && KIND == kBoxes) {               // a branch of its own: without a bias nothing of it is issued
@@ -303,38 +330,13 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
               v[32 + e] = __float_as_uint(__uint_as_float(v[32 + e]) + __shfl_sync(0xffffffffu, b1, e));
             }
           }
-          float factor = 0.f;
-          if (ROUTED) {                                 // whole numbers; behind the end (N is a multiple of 32) lie other experts' sums
-            const bool full = n0 + 64 <= end;
-            float parts[8];                             // eight short chains
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              parts[e] = 0.f;
-#pragma unroll
-              for (int h = 0; h < 8; h += 2)
-                if (e < 4 || full) parts[e] = max_abs(parts[e], __uint_as_float(v[8 * e + h]), __uint_as_float(v[8 * e + h + 1]));
-            }
-            float m = max_abs(max_abs(parts[0], parts[1], parts[2]), max_abs(parts[3], parts[4], parts[5]), max_abs(parts[6], parts[7], 0.f));
-            const bool bad = !(m < INFINITY) && quad * 32 + lane < wk.rows;      // rows behind the last hold anything
-            if (bad) {
-              m = 0.f;
-#pragma unroll
-              for (int e = 0; e < 64; ++e)
-                if ((e < 32 || full) && abs_bits(__uint_as_float(v[e])) < 0x7f800000u) m = fmaxf(m, fabsf(__uint_as_float(v[e])));
-              if (m <= 0x1p-110f) m = 1.f;
-#pragma unroll
-              for (int e = 0; e < 64; ++e) v[e] = __float_as_uint(not_finite_as(__uint_as_float(v[e]), m));
-            }
-            factor = whole_factor(m);
-            ((c & 64) ? steps.y : steps.x) = m * (bad ? -1.f / kWholeMax : 1.f / kWholeMax);
-          }
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             uint32_t o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float a = __uint_as_float(v[8 * q + 2 * e]), b = __uint_as_float(v[8 * q + 2 * e + 1]);
-              o[e] = ROUTED ? whole2(a, b, factor) : pack2<T>(a, b);
+              o[e] = pack2<T>(a, b);
             }
             *reinterpret_cast<uint4*>(dst + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
           }
@@ -358,18 +360,6 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
               if (n + 1 < end) y[1] = o[1];
             }
             __syncwarp();
-          }
-        }
-        if (ROUTED) {
-          const int n0 = wk.n * 128 + half * 128;
-          if (n0 < end && quad * 32 + lane < wk.rows) {
-            float* out = reinterpret_cast<float*>(p.y_scales) + (int64_t)(m_warp + lane) * p.y_ktiles + (n0 >> 6);
-            if ((p.y_ktiles & 1) == 0) {
-              *reinterpret_cast<float2*>(out) = steps;
-            } else {
-              out[0] = steps.x;
-              if (n0 + 64 < end) out[1] = steps.y;
-            }
           }
         }
       } else {
@@ -435,10 +425,10 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
 // Maps and launch, for `rows` rows of x and y in tiles of 128 and `weight_rows` rows of w
 template <typename T, int BN, bool GATED, int CTAS, Kind KIND>
 static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t experts, int64_t tiles, cudaStream_t st) {
-  using R = PairRing<BN, CTAS, GATED>;
+  using R = PairRing<BN, CTAS, GATED, KIND>;
   const int sms = b2l_num_sms();
   p.bias = g.bias;
-  p.y = (uint8_t*)g.y; p.y_scales = (uint8_t*)g.y_scales; p.ldy = g.ldy; p.y_ktiles = KIND == kRouted && !GATED ? cdiv64(g.N, 64) : k_tiles(g.N / 2);
+  p.y = (uint8_t*)g.y; p.y_scales = (uint8_t*)g.y_scales; p.ldy = g.ldy; p.y_ktiles = k_tiles(g.N / 2);
   p.N = (int)g.N; p.K = (int)g.K; p.num_kb = (int)cdiv64(g.K, kStageK); p.ktiles = (int)k_tiles(g.K);
   p.n_tiles = (int)cdiv64(g.N, BN);
   tiles *= p.n_tiles;
@@ -448,7 +438,7 @@ static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t e
   p.wide = (int)(KIND != kRouted && BN == 256 && tiles > pairs && 2 * rest <= pairs ? tiles - rest : tiles);
   p.tiles = (int)(p.wide + 2 * (tiles - p.wide));
   const int grid = CTAS * (int)(tiles < pairs ? tiles : pairs);
-  CUtensorMap tx, tw, txs, tws, ty;
+  CUtensorMap tx, tw, txs, tws, ty, tl;
   int rc = b2l_make_tmap_2d(&tx, g.x, TMA_U8, (uint64_t)rows, (uint64_t)g.K / 2, (uint64_t)g.ldx, kPairRows, 128, true);
   if (rc == B2L_OK) rc = b2l_make_tmap_2d(&tw, g.w, TMA_U8, (uint64_t)(experts * g.N), (uint64_t)g.K / 2, (uint64_t)g.ldw, BN / CTAS, 128, true);
   if (rc == B2L_OK) rc = b2l_make_tmap_2d(&txs, g.x_scales, TMA_U8, (uint64_t)(cdiv64(rows, 128) * p.ktiles * 4), 128, 128, 8, 128, false);
@@ -456,8 +446,11 @@ static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t e
   const bool boxes = !GATED && KIND != kRagged;
   if (rc == B2L_OK && boxes)
     rc = b2l_make_tmap_2d(&ty, g.y, std::is_same<T, __half>::value ? TMA_F16 : TMA_BF16, (uint64_t)rows, (uint64_t)g.N, (uint64_t)g.ldy * 2, 32, 64, true);
+  const bool low = KIND == kRouted && !GATED;
+  if (rc == B2L_OK && low) rc = b2l_make_tmap_2d(&tl, g.y_scales, TMA_F16, (uint64_t)rows, (uint64_t)g.N, (uint64_t)g.ldy * 2, 32, 64, true);
   if (rc != B2L_OK) return rc;
   if (!boxes) ty = tx;
+  if (!low) tl = ty;
   auto kern = pair_kernel<T, BN, GATED, CTAS, KIND>;
   static int configured[64] = {0};
   B2L_CUDA_CHECK(b2l_ensure_dynamic_smem(kern, R::kSmem, configured));
@@ -476,7 +469,7 @@ static int launch_rows(const PairCall& g, PairParams& p, int64_t rows, int64_t e
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = b2l_pdl_enabled() ? 2 : 1;
-  B2L_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tx, tw, txs, tws, ty, p));
+  B2L_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tx, tw, txs, tws, ty, tl, p));
   B2L_LAUNCH_CHECK();
   return B2L_OK;
 }

@@ -188,91 +188,73 @@ scatter_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const 
   }
 }
 
-// A token's expert rows (32 bits, or WHOLE numbers and scales for 64, mxfp4.cuh), weighted, added up in the order of its choices in 32 bits; eight
+// A token's expert rows (32 bits, in one piece or, SPLIT, in two planes of 16), weighted, added up in the order of its choices in 32 bits; eight
 // outputs a thread.
-template <typename T, typename W, bool WHOLE>
+template <typename T, typename W, bool SPLIT>
 __global__ void __launch_bounds__(128)
-combine_kernel(T* __restrict__ out, const void* __restrict__ y, const float* y_scales, const int32_t* __restrict__ place,
+combine_kernel(T* __restrict__ out, const void* __restrict__ y, const void* __restrict__ y_low, const int32_t* __restrict__ place,
                const W* __restrict__ weights, int64_t tokens, int top_k, int64_t n) {
   pdl_prologue();
   const uint32_t chunks = (uint32_t)(n / 8), i = blockIdx.x * 128 + threadIdx.x;
   if (i >= tokens * chunks) return;
-  const uint32_t t = i / chunks, c = i - t * chunks, groups = (uint32_t)((n + 63) / 64);
+  const uint32_t t = i / chunks, c = i - t * chunks;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int j0 = 0; j0 < top_k; j0 += 8) {              // eight rows requested together
-    uint4 q[8], q2[WHOLE ? 1 : 8];
-    float w[8], s[8];
-    bool bad = false;
+    uint4 q[8], r[8];                  // upper and lower halves, or the first four and the others
+    float w[8];
     int from[8];                       // all places first: one after another each would wait for the row before
 #pragma unroll
     for (int j = 0; j < 8; ++j) from[j] = j0 + j < top_k ? ld_upstream(place + (int64_t)t * top_k + j0 + j) : -1;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      q[j] = make_uint4(0u, 0u, 0u, 0u);
-      w[j] = s[j] = 0.f;
-      if (!WHOLE) q2[j] = q[j];
+      q[j] = r[j] = make_uint4(0u, 0u, 0u, 0u);
+      w[j] = 0.f;
       if (from[j] >= 0) {
         const int64_t at = (int64_t)from[j] * n + c * 8;
-        if (WHOLE) {
-          q[j] = ldg_stream_128(reinterpret_cast<const int16_t*>(y) + at);
-          s[j] = y_scales[(int64_t)from[j] * groups + c / 8];
+        if (SPLIT) {
+          q[j] = ldg_stream_128(reinterpret_cast<const uint16_t*>(y) + at);
+          r[j] = ldg_stream_128(reinterpret_cast<const uint16_t*>(y_low) + at);
         } else {
           q[j] = ldg_stream_128(reinterpret_cast<const float*>(y) + at);
-          q2[j] = ldg_stream_128(reinterpret_cast<const float*>(y) + at + 4);
+          r[j] = ldg_stream_128(reinterpret_cast<const float*>(y) + at + 4);
         }
         w[j] = to_f32(weights[(int64_t)t * top_k + j0 + j]);
       }
     }
     auto add = [&](int j) {
-      const uint32_t* e = reinterpret_cast<const uint32_t*>(&q[j]);
-      if (WHOLE) {
-        const float f = w[j] * fabsf(s[j]);
+      const uint32_t *a = reinterpret_cast<const uint32_t*>(&q[j]), *b = reinterpret_cast<const uint32_t*>(&r[j]);
 #pragma unroll
-        for (int h = 0; h < 8; ++h) {
-          // behind the exponent of 2^23 the bits are the number and 32768
-          const uint32_t b = __byte_perm(e[h / 2] ^ 0x80008000u, 0x4b004b00u, h & 1 ? 0x5432 : 0x5410);
-          sum[h] = fmaf(f, __uint_as_float(b) - 8421376.f, sum[h]);
-        }
-        bad = bad || s[j] < 0.f;
-      } else {
-        const uint32_t* e2 = reinterpret_cast<const uint32_t*>(&q2[WHOLE ? 0 : j]);
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          sum[h] = fmaf(w[j], __uint_as_float(e[h]), sum[h]);
-          sum[4 + h] = fmaf(w[j], __uint_as_float(e2[h]), sum[4 + h]);
+      for (int h = 0; h < 4; ++h) {
+        if (SPLIT) {
+          sum[2 * h] = fmaf(w[j], __uint_as_float(__byte_perm(b[h], a[h], 0x5410)), sum[2 * h]);
+          sum[2 * h + 1] = fmaf(w[j], __uint_as_float(__byte_perm(b[h], a[h], 0x7632)), sum[2 * h + 1]);
+        } else {
+          sum[h] = fmaf(w[j], __uint_as_float(a[h]), sum[h]);
+          sum[4 + h] = fmaf(w[j], __uint_as_float(b[h]), sum[4 + h]);
         }
       }
     };
     // by fours where issue is the bound, one by one where latency is
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (WHOLE || j0 + j < top_k) add(j);
+      if (SPLIT || j0 + j < top_k) add(j);
     if (j0 + 4 < top_k) {
 #pragma unroll
       for (int j = 4; j < 8; ++j)
-        if (WHOLE || j0 + j < top_k) add(j);
-    }
-    if (WHOLE && bad) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t* e = reinterpret_cast<const uint32_t*>(&q[j]);
-#pragma unroll
-        for (int h = 0; h < 8; ++h)
-          if (s[j] < 0.f && (e[h / 2] >> (h & 1) * 16 & 0xffffu) == 0x8000u) sum[h] = NAN;
-      }
+        if (SPLIT || j0 + j < top_k) add(j);
     }
   }
   stg_128(out + (int64_t)t * n + c * 8, make_uint4(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]), pack2<T>(sum[6], sum[7])));
 }
 
 template <typename T>
-static int combine(void* out, const void* y, const void* y_scales, const void* place, const void* weights, int wide, int64_t tokens, int top_k,
+static int combine(void* out, const void* y, const void* y_low, const void* place, const void* weights, int wide, int64_t tokens, int top_k,
                    int64_t n, cudaStream_t st) {
   const dim3 grid((unsigned)cdiv64(tokens * (n / 8), 128));
-#define COMBINE(W, WHOLE)                                                                                                              \
-  b2l_launch(combine_kernel<T, W, WHOLE>, grid, dim3(128), (size_t)0, st, (T*)out, y, (const float*)y_scales, (const int32_t*)place,    \
-             (const W*)weights, tokens, top_k, n)
-  if (y_scales) {
+#define COMBINE(W, SPLIT)                                                                                                              \
+  b2l_launch(combine_kernel<T, W, SPLIT>, grid, dim3(128), (size_t)0, st, (T*)out, y, y_low, (const int32_t*)place, (const W*)weights, tokens, \
+             top_k, n)
+  if (y_low) {
     if (wide) COMBINE(float, true);
     else COMBINE(T, true);
   } else {
@@ -287,9 +269,9 @@ static int combine(void* out, const void* y, const void* y_scales, const void* p
 }  // namespace mx4
 
 // Rows of an expert's tile.  64: the weights are the MMA's rows, for few rows an expert (or of few outputs, n of them in the first product); 128: the
-// tokens are, in 256: on a pair of CTAs that share the weights (whole call, us, 64 / 128 / 256; 128 experts of 2048 x 768: two rows each 56 /
-// 65, 24 71 / 79, 48 83 / 85, 64 93 / 88 / 96, 256 257 / 163 / 163, 320 314 / 191 / 188, 1024 949 / 534 / 494; 8 of 4096 x 1792: 320
-// 82 / 65 / 61, 1024 208 / 139 / 132; 8 of 256 x 128, a quarter as many tiles as SMs: 512 16.5 / 19.2, half as many: 1024 22.7 / 20.0).
+// tokens are, in 256: on a pair of CTAs that share the weights (whole call, us, 64 / 128 / 256; 128 experts of 2048 x 768: 24 rows each 78 / 87,
+// 48 94 / 94, 64 108 / 102 / 116, 256 318 / 209 / 212, 320 390 / 247 / 248, 1024 1191 / 702 / 708; 8 of 4096 x 1792: 320
+// 84 / 71 / 66, 1024 228 / 152 / 143; 8 of 256 x 128, a quarter as many tiles as SMs: 512 17.2 / 21.1, half as many: 1024 23.8 / 22.7).
 extern "C" int64_t b2l_mxfp4_moe_tile_rows(int64_t slots, int experts, int64_t n) {
   if (slots <= 800 || slots <= 48LL * experts || cdiv64(slots, 128) * cdiv64(n, 256) * 4 <= b2l_num_sms()) return 64;
   return slots < 320LL * experts ? 128 : 256;
@@ -341,14 +323,14 @@ extern "C" int b2l_mxfp4_moe_scatter(void* place, void* table, void* codes, void
   return B2L_OK;
 }
 
-extern "C" int b2l_mxfp4_moe_combine(void* out, const void* y, const void* y_scales, const void* place, const void* weights, int weights_f32, int64_t tokens,
+extern "C" int b2l_mxfp4_moe_combine(void* out, const void* y, const void* y_low, const void* place, const void* weights, int weights_f32, int64_t tokens,
                                      int top_k, int64_t n, int dtype, void* stream) {
   B2L_REQUIRE(tokens >= 0 && top_k > 0 && n > 0 && n % 8 == 0 && tokens * (n / 8) < (1ll << 31), "mxfp4_moe_combine: tokens=%lld n=%lld (a multiple of 8)",
               (long long)tokens, (long long)n);
   if (tokens == 0) return B2L_OK;
-  B2L_REQUIRE(out && y && place && weights && ((uintptr_t)out | (uintptr_t)y) % 16 == 0, "mxfp4_moe_combine: null or misaligned pointer");
+  B2L_REQUIRE(out && y && place && weights && ((uintptr_t)out | (uintptr_t)y | (uintptr_t)y_low) % 16 == 0, "mxfp4_moe_combine: null or misaligned pointer");
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == B2L_F16) return mx4::combine<__half>(out, y, y_scales, place, weights, weights_f32, tokens, top_k, n, st);
-  if (dtype == B2L_BF16) return mx4::combine<__nv_bfloat16>(out, y, y_scales, place, weights, weights_f32, tokens, top_k, n, st);
+  if (dtype == B2L_F16) return mx4::combine<__half>(out, y, y_low, place, weights, weights_f32, tokens, top_k, n, st);
+  if (dtype == B2L_BF16) return mx4::combine<__nv_bfloat16>(out, y, y_low, place, weights, weights_f32, tokens, top_k, n, st);
   B2L_UNSUPPORTED("mxfp4_moe_combine: dtype %d", dtype);
 }

@@ -286,9 +286,8 @@ def fused_moe_mxfp4(hidden_states: torch.Tensor, w1: MXFP4, w2: MXFP4, topk_weig
 
     ``hidden_states`` 16-bit ``[tokens, h]``; ``w1`` ``[experts, 2 inner, h]`` with rows as ``mxfp4_gate_up`` orders them, ``w2``
     ``[experts, h, inner]``; ``topk_weights`` (fp32 or the activations' type) and ``topk_ids`` (int32 or int64) ``[tokens, k]``.  Tokens are
-    quantised once and sorted by expert, the activation is quantised from the first product's sums, a slot's output is
-    held in 32 bits, for many tokens in whole numbers up to 32767 with a 32-bit scale for 64 of them (half a step: 2^-16 of the largest; one
-    that is not finite reads as NaN), and the weighted sum in 32 bits.  Ids that name no expert add nothing."""
+    quantised once and sorted by expert, the activation is quantised from the first product's sums, and a slot's output and the weighted sum
+    are held in 32 bits.  Ids that name no expert add nothing."""
     if isinstance(w1, MXFP4) and isinstance(w2, MXFP4):
         out = _native.mx4_moe(hidden_states, w1, w2, topk_weights, topk_ids)
         if out is not None:
@@ -337,10 +336,11 @@ def _fused_moe_mxfp4(hidden_states, w1, w2, topk_weights, topk_ids) -> torch.Ten
         aq, as_ = buffer(tiles * tile, inner // 2), buffer(*_tiles(max(tile, 128) * tiles, inner))
         check(L.b2l_mxfp4_grouped_matmul(aq.data_ptr(), as_.data_ptr(), xq.data_ptr(), xs.data_ptr(), w1.codes.data_ptr(),
                                          w1.scales.data_ptr(), table, tiles, tile, experts, rows1, hidden, 1, st))
+        # 32 bits a sum; in tiles of 128 rows or more the upper and the lower halves by themselves
         y = torch.empty((tiles * tile, hidden), dtype=torch.float32 if tile == 64 else torch.int16, device=dev)
-        ys = None if tile == 64 else torch.empty((tiles * tile, -(-hidden // 64)), dtype=torch.float32, device=dev)
-        check(L.b2l_mxfp4_grouped_matmul(y.data_ptr(), ptr(ys), aq.data_ptr(), as_.data_ptr(), w2.codes.data_ptr(), w2.scales.data_ptr(),
+        low = None if tile == 64 else torch.empty_like(y)
+        check(L.b2l_mxfp4_grouped_matmul(y.data_ptr(), ptr(low), aq.data_ptr(), as_.data_ptr(), w2.codes.data_ptr(), w2.scales.data_ptr(),
                                          table, tiles, tile, experts, hidden, inner, 0, st))
-        check(L.b2l_mxfp4_moe_combine(out.data_ptr(), y.data_ptr(), ptr(ys), place, weights.data_ptr(), int(weights.dtype == torch.float32),
+        check(L.b2l_mxfp4_moe_combine(out.data_ptr(), y.data_ptr(), ptr(low), place, weights.data_ptr(), int(weights.dtype == torch.float32),
                                       tokens, top_k, hidden, code, st))
     return out
