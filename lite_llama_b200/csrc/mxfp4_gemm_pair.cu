@@ -134,7 +134,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     pdl_launch_dependents();           // after the allocation (gemm_dense.cu)
   }
   tc_fence_before();
-  sync_all<CTAS>();
+  __syncthreads();                     // the allocation's store to shared memory, which the relaxed barrier does not show
+  if (CTAS == 2) pair_sync_relaxed();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
   if (ROUTED) pdl_wait_prior();        // the table is upstream data

@@ -28,8 +28,8 @@ __device__ __forceinline__ void pair_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The same without a release: for what needs no ordinary store to be seen (barriers initialised behind mbar_fence_init, tensor memory, peers
-// that have read their last word of this CTA's shared memory).  A release waits for the CTA's stores to global memory, 1500 cycles at
-// the end of a kernel.
+// that have read their last word of this CTA's shared memory).  What the CTA's own warps stored, the address of its tensor memory for one,
+// wants a __syncthreads() beside it.  A release waits for the CTA's stores to global memory, 1500 cycles at the end of a kernel.
 __device__ __forceinline__ void pair_sync_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
