@@ -133,8 +133,11 @@ def make_moe_weights(cfg: ModelConfig, router, gate, up, down, method: str, tp: 
     lo, hi = rank * il, (rank + 1) * il
     kw = dict(top_k=cfg.num_experts_per_tok, norm_topk_prob=cfg.norm_topk_prob)
     if method == "mxfp4":
-        w1 = mxfp4_quantize_weight(mxfp4_gate_up(gate[:, lo:hi], up[:, lo:hi]).to(dtype))
-        return MoeWeights(router.to(dtype), w1, mxfp4_quantize_weight(down[:, :, lo:hi].to(dtype)), **kw)
+        # gate and up rows come in runs of 64: a shard of another size (768 / 8 = 96) is filled up with zeros, which add nothing
+        more = -il % 64
+        g, u = (torch.nn.functional.pad(t[:, lo:hi], (0, 0, 0, more)) if more else t[:, lo:hi] for t in (gate, up))
+        d = torch.nn.functional.pad(down[:, :, lo:hi], (0, more)) if more else down[:, :, lo:hi]
+        return MoeWeights(router.to(dtype), mxfp4_quantize_weight(mxfp4_gate_up(g, u).to(dtype)), mxfp4_quantize_weight(d.to(dtype)), **kw)
     if method != "fp8":
         w1 = torch.cat([gate[:, lo:hi], up[:, lo:hi]], dim=1).to(dtype).contiguous()
         return MoeWeights(router.to(dtype), w1, down[:, :, lo:hi].to(dtype).contiguous(), **kw)
