@@ -324,7 +324,8 @@ int b2l_moe_route_topk(void* topk_weights, void* topk_ids_i64, const void* route
  * Format and layout: csrc/mxfp4.cuh.  codes: rows of k / 2 bytes; scales: b2l_mxfp4_scale_bytes(rows, k) bytes per matrix, in tiles
  * of 128 rows x 128 elements.  k is a multiple of 32; rows start on 16 bytes.  Strides of codes are in bytes.
  * b2l_mxfp4_quantize / _dequantize: `matrices` stacked matrices of `rows` rows; fp16, bf16 or fp32.
- * b2l_skip_rmsnorm_mxfp4: sum = x + residual (sum may be residual; residual null: sum is not written), then the RMS norm of it
+ * b2l_skip_rmsnorm_mxfp4: sum = x + residual (sum may be x or residual, row for row, and overlaps neither otherwise; residual null: sum is not
+ * written), then the RMS norm of it
  * times weight, quantised; n <= 16384.
  * b2l_mxfp4_matmul: y[t, n] = x . w (+ bias), 16-bit; x_scales null (where b2l_mxfp4_matmul_takes_16bit says so): x holds elements of
  * dtype, its stride counts them, and the product quantises them itself; gated: silu(gate) * up quantised into y (codes, row stride in bytes)

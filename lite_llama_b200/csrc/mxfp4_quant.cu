@@ -258,6 +258,22 @@ static int launch_norm(void* codes, void* scales, void* sum, const void* x, cons
   return B2L_OK;
 }
 
+// Whether sums may be written while rows of `in` are read: each over its own row, or where no row lies.  Strides in bytes, rows of `bytes`.
+static bool writable(const void* sum, int64_t s_stride, const void* in, int64_t stride, int64_t rows, int64_t bytes) {
+  if (!in || rows == 0) return true;
+  if (rows == 1) stride = s_stride = bytes;
+  if (sum == in && stride == s_stride) return true;
+  int64_t s = (int64_t)(intptr_t)sum, x = (int64_t)(intptr_t)in;
+  const int64_t end = s + (rows - 1) * s_stride + bytes;
+  if (stride < 0) {
+    x += (rows - 1) * stride;
+    stride = -stride;
+  }
+  int64_t row = 0;                     // the first that ends behind the sums' start
+  if (x + bytes <= s) row = stride == 0 ? rows : (s - x - bytes) / stride + 1;
+  return row >= rows || x + row * stride >= end;
+}
+
 }  // namespace mx4
 
 extern "C" int64_t b2l_mxfp4_scale_bytes(int64_t rows, int64_t k) {
@@ -319,10 +335,18 @@ extern "C" int b2l_skip_rmsnorm_mxfp4(void* codes, void* scales, void* sum, cons
   B2L_REQUIRE(((uintptr_t)x | (uintptr_t)residual | (uintptr_t)sum | (uintptr_t)weight) % 16 == 0 &&
                   (x_row_stride | r_row_stride | s_row_stride) % 8 == 0 && (uintptr_t)codes % 4 == 0 && (uintptr_t)scales % 4 == 0,
               "skip_rmsnorm_mxfp4: rows must start on 16 bytes");
+  if (residual) {
+    B2L_REQUIRE(s_row_stride >= n || rows == 1, "skip_rmsnorm_mxfp4: the sums' rows overlap");
+    B2L_REQUIRE(mx4::writable(sum, 2 * s_row_stride, x, 2 * x_row_stride, rows, 2 * n) &&
+                    mx4::writable(sum, 2 * s_row_stride, residual, 2 * r_row_stride, rows, 2 * n),
+                "skip_rmsnorm_mxfp4: the sums overlap other rows than their own of what is read");
+  }
+  if (dtype != B2L_F16 && dtype != B2L_BF16) B2L_UNSUPPORTED("skip_rmsnorm_mxfp4: dtype %d", dtype);
+  B2L_REQUIRE(!residual || (const char*)weight + 2 * n <= (const char*)sum ||
+                  (const char*)sum + 2 * ((rows == 1 ? 0 : (rows - 1) * s_row_stride) + n) <= (const char*)weight,
+              "skip_rmsnorm_mxfp4: the sums overlap the weight");
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == B2L_F16)
     return mx4::launch_norm<__half>(codes, scales, sum, x, residual, weight, rows, n, x_row_stride, r_row_stride, s_row_stride, eps, st);
-  if (dtype == B2L_BF16)
-    return mx4::launch_norm<__nv_bfloat16>(codes, scales, sum, x, residual, weight, rows, n, x_row_stride, r_row_stride, s_row_stride, eps, st);
-  B2L_UNSUPPORTED("skip_rmsnorm_mxfp4: dtype %d", dtype);
+  return mx4::launch_norm<__nv_bfloat16>(codes, scales, sum, x, residual, weight, rows, n, x_row_stride, r_row_stride, s_row_stride, eps, st);
 }

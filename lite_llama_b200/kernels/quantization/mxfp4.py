@@ -175,6 +175,7 @@ def skip_rmsnorm_mxfp4(X: torch.Tensor, residual: torch.Tensor | None, weight: t
     """``(q, residual)``: ``residual += X`` in place (or into ``out_residual``), ``q`` the RMS norm of it times ``weight`` in the
     format, ``[rows, n]`` with the leading dimensions joined.  ``residual=None``: the norm of ``X``, which comes back as the second value.
 
+    What is written may lie in the place of ``X`` or ``residual``, row by row; another overlap is refused.
     The norm is not rounded to 16 bits before it is quantised (:func:`~lite_llama_b200.kernels.skip_rmsnorm` rounds twice), and
     decides borders as exact arithmetic does.  n: a multiple of 32, at most 16384."""
     out = _native.mx4_norm(X, residual, weight, eps, out_residual)
