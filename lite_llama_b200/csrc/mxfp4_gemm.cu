@@ -458,7 +458,7 @@ static int stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w
 //
 // Tiles of 128 rows or more are multiplied with the rows as the MMA's (mxfp4_gemm_pair.cu), where a thread holds a row's
 // outputs: here its lane is an output, and bringing 128 columns out through shared memory took longer than the products (2000 tokens,
-// 128 experts of 2048 x 768, both products 137 us, there 82).  Tiles of 32 rows were no faster at two rows an expert (58.7 against 56.1 us).
+// 128 experts of 2048 x 768, both products 137 us, there 100).  Tiles of 32 rows were no faster at two rows an expert (58.7 against 56.1 us).
 // Bound: the experts' weights, each read from memory once (further tiles of an expert find them in L2).  Persistent, one CTA to
 // an SM with 180 KiB of copies in flight, the accumulator in two buffers: a tile's end overlaps the next one's products.
 // ---------------------------------------------------------------------------------------------------------------

@@ -500,7 +500,8 @@ bool pair_wanted(const PairCall& g) {
 int pair_gemm(const PairCall& g, int dtype, cudaStream_t st) {
   const int64_t m_tiles = cdiv64(g.T, 2 * kPairRows), pairs = b2l_num_sms() / 2;
   // Waves x tile width is what the grid spends on the tensor pipe, and a narrow tile fetches its tokens twice as often (256 -> 128 outputs, us:
-  // 600 x 2048 x 2048 6.2 -> 5.3, 777 x 4608 x 3584 9.2 -> 10.7, three waves for two 1000 x 6144 x 4096 14.7 -> 15.4, gated 16.0 -> 15.7).
+  // 600 x 2048 x 2048 6.2 -> 5.3, 777 x 4608 x 3584 9.2 -> 10.7, three waves for two 1000 x 6144 x 4096 14.2 -> 16.5; gated
+  // 16.2 -> 17.2, 400 x 9728 x 896 9.6 -> 8.2).
   const int64_t w256 = cdiv64(m_tiles * cdiv64(g.N, 256), pairs) * 256, w128 = cdiv64(m_tiles * cdiv64(g.N, 128), pairs) * 128;
   const bool narrow = w128 * (g.gated ? 130 : 140) < w256 * 100;
 #define PAIR(T) (narrow ? (g.gated ? launch_pair<T, 128, true>(g, st) : launch_pair<T, 128, false>(g, st)) \

@@ -24,7 +24,7 @@ class MXFP4(NamedTuple):
 
     ``codes`` uint8 ``[..., rows, k / 2]``, element 2i in the low half of byte i; ``scales`` uint8
     ``[..., ceil(rows / 128), ceil(k / 128), 32, 4, 4]``, indices row % 32, row % 128 / 32, block % 4: the order the tensor cores read
-    (``mxfp4_pack`` makes it from scales in rows).  ``ready``: nothing that is still running on the GPU writes it, so that a product
+    (``mxfp4_pack`` makes it from scales in rows; blocks behind ``k`` are 0, rows behind the last hold anything).  ``ready``: nothing that is still running on the GPU writes it, so that a product
     may request it as its weight while the kernel before is at work.  What the operators here return is not ready in this sense, nor
     are pieces of it (``MXFP4(q.codes[e], q.scales[e], q.ready)``); ``mxfp4_pack`` and ``mxfp4_quantize_weight`` return weights that
     are, and a pair of tensors that other code wrote is."""
@@ -175,9 +175,9 @@ def skip_rmsnorm_mxfp4(X: torch.Tensor, residual: torch.Tensor | None, weight: t
     """``(q, residual)``: ``residual += X`` in place (or into ``out_residual``), ``q`` the RMS norm of it times ``weight`` in the
     format, ``[rows, n]`` with the leading dimensions joined.  ``residual=None``: the norm of ``X``, which comes back as the second value.
 
-    What is written may lie in the place of ``X`` or ``residual``, row by row; another overlap is refused.
-    The norm is not rounded to 16 bits before it is quantised (:func:`~lite_llama_b200.kernels.skip_rmsnorm` rounds twice), and
-    decides borders as exact arithmetic does.  n: a multiple of 32, at most 16384."""
+    What is written may lie in the place of ``X`` or ``residual``, row by row; another overlap is refused.  The norm is not rounded to 16 bits
+    before it is quantised (:func:`~lite_llama_b200.kernels.skip_rmsnorm` rounds twice), and decides borders as exact arithmetic does, with
+    ``eps`` in 32 bits.  n: a multiple of 32, at most 16384."""
     out = _native.mx4_norm(X, residual, weight, eps, out_residual)
     if out is None:
         return _skip_rmsnorm_mxfp4(X, residual, weight, eps, out_residual)
@@ -220,7 +220,7 @@ def mxfp4_matmul(x: torch.Tensor | MXFP4, w: MXFP4, bias: torch.Tensor | None = 
     ``x``: 16-bit ``[..., k]`` (quantised here) or an :class:`MXFP4` ``[rows, k]``; ``w`` ``[n, k]``; ``bias [n]`` in the output's
     type.  The output is of ``x``'s type, for quantised ``x`` of ``out_dtype`` (default fp16).  ``swiglu``: the rows of ``w`` (and
     ``bias``) alternate as ``mxfp4_gate_up`` orders them, and ``silu(gate) * up`` comes back in the format, ``[rows, n / 2]``,
-    quantised from the sums themselves."""
+    quantised from the sums themselves: the codes of exact arithmetic on them."""
     if isinstance(w, MXFP4) and isinstance(x, (torch.Tensor, MXFP4)):
         y = _native.mx4_matmul(x, w, bias, swiglu, out_dtype)
         if y is not None:
