@@ -144,9 +144,10 @@ __device__ __forceinline__ void quantise_unit(const float (&g)[N], const float (
     if (byte == 255u) codes[q] = 0u;
   }
   if (top == 0u) {                     // zeros, or too small for 32 bits
-    unsure = bias != nullptr;
+    unsure = false;
 #pragma unroll
-    for (int j = 0; j < N; ++j) unsure = unsure || (g[j] != 0.f && u[j] != 0.f);
+    for (int j = 0; j < N; ++j)
+      unsure = unsure || (bias ? g[j] + to_f32(bias[j]) != 0.f && u[j] + to_f32(bias[64 + j]) != 0.f : g[j] != 0.f && u[j] != 0.f);
   }
   const uint32_t asked = __ballot_sync(0xffffffffu, unsure && in && byte != 255u);
   if (asked) unit_again<N, T>(g, u, bias, asked, codes, byte);

@@ -43,6 +43,26 @@ def test_values_next_to_borders(t, inner, k, biased):
     assert torch.equal(O.unpack_codes(q.codes), code.expand(t, -1))
 
 
+@pytest.mark.parametrize("t", (1, 9, 40, 100, 300))
+@pytest.mark.parametrize("biased", (False, True))
+def test_gates_whose_exponential_32_bits_have_not(t, biased):
+    """Blocks of gates around -106, times millions: 1e-38, where 32 bits give zero.  Beside them blocks of zeros."""
+    inner, k = 1024, 384
+    gen = torch.Generator().manual_seed(t)
+    g = B.kept(-104 - 4 * torch.rand(inner, generator=gen, dtype=torch.float64))
+    u = B.kept(1e6 * (1 + torch.rand(inner, generator=gen, dtype=torch.float64)))
+    bg, bu = torch.full_like(g, -0.5 if biased else 0.0), torch.zeros_like(g)
+    empty = torch.arange(inner) // 32 % 4 == 1
+    g, bg = torch.where(empty, 0.0, g), torch.where(empty, 0.0, bg)
+    w = packed(*gate_up(g, u, k))
+    bias = K.mxfp4_gate_up(bg[:, None], bu[:, None]).flatten().half().cuda() if biased else None
+    q = K.mxfp4_matmul(B.ones(t, k).half().cuda(), w, bias, swiglu=True)
+    code, byte = (v.cuda() for v in B.wanted(g, u, bg, bu))
+    assert (code[:, ~empty] & 7).any() and not (code[:, empty] & 7).any()
+    assert torch.equal(O.scale_rows(q.scales, t, inner), byte.expand(t, -1))
+    assert torch.equal(O.unpack_codes(q.codes), code.expand(t, -1))
+
+
 @pytest.mark.parametrize("tokens,tile", ((3, 64), (700, 64), (2000, 128), (3000, 256)))
 @pytest.mark.parametrize("dtype", HALVES)
 def test_experts_next_to_borders(tokens, tile, dtype):
